@@ -243,6 +243,89 @@ size_t GpuAttentionNoAllocScratchBytes();
 // (src/kernels_gpu.h:128; there it raises the shared-memory limit instead).
 void GpuAttentionWarmupShmem(int64_t sh_positions);
 
+// ---------------------------------------------------------------- paged KV cache
+//
+// The cache of a batch of sequences, in pages of page_size positions taken from
+// one pool per layer: position p of sequence s is slot p % page_size of page
+// pages[s * max_pages + p / page_size]. A slot holds one position's row of every
+// kv head, as fp16 or as 8-bit codes with an fp32 scale per row. All of it is
+// device memory of the caller's. No counterpart in the reference, whose cache
+// holds one sequence.
+//
+// Q8: a row x is kept as scale = max|x| * fl(1/127) and code = round(x * (1 /
+// scale)) (ties to even, at most 127 either way); it stands for code * scale. A
+// row whose scale would be subnormal is kept as zeros, one that holds an
+// infinity or a NaN as a NaN scale, so that it reads back as NaN.
+enum GpuKvType : uint32_t { kKvF16 = 0, kKvQ8 = 1 };
+
+struct GpuPagedKv {
+  uint32_t type = kKvF16;
+  int32_t n_kv_heads = 0;
+  int32_t head_dim = 0;   // 64 or 128
+  int32_t page_size = 0;  // a power of two, 16 to 256
+  int64_t n_pages = 0;    // at most 2^31 - 1
+  void* k = nullptr;      // [n_pages][n_kv_heads][page_size][head_dim] fp16 bits or int8 codes
+  void* v = nullptr;
+  float* k_scale = nullptr;  // Q8: [n_pages][n_kv_heads][page_size]; F16: unused
+  float* v_scale = nullptr;
+};
+
+struct GpuPageTable {
+  const int32_t* pages = nullptr;  // [n_seqs][max_pages]; entries no token reaches are never read as pages
+  int64_t n_seqs = 0;
+  int64_t max_pages = 0;
+};
+
+// Where each row of a call goes is device data: seq_ids[t] (nullptr: t itself)
+// names the sequence and positions[t] the position. A negative seq_id is
+// padding: nothing is read or written for that row. A row that names no slot
+// (a sequence, position or page out of range) stores nothing in the cache, and
+// what the call gives back for it is NaN. Two rows that name the same slot in
+// one call leave it holding a mixture of both.
+
+// Rows of k and v ([n_tokens][n_kv_heads][head_dim] fp32) into the cache.
+void GpuKvWritePaged(const GpuPagedKv& kv, const GpuPageTable& table, const int32_t* seq_ids,
+                     const int32_t* positions, const float* k_dev, const float* v_dev, int64_t n_tokens);
+
+// GpuQkNormRopeKv over pages: q_out[t,h,:] <- RoPE(RMSNorm(q[t,h,:]) * q_norm) at
+// the row's position (q_out may be q), RoPE(RMSNorm(k) * k_norm) and v into the
+// cache; k and v are not modified. At head_dim 128 q_out and an F16 cache hold
+// the bits that GpuQkNormRopeKv leaves. A position at or past rope_rows is out of
+// range.
+void GpuQkNormRopeKvPaged(const GpuPagedKv& kv, const GpuPageTable& table, const int32_t* seq_ids,
+                          const int32_t* positions, const float* q_dev, const float* k_dev, const float* v_dev,
+                          const float* q_norm, const float* k_norm, int32_t n_heads, const float* rope_tab,
+                          int64_t rope_rows, int64_t n_tokens, float eps, float* q_out);
+
+// The rows back out of the cache: element d of row t of kv head h goes to
+// out[t * token_stride + h * head_stride + d], as fp16 bits (out_f32 false) or
+// fp32. Strides (in elements) are multiples of 8, and rows must not overlap:
+// either whole tokens or whole heads follow each other. token_stride = head_dim,
+// head_stride = max_seq * head_dim is one layer of a contiguous GpuKvCache.
+void GpuKvReadPaged(const GpuPagedKv& kv, const GpuPageTable& table, const int32_t* seq_ids,
+                    const int32_t* positions, int64_t n_tokens, bool out_f32, void* k_out, void* v_out,
+                    int64_t token_stride, int64_t head_stride);
+
+// Attention of one new token per row over the paged cache: row r (q and out
+// [n_rows][n_heads][head_dim] fp32) attends to positions [0, lens[r]) of its
+// sequence, softmax((q . k_j) / sqrt(head_dim)) over them, query head h reading kv
+// head h / (n_heads / n_kv_heads). A row of length 0 gives zeros; padding
+// (negative seq_id) leaves its out row as it was; a length below 0 or past the
+// table's row, a sequence out of range, or a page out of range among the row's
+// positions gives NaN. out must not overlap q. The work is shared out on the
+// device from the lengths themselves, so a captured call holds for any lengths,
+// tables and seq_ids that stand there at replay.
+//
+// workspace: GpuAttentionPagedWorkspaceBytes of device memory, 256-byte aligned,
+// whose bytes are zero before the first call (GpuAttentionPagedWorkspaceInit
+// does that); each call leaves it ready for the next on the same stream. Calls
+// that may run at the same time need a workspace each.
+void GpuAttentionPaged(const GpuPagedKv& kv, const GpuPageTable& table, const int32_t* seq_ids, const int32_t* lens,
+                       const float* q_dev, int32_t n_heads, int64_t n_rows, float* out_dev, void* workspace,
+                       size_t workspace_bytes);
+size_t GpuAttentionPagedWorkspaceBytes(int32_t n_heads, int32_t n_kv_heads, int32_t head_dim);
+void GpuAttentionPagedWorkspaceInit(void* workspace, size_t bytes);
+
 // ---------------------------------------------------------------- quantised matmul
 
 // OUT[t, r] = dot(row r of W, row t of X), i.e. OUT = X . W^T (src/kernels_gpu.h:42-49):

@@ -110,11 +110,37 @@ SIGNATURES = {
 }
 
 
+
+
+class PagedKvC(ctypes.Structure):
+    """rpg_paged_kv_t (include/rpg_paged.h)."""
+    _fields_ = [("type", _u32), ("n_kv_heads", _i32), ("head_dim", _i32), ("page_size", _i32), ("n_pages", _i64),
+                ("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp)]
+
+
+class PageTableC(ctypes.Structure):
+    """rpg_page_table_t (include/rpg_paged.h)."""
+    _fields_ = [("pages", _vp), ("n_seqs", _i64), ("max_pages", _i64)]
+
+
+class PagedOpsC(ctypes.Structure):
+    """rpg_paged_ops_t: the table of the paged cache's functions (include/rpg_paged.h)."""
+    _fields_ = [("size", _i64),
+                ("kv_write", ctypes.CFUNCTYPE(_i32, _vp, _vp, _vp, _vp, _vp, _vp, _i64)),
+                ("qk_norm_rope_kv", ctypes.CFUNCTYPE(_i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp,
+                                                     _i64, _i64, _f32, _vp)),
+                ("kv_read", ctypes.CFUNCTYPE(_i32, _vp, _vp, _vp, _vp, _i64, _i32, _vp, _vp, _i64, _i64)),
+                ("attention", ctypes.CFUNCTYPE(_i32, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _vp, _vp, _i64)),
+                ("attention_workspace", ctypes.CFUNCTYPE(_i64, _i32, _i32, _i32)),
+                ("attention_workspace_init", ctypes.CFUNCTYPE(_i32, _vp, _i64))]
+
+
 class RpgError(RuntimeError):
     """An operator rejected its arguments or a HIP call failed."""
 
 
 _lib: Optional[ctypes.CDLL] = None
+_paged: Optional[PagedOpsC] = None
 
 
 def load_library() -> ctypes.CDLL:
@@ -136,6 +162,17 @@ def load_library() -> ctypes.CDLL:
         fn.argtypes = args
     _lib = lib
     return lib
+
+
+def paged_ops() -> PagedOpsC:
+    """The library's table of paged-cache functions (rpg_paged_ops)."""
+    global _paged
+    if _paged is None:
+        table = PagedOpsC.in_dll(load_library(), "rpg_paged_ops")
+        if table.size < ctypes.sizeof(PagedOpsC):
+            raise RpgError(f"rpg_paged_ops holds {table.size} bytes, {ctypes.sizeof(PagedOpsC)} are needed")
+        _paged = table
+    return _paged
 
 
 def _check(rc: int) -> int:
@@ -842,6 +879,160 @@ def GpuQkNormRopeKv(q, k, v, q_norm, k_norm, n_heads: int, n_kv_heads: int, head
         _addr(rope_tab, 4 * rope_rows * head_dim, torch.float32, "rope_tab"), rope_rows, pos0, seq, eps,
         _addr(k_layer, cache, None, "k_layer"), _addr(v_layer, cache, None, "v_layer"), max_seq,
         1 if write_k_f32 else 0))
+
+
+# ----------------------------------------------------------------------------- paged KV cache
+
+KV_F16 = 0
+KV_Q8 = 1
+
+
+class GpuPagedKv:
+    """One layer's pages of a batch's KV cache (rpg::GpuPagedKv): k and v [n_pages, n_kv_heads, page_size, head_dim],
+    fp16 (float16, int16 or uint16 bits) or int8 codes with k_scale and v_scale [n_pages, n_kv_heads, page_size]
+    float32. Views the tensors, and keeps them. Checked once, here; k and v may also be raw device addresses (all four
+    then are, with `shape` and `kv_type` given, and the caller vouches for the sizes)."""
+
+    def __init__(self, k, v, k_scale=None, v_scale=None, shape=None, kv_type=None):
+        torch = _t()
+        if isinstance(k, int):
+            if shape is None or kv_type not in (KV_F16, KV_Q8):
+                raise RpgError("GpuPagedKv: raw addresses need shape and kv_type")
+            self.device = None
+        else:
+            if shape is not None or kv_type is not None:
+                raise RpgError("GpuPagedKv: shape and kv_type go with raw addresses; tensors have their own")
+            shape = tuple(k.shape)
+            if len(shape) != 4 or tuple(v.shape) != shape or k.dtype != v.dtype:
+                raise RpgError(f"GpuPagedKv: k {tuple(k.shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} have to be "
+                               "alike, [n_pages, n_kv_heads, page_size, head_dim]")
+            kv_type = KV_Q8 if k.dtype == torch.int8 else KV_F16
+            if kv_type == KV_F16 and k.dtype not in (torch.float16, torch.int16, torch.uint16):
+                raise RpgError(f"GpuPagedKv: expected 16-bit or int8 pages, got {k.dtype}")
+            self.device = k.device
+        if kv_type == KV_Q8 and (k_scale is None or v_scale is None):
+            raise RpgError("GpuPagedKv: 8-bit pages need k_scale and v_scale")
+        if kv_type == KV_F16 and (k_scale is not None or v_scale is not None):
+            raise RpgError("GpuPagedKv: fp16 pages have no scales")
+        for name, s in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if isinstance(s, torch.Tensor) and tuple(s.shape) != tuple(shape[:3]):
+                raise RpgError(f"GpuPagedKv: {name} {tuple(s.shape)} has to be {tuple(shape[:3])}")
+        self.kv_type = kv_type
+        self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = (int(n) for n in shape)
+        self.tensors = (k, v, k_scale, v_scale)
+        scale = torch.float32
+        self.c = PagedKvC(kv_type, self.n_kv_heads, self.head_dim, self.page_size, self.n_pages, _addr(k, name="k"),
+                          _addr(v, name="v"), _addr(k_scale, 0, scale, "k_scale"), _addr(v_scale, 0, scale, "v_scale"))
+        if self.device is not None and any(t is not None and t.device != self.device for t in self.tensors):
+            raise RpgError("GpuPagedKv: pages and scales are on different devices")
+        self.ref = ctypes.byref(self.c)
+
+
+class GpuPageTable:
+    """The sequences' pages in order (rpg::GpuPageTable): an int32 tensor [n_seqs, max_pages], or a raw device address
+    with `shape`. Views the tensor, whose entries may change between calls."""
+
+    def __init__(self, pages, shape=None):
+        if not isinstance(pages, int):
+            if pages.dim() != 2 or shape is not None:
+                raise RpgError("GpuPageTable: expected an int32 tensor [n_seqs, max_pages]")
+            shape = pages.shape
+        elif shape is None:
+            raise RpgError("GpuPageTable: a raw address needs shape")
+        self.n_seqs, self.max_pages = (int(n) for n in shape)
+        self.pages = pages
+        self.c = PageTableC(_addr(pages, 0, _t().int32, "pages"), self.n_seqs, self.max_pages)
+        self.ref = ctypes.byref(self.c)
+
+
+def _paged_device(kv: GpuPagedKv, *bufs) -> None:
+    """Refuses tensors that are not where the pages are, and pages that are not on the current device."""
+    if kv.device is None:
+        return
+    for b in bufs:
+        if b is not None and not isinstance(b, int) and b.device != kv.device:
+            raise RpgError(f"a tensor on {b.device} beside a paged cache on {kv.device}")
+    if _t().cuda.current_device() != kv.device.index:
+        raise RpgError(f"the paged cache is on {kv.device}, which is not the current device")
+
+
+def GpuKvWritePaged(kv: GpuPagedKv, table: GpuPageTable, seq_ids, positions, k, v, n_tokens: int) -> None:
+    """Rows of k and v [n_tokens, n_kv_heads, head_dim] into the pages, quantised there if these hold 8 bits. seq_ids
+    and positions are int32 tensors [n_tokens] (seq_ids None: row t is of sequence t; negative: padding)."""
+    torch = _t()
+    _paged_device(kv, table.pages, seq_ids, positions, k, v)
+    row = 4 * n_tokens * kv.n_kv_heads * kv.head_dim
+    _check(paged_ops().kv_write(
+        kv.ref, table.ref, _addr(seq_ids, 4 * n_tokens, torch.int32, "seq_ids"),
+        _addr(positions, 4 * n_tokens, torch.int32, "positions"), _addr(k, row, torch.float32, "k"),
+        _addr(v, row, torch.float32, "v"), n_tokens))
+
+
+def GpuQkNormRopeKvPaged(kv: GpuPagedKv, table: GpuPageTable, seq_ids, positions, q, k, v, q_norm, k_norm,
+                         n_heads: int, rope_tab, rope_rows: int, n_tokens: int, eps: float, q_out) -> None:
+    """q_out <- RoPE(RMSNorm(q) * q_norm) at each row's position, RoPE(RMSNorm(k) * k_norm) and v into the pages.
+    q_out may be q; k and v are not modified."""
+    torch = _t()
+    f32 = torch.float32
+    _paged_device(kv, table.pages, seq_ids, positions, q, k, v, q_norm, k_norm, rope_tab, q_out)
+    d = kv.head_dim
+    qb, kb = 4 * n_tokens * n_heads * d, 4 * n_tokens * kv.n_kv_heads * d
+    _check(paged_ops().qk_norm_rope_kv(
+        kv.ref, table.ref, _addr(seq_ids, 4 * n_tokens, torch.int32, "seq_ids"),
+        _addr(positions, 4 * n_tokens, torch.int32, "positions"), _addr(q, qb, f32, "q"), _addr(k, kb, f32, "k"),
+        _addr(v, kb, f32, "v"), _addr(q_norm, 4 * d, f32, "q_norm"), _addr(k_norm, 4 * d, f32, "k_norm"), n_heads,
+        _addr(rope_tab, 4 * rope_rows * d, f32, "rope_tab"), rope_rows, n_tokens, eps, _addr(q_out, qb, f32, "q_out")))
+
+
+def GpuKvReadPaged(kv: GpuPagedKv, table: GpuPageTable, seq_ids, positions, n_tokens: int, k_out, v_out,
+                   token_stride: int, head_stride: int, out_f32: Optional[bool] = None) -> None:
+    """The rows back out of the pages: element d of row t of kv head h to out[t * token_stride + h * head_stride + d].
+    k_out and v_out are float32 or 16-bit (float16, int16, uint16) tensors; raw addresses need out_f32. Strides
+    (head_dim, max_seq * head_dim) fill a layer of the contiguous cache."""
+    torch = _t()
+    _paged_device(kv, table.pages, seq_ids, positions, k_out, v_out)
+    if out_f32 is None:
+        if not isinstance(k_out, torch.Tensor):
+            raise RpgError("GpuKvReadPaged: raw addresses need out_f32")
+        out_f32 = k_out.dtype == torch.float32
+    for name, t in (("k_out", k_out), ("v_out", v_out)):
+        if isinstance(t, torch.Tensor) and t.dtype not in ((torch.float32,) if out_f32 else
+                                                           (torch.float16, torch.int16, torch.uint16)):
+            raise RpgError(f"GpuKvReadPaged: {name} is {t.dtype}")
+    last = (n_tokens - 1) * token_stride + (kv.n_kv_heads - 1) * head_stride + kv.head_dim
+    nbytes = (4 if out_f32 else 2) * last if n_tokens > 0 else 0
+    _check(paged_ops().kv_read(
+        kv.ref, table.ref, _addr(seq_ids, 4 * n_tokens, torch.int32, "seq_ids"),
+        _addr(positions, 4 * n_tokens, torch.int32, "positions"), n_tokens, 1 if out_f32 else 0,
+        _addr(k_out, nbytes, name="k_out"), _addr(v_out, nbytes, name="v_out"), token_stride, head_stride))
+
+
+def GpuAttentionPagedWorkspace(n_heads: int, n_kv_heads: int, head_dim: int) -> int:
+    """Bytes of the workspace of GpuAttentionPaged for these heads."""
+    return _check(paged_ops().attention_workspace(n_heads, n_kv_heads, head_dim))
+
+
+def GpuAttentionPagedWorkspaceInit(workspace, nbytes: int) -> None:
+    """Zeroes a workspace, as its first call needs it (a tensor made by torch.zeros is ready)."""
+    _check(paged_ops().attention_workspace_init(_addr(workspace, nbytes, name="workspace"), nbytes))
+
+
+def GpuAttentionPaged(kv: GpuPagedKv, table: GpuPageTable, lens, q, n_heads: int, n_rows: int, out, workspace,
+                      seq_ids=None, workspace_bytes: Optional[int] = None) -> None:
+    """One new token per row: row r of q [n_rows, n_heads, head_dim] attends to positions [0, lens[r]) of its
+    sequence, lens an int32 tensor [n_rows]. The workspace is zero before its first call, and belongs to one call at a
+    time (workspace_bytes goes with a raw address)."""
+    torch = _t()
+    _paged_device(kv, table.pages, lens, q, out, workspace, seq_ids)
+    span = 4 * n_rows * n_heads * kv.head_dim
+    if workspace_bytes is None:
+        if not isinstance(workspace, torch.Tensor):
+            raise RpgError("GpuAttentionPaged: a raw workspace needs workspace_bytes")
+        workspace_bytes = workspace.numel() * workspace.element_size()
+    _check(paged_ops().attention(
+        kv.ref, table.ref, _addr(seq_ids, 4 * n_rows, torch.int32, "seq_ids"),
+        _addr(lens, 4 * n_rows, torch.int32, "lens"), _addr(q, span, torch.float32, "q"), n_heads, n_rows,
+        _addr(out, span, torch.float32, "out"), _addr(workspace, workspace_bytes, name="workspace"), workspace_bytes))
 
 
 # ----------------------------------------------------------------------------- measurement
