@@ -7,32 +7,35 @@
 // Exponentials are taken as powers of two, with log2(e) in the scores' scale.
 //
 // What bounds it: the cache is read once, 2 D (+ 4) bytes of keys and values a
-// position and kv head, and 4 D G operations are done on them. Vector arithmetic
-// would take G multiply-adds an element beside its conversion, too much from G = 8
-// on for 8-bit rows (39e12 lane operations a second against some 6e12 bytes), so
-// both products run on the matrix cores, where the G query heads of a kv head are
-// columns of one 16-column tile.
+// position and kv head, and 4 D G operations are done on them. Both products run on
+// the matrix cores, where the G query heads of a kv head are columns of a 16-column
+// tile: rows of S = K Q^T are 16 keys, rows of O^T = V^T P^T 16 elements, so that a
+// lane ends the first with the weights of the keys that it holds in the second.
 //
-// Products (16x16x32, fp16 operands, fp32 sums). Keys and values enter as they are
-// kept: halves, or codes, which are exact in fp16. Queries and weights are fp32 and
-// enter as two fp16 terms of 11 bits, hi + lo, in columns n and n + 8 of the same
-// tile, which a tile of at most 8 heads leaves free: 22 bits for no further matrix
-// instruction. A query row is first scaled by a power of two to a largest magnitude
-// in [2^14, 2^15), weights by 2^14 (8-bit values: with their row's scale, relative
-// to a power of two above the largest scale so far), so that what is lost at fp16's
-// low end is below 2^-38 of the largest. hi is cut off from slightly below the
-// value, so that both terms have its sign and neither is zero: infinities in the
-// cache then give what the one product would (weights below 2^-23 of the largest
-// excepted, which may turn an infinite value into NaN).
-//   S = K Q^T: rows are 16 keys (a lane loads 16 contiguous bytes of a key's row),
-//     columns heads; a lane ends with 4 keys of one column.
-//   O^T = V^T P^T: rows are D / 16 sets of 16 elements, the sum runs over 32 keys.
-//     Which of them a lane group holds is free, so it holds those whose weights it
-//     has from S, and loads their rows D / 16 contiguous elements wide; the
-//     transposition is byte permutes within the lane.
+// fp16 cache (16x16x32, fp32 sums): keys and values enter as they are kept, queries
+// and weights, which are fp32, as two fp16 terms of 11 bits, hi + lo, in columns n
+// and n + 8 of one tile. A query row is first scaled by a power of two to a largest
+// magnitude in [2^14, 2^15), weights by 2^14, so that what fp16's low end loses is
+// below 2^-38 of the largest. hi is cut off from slightly below the value, so that
+// both terms have its sign and neither is zero: infinities in the cache then give
+// what the one product would (weights below 2^-23 of the largest excepted, which may
+// turn an infinite value into NaN).
 //
-// Sharing out: work is counted in units of 64 positions of one (row, kv head, tile
-// of up to 8 heads). Every wave adds up the rows' units by itself from lens and
+// 8-bit cache (16x16x64, int32 sums): the codes enter as they are kept and the sums
+// are exact. Queries are taken to whole numbers below 2^30, relative to a row's
+// largest, and weights, with their values' scales, to whole numbers of 2^-27
+// (relative to a power of two above the scales so far); either enters as four
+// signed digits of 8 bits, in columns n, n + 4, n + 8, n + 12. Weights have 3 bits of
+// headroom: the maximum that they are relative to moves only when a score exceeds
+// it by 3 (log2), and only then are the int32 sums of the output taken to fp32.
+//
+// Keys and values come straight to LDS in whole 128-byte lines, the next step's as
+// soon as this step has read what they replace; the transposition of values is the
+// LDS read's. The pieces of 16 bytes of a row lie permuted by the row's number, which
+// spreads the reads over the banks.
+//
+// Sharing out: work is counted in units of 32 or 64 positions of one (row, kv head,
+// tile of up to 8 heads). Every wave adds up the rows' units by itself from lens and
 // takes an equal, contiguous share of them, so that ragged batches and single long
 // rows fill the card alike and nothing about the lengths is needed on the host. A
 // wave writes what it holds whole; where a (row, tile) is split over waves of one
@@ -54,24 +57,33 @@ namespace {
 using dev::PagedView;
 
 constexpr int kWaves = 4;
-constexpr int kUnitShift = 6;  // 64 positions to a unit
 constexpr int kTileHeads = 8;
 // Workgroups at most; a workspace has two part slots and a counter for each.
-constexpr int kMaxGroups = 768;
+constexpr int kMaxGroups = 512;
 // Bytes between two counters: on lines of their own, as the decode attention's.
 constexpr size_t kCounterBytes = 256;
+#ifndef TUNE_MIN
+#define TUNE_MIN 4
+#endif
+#ifndef TUNE_NT
+#define TUNE_NT " nt"
+#endif
 
 using Half2 = _Float16 __attribute__((ext_vector_type(2)));
 using Half8 = _Float16 __attribute__((ext_vector_type(8)));
 using F32x4 = float __attribute__((ext_vector_type(4)));
+using I32x4 = int __attribute__((ext_vector_type(4)));
+using I32x2 = int __attribute__((ext_vector_type(2)));
+using S16x4 = short __attribute__((ext_vector_type(4)));
 
 constexpr int PartFloats(int d) { return d + 4; }  // o[d], m, l, and two to keep rows 16-byte aligned
 
 // ---------------------------------------------------------------- lane exchange
 
-// x of the lane 8 further on in its row of 16.
-__device__ __forceinline__ float Ror8(float x) {
-  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x128, 0xF, 0xF, false));
+// x of the lane kBy further on in its row of 16.
+template <int kBy>
+__device__ __forceinline__ float Ror(float x) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x120 + kBy, 0xF, 0xF, false));
 }
 
 // f over the four lanes l, l ^ 16, l ^ 32, l ^ 48; every one of them has the result.
@@ -111,43 +123,108 @@ __device__ __forceinline__ Half8 AsHalf8(uint32_t a, uint32_t b, uint32_t c, uin
   return __builtin_bit_cast(Half8, w);
 }
 
-// Two codes (bytes 2 i, 2 i + 1 of w, sign bit flipped) as halves: 1024 + u, less 1152.
-template <int kI>
-__device__ __forceinline__ uint32_t CodePair(uint32_t flipped) {
-  const uint32_t x = __builtin_amdgcn_perm(0x64646464u, flipped, kI == 0 ? 0x04010400u : 0x04030402u);
-  const Half2 bias = {static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)};
-  return Bits(__builtin_bit_cast(Half2, x) - bias);
+// Signed digit `at` (selector bytes: at, 4 + at) of four whole numbers given with
+// 0x80808080 added: x = sum of digit_i 256^i with digit_i = byte i - 128 there.
+__device__ __forceinline__ int Digit4(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t selector) {
+  const uint32_t lo = __builtin_amdgcn_perm(b, a, selector), hi = __builtin_amdgcn_perm(d, c, selector);
+  return static_cast<int>(__builtin_amdgcn_perm(hi, lo, 0x05040100u) ^ 0x80808080u);
 }
 
-// Byte kI of two words (sign bit flipped) as halves, times 2^-9: as a subnormal the
-// byte u stands for u 2^-24, and u 2^-9 - 2^-2 = (u - 128) 2^-9 is one exact fma.
-template <int kI>
-__device__ __forceinline__ uint32_t CodeOfTwo(uint32_t w0, uint32_t w1) {
-  const uint32_t x = __builtin_amdgcn_perm(w1, w0, 0x0C000C00u | kI | ((4 + kI) << 16));
-  const Half2 up = {static_cast<_Float16>(32768.0f), static_cast<_Float16>(32768.0f)};
-  const Half2 off = {static_cast<_Float16>(-0.25f), static_cast<_Float16>(-0.25f)};
-  return Bits(__builtin_elementwise_fma(__builtin_bit_cast(Half2, x), up, off));
+// ---------------------------------------------------------------- LDS
+
+using Lds = __attribute__((address_space(3))) char;
+
+// Loads straight to LDS are written out, and so are the waits for them: the compiler
+// lets an LDS read wait for every such load before it, where the loop below needs it
+// to wait for the older half of them. The waits count on the kernel's main loop to
+// make no other vector memory access in between; any that the compiler does make
+// (a piece's queries and outputs) only makes a wait longer.
+using Resource = dev::U32x4;
+__device__ __forceinline__ Resource RowsResource(const void* base, uint32_t bytes) {
+  const uint64_t at = reinterpret_cast<uint64_t>(base);
+  return Resource{static_cast<uint32_t>(at), static_cast<uint32_t>(at >> 32) & 0xFFFFu, bytes, 0x00020000u};
+}
+__device__ __forceinline__ uint32_t LdsAddress(const void* p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const Lds*)(static_cast<const char*>(p))));
+}
+// kN times 16 bytes a lane from rs: time i from byte off[i % kOff] + 1024 i, lane j's to LDS address `to` + 1024 i +
+// 16 j (an instruction's offset counts on both sides). M0 holds the LDS address, which is read one wait state after it is
+// written; five are waited, which a resource needs whose registers a vector instruction wrote.
+template <int kN, int kOff>
+__device__ __forceinline__ void LoadToLds(Resource rs, const uint32_t (&off)[kOff], uint32_t to) {
+  static_assert(kN == 1 || kN == 2 || kN == 4, "");
+  if constexpr (kN == 1) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen" TUNE_NT " lds"
+                 :
+                 : "s"(to), "v"(off[0]), "s"(rs)
+                 : "memory");
+  } else if constexpr (kN == 2) {
+    asm volatile(
+        "s_mov_b32 m0, %0\n\ts_nop 4\n\t"
+        "buffer_load_dwordx4 %1, %3, 0 offen" TUNE_NT " lds\n\t"
+        "buffer_load_dwordx4 %2, %3, 0 offen offset:1024" TUNE_NT " lds"
+        :
+        : "s"(to), "v"(off[0]), "v"(off[1 % kOff]), "s"(rs)
+        : "memory");
+  } else {
+    asm volatile(
+        "s_mov_b32 m0, %0\n\ts_nop 4\n\t"
+        "buffer_load_dwordx4 %1, %5, 0 offen" TUNE_NT " lds\n\t"
+        "buffer_load_dwordx4 %2, %5, 0 offen offset:1024" TUNE_NT " lds\n\t"
+        "buffer_load_dwordx4 %3, %5, 0 offen offset:2048" TUNE_NT " lds\n\t"
+        "buffer_load_dwordx4 %4, %5, 0 offen offset:0xc00" TUNE_NT " lds"
+        :
+        : "s"(to), "v"(off[0]), "v"(off[1 % kOff]), "v"(off[2 % kOff]), "v"(off[3 % kOff]), "s"(rs)
+        : "memory");
+  }
+}
+// 4 bytes a lane, from an address of its own.
+__device__ __forceinline__ void LoadWordToLds(const float* from, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(to), "v"(from) : "memory");
+}
+// Waits until at most kLeft vector memory accesses are under way.
+template <int kLeft>
+__device__ __forceinline__ void WaitLoads() {
+  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(kLeft) : "memory");
+}
+// Waits for the LDS reads under way, before what they read is loaded over.
+__device__ __forceinline__ void WaitLdsReads() { asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory"); }
+
+// A scalar load: p is the same in every lane, and what it points to does not change while the kernel runs.
+template <class T>
+__device__ __forceinline__ T ScalarLoad(const T* p) {
+  return *(const __attribute__((address_space(4))) T*)(p);
+}
+
+// Four halves, one of each of four rows: in each 16-lane group, lane j receives
+// element j % 4 of the 8 bytes addressed by lanes j / 4, 4 + j / 4, ...
+__device__ __forceinline__ uint2 ReadHalvesAcross(const char* at) {
+  const S16x4 v =
+      __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) S16x4*)(Lds*)(const_cast<char*>(at)));
+  return __builtin_bit_cast(uint2, v);
+}
+// Eight bytes, one of each of eight rows: in each 16-lane group, lane j receives
+// byte j % 8 of the 8 bytes addressed by lanes j / 8, 2 + j / 8, ...
+__device__ __forceinline__ I32x2 ReadBytesAcross(const char* at) {
+  return __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) I32x2*)(Lds*)(const_cast<char*>(at)));
 }
 
 // ---------------------------------------------------------------- sharing out
 
-// Everything here is the same in every lane of a wave.
+// Everything here is the same in every lane of a wave, and kept in scalar registers.
 struct Share {
-  int64_t total;  // units
-  int64_t per;    // a workgroup's units: per, and one more in the first `rem` of them
-  int64_t rem;
-  int32_t groups;
+  uint32_t total;  // units
+  uint32_t per;    // a workgroup's units: per, and one more in the first `rem` of them
+  uint32_t rem;
+  uint32_t groups;
 
-  __device__ __forceinline__ int64_t Begin(int64_t w) const { return w * per + (w < rem ? w : rem); }
+  __device__ __forceinline__ uint32_t Begin(uint32_t w) const { return w * per + min(w, rem); }
   // The workgroup whose share holds unit x.
-  __device__ __forceinline__ int64_t Holder(int64_t x) const {
-    const int64_t big = rem * (per + 1);
-    if ((total >> 32) == 0) {
-      return x < big ? static_cast<uint32_t>(x) / static_cast<uint32_t>(per + 1)
-                     : rem + static_cast<uint32_t>(x - big) / static_cast<uint32_t>(per);
-    }
-    return x < big ? x / (per + 1) : rem + (x - big) / per;
+  __device__ __forceinline__ uint32_t Holder(uint32_t x) const {
+    const uint32_t big = rem * (per + 1);
+    return Scalar(x < big ? x / (per + 1) : rem + (x - big) / per);
   }
+  static __device__ __forceinline__ uint32_t Scalar(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
 };
 
 struct Rows {
@@ -156,59 +233,68 @@ struct Rows {
   int64_t n_seqs;
   int64_t capacity;  // positions that a table row has pages for
   int32_t n_rows;
-  int32_t pairs;  // (kv head, tile) pairs of a row
+  int32_t pairs;       // (kv head, tile) pairs of a row
+  int32_t unit_shift;  // log2 of a unit's positions
 
   __device__ __forceinline__ int64_t Seq(int32_t r) const { return seq_ids != nullptr ? seq_ids[r] : r; }
   __device__ __forceinline__ bool Fine(int64_t seq, int32_t len) const {
     return seq >= 0 && seq < n_seqs && len >= 0 && len <= capacity;
   }
   // Units of one pair of row r; none for a row that is padding, empty or out of range.
-  __device__ __forceinline__ int32_t UnitsOf(int32_t r) const {
-    const int32_t len = lens[r];
-    return Fine(Seq(r), len) ? static_cast<int32_t>((static_cast<int64_t>(len) + 63) >> kUnitShift) : 0;
+  __device__ __forceinline__ uint32_t UnitsOf(int64_t seq, int32_t len) const {
+    return Fine(seq, len) ? (static_cast<uint32_t>(len) + (1u << unit_shift) - 1u) >> unit_shift : 0u;
+  }
+  __device__ __forceinline__ uint32_t UnitsOf(int32_t r) const { return UnitsOf(Seq(r), lens[r]); }
+  // for an r that is the same in every lane
+  __device__ __forceinline__ int64_t ScalarSeq(int32_t r) const {
+    return seq_ids != nullptr ? ScalarLoad(seq_ids + r) : r;
+  }
+  __device__ __forceinline__ uint32_t ScalarUnitsOf(int32_t r) const {
+    return UnitsOf(ScalarSeq(r), ScalarLoad(lens + r));
   }
 };
 
+// Sum of x over the lanes up to and with this one.
+__device__ __forceinline__ uint32_t ScanAdd(uint32_t x) {
+  int v = static_cast<int>(x);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr 1, 2, 4, 8: within rows of 16
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // lane 15's into row 1, lane 47's into row 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // lane 31's into rows 2 and 3
+  return static_cast<uint32_t>(v);
+}
+
 // Units of rows [lo, hi), taken `each` to a lane: what lies before this lane's rows.
-__device__ __forceinline__ int64_t UnitsBefore(const Rows& rows, int32_t lo, int32_t hi, int32_t each, int lane,
-                                               int64_t* total) {
-  int64_t own = 0;
+__device__ __forceinline__ uint32_t UnitsBefore(const Rows& rows, int32_t lo, int32_t hi, int32_t each, int lane,
+                                                uint32_t* total) {
+  uint32_t own = 0;
   const int64_t first = lo + static_cast<int64_t>(lane) * each;
   for (int32_t i = 0; i < each; ++i) {
     if (first + i < hi) own += rows.UnitsOf(static_cast<int32_t>(first + i));
   }
-  own *= rows.pairs;
-  int64_t sum = own;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int64_t up = __shfl_up(sum, off, 64);
-    if (lane >= off) sum += up;
-  }
-  *total = __shfl(sum, 63, 64);
+  own *= static_cast<uint32_t>(rows.pairs);
+  const uint32_t sum = ScanAdd(own);
+  *total = __builtin_amdgcn_readlane(sum, 63);
   return sum - own;
 }
 
-__device__ __forceinline__ int64_t Uniform(int64_t x) {
-  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(x));
-  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(x >> 32));
-  return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
-}
-
 // Row that holds unit x, and what of x lies in it (*rest), from the units before
-// each lane's `each` rows of [lo, hi).
-__device__ __forceinline__ int32_t RowOfUnit(const Rows& rows, int64_t before, int32_t each, int lane, int64_t x,
-                                             int64_t* rest) {
+// each lane's `each` rows.
+__device__ __forceinline__ int32_t RowOfUnit(const Rows& rows, uint32_t before, int32_t each, int lane, uint32_t x,
+                                             uint32_t* rest) {
   int32_t lo = 0, hi = rows.n_rows;
   while (true) {
     // before does not fall from lane to lane, and the last one at or below x is not of an empty set of rows
     const int at = static_cast<int>(__builtin_popcountll(__ballot(before <= x))) - 1;
-    x -= Uniform(__shfl(before, at, 64));
+    x -= __builtin_amdgcn_readlane(before, at);
     const int64_t begin = lo + static_cast<int64_t>(at) * each;
     hi = static_cast<int32_t>(min(begin + each, static_cast<int64_t>(hi)));
     lo = static_cast<int32_t>(begin);
     if (each == 1) break;
     each = (hi - lo + 63) / 64;
-    int64_t unused;
+    uint32_t unused;
     before = UnitsBefore(rows, lo, hi, each, lane, &unused);
   }
   *rest = x;
@@ -219,38 +305,47 @@ __device__ __forceinline__ int32_t RowOfUnit(const Rows& rows, int64_t before, i
 
 // What a wave or workgroup holds of a (row, pair): its units [c0, c1) of n.
 struct Piece {
-  int64_t first;  // number of the pair's first unit
-  int32_t row, pair, c0, c1, n;
+  uint32_t first;  // number of the pair's first unit
+  uint32_t c0, c1, n;
+  int32_t row, pair;
 };
 
 // In scalar registers: a buffer descriptor made from vector ones would be looped over.
 __device__ __forceinline__ Piece UniformPiece(const Piece& p) {
-  return Piece{Uniform(p.first),
-               __builtin_amdgcn_readfirstlane(p.row),
-               __builtin_amdgcn_readfirstlane(p.pair),
-               __builtin_amdgcn_readfirstlane(p.c0),
-               __builtin_amdgcn_readfirstlane(p.c1),
-               __builtin_amdgcn_readfirstlane(p.n)};
+  return Piece{Share::Scalar(p.first), Share::Scalar(p.c0), Share::Scalar(p.c1), Share::Scalar(p.n),
+               __builtin_amdgcn_readfirstlane(p.row),   __builtin_amdgcn_readfirstlane(p.pair)};
 }
 
-template <int D, bool kQ8>
-__global__ __launch_bounds__(64 * kWaves) void PagedAttentionKernel(PagedView view, Rows rows,
-                                                                    const float* __restrict__ q, int32_t n_heads,
-                                                                    int32_t tiles, int32_t tile_heads, float scale_log2,
-                                                                    float* __restrict__ out,
-                                                                    char* __restrict__ workspace) {
-  constexpr int kBytes = kQ8 ? 1 : 2;
-  constexpr int kSub = D == 128 && !kQ8 ? 2 : 4;  // 16-key tiles of a step: 32 registers of keys at most
+// kTiles: 8-bit caches, column tiles of up to 4 heads (1 or 2); else 1, of up to 8.
+template <int D, bool kQ8, int kTiles>
+__global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView view, Rows rows,
+                                                                       const float* __restrict__ q, int32_t n_heads,
+                                                                       int32_t tiles, int32_t tile_heads,
+                                                                       float scale_log2, float* __restrict__ out,
+                                                                       char* __restrict__ workspace) {
+  constexpr int kSub = D == 128 && !kQ8 ? 2 : 4;  // 16-key tiles of a step, which is a unit
   constexpr int kStep = 16 * kSub;
-  constexpr int kRow = D * kBytes;        // bytes of a key's row
-  constexpr int kKLoads = kRow / 64;      // 16-byte loads of a lane for 16 keys
-  constexpr int kSteps = D / 32;          // matrix products of 16 keys
-  constexpr int kE = D / 16;              // elements of a value row to a lane
-  constexpr int kVWords = kE * kBytes / 4;
+  constexpr int kRow = D * (kQ8 ? 1 : 2);  // bytes of a cached row
+  constexpr int kPieces = kRow / 16;       // of 16 bytes
+  constexpr int kLoads = kRow / 64;        // loads of 64 pieces for 16 keys
+  constexpr int kSteps = kRow / 64;        // matrix products of 16 keys
+  constexpr int kE = D / 16;               // tiles of 16 elements of a value row
   constexpr int kPart = PartFloats(D);
-  static_assert((1 << kUnitShift) % kStep == 0, "a unit is whole steps");
+  constexpr int kCopies = kQ8 ? 4 : 2;     // columns of a head, that is lanes that have its final sums
+  constexpr int kHeadCols = 16 / kCopies;
+  constexpr int kOwn = kE / kCopies;       // tiles of 16 elements that each of them writes
 
-  __shared__ __attribute__((aligned(16))) float part[kWaves][2][kTileHeads][kPart];
+  // a wave's step of keys and values, each row's scale behind them
+  constexpr int kStage = kStep * kRow + (kQ8 ? kStep * 4 : 0);
+  constexpr int kStageLoads = kSub * kLoads + (kQ8 ? 1 : 0);
+  __shared__ __attribute__((aligned(16))) char k_lds[kWaves][kStage];
+  __shared__ __attribute__((aligned(16))) char v_lds[kWaves][kStage];
+  static_assert(kTileHeads * kPart * 4 <= kStep * kRow, "a part fits where keys or values were");
+  struct Join {
+    float4 o;
+    float m, l;
+  };
+  __shared__ Join joins[64 * kWaves];
   __shared__ Piece pieces[kWaves][2];
   __shared__ int held[kWaves];
   __shared__ int last_flag;
@@ -259,344 +354,543 @@ __global__ __launch_bounds__(64 * kWaves) void PagedAttentionKernel(PagedView vi
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int n = lane & 15;
   const int g = lane >> 4;
-  const bool is_lo = n >= 8;
+  const int head_col = n % kHeadCols;
+  const int copy = n / kHeadCols;
   const int32_t group = n_heads / view.n_kv;
 
   // the batch's units, and this wave's share
   Share share;
   const int32_t each = (rows.n_rows + 63) / 64;
-  const int64_t before = UnitsBefore(rows, 0, rows.n_rows, each, lane, &share.total);
-  share.total = Uniform(share.total);
-  share.groups = static_cast<int32_t>(min(static_cast<int64_t>(gridDim.x), (share.total + kWaves - 1) / kWaves));
-  const int64_t me = blockIdx.x;
-  int64_t begin = 0, end = 0;
+  const uint32_t before = UnitsBefore(rows, 0, rows.n_rows, each, lane, &share.total);
+  share.groups = min(gridDim.x, (share.total + TUNE_MIN - 1) / TUNE_MIN);
+  const uint32_t me = blockIdx.x;
+  uint32_t begin = 0, end = 0;
   if (me < share.groups) {
-    if ((share.total >> 32) == 0) {
-      const uint32_t t = static_cast<uint32_t>(share.total), w = static_cast<uint32_t>(share.groups);
-      share.per = t / w;
-      share.rem = t % w;
-    } else {
-      share.per = share.total / share.groups;
-      share.rem = share.total % share.groups;
-    }
+    share.per = Share::Scalar(share.total / share.groups);
+    share.rem = share.total - share.per * share.groups;
     begin = share.Begin(me);
     end = share.Begin(me + 1);
   }
-  int64_t u = Uniform(begin + (((end - begin) * wave) >> 2));
-  const int64_t u_end = Uniform(begin + (((end - begin) * (wave + 1)) >> 2));
+  uint32_t u = begin + (((end - begin) * wave) >> 2);
+  const uint32_t u_end = begin + (((end - begin) * (wave + 1)) >> 2);
   static_assert(kWaves == 4, "a wave's share of its workgroup's");
 
-  int my_held = 0;
+  int my_held = 0;  // bit 0: the first piece, bit 1: the last
   if (u < u_end) {
-    int64_t rest;
-    int32_t row = __builtin_amdgcn_readfirstlane(RowOfUnit(rows, before, each, lane, u, &rest));
-    rest = Uniform(rest);
-    int32_t units = __builtin_amdgcn_readfirstlane(rows.UnitsOf(row));
-    int32_t pair = 0, c0 = 0;
-    if ((rest >> 32) == 0) {
-      pair = static_cast<int32_t>(static_cast<uint32_t>(rest) / static_cast<uint32_t>(units));
-      c0 = static_cast<int32_t>(static_cast<uint32_t>(rest) % static_cast<uint32_t>(units));
-    } else {
-      pair = static_cast<int32_t>(rest / units);
-      c0 = static_cast<int32_t>(rest % units);
+    char* const k_mine = k_lds[wave];
+    char* const v_mine = v_lds[wave];
+    // Loads: lane i takes piece i % kPieces of row i / kPieces of each load's rows, and puts there what belongs there:
+    // piece p of key row r lies at p ^ k_swap(r), of value row r at p ^ v_swap(r).
+    const int lrow = lane / kPieces, lpiece = lane % kPieces;
+    constexpr int kLoadRows = 64 / kPieces;
+    const auto k_swap = [](int r) { return kPieces == 16 ? r & 15 : kPieces == 8 ? r & 7 : (r >> 1) & 3; };
+    const auto v_swap = [](int r, int odd) {  // odd: of an odd-numbered tile of 16 keys
+      return !kQ8 ? 2 * (r & 3) : kPieces == 8 ? (r & 3) | (odd << 2) : ((r >> 1) & 1) | (odd << 1);
+    };
+    constexpr int kKeyOffs = kPieces == 16 ? 4 : 1;  // with 16 pieces the rows of a load are permuted as its number says
+    uint32_t k_from[kKeyOffs], v_from[2][1];
+#pragma unroll
+    for (int i = 0; i < kKeyOffs; ++i) {
+      k_from[i] = static_cast<uint32_t>(lrow * kRow + 16 * (lpiece ^ k_swap(i * kLoadRows + lrow)));
     }
-    while (true) {
-      const int32_t c1 = static_cast<int32_t>(min(static_cast<int64_t>(units), c0 + (u_end - u)));
-      const int64_t seq = rows.Seq(row);
-      const int32_t len = rows.lens[row];
-      const int32_t* table = view.pages + seq * view.max_pages;
+#pragma unroll
+    for (int odd = 0; odd < 2; ++odd) {
+      v_from[odd][0] = static_cast<uint32_t>(lrow * kRow + 16 * (lpiece ^ v_swap(lrow, odd)));
+    }
+    // Reads: the key operand's pieces g, 4 + g, ... of row n; the value operand's rows as its keys have weights here
+    const uint32_t k_at = static_cast<uint32_t>(n * kRow + 16 * (g ^ k_swap(n)));
+    uint32_t v_at;
+    if constexpr (kQ8) {
+      const int i = n >> 1;  // key 4 g + i % 4 of tile i / 4, and of tile 2 + i / 4
+      v_at = static_cast<uint32_t>(((i >> 2) * 16 + 4 * g + (i & 3)) * kRow + 16 * v_swap(i & 3, i >> 2) + 8 * (n & 1));
+    } else {
+      const int i = n >> 2;  // key 4 g + i of each tile
+      v_at = static_cast<uint32_t>((4 * g + i) * kRow + 16 * (((n & 3) >> 1) ^ v_swap(i, 0)) + 8 * (n & 1));
+    }
+
+    // where the wave is: unit c of `units` of `pair` of `row`
+    uint32_t rest;
+    int32_t row = RowOfUnit(rows, before, each, lane, u, &rest);
+    uint32_t units = rows.ScalarUnitsOf(row);
+    int32_t pair = static_cast<int32_t>(Share::Scalar(rest / units));
+    uint32_t c = rest - static_cast<uint32_t>(pair) * units;
+    int32_t len = ScalarLoad(rows.lens + row);
+    const int32_t* table = view.pages + rows.ScalarSeq(row) * view.max_pages;
+
+    // Rows of the pool that the 16-key tiles of unit c start at; a tile past the end repeats the unit's first, a page
+    // out of range is read as page 0 and its tile marked.
+    int64_t at[kSub];
+    int bad = 0;
+    const auto find = [&]() {
+      bad = 0;
+      const int32_t pos = static_cast<int32_t>(c) * kStep;
+      const int32_t kh = pair / tiles;
+      int32_t pages[kSub];
+#pragma unroll
+      for (int j = 0; j < kSub; ++j) {
+        pages[j] = ScalarLoad(table + ((pos + 16 * j < len ? pos + 16 * j : pos) >> view.page_shift));
+      }
+#pragma unroll
+      for (int j = 0; j < kSub; ++j) {
+        const int32_t p = pos + 16 * j < len ? pos + 16 * j : pos;
+        const bool fine = static_cast<uint32_t>(pages[j]) < static_cast<uint32_t>(view.n_pages);
+        const int32_t page = fine ? pages[j] : 0;
+        bad |= fine ? 0 : 1 << j;
+        at[j] = ((static_cast<int64_t>(page) * view.n_kv + kh) << view.page_shift) + (p & ((1 << view.page_shift) - 1));
+      }
+    };
+    // the address of this lane's position's scale, of tile g (by masks: from a choice among them the compiler makes an
+    // array in memory)
+    uint32_t is_tile[kSub];
+#pragma unroll
+    for (int j = 0; j < kSub; ++j) is_tile[j] = g == j ? ~0u : 0u;
+    const auto scale_of = [&](const float* scales) {
+      uint32_t lo = 0, hi = 0;
+#pragma unroll
+      for (int j = 0; j < kSub; ++j) {
+        lo |= static_cast<uint32_t>(at[j]) & is_tile[j];
+        hi |= static_cast<uint32_t>(at[j] >> 32) & is_tile[j];
+      }
+      return scales + static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo) + n;
+    };
+    const uint32_t k_to = LdsAddress(k_mine), v_to = LdsAddress(v_mine);
+    const auto load_k = [&]() {
+      WaitLdsReads();
+#pragma unroll
+      for (int j = 0; j < kSub; ++j) {
+        const Resource rs = RowsResource(static_cast<const char*>(view.k) + at[j] * kRow, 16 * kRow);
+        LoadToLds<kLoads>(rs, k_from, k_to + j * kLoads * 1024);
+      }
+      if constexpr (kQ8) LoadWordToLds(scale_of(view.k_scale), k_to + kStep * kRow);
+    };
+    const auto load_v = [&]() {
+      WaitLdsReads();
+#pragma unroll
+      for (int j = 0; j < kSub; ++j) {
+        const Resource rs = RowsResource(static_cast<const char*>(view.v) + at[j] * kRow, 16 * kRow);
+        LoadToLds<kLoads>(rs, v_from[j & 1], v_to + j * kLoads * 1024);
+      }
+      if constexpr (kQ8) LoadWordToLds(scale_of(view.v_scale), v_to + kStep * kRow);
+    };
+
+    find();
+    load_k();
+    load_v();
+
+    // per piece: the queries' terms or digits, and the running state
+    Half8 qh[kQ8 ? 1 : kSteps];
+    I32x4 qi[kQ8 ? kTiles : 1][kQ8 ? kSteps : 1];
+    float to_score[kTiles], m[kTiles], l[kTiles];
+    float ref = 0.0f;  // 8-bit values: a power of two above the scales so far
+    F32x4 acc[kTiles][kE];
+    I32x4 sum[kQ8 ? kTiles : 1][kQ8 ? kE : 1];
+    // the digit that this lane's column stands for, and its weight
+    const uint32_t digit = static_cast<uint32_t>(copy) * 0x0101u + 0x0400u;
+    const float digit_by = __int_as_float((127 + 8 * copy) << 23);
+    int64_t head_row = 0;
+    int32_t heads = 0;
+    const auto begin_piece = [&]() {
       const int32_t kh = pair / tiles;
       const int32_t h0 = (pair - kh * tiles) * tile_heads;
-      const int32_t heads = min(tile_heads, group - h0);
-      const int64_t head_row = static_cast<int64_t>(row) * n_heads + kh * group + h0;
-
-      // rows of the pool that the 16-key tiles of a step start at; a tile past the end repeats the step's first, a
-      // page out of range is read as page 0 and its tile marked in *bad
-      auto find = [&](int32_t pos, int64_t (&at)[kSub]) {
-        int bad = 0;
+      heads = min(tile_heads, group - h0);
+      head_row = static_cast<int64_t>(row) * n_heads + kh * group + h0;
+      ref = 0.0f;
 #pragma unroll
-        for (int j = 0; j < kSub; ++j) {
-          const int32_t p = pos + 16 * j < len ? pos + 16 * j : pos;
-          int32_t page = table[p >> view.page_shift];
-          if (page < 0 || page >= view.n_pages) {
-            page = 0;
-            bad |= 1 << j;
-          }
-          at[j] = ((static_cast<int64_t>(page) * view.n_kv + kh) << view.page_shift) +
-                  (p & ((1 << view.page_shift) - 1));
+      for (int t = 0; t < kTiles; ++t) {
+        const int h = t * kHeadCols + head_col;
+        const bool there = h < heads;
+        const float* qr = q + (head_row + (there ? h : 0)) * D;
+        m[t] = -INFINITY;
+        l[t] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kE; ++i) {
+          acc[t][i] = F32x4{0.0f, 0.0f, 0.0f, 0.0f};
+          if constexpr (kQ8) sum[t][i] = I32x4{0, 0, 0, 0};
         }
-        return bad;
-      };
-      uint4 kw[kSub][kKLoads];
-      const uint32_t k_lane = static_cast<uint32_t>(n * kRow + 16 * g);
-      auto load_k = [&](const int64_t (&at)[kSub]) {
-#pragma unroll
-        for (int j = 0; j < kSub; ++j) {
-          const char* p = static_cast<const char*>(view.k) + at[j] * kRow;
-#pragma unroll
-          for (int i = 0; i < kKLoads; ++i) kw[j][i] = *reinterpret_cast<const uint4*>(p + (k_lane + 64u * i));
-        }
-      };
-
-      int32_t pos = c0 << kUnitShift;
-      const int32_t stop = static_cast<int32_t>(min(static_cast<int64_t>(len), static_cast<int64_t>(c1) << kUnitShift));
-      int64_t at[kSub];
-      int bad = find(pos, at);
-      load_k(at);
-
-      // the queries' terms: column n is head n % 8, hi below 8 and lo above
-      Half8 qt[kSteps];
-      float to_score;
-      {
-        const bool there = (n & 7) < heads;
-        const float* qr = q + (head_row + (there ? n & 7 : 0)) * D;
-        float x[kSteps][8];
-        float top = 0.0f;
+        constexpr int kAt = kQ8 ? 16 : 8;  // elements of a lane for one product
+        float x[kSteps][kAt];
+        float top = 0.0f, odd = 0.0f;
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
-          const int d = kQ8 ? 64 * (s / 2) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g;
-          const float4 a = dev::Load4(qr + d), b = dev::Load4(qr + d + 4);
-          const float e[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            x[s][i] = there ? e[i] : 0.0f;
-            top = fmaxf(top, fabsf(x[s][i]));
+          for (int i = 0; i < kAt; i += 4) {
+            const float4 a = dev::Load4(qr + (4 * s + g) * kAt + i);
+            const float e[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              x[s][i + k] = there ? e[k] : 0.0f;
+              top = fmaxf(top, fabsf(x[s][i + k]));
+              if constexpr (kQ8) odd += x[s][i + k] * 0.0f;  // NaN if one of them is no finite number
+            }
           }
         }
         top = MaxAcrossRows(top);
-        const int e = min(max(268 - (__float_as_int(top) >> 23), 1), 254);  // biased exponent of 2^14 over top's
+        // the power of two that brings top to [2^14, 2^15), or [2^29, 2^30)
+        const int e = min(max((kQ8 ? 283 : 268) - (__float_as_int(top) >> 23), 1), 254);
         const float up = __int_as_float(e << 23);
-        to_score = ldexpf(scale_log2, 127 - e);
+        to_score[t] = ldexpf(scale_log2, 127 - e);
+        if constexpr (kQ8) {
+          to_score[t] = to_score[t] * digit_by + SumAcrossRows(odd);
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-          uint32_t w[4];
+          for (int s = 0; s < kSteps; ++s) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = Term2(x[s][2 * i] * up, x[s][2 * i + 1] * up, is_lo);
-          qt[s] = AsHalf8(w[0], w[1], w[2], w[3]);
+            for (int i = 0; i < 4; ++i) {
+              uint32_t w[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                w[k] = static_cast<uint32_t>(static_cast<int>(__builtin_rintf(x[s][4 * i + k] * up))) + 0x80808080u;
+              }
+              qi[t][s][i] = Digit4(w[0], w[1], w[2], w[3], digit);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int s = 0; s < kSteps; ++s) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = Term2(x[s][2 * i] * up, x[s][2 * i + 1] * up, copy != 0);
+            qh[s] = AsHalf8(w[0], w[1], w[2], w[3]);
+          }
         }
       }
-
-      float m = -INFINITY, l = 0.0f;
-      float ref = 0.0f;  // 8-bit values: what acc's weights are relative to, a power of two above the scales so far
-      F32x4 acc[kE];
+    };
+    // takes the int32 sums to acc, which is scaled by `back`
+    const auto take_sums = [&](const float (&back)[kTiles]) {
+      if constexpr (kQ8) {
 #pragma unroll
-      for (int i = 0; i < kE; ++i) acc[i] = F32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int t = 0; t < kTiles; ++t) {
+#pragma unroll
+          for (int i = 0; i < kE; ++i) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              acc[t][i][r] = fmaf(static_cast<float>(sum[t][i][r]), digit_by, acc[t][i][r]) * back[t];
+            }
+            sum[t][i] = I32x4{0, 0, 0, 0};
+          }
+        }
+      }
+    };
 
-      for (; pos < stop; pos += kStep) {
-        const bool tail = pos + kStep > len;
-        // this step's values and scales
-        uint32_t vw[kSub][4][kVWords];
-        const uint32_t v_lane = static_cast<uint32_t>(4 * g * kRow + n * kE * kBytes);
+    // the scales of keys 4 g .. 4 g + 3 of tile j
+    const auto scales_at = [&](const char* stage, int j) {
+      return *reinterpret_cast<const float4*>(stage + kStep * kRow + 64 * j + 16 * g);
+    };
+
+    begin_piece();
+    uint32_t c_first = c;
+    F32x4 kept[kTiles][kOwn];
+    float kept_m[kTiles], kept_l[kTiles];
+    int32_t since = 0;  // steps since the int32 sums were last taken
+
+    while (true) {
+      const int32_t pos = static_cast<int32_t>(c) * kStep;
+      const bool tail = pos + kStep > len;
+      const int32_t left = len - pos;  // positions from here
+      const int this_bad = bad;
+      // ---- scores, once the keys are there: the values' loads are younger
+      WaitLoads<kStageLoads>();
+      float s[kTiles][kSub][4];
+      if constexpr (kQ8) {
+        I32x4 raw[kTiles][kSub];
 #pragma unroll
         for (int j = 0; j < kSub; ++j) {
-          const char* p = static_cast<const char*>(view.v) + at[j] * kRow;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const char* a = p + (v_lane + static_cast<uint32_t>(i * kRow));
-            if constexpr (kVWords == 4) {
-              const uint4 w = *reinterpret_cast<const uint4*>(a);
-              vw[j][i][0] = w.x, vw[j][i][1] = w.y, vw[j][i][2] = w.z, vw[j][i][3] = w.w;
-            } else if constexpr (kVWords == 2) {
-              const uint2 w = *reinterpret_cast<const uint2*>(a);
-              vw[j][i][0] = w.x, vw[j][i][1] = w.y;
-            } else {
-              vw[j][i][0] = *reinterpret_cast<const uint32_t*>(a);
+          for (int t = 0; t < kTiles; ++t) raw[t][j] = I32x4{0, 0, 0, 0};
+#pragma unroll
+          for (int i = 0; i < kSteps; ++i) {
+            const I32x4 a = *reinterpret_cast<const I32x4*>(k_mine + j * 16 * kRow + (k_at ^ (64u * i)));
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) {
+              raw[t][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, qi[t][i], raw[t][j], 0, 0, 0);
             }
           }
         }
-        float4 ks[kQ8 ? kSub : 1], vs[kQ8 ? kSub : 1];
-        if constexpr (kQ8) {
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
 #pragma unroll
           for (int j = 0; j < kSub; ++j) {
-            ks[j] = dev::Load4(view.k_scale + at[j] + 4 * g);
-            vs[j] = dev::Load4(view.v_scale + at[j] + 4 * g);
-          }
-        }
-        // scores
-        F32x4 s4[kSub];
 #pragma unroll
-        for (int j = 0; j < kSub; ++j) {
-          s4[j] = F32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-          for (int i = 0; i < kKLoads; ++i) {
-            const uint4 w = kw[j][i];
-            if constexpr (kQ8) {
-              const uint32_t f[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const Half8 a = AsHalf8(CodePair<0>(f[2 * h]), CodePair<1>(f[2 * h]), CodePair<0>(f[2 * h + 1]),
-                                        CodePair<1>(f[2 * h + 1]));
-                s4[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qt[2 * i + h], s4[j], 0, 0, 0);
-              }
-            } else {
-              s4[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(AsHalf8(w.x, w.y, w.z, w.w), qt[i], s4[j], 0, 0, 0);
+            for (int i = 0; i < 4; ++i) {
+              float x = static_cast<float>(raw[t][j][i]) * to_score[t];
+              x += Ror<8>(x);
+              s[t][j][i] = x + Ror<4>(x);
             }
           }
         }
-        // the next step's keys
-        const int this_bad = bad;
-        if (pos + kStep < stop) {
-          bad = find(pos + kStep, at);
-          load_k(at);
-        }
-        float s[kSub][4];
-        float top = m;
+      } else {
 #pragma unroll
         for (int j = 0; j < kSub; ++j) {
-          const float by[4] = {kQ8 ? ks[kQ8 ? j : 0].x : 0.0f, kQ8 ? ks[kQ8 ? j : 0].y : 0.0f,
-                               kQ8 ? ks[kQ8 ? j : 0].z : 0.0f, kQ8 ? ks[kQ8 ? j : 0].w : 0.0f};
+          F32x4 raw = F32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int i = 0; i < kSteps; ++i) {
+            const Half8 a = *reinterpret_cast<const Half8*>(k_mine + j * 16 * kRow + (k_at ^ (64u * i)));
+            raw = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[i], raw, 0, 0, 0);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[0][j][i] = (raw[i] + Ror<8>(raw[i])) * to_score[0];
+        }
+      }
+      // ---- the next unit, and its keys
+      ++u;
+      const bool more = u < u_end;
+      const uint32_t c_end = c + 1;
+      const uint32_t piece_units = units;
+      const int32_t piece_row = row, piece_pair = pair;
+      bool turn = !more;  // this unit is its piece's last
+      float4 ks[kQ8 ? kSub : 1], vs[kQ8 ? kSub : 1];
+      if constexpr (kQ8) {
+#pragma unroll
+        for (int j = 0; j < kSub; ++j) ks[j] = scales_at(k_mine, j);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (more) {
+        ++c;
+        if (c == units) {
+          turn = true;
+          c = 0;
+          if (++pair == rows.pairs) {
+            pair = 0;
+            do {
+              ++row;
+              units = row < rows.n_rows ? rows.ScalarUnitsOf(row) : 1;
+            } while (units == 0);
+            row = min(row, rows.n_rows - 1);  // past the last only if the lengths change while this runs
+            len = ScalarLoad(rows.lens + row);
+            table = view.pages + rows.ScalarSeq(row) * view.max_pages;
+          }
+        }
+        find();
+        load_k();
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      // ---- weights
+      float top[kTiles];
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) {
+        top[t] = m[t];
+#pragma unroll
+        for (int j = 0; j < kSub; ++j) {
+          const float by[4] = {kQ8 ? ks[kQ8 ? j : 0].x : 1.0f, kQ8 ? ks[kQ8 ? j : 0].y : 1.0f,
+                               kQ8 ? ks[kQ8 ? j : 0].z : 1.0f, kQ8 ? ks[kQ8 ? j : 0].w : 1.0f};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            float x = (s4[j][i] + Ror8(s4[j][i])) * to_score;
-            if constexpr (kQ8) x *= by[i];
-            if (this_bad & (1 << j)) x = NAN;
-            if (tail && pos + 16 * j + 4 * g + i >= len) x = -INFINITY;
-            s[j][i] = x;
-            top = fmaxf(top, x);
+            if constexpr (kQ8) s[t][j][i] *= by[i];
+            if (this_bad & (1 << j)) s[t][j][i] = NAN;
+            if (tail && 16 * j + 4 * g + i >= left) s[t][j][i] = -INFINITY;
+            top[t] = fmaxf(top[t], s[t][j][i]);
           }
         }
-        top = MaxAcrossRows(top);
-        const float safe = top == -INFINITY ? 0.0f : top;
-        float back = __builtin_amdgcn_exp2f(m - safe);
-        m = top;
-        l *= back;
-        float up = 0x1p14f;
-        if constexpr (kQ8) {
-          if (tail) {
+        top[t] = MaxAcrossRows(top[t]);
+      }
+      // the values are there: the next keys' loads, if any, are younger
+      if (more) {
+        WaitLoads<kStageLoads>();
+      } else {
+        WaitLoads<0>();
+      }
+      if constexpr (kQ8) {
 #pragma unroll
-            for (int j = 0; j < kSub; ++j) {
-              const int32_t p = pos + 16 * j + 4 * g;
-              vs[j].x = p < len ? vs[j].x : 0.0f;
-              vs[j].y = p + 1 < len ? vs[j].y : 0.0f;
-              vs[j].z = p + 2 < len ? vs[j].z : 0.0f;
-              vs[j].w = p + 3 < len ? vs[j].w : 0.0f;
-            }
-          }
-          float big = 0.0f;
+        for (int j = 0; j < kSub; ++j) vs[j] = scales_at(v_mine, j);
+      }
+      float safe[kTiles];
+      float up = 0x1p14f;
+      if constexpr (kQ8) {
+        if (tail) {
 #pragma unroll
-          for (int j = 0; j < kSub; ++j) big = fmaxf(big, fmaxf(fmaxf(vs[j].x, vs[j].y), fmaxf(vs[j].z, vs[j].w)));
-          big = MaxAcrossRows(big);
-          if (big >= ref) {  // the same in every lane
-            const int e = min(max((__float_as_int(big) >> 23) + 1, 27), 254);
-            const float to = __int_as_float(e << 23);
-            back *= ref * __int_as_float((254 - e) << 23);  // ref / to
-            ref = to;
+          for (int j = 0; j < kSub; ++j) {
+            const int32_t p = 16 * j + 4 * g;
+            vs[j].x = p < left ? vs[j].x : 0.0f;
+            vs[j].y = p + 1 < left ? vs[j].y : 0.0f;
+            vs[j].z = p + 2 < left ? vs[j].z : 0.0f;
+            vs[j].w = p + 3 < left ? vs[j].w : 0.0f;
           }
-          up *= __int_as_float((254 << 23) - __float_as_int(ref));  // 2^14 / ref
         }
+        // as whole numbers, where a NaN is larger than any number
+        uint32_t big = 0;
+#pragma unroll
+        for (int j = 0; j < kSub; ++j) {
+          big = max(max(big, max(__float_as_uint(vs[j].x), __float_as_uint(vs[j].y))),
+                    max(__float_as_uint(vs[j].z), __float_as_uint(vs[j].w)));
+        }
+        big = __float_as_uint(AcrossRows(__uint_as_float(big), [](float a, float b) {
+          return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b)));
+        }));
+        bool flush = big >= __float_as_uint(ref) || ++since >= 1024;  // 1024 steps: int32 holds 2^17 products of 2^14
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) flush |= top[t] > m[t] + 3.0f;
+        if (__any(flush)) {
+          float back[kTiles], by = 1.0f;
+          if (big >= __float_as_uint(ref)) {
+            const int e = min(max(static_cast<int>(big >> 23) + 1, 27), 254);
+            by = ref * __int_as_float((254 - e) << 23);
+            ref = __int_as_float(e << 23);
+          }
+#pragma unroll
+          for (int t = 0; t < kTiles; ++t) {
+            const float to = top[t] > m[t] + 3.0f ? top[t] : m[t];
+            const float by_max = __builtin_amdgcn_exp2f(m[t] - (to == -INFINITY ? 0.0f : to));
+            m[t] = to;
+            l[t] *= by_max;
+            back[t] = by * by_max;
+          }
+          take_sums(back);
+          since = 0;
+        }
+        if (big >= 0x7F800000u) {
+#pragma unroll
+          for (int t = 0; t < kTiles; ++t) l[t] = NAN;
+        }
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) safe[t] = m[t] == -INFINITY ? 0.0f : m[t];
+        up = 0x1p27f * __int_as_float((254 << 23) - __float_as_int(ref));  // 2^27 / ref
+      } else {
+        if (tail) {  // what stands behind the last position may not even be a number
+#pragma unroll
+          for (int i = 0; i < kStep * kRow / 1024; ++i) {
+            const int to = 1024 * i + 16 * lane;
+            if (to / kRow >= left) *reinterpret_cast<uint4*>(v_mine + to) = make_uint4(0u, 0u, 0u, 0u);
+          }
+        }
+        safe[0] = top[0] == -INFINITY ? 0.0f : top[0];
+        const float back = __builtin_amdgcn_exp2f(m[0] - safe[0]);
+        m[0] = top[0];
+        l[0] *= back;
         if (__any(back != 1.0f)) {
 #pragma unroll
-          for (int i = 0; i < kE; ++i) acc[i] *= back;
+          for (int i = 0; i < kE; ++i) acc[0][i] *= back;
         }
-        // weights: p, and its terms in the order of the lane's keys
+      }
+      // ---- the output's sums
+      if constexpr (kQ8) {
+        I32x4 w[kTiles];  // tile j of 16 keys: bytes 4 j ..
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+#pragma unroll
+          for (int j = 0; j < kSub; ++j) {
+            const float by[4] = {vs[j].x, vs[j].y, vs[j].z, vs[j].w};
+            uint32_t d[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float p = __builtin_amdgcn_exp2f(s[t][j][i] - safe[t]);
+              l[t] += p;
+              d[i] = static_cast<uint32_t>(static_cast<int>(fmaf(p * by[i], up, 0.5f))) + 0x80808080u;
+            }
+            w[t][j] = Digit4(d[0], d[1], d[2], d[3], digit);
+          }
+        }
+        I32x2 a[kE][2];
+#pragma unroll
+        for (int i = 0; i < kE; ++i) {
+          const char* from = v_mine + (v_at ^ (16u * i));
+          a[i][0] = ReadBytesAcross(from);
+          a[i][1] = ReadBytesAcross(from + 32 * kRow);
+        }
+#pragma unroll
+        for (int i = 0; i < kE; ++i) {
+#pragma unroll
+          for (int t = 0; t < kTiles; ++t) {
+            sum[t][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(I32x4{a[i][0][0], a[i][0][1], a[i][1][0], a[i][1][1]}, w[t],
+                                                              sum[t][i], 0, 0, 0);
+          }
+        }
+      } else {
         uint32_t pt[kSub][2];
 #pragma unroll
         for (int j = 0; j < kSub; ++j) {
           float w[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            w[i] = __builtin_amdgcn_exp2f(s[j][i] - safe);
-            l += w[i];
+            w[i] = __builtin_amdgcn_exp2f(s[0][j][i] - safe[0]);
+            l[0] += w[i];
           }
-          if constexpr (kQ8) {
-            w[0] *= vs[j].x, w[1] *= vs[j].y, w[2] *= vs[j].z, w[3] *= vs[j].w;
-          }
-          pt[j][0] = Term2(w[0] * up, w[1] * up, is_lo);
-          pt[j][1] = Term2(w[2] * up, w[3] * up, is_lo);
-        }
-        if (tail) {  // what stands behind the last position is not even a number
-#pragma unroll
-          for (int j = 0; j < kSub; ++j) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const bool keep = pos + 16 * j + 4 * g + i < len;
-#pragma unroll
-              for (int w = 0; w < kVWords; ++w) vw[j][i][w] = keep ? vw[j][i][w] : 0u;
-            }
-          }
+          pt[j][0] = Term2(w[0] * up, w[1] * up, copy != 0);
+          pt[j][1] = Term2(w[2] * up, w[3] * up, copy != 0);
         }
 #pragma unroll
         for (int t = 0; t < kSub / 2; ++t) {
           const Half8 b = AsHalf8(pt[2 * t][0], pt[2 * t][1], pt[2 * t + 1][0], pt[2 * t + 1][1]);
-          auto& v0 = vw[2 * t];
-          auto& v1 = vw[2 * t + 1];
-          if constexpr (kQ8) {
+          uint2 a[kE][2];
 #pragma unroll
-            for (int w = 0; w < kVWords; ++w) {
-              uint32_t f[8];
+          for (int i = 0; i < kE; ++i) {
+            const char* from = v_mine + t * 32 * kRow + (v_at ^ (32u * i));
+            a[i][0] = ReadHalvesAcross(from);
+            a[i][1] = ReadHalvesAcross(from + 16 * kRow);
+          }
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                f[i] = v0[i][w] ^ 0x80808080u;
-                f[4 + i] = v1[i][w] ^ 0x80808080u;
-              }
-              auto one = [&](auto byte) {
-                constexpr int kI = decltype(byte)::value;
-                const Half8 a = AsHalf8(CodeOfTwo<kI>(f[0], f[1]), CodeOfTwo<kI>(f[2], f[3]),
-                                        CodeOfTwo<kI>(f[4], f[5]), CodeOfTwo<kI>(f[6], f[7]));
-                acc[4 * w + kI] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, acc[4 * w + kI], 0, 0, 0);
-              };
-              one(std::integral_constant<int, 0>{});
-              one(std::integral_constant<int, 1>{});
-              one(std::integral_constant<int, 2>{});
-              one(std::integral_constant<int, 3>{});
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < kE; ++i) {
-              const uint32_t sel = i & 1 ? 0x07060302u : 0x05040100u;
-              const int w = i / 2;
-              const Half8 a = AsHalf8(__builtin_amdgcn_perm(v0[1][w], v0[0][w], sel),
-                                      __builtin_amdgcn_perm(v0[3][w], v0[2][w], sel),
-                                      __builtin_amdgcn_perm(v1[1][w], v1[0][w], sel),
-                                      __builtin_amdgcn_perm(v1[3][w], v1[2][w], sel));
-              acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, acc[i], 0, 0, 0);
-            }
+          for (int i = 0; i < kE; ++i) {
+            acc[0][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                AsHalf8(a[i][0].x, a[i][0].y, a[i][1].x, a[i][1].y), b, acc[0][i], 0, 0, 0);
           }
         }
       }
+      __builtin_amdgcn_sched_barrier(0);
+      if (more) load_v();
+      if (!turn) continue;
 
-      // the piece's (m, l, o): out, or to LDS where it is not the whole of its pair
-      const float total = SumAcrossRows(l);
-      const bool whole = c0 == 0 && c1 == units;
-      const float unit = kQ8 ? ref * 0x1p-5f : 0x1p-14f;
-      const float by = whole ? unit / total : unit;
-      float* to = whole ? out + (head_row + n) * D : &part[wave][my_held][n & 7][0];
-      float o[4][kE];
+      // ---- the piece's (m, l, o): out, or kept where it is not the whole of its pair
+      if constexpr (kQ8) {
+        float same[kTiles];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-#pragma unroll
-        for (int i = 0; i < kE; ++i) o[r][i] = (acc[i][r] + Ror8(acc[i][r])) * by;
+        for (int t = 0; t < kTiles; ++t) same[t] = 1.0f;
+        take_sums(same);
       }
-      if (n < heads) {
+      const bool whole = c_first == 0 && c_end == piece_units;
+      const float unit = kQ8 ? ref * 0x1p-27f : 0x1p-14f;
+      if (!whole) {
+        const int which = more ? 0 : 1;
+        if (lane == 0) pieces[wave][which] = Piece{u - c_end, c_first, c_end, piece_units, piece_row, piece_pair};
+        my_held |= 1 << which;
+      }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
+      for (int t = 0; t < kTiles; ++t) {
+        const float total = SumAcrossRows(l[t]);
+        const float by = whole ? unit / total : unit;
+        const int h = t * kHeadCols + head_col;
+        F32x4 own[kOwn];
 #pragma unroll
-          for (int i = 0; i < kE; i += 4) {
-            *reinterpret_cast<float4*>(to + kE * (4 * g + r) + i) =
-                make_float4(o[r][i], o[r][i + 1], o[r][i + 2], o[r][i + 3]);
+        for (int i = 0; i < kE; ++i) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float x = acc[t][i][r];
+            x += Ror<8>(x);
+            if constexpr (kQ8) x += Ror<4>(x);
+            x *= by;
+            own[i % kOwn][r] = i < kOwn || copy == i / kOwn ? x : own[i % kOwn][r];
           }
         }
-        if (!whole && g == 0) {
-          to[D] = m;
-          to[D + 1] = total;
+        if (!whole && more) {
+#pragma unroll
+          for (int i = 0; i < kOwn; ++i) kept[t][i] = own[i];
+          kept_m[t] = m[t];
+          kept_l[t] = total;
+        } else if (h < heads) {
+          float* to = whole ? out + (head_row + h) * D : reinterpret_cast<float*>(v_mine) + h * kPart;
+#pragma unroll
+          for (int i = 0; i < kOwn; ++i) *reinterpret_cast<F32x4*>(to + 16 * (copy * kOwn + i) + 4 * g) = own[i];
+          if (!whole && copy == 0 && g == 0) {
+            to[D] = m[t];
+            to[D + 1] = total;
+          }
         }
       }
-      if (!whole) {
-        if (lane == 0) {
-          pieces[wave][my_held] = Piece{u - c0, row, pair, c0, c1, units};
+      if (!more) break;
+      c_first = c;
+      begin_piece();
+    }
+    // the first piece, now that its keys' place is free
+    if (my_held & 1) {
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) {
+        const int h = t * kHeadCols + head_col;
+        if (h < tile_heads) {  // what lies past the piece's heads is not read
+          float* to = reinterpret_cast<float*>(k_mine) + h * kPart;
+#pragma unroll
+          for (int i = 0; i < kOwn; ++i) *reinterpret_cast<F32x4*>(to + 16 * (copy * kOwn + i) + 4 * g) = kept[t][i];
+          if (copy == 0 && g == 0) {
+            to[D] = kept_m[t];
+            to[D + 1] = kept_l[t];
+          }
         }
-        ++my_held;
-      }
-      u += c1 - c0;
-      if (u >= u_end) break;
-      c0 = 0;
-      if (++pair == rows.pairs) {
-        pair = 0;
-        do {
-          ++row;
-          units = row < rows.n_rows ? __builtin_amdgcn_readfirstlane(rows.UnitsOf(row)) : 1;
-        } while (units == 0);
-        if (row >= rows.n_rows) break;  // only if the lengths change while this runs
       }
     }
   }
@@ -604,11 +898,12 @@ __global__ __launch_bounds__(64 * kWaves) void PagedAttentionKernel(PagedView vi
   __syncthreads();
 
   // The workgroup's pieces in order, neighbours of one pair joined.
+  const auto part = [&](int i) { return reinterpret_cast<const float*>(i & 1 ? v_lds[i >> 1] : k_lds[i >> 1]); };
   float* const slots = reinterpret_cast<float*>(workspace + kMaxGroups * kCounterBytes);
   const int64_t slot_floats = static_cast<int64_t>(tile_heads) * kPart;
   int from = 0;  // wave * 2 + which
   while (from < 2 * kWaves) {
-    if ((from & 1) >= held[from >> 1]) {
+    if (!(held[from >> 1] >> (from & 1) & 1)) {
       ++from;
       continue;
     }
@@ -616,7 +911,7 @@ __global__ __launch_bounds__(64 * kWaves) void PagedAttentionKernel(PagedView vi
     int list = 1 << from;
     int to = from + 1;
     for (; to < 2 * kWaves; ++to) {
-      if ((to & 1) >= held[to >> 1]) continue;
+      if (!(held[to >> 1] >> (to & 1) & 1)) continue;
       const Piece next = UniformPiece(pieces[to >> 1][to & 1]);
       if (next.first != run.first) break;
       run.c1 = next.c1;
@@ -629,20 +924,20 @@ __global__ __launch_bounds__(64 * kWaves) void PagedAttentionKernel(PagedView vi
     const int64_t head_row = static_cast<int64_t>(run.row) * n_heads + kh * group + h0;
     const bool whole = run.c0 == 0 && run.c1 == run.n;
     const bool leads = run.first + run.c0 == begin;  // the workgroup's first piece
-    float* slot = slots + (2 * me + (leads ? 0 : 1)) * slot_floats;
+    float* slot = slots + (2 * static_cast<int64_t>(me) + (leads ? 0 : 1)) * slot_floats;
     const __amdgpu_buffer_rsrc_t rs = dev::OutResource(slot, static_cast<uint32_t>(slot_floats * 4));
     for (int i = threadIdx.x; i < heads * (D / 4); i += 64 * kWaves) {
       const int h = i / (D / 4), d = 4 * (i % (D / 4));
       float top = -INFINITY;
       for (int k = 0; k < 2 * kWaves; ++k) {
-        if (list >> k & 1) top = fmaxf(top, part[k >> 1][k & 1][h][D]);
+        if (list >> k & 1) top = fmaxf(top, part(k)[h * kPart + D]);
       }
       const float safe = top == -INFINITY ? 0.0f : top;
       float l = 0.0f;
       float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       for (int k = 0; k < 2 * kWaves; ++k) {
         if (!(list >> k & 1)) continue;
-        const float* p = part[k >> 1][k & 1][h];
+        const float* p = part(k) + h * kPart;
         const float f = __builtin_amdgcn_exp2f(p[D] - safe);
         const float4 x = *reinterpret_cast<const float4*>(p + d);
         l = fmaf(p[D + 1], f, l);
@@ -664,38 +959,61 @@ __global__ __launch_bounds__(64 * kWaves) void PagedAttentionKernel(PagedView vi
     // then reads, with device-coherent loads, is all there. No workgroup waits for another.
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    const int64_t wa = share.Holder(run.first), wb = share.Holder(run.first + run.n - 1);
+    const uint32_t wa = share.Holder(run.first), wb = share.Holder(run.first + run.n - 1);
     uint32_t* counter = reinterpret_cast<uint32_t*>(workspace + wa * kCounterBytes);
     if (threadIdx.x == 0) {
-      last_flag = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
-                  static_cast<uint32_t>(wb - wa);
+      last_flag = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == wb - wa;
     }
     __syncthreads();
     if (last_flag) {
-      // wa's part is in its first slot only if the pair starts where its share does
-      const bool first_leads = share.Begin(wa) == run.first;
-      const __amdgpu_buffer_rsrc_t all =
-          dev::OutResource(slots + 2 * wa * slot_floats, static_cast<uint32_t>((2 * (wb - wa) + 2) * slot_floats * 4));
+      // The parts in order. wa's is in its first slot only if the pair starts where its share does. Four elements of a
+      // head to a thread, and as many sets of threads as there are, each taking every sets-th part, kBatch of them
+      // requested at a time: a round trip past the L2 costs more than the arithmetic.
+      constexpr int kBatch = 8;
+      const uint32_t first_leads = share.Begin(wa) == run.first ? 0u : 1u;
+      const __amdgpu_buffer_rsrc_t all = dev::OutResource(
+          slots + 2 * static_cast<int64_t>(wa) * slot_floats, static_cast<uint32_t>((2 * (wb - wa) + 2) * slot_floats * 4));
       const int parts = static_cast<int>(wb - wa) + 1;
-      auto slot_at = [&](int w) {
-        return static_cast<uint32_t>((2 * w + (w == 0 && !first_leads ? 1 : 0)) * slot_floats * 4);
+      const int columns = heads * (D / 4);
+      const int sets = 64 * kWaves / columns;
+      const int set = static_cast<int>(threadIdx.x) / columns, column = static_cast<int>(threadIdx.x) % columns;
+      const int h = column / (D / 4), d = 4 * (column % (D / 4));
+      const uint32_t ml_at = 4u * static_cast<uint32_t>(h * kPart + D), o_at = 4u * static_cast<uint32_t>(h * kPart + d);
+      const uint32_t slot_bytes = static_cast<uint32_t>(slot_floats * 4);
+      float top = -INFINITY, l = 0.0f;
+      float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      const auto join = [&](float m2, float l2, float4 o2) {
+        const float to = fmaxf(top, m2);
+        const float safe = to == -INFINITY ? 0.0f : to;
+        const float f = __builtin_amdgcn_exp2f(top - safe), f2 = __builtin_amdgcn_exp2f(m2 - safe);
+        top = to;
+        l = fmaf(l2, f2, l * f);
+        o = make_float4(fmaf(o2.x, f2, o.x * f), fmaf(o2.y, f2, o.y * f), fmaf(o2.z, f2, o.z * f),
+                        fmaf(o2.w, f2, o.w * f));
       };
-      for (int i = threadIdx.x; i < heads * (D / 4); i += 64 * kWaves) {
-        const int h = i / (D / 4), d = 4 * (i % (D / 4));
-        const uint32_t ml = 4u * static_cast<uint32_t>(h * kPart + D), at = 4u * static_cast<uint32_t>(h * kPart + d);
-        float top = -INFINITY;
-        for (int w = 0; w < parts; ++w) {
-          top = fmaxf(top, dev::LoadBuf1<dev::kLoadDevicePolicy>(all, slot_at(w) + ml));
+      if (set < sets) {
+        for (int w = set; w < parts; w += kBatch * sets) {
+          uint2 ml[kBatch];
+          float4 x[kBatch];
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) {
+            const int p = min(w + i * sets, parts - 1);
+            const uint32_t at = (2u * static_cast<uint32_t>(p) + (p == 0 ? first_leads : 0u)) * slot_bytes;
+            ml[i] = dev::LoadBufU2<dev::kLoadDevicePolicy>(all, at + ml_at);
+            x[i] = dev::LoadBuf4<dev::kLoadDevicePolicy>(all, at + o_at);
+          }
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) {
+            if (w + i * sets < parts) join(__uint_as_float(ml[i].x), __uint_as_float(ml[i].y), x[i]);
+          }
         }
-        const float safe = top == -INFINITY ? 0.0f : top;
-        float l = 0.0f;
-        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int w = 0; w < parts; ++w) {
-          const uint2 x2 = dev::LoadBufU2<dev::kLoadDevicePolicy>(all, slot_at(w) + ml);
-          const float f = __builtin_amdgcn_exp2f(__uint_as_float(x2.x) - safe);
-          const float4 x = dev::LoadBuf4<dev::kLoadDevicePolicy>(all, slot_at(w) + at);
-          l = fmaf(__uint_as_float(x2.y), f, l);
-          o = make_float4(fmaf(x.x, f, o.x), fmaf(x.y, f, o.y), fmaf(x.z, f, o.z), fmaf(x.w, f, o.w));
+        joins[threadIdx.x] = Join{o, top, l};
+      }
+      __syncthreads();
+      if (set == 0) {
+        for (int i = 1; i < min(sets, parts); ++i) {
+          const Join& j = joins[i * columns + column];
+          join(j.m, j.l, j.o);
         }
         const float inv = 1.0f / l;
         dev::Store4(out + (head_row + h) * D + d, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
@@ -771,18 +1089,20 @@ void GpuAttentionPaged(const GpuPagedKv& kv, const GpuPageTable& table, const in
   int32_t tiles, tile_heads;
   TilesOf(n_heads / kv.n_kv_heads, &tiles, &tile_heads);
   const Rows rows{seq_ids, lens, table.n_seqs, table.max_pages * kv.page_size, static_cast<int32_t>(n_rows),
-                  kv.n_kv_heads * tiles};
-  // no more workgroups than the longest possible rows would give four units to
-  const int64_t most = (std::min<int64_t>(rows.capacity, 0x7FFFFFFF) + 63) / 64;
-  int64_t groups = kMaxGroups;
-  if (most * rows.pairs < int64_t{4} * kMaxGroups) {
-    groups = std::min<int64_t>(groups, (n_rows * most * rows.pairs + kWaves - 1) / kWaves);
-  }
+                  kv.n_kv_heads * tiles, kv.head_dim == 128 && kv.type == kKvF16 ? 5 : 6};
+  const int64_t most = (std::min<int64_t>(rows.capacity, 0x7FFFFFFF) >> rows.unit_shift) + 1;
+  RPG_CHECK(n_rows <= 0x7FFFFFFF / most / rows.pairs,
+            "AttentionPaged: %lld rows of up to %lld positions and %d heads are too many for one call",
+            static_cast<long long>(n_rows), static_cast<long long>(rows.capacity), rows.pairs);
+  // no more workgroups than the longest possible rows would give work to
+  const int64_t groups = std::min<int64_t>(kMaxGroups, (n_rows * most * rows.pairs + TUNE_MIN - 1) / TUNE_MIN);
   const float scale_log2 =
       static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(kv.head_dim)));
-  const bool q8 = kv.type == kKvQ8;
-  auto* kern = kv.head_dim == 128 ? (q8 ? PagedAttentionKernel<128, true> : PagedAttentionKernel<128, false>)
-                                  : (q8 ? PagedAttentionKernel<64, true> : PagedAttentionKernel<64, false>);
+  auto* kern = kv.head_dim == 128 ? PagedAttentionKernel<128, false, 1> : PagedAttentionKernel<64, false, 1>;
+  if (kv.type == kKvQ8) {
+    kern = tile_heads > 4 ? (kv.head_dim == 128 ? PagedAttentionKernel<128, true, 2> : PagedAttentionKernel<64, true, 2>)
+                          : (kv.head_dim == 128 ? PagedAttentionKernel<128, true, 1> : PagedAttentionKernel<64, true, 1>);
+  }
   Launch("PagedAttentionKernel", kern, dim3(static_cast<unsigned>(groups)), dim3(64 * kWaves), dev::ViewOf(kv, table),
          rows, q_dev, n_heads, tiles, tile_heads, scale_log2, out_dev, static_cast<char*>(workspace));
 }
