@@ -62,9 +62,16 @@ constexpr int kTileHeads = 8;
 constexpr int kMaxGroups = 512;
 // Bytes between two counters: on lines of their own, as the decode attention's.
 constexpr size_t kCounterBytes = 256;
-#ifndef TUNE_MIN
-#define TUNE_MIN 4
+#ifndef TUNE_WHOLE
+#define TUNE_WHOLE 4u
 #endif
+#ifndef TUNE_MANY
+#define TUNE_MANY 8192u
+#endif
+// Stores of a part to the workspace: device scope. With the streaming hint too their
+// acknowledgement came later (1 x 32768 positions of one kv head 24.2 against 21.7 us).
+constexpr int kPartPolicy = 16;
+
 #ifndef TUNE_NT
 #define TUNE_NT " nt"
 #endif
@@ -76,7 +83,12 @@ using I32x4 = int __attribute__((ext_vector_type(4)));
 using I32x2 = int __attribute__((ext_vector_type(2)));
 using S16x4 = short __attribute__((ext_vector_type(4)));
 
-constexpr int PartFloats(int d) { return d + 4; }  // o[d], m, l, and two to keep rows 16-byte aligned
+constexpr int PartFloats(int d) { return d + 4; }  // in LDS: o[d], m, l, and two to keep rows 16-byte aligned
+constexpr uint32_t kLine = 128;
+// In the workspace: o[heads][d], and a line of (m, l)
+__host__ __device__ constexpr uint32_t SlotBytes(int32_t d, int32_t heads) {
+  return static_cast<uint32_t>(heads * d) * 4u + kLine;
+}
 
 // ---------------------------------------------------------------- lane exchange
 
@@ -211,42 +223,66 @@ __device__ __forceinline__ I32x2 ReadBytesAcross(const char* at) {
 
 // ---------------------------------------------------------------- sharing out
 
+__device__ __forceinline__ uint32_t Scalar(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// How a pair's units are cut into items, of which a workgroup takes whole ones. From kManyUnits in the batch on an item is
+// a unit, so that all workgroups get alike. With fewer, joining what two workgroups hold of a pair (a round trip to memory
+// to store, one to count, one to read) costs more than some units more in turn: a pair of up to kWholeUnits is one item, a
+// longer one is cut evenly into items of at most 2^step, about what each workgroup then gets.
+constexpr uint32_t kManyUnits = TUNE_MANY;
+constexpr uint32_t kWholeUnits = TUNE_WHOLE;
+
+struct Cut {
+  bool units;
+  uint32_t step;
+
+  // for a batch of `all` units
+  __device__ __forceinline__ explicit Cut(uint32_t all) {
+    units = all >= kManyUnits;
+    step = all <= 4 * kMaxGroups ? 2 : all <= 8 * kMaxGroups ? 3 : 4;
+  }
+  __device__ __forceinline__ uint32_t Items(uint32_t n) const {
+    return units ? n : n <= kWholeUnits ? min(n, 1u) : (n + (1u << step) - 1u) >> step;
+  }
+};
+
 // Everything here is the same in every lane of a wave, and kept in scalar registers.
 struct Share {
-  uint32_t total;  // units
-  uint32_t per;    // a workgroup's units: per, and one more in the first `rem` of them
+  uint32_t per;  // a workgroup's items: per, and one more in the first `rem` of them
   uint32_t rem;
-  uint32_t groups;
 
+  __device__ __forceinline__ Share(uint32_t items, uint32_t groups) {
+    per = Scalar(items / groups);
+    rem = items - per * groups;
+  }
   __device__ __forceinline__ uint32_t Begin(uint32_t w) const { return w * per + min(w, rem); }
-  // The workgroup whose share holds unit x.
+  // The workgroup whose share holds item x.
   __device__ __forceinline__ uint32_t Holder(uint32_t x) const {
     const uint32_t big = rem * (per + 1);
     return Scalar(x < big ? x / (per + 1) : rem + (x - big) / per);
   }
-  static __device__ __forceinline__ uint32_t Scalar(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
 };
 
 struct Rows {
   const int32_t* seq_ids;
   const int32_t* lens;
-  int64_t n_seqs;
-  int64_t capacity;  // positions that a table row has pages for
+  int32_t n_seqs;
+  int32_t capacity;  // positions that a table row has pages for, at most the largest int32
   int32_t n_rows;
   int32_t pairs;       // (kv head, tile) pairs of a row
   int32_t unit_shift;  // log2 of a unit's positions
 
-  __device__ __forceinline__ int64_t Seq(int32_t r) const { return seq_ids != nullptr ? seq_ids[r] : r; }
-  __device__ __forceinline__ bool Fine(int64_t seq, int32_t len) const {
+  __device__ __forceinline__ int32_t Seq(int32_t r) const { return seq_ids != nullptr ? seq_ids[r] : r; }
+  __device__ __forceinline__ bool Fine(int32_t seq, int32_t len) const {
     return seq >= 0 && seq < n_seqs && len >= 0 && len <= capacity;
   }
   // Units of one pair of row r; none for a row that is padding, empty or out of range.
-  __device__ __forceinline__ uint32_t UnitsOf(int64_t seq, int32_t len) const {
+  __device__ __forceinline__ uint32_t UnitsOf(int32_t seq, int32_t len) const {
     return Fine(seq, len) ? (static_cast<uint32_t>(len) + (1u << unit_shift) - 1u) >> unit_shift : 0u;
   }
   __device__ __forceinline__ uint32_t UnitsOf(int32_t r) const { return UnitsOf(Seq(r), lens[r]); }
   // for an r that is the same in every lane
-  __device__ __forceinline__ int64_t ScalarSeq(int32_t r) const {
+  __device__ __forceinline__ int32_t ScalarSeq(int32_t r) const {
     return seq_ids != nullptr ? ScalarLoad(seq_ids + r) : r;
   }
   __device__ __forceinline__ uint32_t ScalarUnitsOf(int32_t r) const {
@@ -266,40 +302,126 @@ __device__ __forceinline__ uint32_t ScanAdd(uint32_t x) {
   return static_cast<uint32_t>(v);
 }
 
-// Units of rows [lo, hi), taken `each` to a lane: what lies before this lane's rows.
-__device__ __forceinline__ uint32_t UnitsBefore(const Rows& rows, int32_t lo, int32_t hi, int32_t each, int lane,
-                                                uint32_t* total) {
-  uint32_t own = 0;
-  const int64_t first = lo + static_cast<int64_t>(lane) * each;
-  for (int32_t i = 0; i < each; ++i) {
-    if (first + i < hi) own += rows.UnitsOf(static_cast<int32_t>(first + i));
-  }
-  own *= static_cast<uint32_t>(rows.pairs);
-  const uint32_t sum = ScanAdd(own);
-  *total = __builtin_amdgcn_readlane(sum, 63);
-  return sum - own;
-}
+// Unit c of `units` of `pair` of `row`.
+struct Place {
+  int32_t row, pair;
+  uint32_t c, units;
+};
 
-// Row that holds unit x, and what of x lies in it (*rest), from the units before
-// each lane's `each` rows.
-__device__ __forceinline__ int32_t RowOfUnit(const Rows& rows, uint32_t before, int32_t each, int lane, uint32_t x,
-                                             uint32_t* rest) {
-  int32_t lo = 0, hi = rows.n_rows;
-  while (true) {
-    // before does not fall from lane to lane, and the last one at or below x is not of an empty set of rows
-    const int at = static_cast<int>(__builtin_popcountll(__ballot(before <= x))) - 1;
-    x -= __builtin_amdgcn_readlane(before, at);
-    const int64_t begin = lo + static_cast<int64_t>(at) * each;
-    hi = static_cast<int32_t>(min(begin + each, static_cast<int64_t>(hi)));
-    lo = static_cast<int32_t>(begin);
-    if (each == 1) break;
-    each = (hi - lo + 63) / 64;
-    uint32_t unused;
-    before = UnitsBefore(rows, lo, hi, each, lane, &unused);
+// The batch as a wave sees it: rows are taken `each` to a lane, with the units and the items before them. (A short call's
+// start is bound by fetching its instructions, so what is needed in several places is written in one.)
+struct Batch {
+  const Rows& rows;
+  Cut cut{0};
+  int lane;
+  int32_t each;
+  uint32_t units, items;
+  uint32_t units_before, items_before;
+  int32_t own_len = 0, own_seq = -1;  // where each is 1: of row `lane`
+  uint32_t own_units = 0;
+
+  __device__ __forceinline__ Batch(const Rows& r, int l) : rows(r), lane(l) {
+    each = (rows.n_rows + 63) / 64;
+    if (each == 1 && lane < rows.n_rows) {
+      own_len = rows.lens[lane];
+      own_seq = rows.Seq(lane);
+      own_units = rows.UnitsOf(own_seq, own_len);
+    }
+    units_before = Before(0, rows.n_rows, each, false, &units);
+    cut = Cut(units);
+    items = units;
+    items_before = units_before;
+    if (!cut.units) items_before = Before(0, rows.n_rows, each, true, &items);
   }
-  *rest = x;
-  return lo;
-}
+
+  // Of rows [lo, hi), taken `some` to a lane: the units, or items, before this lane's.
+  __device__ __forceinline__ uint32_t Before(int32_t lo, int32_t hi, int32_t some, bool of_items, uint32_t* total) const {
+    uint32_t own = 0;
+    if (each == 1) {
+      own = of_items ? cut.Items(own_units) : own_units;
+    } else {
+      const int64_t first = lo + static_cast<int64_t>(lane) * some;
+#pragma unroll 2
+      for (int32_t i = 0; i < some; ++i) {
+        if (first + i < hi) {
+          const uint32_t n = rows.UnitsOf(static_cast<int32_t>(first + i));
+          own += of_items ? cut.Items(n) : n;
+        }
+      }
+    }
+    own *= static_cast<uint32_t>(rows.pairs);
+    const uint32_t sum = ScanAdd(own);
+    *total = __builtin_amdgcn_readlane(sum, 63);
+    return sum - own;
+  }
+
+  // Of one row, the same in every lane
+  __device__ __forceinline__ uint32_t UnitsOf(int32_t r) const {
+    return each == 1 ? __builtin_amdgcn_readlane(own_units, r) : rows.ScalarUnitsOf(r);
+  }
+  __device__ __forceinline__ int32_t LenOf(int32_t r) const {
+    return each == 1 ? __builtin_amdgcn_readlane(own_len, r) : ScalarLoad(rows.lens + r);
+  }
+  __device__ __forceinline__ int64_t SeqOf(int32_t r) const {
+    return each == 1 ? __builtin_amdgcn_readlane(own_seq, r) : rows.ScalarSeq(r);
+  }
+
+  // Where item x (unit x, unless by_items) begins: its place, its number among the units, and in *past that of the first
+  // unit behind it.
+  __device__ __forceinline__ uint32_t Locate(uint32_t x, bool by_items, Place* p, uint32_t* past) const {
+    int32_t lo = 0, hi = rows.n_rows, some = each;
+    uint32_t ub = units_before, ib = items_before, before = 0;
+#pragma unroll 1
+    while (true) {
+      // the counts do not fall from lane to lane, and the last lane at or below x does not stand for empty rows
+      const uint32_t b = by_items ? ib : ub;
+      const int at = static_cast<int>(__builtin_popcountll(__ballot(b <= x))) - 1;
+      x -= __builtin_amdgcn_readlane(b, at);
+      before += __builtin_amdgcn_readlane(ub, at);
+      lo += at * some;
+      if (some == 1) break;
+      hi = min(lo + some, hi);
+      some = (hi - lo + 63) / 64;
+      uint32_t unused;
+#pragma unroll 1
+      for (int pass = 0; pass < 2; ++pass) {
+        ub = ib;
+        ib = Before(lo, hi, some, pass == 1, &unused);
+      }
+    }
+    p->row = lo;
+    p->units = UnitsOf(lo);
+    const uint32_t k = by_items ? cut.Items(p->units) : p->units;
+    uint32_t pair = 0;
+    if (x >= k) pair = Scalar(x / k);
+    const uint32_t i = x - pair * k;
+    p->pair = static_cast<int32_t>(pair);
+    const uint32_t first = before + pair * p->units;
+    if (!by_items) {
+      p->c = i;
+      *past = first + i + 1;
+    } else if (k == 1) {
+      p->c = 0;
+      *past = first + p->units;
+    } else {  // k items of q units, and one more in the first r of them
+      const uint32_t q = Scalar(p->units / k), r = p->units - q * k;
+      p->c = i * q + min(i, r);
+      *past = first + p->c + q + (i < r ? 1 : 0);
+    }
+    return first + p->c;
+  }
+
+  // The first item of a pair of n units, whose first unit is `first`.
+  __device__ __forceinline__ uint32_t ItemOfPair(uint32_t first, int32_t row, int32_t pair, uint32_t n) const {
+    if (cut.units) return first;
+    const int32_t at = each == 1 ? row : static_cast<int32_t>(Scalar(static_cast<uint32_t>(row) / static_cast<uint32_t>(each)));
+    uint32_t items_of_rows = 0;
+#pragma unroll 1
+    for (int32_t r = at * each; r < row; ++r) items_of_rows += cut.Items(UnitsOf(r));
+    return __builtin_amdgcn_readlane(items_before, at) + items_of_rows * static_cast<uint32_t>(rows.pairs) +
+           static_cast<uint32_t>(pair) * cut.Items(n);
+  }
+};
 
 // ---------------------------------------------------------------- the kernel
 
@@ -312,8 +434,57 @@ struct Piece {
 
 // In scalar registers: a buffer descriptor made from vector ones would be looped over.
 __device__ __forceinline__ Piece UniformPiece(const Piece& p) {
-  return Piece{Share::Scalar(p.first), Share::Scalar(p.c0), Share::Scalar(p.c1), Share::Scalar(p.n),
+  return Piece{Scalar(p.first), Scalar(p.c0), Scalar(p.c1), Scalar(p.n),
                __builtin_amdgcn_readfirstlane(p.row),   __builtin_amdgcn_readfirstlane(p.pair)};
+}
+
+// The query heads of a piece.
+struct HeadsOf {
+  int32_t heads;
+  int64_t head_row;  // row of the first in q and out
+
+  __device__ __forceinline__ HeadsOf(const Piece& p, int32_t n_heads, int32_t group, int32_t tiles, int32_t tile_heads) {
+    const int32_t kh = p.pair / tiles;
+    const int32_t h0 = (p.pair - kh * tiles) * tile_heads;
+    heads = min(tile_heads, group - h0);
+    head_row = static_cast<int64_t>(p.row) * n_heads + kh * group + h0;
+  }
+};
+
+// A pair of up to kJoinAtOnce parts is joined in one step; of more in two, each kFan parts in the first. (One step of 256
+// parts took 34 us of a call where two take 22; at 64 parts they are alike.)
+constexpr uint32_t kJoinAtOnce = 32;
+constexpr uint32_t kFan = 16;
+
+// The workgroups wa, wa + 1, ... that hold parts of a piece's pair, and workgroup me's place among them.
+struct Parts {
+  uint32_t wa = 0, parts = 0, blocks = 0, block = 0, block_parts = 0;
+  bool leads = false;  // the pair's first part is the first thing that workgroup wa holds
+
+  __device__ __forceinline__ Parts() {}
+  __device__ __forceinline__ Parts(const Piece& p, const Batch& batch, const Share& share, uint32_t me) {
+    const uint32_t item = batch.ItemOfPair(p.first, p.row, p.pair, p.n);
+    wa = share.Holder(item);
+    leads = share.Begin(wa) == item;
+    parts = share.Holder(item + batch.cut.Items(p.n) - 1) - wa + 1;
+    blocks = parts <= kJoinAtOnce ? 1 : (parts + kFan - 1) / kFan;
+    block = blocks == 1 ? 0 : (me - wa) / kFan;
+    block_parts = blocks == 1 ? parts : min(kFan, parts - block * kFan);
+  }
+  // Counters, in words of the workspace. A workgroup is the first holder of one split pair at most, and a later block's
+  // first holder of one at most.
+  __device__ __forceinline__ uint32_t PairCounter() const { return wa * (kCounterBytes / 4); }
+  __device__ __forceinline__ uint32_t BlockCounter() const {
+    return (wa + block * kFan) * (kCounterBytes / 4) + (block == 0 ? 1 : 2);
+  }
+};
+
+// Counts in at a counter; whether that was the last of `all`, which leaves the counter ready for the next call.
+__device__ __forceinline__ int Count(char* workspace, uint32_t counter, uint32_t all) {
+  uint32_t* at = reinterpret_cast<uint32_t*>(workspace) + counter;
+  const bool last = __hip_atomic_fetch_add(at, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == all - 1;
+  if (last) __hip_atomic_store(at, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return last ? 1 : 0;
 }
 
 // kTiles: 8-bit caches, column tiles of up to 4 heads (1 or 2); else 1, of up to 8.
@@ -348,7 +519,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
   __shared__ Join joins[64 * kWaves];
   __shared__ Piece pieces[kWaves][2];
   __shared__ int held[kWaves];
-  __shared__ int last_flag;
+  __shared__ int flags[2];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
@@ -359,21 +530,46 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
   const int32_t group = n_heads / view.n_kv;
 
   // the batch's units, and this wave's share
-  Share share;
-  const int32_t each = (rows.n_rows + 63) / 64;
-  const uint32_t before = UnitsBefore(rows, 0, rows.n_rows, each, lane, &share.total);
-  share.groups = min(gridDim.x, (share.total + TUNE_MIN - 1) / TUNE_MIN);
+  const Batch batch(rows, lane);
+  const uint32_t groups = min(gridDim.x, batch.cut.units ? (batch.units + 3) / 4 : batch.items);
+  const Share share(batch.items, max(groups, 1u));
   const uint32_t me = blockIdx.x;
-  uint32_t begin = 0, end = 0;
-  if (me < share.groups) {
-    share.per = Share::Scalar(share.total / share.groups);
-    share.rem = share.total - share.per * share.groups;
-    begin = share.Begin(me);
-    end = share.Begin(me + 1);
+  Place first;  // where the workgroup's share begins, and then the wave's
+  uint32_t begin = 0, end = 0, u = 0, u_end = 0;
+  if (me < groups) {
+    const uint32_t next = share.Begin(me + 1);
+    uint32_t x = share.Begin(me), past = 0;
+    bool by_items = !batch.cut.units;
+    int query = 0;
+#pragma unroll 1
+    while (true) {
+      Place p;
+      const uint32_t found = batch.Locate(x, by_items, &p, &past);
+      if (query != 1) first = p;
+      if (query == 2) break;
+      if (query == 0) {
+        begin = found;
+        end = next == batch.items ? batch.units : by_items ? past : next;
+        if (by_items && next != batch.items && next != x + 1) {
+          x = next;
+          query = 1;
+          continue;
+        }
+      } else {
+        end = found;
+      }
+      u = begin + (((end - begin) * wave) >> 2);
+      u_end = begin + (((end - begin) * (wave + 1)) >> 2);
+      static_assert(kWaves == 4, "a wave's share of its workgroup's");
+      if (u == u_end || first.c + (u - begin) < first.units) {
+        first.c += u - begin;
+        break;
+      }
+      x = u;
+      by_items = false;
+      query = 2;
+    }
   }
-  uint32_t u = begin + (((end - begin) * wave) >> 2);
-  const uint32_t u_end = begin + (((end - begin) * (wave + 1)) >> 2);
-  static_assert(kWaves == 4, "a wave's share of its workgroup's");
 
   int my_held = 0;  // bit 0: the first piece, bit 1: the last
   if (u < u_end) {
@@ -409,13 +605,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
     }
 
     // where the wave is: unit c of `units` of `pair` of `row`
-    uint32_t rest;
-    int32_t row = RowOfUnit(rows, before, each, lane, u, &rest);
-    uint32_t units = rows.ScalarUnitsOf(row);
-    int32_t pair = static_cast<int32_t>(Share::Scalar(rest / units));
-    uint32_t c = rest - static_cast<uint32_t>(pair) * units;
-    int32_t len = ScalarLoad(rows.lens + row);
-    const int32_t* table = view.pages + rows.ScalarSeq(row) * view.max_pages;
+    int32_t row = first.row, pair = first.pair;
+    uint32_t c = first.c, units = first.units;
+    int32_t len = batch.LenOf(row);
+    const int32_t* table = view.pages + batch.SeqOf(row) * view.max_pages;
 
     // Rows of the pool that the 16-key tiles of unit c start at; a tile past the end repeats the unit's first, a page
     // out of range is read as page 0 and its tile marked.
@@ -554,19 +747,16 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
         }
       }
     };
-    // takes the int32 sums to acc, which is scaled by `back`
-    const auto take_sums = [&](const float (&back)[kTiles]) {
+    // takes the int32 sums to acc, which is then scaled by `back`
+    const auto take_sums = [&](int t, float back) {
       if constexpr (kQ8) {
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
+        for (int i = 0; i < kE; ++i) {
 #pragma unroll
-          for (int i = 0; i < kE; ++i) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              acc[t][i][r] = fmaf(static_cast<float>(sum[t][i][r]), digit_by, acc[t][i][r]) * back[t];
-            }
-            sum[t][i] = I32x4{0, 0, 0, 0};
+          for (int r = 0; r < 4; ++r) {
+            acc[t][i][r] = fmaf(static_cast<float>(sum[t][i][r]), digit_by, acc[t][i][r]) * back;
           }
+          sum[t][i] = I32x4{0, 0, 0, 0};
         }
       }
     };
@@ -576,22 +766,26 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
       return *reinterpret_cast<const float4*>(stage + kStep * kRow + 64 * j + 16 * g);
     };
 
-    begin_piece();
     uint32_t c_first = c;
+    bool turned = true;  // the unit at hand is its piece's first
     F32x4 kept[kTiles][kOwn];
     float kept_m[kTiles], kept_l[kTiles];
     int32_t since = 0;  // steps since the int32 sums were last taken
 
     while (true) {
+      if (turned) {
+        begin_piece();
+        turned = false;
+      }
       const int32_t pos = static_cast<int32_t>(c) * kStep;
       const bool tail = pos + kStep > len;
       const int32_t left = len - pos;  // positions from here
       const int this_bad = bad;
       // ---- scores, once the keys are there: the values' loads are younger
       WaitLoads<kStageLoads>();
-      float s[kTiles][kSub][4];
+      float s[kSub][4];  // of one column tile
+      I32x4 raw[kQ8 ? kTiles : 1][kSub];
       if constexpr (kQ8) {
-        I32x4 raw[kTiles][kSub];
 #pragma unroll
         for (int j = 0; j < kSub; ++j) {
 #pragma unroll
@@ -605,29 +799,17 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
             }
           }
         }
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
-#pragma unroll
-          for (int j = 0; j < kSub; ++j) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              float x = static_cast<float>(raw[t][j][i]) * to_score[t];
-              x += Ror<8>(x);
-              s[t][j][i] = x + Ror<4>(x);
-            }
-          }
-        }
       } else {
 #pragma unroll
         for (int j = 0; j < kSub; ++j) {
-          F32x4 raw = F32x4{0.0f, 0.0f, 0.0f, 0.0f};
+          F32x4 sums = F32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
           for (int i = 0; i < kSteps; ++i) {
             const Half8 a = *reinterpret_cast<const Half8*>(k_mine + j * 16 * kRow + (k_at ^ (64u * i)));
-            raw = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[i], raw, 0, 0, 0);
+            sums = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[i], sums, 0, 0, 0);
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[0][j][i] = (raw[i] + Ror<8>(raw[i])) * to_score[0];
+          for (int i = 0; i < 4; ++i) s[j][i] = (sums[i] + Ror<8>(sums[i])) * to_score[0];
         }
       }
       // ---- the next unit, and its keys
@@ -652,11 +834,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
             pair = 0;
             do {
               ++row;
-              units = row < rows.n_rows ? rows.ScalarUnitsOf(row) : 1;
+              units = row < rows.n_rows ? batch.UnitsOf(row) : 1;
             } while (units == 0);
             row = min(row, rows.n_rows - 1);  // past the last only if the lengths change while this runs
-            len = ScalarLoad(rows.lens + row);
-            table = view.pages + rows.ScalarSeq(row) * view.max_pages;
+            len = batch.LenOf(row);
+            table = view.pages + batch.SeqOf(row) * view.max_pages;
           }
         }
         find();
@@ -664,37 +846,39 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
       }
       __builtin_amdgcn_sched_barrier(0);
       // ---- weights
-      float top[kTiles];
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t) {
-        top[t] = m[t];
+      // a column tile's scores, and their maximum with m
+      const auto take_scores = [&](int t) {
+        float top = m[t];
 #pragma unroll
         for (int j = 0; j < kSub; ++j) {
           const float by[4] = {kQ8 ? ks[kQ8 ? j : 0].x : 1.0f, kQ8 ? ks[kQ8 ? j : 0].y : 1.0f,
                                kQ8 ? ks[kQ8 ? j : 0].z : 1.0f, kQ8 ? ks[kQ8 ? j : 0].w : 1.0f};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            if constexpr (kQ8) s[t][j][i] *= by[i];
-            if (this_bad & (1 << j)) s[t][j][i] = NAN;
-            if (tail && 16 * j + 4 * g + i >= left) s[t][j][i] = -INFINITY;
-            top[t] = fmaxf(top[t], s[t][j][i]);
+            if constexpr (kQ8) {
+              float x = static_cast<float>(raw[t][j][i]) * to_score[t];
+              x += Ror<8>(x);
+              s[j][i] = (x + Ror<4>(x)) * by[i];
+            }
+            if (this_bad & (1 << j)) s[j][i] = NAN;
+            if (tail && 16 * j + 4 * g + i >= left) s[j][i] = -INFINITY;
+            top = fmaxf(top, s[j][i]);
           }
         }
-        top[t] = MaxAcrossRows(top[t]);
-      }
+        return MaxAcrossRows(top);
+      };
+      float first_top = 0.0f;
+      if constexpr (kTiles == 1) first_top = take_scores(0);
       // the values are there: the next keys' loads, if any, are younger
       if (more) {
         WaitLoads<kStageLoads>();
       } else {
         WaitLoads<0>();
       }
+      // ---- the output's sums
       if constexpr (kQ8) {
 #pragma unroll
         for (int j = 0; j < kSub; ++j) vs[j] = scales_at(v_mine, j);
-      }
-      float safe[kTiles];
-      float up = 0x1p14f;
-      if constexpr (kQ8) {
         if (tail) {
 #pragma unroll
           for (int j = 0; j < kSub; ++j) {
@@ -705,7 +889,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
             vs[j].w = p + 3 < left ? vs[j].w : 0.0f;
           }
         }
-        // as whole numbers, where a NaN is larger than any number
+        // the largest, as whole numbers, where a NaN is larger than any number
         uint32_t big = 0;
 #pragma unroll
         for (int j = 0; j < kSub; ++j) {
@@ -715,11 +899,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
         big = __float_as_uint(AcrossRows(__uint_as_float(big), [](float a, float b) {
           return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b)));
         }));
-        bool flush = big >= __float_as_uint(ref) || ++since >= 1024;  // 1024 steps: int32 holds 2^17 products of 2^14
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t) flush |= top[t] > m[t] + 3.0f;
-        if (__any(flush)) {
-          float back[kTiles], by = 1.0f;
+        big = __builtin_amdgcn_readfirstlane(big);
+        if (big >= __float_as_uint(ref) || ++since >= 1024) {  // 1024 steps: int32 holds 2^17 products of 2^14
+          float by = 1.0f;
           if (big >= __float_as_uint(ref)) {
             const int e = min(max(static_cast<int>(big >> 23) + 1, 27), 254);
             by = ref * __int_as_float((254 - e) << 23);
@@ -727,57 +909,39 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
           }
 #pragma unroll
           for (int t = 0; t < kTiles; ++t) {
-            const float to = top[t] > m[t] + 3.0f ? top[t] : m[t];
-            const float by_max = __builtin_amdgcn_exp2f(m[t] - (to == -INFINITY ? 0.0f : to));
-            m[t] = to;
-            l[t] *= by_max;
-            back[t] = by * by_max;
+            take_sums(t, by);
+            if (big >= 0x7F800000u) l[t] = NAN;
           }
-          take_sums(back);
           since = 0;
         }
-        if (big >= 0x7F800000u) {
-#pragma unroll
-          for (int t = 0; t < kTiles; ++t) l[t] = NAN;
-        }
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t) safe[t] = m[t] == -INFINITY ? 0.0f : m[t];
-        up = 0x1p27f * __int_as_float((254 << 23) - __float_as_int(ref));  // 2^27 / ref
-      } else {
-        if (tail) {  // what stands behind the last position may not even be a number
-#pragma unroll
-          for (int i = 0; i < kStep * kRow / 1024; ++i) {
-            const int to = 1024 * i + 16 * lane;
-            if (to / kRow >= left) *reinterpret_cast<uint4*>(v_mine + to) = make_uint4(0u, 0u, 0u, 0u);
-          }
-        }
-        safe[0] = top[0] == -INFINITY ? 0.0f : top[0];
-        const float back = __builtin_amdgcn_exp2f(m[0] - safe[0]);
-        m[0] = top[0];
-        l[0] *= back;
-        if (__any(back != 1.0f)) {
-#pragma unroll
-          for (int i = 0; i < kE; ++i) acc[0][i] *= back;
-        }
-      }
-      // ---- the output's sums
-      if constexpr (kQ8) {
+        const float up = 0x1p27f * __int_as_float((254 << 23) - __float_as_int(ref));  // 2^27 / ref
         I32x4 w[kTiles];  // tile j of 16 keys: bytes 4 j ..
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) {
+          if constexpr (kTiles > 1) __builtin_amdgcn_sched_barrier(0);  // one after the other: registers
+          const float top = kTiles == 1 ? first_top : take_scores(t);
+          if (__any(top > m[t] + 3.0f)) {
+            const float to = top > m[t] + 3.0f ? top : m[t];
+            const float back = __builtin_amdgcn_exp2f(m[t] - (to == -INFINITY ? 0.0f : to));
+            m[t] = to;
+            l[t] *= back;
+            take_sums(t, back);
+          }
+          const float safe = m[t] == -INFINITY ? 0.0f : m[t];
 #pragma unroll
           for (int j = 0; j < kSub; ++j) {
             const float by[4] = {vs[j].x, vs[j].y, vs[j].z, vs[j].w};
             uint32_t d[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const float p = __builtin_amdgcn_exp2f(s[t][j][i] - safe[t]);
+              const float p = __builtin_amdgcn_exp2f(s[j][i] - safe);
               l[t] += p;
               d[i] = static_cast<uint32_t>(static_cast<int>(fmaf(p * by[i], up, 0.5f))) + 0x80808080u;
             }
             w[t][j] = Digit4(d[0], d[1], d[2], d[3], digit);
           }
         }
+        if constexpr (kTiles > 1) __builtin_amdgcn_sched_barrier(0);
         I32x2 a[kE][2];
 #pragma unroll
         for (int i = 0; i < kE; ++i) {
@@ -794,13 +958,29 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
           }
         }
       } else {
+        if (tail) {  // what stands behind the last position may not even be a number
+#pragma unroll
+          for (int i = 0; i < kStep * kRow / 1024; ++i) {
+            const int to = 1024 * i + 16 * lane;
+            if (to / kRow >= left) *reinterpret_cast<uint4*>(v_mine + to) = make_uint4(0u, 0u, 0u, 0u);
+          }
+        }
+        const float safe = first_top == -INFINITY ? 0.0f : first_top;
+        const float back = __builtin_amdgcn_exp2f(m[0] - safe);
+        m[0] = first_top;
+        l[0] *= back;
+        if (__any(back != 1.0f)) {
+#pragma unroll
+          for (int i = 0; i < kE; ++i) acc[0][i] *= back;
+        }
+        constexpr float up = 0x1p14f;
         uint32_t pt[kSub][2];
 #pragma unroll
         for (int j = 0; j < kSub; ++j) {
           float w[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            w[i] = __builtin_amdgcn_exp2f(s[0][j][i] - safe[0]);
+            w[i] = __builtin_amdgcn_exp2f(s[j][i] - safe);
             l[0] += w[i];
           }
           pt[j][0] = Term2(w[0] * up, w[1] * up, copy != 0);
@@ -829,10 +1009,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
 
       // ---- the piece's (m, l, o): out, or kept where it is not the whole of its pair
       if constexpr (kQ8) {
-        float same[kTiles];
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) same[t] = 1.0f;
-        take_sums(same);
+        for (int t = 0; t < kTiles; ++t) take_sums(t, 1.0f);
       }
       const bool whole = c_first == 0 && c_end == piece_units;
       const float unit = kQ8 ? ref * 0x1p-27f : 0x1p-14f;
@@ -875,7 +1053,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
       }
       if (!more) break;
       c_first = c;
-      begin_piece();
+      turned = true;
     }
     // the first piece, now that its keys' place is free
     if (my_held & 1) {
@@ -897,10 +1075,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
   if (lane == 0) held[wave] = my_held;
   __syncthreads();
 
-  // The workgroup's pieces in order, neighbours of one pair joined.
+  // The workgroup's pieces in order, neighbours of one pair joined: to out where that is the whole of a pair, else (the
+  // workgroup's first and last at most) to its slots in the workspace, of the outputs and then a line of (m, l).
   const auto part = [&](int i) { return reinterpret_cast<const float*>(i & 1 ? v_lds[i >> 1] : k_lds[i >> 1]); };
-  float* const slots = reinterpret_cast<float*>(workspace + kMaxGroups * kCounterBytes);
-  const int64_t slot_floats = static_cast<int64_t>(tile_heads) * kPart;
+  const uint32_t slot_bytes = SlotBytes(D, tile_heads);
+  char* const slots = workspace + kMaxGroups * kCounterBytes;
+  Piece open[2];
+  int n_open = 0;
   int from = 0;  // wave * 2 + which
   while (from < 2 * kWaves) {
     if (!(held[from >> 1] >> (from & 1) & 1)) {
@@ -918,70 +1099,92 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
       list |= 1 << to;
     }
     from = to;
-    const int32_t kh = run.pair / tiles;
-    const int32_t h0 = (run.pair - kh * tiles) * tile_heads;
-    const int32_t heads = min(tile_heads, group - h0);
-    const int64_t head_row = static_cast<int64_t>(run.row) * n_heads + kh * group + h0;
+    const HeadsOf of(run, n_heads, group, tiles, tile_heads);
     const bool whole = run.c0 == 0 && run.c1 == run.n;
     const bool leads = run.first + run.c0 == begin;  // the workgroup's first piece
-    float* slot = slots + (2 * static_cast<int64_t>(me) + (leads ? 0 : 1)) * slot_floats;
-    const __amdgpu_buffer_rsrc_t rs = dev::OutResource(slot, static_cast<uint32_t>(slot_floats * 4));
-    for (int i = threadIdx.x; i < heads * (D / 4); i += 64 * kWaves) {
+    const __amdgpu_buffer_rsrc_t rs =
+        dev::OutResource(slots + (2 * static_cast<int64_t>(me) + (leads ? 0 : 1)) * slot_bytes, slot_bytes);
+    for (int i = threadIdx.x; i < of.heads * (D / 4); i += 64 * kWaves) {
       const int h = i / (D / 4), d = 4 * (i % (D / 4));
-      float top = -INFINITY;
+      float4 x[2 * kWaves];
+#pragma unroll
+      for (int k = 0; k < 2 * kWaves; ++k) x[k] = *reinterpret_cast<const float4*>(part(k) + h * kPart + d);
+      // what the pieces in the list count for under their common maximum; none of a piece that is not in the list, whose
+      // place holds anything
+      float2 ml[2 * kWaves];
+#pragma unroll
+      for (int k = 0; k < 2 * kWaves; ++k) ml[k] = *reinterpret_cast<const float2*>(part(k) + h * kPart + D);
+      float top = -INFINITY, l = 0.0f;
+#pragma unroll
       for (int k = 0; k < 2 * kWaves; ++k) {
-        if (list >> k & 1) top = fmaxf(top, part(k)[h * kPart + D]);
+        ml[k].x = list >> k & 1 ? ml[k].x : -INFINITY;
+        top = fmaxf(top, ml[k].x);
       }
       const float safe = top == -INFINITY ? 0.0f : top;
-      float l = 0.0f;
       float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
       for (int k = 0; k < 2 * kWaves; ++k) {
-        if (!(list >> k & 1)) continue;
-        const float* p = part(k) + h * kPart;
-        const float f = __builtin_amdgcn_exp2f(p[D] - safe);
-        const float4 x = *reinterpret_cast<const float4*>(p + d);
-        l = fmaf(p[D + 1], f, l);
-        o = make_float4(fmaf(x.x, f, o.x), fmaf(x.y, f, o.y), fmaf(x.z, f, o.z), fmaf(x.w, f, o.w));
+        if (list >> k & 1) {  // the same in every lane
+          const float f = __builtin_amdgcn_exp2f(ml[k].x - safe);
+          l = fmaf(ml[k].y, f, l);
+          o = make_float4(fmaf(x[k].x, f, o.x), fmaf(x[k].y, f, o.y), fmaf(x[k].z, f, o.z), fmaf(x[k].w, f, o.w));
+        }
       }
       if (whole) {
         const float inv = 1.0f / l;
-        dev::Store4(out + (head_row + h) * D + d, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+        dev::Store4(out + (of.head_row + h) * D + d, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
       } else {
-        dev::StoreBuf4<dev::kStoreDeviceThroughPolicy>(rs, 4u * static_cast<uint32_t>(h * kPart + d), o);
+        dev::StoreBuf4<kPartPolicy>(rs, 16u * static_cast<uint32_t>(i), o);
         if (d == 0) {
-          dev::StoreBufU2<dev::kStoreDeviceThroughPolicy>(rs, 4u * static_cast<uint32_t>(h * kPart + D),
-                                                          make_uint2(__float_as_uint(top), __float_as_uint(l)));
+          dev::StoreBufU2<kPartPolicy>(rs, slot_bytes - kLine + 8u * h,
+                                       make_uint2(__float_as_uint(top), __float_as_uint(l)));
         }
       }
     }
     if (whole) continue;
-    // Device-scope write-through stores, acknowledged before the count: what the last workgroup of the pair to arrive
-    // then reads, with device-coherent loads, is all there. No workgroup waits for another.
+    open[n_open == 0 ? 0 : 1] = run;
+    ++n_open;
+  }
+
+  // Device-scope write-through stores, acknowledged before the count: what the last workgroup of a pair to arrive then
+  // reads, with device-coherent loads, is all there. No workgroup waits for another. Where a pair has more parts than
+  // kJoinAtOnce, the last of each kFan joins those and counts for them.
+  if (n_open > 0) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    const uint32_t wa = share.Holder(run.first), wb = share.Holder(run.first + run.n - 1);
-    uint32_t* counter = reinterpret_cast<uint32_t*>(workspace + wa * kCounterBytes);
-    if (threadIdx.x == 0) {
-      last_flag = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == wb - wa;
+    // which parts of their pairs they are: kept where the loop after the count finds them
+    Parts of_first, of_last;
+#pragma unroll 1
+    for (int i = 0; i < n_open; ++i) {
+      const Parts of(open[i == 0 ? 0 : 1], batch, share, me);
+      if (i == 0) of_first = of;
+      of_last = of;
+    }
+    if (threadIdx.x < n_open) {  // both at once
+      const Parts& of = threadIdx.x == 0 ? of_first : of_last;
+      flags[threadIdx.x] = Count(workspace, of.blocks > 1 ? of.BlockCounter() : of.PairCounter(), of.block_parts);
     }
     __syncthreads();
-    if (last_flag) {
-      // The parts in order. wa's is in its first slot only if the pair starts where its share does. Four elements of a
-      // head to a thread, and as many sets of threads as there are, each taking every sets-th part, kBatch of them
-      // requested at a time: a round trip past the L2 costs more than the arithmetic.
+#pragma unroll 1
+    for (int i = 0; i < n_open; ++i) {
+      if (!__builtin_amdgcn_readfirstlane(flags[i])) continue;
+      const Piece run = open[i == 0 ? 0 : 1];
+      const Parts of = i == 0 ? of_first : of_last;
+      const HeadsOf heads(run, n_heads, group, tiles, tile_heads);
+      const uint32_t first_leads = of.leads ? 0u : 1u;
+      const __amdgpu_buffer_rsrc_t all = dev::OutResource(slots + 2 * static_cast<int64_t>(of.wa) * slot_bytes,
+                                                          (2 * of.parts) * slot_bytes);
+      // wa's part is in its first slot only if the pair starts where its share does
+      const auto slot_of = [&](uint32_t p) { return (2u * p + (p == 0 ? first_leads : 0u)) * slot_bytes; };
+      // Four elements of a head to a thread, and as many sets of threads as there are, each taking every sets-th part,
+      // kBatch of them requested at a time: a round trip past the L2 costs more than the arithmetic.
       constexpr int kBatch = 8;
-      const uint32_t first_leads = share.Begin(wa) == run.first ? 0u : 1u;
-      const __amdgpu_buffer_rsrc_t all = dev::OutResource(
-          slots + 2 * static_cast<int64_t>(wa) * slot_floats, static_cast<uint32_t>((2 * (wb - wa) + 2) * slot_floats * 4));
-      const int parts = static_cast<int>(wb - wa) + 1;
-      const int columns = heads * (D / 4);
+      const int columns = heads.heads * (D / 4);
       const int sets = 64 * kWaves / columns;
       const int set = static_cast<int>(threadIdx.x) / columns, column = static_cast<int>(threadIdx.x) % columns;
-      const int h = column / (D / 4), d = 4 * (column % (D / 4));
-      const uint32_t ml_at = 4u * static_cast<uint32_t>(h * kPart + D), o_at = 4u * static_cast<uint32_t>(h * kPart + d);
-      const uint32_t slot_bytes = static_cast<uint32_t>(slot_floats * 4);
-      float top = -INFINITY, l = 0.0f;
-      float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      const int h = column / (D / 4);
+      float top, l;
+      float4 o;
       const auto join = [&](float m2, float l2, float4 o2) {
         const float to = fmaxf(top, m2);
         const float safe = to == -INFINITY ? 0.0f : to;
@@ -991,37 +1194,69 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
         o = make_float4(fmaf(o2.x, f2, o.x * f), fmaf(o2.y, f2, o.y * f), fmaf(o2.z, f2, o.z * f),
                         fmaf(o2.w, f2, o.w * f));
       };
-      if (set < sets) {
-        for (int w = set; w < parts; w += kBatch * sets) {
-          uint2 ml[kBatch];
-          float4 x[kBatch];
+      // parts p0, p0 + step, ...: the sum is in set 0
+      uint32_t p0 = of.block * kFan, step = 1;
+      int count = static_cast<int>(of.block_parts);
+      bool done = of.blocks == 1;
+#pragma unroll 1
+      while (true) {
+        top = -INFINITY, l = 0.0f;
+        o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (set < sets) {
+#pragma unroll 1
+          for (int w = set; w < count; w += kBatch * sets) {
+            uint2 ml[kBatch];
+            float4 x[kBatch];
 #pragma unroll
-          for (int i = 0; i < kBatch; ++i) {
-            const int p = min(w + i * sets, parts - 1);
-            const uint32_t at = (2u * static_cast<uint32_t>(p) + (p == 0 ? first_leads : 0u)) * slot_bytes;
-            ml[i] = dev::LoadBufU2<dev::kLoadDevicePolicy>(all, at + ml_at);
-            x[i] = dev::LoadBuf4<dev::kLoadDevicePolicy>(all, at + o_at);
+            for (int k = 0; k < kBatch; ++k) {
+              if (w + k * sets < count) {
+                const uint32_t at = slot_of(p0 + static_cast<uint32_t>(w + k * sets) * step);
+                ml[k] = dev::LoadBufU2<dev::kLoadDevicePolicy>(all, at + slot_bytes - kLine + 8u * h);
+                x[k] = dev::LoadBuf4<dev::kLoadDevicePolicy>(all, at + 16u * column);
+              }
+            }
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+              if (w + k * sets < count) join(__uint_as_float(ml[k].x), __uint_as_float(ml[k].y), x[k]);
+            }
           }
-#pragma unroll
-          for (int i = 0; i < kBatch; ++i) {
-            if (w + i * sets < parts) join(__uint_as_float(ml[i].x), __uint_as_float(ml[i].y), x[i]);
+          joins[threadIdx.x] = Join{o, top, l};
+        }
+        __syncthreads();
+        if (set == 0) {
+#pragma unroll 1
+          for (int k = 1; k < min(sets, count); ++k) {
+            const Join& j = joins[k * columns + column];
+            join(j.m, j.l, j.o);
           }
         }
-        joins[threadIdx.x] = Join{o, top, l};
+        __syncthreads();  // joins may be written again
+        if (done) break;
+        // a block's sum takes its first part's place, and counts
+        if (set == 0) {
+          const uint32_t at = slot_of(p0);
+          dev::StoreBuf4<kPartPolicy>(all, at + 16u * column, o);
+          if (column % (D / 4) == 0) {
+            dev::StoreBufU2<kPartPolicy>(all, at + slot_bytes - kLine + 8u * h,
+                                         make_uint2(__float_as_uint(top), __float_as_uint(l)));
+          }
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (threadIdx.x == 0) flags[i] = Count(workspace, of.PairCounter(), of.blocks);
+        __syncthreads();
+        if (!__builtin_amdgcn_readfirstlane(flags[i])) break;
+        p0 = 0;
+        step = kFan;
+        count = static_cast<int>(of.blocks);
+        done = true;
       }
-      __syncthreads();
+      if (!done) continue;
       if (set == 0) {
-        for (int i = 1; i < min(sets, parts); ++i) {
-          const Join& j = joins[i * columns + column];
-          join(j.m, j.l, j.o);
-        }
         const float inv = 1.0f / l;
-        dev::Store4(out + (head_row + h) * D + d, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+        dev::Store4(out + heads.head_row * D + 4 * column, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
       }
-      // every workgroup of the pair has counted in: ready for the next call
-      if (threadIdx.x == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
-    __syncthreads();  // last_flag is read before the next run writes it
   }
 
   // rows with nothing to attend to: zeros, or NaN where the row is out of range
@@ -1058,8 +1293,7 @@ size_t GpuAttentionPagedWorkspaceBytes(int32_t n_heads, int32_t n_kv_heads, int3
   CheckHeads("AttentionPagedWorkspace", n_heads, n_kv_heads, head_dim);
   int32_t tiles, tile_heads;
   TilesOf(n_heads / n_kv_heads, &tiles, &tile_heads);
-  return kMaxGroups * (kCounterBytes + 2 * sizeof(float) * static_cast<size_t>(tile_heads) *
-                                           static_cast<size_t>(PartFloats(head_dim)));
+  return kMaxGroups * (kCounterBytes + 2 * static_cast<size_t>(SlotBytes(head_dim, tile_heads)));
 }
 
 void GpuAttentionPagedWorkspaceInit(void* workspace, size_t bytes) {
@@ -1088,14 +1322,18 @@ void GpuAttentionPaged(const GpuPagedKv& kv, const GpuPageTable& table, const in
             "AttentionPaged: a workspace of %zu bytes, 256-byte aligned, is needed (%zu given)", need, workspace_bytes);
   int32_t tiles, tile_heads;
   TilesOf(n_heads / kv.n_kv_heads, &tiles, &tile_heads);
-  const Rows rows{seq_ids, lens, table.n_seqs, table.max_pages * kv.page_size, static_cast<int32_t>(n_rows),
-                  kv.n_kv_heads * tiles, kv.head_dim == 128 && kv.type == kKvF16 ? 5 : 6};
-  const int64_t most = (std::min<int64_t>(rows.capacity, 0x7FFFFFFF) >> rows.unit_shift) + 1;
+  const Rows rows{seq_ids, lens, static_cast<int32_t>(table.n_seqs),
+                  static_cast<int32_t>(std::min<int64_t>(table.max_pages * kv.page_size, 0x7FFFFFFF)),
+                  static_cast<int32_t>(n_rows), kv.n_kv_heads * tiles, kv.head_dim == 128 && kv.type == kKvF16 ? 5 : 6};
+  const int64_t most = (static_cast<int64_t>(rows.capacity) >> rows.unit_shift) + 1;
   RPG_CHECK(n_rows <= 0x7FFFFFFF / most / rows.pairs,
             "AttentionPaged: %lld rows of up to %lld positions and %d heads are too many for one call",
             static_cast<long long>(n_rows), static_cast<long long>(rows.capacity), rows.pairs);
-  // no more workgroups than the longest possible rows would give work to
-  const int64_t groups = std::min<int64_t>(kMaxGroups, (n_rows * most * rows.pairs + TUNE_MIN - 1) / TUNE_MIN);
+  // no more workgroups than the longest possible rows would give work to; for a few rows one to a compute unit, since more
+  // parts of a row cost more to join than the card gives for them (1 x 32768 positions, 8 kv heads: 22.7 against 25.0 us)
+  const int64_t all_pairs = n_rows * rows.pairs;
+  const int64_t at_once = all_pairs * kJoinAtOnce < kMaxGroups ? kMaxGroups / 2 : kMaxGroups;
+  const int64_t groups = std::min<int64_t>(at_once, (all_pairs * most + kWaves - 1) / kWaves);
   const float scale_log2 =
       static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(kv.head_dim)));
   auto* kern = kv.head_dim == 128 ? PagedAttentionKernel<128, false, 1> : PagedAttentionKernel<64, false, 1>;
