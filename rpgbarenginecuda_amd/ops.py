@@ -926,6 +926,10 @@ class GpuPagedKv:
         if self.device is not None and any(t is not None and t.device != self.device for t in self.tensors):
             raise RpgError("GpuPagedKv: pages and scales are on different devices")
         self.ref = ctypes.byref(self.c)
+        self.row_elems = self.n_kv_heads * self.head_dim
+        self.tensor_type = torch.Tensor
+        self.device_index = None if self.device is None else self.device.index
+        self.current_device = torch.cuda.current_device
 
 
 class GpuPageTable:
@@ -943,29 +947,41 @@ class GpuPageTable:
         self.pages = pages
         self.c = PageTableC(_addr(pages, 0, _t().int32, "pages"), self.n_seqs, self.max_pages)
         self.ref = ctypes.byref(self.c)
+        self.device_index = None if isinstance(pages, int) else pages.get_device()
 
 
-def _paged_device(kv: GpuPagedKv, *bufs) -> None:
-    """Refuses tensors that are not where the pages are, and pages that are not on the current device."""
-    if kv.device is None:
-        return
-    for b in bufs:
-        if b is not None and not isinstance(b, int) and b.device != kv.device:
-            raise RpgError(f"a tensor on {b.device} beside a paged cache on {kv.device}")
-    if _t().cuda.current_device() != kv.device.index:
-        raise RpgError(f"the paged cache is on {kv.device}, which is not the current device")
+def _paged_addr(kv: GpuPagedKv, buf, nbytes: int, dtype, name: str):
+    """_addr for a buffer that has to be where the pages are. The calls over pages are short enough for the checks of
+    their many tensors to count, so one that is in order passes through as few of them as there are."""
+    if (type(buf) is kv.tensor_type and buf.dtype is dtype and buf.get_device() == kv.device_index
+            and buf.nbytes >= nbytes and buf.is_contiguous()):
+        return buf.data_ptr()
+    at = _addr(buf, nbytes, dtype, name)
+    if kv.device is not None and isinstance(buf, _t().Tensor) and buf.device != kv.device:
+        raise RpgError(f"{name}: a tensor on {buf.device} beside a paged cache on {kv.device}")
+    return at
+
+
+def _paged_call(kv: GpuPagedKv, table: GpuPageTable) -> PagedOpsC:
+    """The functions, for pages on the current device."""
+    if kv.device is not None:
+        if table.device_index not in (kv.device_index, None):
+            raise RpgError(f"a page table on device {table.device_index} beside a paged cache on {kv.device}")
+        if kv.current_device() != kv.device_index:
+            raise RpgError(f"the paged cache is on {kv.device}, which is not the current device")
+    return _paged or paged_ops()
 
 
 def GpuKvWritePaged(kv: GpuPagedKv, table: GpuPageTable, seq_ids, positions, k, v, n_tokens: int) -> None:
     """Rows of k and v [n_tokens, n_kv_heads, head_dim] into the pages, quantised there if these hold 8 bits. seq_ids
     and positions are int32 tensors [n_tokens] (seq_ids None: row t is of sequence t; negative: padding)."""
     torch = _t()
-    _paged_device(kv, table.pages, seq_ids, positions, k, v)
-    row = 4 * n_tokens * kv.n_kv_heads * kv.head_dim
-    _check(paged_ops().kv_write(
-        kv.ref, table.ref, _addr(seq_ids, 4 * n_tokens, torch.int32, "seq_ids"),
-        _addr(positions, 4 * n_tokens, torch.int32, "positions"), _addr(k, row, torch.float32, "k"),
-        _addr(v, row, torch.float32, "v"), n_tokens))
+    f32, i32 = torch.float32, torch.int32
+    row = 4 * n_tokens * kv.row_elems
+    _check(_paged_call(kv, table).kv_write(
+        kv.ref, table.ref, _paged_addr(kv, seq_ids, 4 * n_tokens, i32, "seq_ids"),
+        _paged_addr(kv, positions, 4 * n_tokens, i32, "positions"), _paged_addr(kv, k, row, f32, "k"),
+        _paged_addr(kv, v, row, f32, "v"), n_tokens))
 
 
 def GpuQkNormRopeKvPaged(kv: GpuPagedKv, table: GpuPageTable, seq_ids, positions, q, k, v, q_norm, k_norm,
@@ -973,38 +989,39 @@ def GpuQkNormRopeKvPaged(kv: GpuPagedKv, table: GpuPageTable, seq_ids, positions
     """q_out <- RoPE(RMSNorm(q) * q_norm) at each row's position, RoPE(RMSNorm(k) * k_norm) and v into the pages.
     q_out may be q; k and v are not modified."""
     torch = _t()
-    f32 = torch.float32
-    _paged_device(kv, table.pages, seq_ids, positions, q, k, v, q_norm, k_norm, rope_tab, q_out)
+    f32, i32 = torch.float32, torch.int32
     d = kv.head_dim
-    qb, kb = 4 * n_tokens * n_heads * d, 4 * n_tokens * kv.n_kv_heads * d
-    _check(paged_ops().qk_norm_rope_kv(
-        kv.ref, table.ref, _addr(seq_ids, 4 * n_tokens, torch.int32, "seq_ids"),
-        _addr(positions, 4 * n_tokens, torch.int32, "positions"), _addr(q, qb, f32, "q"), _addr(k, kb, f32, "k"),
-        _addr(v, kb, f32, "v"), _addr(q_norm, 4 * d, f32, "q_norm"), _addr(k_norm, 4 * d, f32, "k_norm"), n_heads,
-        _addr(rope_tab, 4 * rope_rows * d, f32, "rope_tab"), rope_rows, n_tokens, eps, _addr(q_out, qb, f32, "q_out")))
+    qb, kb = 4 * n_tokens * n_heads * d, 4 * n_tokens * kv.row_elems
+    _check(_paged_call(kv, table).qk_norm_rope_kv(
+        kv.ref, table.ref, _paged_addr(kv, seq_ids, 4 * n_tokens, i32, "seq_ids"),
+        _paged_addr(kv, positions, 4 * n_tokens, i32, "positions"), _paged_addr(kv, q, qb, f32, "q"),
+        _paged_addr(kv, k, kb, f32, "k"), _paged_addr(kv, v, kb, f32, "v"), _paged_addr(kv, q_norm, 4 * d, f32, "q_norm"),
+        _paged_addr(kv, k_norm, 4 * d, f32, "k_norm"), n_heads,
+        _paged_addr(kv, rope_tab, 4 * rope_rows * d, f32, "rope_tab"), rope_rows, n_tokens, eps,
+        _paged_addr(kv, q_out, qb, f32, "q_out")))
 
 
 def GpuKvReadPaged(kv: GpuPagedKv, table: GpuPageTable, seq_ids, positions, n_tokens: int, k_out, v_out,
                    token_stride: int, head_stride: int, out_f32: Optional[bool] = None) -> None:
     """The rows back out of the pages: element d of row t of kv head h to out[t * token_stride + h * head_stride + d].
-    k_out and v_out are float32 or 16-bit (float16, int16, uint16) tensors; raw addresses need out_f32. Strides
-    (head_dim, max_seq * head_dim) fill a layer of the contiguous cache."""
+    k_out and v_out are float32 or 16-bit (float16, int16, uint16) tensors of one type; raw addresses need out_f32.
+    Strides (head_dim, max_seq * head_dim) fill a layer of the contiguous cache."""
     torch = _t()
-    _paged_device(kv, table.pages, seq_ids, positions, k_out, v_out)
+    i32 = torch.int32
+    dtype = getattr(k_out, "dtype", None)
     if out_f32 is None:
-        if not isinstance(k_out, torch.Tensor):
+        if dtype is None:
             raise RpgError("GpuKvReadPaged: raw addresses need out_f32")
-        out_f32 = k_out.dtype == torch.float32
-    for name, t in (("k_out", k_out), ("v_out", v_out)):
-        if isinstance(t, torch.Tensor) and t.dtype not in ((torch.float32,) if out_f32 else
-                                                           (torch.float16, torch.int16, torch.uint16)):
-            raise RpgError(f"GpuKvReadPaged: {name} is {t.dtype}")
+        out_f32 = dtype is torch.float32
+    if dtype is not None and dtype not in ((torch.float32,) if out_f32 else (torch.float16, torch.int16, torch.uint16)):
+        raise RpgError(f"GpuKvReadPaged: k_out is {dtype}")
     last = (n_tokens - 1) * token_stride + (kv.n_kv_heads - 1) * head_stride + kv.head_dim
     nbytes = (4 if out_f32 else 2) * last if n_tokens > 0 else 0
-    _check(paged_ops().kv_read(
-        kv.ref, table.ref, _addr(seq_ids, 4 * n_tokens, torch.int32, "seq_ids"),
-        _addr(positions, 4 * n_tokens, torch.int32, "positions"), n_tokens, 1 if out_f32 else 0,
-        _addr(k_out, nbytes, name="k_out"), _addr(v_out, nbytes, name="v_out"), token_stride, head_stride))
+    _check(_paged_call(kv, table).kv_read(
+        kv.ref, table.ref, _paged_addr(kv, seq_ids, 4 * n_tokens, i32, "seq_ids"),
+        _paged_addr(kv, positions, 4 * n_tokens, i32, "positions"), n_tokens, 1 if out_f32 else 0,
+        _paged_addr(kv, k_out, nbytes, dtype, "k_out"), _paged_addr(kv, v_out, nbytes, dtype, "v_out"), token_stride,
+        head_stride))
 
 
 def GpuAttentionPagedWorkspace(n_heads: int, n_kv_heads: int, head_dim: int) -> int:
@@ -1023,16 +1040,18 @@ def GpuAttentionPaged(kv: GpuPagedKv, table: GpuPageTable, lens, q, n_heads: int
     sequence, lens an int32 tensor [n_rows]. The workspace is zero before its first call, and belongs to one call at a
     time (workspace_bytes goes with a raw address)."""
     torch = _t()
-    _paged_device(kv, table.pages, lens, q, out, workspace, seq_ids)
+    f32, i32 = torch.float32, torch.int32
     span = 4 * n_rows * n_heads * kv.head_dim
+    dtype = getattr(workspace, "dtype", None)
     if workspace_bytes is None:
-        if not isinstance(workspace, torch.Tensor):
+        if dtype is None:
             raise RpgError("GpuAttentionPaged: a raw workspace needs workspace_bytes")
-        workspace_bytes = workspace.numel() * workspace.element_size()
-    _check(paged_ops().attention(
-        kv.ref, table.ref, _addr(seq_ids, 4 * n_rows, torch.int32, "seq_ids"),
-        _addr(lens, 4 * n_rows, torch.int32, "lens"), _addr(q, span, torch.float32, "q"), n_heads, n_rows,
-        _addr(out, span, torch.float32, "out"), _addr(workspace, workspace_bytes, name="workspace"), workspace_bytes))
+        workspace_bytes = workspace.nbytes
+    _check(_paged_call(kv, table).attention(
+        kv.ref, table.ref, _paged_addr(kv, seq_ids, 4 * n_rows, i32, "seq_ids"),
+        _paged_addr(kv, lens, 4 * n_rows, i32, "lens"), _paged_addr(kv, q, span, f32, "q"), n_heads, n_rows,
+        _paged_addr(kv, out, span, f32, "out"), _paged_addr(kv, workspace, workspace_bytes, dtype, "workspace"),
+        workspace_bytes))
 
 
 # ----------------------------------------------------------------------------- measurement
