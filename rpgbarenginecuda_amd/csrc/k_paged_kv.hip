@@ -4,7 +4,7 @@
 // described in kernels_gpu.h.
 //
 // Every kernel here moves each byte once and computes a few operations on it, so
-// memory bounds it (launch latency for a few tokens). A head row of D elements is
+// memory bounds it (launch latency for a few tokens: 2.4 us for one). A head row of D elements is
 // spread over D / 16 lanes, 16 elements each, arranged as head_row.h arranges 128
 // of them over 8 lanes: both members of every rotated pair (i, i + D/2) sit in one
 // lane, and the sums and maxima over a row are butterflies over its lanes.
@@ -51,6 +51,14 @@ constexpr int kBlock = 256;
 
 bool Aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// Workgroups go to the eight XCDs in turn. Each XCD takes one stretch of the tokens
+// instead of every eighth workgroup, so that neighbouring slots, and the 32 scales in
+// a line of them, meet in one L2: 16.2 -> 14.9 us for 8 x 1024 tokens written as 8 bits.
+__device__ __forceinline__ uint32_t WorkgroupInStretch() {
+  const uint32_t x = blockIdx.x & 7, each = gridDim.x >> 3, rest = gridDim.x & 7;
+  return x * each + (x < rest ? x : rest) + (blockIdx.x >> 3);
+}
+
 // A lane's 16 elements of a head row: a[c] is elements 4l + (D/4)c of the first
 // half, b[c] the same of the second. At D = 128 this is dev::HeadRow.
 struct Row {
@@ -63,16 +71,6 @@ struct RowOf {
   static constexpr int kLanes = D / 16;
 
   static __device__ __forceinline__ int Offset(int l, int c) { return 4 * l + (D / 4) * c; }
-
-  static __device__ __forceinline__ Row LoadStream(const float* p, int l) {
-    Row r;
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      r.a[c] = dev::LoadStream4(p + Offset(l, c));
-      r.b[c] = dev::LoadStream4(p + D / 2 + Offset(l, c));
-    }
-    return r;
-  }
 
   static __device__ __forceinline__ Row Load(const float* p, int l) {
     Row r;
@@ -119,11 +117,19 @@ struct RowOf {
     }
   }
 
+  // As fp16, 16 bytes a store: the lanes of a pair swap one of their two chunks of each half (as head_row.h does), so
+  // that a store instruction writes whole lines.
   static __device__ __forceinline__ void StoreHalf(uint16_t* p, int l, const Row& r) {
+    const bool odd = (l & 1) != 0;
+    const int at = odd ? D / 4 + 4 * (l - 1) : 4 * l;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      *reinterpret_cast<uint2*>(p + Offset(l, c)) = dev::PackHalf4(r.a[c]);
-      *reinterpret_cast<uint2*>(p + D / 2 + Offset(l, c)) = dev::PackHalf4(r.b[c]);
+    for (int s = 0; s < 2; ++s) {
+      const uint2 c0 = dev::PackHalf4(s == 0 ? r.a[0] : r.b[0]);
+      const uint2 c1 = dev::PackHalf4(s == 0 ? r.a[1] : r.b[1]);
+      const uint2 send = odd ? c0 : c1;
+      const uint2 recv = make_uint2(Quad<0xB1>(send.x), Quad<0xB1>(send.y));
+      *reinterpret_cast<uint4*>(p + D / 2 * s + at) =
+          odd ? make_uint4(recv.x, recv.y, c1.x, c1.y) : make_uint4(c0.x, c0.y, recv.x, recv.y);
     }
   }
 
@@ -139,14 +145,34 @@ struct RowOf {
     if (s < FLT_MIN) s = 0.0f;
     const float inv = finite && s > 0.0f ? 1.0f / s : 0.0f;
     if (l == 0) *scale = finite ? s : __builtin_nanf("");
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      *reinterpret_cast<uint32_t*>(p + Offset(l, c)) = Codes4(r.a[c], inv, finite);
-      *reinterpret_cast<uint32_t*>(p + D / 2 + Offset(l, c)) = Codes4(r.b[c], inv, finite);
-    }
+    // word b of a lane is its four codes of quarter b of the row. The four lanes of a quad trade them, so that lane i has
+    // the quad's words of quarter i, 16 bytes in a row.
+    uint32_t w[4] = {Codes4(r.a[0], inv, finite), Codes4(r.a[1], inv, finite), Codes4(r.b[0], inv, finite),
+                     Codes4(r.b[1], inv, finite)};
+    const int i = l & 3;
+    // lanes 1 apart trade the words of odd against even quarters, then lanes 2 apart those of 2 and 3 against 0 and 1
+    Trade<0xB1>((i & 1) != 0, &w[0], &w[1]);
+    Trade<0xB1>((i & 1) != 0, &w[2], &w[3]);
+    Trade<0x4E>((i & 2) != 0, &w[0], &w[2]);
+    Trade<0x4E>((i & 2) != 0, &w[1], &w[3]);
+    *reinterpret_cast<uint4*>(p + D / 4 * i + 16 * (l >> 2)) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 
  private:
+  // x of the lane that kPerm (a quad_perm) names: 0xB1 the neighbour, 0x4E the one 2 apart.
+  template <int kPerm>
+  static __device__ __forceinline__ uint32_t Quad(uint32_t x) {
+    return static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(x), kPerm, 0xF, 0xF, false));
+  }
+
+  // A lower lane's b against the upper lane's a.
+  template <int kPerm>
+  static __device__ __forceinline__ void Trade(bool upper, uint32_t* a, uint32_t* b) {
+    const uint32_t got = Quad<kPerm>(upper ? *a : *b);
+    *a = upper ? got : *a;
+    *b = upper ? *b : got;
+  }
+
   // Largest magnitude of four, infinity if one of them is not a finite number.
   static __device__ __forceinline__ float Top4(float4 v) {
     const auto mag = [](float x) { return fabsf(x) <= FLT_MAX ? fabsf(x) : INFINITY; };
@@ -164,33 +190,50 @@ struct RowOf {
 
 // Work units of a token: with kNorm its n_heads query rows, then the n_kv key rows,
 // then the n_kv value rows; D / 16 lanes each.
+//
+// Plain loads, since the projections before this kernel have just written q, k and v;
+// nontemporal stores of the queries; plain stores of the cache's rows, whole lines with
+// 16 bytes a lane. Measured at 2811 tokens of 16 + 8 + 8 heads into 8 bits, 75 MB:
+// 14.0 us = 5.4 TB/s; with nontemporal loads 17.0, with plain stores of the queries
+// 14.5, with write-through ones 15.8; held to 64 registers (spills) twice as long.
 template <int D, bool kQ8, bool kNorm>
 __global__ __launch_bounds__(kBlock) void PagedWriteKernel(
     PagedView view, const int32_t* __restrict__ seq_ids, const int32_t* __restrict__ positions, const float* q,
     const float* __restrict__ k, const float* __restrict__ v, const float* __restrict__ qw,
     const float* __restrict__ kw, int32_t n_heads, const float* __restrict__ tab, int64_t rope_rows, float eps,
-    float* q_out, int64_t n_units) {
+    float* q_out, uint32_t n_units) {
+  // the arguments in one batch of scalar loads at entry (the empty asm takes them as scalar inputs), not each before its
+  // first use
+  asm volatile("" ::"s"(seq_ids), "s"(positions), "s"(q), "s"(k), "s"(v), "s"(qw), "s"(kw), "s"(n_heads), "s"(tab),
+               "s"(rope_rows), "s"(eps), "s"(q_out), "s"(n_units), "s"(view.pages), "s"(view.n_seqs), "s"(view.max_pages),
+               "s"(view.n_pages), "s"(view.n_kv), "s"(view.page_shift));
   using R = RowOf<D>;
   const int l = threadIdx.x % R::kLanes;
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * (kBlock / R::kLanes) + threadIdx.x / R::kLanes;
+  const uint32_t unit = WorkgroupInStretch() * (kBlock / R::kLanes) + threadIdx.x / R::kLanes;
   if (unit >= n_units) return;
-  const int32_t nq = kNorm ? n_heads : 0;
-  const int32_t per_tok = nq + 2 * view.n_kv;
-  const int64_t t = unit / per_tok;
-  const int32_t j = static_cast<int32_t>(unit - t * per_tok);
+  const uint32_t nq = kNorm ? n_heads : 0;
+  const uint32_t per_tok = nq + 2 * view.n_kv;
+  const uint32_t token = unit / per_tok;
+  const uint32_t j = unit - token * per_tok;
+  const int64_t t = token;
   const bool is_q = j < nq;
   const bool is_v = j >= nq + view.n_kv;
-  const int32_t h = is_q ? j : is_v ? j - nq - view.n_kv : j - nq;
+  const uint32_t h = is_q ? j : is_v ? j - nq - view.n_kv : j - nq;
   const float* src = is_q ? q + (t * n_heads + h) * D : (is_v ? v : k) + (t * view.n_kv + h) * D;
-  Row r = R::LoadStream(src, l);
   const int32_t pos = positions[t];
-  Slot slot = dev::FindSlot(view, seq_ids != nullptr ? seq_ids[t] : t, pos);
+  const int64_t seq = seq_ids != nullptr ? seq_ids[t] : t;
+  Row r = R::Load(src, l);
+  Row w{}, trig{};
+  if (kNorm && !is_v) {  // a row of the table is read by this token alone: its load starts before the slot is known
+    w = R::Load(is_q ? qw : kw, l);
+    trig = R::Load(tab + (pos >= 0 && pos < rope_rows ? static_cast<int64_t>(pos) : 0) * D, l);
+  }
+  Slot slot = dev::FindSlot(view, seq, pos);
   if (slot.state == SlotState::kPadding) return;
   if (kNorm && pos >= rope_rows) slot.state = SlotState::kBad;
   const bool ok = slot.state == SlotState::kOk;
-  if (kNorm && !is_v && ok) {
-    const Row trig = R::Load(tab + static_cast<int64_t>(pos) * D, l);
-    R::Norm(r, R::Load(is_q ? qw : kw, l), eps);
+  if (kNorm && !is_v) {
+    R::Norm(r, w, eps);
     R::Rotate(r, trig);
   }
   if (is_q) {
@@ -213,66 +256,84 @@ __global__ __launch_bounds__(kBlock) void PagedWriteKernel(
   }
 }
 
-// Eight elements of a cached row as fp32: codes times the scale, or the halves.
-template <bool kQ8>
-__device__ __forceinline__ void LoadCached8(const void* pool, const float* scale, int64_t row, int64_t at, float (&x)[8]) {
+// kN (4 or 8) elements of a cached row as fp32: codes times the scale, or the halves.
+template <bool kQ8, int kN>
+__device__ __forceinline__ void LoadCached(const void* pool, const float* scale, int64_t row, int64_t at, float (&x)[kN]) {
   if constexpr (kQ8) {
     const float s = scale[row];
-    const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(pool) + at);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      x[i] = static_cast<float>(static_cast<int8_t>((i < 4 ? w.x : w.y) >> (8 * (i & 3)))) * s;
+    uint32_t w[kN / 4];
+    const int8_t* p = static_cast<const int8_t*>(pool) + at;
+    if constexpr (kN == 8) {
+      const dev::U32x2 d = *reinterpret_cast<const dev::U32x2*>(p);
+      w[0] = d.x, w[1] = d.y;
+    } else {
+      w[0] = *reinterpret_cast<const uint32_t*>(p);
     }
-  } else {
-    const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(pool) + at);
-    const uint32_t d[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      x[i] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(d[i / 2] >> (16 * (i & 1)))));
+    for (int i = 0; i < kN; ++i) x[i] = static_cast<float>(static_cast<int8_t>(w[i / 4] >> (8 * (i & 3)))) * s;
+  } else {
+    uint32_t w[kN / 2];
+    const uint16_t* p = static_cast<const uint16_t*>(pool) + at;
+    if constexpr (kN == 8) {
+      const dev::U32x4 d = *reinterpret_cast<const dev::U32x4*>(p);
+      w[0] = d.x, w[1] = d.y, w[2] = d.z, w[3] = d.w;
+    } else {
+      const dev::U32x2 d = *reinterpret_cast<const dev::U32x2*>(p);
+      w[0] = d.x, w[1] = d.y;
+    }
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      x[i] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1)))));
     }
   }
 }
 
-template <bool kF32>
-__device__ __forceinline__ void StoreRead8(void* out, int64_t at, const float (&x)[8]) {
-  if constexpr (kF32) {
-    float* p = static_cast<float*>(out) + at;
-    dev::StoreStream4(p, make_float4(x[0], x[1], x[2], x[3]));
-    dev::StoreStream4(p + 4, make_float4(x[4], x[5], x[6], x[7]));
+// One 16-byte store: 4 floats, or 8 halves.
+template <int kN>
+__device__ __forceinline__ void StoreRead(void* out, int64_t at, const float (&x)[kN]) {
+  if constexpr (kN == 4) {
+    dev::StoreStream4(static_cast<float*>(out) + at, make_float4(x[0], x[1], x[2], x[3]));
   } else {
     const uint2 a = dev::PackHalf4(make_float4(x[0], x[1], x[2], x[3]));
     const uint2 b = dev::PackHalf4(make_float4(x[4], x[5], x[6], x[7]));
-    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at) = make_uint4(a.x, a.y, b.x, b.y);
+    const dev::U32x4 w = {a.x, a.y, b.x, b.y};
+    __builtin_nontemporal_store(w, reinterpret_cast<dev::U32x4*>(static_cast<uint16_t*>(out) + at));
   }
 }
 
-// One work unit per (token, kv head): D / 8 lanes move 8 elements each of its key
-// and of its value row.
+// One work unit per (token, kv head): a lane moves 16 bytes of output of its key and
+// of its value row. Plain loads and nontemporal stores: 10.5 us for 6 x 700 tokens of
+// 8 fp16 heads (52 MB, 4.9 TB/s); with nontemporal loads 12.0, with plain stores 11.4.
 template <int D, bool kQ8, bool kF32>
 __global__ __launch_bounds__(kBlock) void PagedReadKernel(PagedView view, const int32_t* __restrict__ seq_ids,
                                                           const int32_t* __restrict__ positions, void* k_out,
                                                           void* v_out, int64_t token_stride, int64_t head_stride,
-                                                          int64_t n_units) {
-  constexpr int kLanes = D / 8;
+                                                          uint32_t n_units) {
+  asm volatile("" ::"s"(seq_ids), "s"(positions), "s"(k_out), "s"(v_out), "s"(token_stride), "s"(head_stride),
+               "s"(n_units), "s"(view.pages), "s"(view.n_seqs), "s"(view.max_pages), "s"(view.n_pages), "s"(view.n_kv),
+               "s"(view.page_shift), "s"(view.k), "s"(view.v), "s"(view.k_scale), "s"(view.v_scale));
+  constexpr int kN = kF32 ? 4 : 8;
+  constexpr int kLanes = D / kN;
   const int l = threadIdx.x % kLanes;
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * (kBlock / kLanes) + threadIdx.x / kLanes;
+  const uint32_t unit = WorkgroupInStretch() * (kBlock / kLanes) + threadIdx.x / kLanes;
   if (unit >= n_units) return;
-  const int64_t t = unit / view.n_kv;
-  const int32_t h = static_cast<int32_t>(unit - t * view.n_kv);
+  const uint32_t token = unit / static_cast<uint32_t>(view.n_kv);
+  const uint32_t h = unit - token * static_cast<uint32_t>(view.n_kv);
+  const int64_t t = token;
   const Slot slot = dev::FindSlot(view, seq_ids != nullptr ? seq_ids[t] : t, positions[t]);
   if (slot.state == SlotState::kPadding) return;
-  float kx[8], vx[8];
+  float kx[kN], vx[kN];
   if (slot.state == SlotState::kOk) {
     const int64_t row = slot.first + (static_cast<int64_t>(h) << view.page_shift);
-    LoadCached8<kQ8>(view.k, view.k_scale, row, row * D + 8 * l, kx);
-    LoadCached8<kQ8>(view.v, view.v_scale, row, row * D + 8 * l, vx);
+    LoadCached<kQ8>(view.k, view.k_scale, row, row * D + kN * l, kx);
+    LoadCached<kQ8>(view.v, view.v_scale, row, row * D + kN * l, vx);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) kx[i] = vx[i] = __builtin_nanf("");
+    for (int i = 0; i < kN; ++i) kx[i] = vx[i] = __builtin_nanf("");
   }
-  const int64_t at = t * token_stride + h * head_stride + 8 * l;
-  StoreRead8<kF32>(k_out, at, kx);
-  StoreRead8<kF32>(v_out, at, vx);
+  const int64_t at = t * token_stride + h * head_stride + kN * l;
+  StoreRead(k_out, at, kx);
+  StoreRead(v_out, at, vx);
 }
 
 void CheckRows(const char* what, const GpuPageTable& table, const int32_t* seq_ids, const int32_t* positions,
@@ -292,7 +353,13 @@ void LaunchWrite(const char* name, const GpuPagedKv& kv, const GpuPageTable& tab
   auto* kern = kv.head_dim == 128 ? (q8 ? PagedWriteKernel<128, true, kNorm> : PagedWriteKernel<128, false, kNorm>)
                                   : (q8 ? PagedWriteKernel<64, true, kNorm> : PagedWriteKernel<64, false, kNorm>);
   Launch(name, kern, dim3(GridFor(units, kBlock / (kv.head_dim / 16))), dim3(kBlock), dev::ViewOf(kv, table), seq_ids,
-         positions, q, k, v, qw, kw, n_heads, tab, rope_rows, eps, q_out, units);
+         positions, q, k, v, qw, kw, n_heads, tab, rope_rows, eps, q_out, static_cast<uint32_t>(units));
+}
+
+// Head rows of a call are counted in 32 bits.
+void CheckUnits(const char* what, int64_t n_tokens, int64_t rows_per_token) {
+  RPG_CHECK(n_tokens <= 0x7FFFFFFF / rows_per_token, "%s: %lld tokens of %lld rows are too many for one call", what,
+            static_cast<long long>(n_tokens), static_cast<long long>(rows_per_token));
 }
 
 }  // namespace
@@ -305,6 +372,7 @@ void GpuKvWritePaged(const GpuPagedKv& kv, const GpuPageTable& table, const int3
   CheckRows("KvWritePaged", table, seq_ids, positions, n_tokens);
   RPG_CHECK(k_dev != nullptr && v_dev != nullptr, "KvWritePaged got a null pointer");
   RPG_CHECK(Aligned16(k_dev) && Aligned16(v_dev), "KvWritePaged: k and v have to be 16-byte aligned");
+  CheckUnits("KvWritePaged", n_tokens, 2 * static_cast<int64_t>(kv.n_kv_heads));
   LaunchWrite<false>("PagedWriteKernel", kv, table, seq_ids, positions, nullptr, k_dev, v_dev, nullptr, nullptr, 0,
                      nullptr, 0, 0.0f, nullptr, n_tokens);
 }
@@ -326,6 +394,7 @@ void GpuQkNormRopeKvPaged(const GpuPagedKv& kv, const GpuPageTable& table, const
   const int64_t q_bytes = n_tokens * n_heads * kv.head_dim * 4;
   RPG_CHECK(q_out == q_dev || !Overlap(q_dev, q_bytes, q_out, q_bytes),
             "QkNormRopeKvPaged: q_out has to be q itself or apart from it");
+  CheckUnits("QkNormRopeKvPaged", n_tokens, n_heads + 2 * static_cast<int64_t>(kv.n_kv_heads));
   LaunchWrite<true>("PagedQkNormRopeWriteKernel", kv, table, seq_ids, positions, q_dev, k_dev, v_dev, q_norm, k_norm,
                     n_heads, rope_tab, rope_rows, eps, q_out, n_tokens);
 }
@@ -348,6 +417,7 @@ void GpuKvReadPaged(const GpuPagedKv& kv, const GpuPageTable& table, const int32
                 head_stride >= (n_tokens - 1) * token_stride + kv.head_dim,
             "KvReadPaged: rows of strides %lld and %lld overlap", static_cast<long long>(token_stride),
             static_cast<long long>(head_stride));
+  CheckUnits("KvReadPaged", n_tokens, kv.n_kv_heads);
   const int64_t units = n_tokens * kv.n_kv_heads;
   const bool q8 = kv.type == kKvQ8;
   auto* kern = kv.head_dim == 128
@@ -355,8 +425,9 @@ void GpuKvReadPaged(const GpuPagedKv& kv, const GpuPageTable& table, const int32
                          : (out_f32 ? PagedReadKernel<128, false, true> : PagedReadKernel<128, false, false>))
                    : (q8 ? (out_f32 ? PagedReadKernel<64, true, true> : PagedReadKernel<64, true, false>)
                          : (out_f32 ? PagedReadKernel<64, false, true> : PagedReadKernel<64, false, false>));
-  Launch("PagedReadKernel", kern, dim3(GridFor(units, kBlock / (kv.head_dim / 8))), dim3(kBlock),
-         dev::ViewOf(kv, table), seq_ids, positions, k_out, v_out, token_stride, head_stride, units);
+  Launch("PagedReadKernel", kern, dim3(GridFor(units, kBlock / (kv.head_dim / (out_f32 ? 4 : 8)))), dim3(kBlock),
+         dev::ViewOf(kv, table), seq_ids, positions, k_out, v_out, token_stride, head_stride,
+         static_cast<uint32_t>(units));
 }
 
 }  // namespace rpg
