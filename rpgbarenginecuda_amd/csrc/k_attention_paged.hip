@@ -62,19 +62,9 @@ constexpr int kTileHeads = 8;
 constexpr int kMaxGroups = 512;
 // Bytes between two counters: on lines of their own, as the decode attention's.
 constexpr size_t kCounterBytes = 256;
-#ifndef TUNE_WHOLE
-#define TUNE_WHOLE 4u
-#endif
-#ifndef TUNE_MANY
-#define TUNE_MANY 8192u
-#endif
 // Stores of a part to the workspace: device scope. With the streaming hint too their
 // acknowledgement came later (1 x 32768 positions of one kv head 24.2 against 21.7 us).
 constexpr int kPartPolicy = 16;
-
-#ifndef TUNE_NT
-#define TUNE_NT " nt"
-#endif
 
 using Half2 = _Float16 __attribute__((ext_vector_type(2)));
 using Half8 = _Float16 __attribute__((ext_vector_type(8)));
@@ -166,25 +156,25 @@ template <int kN, int kOff>
 __device__ __forceinline__ void LoadToLds(Resource rs, const uint32_t (&off)[kOff], uint32_t to) {
   static_assert(kN == 1 || kN == 2 || kN == 4, "");
   if constexpr (kN == 1) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen" TUNE_NT " lds"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds"
                  :
                  : "s"(to), "v"(off[0]), "s"(rs)
                  : "memory");
   } else if constexpr (kN == 2) {
     asm volatile(
         "s_mov_b32 m0, %0\n\ts_nop 4\n\t"
-        "buffer_load_dwordx4 %1, %3, 0 offen" TUNE_NT " lds\n\t"
-        "buffer_load_dwordx4 %2, %3, 0 offen offset:1024" TUNE_NT " lds"
+        "buffer_load_dwordx4 %1, %3, 0 offen nt lds\n\t"
+        "buffer_load_dwordx4 %2, %3, 0 offen offset:1024 nt lds"
         :
         : "s"(to), "v"(off[0]), "v"(off[1 % kOff]), "s"(rs)
         : "memory");
   } else {
     asm volatile(
         "s_mov_b32 m0, %0\n\ts_nop 4\n\t"
-        "buffer_load_dwordx4 %1, %5, 0 offen" TUNE_NT " lds\n\t"
-        "buffer_load_dwordx4 %2, %5, 0 offen offset:1024" TUNE_NT " lds\n\t"
-        "buffer_load_dwordx4 %3, %5, 0 offen offset:2048" TUNE_NT " lds\n\t"
-        "buffer_load_dwordx4 %4, %5, 0 offen offset:0xc00" TUNE_NT " lds"
+        "buffer_load_dwordx4 %1, %5, 0 offen nt lds\n\t"
+        "buffer_load_dwordx4 %2, %5, 0 offen offset:1024 nt lds\n\t"
+        "buffer_load_dwordx4 %3, %5, 0 offen offset:2048 nt lds\n\t"
+        "buffer_load_dwordx4 %4, %5, 0 offen offset:0xc00 nt lds"
         :
         : "s"(to), "v"(off[0]), "v"(off[1 % kOff]), "v"(off[2 % kOff]), "v"(off[3 % kOff]), "s"(rs)
         : "memory");
@@ -229,8 +219,8 @@ __device__ __forceinline__ uint32_t Scalar(uint32_t x) { return __builtin_amdgcn
 // a unit, so that all workgroups get alike. With fewer, joining what two workgroups hold of a pair (a round trip to memory
 // to store, one to count, one to read) costs more than some units more in turn: a pair of up to kWholeUnits is one item, a
 // longer one is cut evenly into items of at most 2^step, about what each workgroup then gets.
-constexpr uint32_t kManyUnits = TUNE_MANY;
-constexpr uint32_t kWholeUnits = TUNE_WHOLE;
+constexpr uint32_t kManyUnits = 8192;
+constexpr uint32_t kWholeUnits = 4;
 
 struct Cut {
   bool units;
@@ -505,6 +495,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
   constexpr int kCopies = kQ8 ? 4 : 2;     // columns of a head, that is lanes that have its final sums
   constexpr int kHeadCols = 16 / kCopies;
   constexpr int kOwn = kE / kCopies;       // tiles of 16 elements that each of them writes
+  // Whether the int32 sums of values live from step to step. For two column tiles they and the fp32 ones would not both
+  // fit in the registers, and each step's are taken to fp32 at once.
+  constexpr bool kKeepSums = kQ8 && kTiles == 1;
 
   // a wave's step of keys and values, each row's scale behind them
   constexpr int kStage = kStep * kRow + (kQ8 ? kStep * 4 : 0);
@@ -676,7 +669,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
     float to_score[kTiles], m[kTiles], l[kTiles];
     float ref = 0.0f;  // 8-bit values: a power of two above the scales so far
     F32x4 acc[kTiles][kE];
-    I32x4 sum[kQ8 ? kTiles : 1][kQ8 ? kE : 1];
+    I32x4 sum[kKeepSums ? kE : 1];
     // the digit that this lane's column stands for, and its weight
     const uint32_t digit = static_cast<uint32_t>(copy) * 0x0101u + 0x0400u;
     const float digit_by = __int_as_float((127 + 8 * copy) << 23);
@@ -698,7 +691,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
 #pragma unroll
         for (int i = 0; i < kE; ++i) {
           acc[t][i] = F32x4{0.0f, 0.0f, 0.0f, 0.0f};
-          if constexpr (kQ8) sum[t][i] = I32x4{0, 0, 0, 0};
+          if constexpr (kKeepSums) sum[i] = I32x4{0, 0, 0, 0};
         }
         constexpr int kAt = kQ8 ? 16 : 8;  // elements of a lane for one product
         float x[kSteps][kAt];
@@ -754,9 +747,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
         for (int i = 0; i < kE; ++i) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            acc[t][i][r] = fmaf(static_cast<float>(sum[t][i][r]), digit_by, acc[t][i][r]) * back;
+            if constexpr (kKeepSums) {
+              acc[t][i][r] = fmaf(static_cast<float>(sum[i][r]), digit_by, acc[t][i][r]) * back;
+            } else {
+              acc[t][i][r] *= back;
+            }
           }
-          sum[t][i] = I32x4{0, 0, 0, 0};
+          if constexpr (kKeepSums) sum[i] = I32x4{0, 0, 0, 0};
         }
       }
     };
@@ -783,7 +780,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
       const int this_bad = bad;
       // ---- scores, once the keys are there: the values' loads are younger
       WaitLoads<kStageLoads>();
-      float s[kSub][4];  // of one column tile
+      float s[kTiles][kSub][4];
       I32x4 raw[kQ8 ? kTiles : 1][kSub];
       if constexpr (kQ8) {
 #pragma unroll
@@ -809,7 +806,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
             sums = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[i], sums, 0, 0, 0);
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[j][i] = (sums[i] + Ror<8>(sums[i])) * to_score[0];
+          for (int i = 0; i < 4; ++i) s[0][j][i] = (sums[i] + Ror<8>(sums[i])) * to_score[0];
         }
       }
       // ---- the next unit, and its keys
@@ -823,6 +820,23 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
       if constexpr (kQ8) {
 #pragma unroll
         for (int j = 0; j < kSub; ++j) ks[j] = scales_at(k_mine, j);
+      }
+      // the products of queries' and keys' codes as scores
+      const auto scale_scores = [&](int t) {
+#pragma unroll
+        for (int j = 0; j < kSub; ++j) {
+          const float by[4] = {ks[j].x, ks[j].y, ks[j].z, ks[j].w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float x = static_cast<float>(raw[t][j][i]) * to_score[t];
+            x += Ror<8>(x);
+            s[t][j][i] = (x + Ror<4>(x)) * by[i];
+          }
+        }
+      };
+      if constexpr (kTiles > 1) {  // before the loads and not, as below, while they run: the scales' registers are needed
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) scale_scores(t);
       }
       __builtin_amdgcn_sched_barrier(0);
       if (more) {
@@ -848,21 +862,15 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
       // ---- weights
       // a column tile's scores, and their maximum with m
       const auto take_scores = [&](int t) {
+        if constexpr (kQ8 && kTiles == 1) scale_scores(t);
         float top = m[t];
 #pragma unroll
         for (int j = 0; j < kSub; ++j) {
-          const float by[4] = {kQ8 ? ks[kQ8 ? j : 0].x : 1.0f, kQ8 ? ks[kQ8 ? j : 0].y : 1.0f,
-                               kQ8 ? ks[kQ8 ? j : 0].z : 1.0f, kQ8 ? ks[kQ8 ? j : 0].w : 1.0f};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            if constexpr (kQ8) {
-              float x = static_cast<float>(raw[t][j][i]) * to_score[t];
-              x += Ror<8>(x);
-              s[j][i] = (x + Ror<4>(x)) * by[i];
-            }
-            if (this_bad & (1 << j)) s[j][i] = NAN;
-            if (tail && 16 * j + 4 * g + i >= left) s[j][i] = -INFINITY;
-            top = fmaxf(top, s[j][i]);
+            if (this_bad & (1 << j)) s[t][j][i] = NAN;
+            if (tail && 16 * j + 4 * g + i >= left) s[t][j][i] = -INFINITY;
+            top = fmaxf(top, s[t][j][i]);
           }
         }
         return MaxAcrossRows(top);
@@ -900,7 +908,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
           return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b)));
         }));
         big = __builtin_amdgcn_readfirstlane(big);
-        if (big >= __float_as_uint(ref) || ++since >= 1024) {  // 1024 steps: int32 holds 2^17 products of 2^14
+        if (big >= __float_as_uint(ref) || (kKeepSums && ++since >= 1024)) {  // 1024 steps: int32 holds 2^17 products of 2^14
           float by = 1.0f;
           if (big >= __float_as_uint(ref)) {
             const int e = min(max(static_cast<int>(big >> 23) + 1, 27), 254);
@@ -934,7 +942,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
             uint32_t d[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const float p = __builtin_amdgcn_exp2f(s[j][i] - safe);
+              const float p = __builtin_amdgcn_exp2f(s[t][j][i] - safe);
               l[t] += p;
               d[i] = static_cast<uint32_t>(static_cast<int>(fmaf(p * by[i], up, 0.5f))) + 0x80808080u;
             }
@@ -953,8 +961,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
         for (int i = 0; i < kE; ++i) {
 #pragma unroll
           for (int t = 0; t < kTiles; ++t) {
-            sum[t][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(I32x4{a[i][0][0], a[i][0][1], a[i][1][0], a[i][1][1]}, w[t],
-                                                              sum[t][i], 0, 0, 0);
+            const I32x4 v = I32x4{a[i][0][0], a[i][0][1], a[i][1][0], a[i][1][1]};
+            if constexpr (kKeepSums) {
+              sum[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(v, w[t], sum[i], 0, 0, 0);
+            } else {
+              const I32x4 x = __builtin_amdgcn_mfma_i32_16x16x64_i8(v, w[t], I32x4{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) acc[t][i][r] = fmaf(static_cast<float>(x[r]), digit_by, acc[t][i][r]);
+            }
           }
         }
       } else {
@@ -980,7 +994,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
           float w[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            w[i] = __builtin_amdgcn_exp2f(s[j][i] - safe);
+            w[i] = __builtin_amdgcn_exp2f(s[0][j][i] - safe);
             l[0] += w[i];
           }
           pt[j][0] = Term2(w[0] * up, w[1] * up, copy != 0);
@@ -1008,10 +1022,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
       if (!turn) continue;
 
       // ---- the piece's (m, l, o): out, or kept where it is not the whole of its pair
-      if constexpr (kQ8) {
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t) take_sums(t, 1.0f);
-      }
+      if constexpr (kKeepSums) take_sums(0, 1.0f);
       const bool whole = c_first == 0 && c_end == piece_units;
       const float unit = kQ8 ? ref * 0x1p-27f : 0x1p-14f;
       if (!whole) {
