@@ -663,10 +663,19 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
     load_k();
     load_v();
 
+    // Where there are two column tiles, the lanes of odd copies of a column do the second tile's softmax and those of even
+    // copies the first's: of the four lanes that have a score two would only do it again. x of tile t in every lane:
+    const bool second = kTiles > 1 && (copy & 1) != 0;
+    const auto of_tile = [&](int t, float x) {
+      if constexpr (kTiles == 1) return x;
+      const float other = Ror<4>(x);  // by all lanes
+      return second == (t == 1) ? x : other;
+    };
+
     // per piece: the queries' terms or digits, and the running state
     Half8 qh[kQ8 ? 1 : kSteps];
     I32x4 qi[kQ8 ? kTiles : 1][kQ8 ? kSteps : 1];
-    float to_score[kTiles], m[kTiles], l[kTiles];
+    float to_score[kTiles], m, l;
     float ref = 0.0f;  // 8-bit values: a power of two above the scales so far
     F32x4 acc[kTiles][kE];
     I32x4 sum[kKeepSums ? kE : 1];
@@ -681,13 +690,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
       heads = min(tile_heads, group - h0);
       head_row = static_cast<int64_t>(row) * n_heads + kh * group + h0;
       ref = 0.0f;
+      m = -INFINITY;
+      l = 0.0f;
 #pragma unroll
       for (int t = 0; t < kTiles; ++t) {
         const int h = t * kHeadCols + head_col;
         const bool there = h < heads;
         const float* qr = q + (head_row + (there ? h : 0)) * D;
-        m[t] = -INFINITY;
-        l[t] = 0.0f;
 #pragma unroll
         for (int i = 0; i < kE; ++i) {
           acc[t][i] = F32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -780,7 +789,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
       const int this_bad = bad;
       // ---- scores, once the keys are there: the values' loads are younger
       WaitLoads<kStageLoads>();
-      float s[kTiles][kSub][4];
+      float s[kSub][4];
       I32x4 raw[kQ8 ? kTiles : 1][kSub];
       if constexpr (kQ8) {
 #pragma unroll
@@ -806,7 +815,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
             sums = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[i], sums, 0, 0, 0);
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[0][j][i] = (sums[i] + Ror<8>(sums[i])) * to_score[0];
+          for (int i = 0; i < 4; ++i) s[j][i] = (sums[i] + Ror<8>(sums[i])) * to_score[0];
         }
       }
       // ---- the next unit, and its keys
@@ -821,23 +830,25 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
 #pragma unroll
         for (int j = 0; j < kSub; ++j) ks[j] = scales_at(k_mine, j);
       }
-      // the products of queries' and keys' codes as scores
-      const auto scale_scores = [&](int t) {
+      // the products of queries' and keys' codes as scores: sums over the digits' columns
+      const auto scale_scores = [&]() {
 #pragma unroll
         for (int j = 0; j < kSub; ++j) {
           const float by[4] = {ks[j].x, ks[j].y, ks[j].z, ks[j].w};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            float x = static_cast<float>(raw[t][j][i]) * to_score[t];
-            x += Ror<8>(x);
-            s[t][j][i] = (x + Ror<4>(x)) * by[i];
+            float x[kTiles];
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) {
+              x[t] = static_cast<float>(raw[t][j][i]) * to_score[t];
+              x[t] += Ror<8>(x[t]);
+            }
+            const float mine = second ? x[kTiles - 1] : x[0], other = second ? x[0] : x[kTiles - 1];
+            s[j][i] = (mine + Ror<4>(other)) * by[i];
           }
         }
       };
-      if constexpr (kTiles > 1) {  // before the loads and not, as below, while they run: the scales' registers are needed
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t) scale_scores(t);
-      }
+      if constexpr (kTiles > 1) scale_scores();  // before the loads and not, as below, while they run: registers
       __builtin_amdgcn_sched_barrier(0);
       if (more) {
         ++c;
@@ -860,23 +871,18 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
       }
       __builtin_amdgcn_sched_barrier(0);
       // ---- weights
-      // a column tile's scores, and their maximum with m
-      const auto take_scores = [&](int t) {
-        if constexpr (kQ8 && kTiles == 1) scale_scores(t);
-        float top = m[t];
+      if constexpr (kQ8 && kTiles == 1) scale_scores();
+      float top = m;
 #pragma unroll
-        for (int j = 0; j < kSub; ++j) {
+      for (int j = 0; j < kSub; ++j) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (this_bad & (1 << j)) s[t][j][i] = NAN;
-            if (tail && 16 * j + 4 * g + i >= left) s[t][j][i] = -INFINITY;
-            top = fmaxf(top, s[t][j][i]);
-          }
+        for (int i = 0; i < 4; ++i) {
+          if (this_bad & (1 << j)) s[j][i] = NAN;
+          if (tail && 16 * j + 4 * g + i >= left) s[j][i] = -INFINITY;
+          top = fmaxf(top, s[j][i]);
         }
-        return MaxAcrossRows(top);
-      };
-      float first_top = 0.0f;
-      if constexpr (kTiles == 1) first_top = take_scores(0);
+      }
+      top = MaxAcrossRows(top);
       // the values are there: the next keys' loads, if any, are younger
       if (more) {
         WaitLoads<kStageLoads>();
@@ -916,40 +922,38 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
             ref = __int_as_float(e << 23);
           }
 #pragma unroll
-          for (int t = 0; t < kTiles; ++t) {
-            take_sums(t, by);
-            if (big >= 0x7F800000u) l[t] = NAN;
-          }
+          for (int t = 0; t < kTiles; ++t) take_sums(t, by);
+          if (big >= 0x7F800000u) l = NAN;
           since = 0;
         }
         const float up = 0x1p27f * __int_as_float((254 << 23) - __float_as_int(ref));  // 2^27 / ref
+        if (__any(top > m + 3.0f)) {
+          const float to = top > m + 3.0f ? top : m;
+          const float back = __builtin_amdgcn_exp2f(m - (to == -INFINITY ? 0.0f : to));
+          m = to;
+          l *= back;
+#pragma unroll
+          for (int t = 0; t < kTiles; ++t) take_sums(t, of_tile(t, back));
+        }
+        const float safe = m == -INFINITY ? 0.0f : m;
         I32x4 w[kTiles];  // tile j of 16 keys: bytes 4 j ..
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
-          if constexpr (kTiles > 1) __builtin_amdgcn_sched_barrier(0);  // one after the other: registers
-          const float top = kTiles == 1 ? first_top : take_scores(t);
-          if (__any(top > m[t] + 3.0f)) {
-            const float to = top > m[t] + 3.0f ? top : m[t];
-            const float back = __builtin_amdgcn_exp2f(m[t] - (to == -INFINITY ? 0.0f : to));
-            m[t] = to;
-            l[t] *= back;
-            take_sums(t, back);
-          }
-          const float safe = m[t] == -INFINITY ? 0.0f : m[t];
+        for (int j = 0; j < kSub; ++j) {
+          const float by[4] = {vs[j].x, vs[j].y, vs[j].z, vs[j].w};
+          uint32_t d[kTiles][4];
 #pragma unroll
-          for (int j = 0; j < kSub; ++j) {
-            const float by[4] = {vs[j].x, vs[j].y, vs[j].z, vs[j].w};
-            uint32_t d[4];
+          for (int i = 0; i < 4; ++i) {
+            const float p = __builtin_amdgcn_exp2f(s[j][i] - safe);
+            l += p;
+            const int x = static_cast<int>(fmaf(p * by[i], up, 0.5f));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float p = __builtin_amdgcn_exp2f(s[t][j][i] - safe);
-              l[t] += p;
-              d[i] = static_cast<uint32_t>(static_cast<int>(fmaf(p * by[i], up, 0.5f))) + 0x80808080u;
+            for (int t = 0; t < kTiles; ++t) {
+              d[t][i] = __float_as_uint(of_tile(t, __int_as_float(x + static_cast<int>(0x80808080u))));
             }
-            w[t][j] = Digit4(d[0], d[1], d[2], d[3], digit);
           }
+#pragma unroll
+          for (int t = 0; t < kTiles; ++t) w[t][j] = Digit4(d[t][0], d[t][1], d[t][2], d[t][3], digit);
         }
-        if constexpr (kTiles > 1) __builtin_amdgcn_sched_barrier(0);
         I32x2 a[kE][2];
 #pragma unroll
         for (int i = 0; i < kE; ++i) {
@@ -979,10 +983,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
             if (to / kRow >= left) *reinterpret_cast<uint4*>(v_mine + to) = make_uint4(0u, 0u, 0u, 0u);
           }
         }
-        const float safe = first_top == -INFINITY ? 0.0f : first_top;
-        const float back = __builtin_amdgcn_exp2f(m[0] - safe);
-        m[0] = first_top;
-        l[0] *= back;
+        const float safe = top == -INFINITY ? 0.0f : top;
+        const float back = __builtin_amdgcn_exp2f(m - safe);
+        m = top;
+        l *= back;
         if (__any(back != 1.0f)) {
 #pragma unroll
           for (int i = 0; i < kE; ++i) acc[0][i] *= back;
@@ -994,8 +998,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
           float w[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            w[i] = __builtin_amdgcn_exp2f(s[0][j][i] - safe);
-            l[0] += w[i];
+            w[i] = __builtin_amdgcn_exp2f(s[j][i] - safe);
+            l += w[i];
           }
           pt[j][0] = Term2(w[0] * up, w[1] * up, copy != 0);
           pt[j][1] = Term2(w[2] * up, w[3] * up, copy != 0);
@@ -1030,9 +1034,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
         if (lane == 0) pieces[wave][which] = Piece{u - c_end, c_first, c_end, piece_units, piece_row, piece_pair};
         my_held |= 1 << which;
       }
+      l = SumAcrossRows(l);
 #pragma unroll
       for (int t = 0; t < kTiles; ++t) {
-        const float total = SumAcrossRows(l[t]);
+        const float total = of_tile(t, l), top = of_tile(t, m);
         const float by = whole ? unit / total : unit;
         const int h = t * kHeadCols + head_col;
         F32x4 own[kOwn];
@@ -1050,14 +1055,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
         if (!whole && more) {
 #pragma unroll
           for (int i = 0; i < kOwn; ++i) kept[t][i] = own[i];
-          kept_m[t] = m[t];
+          kept_m[t] = top;
           kept_l[t] = total;
         } else if (h < heads) {
           float* to = whole ? out + (head_row + h) * D : reinterpret_cast<float*>(v_mine) + h * kPart;
 #pragma unroll
           for (int i = 0; i < kOwn; ++i) *reinterpret_cast<F32x4*>(to + 16 * (copy * kOwn + i) + 4 * g) = own[i];
           if (!whole && copy == 0 && g == 0) {
-            to[D] = m[t];
+            to[D] = top;
             to[D + 1] = total;
           }
         }
