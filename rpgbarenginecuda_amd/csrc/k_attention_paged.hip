@@ -428,13 +428,16 @@ __device__ __forceinline__ Piece UniformPiece(const Piece& p) {
                __builtin_amdgcn_readfirstlane(p.row),   __builtin_amdgcn_readfirstlane(p.pair)};
 }
 
+// One tile is the rule, and a division takes as long as twenty other instructions.
+__device__ __forceinline__ int32_t KvHeadOf(int32_t pair, int32_t tiles) { return tiles == 1 ? pair : pair / tiles; }
+
 // The query heads of a piece.
 struct HeadsOf {
   int32_t heads;
   int64_t head_row;  // row of the first in q and out
 
   __device__ __forceinline__ HeadsOf(const Piece& p, int32_t n_heads, int32_t group, int32_t tiles, int32_t tile_heads) {
-    const int32_t kh = p.pair / tiles;
+    const int32_t kh = KvHeadOf(p.pair, tiles);
     const int32_t h0 = (p.pair - kh * tiles) * tile_heads;
     heads = min(tile_heads, group - h0);
     head_row = static_cast<int64_t>(p.row) * n_heads + kh * group + h0;
@@ -610,7 +613,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
     const auto find = [&]() {
       bad = 0;
       const int32_t pos = static_cast<int32_t>(c) * kStep;
-      const int32_t kh = pair / tiles;
+      const int32_t kh = KvHeadOf(pair, tiles);
       int32_t pages[kSub];
 #pragma unroll
       for (int j = 0; j < kSub; ++j) {
@@ -685,7 +688,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
     int64_t head_row = 0;
     int32_t heads = 0;
     const auto begin_piece = [&]() {
-      const int32_t kh = pair / tiles;
+      const int32_t kh = KvHeadOf(pair, tiles);
       const int32_t h0 = (pair - kh * tiles) * tile_heads;
       heads = min(tile_heads, group - h0);
       head_row = static_cast<int64_t>(row) * n_heads + kh * group + h0;
@@ -1277,8 +1280,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
 
   // rows with nothing to attend to: zeros, or NaN where the row is out of range
   for (int64_t r = me; r < rows.n_rows; r += gridDim.x) {
-    const int64_t seq = rows.Seq(static_cast<int32_t>(r));
-    const int32_t len = rows.lens[r];
+    const int32_t seq = static_cast<int32_t>(batch.SeqOf(static_cast<int32_t>(r)));
+    const int32_t len = batch.LenOf(static_cast<int32_t>(r));
     if (seq < 0) continue;
     const bool fine = rows.Fine(seq, len);
     if (fine && len > 0) continue;
@@ -1349,7 +1352,7 @@ void GpuAttentionPaged(const GpuPagedKv& kv, const GpuPageTable& table, const in
   // parts of a row cost more to join than the card gives for them (1 x 32768 positions, 8 kv heads: 22.7 against 25.0 us)
   const int64_t all_pairs = n_rows * rows.pairs;
   const int64_t at_once = all_pairs * kJoinAtOnce < kMaxGroups ? kMaxGroups / 2 : kMaxGroups;
-  const int64_t groups = std::min<int64_t>(at_once, (all_pairs * most + kWaves - 1) / kWaves);
+  const int64_t groups = std::min<int64_t>(at_once, all_pairs * ((most + kWholeUnits - 1) / kWholeUnits));
   const float scale_log2 =
       static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(kv.head_dim)));
   auto* kern = kv.head_dim == 128 ? PagedAttentionKernel<128, false, 1> : PagedAttentionKernel<64, false, 1>;
