@@ -422,12 +422,6 @@ struct Piece {
   int32_t row, pair;
 };
 
-// In scalar registers: a buffer descriptor made from vector ones would be looped over.
-__device__ __forceinline__ Piece UniformPiece(const Piece& p) {
-  return Piece{Scalar(p.first), Scalar(p.c0), Scalar(p.c1), Scalar(p.n),
-               __builtin_amdgcn_readfirstlane(p.row),   __builtin_amdgcn_readfirstlane(p.pair)};
-}
-
 // One tile is the rule, and a division takes as long as twenty other instructions.
 __device__ __forceinline__ int32_t KvHeadOf(int32_t pair, int32_t tiles) { return tiles == 1 ? pair : pair / tiles; }
 
@@ -1101,23 +1095,23 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
   char* const slots = workspace + kMaxGroups * kCounterBytes;
   Piece open[2];
   int n_open = 0;
-  int from = 0;  // wave * 2 + which
-  while (from < 2 * kWaves) {
-    if (!(held[from >> 1] >> (from & 1) & 1)) {
-      ++from;
-      continue;
-    }
-    Piece run = UniformPiece(pieces[from >> 1][from & 1]);
-    int list = 1 << from;
-    int to = from + 1;
-    for (; to < 2 * kWaves; ++to) {
-      if (!(held[to >> 1] >> (to & 1) & 1)) continue;
-      const Piece next = UniformPiece(pieces[to >> 1][to & 1]);
-      if (next.first != run.first) break;
-      run.c1 = next.c1;
-      list |= 1 << to;
-    }
-    from = to;
+  const int of_lane = lane < 2 * kWaves ? lane : 0;  // lane i has piece i % 2 of wave i / 2
+  const Piece mine = pieces[of_lane >> 1][of_lane & 1];
+  const bool there = lane < 2 * kWaves && (held[of_lane >> 1] >> (of_lane & 1) & 1) != 0;
+  uint64_t open_lanes = __ballot(there);
+  while (open_lanes != 0) {
+    const int from = __builtin_ctzll(open_lanes);
+    const auto field = [&](uint32_t x, int i) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(x, i)); };
+    Piece run;
+    run.first = field(mine.first, from);
+    const uint64_t same = __ballot(there && mine.first == run.first);  // one behind the other
+    run.c0 = field(mine.c0, from);
+    run.c1 = field(mine.c1, 63 - __builtin_clzll(same));
+    run.n = field(mine.n, from);
+    run.row = static_cast<int32_t>(field(static_cast<uint32_t>(mine.row), from));
+    run.pair = static_cast<int32_t>(field(static_cast<uint32_t>(mine.pair), from));
+    const int list = static_cast<int>(same);
+    open_lanes &= ~same;
     const HeadsOf of(run, n_heads, group, tiles, tile_heads);
     const bool whole = run.c0 == 0 && run.c1 == run.n;
     const bool leads = run.first + run.c0 == begin;  // the workgroup's first piece
