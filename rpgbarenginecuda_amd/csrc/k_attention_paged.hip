@@ -1163,9 +1163,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
   // reads, with device-coherent loads, is all there. No workgroup waits for another. Where a pair has more parts than
   // kJoinAtOnce, the last of each kFan joins those and counts for them.
   if (n_open > 0) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    // which parts of their pairs they are: kept where the loop after the count finds them
+    // which parts of their pairs they are, while the stores are under way
     Parts of_first, of_last;
 #pragma unroll 1
     for (int i = 0; i < n_open; ++i) {
@@ -1173,6 +1171,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
       if (i == 0) of_first = of;
       of_last = of;
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
     if (threadIdx.x < n_open) {  // both at once
       const Parts& of = threadIdx.x == 0 ? of_first : of_last;
       flags[threadIdx.x] = Count(workspace, of.blocks > 1 ? of.BlockCounter() : of.PairCounter(), of.block_parts);
@@ -1193,8 +1193,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
       // kBatch of them requested at a time: a round trip past the L2 costs more than the arithmetic.
       constexpr int kBatch = 8;
       const int columns = heads.heads * (D / 4);
-      const int sets = 64 * kWaves / columns;
-      const int set = static_cast<int>(threadIdx.x) / columns, column = static_cast<int>(threadIdx.x) % columns;
+      // whole quotients of small numbers, a half away from where the reciprocal's error would show
+      const float per_set = __builtin_amdgcn_rcpf(static_cast<float>(heads.heads));
+      const int sets = static_cast<int>((64 * kWaves / (D / 4) + 0.5f) * per_set);
+      const int set = static_cast<int>((static_cast<float>(threadIdx.x / (D / 4)) + 0.5f) * per_set);
+      const int column = static_cast<int>(threadIdx.x) - set * columns;
       const int h = column / (D / 4);
       float top, l;
       float4 o;
