@@ -85,6 +85,38 @@ def test_attention_vs_f64(gpu, kind, heads, n_kv, d, page, lens):
     assert np.array_equal(got, attend(gpu, kv, table, lens, q))  # shares are joined in one order
 
 
+# What follows is shared out otherwise: from 8192 units (of 32 positions for fp16 rows of 128, else 64) all workgroups get
+# alike; a row in more than 32 parts is joined in two steps; above 64 rows a lane stands for several, above 4096 the search
+# for a row has a step more.
+SHARED = [
+    # kind, heads, n_kv, d, page, lens
+    (F16, 4, 2, 128, 64, [(0, 2000, 1999, 700)[i % 4] + i for i in range(120)]),
+    (Q8, 5, 1, 64, 32, [(4100 if i % 5 else 0) - i for i in range(150)]),
+    (Q8, 2, 2, 128, 64, [4000, 1, 0, 5000, 77] * 16),
+    (Q8, 8, 1, 128, 256, [8190] * 66),
+    (F16, 2, 1, 64, 16, [140000, 140001, 140002, 120000]),
+    (Q8, 5, 1, 128, 64, [20000]),
+    (F16, 2, 2, 128, 16, [12000, 0, 31]),
+    (F16, 1, 1, 64, 16, [(11 * i) % 40 for i in range(5000)]),
+    (Q8, 2, 2, 64, 16, [(11 * i) % 90 for i in range(5000)]),
+]
+
+
+@pytest.mark.parametrize("kind,heads,n_kv,d,page,lens", SHARED)
+def test_ways_of_sharing_out(gpu, kind, heads, n_kv, d, page, lens):
+    lens = [max(n, 0) for n in lens]
+    rng = np.random.default_rng(heads * 1000 + len(lens))
+    pages = Pages(rng, kind, n_kv, d, page, lens).fill_random(rng, lens)
+    q = rng.normal(0, 1.5, (len(lens), heads, d)).astype(np.float32)
+    kv, table = pages.device(gpu)
+    got = attend(gpu, kv, table, lens, q)
+    n = len(lens)
+    look = range(n) if sum(lens) <= 250_000 else sorted({0, n - 1, *(int(r) for r in rng.choice(n, 20))})
+    check(got[list(look)], pages, [lens[r] for r in look], q[list(look)], list(look))
+    assert np.all(np.isfinite(got))
+    assert np.array_equal(got, attend(gpu, kv, table, lens, q))
+
+
 @pytest.mark.parametrize("kind", [F16, Q8])
 def test_magnitudes(gpu, kind):
     """Queries and keys that make one position take everything, or all count alike; tiny, huge and zero queries; value
@@ -373,3 +405,61 @@ def test_a_batch_is_served(gpu, ora, kind, n_kv, group, page):
                 gpu.GpuAttentionFromCache(heads, n_kv, d, now[i], qq, 1, flat[i][0], flat[i][1], room, other)
                 _, smag, vmax = attention(host(rot)[i], pages.rows("k", i, now[i] + 1), pages.rows("v", i, now[i] + 1))
                 assert np.all(np.abs(host(other[0]) - host(got[i])).max(-1) <= 2 * bound(d, now[i] + 1, smag, vmax))
+
+
+@pytest.mark.parametrize("kind", [F16, Q8])
+def test_captured_steps_of_a_batch(gpu, kind):
+    """A step of a batch as one graph: norm, rotation and write, then attention, with positions and lengths counted up in
+    it. Replays, with eager calls of the same operators on other buffers in between, give the eager steps' bits."""
+    import torch
+
+    rng = np.random.default_rng(33)
+    heads, n_kv, d, eps, room = 10, 2, 128, 1e-6, 512
+    had = [300, 15, 63, 0]
+    n = len(had)
+    lens = [h + 8 for h in had]
+    pages = Pages(rng, kind, n_kv, d, 16, lens).fill_random(rng, had)
+    tab = dev(gpu.build_rope_table(d, 1e6, room))
+    qw, kw = dev((1 + 0.3 * rng.normal(0, 1, (2, d))).astype(np.float32))
+    seq = dev([0, 1, 2, -1], np.int32)  # the last row is padding
+    raw = [dev(rng.normal(0, 1, (8, n, h, d)).astype(np.float32)) for h in (heads, n_kv, n_kv)]
+
+    class Side:
+        def __init__(self):
+            self.kv, self.table = pages.device(gpu)
+            self.work = workspace(gpu, heads, n_kv, d)
+            self.pos, self.lens = dev(had, np.int32), dev(had, np.int32)
+            self.q, self.k, self.v = (torch.zeros_like(x[0]) for x in raw)
+            self.out = torch.full_like(self.q, 7.0)
+
+        def step(self):
+            gpu.GpuQkNormRopeKvPaged(self.kv, self.table, seq, self.pos, self.q, self.k, self.v, qw, kw, heads, tab, room,
+                                     n, eps, self.q)
+            self.lens.copy_(self.pos + 1)
+            gpu.GpuAttentionPaged(self.kv, self.table, self.lens, self.q, heads, n, self.out, self.work, seq_ids=seq)
+            self.pos.add_(1)
+
+        def take(self, i):
+            for to, x in zip((self.q, self.k, self.v), raw):
+                to.copy_(x[i])
+
+    eager, replayed = Side(), Side()
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream), gpu.ScopedEngineStream(stream):
+        replayed.step()
+    for i in range(8):
+        eager.take(i)
+        replayed.take(i)
+        with gpu.ScopedEngineStream(torch.cuda.current_stream()):
+            eager.step()
+        graph.replay()
+        want, got = host(eager.out), host(replayed.out)
+        assert np.array_equal(got, want)
+        assert np.all(want[3] == 7)
+        for name, t in zip(("k", "v", "ks", "vs"), eager.kv.tensors):
+            if t is not None:
+                a = host(t)
+                setattr(pages, name, a.view(np.uint16) if a.dtype == np.int16 else a)
+        check(want[:3], pages, [h + i + 1 for h in had[:3]], host(eager.q)[:3])
+        assert pages.same_as(replayed.kv)

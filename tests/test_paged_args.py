@@ -140,6 +140,38 @@ def test_attention_refusals(ops):
                                   workspace_bytes=a["bytes"])
 
 
+def test_calls_too_large_to_count(ops):
+    """Head rows of a write or a read, and units of an attention call, are counted in 32 bits."""
+    far = 1 << 62  # past whatever the counts below make of q
+    kv, t = views(ops, n_seqs=1 << 30)
+    for n in ((1 << 31) // 16, 1 << 40):
+        with pytest.raises(ops.RpgError, match="too many for one call"):
+            ops.GpuKvWritePaged(kv, t, FAKE, FAKE, FAKE, FAKE, n)
+        with pytest.raises(ops.RpgError, match="too many for one call"):
+            ops.GpuQkNormRopeKvPaged(kv, t, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 16, FAKE, 100, n, 1e-6, FAKE)
+        with pytest.raises(ops.RpgError, match="too many for one call"):
+            ops.GpuKvReadPaged(kv, t, FAKE, FAKE, 2 * n, FAKE, far, 1024, 128, out_f32=False)
+    need = ops.GpuAttentionPagedWorkspace(16, 8, 128)
+    # 2^20 rows that may have 2^17 positions each: 2^12 units of 32 for 8 kv heads
+    kv, t = views(ops, max_pages=1 << 13, n_seqs=1 << 20)
+    with pytest.raises(ops.RpgError, match="too many for one call"):
+        ops.GpuAttentionPaged(kv, t, FAKE, FAKE, 16, 1 << 20, far, 1 << 41, seq_ids=FAKE, workspace_bytes=need)
+
+
+def test_other_devices_are_refused(ops):
+    import torch
+
+    kv, t = views(ops)
+    kv.device, kv.device_index, t.device_index = torch.device("cuda", 1), 1, 0
+    for call in calls(ops, kv, t):
+        with pytest.raises(ops.RpgError, match="page table on device 0"):
+            call()
+    t.device_index, kv.current_device = 1, lambda: 0
+    for call in calls(ops, kv, t):
+        with pytest.raises(ops.RpgError, match="not the current device"):
+            call()
+
+
 def test_workspace_sizes(ops):
     for heads, kv, d in ((1, 1, 64), (16, 8, 128), (64, 1, 128)):
         assert ops.GpuAttentionPagedWorkspace(heads, kv, d) > 0
