@@ -27,7 +27,10 @@
 // (relative to a power of two above the scales so far); either enters as four
 // signed digits of 8 bits, in columns n, n + 4, n + 8, n + 12. Weights have 3 bits of
 // headroom: the maximum that they are relative to moves only when a score exceeds
-// it by 3 (log2), and only then are the int32 sums of the output taken to fp32.
+// it by 3 (log2), and only then are the int32 sums of the output taken to fp32. (Of
+// more than four heads, two column tiles, each step's at once: there is no room for
+// both. The vector instructions then bound it: 16 x 4000 positions, 64 / 8 heads,
+// 136 MB in 36.5 us.)
 //
 // Keys and values come straight to LDS in whole 128-byte lines, the next step's as
 // soon as this step has read what they replace; the transposition of values is the
@@ -41,6 +44,20 @@
 // wave writes what it holds whole; where a (row, tile) is split over waves of one
 // workgroup they join in LDS, and where it is split over workgroups each leaves its
 // part in the workspace and the last to arrive joins them, in order.
+//
+// Measured (kernel times; "units" as above): 32 rows of up to 4096 positions in fp16,
+// 16 / 8 heads, 269 MB: 50.7 us, 5.3 TB/s; 128 rows of up to 8192 in 8 bits, 32 / 8
+// heads, 1152 MB: 203 us, 5.7 TB/s (fp16, 2230 MB: 357 us, 6.2 TB/s), where a pure
+// read of as much reaches 7.0. While all workgroups run the reads come at about that
+// rate; the rest is the end, where the workgroup that a compute unit took second is
+// a fifth slower than its first (its loads wait behind), and every other XCD a tenth.
+// Shares to match (42 to 58) took 128 x 8192 to 192 us but 64 x 4096 from 93 to 100,
+// and dealing the last fifth out late, in shares of their own, cost what it gained.
+// One row of 32768 positions in 8 bits, 8 kv heads, 69 MB: 21.7 us, of which about
+// ten read at full rate; 1 x 500 positions 9.3 us and 1 x 60 7.1 us are the chain of
+// round trips: lengths 0.5, the search for the share 0.7, page table 0.2, keys 1.5,
+// products and weights 1.9, join in LDS 0.6 and, where a pair is split, store and
+// count 1.3 and the last one's read and join 1.5.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -56,6 +73,9 @@ namespace {
 
 using dev::PagedView;
 
+// Four waves of up to 17 KB of keys and values each: two workgroups to a compute unit. (Eight waves and one workgroup
+// were slower on short calls, 1 x 500 positions 12.1 against 10.5 us, and alike on long ones; four waves and one
+// workgroup with two steps under way each were slower on long ones.)
 constexpr int kWaves = 4;
 constexpr int kTileHeads = 8;
 // Workgroups at most; a workspace has two part slots and a counter for each.
@@ -150,7 +170,8 @@ __device__ __forceinline__ uint32_t LdsAddress(const void* p) {
   return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const Lds*)(static_cast<const char*>(p))));
 }
 // kN times 16 bytes a lane from rs: time i from byte off[i % kOff] + 1024 i, lane j's to LDS address `to` + 1024 i +
-// 16 j (an instruction's offset counts on both sides). M0 holds the LDS address, which is read one wait state after it is
+// 16 j (an instruction's offset counts on both sides). What is read once is loaded with the streaming hint: without it
+// 32 x 4096 positions took 59 us and not 53, 128 x 8192 236 and not 211. M0 holds the LDS address, which is read one wait state after it is
 // written; five are waited, which a resource needs whose registers a vector instruction wrote.
 template <int kN, int kOff>
 __device__ __forceinline__ void LoadToLds(Resource rs, const uint32_t (&off)[kOff], uint32_t to) {
@@ -219,6 +240,7 @@ __device__ __forceinline__ uint32_t Scalar(uint32_t x) { return __builtin_amdgcn
 // a unit, so that all workgroups get alike. With fewer, joining what two workgroups hold of a pair (a round trip to memory
 // to store, one to count, one to read) costs more than some units more in turn: a pair of up to kWholeUnits is one item, a
 // longer one is cut evenly into items of at most 2^step, about what each workgroup then gets.
+// (kWholeUnits 16 and so one workgroup for 500 positions: 11.6 us against 10.5 for four and their join.)
 constexpr uint32_t kManyUnits = 8192;
 constexpr uint32_t kWholeUnits = 4;
 
