@@ -15,10 +15,11 @@
  * kept as zeros, one that holds an infinity or a NaN as a NaN scale.
  *
  * seq_ids[t] (NULL: t itself) names row t's sequence, positions[t] its position;
- * both are device arrays. A negative seq_id is padding: nothing is read or
- * written for that row. A row that names no slot (a sequence, position or page
- * out of range) stores nothing in the cache, and what the call gives back for it
- * is NaN. Rows of one call that name the same slot leave a mixture there.
+ * both are device arrays, which like lengths and tables must stay as they are
+ * while the call runs. A negative seq_id is padding: no slot is read or written
+ * for that row, and no output. A row that names no slot (a sequence, position or
+ * page out of range) stores nothing in the cache, and what the call gives back
+ * for it is NaN. Rows of one call that name the same slot leave a mixture there.
  *
  * No counterparts in the reference, whose cache holds one sequence
  * (src/kv_cache_gpu.h:1-30); each entry names the operator it stands beside.

@@ -629,15 +629,16 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
     const auto find = [&]() {
       bad = 0;
       const int32_t pos = static_cast<int32_t>(c) * kStep;
+      const int32_t left = len - pos;  // no sum of positions here or below may pass the largest int32
       const int32_t kh = KvHeadOf(pair, tiles);
       int32_t pages[kSub];
 #pragma unroll
       for (int j = 0; j < kSub; ++j) {
-        pages[j] = ScalarLoad(table + ((pos + 16 * j < len ? pos + 16 * j : pos) >> view.page_shift));
+        pages[j] = ScalarLoad(table + ((16 * j < left ? pos + 16 * j : pos) >> view.page_shift));
       }
 #pragma unroll
       for (int j = 0; j < kSub; ++j) {
-        const int32_t p = pos + 16 * j < len ? pos + 16 * j : pos;
+        const int32_t p = 16 * j < left ? pos + 16 * j : pos;
         const bool fine = static_cast<uint32_t>(pages[j]) < static_cast<uint32_t>(view.n_pages);
         const int32_t page = fine ? pages[j] : 0;
         bad |= fine ? 0 : 1 << j;
@@ -803,8 +804,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
         turned = false;
       }
       const int32_t pos = static_cast<int32_t>(c) * kStep;
-      const bool tail = pos + kStep > len;
       const int32_t left = len - pos;  // positions from here
+      const bool tail = left < kStep;
       const int this_bad = bad;
       // ---- scores, once the keys are there: the values' loads are younger
       WaitLoads<kStageLoads>();
@@ -1353,11 +1354,16 @@ void GpuAttentionPaged(const GpuPagedKv& kv, const GpuPageTable& table, const in
             static_cast<long long>(n_rows), static_cast<long long>(table.n_seqs));
   RPG_CHECK(((reinterpret_cast<uintptr_t>(q_dev) | reinterpret_cast<uintptr_t>(out_dev)) & 15) == 0,
             "AttentionPaged: q and out have to be 16-byte aligned");
+  RPG_CHECK(((reinterpret_cast<uintptr_t>(seq_ids) | reinterpret_cast<uintptr_t>(lens)) & 3) == 0,
+            "AttentionPaged: seq_ids and lens have to be 4-byte aligned");
   const int64_t q_bytes = n_rows * n_heads * kv.head_dim * 4;
   RPG_CHECK(!Overlap(q_dev, q_bytes, out_dev, q_bytes), "AttentionPaged: out must not overlap q");
   const size_t need = GpuAttentionPagedWorkspaceBytes(n_heads, kv.n_kv_heads, kv.head_dim);
   RPG_CHECK((reinterpret_cast<uintptr_t>(workspace) & 255) == 0 && workspace_bytes >= need,
             "AttentionPaged: a workspace of %zu bytes, 256-byte aligned, is needed (%zu given)", need, workspace_bytes);
+  RPG_CHECK(!Overlap(out_dev, q_bytes, workspace, static_cast<int64_t>(need)) &&
+                !Overlap(q_dev, q_bytes, workspace, static_cast<int64_t>(need)),
+            "AttentionPaged: the workspace must not overlap q or out");
   int32_t tiles, tile_heads;
   TilesOf(n_heads / kv.n_kv_heads, &tiles, &tile_heads);
   const Rows rows{seq_ids, lens, static_cast<int32_t>(table.n_seqs),

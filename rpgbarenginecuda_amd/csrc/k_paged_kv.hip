@@ -339,6 +339,8 @@ __global__ __launch_bounds__(kBlock) void PagedReadKernel(PagedView view, const 
 void CheckRows(const char* what, const GpuPageTable& table, const int32_t* seq_ids, const int32_t* positions,
                int64_t n_tokens) {
   RPG_CHECK(positions != nullptr, "%s got null positions", what);
+  RPG_CHECK(((reinterpret_cast<uintptr_t>(seq_ids) | reinterpret_cast<uintptr_t>(positions)) & 3) == 0,
+            "%s: seq_ids and positions have to be 4-byte aligned", what);
   RPG_CHECK(seq_ids != nullptr || n_tokens <= table.n_seqs, "%s: %lld tokens without seq_ids, but %lld sequences",
             what, static_cast<long long>(n_tokens), static_cast<long long>(table.n_seqs));
 }
@@ -384,17 +386,22 @@ void GpuQkNormRopeKvPaged(const GpuPagedKv& kv, const GpuPageTable& table, const
   CheckPagedKv("QkNormRopeKvPaged", kv, table);
   RPG_CHECK(n_tokens >= 0, "QkNormRopeKvPaged: %lld tokens", static_cast<long long>(n_tokens));
   RPG_CHECK(n_heads > 0 && n_heads <= (1 << 20), "QkNormRopeKvPaged: n_heads %d out of range", n_heads);
-  RPG_CHECK(rope_rows > 0, "QkNormRopeKvPaged: a RoPE table of %lld rows", static_cast<long long>(rope_rows));
+  RPG_CHECK(rope_rows > 0 && rope_rows <= 0x7FFFFFFF, "QkNormRopeKvPaged: a RoPE table of %lld rows", static_cast<long long>(rope_rows));
   if (n_tokens == 0) return;
   CheckRows("QkNormRopeKvPaged", table, seq_ids, positions, n_tokens);
   RPG_CHECK(q_dev && k_dev && v_dev && q_norm && k_norm && rope_tab && q_out, "QkNormRopeKvPaged got a null pointer");
   RPG_CHECK(Aligned16(q_dev) && Aligned16(k_dev) && Aligned16(v_dev) && Aligned16(q_norm) && Aligned16(k_norm) &&
                 Aligned16(rope_tab) && Aligned16(q_out),
             "QkNormRopeKvPaged: every buffer has to be 16-byte aligned");
-  const int64_t q_bytes = n_tokens * n_heads * kv.head_dim * 4;
+  CheckUnits("QkNormRopeKvPaged", n_tokens, n_heads + 2 * static_cast<int64_t>(kv.n_kv_heads));
+  const int64_t row = kv.head_dim * 4;
+  const int64_t q_bytes = n_tokens * n_heads * row, kv_bytes = n_tokens * kv.n_kv_heads * row;
   RPG_CHECK(q_out == q_dev || !Overlap(q_dev, q_bytes, q_out, q_bytes),
             "QkNormRopeKvPaged: q_out has to be q itself or apart from it");
-  CheckUnits("QkNormRopeKvPaged", n_tokens, n_heads + 2 * static_cast<int64_t>(kv.n_kv_heads));
+  RPG_CHECK(!Overlap(k_dev, kv_bytes, q_out, q_bytes) && !Overlap(v_dev, kv_bytes, q_out, q_bytes) &&
+                !Overlap(q_norm, row, q_out, q_bytes) && !Overlap(k_norm, row, q_out, q_bytes) &&
+                !Overlap(rope_tab, rope_rows * row, q_out, q_bytes),
+            "QkNormRopeKvPaged: q_out must not overlap k, v, the norms or the RoPE table");
   LaunchWrite<true>("PagedQkNormRopeWriteKernel", kv, table, seq_ids, positions, q_dev, k_dev, v_dev, q_norm, k_norm,
                     n_heads, rope_tab, rope_rows, eps, q_out, n_tokens);
 }
@@ -417,6 +424,7 @@ void GpuKvReadPaged(const GpuPagedKv& kv, const GpuPageTable& table, const int32
                 head_stride >= (n_tokens - 1) * token_stride + kv.head_dim,
             "KvReadPaged: rows of strides %lld and %lld overlap", static_cast<long long>(token_stride),
             static_cast<long long>(head_stride));
+  RPG_CHECK(k_out != v_out, "KvReadPaged: k_out and v_out are the same");
   CheckUnits("KvReadPaged", n_tokens, kv.n_kv_heads);
   const int64_t units = n_tokens * kv.n_kv_heads;
   const bool q8 = kv.type == kKvQ8;

@@ -277,8 +277,10 @@ struct GpuPageTable {
 };
 
 // Where each row of a call goes is device data: seq_ids[t] (nullptr: t itself)
-// names the sequence and positions[t] the position. A negative seq_id is
-// padding: nothing is read or written for that row. A row that names no slot
+// names the sequence and positions[t] the position; they, like the lengths and
+// the table, must stay as they are while the call runs. A negative seq_id is
+// padding: no slot is read or written for that row, and no output. A row that
+// names no slot
 // (a sequence, position or page out of range) stores nothing in the cache, and
 // what the call gives back for it is NaN. Two rows that name the same slot in
 // one call leave it holding a mixture of both.
@@ -289,7 +291,7 @@ void GpuKvWritePaged(const GpuPagedKv& kv, const GpuPageTable& table, const int3
 
 // GpuQkNormRopeKv over pages: q_out[t,h,:] <- RoPE(RMSNorm(q[t,h,:]) * q_norm) at
 // the row's position (q_out may be q), RoPE(RMSNorm(k) * k_norm) and v into the
-// cache; k and v are not modified. At head_dim 128 q_out and an F16 cache hold
+// cache; k and v are not modified, nor may q_out overlap them. At head_dim 128 q_out and an F16 cache hold
 // the bits that GpuQkNormRopeKv leaves. A position at or past rope_rows is out of
 // range.
 void GpuQkNormRopeKvPaged(const GpuPagedKv& kv, const GpuPageTable& table, const int32_t* seq_ids,
@@ -312,7 +314,8 @@ void GpuKvReadPaged(const GpuPagedKv& kv, const GpuPageTable& table, const int32
 // head h / (n_heads / n_kv_heads). A row of length 0 gives zeros; padding
 // (negative seq_id) leaves its out row as it was; a length below 0 or past the
 // table's row, a sequence out of range, or a page out of range among the row's
-// positions gives NaN. out must not overlap q. The work is shared out on the
+// positions gives NaN. (An infinite value whose weight is below 2^-23 of the
+// largest may give NaN instead of the infinity.) out must not overlap q. The work is shared out on the
 // device from the lengths themselves, so a captured call holds for any lengths,
 // tables and seq_ids that stand there at replay.
 //

@@ -346,6 +346,34 @@ def test_pages_past_32_bit_offsets(gpu):
     check(attend(gpu, kv, table, [600], q), few, [600], q)
 
 
+@pytest.mark.parametrize("kind", [F16, Q8])
+def test_the_longest_row_there_is(gpu, kind):
+    """2^31 - 1 positions: a table whose entries are all one page, but for the last, whose last slot holds NaN and is the
+    one position that the length leaves out.
+
+    Each of the 256 slots counts 2^23 times, but for 255 of the first page and all but one of the last. A lane adds up
+    16 weights for each of its wave's 2^25 / 2048 units one after the other, in fp32, and outputs likewise: 2^18 roundings
+    of half a step, of the sum of the weights and of the outputs, so 2 * 2^18 * 2^-24 of the largest value, beside which
+    the bound of a short row is nothing."""
+    rng = np.random.default_rng(34)
+    d, page, n = 64, 256, 2 ** 31 - 1
+    pages = Pages(rng, kind, 1, d, page, [2 * page], spare=0).fill_random(rng, [2 * page])
+    main, last = pages.table[0]
+    pages.put(0, 2 * page - 1, np.full((1, d), np.nan, np.float32), np.full((1, d), np.nan, np.float32))
+    kv, _ = pages.device(gpu)
+    table = np.full((1, 2 ** 23), main, np.int32)
+    table[0, -1] = last
+    q = rng.normal(0, 1, (1, 2, d)).astype(np.float32)
+    got = attend(gpu, kv, gpu.GpuPageTable(dev(table)), [n], q)
+    k, v = pages.rows("k", 0, 2 * page - 1)[:, 0], pages.rows("v", 0, 2 * page - 1)[:, 0]
+    times = np.where(np.arange(2 * page - 1) < page, 2.0 ** 23 - 1, 1.0)
+    s = q[0].astype(np.float64) @ k.T / np.sqrt(d)
+    w = np.exp(s - s.max(-1, keepdims=True)) * times
+    want = w @ v / w.sum(-1, keepdims=True)
+    vmax = np.abs(v).max()
+    assert np.all(np.abs(got[0] - want) <= 2.0 ** -5 * vmax + bound(d, 512, np.abs(s).max() * d, vmax))
+
+
 @pytest.mark.parametrize("kind,n_kv,group,page", [(F16, 8, 2, 16), (Q8, 8, 4, 64), (F16, 2, 8, 32)])
 def test_a_batch_is_served(gpu, ora, kind, n_kv, group, page):
     """Two prompts put into pages, one read back into the contiguous cache for its attention there; then steps of one

@@ -158,6 +158,31 @@ def test_calls_too_large_to_count(ops):
         ops.GpuAttentionPaged(kv, t, FAKE, FAKE, 16, 1 << 20, far, 1 << 41, seq_ids=FAKE, workspace_bytes=need)
 
 
+def test_buffers_that_overlap_or_lie_askew_are_refused(ops):
+    kv, t = views(ops)
+    far = 1 << 40
+    for name in ("k", "v", "q_norm", "k_norm", "tab"):
+        a = dict(q=far, k=1 << 41, v=1 << 42, q_norm=1 << 43, k_norm=1 << 44, tab=1 << 45, out=1 << 46)
+        size = 2 * 16 * 128 * 4
+        for out in (a[name], a[name] - size + 16):
+            with pytest.raises(ops.RpgError, match="must not overlap k, v"):
+                ops.GpuQkNormRopeKvPaged(kv, t, FAKE, FAKE, a["q"], a["k"], a["v"], a["q_norm"], a["k_norm"], 16, a["tab"],
+                                         100, 2, 1e-6, out)
+    with pytest.raises(ops.RpgError, match="k_out and v_out are the same"):
+        ops.GpuKvReadPaged(kv, t, FAKE, FAKE, 2, far, far, 1024, 128, out_f32=False)
+    for seq, pos in ((FAKE + 2, FAKE), (FAKE, FAKE + 1), (None, FAKE + 3)):
+        with pytest.raises(ops.RpgError, match="4-byte aligned"):
+            ops.GpuKvWritePaged(kv, t, seq, pos, FAKE, FAKE, 2)
+        with pytest.raises(ops.RpgError, match="4-byte aligned"):
+            ops.GpuKvReadPaged(kv, t, seq, pos, 2, far, 1 << 41, 1024, 128, out_f32=False)
+        with pytest.raises(ops.RpgError, match="4-byte aligned"):
+            ops.GpuAttentionPaged(kv, t, pos, FAKE, 16, 2, far, 1 << 41, seq_ids=seq, workspace_bytes=1 << 30)
+    need = ops.GpuAttentionPagedWorkspace(16, 8, 128)
+    for q, out in ((far, (1 << 41) + need - 16 & ~15), (far, (1 << 41) - 16), ((1 << 41) + 256, far)):
+        with pytest.raises(ops.RpgError, match="workspace must not overlap"):
+            ops.GpuAttentionPaged(kv, t, FAKE, q, 16, 2, out, 1 << 41, seq_ids=FAKE, workspace_bytes=need)
+
+
 def test_other_devices_are_refused(ops):
     import torch
 
