@@ -850,7 +850,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
 #pragma unroll
         for (int j = 0; j < kSub; ++j) ks[j] = scales_at(k_mine, j);
       }
-      // the products of queries' and keys' codes as scores: sums over the digits' columns
+      // The products of queries' and keys' codes as scores: sums over the digits' columns, in an order that gives all lanes
+      // of a head the same bits, since each takes another digit of the weight that comes of it.
       const auto scale_scores = [&]() {
 #pragma unroll
         for (int j = 0; j < kSub; ++j) {
@@ -859,12 +860,15 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
           for (int i = 0; i < 4; ++i) {
             float x[kTiles];
 #pragma unroll
-            for (int t = 0; t < kTiles; ++t) {
-              x[t] = static_cast<float>(raw[t][j][i]) * to_score[t];
-              x[t] += Ror<8>(x[t]);
+            for (int t = 0; t < kTiles; ++t) x[t] = static_cast<float>(raw[t][j][i]) * to_score[t];
+            if constexpr (kTiles == 1) {
+              const float half = x[0] + Ror<8>(x[0]);
+              s[j][i] = (half + Ror<4>(half)) * by[i];
+            } else {
+              const float mine = second ? x[1] : x[0], other = second ? x[0] : x[1];
+              const float half = mine + Ror<4>(other);
+              s[j][i] = (half + Ror<8>(half)) * by[i];
             }
-            const float mine = second ? x[kTiles - 1] : x[0], other = second ? x[0] : x[kTiles - 1];
-            s[j][i] = (mine + Ror<4>(other)) * by[i];
           }
         }
       };
@@ -892,15 +896,21 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
       __builtin_amdgcn_sched_barrier(0);
       // ---- weights
       if constexpr (kQ8 && kTiles == 1) scale_scores();
+      if (__builtin_expect(tail || this_bad != 0, 0)) {
+#pragma unroll
+        for (int j = 0; j < kSub; ++j) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (this_bad & (1 << j)) s[j][i] = NAN;
+            if (16 * j + 4 * g + i >= left) s[j][i] = -INFINITY;
+          }
+        }
+      }
       float top = m;
 #pragma unroll
       for (int j = 0; j < kSub; ++j) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (this_bad & (1 << j)) s[j][i] = NAN;
-          if (tail && 16 * j + 4 * g + i >= left) s[j][i] = -INFINITY;
-          top = fmaxf(top, s[j][i]);
-        }
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, s[j][i]);
       }
       top = MaxAcrossRows(top);
       // the values are there: the next keys' loads, if any, are younger
@@ -960,19 +970,22 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
 #pragma unroll
         for (int j = 0; j < kSub; ++j) {
           const float by[4] = {vs[j].x, vs[j].y, vs[j].z, vs[j].w};
-          uint32_t d[kTiles][4];
+          uint32_t d[kTiles][4];  // this lane's tile's, and the other's
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float p = __builtin_amdgcn_exp2f(s[j][i] - safe);
             l += p;
-            const int x = static_cast<int>(fmaf(p * by[i], up, 0.5f));
-#pragma unroll
-            for (int t = 0; t < kTiles; ++t) {
-              d[t][i] = __float_as_uint(of_tile(t, __int_as_float(x + static_cast<int>(0x80808080u))));
-            }
+            d[0][i] = static_cast<uint32_t>(static_cast<int>(fmaf(p * by[i], up, 0.5f))) + 0x80808080u;
+            if constexpr (kTiles > 1) d[1][i] = __float_as_uint(Ror<4>(__uint_as_float(d[0][i])));
           }
-#pragma unroll
-          for (int t = 0; t < kTiles; ++t) w[t][j] = Digit4(d[t][0], d[t][1], d[t][2], d[t][3], digit);
+          const int mine = Digit4(d[0][0], d[0][1], d[0][2], d[0][3], digit);
+          if constexpr (kTiles == 1) {
+            w[0][j] = mine;
+          } else {
+            const int other = Digit4(d[1][0], d[1][1], d[1][2], d[1][3], digit);
+            w[0][j] = second ? other : mine;
+            w[1][j] = second ? mine : other;
+          }
         }
         I32x2 a[kE][2];
 #pragma unroll
