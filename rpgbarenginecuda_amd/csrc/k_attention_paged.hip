@@ -679,6 +679,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
       if constexpr (kQ8) LoadWordToLds(scale_of(view.v_scale), v_to + kStep * kRow);
     };
 
+    // of a compute unit's two workgroups the second waits behind the first wherever both have something to issue: going
+    // first there, it ends sooner (128 x 8192 positions in 8 bits 200.4 -> 195.4 us; other calls within a percent)
+    if (me >= gridDim.x / 2) __builtin_amdgcn_s_setprio(1);
     find();
     load_k();
     load_v();
