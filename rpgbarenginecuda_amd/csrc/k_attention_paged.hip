@@ -29,8 +29,8 @@
 // headroom: the maximum that they are relative to moves only when a score exceeds
 // it by 3 (log2), and only then are the int32 sums of the output taken to fp32. (Of
 // more than four heads, two column tiles, each step's at once: there is no room for
-// both. The vector instructions then bound it: 16 x 4000 positions, 64 / 8 heads,
-// 136 MB in 36.5 us.)
+// both. 16 x 4000 positions, 64 / 8 heads, 136 MB: 35.4 us.) Of the four lanes that
+// have a score's digits each does a part of the softmax.
 //
 // Keys and values come straight to LDS in whole 128-byte lines, the next step's as
 // soon as this step has read what they replace; the transposition of values is the
@@ -47,13 +47,14 @@
 //
 // Measured (kernel times; "units" as above): 32 rows of up to 4096 positions in fp16,
 // 16 / 8 heads, 269 MB: 50.7 us, 5.3 TB/s; 128 rows of up to 8192 in 8 bits, 32 / 8
-// heads, 1152 MB: 203 us, 5.7 TB/s (fp16, 2230 MB: 357 us, 6.2 TB/s), where a pure
+// heads, 1152 MB: 192 us, 6.0 TB/s (fp16, 2230 MB: 357 us, 6.2 TB/s), where a pure
 // read of as much reaches 7.0. While all workgroups run the reads come at about that
-// rate; the rest is the end, where the workgroup that a compute unit took second is
-// a fifth slower than its first (its loads wait behind), and every other XCD a tenth.
-// Shares to match (42 to 58) took 128 x 8192 to 192 us but 64 x 4096 from 93 to 100,
-// and dealing the last fifth out late, in shares of their own, cost what it gained.
-// One row of 32768 positions in 8 bits, 8 kv heads, 69 MB: 21.7 us, of which about
+// rate; the rest is the end, where every other XCD is a tenth slower and of a compute
+// unit's two workgroups the one whose loads come behind a fifth. Shares to match gained
+// a few percent on ragged batches and lost as much where equal shares split no row
+// (64 x 4096 positions from 93 to 100 us), and dealing the last fifth out late, in
+// shares of their own, cost what it gained.
+// One row of 32768 positions in 8 bits, 8 kv heads, 69 MB: 21.1 us, of which about
 // ten read at full rate; 1 x 500 positions 9.3 us and 1 x 60 7.1 us are the chain of
 // round trips: lengths 0.5, the search for the share 0.7, page table 0.2, keys 1.5,
 // products and weights 1.9, join in LDS 0.6 and, where a pair is split, store and
@@ -102,7 +103,7 @@ __host__ __device__ constexpr uint32_t SlotBytes(int32_t d, int32_t heads) {
 
 // ---------------------------------------------------------------- lane exchange
 
-// x of the lane kBy further on in its row of 16.
+// x of the lane kBy before it in its row of 16, which goes round.
 template <int kBy>
 __device__ __forceinline__ float Ror(float x) {
   return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x120 + kBy, 0xF, 0xF, false));
@@ -686,8 +687,15 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
     load_k();
     load_v();
 
-    // Where there are two column tiles, the lanes of odd copies of a column do the second tile's softmax and those of even
-    // copies the first's: of the four lanes that have a score two would only do it again. x of tile t in every lane:
+    // 8-bit caches: of the four lanes that have the copies of a column, each takes a part of the softmax and not all the
+    // whole of it. Where there are two column tiles, odd copies take the second, even ones the first, and of the step's
+    // tiles of 16 keys copies 2 and 3 the upper half; with one column tile odd copies take the upper half.
+    constexpr int kMine = kQ8 ? kSub / 2 : kSub;  // tiles of 16 keys for a lane
+    const bool upper = kQ8 && (kTiles > 1 ? copy >= 2 : (copy & 1) != 0);
+    const int mine_at = upper ? kMine : 0;
+    // the lane of the same column tile that has the other half
+    const auto other_half = [](float x) { return kTiles > 1 ? Ror<8>(x) : Ror<4>(x); };
+    // x of column tile t in every lane
     const bool second = kTiles > 1 && (copy & 1) != 0;
     const auto of_tile = [&](int t, float x) {
       if constexpr (kTiles == 1) return x;
@@ -812,7 +820,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
       const int this_bad = bad;
       // ---- scores, once the keys are there: the values' loads are younger
       WaitLoads<kStageLoads>();
-      float s[kSub][4];
+      float s[kMine][4];
       I32x4 raw[kQ8 ? kTiles : 1][kSub];
       if constexpr (kQ8) {
 #pragma unroll
@@ -848,30 +856,38 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
       const uint32_t piece_units = units;
       const int32_t piece_row = row, piece_pair = pair;
       bool turn = !more;  // this unit is its piece's last
-      float4 ks[kQ8 ? kSub : 1], vs[kQ8 ? kSub : 1];
+      float4 ks[kMine], vs[kMine];
       if constexpr (kQ8) {
 #pragma unroll
-        for (int j = 0; j < kSub; ++j) ks[j] = scales_at(k_mine, j);
+        for (int j = 0; j < kMine; ++j) ks[j] = scales_at(k_mine, mine_at + j);
       }
-      // The products of queries' and keys' codes as scores: sums over the digits' columns, in an order that gives all lanes
-      // of a head the same bits, since each takes another digit of the weight that comes of it.
+      // The products of queries' and keys' codes as scores: sums over the digits' columns, each of the half of the keys and
+      // the tile that are the lane's. With one column tile two lanes have the same score: the sums' order gives them the
+      // same bits, since each takes another digit of the weight that comes of it.
       const auto scale_scores = [&]() {
+        float x[kSub][4];
 #pragma unroll
         for (int j = 0; j < kSub; ++j) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float first = static_cast<float>(raw[0][j][i]) * to_score[0];
+            if constexpr (kTiles == 1) {
+              x[j][i] = first + Ror<8>(first);
+            } else {
+              const float last = static_cast<float>(raw[kTiles - 1][j][i]) * to_score[kTiles - 1];
+              const float send = second ? first : last;
+              x[j][i] = (second ? last : first) + Ror<4>(send);
+            }
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < kMine; ++j) {
           const float by[4] = {ks[j].x, ks[j].y, ks[j].z, ks[j].w};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            float x[kTiles];
-#pragma unroll
-            for (int t = 0; t < kTiles; ++t) x[t] = static_cast<float>(raw[t][j][i]) * to_score[t];
-            if constexpr (kTiles == 1) {
-              const float half = x[0] + Ror<8>(x[0]);
-              s[j][i] = (half + Ror<4>(half)) * by[i];
-            } else {
-              const float mine = second ? x[1] : x[0], other = second ? x[0] : x[1];
-              const float half = mine + Ror<4>(other);
-              s[j][i] = (half + Ror<8>(half)) * by[i];
-            }
+            const float lo = x[j][i], hi = x[kSub - kMine + j][i];
+            const float send = upper ? lo : hi;
+            s[j][i] = ((upper ? hi : lo) + other_half(send)) * by[i];
           }
         }
       };
@@ -901,20 +917,21 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
       if constexpr (kQ8 && kTiles == 1) scale_scores();
       if (__builtin_expect(tail || this_bad != 0, 0)) {
 #pragma unroll
-        for (int j = 0; j < kSub; ++j) {
+        for (int j = 0; j < kMine; ++j) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            if (this_bad & (1 << j)) s[j][i] = NAN;
-            if (16 * j + 4 * g + i >= left) s[j][i] = -INFINITY;
+            if (this_bad >> (mine_at + j) & 1) s[j][i] = NAN;
+            if (16 * (mine_at + j) + 4 * g + i >= left) s[j][i] = -INFINITY;
           }
         }
       }
       float top = m;
 #pragma unroll
-      for (int j = 0; j < kSub; ++j) {
+      for (int j = 0; j < kMine; ++j) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) top = fmaxf(top, s[j][i]);
       }
+      if constexpr (kQ8) top = fmaxf(top, other_half(top));
       top = MaxAcrossRows(top);
       // the values are there: the next keys' loads, if any, are younger
       if (more) {
@@ -925,11 +942,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
       // ---- the output's sums
       if constexpr (kQ8) {
 #pragma unroll
-        for (int j = 0; j < kSub; ++j) vs[j] = scales_at(v_mine, j);
+        for (int j = 0; j < kMine; ++j) vs[j] = scales_at(v_mine, mine_at + j);
         if (tail) {
 #pragma unroll
-          for (int j = 0; j < kSub; ++j) {
-            const int32_t p = 16 * j + 4 * g;
+          for (int j = 0; j < kMine; ++j) {
+            const int32_t p = 16 * (mine_at + j) + 4 * g;
             vs[j].x = p < left ? vs[j].x : 0.0f;
             vs[j].y = p + 1 < left ? vs[j].y : 0.0f;
             vs[j].z = p + 2 < left ? vs[j].z : 0.0f;
@@ -939,10 +956,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
         // the largest, as whole numbers, where a NaN is larger than any number
         uint32_t big = 0;
 #pragma unroll
-        for (int j = 0; j < kSub; ++j) {
+        for (int j = 0; j < kMine; ++j) {
           big = max(max(big, max(__float_as_uint(vs[j].x), __float_as_uint(vs[j].y))),
                     max(__float_as_uint(vs[j].z), __float_as_uint(vs[j].w)));
         }
+        big = max(big, __float_as_uint(other_half(__uint_as_float(big))));
         big = __float_as_uint(AcrossRows(__uint_as_float(big), [](float a, float b) {
           return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b)));
         }));
@@ -971,23 +989,35 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
         const float safe = m == -INFINITY ? 0.0f : m;
         I32x4 w[kTiles];  // tile j of 16 keys: bytes 4 j ..
 #pragma unroll
-        for (int j = 0; j < kSub; ++j) {
+        for (int j = 0; j < kMine; ++j) {
           const float by[4] = {vs[j].x, vs[j].y, vs[j].z, vs[j].w};
-          uint32_t d[kTiles][4];  // this lane's tile's, and the other's
+          float d[4];  // whole numbers, and so below
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float p = __builtin_amdgcn_exp2f(s[j][i] - safe);
             l += p;
-            d[0][i] = static_cast<uint32_t>(static_cast<int>(fmaf(p * by[i], up, 0.5f))) + 0x80808080u;
-            if constexpr (kTiles > 1) d[1][i] = __float_as_uint(Ror<4>(__uint_as_float(d[0][i])));
+            d[i] = __uint_as_float(static_cast<uint32_t>(static_cast<int>(fmaf(p * by[i], up, 0.5f))) + 0x80808080u);
           }
-          const int mine = Digit4(d[0][0], d[0][1], d[0][2], d[0][3], digit);
+          // this lane's digit of its own four weights, and of those of the lanes that have the others
+          const auto digits = [&](auto of) {
+            return Digit4(__float_as_uint(of(d[0])), __float_as_uint(of(d[1])), __float_as_uint(of(d[2])),
+                          __float_as_uint(of(d[3])), digit);
+          };
+          const int own = digits([](float x) { return x; });
+          const int half = digits(other_half);
+          const int lo = upper ? half : own, hi = upper ? own : half;
           if constexpr (kTiles == 1) {
-            w[0][j] = mine;
+            w[0][j] = lo;
+            w[0][kSub - kMine + j] = hi;
           } else {
-            const int other = Digit4(d[1][0], d[1][1], d[1][2], d[1][3], digit);
-            w[0][j] = second ? other : mine;
-            w[1][j] = second ? mine : other;
+            // of the other tile: the next copy has its lower half for copies 0 and 3, the one before for 1 and 2
+            const int next = digits([](float x) { return Ror<12>(x); });
+            const int last = digits([](float x) { return Ror<4>(x); });
+            const int lo2 = second != upper ? last : next, hi2 = second != upper ? next : last;
+            w[0][j] = second ? lo2 : lo;
+            w[0][kSub - kMine + j] = second ? hi2 : hi;
+            w[1][j] = second ? lo : lo2;
+            w[1][kSub - kMine + j] = second ? hi : hi2;
           }
         }
         I32x2 a[kE][2];
@@ -1070,6 +1100,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(PagedView
         if (lane == 0) pieces[wave][which] = Piece{u - c_end, c_first, c_end, piece_units, piece_row, piece_pair};
         my_held |= 1 << which;
       }
+      if constexpr (kQ8) l += other_half(l);
       l = SumAcrossRows(l);
 #pragma unroll
       for (int t = 0; t < kTiles; ++t) {
