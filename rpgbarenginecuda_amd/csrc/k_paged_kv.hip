@@ -196,12 +196,40 @@ struct RowOf {
 // 16 bytes a lane. Measured at 2811 tokens of 16 + 8 + 8 heads into 8 bits, 75 MB:
 // 14.0 us = 5.4 TB/s; with nontemporal loads 17.0, with plain stores of the queries
 // 14.5, with write-through ones 15.8; held to 64 registers (spills) twice as long.
+// One argument: a launch takes longer for every pointer among its arguments (nine of them, 0.5 us of host time).
+struct WriteArgs {
+  PagedView view;
+  const int32_t* seq_ids;
+  const int32_t* positions;
+  const float* q;
+  const float* k;
+  const float* v;
+  const float* q_norm;
+  const float* k_norm;
+  const float* tab;
+  float* q_out;
+  int64_t rope_rows;
+  int32_t n_heads;
+  float eps;
+  uint32_t n_units;
+};
+
 template <int D, bool kQ8, bool kNorm>
-__global__ __launch_bounds__(kBlock) void PagedWriteKernel(
-    PagedView view, const int32_t* __restrict__ seq_ids, const int32_t* __restrict__ positions, const float* q,
-    const float* __restrict__ k, const float* __restrict__ v, const float* __restrict__ qw,
-    const float* __restrict__ kw, int32_t n_heads, const float* __restrict__ tab, int64_t rope_rows, float eps,
-    float* q_out, uint32_t n_units) {
+__global__ __launch_bounds__(kBlock) void PagedWriteKernel(const WriteArgs args) {
+  const PagedView view = args.view;
+  const int32_t* __restrict__ seq_ids = args.seq_ids;
+  const int32_t* __restrict__ positions = args.positions;
+  const float* q = args.q;
+  const float* __restrict__ k = args.k;
+  const float* __restrict__ v = args.v;
+  const float* __restrict__ qw = args.q_norm;
+  const float* __restrict__ kw = args.k_norm;
+  const float* __restrict__ tab = args.tab;
+  float* q_out = args.q_out;
+  const int64_t rope_rows = args.rope_rows;
+  const int32_t n_heads = args.n_heads;
+  const float eps = args.eps;
+  const uint32_t n_units = args.n_units;
   // the arguments in one batch of scalar loads at entry (the empty asm takes them as scalar inputs), not each before its
   // first use
   asm volatile("" ::"s"(seq_ids), "s"(positions), "s"(q), "s"(k), "s"(v), "s"(qw), "s"(kw), "s"(n_heads), "s"(tab),
@@ -304,11 +332,26 @@ __device__ __forceinline__ void StoreRead(void* out, int64_t at, const float (&x
 // One work unit per (token, kv head): a lane moves 16 bytes of output of its key and
 // of its value row. Plain loads and nontemporal stores: 10.5 us for 6 x 700 tokens of
 // 8 fp16 heads (52 MB, 4.9 TB/s); with nontemporal loads 12.0, with plain stores 11.4.
+struct ReadArgs {
+  PagedView view;
+  const int32_t* seq_ids;
+  const int32_t* positions;
+  void* k_out;
+  void* v_out;
+  int64_t token_stride;
+  int64_t head_stride;
+  uint32_t n_units;
+};
+
 template <int D, bool kQ8, bool kF32>
-__global__ __launch_bounds__(kBlock) void PagedReadKernel(PagedView view, const int32_t* __restrict__ seq_ids,
-                                                          const int32_t* __restrict__ positions, void* k_out,
-                                                          void* v_out, int64_t token_stride, int64_t head_stride,
-                                                          uint32_t n_units) {
+__global__ __launch_bounds__(kBlock) void PagedReadKernel(const ReadArgs args) {
+  const PagedView view = args.view;
+  const int32_t* __restrict__ seq_ids = args.seq_ids;
+  const int32_t* __restrict__ positions = args.positions;
+  void* k_out = args.k_out;
+  void* v_out = args.v_out;
+  const int64_t token_stride = args.token_stride, head_stride = args.head_stride;
+  const uint32_t n_units = args.n_units;
   asm volatile("" ::"s"(seq_ids), "s"(positions), "s"(k_out), "s"(v_out), "s"(token_stride), "s"(head_stride),
                "s"(n_units), "s"(view.pages), "s"(view.n_seqs), "s"(view.max_pages), "s"(view.n_pages), "s"(view.n_kv),
                "s"(view.page_shift), "s"(view.k), "s"(view.v), "s"(view.k_scale), "s"(view.v_scale));
@@ -346,16 +389,13 @@ void CheckRows(const char* what, const GpuPageTable& table, const int32_t* seq_i
 }
 
 template <bool kNorm>
-void LaunchWrite(const char* name, const GpuPagedKv& kv, const GpuPageTable& table, const int32_t* seq_ids,
-                 const int32_t* positions, const float* q, const float* k, const float* v, const float* qw,
-                 const float* kw, int32_t n_heads, const float* tab, int64_t rope_rows, float eps, float* q_out,
-                 int64_t n_tokens) {
-  const int64_t units = n_tokens * ((kNorm ? n_heads : 0) + 2 * static_cast<int64_t>(kv.n_kv_heads));
+void LaunchWrite(const char* name, const GpuPagedKv& kv, WriteArgs args, int64_t n_tokens) {
+  const int64_t units = n_tokens * ((kNorm ? args.n_heads : 0) + 2 * static_cast<int64_t>(kv.n_kv_heads));
+  args.n_units = static_cast<uint32_t>(units);
   const bool q8 = kv.type == kKvQ8;
   auto* kern = kv.head_dim == 128 ? (q8 ? PagedWriteKernel<128, true, kNorm> : PagedWriteKernel<128, false, kNorm>)
                                   : (q8 ? PagedWriteKernel<64, true, kNorm> : PagedWriteKernel<64, false, kNorm>);
-  Launch(name, kern, dim3(GridFor(units, kBlock / (kv.head_dim / 16))), dim3(kBlock), dev::ViewOf(kv, table), seq_ids,
-         positions, q, k, v, qw, kw, n_heads, tab, rope_rows, eps, q_out, static_cast<uint32_t>(units));
+  Launch(name, kern, dim3(GridFor(units, kBlock / (kv.head_dim / 16))), dim3(kBlock), args);
 }
 
 // Head rows of a call are counted in 32 bits.
@@ -375,8 +415,10 @@ void GpuKvWritePaged(const GpuPagedKv& kv, const GpuPageTable& table, const int3
   RPG_CHECK(k_dev != nullptr && v_dev != nullptr, "KvWritePaged got a null pointer");
   RPG_CHECK(Aligned16(k_dev) && Aligned16(v_dev), "KvWritePaged: k and v have to be 16-byte aligned");
   CheckUnits("KvWritePaged", n_tokens, 2 * static_cast<int64_t>(kv.n_kv_heads));
-  LaunchWrite<false>("PagedWriteKernel", kv, table, seq_ids, positions, nullptr, k_dev, v_dev, nullptr, nullptr, 0,
-                     nullptr, 0, 0.0f, nullptr, n_tokens);
+  LaunchWrite<false>("PagedWriteKernel", kv,
+                     WriteArgs{dev::ViewOf(kv, table), seq_ids, positions, nullptr, k_dev, v_dev, nullptr, nullptr, nullptr,
+                               nullptr, 0, 0, 0.0f, 0},
+                     n_tokens);
 }
 
 void GpuQkNormRopeKvPaged(const GpuPagedKv& kv, const GpuPageTable& table, const int32_t* seq_ids,
@@ -402,8 +444,10 @@ void GpuQkNormRopeKvPaged(const GpuPagedKv& kv, const GpuPageTable& table, const
                 !Overlap(q_norm, row, q_out, q_bytes) && !Overlap(k_norm, row, q_out, q_bytes) &&
                 !Overlap(rope_tab, rope_rows * row, q_out, q_bytes),
             "QkNormRopeKvPaged: q_out must not overlap k, v, the norms or the RoPE table");
-  LaunchWrite<true>("PagedQkNormRopeWriteKernel", kv, table, seq_ids, positions, q_dev, k_dev, v_dev, q_norm, k_norm,
-                    n_heads, rope_tab, rope_rows, eps, q_out, n_tokens);
+  LaunchWrite<true>("PagedQkNormRopeWriteKernel", kv,
+                    WriteArgs{dev::ViewOf(kv, table), seq_ids, positions, q_dev, k_dev, v_dev, q_norm, k_norm, rope_tab,
+                              q_out, rope_rows, n_heads, eps, 0},
+                    n_tokens);
 }
 
 void GpuKvReadPaged(const GpuPagedKv& kv, const GpuPageTable& table, const int32_t* seq_ids,
@@ -434,8 +478,8 @@ void GpuKvReadPaged(const GpuPagedKv& kv, const GpuPageTable& table, const int32
                    : (q8 ? (out_f32 ? PagedReadKernel<64, true, true> : PagedReadKernel<64, true, false>)
                          : (out_f32 ? PagedReadKernel<64, false, true> : PagedReadKernel<64, false, false>));
   Launch("PagedReadKernel", kern, dim3(GridFor(units, kBlock / (kv.head_dim / (out_f32 ? 4 : 8)))), dim3(kBlock),
-         dev::ViewOf(kv, table), seq_ids, positions, k_out, v_out, token_stride, head_stride,
-         static_cast<uint32_t>(units));
+         ReadArgs{dev::ViewOf(kv, table), seq_ids, positions, k_out, v_out, token_stride, head_stride,
+                  static_cast<uint32_t>(units)});
 }
 
 }  // namespace rpg

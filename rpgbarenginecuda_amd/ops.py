@@ -927,9 +927,17 @@ class GpuPagedKv:
             raise RpgError("GpuPagedKv: pages and scales are on different devices")
         self.ref = ctypes.byref(self.c)
         self.row_elems = self.n_kv_heads * self.head_dim
-        self.tensor_type = torch.Tensor
         self.device_index = None if self.device is None else self.device.index
-        self.current_device = torch.cuda.current_device
+        self.current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+        self.float_at = _paged_addr(self, torch.float32)
+        self.int_at = _paged_addr(self, torch.int32)
+        self._at = {torch.float32: self.float_at, torch.int32: self.int_at}
+
+    def at(self, dtype):
+        """_paged_addr's function for these pages and dtype."""
+        if dtype not in self._at:
+            self._at[dtype] = _paged_addr(self, dtype)
+        return self._at[dtype]
 
 
 class GpuPageTable:
@@ -950,15 +958,22 @@ class GpuPageTable:
         self.device_index = None if isinstance(pages, int) else pages.get_device()
 
 
-def _paged_addr(kv: GpuPagedKv, buf, nbytes: int, dtype, name: str):
-    """_addr for a buffer that has to be where the pages are. The calls over pages are short enough for the checks of
-    their many tensors to count, so one that is in order passes through as few of them as there are."""
-    if (type(buf) is kv.tensor_type and buf.dtype is dtype and buf.get_device() == kv.device_index
-            and buf.nbytes >= nbytes and buf.is_contiguous()):
-        return buf.data_ptr()
-    at = _addr(buf, nbytes, dtype, name)
-    if kv.device is not None and isinstance(buf, _t().Tensor) and buf.device != kv.device:
-        raise RpgError(f"{name}: a tensor on {buf.device} beside a paged cache on {kv.device}")
+def _paged_addr(kv: GpuPagedKv, dtype):
+    """The function (buffer, bytes, name) -> address for buffers of dtype that have to be where the pages are: _addr, and
+    the device. The calls over pages are short enough for the checks of their many tensors to count, so that a tensor
+    that is in order passes through as few of them as there are."""
+    torch = _t()
+    tensor, index = torch.Tensor, kv.device_index
+
+    def at(buf, nbytes: int, name: str):
+        if (type(buf) is tensor and buf.dtype is dtype and buf.get_device() == index and buf.nbytes >= nbytes
+                and buf.is_contiguous()):
+            return buf.data_ptr()
+        addr = _addr(buf, nbytes, dtype, name)
+        if kv.device is not None and isinstance(buf, tensor) and buf.device != kv.device:
+            raise RpgError(f"{name}: a tensor on {buf.device} beside a paged cache on {kv.device}")
+        return addr
+
     return at
 
 
@@ -975,30 +990,25 @@ def _paged_call(kv: GpuPagedKv, table: GpuPageTable) -> PagedOpsC:
 def GpuKvWritePaged(kv: GpuPagedKv, table: GpuPageTable, seq_ids, positions, k, v, n_tokens: int) -> None:
     """Rows of k and v [n_tokens, n_kv_heads, head_dim] into the pages, quantised there if these hold 8 bits. seq_ids
     and positions are int32 tensors [n_tokens] (seq_ids None: row t is of sequence t; negative: padding)."""
-    torch = _t()
-    f32, i32 = torch.float32, torch.int32
+    int_at, float_at = kv.int_at, kv.float_at
     row = 4 * n_tokens * kv.row_elems
     _check(_paged_call(kv, table).kv_write(
-        kv.ref, table.ref, _paged_addr(kv, seq_ids, 4 * n_tokens, i32, "seq_ids"),
-        _paged_addr(kv, positions, 4 * n_tokens, i32, "positions"), _paged_addr(kv, k, row, f32, "k"),
-        _paged_addr(kv, v, row, f32, "v"), n_tokens))
+        kv.ref, table.ref, int_at(seq_ids, 4 * n_tokens, "seq_ids"), int_at(positions, 4 * n_tokens, "positions"),
+        float_at(k, row, "k"), float_at(v, row, "v"), n_tokens))
 
 
 def GpuQkNormRopeKvPaged(kv: GpuPagedKv, table: GpuPageTable, seq_ids, positions, q, k, v, q_norm, k_norm,
                          n_heads: int, rope_tab, rope_rows: int, n_tokens: int, eps: float, q_out) -> None:
     """q_out <- RoPE(RMSNorm(q) * q_norm) at each row's position, RoPE(RMSNorm(k) * k_norm) and v into the pages.
     q_out may be q; k and v are not modified."""
-    torch = _t()
-    f32, i32 = torch.float32, torch.int32
+    int_at, float_at = kv.int_at, kv.float_at
     d = kv.head_dim
     qb, kb = 4 * n_tokens * n_heads * d, 4 * n_tokens * kv.row_elems
     _check(_paged_call(kv, table).qk_norm_rope_kv(
-        kv.ref, table.ref, _paged_addr(kv, seq_ids, 4 * n_tokens, i32, "seq_ids"),
-        _paged_addr(kv, positions, 4 * n_tokens, i32, "positions"), _paged_addr(kv, q, qb, f32, "q"),
-        _paged_addr(kv, k, kb, f32, "k"), _paged_addr(kv, v, kb, f32, "v"), _paged_addr(kv, q_norm, 4 * d, f32, "q_norm"),
-        _paged_addr(kv, k_norm, 4 * d, f32, "k_norm"), n_heads,
-        _paged_addr(kv, rope_tab, 4 * rope_rows * d, f32, "rope_tab"), rope_rows, n_tokens, eps,
-        _paged_addr(kv, q_out, qb, f32, "q_out")))
+        kv.ref, table.ref, int_at(seq_ids, 4 * n_tokens, "seq_ids"), int_at(positions, 4 * n_tokens, "positions"),
+        float_at(q, qb, "q"), float_at(k, kb, "k"), float_at(v, kb, "v"), float_at(q_norm, 4 * d, "q_norm"),
+        float_at(k_norm, 4 * d, "k_norm"), n_heads, float_at(rope_tab, 4 * rope_rows * d, "rope_tab"), rope_rows,
+        n_tokens, eps, float_at(q_out, qb, "q_out")))
 
 
 def GpuKvReadPaged(kv: GpuPagedKv, table: GpuPageTable, seq_ids, positions, n_tokens: int, k_out, v_out,
@@ -1007,7 +1017,7 @@ def GpuKvReadPaged(kv: GpuPagedKv, table: GpuPageTable, seq_ids, positions, n_to
     k_out and v_out are float32 or 16-bit (float16, int16, uint16) tensors of one type; raw addresses need out_f32.
     Strides (head_dim, max_seq * head_dim) fill a layer of the contiguous cache."""
     torch = _t()
-    i32 = torch.int32
+    int_at = kv.int_at
     dtype = getattr(k_out, "dtype", None)
     if out_f32 is None:
         if dtype is None:
@@ -1017,10 +1027,10 @@ def GpuKvReadPaged(kv: GpuPagedKv, table: GpuPageTable, seq_ids, positions, n_to
         raise RpgError(f"GpuKvReadPaged: k_out is {dtype}")
     last = (n_tokens - 1) * token_stride + (kv.n_kv_heads - 1) * head_stride + kv.head_dim
     nbytes = (4 if out_f32 else 2) * last if n_tokens > 0 else 0
+    out_at = kv.at(dtype)
     _check(_paged_call(kv, table).kv_read(
-        kv.ref, table.ref, _paged_addr(kv, seq_ids, 4 * n_tokens, i32, "seq_ids"),
-        _paged_addr(kv, positions, 4 * n_tokens, i32, "positions"), n_tokens, 1 if out_f32 else 0,
-        _paged_addr(kv, k_out, nbytes, dtype, "k_out"), _paged_addr(kv, v_out, nbytes, dtype, "v_out"), token_stride,
+        kv.ref, table.ref, int_at(seq_ids, 4 * n_tokens, "seq_ids"), int_at(positions, 4 * n_tokens, "positions"),
+        n_tokens, 1 if out_f32 else 0, out_at(k_out, nbytes, "k_out"), out_at(v_out, nbytes, "v_out"), token_stride,
         head_stride))
 
 
@@ -1039,8 +1049,7 @@ def GpuAttentionPaged(kv: GpuPagedKv, table: GpuPageTable, lens, q, n_heads: int
     """One new token per row: row r of q [n_rows, n_heads, head_dim] attends to positions [0, lens[r]) of its
     sequence, lens an int32 tensor [n_rows]. The workspace is zero before its first call, and belongs to one call at a
     time (workspace_bytes goes with a raw address)."""
-    torch = _t()
-    f32, i32 = torch.float32, torch.int32
+    int_at, float_at = kv.int_at, kv.float_at
     span = 4 * n_rows * n_heads * kv.head_dim
     dtype = getattr(workspace, "dtype", None)
     if workspace_bytes is None:
@@ -1048,10 +1057,9 @@ def GpuAttentionPaged(kv: GpuPagedKv, table: GpuPageTable, lens, q, n_heads: int
             raise RpgError("GpuAttentionPaged: a raw workspace needs workspace_bytes")
         workspace_bytes = workspace.nbytes
     _check(_paged_call(kv, table).attention(
-        kv.ref, table.ref, _paged_addr(kv, seq_ids, 4 * n_rows, i32, "seq_ids"),
-        _paged_addr(kv, lens, 4 * n_rows, i32, "lens"), _paged_addr(kv, q, span, f32, "q"), n_heads, n_rows,
-        _paged_addr(kv, out, span, f32, "out"), _paged_addr(kv, workspace, workspace_bytes, dtype, "workspace"),
-        workspace_bytes))
+        kv.ref, table.ref, int_at(seq_ids, 4 * n_rows, "seq_ids"), int_at(lens, 4 * n_rows, "lens"),
+        float_at(q, span, "q"), n_heads, n_rows, float_at(out, span, "out"),
+        kv.at(dtype)(workspace, workspace_bytes, "workspace"), workspace_bytes))
 
 
 # ----------------------------------------------------------------------------- measurement
