@@ -335,7 +335,7 @@ struct Batch {
 
   __device__ __forceinline__ Batch(const Rows& r, int l) : rows(r), lane(l) {
     each = (rows.n_rows + 63) / 64;
-    if (each == 1 && lane < rows.n_rows) {
+    if (__builtin_expect(each == 1, 1) && lane < rows.n_rows) {
       own_len = rows.lens[lane];
       own_seq = rows.Seq(lane);
       own_units = rows.UnitsOf(own_seq, own_len);
@@ -350,7 +350,7 @@ struct Batch {
   // Of rows [lo, hi), taken `some` to a lane: the units, or items, before this lane's.
   __device__ __forceinline__ uint32_t Before(int32_t lo, int32_t hi, int32_t some, bool of_items, uint32_t* total) const {
     uint32_t own = 0;
-    if (each == 1) {
+    if (__builtin_expect(each == 1, 1)) {
       own = of_items ? cut.Items(own_units) : own_units;
     } else {
       const int64_t first = lo + static_cast<int64_t>(lane) * some;
@@ -370,13 +370,13 @@ struct Batch {
 
   // Of one row, the same in every lane
   __device__ __forceinline__ uint32_t UnitsOf(int32_t r) const {
-    return each == 1 ? __builtin_amdgcn_readlane(own_units, r) : rows.ScalarUnitsOf(r);
+    return __builtin_expect(each == 1, 1) ? __builtin_amdgcn_readlane(own_units, r) : rows.ScalarUnitsOf(r);
   }
   __device__ __forceinline__ int32_t LenOf(int32_t r) const {
-    return each == 1 ? __builtin_amdgcn_readlane(own_len, r) : ScalarLoad(rows.lens + r);
+    return __builtin_expect(each == 1, 1) ? __builtin_amdgcn_readlane(own_len, r) : ScalarLoad(rows.lens + r);
   }
   __device__ __forceinline__ int64_t SeqOf(int32_t r) const {
-    return each == 1 ? __builtin_amdgcn_readlane(own_seq, r) : rows.ScalarSeq(r);
+    return __builtin_expect(each == 1, 1) ? __builtin_amdgcn_readlane(own_seq, r) : rows.ScalarSeq(r);
   }
 
   // Where item x (unit x, unless by_items) begins: its place, its number among the units, and in *past that of the first
@@ -392,7 +392,7 @@ struct Batch {
       x -= __builtin_amdgcn_readlane(b, at);
       before += __builtin_amdgcn_readlane(ub, at);
       lo += at * some;
-      if (some == 1) break;
+      if (__builtin_expect(some == 1, 1)) break;
       hi = min(lo + some, hi);
       some = (hi - lo + 63) / 64;
       uint32_t unused;
@@ -505,6 +505,7 @@ struct AttentionArgs {
   float* out;
   char* workspace;
   int32_t n_heads;
+  int32_t group;  // query heads of a kv head
   int32_t tiles;
   int32_t tile_heads;
   float scale_log2;
@@ -518,7 +519,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Att
   const float* __restrict__ q = args.q;
   float* __restrict__ out = args.out;
   char* __restrict__ workspace = args.workspace;
-  const int32_t n_heads = args.n_heads, tiles = args.tiles, tile_heads = args.tile_heads;
+  const int32_t n_heads = args.n_heads, group = args.group, tiles = args.tiles, tile_heads = args.tile_heads;
   const float scale_log2 = args.scale_log2;
   constexpr int kSub = D == 128 && !kQ8 ? 2 : 4;  // 16-key tiles of a step, which is a unit
   constexpr int kStep = 16 * kSub;
@@ -556,7 +557,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Att
   const int g = lane >> 4;
   const int head_col = n % kHeadCols;
   const int copy = n / kHeadCols;
-  const int32_t group = n_heads / view.n_kv;
 
   // the batch's units, and this wave's share
   const Batch batch(rows, lane);
@@ -1449,8 +1449,8 @@ void GpuAttentionPaged(const GpuPagedKv& kv, const GpuPageTable& table, const in
                           : (kv.head_dim == 128 ? PagedAttentionKernel<128, true, 1> : PagedAttentionKernel<64, true, 1>);
   }
   Launch("PagedAttentionKernel", kern, dim3(static_cast<unsigned>(groups)), dim3(64 * kWaves),
-         AttentionArgs{dev::ViewOf(kv, table), rows, q_dev, out_dev, static_cast<char*>(workspace), n_heads, tiles,
-                       tile_heads, scale_log2});
+         AttentionArgs{dev::ViewOf(kv, table), rows, q_dev, out_dev, static_cast<char*>(workspace), n_heads,
+                       n_heads / kv.n_kv_heads, tiles, tile_heads, scale_log2});
 }
 
 }  // namespace rpg
