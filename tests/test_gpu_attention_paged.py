@@ -248,6 +248,32 @@ def test_non_finite_queries_and_poisoned_rows(gpu):
     assert np.all(np.isfinite(got[2, :2])) and np.all(np.isnan(got[2, 2:]))
 
 
+@pytest.mark.parametrize("heads,d", [(8, 128), (5, 64), (7, 128)])
+def test_more_than_four_heads_of_an_8_bit_cache(gpu, heads, d):
+    """Two column tiles: large and small queries and values, and what is not a number in one head, row or page alone."""
+    rng = np.random.default_rng(35)
+    lens = [300, 250, 70, 130, 129, 64]
+    pages = Pages(rng, Q8, 1, d, 16, lens).fill_random(rng, lens, k_amp=2.0)
+    for pos in range(lens[1]):
+        pages.put(1, pos, rng.normal(0, 1, (1, d)).astype(np.float32),
+                  (10.0 ** rng.integers(-30, 30) * rng.normal(0, 1, (1, d))).astype(np.float32))
+    pages.put(2, 40, np.full((1, d), np.nan, np.float32), np.ones((1, d), np.float32))
+    pages.put(5, 63, np.ones((1, d), np.float32), np.full((1, d), np.inf, np.float32))
+    pages.table[3, 4] = pages.n_pages
+    q = rng.normal(0, 1, (6, heads, d)).astype(np.float32)
+    q[0, 0] *= 30
+    q[0, heads - 1] *= np.float32(1e-30)
+    q[4, 1, 2] = np.nan
+    q[4, heads - 1, 3] = -np.inf
+    kv, table = pages.device(gpu)
+    got = attend(gpu, kv, table, lens, q)
+    assert np.all(np.isnan(got[[2, 3, 5]]))
+    check(got[:2], pages, lens[:2], q[:2])
+    fine = [h for h in range(heads) if h not in (1, heads - 1)]
+    assert np.all(np.isnan(got[4][[1, heads - 1]]))
+    check(got[4:5][:, fine], pages, lens[4:5], q[4:5][:, fine], [4])
+
+
 def test_rows_may_share_a_sequence(gpu):
     """A turn of several tokens: each row sees its own length of the one sequence; rows in any order, pages shared."""
     rng = np.random.default_rng(26)
