@@ -241,9 +241,11 @@ __device__ __forceinline__ uint32_t Scalar(uint32_t x) { return __builtin_amdgcn
 // a unit, so that all workgroups get alike. With fewer, joining what two workgroups hold of a pair (a round trip to memory
 // to store, one to count, one to read) costs more than some units more in turn: a pair of up to kWholeUnits is one item, a
 // longer one is cut evenly into items of at most 2^step, about what each workgroup then gets.
-// (kWholeUnits 16 and so one workgroup for 500 positions: 11.6 us against 10.5 for four and their join.)
+// (One row of 250 positions, 8 units for each of 8 kv heads: 9.0 us whole, 9.9 in two items each; of 500, 16 units: 11.6
+// whole, 10.5 in four items each.)
 constexpr uint32_t kManyUnits = 8192;
-constexpr uint32_t kWholeUnits = 4;
+constexpr uint32_t kWholeUnits = 8;
+constexpr uint32_t kLeastStep = 2;
 
 struct Cut {
   bool units;
@@ -252,7 +254,7 @@ struct Cut {
   // for a batch of `all` units
   __device__ __forceinline__ explicit Cut(uint32_t all) {
     units = all >= kManyUnits;
-    step = all <= 4 * kMaxGroups ? 2 : all <= 8 * kMaxGroups ? 3 : 4;
+    step = kLeastStep + (all <= 4 * kMaxGroups ? 0 : all <= 8 * kMaxGroups ? 1 : 2);
   }
   __device__ __forceinline__ uint32_t Items(uint32_t n) const {
     return units ? n : n <= kWholeUnits ? min(n, 1u) : (n + (1u << step) - 1u) >> step;
@@ -1440,7 +1442,7 @@ void GpuAttentionPaged(const GpuPagedKv& kv, const GpuPageTable& table, const in
   // parts of a row cost more to join than the card gives for them (1 x 32768 positions, 8 kv heads: 22.7 against 25.0 us)
   const int64_t all_pairs = n_rows * rows.pairs;
   const int64_t at_once = all_pairs * kJoinAtOnce < kMaxGroups ? kMaxGroups / 2 : kMaxGroups;
-  const int64_t groups = std::min<int64_t>(at_once, all_pairs * ((most + kWholeUnits - 1) / kWholeUnits));
+  const int64_t groups = std::min<int64_t>(at_once, all_pairs * ((most + (1 << kLeastStep) - 1) >> kLeastStep));
   const float scale_log2 =
       static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(kv.head_dim)));
   auto* kern = kv.head_dim == 128 ? PagedAttentionKernel<128, false, 1> : PagedAttentionKernel<64, false, 1>;
