@@ -47,7 +47,7 @@
 //
 // Measured (kernel times; "units" as above): 32 rows of up to 4096 positions in fp16,
 // 16 / 8 heads, 269 MB: 50.7 us, 5.3 TB/s; 128 rows of up to 8192 in 8 bits, 32 / 8
-// heads, 1152 MB: 192 us, 6.0 TB/s (fp16, 2230 MB: 357 us, 6.2 TB/s), where a pure
+// heads, 1152 MB: 189 us, 6.1 TB/s (fp16, 2230 MB: 357 us, 6.2 TB/s), where a pure
 // read of as much reaches 7.0. While all workgroups run the reads come at about that
 // rate; the rest is the end, where every other XCD is a tenth slower and of a compute
 // unit's two workgroups the one whose loads come behind a fifth. Shares to match gained
@@ -55,7 +55,7 @@
 // (64 x 4096 positions from 93 to 100 us), and dealing the last fifth out late, in
 // shares of their own, cost what it gained.
 // One row of 32768 positions in 8 bits, 8 kv heads, 69 MB: 21.1 us, of which about
-// ten read at full rate; 1 x 500 positions 9.3 us and 1 x 60 7.1 us are the chain of
+// ten read at full rate; 1 x 500 positions 8.9 us and 1 x 60 7.0 us are the chain of
 // round trips: lengths 0.5, the search for the share 0.7, page table 0.2, keys 1.5,
 // products and weights 1.9, join in LDS 0.6 and, where a pair is split, store and
 // count 1.3 and the last one's read and join 1.5.
