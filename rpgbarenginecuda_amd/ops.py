@@ -929,14 +929,14 @@ class GpuPagedKv:
         self.row_elems = self.n_kv_heads * self.head_dim
         self.device_index = None if self.device is None else self.device.index
         self.current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
-        self.float_at = _paged_addr(self, torch.float32)
-        self.int_at = _paged_addr(self, torch.int32)
+        self.float_at = _paged_addr(self.device, torch.float32)
+        self.int_at = _paged_addr(self.device, torch.int32)
         self._at = {torch.float32: self.float_at, torch.int32: self.int_at}
 
     def at(self, dtype):
         """_paged_addr's function for these pages and dtype."""
         if dtype not in self._at:
-            self._at[dtype] = _paged_addr(self, dtype)
+            self._at[dtype] = _paged_addr(self.device, dtype)
         return self._at[dtype]
 
 
@@ -958,20 +958,21 @@ class GpuPageTable:
         self.device_index = None if isinstance(pages, int) else pages.get_device()
 
 
-def _paged_addr(kv: GpuPagedKv, dtype):
-    """The function (buffer, bytes, name) -> address for buffers of dtype that have to be where the pages are: _addr, and
-    the device. The calls over pages are short enough for the checks of their many tensors to count, so that a tensor
-    that is in order passes through as few of them as there are."""
+def _paged_addr(device, dtype):
+    """The function (buffer, bytes, name) -> address for buffers of dtype that have to be on the pages' device (None:
+    raw addresses): _addr, and the device. It does not hold the pages, whose view holds it. The calls over pages are
+    short enough for the checks of their many tensors to count, so that a tensor that is in order passes through as few
+    of them as there are."""
     torch = _t()
-    tensor, index = torch.Tensor, kv.device_index
+    tensor, index = torch.Tensor, None if device is None else device.index
 
     def at(buf, nbytes: int, name: str):
         if (type(buf) is tensor and buf.dtype is dtype and buf.get_device() == index and buf.nbytes >= nbytes
                 and buf.is_contiguous()):
             return buf.data_ptr()
         addr = _addr(buf, nbytes, dtype, name)
-        if kv.device is not None and isinstance(buf, tensor) and buf.device != kv.device:
-            raise RpgError(f"{name}: a tensor on {buf.device} beside a paged cache on {kv.device}")
+        if device is not None and isinstance(buf, tensor) and buf.device != device:
+            raise RpgError(f"{name}: a tensor on {buf.device} beside a paged cache on {device}")
         return addr
 
     return at

@@ -234,6 +234,23 @@ def test_python_views_check_their_tensors(ops):
         ops.GpuPageTable(torch.zeros(4, 2, dtype=torch.int32))
 
 
+def test_pages_go_with_their_view(ops):
+    """Nothing that a view holds holds the view: the pages' memory is free when it goes, without a collection."""
+    import gc
+    import weakref
+
+    gc.disable()
+    try:
+        kv, t = views(ops)
+        for call in calls(ops, kv, t, n=0):
+            call()
+        gone = [weakref.ref(kv), weakref.ref(t)]
+        del kv, t, call
+        assert [r() for r in gone] == [None, None]
+    finally:
+        gc.enable()
+
+
 def test_table_of_functions_matches_its_header(ops):
     """The struct in include/rpg_paged.h and its Python mirror have the same entries, in order."""
     import os
