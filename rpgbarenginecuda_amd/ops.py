@@ -932,12 +932,14 @@ class GpuPagedKv:
         self.float_at = _paged_addr(self.device, torch.float32)
         self.int_at = _paged_addr(self.device, torch.int32)
         self._at = {torch.float32: self.float_at, torch.int32: self.int_at}
+        self.out_types = {torch.float32: True, torch.float16: False, torch.int16: False, torch.uint16: False}
 
     def at(self, dtype):
         """_paged_addr's function for these pages and dtype."""
-        if dtype not in self._at:
-            self._at[dtype] = _paged_addr(self.device, dtype)
-        return self._at[dtype]
+        found = self._at.get(dtype)
+        if found is None:
+            found = self._at[dtype] = _paged_addr(self.device, dtype)
+        return found
 
 
 class GpuPageTable:
@@ -1017,15 +1019,15 @@ def GpuKvReadPaged(kv: GpuPagedKv, table: GpuPageTable, seq_ids, positions, n_to
     """The rows back out of the pages: element d of row t of kv head h to out[t * token_stride + h * head_stride + d].
     k_out and v_out are float32 or 16-bit (float16, int16, uint16) tensors of one type; raw addresses need out_f32.
     Strides (head_dim, max_seq * head_dim) fill a layer of the contiguous cache."""
-    torch = _t()
     int_at = kv.int_at
     dtype = getattr(k_out, "dtype", None)
-    if out_f32 is None:
-        if dtype is None:
-            raise RpgError("GpuKvReadPaged: raw addresses need out_f32")
-        out_f32 = dtype is torch.float32
-    if dtype is not None and dtype not in ((torch.float32,) if out_f32 else (torch.float16, torch.int16, torch.uint16)):
-        raise RpgError(f"GpuKvReadPaged: k_out is {dtype}")
+    if dtype is None and out_f32 is None:
+        raise RpgError("GpuKvReadPaged: raw addresses need out_f32")
+    if dtype is not None:
+        f32 = kv.out_types.get(dtype)
+        if f32 is None or (out_f32 is not None and bool(out_f32) != f32):
+            raise RpgError(f"GpuKvReadPaged: k_out is {dtype}")
+        out_f32 = f32
     last = (n_tokens - 1) * token_stride + (kv.n_kv_heads - 1) * head_stride + kv.head_dim
     nbytes = (4 if out_f32 else 2) * last if n_tokens > 0 else 0
     out_at = kv.at(dtype)

@@ -123,6 +123,17 @@ def test_read_refusals(ops):
         ops.GpuKvReadPaged(kv, t, FAKE, FAKE, 2, FAKE, FAKE, 1024, 128)
 
 
+def test_read_refuses_other_types(ops):
+    import torch
+
+    kv, t = views(ops)
+    for dtype, f32 in ((torch.int32, None), (torch.float64, None), (torch.bfloat16, False), (torch.float16, True),
+                       (torch.float32, False)):
+        out = torch.zeros(2, 8, 128, dtype=dtype)
+        with pytest.raises(ops.RpgError, match="k_out is torch"):
+            ops.GpuKvReadPaged(kv, t, FAKE, FAKE, 2, out, out, 1024, 128, out_f32=f32)
+
+
 def test_attention_refusals(ops):
     kv, t = views(ops)
     need = ops.GpuAttentionPagedWorkspace(16, 8, 128)
