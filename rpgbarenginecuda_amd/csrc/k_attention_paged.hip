@@ -21,16 +21,16 @@
 // what the one product would (weights below 2^-23 of the largest excepted, which may
 // turn an infinite value into NaN).
 //
-// 8-bit cache (16x16x64, int32 sums): the codes enter as they are kept and the sums
-// are exact. Queries are taken to whole numbers below 2^30, relative to a row's
-// largest, and weights, with their values' scales, to whole numbers of 2^-27
-// (relative to a power of two above the scales so far); either enters as four
-// signed digits of 8 bits, in columns n, n + 4, n + 8, n + 12. Weights have 3 bits of
-// headroom: the maximum that they are relative to moves only when a score exceeds
-// it by 3 (log2), and only then are the int32 sums of the output taken to fp32. (Of
-// more than four heads, two column tiles, each step's at once: there is no room for
-// both. 16 x 4000 positions, 64 / 8 heads, 136 MB: 35.4 us.) Of the four lanes that
-// have a score's digits each does a part of the softmax.
+// 8-bit cache (16x16x64, int32 sums): the codes enter as they are kept and a step's sums are exact. Queries are taken to
+// whole numbers below 2^30, relative to a row's largest. What the codes of values are multiplied by is weight times their
+// row's scale, p_j c_j: whole numbers of 2^-29 of the power of two at or below the largest of the head's 64 of this step.
+// That is what counts in the step, so a row of a large scale and no weight costs the others nothing; each is off by at
+// most 2^-30 of a term that is there. Either enters as four signed digits of 8 bits, in columns n, n + 4, n + 8, n + 12. A
+// step's sums are then taken to fp32, where the output's have a power of two of their own, moved only where a step's
+// largest passes it by 2^64: codes times scales of any size there is have room. (int32 sums kept from step to step, which
+// need one power of two for all of them, were no faster: 128 x 8192 positions 188.5 us against 189.5, 1 x 32768 20.8
+// against 20.2, 45 x 2000 25.3 against 25.8.) The maximum that weights are relative to moves only where a score exceeds it
+// by 3 (log2). Of the four lanes that have a score's digits each does a part of the softmax.
 //
 // Keys and values come straight to LDS in whole 128-byte lines, the next step's as
 // soon as this step has read what they replace; the transposition of values is the
@@ -534,9 +534,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Att
   constexpr int kCopies = kQ8 ? 4 : 2;     // columns of a head, that is lanes that have its final sums
   constexpr int kHeadCols = 16 / kCopies;
   constexpr int kOwn = kE / kCopies;       // tiles of 16 elements that each of them writes
-  // Whether the int32 sums of values live from step to step. For two column tiles they and the fp32 ones would not both
-  // fit in the registers, and each step's are taken to fp32 at once.
-  constexpr bool kKeepSums = kQ8 && kTiles == 1;
 
   // a wave's step of keys and values, each row's scale behind them
   constexpr int kStage = kStep * kRow + (kQ8 ? kStep * 4 : 0);
@@ -725,9 +722,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Att
     Half8 qh[kQ8 ? 1 : kSteps];
     I32x4 qi[kQ8 ? kTiles : 1][kQ8 ? kSteps : 1];
     float to_score[kTiles], m, l;
-    float ref = 0.0f;  // 8-bit values: a power of two above the scales so far
+    // 8-bit values: the power of two (times what m moved by since) that acc holds them multiplied by; infinity where that
+    // is nothing yet
+    float shrink = INFINITY;
     F32x4 acc[kTiles][kE];
-    I32x4 sum[kKeepSums ? kE : 1];
     // the digit that this lane's column stands for, and its weight
     const uint32_t digit = static_cast<uint32_t>(copy) * 0x0101u + 0x0400u;
     const float digit_by = __int_as_float((127 + 8 * copy) << 23);
@@ -738,7 +736,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Att
       const int32_t h0 = (pair - kh * tiles) * tile_heads;
       heads = min(tile_heads, group - h0);
       head_row = static_cast<int64_t>(row) * n_heads + kh * group + h0;
-      ref = 0.0f;
+      shrink = INFINITY;
       m = -INFINITY;
       l = 0.0f;
 #pragma unroll
@@ -747,10 +745,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Att
         const bool there = h < heads;
         const float* qr = q + (head_row + (there ? h : 0)) * D;
 #pragma unroll
-        for (int i = 0; i < kE; ++i) {
-          acc[t][i] = F32x4{0.0f, 0.0f, 0.0f, 0.0f};
-          if constexpr (kKeepSums) sum[i] = I32x4{0, 0, 0, 0};
-        }
+        for (int i = 0; i < kE; ++i) acc[t][i] = F32x4{0.0f, 0.0f, 0.0f, 0.0f};
         constexpr int kAt = kQ8 ? 16 : 8;  // elements of a lane for one product
         float x[kSteps][kAt];
         float top = 0.0f, odd = 0.0f;
@@ -798,24 +793,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Att
         }
       }
     };
-    // takes the int32 sums to acc, which is then scaled by `back`
-    const auto take_sums = [&](int t, float back) {
-      if constexpr (kQ8) {
-#pragma unroll
-        for (int i = 0; i < kE; ++i) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            if constexpr (kKeepSums) {
-              acc[t][i][r] = fmaf(static_cast<float>(sum[i][r]), digit_by, acc[t][i][r]) * back;
-            } else {
-              acc[t][i][r] *= back;
-            }
-          }
-          if constexpr (kKeepSums) sum[i] = I32x4{0, 0, 0, 0};
-        }
-      }
-    };
-
     // the scales of keys 4 g .. 4 g + 3 of tile j
     const auto scales_at = [&](const char* stage, int j) {
       return *reinterpret_cast<const float4*>(stage + kStep * kRow + 64 * j + 16 * g);
@@ -825,7 +802,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Att
     bool turned = true;  // the unit at hand is its piece's first
     F32x4 kept[kTiles][kOwn];
     float kept_m[kTiles], kept_l[kTiles];
-    int32_t since = 0;  // steps since the int32 sums were last taken
 
     while (true) {
       if (turned) {
@@ -951,6 +927,24 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Att
       }
       if constexpr (kQ8) top = fmaxf(top, other_half(top));
       top = MaxAcrossRows(top);
+      if constexpr (kQ8) {
+        if (__any(top > m + 3.0f)) {  // acc stays: what it holds, relative to a larger m, is less, and so multiplied by more
+          const float to = top > m + 3.0f ? top : m;
+          const float safe = to == -INFINITY ? 0.0f : to;
+          l *= __builtin_amdgcn_exp2f(m - safe);
+          shrink *= __builtin_amdgcn_exp2f(safe - m);
+          m = to;
+        }
+        const float safe = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int j = 0; j < kMine; ++j) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            s[j][i] = __builtin_amdgcn_exp2f(s[j][i] - safe);
+            l += s[j][i];
+          }
+        }
+      }
       // the values are there: the next keys' loads, if any, are younger
       if (more) {
         WaitLoads<kStageLoads>();
@@ -971,50 +965,47 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Att
             vs[j].w = p + 3 < left ? vs[j].w : 0.0f;
           }
         }
-        // the largest, as whole numbers, where a NaN is larger than any number
+        // weights times scales, and the head's largest of the step (as whole numbers, where a NaN is larger than any number)
         uint32_t big = 0;
 #pragma unroll
         for (int j = 0; j < kMine; ++j) {
-          big = max(max(big, max(__float_as_uint(vs[j].x), __float_as_uint(vs[j].y))),
-                    max(__float_as_uint(vs[j].z), __float_as_uint(vs[j].w)));
-        }
-        big = max(big, __float_as_uint(other_half(__uint_as_float(big))));
-        big = __float_as_uint(AcrossRows(__uint_as_float(big), [](float a, float b) {
-          return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b)));
-        }));
-        big = __builtin_amdgcn_readfirstlane(big);
-        if (big >= __float_as_uint(ref) || (kKeepSums && ++since >= 1024)) {  // 1024 steps: int32 holds 2^17 products of 2^14
-          float by = 1.0f;
-          if (big >= __float_as_uint(ref)) {
-            const int e = min(max(static_cast<int>(big >> 23) + 1, 27), 254);
-            by = ref * __int_as_float((254 - e) << 23);
-            ref = __int_as_float(e << 23);
+          const float by[4] = {vs[j].x, vs[j].y, vs[j].z, vs[j].w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            s[j][i] *= by[i];
+            big = max(big, __float_as_uint(s[j][i]));
           }
-#pragma unroll
-          for (int t = 0; t < kTiles; ++t) take_sums(t, by);
-          if (big >= 0x7F800000u) l = NAN;
-          since = 0;
         }
-        const float up = 0x1p27f * __int_as_float((254 << 23) - __float_as_int(ref));  // 2^27 / ref
-        if (__any(top > m + 3.0f)) {
-          const float to = top > m + 3.0f ? top : m;
-          const float back = __builtin_amdgcn_exp2f(m - (to == -INFINITY ? 0.0f : to));
-          m = to;
-          l *= back;
+        const auto larger = [](float a, float b) { return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b))); };
+        big = __float_as_uint(AcrossRows(larger(__uint_as_float(big), other_half(__uint_as_float(big))), larger));
+        l = big >= 0x7F800000u ? NAN : l;
+        const float largest = __uint_as_float(big);
+        // the largest is in [2^e, 2^(e + 1)): the step's are whole numbers of 2^(e - 29), less than 2^30 of them
+        const uint32_t biased = min(max(big >> 23, 1u), 253u);
+        const float up = __uint_as_float((254u - biased) << 23), down = __uint_as_float(biased << 23);
+        if (__any(largest * shrink > 0x1p64f)) {
+          const bool grew = largest * shrink > 0x1p64f;
+          const float back = grew ? up * __builtin_amdgcn_rcpf(shrink) : 1.0f;
+          shrink = grew ? up : shrink;
 #pragma unroll
-          for (int t = 0; t < kTiles; ++t) take_sums(t, of_tile(t, back));
+          for (int t = 0; t < kTiles; ++t) {
+            const float by = of_tile(t, back);
+#pragma unroll
+            for (int i = 0; i < kE; ++i) acc[t][i] *= by;
+          }
         }
-        const float safe = m == -INFINITY ? 0.0f : m;
+        // a whole number of this lane's digit, in acc
+        const float unit = largest > 0.0f ? down * shrink : 0.0f;
+        float units[kTiles];
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) units[t] = of_tile(t, unit) * (digit_by * 0x1p-29f);
         I32x4 w[kTiles];  // tile j of 16 keys: bytes 4 j ..
 #pragma unroll
         for (int j = 0; j < kMine; ++j) {
-          const float by[4] = {vs[j].x, vs[j].y, vs[j].z, vs[j].w};
           float d[4];  // whole numbers, and so below
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float p = __builtin_amdgcn_exp2f(s[j][i] - safe);
-            l += p;
-            d[i] = __uint_as_float(static_cast<uint32_t>(static_cast<int>(fmaf(p * by[i], up, 0.5f))) + 0x80808080u);
+            d[i] = __uint_as_float(static_cast<uint32_t>(static_cast<int>(fmaf(s[j][i] * up, 0x1p29f, 0.5f))) + 0x80808080u);
           }
           // this lane's digit of its own four weights, and of those of the lanes that have the others
           const auto digits = [&](auto of) {
@@ -1047,16 +1038,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Att
         }
 #pragma unroll
         for (int i = 0; i < kE; ++i) {
+          const I32x4 v = I32x4{a[i][0][0], a[i][0][1], a[i][1][0], a[i][1][1]};
 #pragma unroll
           for (int t = 0; t < kTiles; ++t) {
-            const I32x4 v = I32x4{a[i][0][0], a[i][0][1], a[i][1][0], a[i][1][1]};
-            if constexpr (kKeepSums) {
-              sum[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(v, w[t], sum[i], 0, 0, 0);
-            } else {
-              const I32x4 x = __builtin_amdgcn_mfma_i32_16x16x64_i8(v, w[t], I32x4{0, 0, 0, 0}, 0, 0, 0);
+            const I32x4 x = __builtin_amdgcn_mfma_i32_16x16x64_i8(v, w[t], I32x4{0, 0, 0, 0}, 0, 0, 0);
 #pragma unroll
-              for (int r = 0; r < 4; ++r) acc[t][i][r] = fmaf(static_cast<float>(x[r]), digit_by, acc[t][i][r]);
-            }
+            for (int r = 0; r < 4; ++r) acc[t][i][r] = fmaf(static_cast<float>(x[r]), units[t], acc[t][i][r]);
           }
         }
       } else {
@@ -1110,9 +1097,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Att
       if (!turn) continue;
 
       // ---- the piece's (m, l, o): out, or kept where it is not the whole of its pair
-      if constexpr (kKeepSums) take_sums(0, 1.0f);
       const bool whole = c_first == 0 && c_end == piece_units;
-      const float unit = kQ8 ? ref * 0x1p-27f : 0x1p-14f;
       if (!whole) {
         const int which = more ? 0 : 1;
         if (lane == 0) pieces[wave][which] = Piece{u - c_end, c_first, c_end, piece_units, piece_row, piece_pair};
@@ -1123,7 +1108,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Att
 #pragma unroll
       for (int t = 0; t < kTiles; ++t) {
         const float total = of_tile(t, l), top = of_tile(t, m);
-        const float by = whole ? unit / total : unit;
+        // 8-bit values: one factor after the other, since their product may be too small a number
+        const float unit = kQ8 ? 1.0f / of_tile(t, shrink) : 1.0f;
+        const float by = (kQ8 ? 1.0f : 0x1p-14f) / (whole ? total : 1.0f);
         const int h = t * kHeadCols + head_col;
         F32x4 own[kOwn];
 #pragma unroll
@@ -1134,6 +1121,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Att
             x += Ror<8>(x);
             if constexpr (kQ8) x += Ror<4>(x);
             x *= by;
+            if constexpr (kQ8) x *= unit;
             own[i % kOwn][r] = i < kOwn || copy == i / kOwn ? x : own[i % kOwn][r];
           }
         }

@@ -130,3 +130,40 @@ def bound(d, n, smag, vmax):
     their shares add (n + 64) 2^-24 vmax. Wrong rows, heads or borders are off by orders of magnitude more."""
     delta = (d + 12) * U * smag
     return (np.expm1(2 * delta) + (n + 64) * U) * vmax + 1e-30
+
+
+def attention_within(q, k, v, kind):
+    """One row of at least one position: attention()'s output and how far from it each element may be, [heads, d] both.
+
+    Weights first. A score is off by delta_j = (d + 12) 2^-24 sum_d |q_d k_jd| / sqrt(d) as at bound(), and by what is cut
+    off of queries relative to their row's largest element: half a unit of whole numbers below 2^30, that is 2^-30 of it
+    (fp16: below 2^-38), for every |k_jd|. So w_j = p_j / sum p counts for (1 + e_j) w_j, |e_j| <= e^delta_j - 1 and 4
+    roundings. With E = sum_j w_j |e_j|: numerators are off by sum_j w_j |e_j v_jd|, the denominator by E, the quotient by
+    (sum_j w_j |e_j v_jd| + E A_d) / (1 - E), A_d = sum_j w_j |v_jd|.
+
+    Sums: at most n + 64 roundings of half a step of partial sums no larger than A_d.
+
+    8-bit rows: p_j times the row's scale enters as a whole number whose unit is at most 2^-29 of the largest of its 64
+    positions, so that each is off by 2^-30 of that: together 64 times that times a code of 127, for every 64 positions.
+    With B = sum_j w_j max_d |v_jd|, of which the largest of 64 is a part: 64 2^-30 B = 2^-24 B. fp16 rows: p_j, at most
+    1, enters as two fp16 terms of p_j 2^14, of which the second may end at 2^-24: n 2^-39 / sum p, times max |v|.
+
+    Weights below 2^-126 of the largest (2^-120 with the lag of the maximum) may count as none: n 2^-120 max |v|."""
+    heads, d = q.shape
+    n, g = len(k), heads // k.shape[1]
+    q = q.astype(np.float64)
+    out, limit = np.zeros((heads, d)), np.zeros((heads, d))
+    for h in range(heads):
+        kk, vv = k[:, h // g], v[:, h // g]
+        s = kk @ q[h] / np.sqrt(d)
+        w = np.exp(s - s.max())
+        w /= w.sum()
+        a, b = w @ np.abs(vv), w @ np.abs(vv).max(-1)
+        cut = 2.0 ** (-30 if kind == Q8 else -38) * np.abs(q[h]).max()
+        delta = ((d + 12) * U * np.abs(kk) @ np.abs(q[h]) + cut * np.abs(kk).sum(-1)) / np.sqrt(d)
+        we = w * np.expm1(delta)
+        out[h] = w @ vv
+        limit[h] = (we @ np.abs(vv) + we.sum() * a) / (1 - we.sum()) + (n + 64 + 8) * U * a
+        vmax = np.abs(vv).max()
+        limit[h] += n * 2.0 ** -120 * vmax + (2.0 ** -24 * b if kind == Q8 else n * 2.0 ** -39 * w.max() * vmax)
+    return out, limit
