@@ -722,6 +722,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Att
     Half8 qh[kQ8 ? 1 : kSteps];
     I32x4 qi[kQ8 ? kTiles : 1][kQ8 ? kSteps : 1];
     float to_score[kTiles], m, l;
+    int key_exp = 0;  // 8-bit keys: the power of two that their scales are multiplied by, of the lane's tile
     // 8-bit values: the power of two (times what m moved by since) that acc holds them multiplied by; infinity where that
     // is nothing yet
     float shrink = INFINITY;
@@ -764,12 +765,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Att
           }
         }
         top = MaxAcrossRows(top);
-        // the power of two that brings top to [2^14, 2^15), or [2^29, 2^30)
-        const int e = min(max((kQ8 ? 283 : 268) - (__float_as_int(top) >> 23), 1), 254);
-        const float up = __int_as_float(e << 23);
-        to_score[t] = ldexpf(scale_log2, 127 - e);
         if constexpr (kQ8) {
-          to_score[t] = to_score[t] * digit_by + SumAcrossRows(odd);
+          // the power of two that brings top to [2^29, 2^30), taken back with the keys' scales: a product of a query that is
+          // far from 1 and of one code need not be an fp32 number
+          const int by = 30 - __builtin_amdgcn_frexp_expf(top);
+          if (kTiles == 1 || second == (t == 1)) key_exp = -by;
+          to_score[t] = scale_log2 * digit_by + SumAcrossRows(odd);
 #pragma unroll
           for (int s = 0; s < kSteps; ++s) {
 #pragma unroll
@@ -777,12 +778,15 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Att
               uint32_t w[4];
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
-                w[k] = static_cast<uint32_t>(static_cast<int>(__builtin_rintf(x[s][4 * i + k] * up))) + 0x80808080u;
+                w[k] = static_cast<uint32_t>(static_cast<int>(__builtin_rintf(ldexpf(x[s][4 * i + k], by)))) + 0x80808080u;
               }
               qi[t][s][i] = Digit4(w[0], w[1], w[2], w[3], digit);
             }
           }
         } else {
+          const int e = min(max(268 - (__float_as_int(top) >> 23), 1), 254);  // brings top to [2^14, 2^15)
+          const float up = __int_as_float(e << 23);
+          to_score[t] = ldexpf(scale_log2, 127 - e);
 #pragma unroll
           for (int s = 0; s < kSteps; ++s) {
             uint32_t w[4];
@@ -876,7 +880,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Att
         }
 #pragma unroll
         for (int j = 0; j < kMine; ++j) {
-          const float by[4] = {ks[j].x, ks[j].y, ks[j].z, ks[j].w};
+          const float by[4] = {ldexpf(ks[j].x, key_exp), ldexpf(ks[j].y, key_exp), ldexpf(ks[j].z, key_exp),
+                               ldexpf(ks[j].w, key_exp)};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float lo = x[j][i], hi = x[kSub - kMine + j][i];

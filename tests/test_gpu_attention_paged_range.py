@@ -96,6 +96,21 @@ def test_values_all_small_or_all_large(gpu, heads, d, exponent):
     assert np.all(np.abs(got).max(-1) > 0.02 * 2.0 ** exponent)
 
 
+@pytest.mark.parametrize("heads,d", [(4, 128), (8, 128), (1, 64), (6, 64)])
+def test_queries_and_keys_far_from_one(gpu, heads, d):
+    """Queries of 2^e and 8-bit keys of 2^-e: scores of ordinary size, between queries whose products with one code pass
+    fp32's range on either side."""
+    rng = np.random.default_rng(heads * d + 3)
+    exponents, n = [118, 100, 60, -100, -110, -125], 200
+    ks = [rng.normal(0, 1, (n, 1, d)) * 2.0 ** -e for e in exponents]
+    vs = [rng.normal(0, 1, (n, 1, d)) for _ in exponents]
+    q = rng.normal(0, 1, (len(exponents), heads, d)) * 2.0 ** np.array(exponents, np.float64)[:, None, None]
+    q[0, 0] = 0
+    if heads > 1:
+        q[1, 1] *= 2.0 ** -140  # beside heads of another size
+    check(gpu, Q8, q.astype(np.float32), ks, vs)
+
+
 @pytest.mark.parametrize("kind", [F16, Q8])
 @pytest.mark.parametrize("heads,d", [(2, 128), (8, 128), (4, 64)])
 def test_many_small_weights_beside_a_large_one(gpu, heads, d, kind):
