@@ -172,39 +172,40 @@ __device__ __forceinline__ uint32_t LdsAddress(const void* p) {
 }
 // kN times 16 bytes a lane from rs: time i from byte off[i % kOff] + 1024 i, lane j's to LDS address `to` + 1024 i +
 // 16 j (an instruction's offset counts on both sides). What is read once is loaded with the streaming hint: without it
-// 32 x 4096 positions took 59 us and not 53, 128 x 8192 236 and not 211. M0 holds the LDS address, which is read one wait state after it is
-// written; five are waited, which a resource needs whose registers a vector instruction wrote.
+// 32 x 4096 positions took 59 us and not 53, 128 x 8192 236 and not 211. M0 holds the
+// LDS address: an operand, so that the compiler writes it and knows what is there. It is read one wait state after it is
+// written; five are waited, which M0 and a resource need where a vector instruction wrote them.
 template <int kN, int kOff>
 __device__ __forceinline__ void LoadToLds(Resource rs, const uint32_t (&off)[kOff], uint32_t to) {
   static_assert(kN == 1 || kN == 2 || kN == 4, "");
   if constexpr (kN == 1) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds"
+    asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds"
                  :
-                 : "s"(to), "v"(off[0]), "s"(rs)
+                 : "{m0}"(to), "v"(off[0]), "s"(rs)
                  : "memory");
   } else if constexpr (kN == 2) {
     asm volatile(
-        "s_mov_b32 m0, %0\n\ts_nop 4\n\t"
+        "s_nop 4\n\t"
         "buffer_load_dwordx4 %1, %3, 0 offen nt lds\n\t"
         "buffer_load_dwordx4 %2, %3, 0 offen offset:1024 nt lds"
         :
-        : "s"(to), "v"(off[0]), "v"(off[1 % kOff]), "s"(rs)
+        : "{m0}"(to), "v"(off[0]), "v"(off[1 % kOff]), "s"(rs)
         : "memory");
   } else {
     asm volatile(
-        "s_mov_b32 m0, %0\n\ts_nop 4\n\t"
+        "s_nop 4\n\t"
         "buffer_load_dwordx4 %1, %5, 0 offen nt lds\n\t"
         "buffer_load_dwordx4 %2, %5, 0 offen offset:1024 nt lds\n\t"
         "buffer_load_dwordx4 %3, %5, 0 offen offset:2048 nt lds\n\t"
         "buffer_load_dwordx4 %4, %5, 0 offen offset:0xc00 nt lds"
         :
-        : "s"(to), "v"(off[0]), "v"(off[1 % kOff]), "v"(off[2 % kOff]), "v"(off[3 % kOff]), "s"(rs)
+        : "{m0}"(to), "v"(off[0]), "v"(off[1 % kOff]), "v"(off[2 % kOff]), "v"(off[3 % kOff]), "s"(rs)
         : "memory");
   }
 }
 // 4 bytes a lane, from an address of its own.
 __device__ __forceinline__ void LoadWordToLds(const float* from, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(to), "v"(from) : "memory");
+  asm volatile("s_nop 4\n\tglobal_load_lds_dword %1, off" : : "{m0}"(to), "v"(from) : "memory");
 }
 // Waits until at most kLeft vector memory accesses are under way.
 template <int kLeft>
