@@ -76,8 +76,9 @@ typedef struct {
 
   /* The rows back: element d of row t of kv head h to out[t * token_stride +
    * h * head_stride + d], fp16 bits (out_f32 0) or fp32 (1). Strides are in
-   * elements, multiples of 8, and rows must not overlap. (head_dim, max_seq *
-   * head_dim) gives a layer of an rpg_kv. */
+   * elements, multiples of 8, and rows must not overlap, nor those of k_out those
+   * of v_out (which may lie between them). (head_dim, max_seq * head_dim) gives a
+   * layer of an rpg_kv. */
   int32_t (*kv_read)(const rpg_paged_kv_t* kv, const rpg_page_table_t* table, const int32_t* seq_ids,
                      const int32_t* positions, int64_t n_tokens, int32_t out_f32, void* k_out, void* v_out,
                      int64_t token_stride, int64_t head_stride);

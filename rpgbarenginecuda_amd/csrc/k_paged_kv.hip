@@ -10,6 +10,7 @@
 // lane, and the sums and maxima over a row are butterflies over its lanes.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cfloat>
 
 #include "dev_util.h"
@@ -398,6 +399,21 @@ void LaunchWrite(const char* name, const GpuPagedKv& kv, WriteArgs args, int64_t
   Launch(name, kern, dim3(GridFor(units, kBlock / (kv.head_dim / 16))), dim3(kBlock), args);
 }
 
+// Whether a row of `bytes` at t * token_stride + h * head_stride (t < n_tokens, h < n_heads) and another `apart` behind such
+// a place share a byte; strides and distances in bytes. For each difference of heads, the difference of tokens that brings
+// the two nearest.
+bool RowsMeet(int64_t apart, int64_t bytes, int64_t n_tokens, int64_t token_stride, int64_t n_heads, int64_t head_stride) {
+  for (int64_t dh = 1 - n_heads; dh < n_heads; ++dh) {
+    const int64_t x = apart + dh * head_stride;
+    const int64_t whole = -x / token_stride;
+    for (int64_t dt = whole - 1; dt <= whole + 1; ++dt) {
+      const int64_t at = x + std::clamp(dt, 1 - n_tokens, n_tokens - 1) * token_stride;
+      if (at > -bytes && at < bytes) return true;
+    }
+  }
+  return false;
+}
+
 // Head rows of a call are counted in 32 bits.
 void CheckUnits(const char* what, int64_t n_tokens, int64_t rows_per_token) {
   RPG_CHECK(n_tokens <= 0x7FFFFFFF / rows_per_token, "%s: %lld tokens of %lld rows are too many for one call", what,
@@ -470,6 +486,12 @@ void GpuKvReadPaged(const GpuPagedKv& kv, const GpuPageTable& table, const int32
             static_cast<long long>(head_stride));
   RPG_CHECK(k_out != v_out, "KvReadPaged: k_out and v_out are the same");
   CheckUnits("KvReadPaged", n_tokens, kv.n_kv_heads);
+  const int64_t size = out_f32 ? 4 : 2, row = size * kv.head_dim;
+  const int64_t span = size * ((n_tokens - 1) * token_stride + (kv.n_kv_heads - 1) * head_stride) + row;
+  RPG_CHECK(!Overlap(k_out, span, v_out, span) ||
+                !RowsMeet(static_cast<const char*>(v_out) - static_cast<const char*>(k_out), row, n_tokens,
+                          size * token_stride, kv.n_kv_heads, size * head_stride),
+            "KvReadPaged: rows of k_out and v_out overlap");
   const int64_t units = n_tokens * kv.n_kv_heads;
   const bool q8 = kv.type == kKvQ8;
   auto* kern = kv.head_dim == 128

@@ -302,7 +302,8 @@ void GpuQkNormRopeKvPaged(const GpuPagedKv& kv, const GpuPageTable& table, const
 // The rows back out of the cache: element d of row t of kv head h goes to
 // out[t * token_stride + h * head_stride + d], as fp16 bits (out_f32 false) or
 // fp32. Strides (in elements) are multiples of 8, and rows must not overlap:
-// either whole tokens or whole heads follow each other. token_stride = head_dim,
+// either whole tokens or whole heads follow each other. Rows of v_out may lie
+// between those of k_out, but not over them. token_stride = head_dim,
 // head_stride = max_seq * head_dim is one layer of a contiguous GpuKvCache.
 void GpuKvReadPaged(const GpuPagedKv& kv, const GpuPageTable& table, const int32_t* seq_ids,
                     const int32_t* positions, int64_t n_tokens, bool out_f32, void* k_out, void* v_out,

@@ -95,6 +95,34 @@ def test_read_into_the_contiguous_cache(gpu):
     assert torch.equal(a, b)
 
 
+def test_read_into_one_buffer(gpu):
+    """Keys and values of a token, or of a head, one behind the other in one buffer, or with as much room between."""
+    import torch
+
+    from test_paged_args import shifted_reads
+
+    rng = np.random.default_rng(6)
+    n_kv, d, n = 2, 64, 3
+    pages = Pages(rng, F16, n_kv, d, 16, [n])
+    kv, table = pages.device(gpu)
+    k, v = rows(rng, n, n_kv, d), rows(rng, n, n_kv, d)
+    pos, seq = dev(np.arange(n), np.int32), dev(np.zeros(n), np.int32)
+    gpu.GpuKvWritePaged(kv, table, seq, pos, dev(k), dev(v), n)
+    apart = [c for c in shifted_reads(d, n, n_kv) if not c[-1]]
+    assert len(apart) > 100
+    for shift, ts, hs, f32, _ in apart:
+        dtype, size = (torch.float32, 4) if f32 else (torch.float16, 2)
+        buf = torch.full((8192,), 7.0, dtype=dtype, device="cuda")
+        at = [2048, 2048 + shift // size]
+        gpu.GpuKvReadPaged(kv, table, seq, pos, n, buf[at[0]:], buf[at[1]:], ts, hs)
+        want = np.full(8192, 7, np.float32)
+        for x, first in zip((k, v), at):
+            for t in range(n):
+                for h in range(n_kv):
+                    want[first + t * ts + h * hs:][:d] = x[t, h].astype(np.float16)
+        assert np.array_equal(host(buf).astype(np.float32), want)
+
+
 def test_values_at_the_ends_of_the_range(gpu):
     """Rows of zeros, of subnormals, of the largest numbers, with ties, infinities and NaN in them."""
     d = 64

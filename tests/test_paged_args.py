@@ -194,6 +194,30 @@ def test_buffers_that_overlap_or_lie_askew_are_refused(ops):
             ops.GpuAttentionPaged(kv, t, FAKE, q, 16, 2, out, 1 << 41, seq_ids=FAKE, workspace_bytes=need)
 
 
+def shifted_reads(d=64, n=3, n_kv=2):
+    """(bytes from k_out to v_out, token and head stride in elements, fp32, whether two of their rows share an element) of
+    outputs that lie in one another."""
+    for ts, hs in ((n_kv * d, d), (2 * n_kv * d, d), (2 * n_kv * d, 2 * d), (d, 4 * d), (2 * d, 16 * d), (n_kv * d + 8, d)):
+        rows = [t * ts + h * hs for t in range(n) for h in range(n_kv)]
+        for f32 in (False, True):
+            size = 4 if f32 else 2
+            for apart in range(-(rows[-1] + 2 * d) * size, (rows[-1] + 2 * d) * size, 16):
+                shift = apart // size
+                if apart:
+                    yield apart, ts, hs, f32, any(abs(a + shift - b) < d for a in rows for b in rows)
+
+
+def test_read_refuses_outputs_whose_rows_overlap(ops):
+    kv, t = views(ops, shape=(10, 2, 16, 64))
+    far, seen = 1 << 40, 0
+    for apart, ts, hs, f32, meet in shifted_reads():
+        if meet:
+            seen += 1
+            with pytest.raises(ops.RpgError, match="rows of k_out and v_out overlap"):
+                ops.GpuKvReadPaged(kv, t, FAKE, FAKE, 3, far, far + apart, ts, hs, out_f32=f32)
+    assert seen > 500
+
+
 def test_other_devices_are_refused(ops):
     import torch
 
