@@ -895,6 +895,9 @@ class GpuPagedKv:
 
     def __init__(self, k, v, k_scale=None, v_scale=None, shape=None, kv_type=None):
         torch = _t()
+        raw = {isinstance(t, int) for t in (k, v, k_scale, v_scale) if t is not None}
+        if k is None or v is None or len(raw) > 1:
+            raise RpgError("GpuPagedKv: k, v and their scales are all tensors or all raw addresses")
         if isinstance(k, int):
             if shape is None or kv_type not in (KV_F16, KV_Q8):
                 raise RpgError("GpuPagedKv: raw addresses need shape and kv_type")

@@ -269,6 +269,18 @@ def test_python_views_check_their_tensors(ops):
         ops.GpuPageTable(torch.zeros(4, 2, dtype=torch.int32))
 
 
+def test_pages_are_all_tensors_or_all_raw_addresses(ops):
+    import torch
+
+    k = torch.zeros(4, 2, 16, 64, dtype=torch.int8)
+    s = torch.zeros(4, 2, 16)
+    for args in ((k, k, FAKE, FAKE), (k, k, s, FAKE), (k, FAKE, s, s), (FAKE, k, FAKE, FAKE), (FAKE, FAKE, s, s),
+                 (FAKE, FAKE, FAKE, s), (k, None, s, s), (None, None)):
+        for given in ({}, dict(shape=(4, 2, 16, 64), kv_type=ops.KV_Q8)):
+            with pytest.raises(ops.RpgError, match="all tensors or all raw addresses"):
+                ops.GpuPagedKv(*args, **given)
+
+
 def test_pages_go_with_their_view(ops):
     """Nothing that a view holds holds the view: the pages' memory is free when it goes, without a collection."""
     import gc
