@@ -462,6 +462,39 @@ def test_a_batch_is_served(gpu, ora, kind, n_kv, group, page):
 
 
 @pytest.mark.parametrize("kind", [F16, Q8])
+def test_prompts_of_head_64_are_served_a_row_a_token(gpu, kind):
+    """Heads of 64: a prompt and a later turn of two conversations written into pages, each token attending as a row of
+    its own to the positions up to it (the contiguous attention serves heads of 128 alone)."""
+    import torch
+
+    rng = np.random.default_rng(37)
+    heads, n_kv, d, eps, room = 8, 2, 64, 1e-6, 128
+    turns = [([0, 0], [50, 33]), ([50, 33], [7, 20])]  # positions held before, and new ones
+    pages = Pages(rng, kind, n_kv, d, 16, [57, 53])
+    kv, table = pages.device(gpu)
+    tab = dev(gpu.build_rope_table(d, 1e6, room))
+    qw, kw = dev((1 + 0.3 * rng.normal(0, 1, (2, d))).astype(np.float32))
+    work = workspace(gpu, heads, n_kv, d)
+    for past, new in turns:
+        seqs = np.repeat([0, 1], new)
+        at = np.concatenate([p + np.arange(m) for p, m in zip(past, new)])
+        n = len(at)
+        q, k, v = (dev(rng.normal(0, 1, (n, h, d)).astype(np.float32)) for h in (heads, n_kv, n_kv))
+        seq, pos, out = dev(seqs, np.int32), dev(at, np.int32), torch.empty_like(q)
+        gpu.GpuQkNormRopeKvPaged(kv, table, seq, pos, q, k, v, qw, kw, heads, tab, room, n, eps, q)
+        gpu.GpuAttentionPaged(kv, table, pos + 1, q, heads, n, out, work, seq_ids=seq)
+        torch.cuda.synchronize()
+        for name, t in zip(("k", "v", "ks", "vs"), kv.tensors):
+            if t is not None:
+                a = host(t)
+                setattr(pages, name, a.view(np.uint16) if a.dtype == np.int16 else a)
+        check(host(out), pages, list(at + 1), host(q), list(seqs))
+    layer = torch.zeros((2, n_kv, room, d), dtype=torch.int16, device="cuda")
+    with pytest.raises(gpu.RpgError, match="supports head_dim 128"):
+        gpu.GpuAttentionFromCache(heads, n_kv, d, 0, q, n, layer[0], layer[1], room, out)
+
+
+@pytest.mark.parametrize("kind", [F16, Q8])
 def test_captured_steps_of_a_batch(gpu, kind):
     """A step of a batch as one graph: norm, rotation and write, then attention, with positions and lengths counted up in
     it. Replays, with eager calls of the same operators on other buffers in between, give the eager steps' bits."""
