@@ -84,7 +84,11 @@ typedef struct {
                      int64_t token_stride, int64_t head_stride);
 
   /* Row r of q ([n_rows][n_heads][head_dim]) attends to positions [0, lens[r]) of
-   * its sequence; length 0 gives zeros. A captured call holds for any lengths,
+   * its sequence; length 0 gives zeros. Scores, weights and sums have fp32's
+   * precision, with three limits: what a query holds below 2^-30 of its row's largest
+   * element does not count; values past 2^93 may add up to an infinity; an infinite
+   * value of a weight below 2^-23 of the largest may give NaN in place of the
+   * infinity. A captured call holds for any lengths,
    * tables and seq_ids at replay. out must not overlap q. Calls that may run at
    * the same time need a workspace each. Beside rpg_op_attention_from_cache. */
   int32_t (*attention)(const rpg_paged_kv_t* kv, const rpg_page_table_t* table, const int32_t* seq_ids,

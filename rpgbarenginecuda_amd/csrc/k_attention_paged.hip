@@ -45,20 +45,22 @@
 // workgroup they join in LDS, and where it is split over workgroups each leaves its
 // part in the workspace and the last to arrive joins them, in order.
 //
-// Measured (kernel times; "units" as above): 32 rows of up to 4096 positions in fp16,
-// 16 / 8 heads, 269 MB: 50.7 us, 5.3 TB/s; 128 rows of up to 8192 in 8 bits, 32 / 8
-// heads, 1152 MB: 189 us, 6.1 TB/s (fp16, 2230 MB: 357 us, 6.2 TB/s), where a pure
-// read of as much reaches 7.0. While all workgroups run the reads come at about that
+// Measured (the kernel between events that its dispatch carries, as every time in this
+// file): 32 rows of up to 4096 positions in fp16, 16 / 8 heads, 269 MB: 50.3 us,
+// 5.3 TB/s; 128 rows of up to 8192 in 8 bits, 32 / 8 heads, 1152 MB: 189.5 us, 6.1
+// TB/s (fp16, 2230 MB: 355 us, 6.3 TB/s); 16 rows of 4000 in 8 bits, 64 / 8 heads, two
+// column tiles, 136 MB: 35.0 us, 3.9 TB/s; where a pure read of as much reaches 7.0. While all workgroups run the reads come at about that
 // rate; the rest is the end, where every other XCD is a tenth slower and of a compute
 // unit's two workgroups the one whose loads come behind a fifth. Shares to match gained
 // a few percent on ragged batches and lost as much where equal shares split no row
 // (64 x 4096 positions from 93 to 100 us), and dealing the last fifth out late, in
 // shares of their own, cost what it gained.
-// One row of 32768 positions in 8 bits, 8 kv heads, 69 MB: 21.1 us, of which about
-// ten read at full rate; 1 x 500 positions 8.9 us and 1 x 60 7.0 us are the chain of
-// round trips: lengths 0.5, the search for the share 0.7, page table 0.2, keys 1.5,
-// products and weights 1.9, join in LDS 0.6 and, where a pair is split, store and
-// count 1.3 and the last one's read and join 1.5.
+// 1 x 500 positions, 9 us, and 1 x 60, 7.0 us, are the chain of round trips: lengths
+// 0.5, the search for the share 0.7, page table 0.2, keys 1.5, products and weights
+// 1.9, join in LDS 0.6 and, where a pair is split, store and count 1.3 and the last
+// one's read and join 1.5. One row of 32768 positions in 8 bits, 8 kv heads, 69 MB:
+// 20.5 us, that chain with a join of 32 parts at its end and 10.7 us of reading in its
+// middle (each further 32768 positions take 10.7 us, 6.5 TB/s, up to 262144: 95 us).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -75,8 +77,8 @@ namespace {
 using dev::PagedView;
 
 // Four waves of up to 17 KB of keys and values each: two workgroups to a compute unit. (Eight waves and one workgroup
-// were slower on short calls, 1 x 500 positions 12.1 against 10.5 us, and alike on long ones; four waves and one
-// workgroup with two steps under way each were slower on long ones.)
+// were slower on short calls, 1 x 500 positions by 15%, and alike on long ones; four waves and one workgroup with two
+// steps under way each were slower on long ones.)
 constexpr int kWaves = 4;
 constexpr int kTileHeads = 8;
 // Workgroups at most; a workspace has two part slots and a counter for each.
@@ -84,7 +86,7 @@ constexpr int kMaxGroups = 512;
 // Bytes between two counters: on lines of their own, as the decode attention's.
 constexpr size_t kCounterBytes = 256;
 // Stores of a part to the workspace: device scope. With the streaming hint too their
-// acknowledgement came later (1 x 32768 positions of one kv head 24.2 against 21.7 us).
+// acknowledgement comes later (1 x 32768 positions in fp16 of one kv head 17.8 against 16.6 us).
 constexpr int kPartPolicy = 16;
 
 using Half2 = _Float16 __attribute__((ext_vector_type(2)));
@@ -172,7 +174,7 @@ __device__ __forceinline__ uint32_t LdsAddress(const void* p) {
 }
 // kN times 16 bytes a lane from rs: time i from byte off[i % kOff] + 1024 i, lane j's to LDS address `to` + 1024 i +
 // 16 j (an instruction's offset counts on both sides). What is read once is loaded with the streaming hint: without it
-// 32 x 4096 positions took 59 us and not 53, 128 x 8192 236 and not 211. M0 holds the
+// 32 x 4096 positions take 55.4 us and not 50.0, 128 x 8192 in 8 bits 214 and not 190. M0 holds the
 // LDS address: an operand, so that the compiler writes it and knows what is there. It is read one wait state after it is
 // written; five are waited, which M0 and a resource need where a vector instruction wrote them.
 template <int kN, int kOff>
@@ -242,8 +244,8 @@ __device__ __forceinline__ uint32_t Scalar(uint32_t x) { return __builtin_amdgcn
 // a unit, so that all workgroups get alike. With fewer, joining what two workgroups hold of a pair (a round trip to memory
 // to store, one to count, one to read) costs more than some units more in turn: a pair of up to kWholeUnits is one item, a
 // longer one is cut evenly into items of at most 2^step, about what each workgroup then gets.
-// (One row of 250 positions, 8 units for each of 8 kv heads: 9.0 us whole, 9.9 in two items each; of 500, 16 units: 11.6
-// whole, 10.5 in four items each.)
+// (One row of 250 positions, 8 units for each of 8 kv heads: 8.1 us whole, 9.1 in two items each; of 500, 16 units: 10.3
+// whole, 9.6 in four items each.)
 constexpr uint32_t kManyUnits = 8192;
 constexpr uint32_t kWholeUnits = 8;
 constexpr uint32_t kLeastStep = 2;
@@ -464,8 +466,9 @@ struct HeadsOf {
   }
 };
 
-// A pair of up to kJoinAtOnce parts is joined in one step; of more in two, each kFan parts in the first. (One step of 256
-// parts took 34 us of a call where two take 22; at 64 parts they are alike.)
+// A pair of up to kJoinAtOnce parts is joined in one step; of more in two, each kFan parts in the first. (In one step, 256
+// parts of 1 x 32768 positions of one kv head make 49.5 us of 16.6, 128 of 1 x 65536 of two 26.9 of 20.4; at 64 parts
+// they were alike.)
 constexpr uint32_t kJoinAtOnce = 32;
 constexpr uint32_t kFan = 16;
 
@@ -697,7 +700,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Att
     };
 
     // of a compute unit's two workgroups the second waits behind the first wherever both have something to issue: going
-    // first there, it ends sooner (128 x 8192 positions in 8 bits 200.4 -> 195.4 us; other calls within a percent)
+    // first there, it ends sooner (128 x 8192 positions in 8 bits 195.2 -> 190.4 us; other calls within a percent)
     if (me >= gridDim.x / 2) __builtin_amdgcn_s_setprio(1);
     find();
     load_k();
@@ -1432,8 +1435,10 @@ void GpuAttentionPaged(const GpuPagedKv& kv, const GpuPageTable& table, const in
   RPG_CHECK(n_rows <= 0x7FFFFFFF / most / rows.pairs,
             "AttentionPaged: %lld rows of up to %lld positions and %d heads are too many for one call",
             static_cast<long long>(n_rows), static_cast<long long>(rows.capacity), rows.pairs);
-  // no more workgroups than the longest possible rows would give work to; for a few rows one to a compute unit, since more
-  // parts of a row cost more to join than the card gives for them (1 x 32768 positions, 8 kv heads: 22.7 against 25.0 us)
+  // no more workgroups than the longest possible rows would give work to; for a few pairs one to a compute unit, since more
+  // parts of a pair cost more to join, at any length, than the card gives for them. With two to a compute unit instead, 8 pairs of one row in 8 bits: of 32768 positions 21.8 us against 20.5, of 131072 54.2
+  // against 52.5, of 262144 97.5 against 95.1 (fp16 173 against 170); one pair of 262144 23.9 against 21.8; 15 of 32768
+  // 31.2 against 29.3 (fp16 49.2 against 50.0)
   const int64_t all_pairs = n_rows * rows.pairs;
   const int64_t at_once = all_pairs * kJoinAtOnce < kMaxGroups ? kMaxGroups / 2 : kMaxGroups;
   const int64_t groups = std::min<int64_t>(at_once, all_pairs * ((most + (1 << kLeastStep) - 1) >> kLeastStep));

@@ -54,7 +54,7 @@ bool Aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 
 // Workgroups go to the eight XCDs in turn. Each XCD takes one stretch of the tokens
 // instead of every eighth workgroup, so that neighbouring slots, and the 32 scales in
-// a line of them, meet in one L2: 16.2 -> 14.9 us for 8 x 1024 tokens written as 8 bits.
+// a line of them, meet in one L2: 16.0 -> 15.1 us for 8 x 1024 tokens written as 8 bits.
 __device__ __forceinline__ uint32_t WorkgroupInStretch() {
   const uint32_t x = blockIdx.x & 7, each = gridDim.x >> 3, rest = gridDim.x & 7;
   return x * each + (x < rest ? x : rest) + (blockIdx.x >> 3);
@@ -195,8 +195,9 @@ struct RowOf {
 // Plain loads, since the projections before this kernel have just written q, k and v;
 // nontemporal stores of the queries; plain stores of the cache's rows, whole lines with
 // 16 bytes a lane. Measured at 2811 tokens of 16 + 8 + 8 heads into 8 bits, 75 MB:
-// 14.0 us = 5.4 TB/s; with nontemporal loads 17.0, with plain stores of the queries
-// 14.5, with write-through ones 15.8; held to 64 registers (spills) twice as long.
+// 14.2 us = 5.3 TB/s; with nontemporal loads 17.2, with plain stores of the queries
+// 16.0, with write-through ones a tenth more; held to 64 registers (spills) twice as long.
+// (Times in this file: the kernel between events that its dispatch carries.)
 // One argument: a launch takes longer for every pointer among its arguments (nine of them, 0.5 us of host time).
 struct WriteArgs {
   PagedView view;
@@ -331,8 +332,8 @@ __device__ __forceinline__ void StoreRead(void* out, int64_t at, const float (&x
 }
 
 // One work unit per (token, kv head): a lane moves 16 bytes of output of its key and
-// of its value row. Plain loads and nontemporal stores: 10.5 us for 6 x 700 tokens of
-// 8 fp16 heads (52 MB, 4.9 TB/s); with nontemporal loads 12.0, with plain stores 11.4.
+// of its value row. Plain loads and nontemporal stores: 10.4 us for 6 x 700 tokens of
+// 8 fp16 heads (52 MB, 5.0 TB/s); with nontemporal loads 12.7, with plain stores 11.0.
 struct ReadArgs {
   PagedView view;
   const int32_t* seq_ids;

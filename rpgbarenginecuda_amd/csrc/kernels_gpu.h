@@ -315,10 +315,17 @@ void GpuKvReadPaged(const GpuPagedKv& kv, const GpuPageTable& table, const int32
 // head h / (n_heads / n_kv_heads). A row of length 0 gives zeros; padding
 // (negative seq_id) leaves its out row as it was; a length below 0 or past the
 // table's row, a sequence out of range, or a page out of range among the row's
-// positions gives NaN. (An infinite value whose weight is below 2^-23 of the
-// largest may give NaN instead of the infinity.) out must not overlap q. The work is shared out on the
+// positions gives NaN. out must not overlap q. The work is shared out on the
 // device from the lengths themselves, so a captured call holds for any lengths,
-// tables and seq_ids that stand there at replay.
+// tables and seq_ids that stand there at replay. A call whose rows have room for
+// 2^31 units (32 positions of a kv head and 8 of its query heads) is refused.
+//
+// Scores, weights and sums have fp32's precision, within these limits: of a query,
+// what is below 2^-30 of its row's largest element (fp16 pages: 2^-38) does not
+// count; a weight below 2^-120 of the row's largest may count as none; weights times
+// values that add up to more than fp32 holds before the sum of weights divides them
+// (values past 2^93) may give an infinity; an infinite value whose weight is below
+// 2^-23 of the largest may give NaN instead of the infinity.
 //
 // workspace: GpuAttentionPagedWorkspaceBytes of device memory, 256-byte aligned,
 // whose bytes are zero before the first call (GpuAttentionPagedWorkspaceInit
