@@ -726,7 +726,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Att
     Half8 qh[kQ8 ? 1 : kSteps];
     I32x4 qi[kQ8 ? kTiles : 1][kQ8 ? kSteps : 1];
     float to_score[kTiles], m, l;
-    int key_exp = 0;  // 8-bit keys: the power of two that their scales are multiplied by, of the lane's tile
+    int key_exp = 0;  // 8-bit keys: the power of two that their scales are multiplied by, for the lane's tile
     // 8-bit values: the power of two (times what m moved by since) that acc holds them multiplied by; infinity where that
     // is nothing yet
     float shrink = INFINITY;
@@ -770,11 +770,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Att
         }
         top = MaxAcrossRows(top);
         if constexpr (kQ8) {
-          // the power of two that brings top to [2^29, 2^30), taken back with the keys' scales: a product of a query that is
-          // far from 1 and of one code need not be an fp32 number
+          // the power of two that brings top to [2^29, 2^30), taken back with the products where these stay in fp32's range
+          // (below 2^43 before it), and what is left of it for queries far from 1 with the keys' scales
           const int by = 30 - __builtin_amdgcn_frexp_expf(top);
-          if (kTiles == 1 || second == (t == 1)) key_exp = -by;
-          to_score[t] = scale_log2 * digit_by + SumAcrossRows(odd);
+          const int back = min(max(-by, -80), 80);
+          if (kTiles == 1 || second == (t == 1)) key_exp = -by - back;
+          to_score[t] = ldexpf(scale_log2 * digit_by, back) + SumAcrossRows(odd);
 #pragma unroll
           for (int s = 0; s < kSteps; ++s) {
 #pragma unroll

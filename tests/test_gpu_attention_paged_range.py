@@ -111,6 +111,23 @@ def test_queries_and_keys_far_from_one(gpu, heads, d):
     check(gpu, Q8, q.astype(np.float32), ks, vs)
 
 
+@pytest.mark.parametrize("heads,d", [(2, 128), (8, 128), (1, 64), (5, 64)])
+def test_large_queries_and_keys_in_elements_apart(gpu, heads, d):
+    """Queries of 2^120 in one half of the elements and 8-bit keys of 2^100 in the other: every score is 0, every weight
+    1 / n, and the outputs are the values' means to within n + 64 roundings and the values' own rounding to 2^-24."""
+    rng = np.random.default_rng(heads + d + 4)
+    n = 150
+    k, q = np.zeros((n, 1, d)), np.zeros((1, heads, d), np.float32)
+    k[:, :, d // 2:] = rng.normal(0, 1, (n, 1, d // 2)) * 2.0 ** 100
+    q[:, :, :d // 2] = rng.normal(0, 1, (1, heads, d // 2)) * 2.0 ** 120
+    pages = Pages(rng, Q8, 1, d, 16, [n])
+    hold(pages, 0, k, rng.normal(0, 1, (n, 1, d)))
+    kv, table = pages.device(gpu)
+    got = attend(gpu, kv, table, [n], q)
+    v = pages.rows("v", 0, n)[:, 0]
+    assert np.all(np.abs(got[0] - v.mean(0)) <= (n + 64 + 2) * 2.0 ** -24 * np.abs(v).max(-1).mean())
+
+
 @pytest.mark.parametrize("kind", [F16, Q8])
 @pytest.mark.parametrize("heads,d", [(2, 128), (8, 128), (4, 64)])
 def test_many_small_weights_beside_a_large_one(gpu, heads, d, kind):
