@@ -1437,7 +1437,7 @@ void GpuAttentionPaged(const GpuPagedKv& kv, const GpuPageTable& table, const in
             "AttentionPaged: %lld rows of up to %lld positions and %d heads are too many for one call",
             static_cast<long long>(n_rows), static_cast<long long>(rows.capacity), rows.pairs);
   // no more workgroups than the longest possible rows would give work to; for a few pairs one to a compute unit, since more
-  // parts of a pair cost more to join, at any length, than the card gives for them. With two to a compute unit instead, 8 pairs of one row in 8 bits: of 32768 positions 21.8 us against 20.5, of 131072 54.2
+  // parts of a pair cost more to join than the card gives for them, also at great lengths. With two to a compute unit instead, 8 pairs of one row in 8 bits: of 32768 positions 21.8 us against 20.5, of 131072 54.2
   // against 52.5, of 262144 97.5 against 95.1 (fp16 173 against 170); one pair of 262144 23.9 against 21.8; 15 of 32768
   // 31.2 against 29.3 (fp16 49.2 against 50.0)
   const int64_t all_pairs = n_rows * rows.pairs;
