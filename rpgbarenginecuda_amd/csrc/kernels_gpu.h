@@ -143,6 +143,28 @@ class GpuKvCache {
 // n_pos = min(max_pos, context_length), at least 1.
 std::vector<float> BuildRopeTable(int32_t head_dim, double theta, int64_t n_pos);
 
+// The same for contexts longer than the model was trained on. With w_i = 1 /
+// theta^(2i / rot_dim), the frequency of pair i is
+//   kRopePlain   w_i (BuildRopeTable's bits);
+//   kRopeLinear  w_i / factor, as if positions were divided;
+//   kRopeNtk     w_i of theta * factor^(rot_dim / (rot_dim - 2)) (rot_dim 2: w_i),
+//                so that the slowest pair's is divided and the fastest one's stays;
+//   kRopeYarn    w_i (r / factor + 1 - r), r rising from 0 to 1 between the pairs that
+//                turn beta_fast and beta_slow times over the original positions (their
+//                indices floored and rounded up; Peng et al., YaRN, 2023).
+// cos and sin are multiplied by `attention`, or where that is 0 by 0.1 ln(factor) + 1
+// (kRopeYarn) or 1. The table serves every operator that takes one.
+enum RopeScalingType : uint32_t { kRopePlain = 0, kRopeLinear = 1, kRopeNtk = 2, kRopeYarn = 3 };
+struct RopeScaling {
+  uint32_t type = kRopePlain;
+  double factor = 1.0;  // at least 1
+  int64_t original_positions = 0;
+  double beta_fast = 32.0;
+  double beta_slow = 1.0;
+  double attention = 0.0;
+};
+std::vector<float> BuildRopeTableScaled(int32_t rot_dim, double theta, int64_t n_pos, const RopeScaling& scaling);
+
 // ---------------------------------------------------------------- reference operators
 
 void GpuDequantRow(uint32_t type, const uint8_t* src_dev, int64_t n_elems, float* dst_dev);
@@ -161,6 +183,20 @@ void GpuSiluMulInPlace(float* gate_dev, const float* up_dev, int64_t n);
 void GpuVecAddInPlace(float* a_dev, const float* b_dev, int64_t n);
 
 void GpuEmbeddingLookup(const GpuTensor& emb, const int32_t* toks_dev, int64_t seq, float* x_dev);
+
+// GpuRope for rows at any positions and in any of the usual forms, queries and keys
+// in one launch: q_out <- q ([n_rows][n_heads][head_dim]) and k_out <- k
+// ([n_rows][n_kv_heads][head_dim]), where the first rot_dim elements of a head are
+// rotated in pairs (i, i + rot_dim / 2), interleaved (2i, 2i + 1), by
+//   a <- a cos - b sin,  b <- b cos + a sin
+// with row positions[r] of rope_tab ([rope_rows][rot_dim], cos | sin), and the others
+// copied. A position outside [0, rope_rows) gives NaN in the rotated elements. An
+// output may be its input; else it must overlap neither an input nor the other
+// output. k and k_out may be null with n_kv_heads 0. No counterpart in the reference,
+// whose rows stand at consecutive positions (src/kernels_gpu.h:71-72).
+void GpuRopeRows(const float* q, const float* k, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
+                 int32_t rot_dim, bool interleaved, const float* rope_tab, int64_t rope_rows,
+                 const int32_t* positions, int64_t n_rows, float* q_out, float* k_out);
 
 // ---------------------------------------------------------------- fused operators
 

@@ -1,4 +1,5 @@
 // GpuKvCache storage and the host-built RoPE table.
+#include <algorithm>
 #include <cmath>
 #include <cstdio>
 #include <limits>
@@ -64,21 +65,55 @@ std::string GpuKvCache::Describe() const {
 // it in the last double bit for about a third of the i, which moves some fp32 table
 // entries at positions past ~6500.
 std::vector<float> BuildRopeTable(int32_t head_dim, double theta, int64_t n_pos) {
-  RPG_CHECK(head_dim > 0 && head_dim % 2 == 0, "RoPE needs an even head size, got %d", head_dim);
+  return BuildRopeTableScaled(head_dim, theta, n_pos, RopeScaling());
+}
+
+std::vector<float> BuildRopeTableScaled(int32_t rot_dim, double theta, int64_t n_pos, const RopeScaling& scaling) {
+  RPG_CHECK(rot_dim > 0 && rot_dim % 2 == 0, "RoPE needs an even head size, got %d", rot_dim);
   RPG_CHECK(theta > 0.0, "RoPE base theta must be positive, got %g", theta);
+  const uint32_t type = scaling.type;
+  const double factor = scaling.factor;
+  RPG_CHECK(type <= kRopeYarn, "RoPE scaling %u is none of plain, linear, NTK and YaRN", type);
+  RPG_CHECK(type == kRopePlain || (factor >= 1.0 && std::isfinite(factor)), "RoPE scaling factor %g is not 1 or more",
+            factor);
+  RPG_CHECK(scaling.attention >= 0.0 && std::isfinite(scaling.attention), "RoPE attention factor %g is out of range",
+            scaling.attention);
   const int64_t rows = n_pos > 0 ? n_pos : 1;
-  const int32_t pairs = head_dim / 2;
+  RPG_CHECK(rows <= (int64_t(1) << 40) / rot_dim, "a RoPE table of %lld positions is too large",
+            static_cast<long long>(rows));
+  const int32_t pairs = rot_dim / 2;
+  const double base =
+      type == kRopeNtk && rot_dim > 2 ? theta * std::pow(factor, static_cast<double>(rot_dim) / (rot_dim - 2)) : theta;
+  double from = 0.0, to = 0.0;  // YaRN: the pairs that the ramp lies between
+  if (type == kRopeYarn) {
+    RPG_CHECK(scaling.original_positions > 0 && scaling.beta_slow > 0.0 && scaling.beta_fast >= scaling.beta_slow &&
+                  std::isfinite(scaling.beta_fast) && theta > 1.0,
+              "YaRN needs the original number of positions, 0 < beta_slow <= beta_fast and theta above 1");
+    const auto pair_of = [&](double turns) {
+      return rot_dim * std::log(static_cast<double>(scaling.original_positions) / (turns * 2.0 * M_PI)) /
+             (2.0 * std::log(theta));
+    };
+    from = std::max(std::floor(pair_of(scaling.beta_fast)), 0.0);
+    to = std::min(std::ceil(pair_of(scaling.beta_slow)), rot_dim - 1.0);
+  }
   std::vector<double> freq(static_cast<size_t>(pairs));
   for (int32_t i = 0; i < pairs; ++i) {
-    freq[static_cast<size_t>(i)] = 1.0 / std::pow(theta, static_cast<double>(2 * i) / static_cast<double>(head_dim));
+    double w = 1.0 / std::pow(base, static_cast<double>(2 * i) / static_cast<double>(rot_dim));
+    if (type == kRopeLinear) w /= factor;
+    if (type == kRopeYarn) {
+      const double r = std::min(std::max((i - from) / std::max(to - from, 0.001), 0.0), 1.0);
+      w = w / factor * r + w * (1.0 - r);
+    }
+    freq[static_cast<size_t>(i)] = w;
   }
-  std::vector<float> tab(static_cast<size_t>(rows * head_dim));
+  const double by = scaling.attention != 0.0 ? scaling.attention : type == kRopeYarn ? 0.1 * std::log(factor) + 1.0 : 1.0;
+  std::vector<float> tab(static_cast<size_t>(rows * rot_dim));
   float* out = tab.data();
-  for (int64_t p = 0; p < rows; ++p, out += head_dim) {
+  for (int64_t p = 0; p < rows; ++p, out += rot_dim) {
     for (int32_t i = 0; i < pairs; ++i) {
       const double angle = static_cast<double>(p) * freq[static_cast<size_t>(i)];
-      out[i] = static_cast<float>(std::cos(angle));
-      out[pairs + i] = static_cast<float>(std::sin(angle));
+      out[i] = static_cast<float>(by * std::cos(angle));
+      out[pairs + i] = static_cast<float>(by * std::sin(angle));
     }
   }
   return tab;

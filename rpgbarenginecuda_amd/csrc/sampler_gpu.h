@@ -25,6 +25,7 @@
 #ifndef RPG_AMD_SAMPLER_GPU_H_
 #define RPG_AMD_SAMPLER_GPU_H_
 
+#include <cstddef>
 #include <cstdint>
 
 namespace rpg {
@@ -68,6 +69,48 @@ void GpuSampleTokenDev(const float* logits_dev, int64_t n, const SampleOptions& 
 // Allocates the sampler's scratch block; call once before capturing a graph
 // that samples or takes an argmax (reference src/sampler_gpu.h:130).
 void GpuSamplerWarmup();
+
+// ---------------------------------------------------------------- a batch's next tokens
+//
+// One token for each row of logits ([n_rows], row_stride floats apart, n of them), from
+// a given random number for each. Beside GpuSampleTokenDev, whose u is
+// DevCounterUniform's; no counterpart in the reference, which samples one row.
+//
+// Semantics: tokens are ordered by falling logit, equal ones by rising index. With
+// weights w = exp((x - max x) / temperature), kept are
+//   * the first top_k in that order (0 < top_k; else all), ties cut by index (the one-row
+//     sampler keeps all that are tied with the k-th),
+//   * of these the fewest first ones whose weight is at least top_p times that of all
+//     of these (0 < top_p < 1; else all),
+//   * of these those of w >= min_p (0 < min_p, above 1 as 1; else all).
+// The token is the first in index order up to which the kept weights add up to more
+// than u times their sum. u is taken into [0, 1), a NaN as 0. temperature <= 0 or NaN
+// takes the first in order, with probability 1. A NaN logit counts as minus infinity,
+// whose weight is 0; a row of nothing else gives token -1 and probability 0. Where the
+// largest is plus infinity all others weigh 0.
+//
+// Weights are formed in double (within 2^-50 of their value) and summed as integers of
+// 2^-s, s = 62 - ceil(log2 n), so that no order of summing shows and ties add up to
+// what they should: borders lie within n 2^-(s+1) of where exact weights have them.
+struct SampleBatchOptions {
+  // device arrays of n_rows, each may be null: 1, off, off, off
+  const float* temperature = nullptr;
+  const int32_t* top_k = nullptr;
+  const float* top_p = nullptr;
+  const float* min_p = nullptr;
+};
+
+// probs_dev (may be null): the token's share of the kept weight. All arrays are read on
+// the device: a captured call holds for what stands there at replay. workspace:
+// GpuSampleBatchWorkspaceBytes of device memory, 256-byte aligned, whose bytes are zero
+// before the first call (GpuSampleBatchWorkspaceInit does that); each call leaves it
+// ready for the next on the same stream, of any n_rows and n that need no more. Calls
+// that may run at the same time need a workspace each.
+void GpuSampleBatch(const float* logits_dev, int64_t n_rows, int64_t n, int64_t row_stride,
+                    const SampleBatchOptions& opt, const float* u_dev, int32_t* tokens_dev, float* probs_dev,
+                    void* workspace, size_t workspace_bytes);
+size_t GpuSampleBatchWorkspaceBytes(int64_t n_rows, int64_t n);
+void GpuSampleBatchWorkspaceInit(void* workspace, size_t bytes);
 
 }  // namespace rpg
 

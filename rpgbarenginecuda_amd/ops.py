@@ -135,12 +135,30 @@ class PagedOpsC(ctypes.Structure):
                 ("attention_workspace_init", ctypes.CFUNCTYPE(_i32, _vp, _i64))]
 
 
+class RopeScalingC(ctypes.Structure):
+    """rpg_rope_scaling_t (include/rpg_batch.h)."""
+    _fields_ = [("type", _u32), ("factor", _f64), ("original_positions", _i64), ("beta_fast", _f64),
+                ("beta_slow", _f64), ("attention", _f64)]
+
+
+class BatchOpsC(ctypes.Structure):
+    """rpg_batch_ops_t: the table of functions for a step of many conversations (include/rpg_batch.h)."""
+    _fields_ = [("size", _i64),
+                ("rope_table", ctypes.CFUNCTYPE(_i32, _i32, _f64, _i64, _vp, _vp)),
+                ("rope_rows", ctypes.CFUNCTYPE(_i32, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _i64, _vp, _i64, _vp,
+                                               _vp)),
+                ("sample", ctypes.CFUNCTYPE(_i32, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64)),
+                ("sample_workspace", ctypes.CFUNCTYPE(_i64, _i64, _i64)),
+                ("sample_workspace_init", ctypes.CFUNCTYPE(_i32, _vp, _i64))]
+
+
 class RpgError(RuntimeError):
     """An operator rejected its arguments or a HIP call failed."""
 
 
 _lib: Optional[ctypes.CDLL] = None
 _paged: Optional[PagedOpsC] = None
+_batch: Optional[BatchOpsC] = None
 
 
 def load_library() -> ctypes.CDLL:
@@ -173,6 +191,17 @@ def paged_ops() -> PagedOpsC:
             raise RpgError(f"rpg_paged_ops holds {table.size} bytes, {ctypes.sizeof(PagedOpsC)} are needed")
         _paged = table
     return _paged
+
+
+def batch_ops() -> BatchOpsC:
+    """The library's table of functions for a step of many conversations (rpg_batch_ops)."""
+    global _batch
+    if _batch is None:
+        table = BatchOpsC.in_dll(load_library(), "rpg_batch_ops")
+        if table.size < ctypes.sizeof(BatchOpsC):
+            raise RpgError(f"rpg_batch_ops holds {table.size} bytes, {ctypes.sizeof(BatchOpsC)} are needed")
+        _batch = table
+    return _batch
 
 
 def _check(rc: int) -> int:
@@ -1066,6 +1095,96 @@ def GpuAttentionPaged(kv: GpuPagedKv, table: GpuPageTable, lens, q, n_heads: int
         kv.ref, table.ref, int_at(seq_ids, 4 * n_rows, "seq_ids"), int_at(lens, 4 * n_rows, "lens"),
         float_at(q, span, "q"), n_heads, n_rows, float_at(out, span, "out"),
         kv.at(dtype)(workspace, workspace_bytes, "workspace"), workspace_bytes))
+
+
+# ----------------------------------------------------------------------------- a step of many conversations
+
+ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
+
+
+def build_rope_table_scaled(rot_dim: int, theta: float, n_pos: int, scaling: str = "none", factor: float = 1.0,
+                            original_positions: int = 0, beta_fast: float = 32.0, beta_slow: float = 1.0,
+                            attention: float = 0.0):
+    """Host RoPE table as a numpy float32 array [n_pos, rot_dim] (cos | sin), its frequencies scaled for contexts longer
+    than the model was trained on: "linear" (positions divided by factor), "ntk" (theta raised) or "yarn" (slow pairs
+    divided, and cos and sin times `attention`, which is 0.1 ln(factor) + 1 unless given). "none" has the bits of
+    build_rope_table."""
+    import numpy as np
+
+    if scaling not in ROPE_SCALINGS:
+        raise RpgError(f"build_rope_table_scaled: scaling {scaling!r} is none of {sorted(ROPE_SCALINGS)}")
+    if n_pos <= 0 or rot_dim <= 0:
+        raise RpgError(f"build_rope_table_scaled: {n_pos} positions of {rot_dim} elements")
+    out = np.empty((n_pos, rot_dim), dtype=np.float32)
+    how = RopeScalingC(ROPE_SCALINGS[scaling], float(factor), int(original_positions), float(beta_fast),
+                       float(beta_slow), float(attention))
+    _check(batch_ops().rope_table(rot_dim, float(theta), n_pos, ctypes.byref(how),
+                                  out.ctypes.data_as(ctypes.c_void_p)))
+    return out
+
+
+class _Here:
+    """Addresses of one call's tensors, which all have to be on the current device."""
+
+    def __init__(self, what: str):
+        self.what = what
+        self.device = None
+
+    def __call__(self, buf, nbytes: int, dtype, name: str):
+        addr = _addr(buf, nbytes, dtype, name)
+        if buf is not None and not isinstance(buf, int):
+            if self.device is None:
+                self.device = _t().cuda.current_device()
+            if buf.get_device() != self.device:
+                raise RpgError(f"{self.what}: {name} is on device {buf.get_device()}, not the current device {self.device}")
+        return addr
+
+
+def GpuRopeRows(q, k, n_heads: int, n_kv_heads: int, head_dim: int, rot_dim: int, interleaved: bool, rope_tab,
+                rope_rows: int, positions, n_rows: int, q_out, k_out) -> None:
+    """q_out <- q [n_rows, n_heads, head_dim] and k_out <- k [n_rows, n_kv_heads, head_dim], the first rot_dim elements of
+    each head rotated by row positions[r] (int32) of rope_tab [rope_rows, rot_dim]: pairs (i, i + rot_dim / 2), or
+    (2 i, 2 i + 1) if interleaved. Outputs may be the inputs; k and k_out may be None with n_kv_heads 0."""
+    torch = _t()
+    at, f32 = _Here("GpuRopeRows"), torch.float32
+    qb, kb = 4 * n_rows * n_heads * head_dim, 4 * n_rows * n_kv_heads * head_dim
+    _check((_batch or batch_ops()).rope_rows(
+        at(q, qb, f32, "q"), at(k, kb, f32, "k"), n_heads, n_kv_heads, head_dim, rot_dim, 1 if interleaved else 0,
+        at(rope_tab, 4 * rope_rows * rot_dim, f32, "rope_tab"), rope_rows,
+        at(positions, 4 * n_rows, torch.int32, "positions"), n_rows, at(q_out, qb, f32, "q_out"),
+        at(k_out, kb, f32, "k_out")))
+
+
+def GpuSampleBatchWorkspace(n_rows: int, n: int) -> int:
+    """Bytes of the workspace of GpuSampleBatch for n_rows of n logits."""
+    return _check(batch_ops().sample_workspace(n_rows, n))
+
+
+def GpuSampleBatchWorkspaceInit(workspace, nbytes: int) -> None:
+    """Zeroes a workspace, as its first call needs it (a tensor made by torch.zeros is ready)."""
+    _check(batch_ops().sample_workspace_init(_addr(workspace, nbytes, name="workspace"), nbytes))
+
+
+def GpuSampleBatch(logits, n_rows: int, n: int, u, tokens, workspace, temperature=None, top_k=None, top_p=None,
+                   min_p=None, probs=None, row_stride: Optional[int] = None,
+                   workspace_bytes: Optional[int] = None) -> None:
+    """tokens[r] (int32) <- a token of row r of logits [n_rows, n] (rows row_stride floats apart, n if not given), chosen
+    by u[r] in [0, 1) after temperature, top_k, top_p and min_p, each a device tensor of n_rows settings (top_k int32,
+    else float32) or None; probs[r] <- its share of the weight that these leave. The workspace is zero before its first
+    call, and belongs to one call at a time (workspace_bytes goes with a raw address)."""
+    torch = _t()
+    at, f32, i32 = _Here("GpuSampleBatch"), torch.float32, torch.int32
+    row_stride = n if row_stride is None else row_stride
+    if workspace_bytes is None:
+        if not isinstance(workspace, torch.Tensor):
+            raise RpgError("GpuSampleBatch: a raw workspace needs workspace_bytes")
+        workspace_bytes = workspace.nbytes
+    each = 4 * n_rows
+    _check((_batch or batch_ops()).sample(
+        at(logits, 4 * ((n_rows - 1) * row_stride + n) if n_rows > 0 else 0, f32, "logits"), n_rows, n, row_stride,
+        at(temperature, each, f32, "temperature"), at(top_k, each, i32, "top_k"), at(top_p, each, f32, "top_p"),
+        at(min_p, each, f32, "min_p"), at(u, each, f32, "u"), at(tokens, each, i32, "tokens"),
+        at(probs, each, f32, "probs"), at(workspace, workspace_bytes, None, "workspace"), workspace_bytes))
 
 
 # ----------------------------------------------------------------------------- measurement
