@@ -98,6 +98,21 @@ typedef struct {
    * zeroing of one (256-byte aligned) that it needs before its first call. */
   int64_t (*attention_workspace)(int32_t n_heads, int32_t n_kv_heads, int32_t head_dim);
   int32_t (*attention_workspace_init)(void* workspace, int64_t bytes);
+
+  /* attention for a batch whose sequences share their beginnings: rows
+   * [group_rows[g], group_rows[g + 1]) form group g, whose sequences' tables begin
+   * with the same group_pages[g] pages. These are attended to once for the group,
+   * what is behind them by each row; a row that has not all of them, or is in no
+   * group, by itself. Both are device arrays, read when the call runs; at most 64
+   * groups. The pages are taken from the group's first row that has them all. Limits
+   * as for attention; an infinity or a NaN among a group's keys and values, or a page
+   * out of range, gives NaN. The workspace is attention_shared_workspace's (zeroed by
+   * attention_workspace_init), for n_rows or more. */
+  int32_t (*attention_shared)(const rpg_paged_kv_t* kv, const rpg_page_table_t* table, const int32_t* seq_ids,
+                              const int32_t* lens, const int32_t* group_rows, const int32_t* group_pages,
+                              int32_t n_groups, const float* q, int32_t n_heads, int64_t n_rows, float* out,
+                              void* workspace, int64_t workspace_bytes);
+  int64_t (*attention_shared_workspace)(int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, int64_t n_rows);
 } rpg_paged_ops_t;
 
 RPG_OPS_API extern const rpg_paged_ops_t rpg_paged_ops;

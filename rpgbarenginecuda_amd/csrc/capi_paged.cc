@@ -99,12 +99,32 @@ int32_t AttentionWorkspaceInit(void* workspace, int64_t bytes) {
   });
 }
 
+int32_t AttentionShared(const rpg_paged_kv_t* kv, const rpg_page_table_t* table, const int32_t* seq_ids,
+                        const int32_t* lens, const int32_t* group_rows, const int32_t* group_pages, int32_t n_groups,
+                        const float* q, int32_t n_heads, int64_t n_rows, float* out, void* workspace,
+                        int64_t workspace_bytes) {
+  return Guard([&] {
+    RPG_CHECK(workspace_bytes >= 0, "AttentionPagedShared: a workspace of negative size");
+    rpg::GpuAttentionPagedShared(Kv(kv), Table(table), seq_ids, lens, group_rows, group_pages, n_groups, q, n_heads,
+                                 n_rows, out, workspace, static_cast<size_t>(workspace_bytes));
+  });
+}
+
+int64_t AttentionSharedWorkspace(int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, int64_t n_rows) {
+  int64_t bytes = 0;
+  const int32_t rc = Guard([&] {
+    bytes = static_cast<int64_t>(rpg::GpuAttentionPagedSharedWorkspaceBytes(n_heads, n_kv_heads, head_dim, n_rows));
+  });
+  return rc < 0 ? rc : bytes;
+}
+
 }  // namespace
 
 // hipcc passes over a .cc for the device too and would place a constant there.
 #ifndef __HIP_DEVICE_COMPILE__
 extern "C" {
 const rpg_paged_ops_t rpg_paged_ops = {sizeof(rpg_paged_ops_t), KvWrite,   QkNormRopeKv,       KvRead,
-                                       Attention,               AttentionWorkspace, AttentionWorkspaceInit};
+                                       Attention,               AttentionWorkspace, AttentionWorkspaceInit,
+                                       AttentionShared,         AttentionSharedWorkspace};
 }
 #endif

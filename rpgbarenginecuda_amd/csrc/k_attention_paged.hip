@@ -65,7 +65,9 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
+#include "attention_dev.h"
 #include "dev_util.h"
 #include "kernels_gpu.h"
 #include "launch.h"
@@ -74,6 +76,7 @@
 namespace rpg {
 namespace {
 
+using namespace attn;
 using dev::PagedView;
 
 // Four waves of up to 17 KB of keys and values each: two workgroups to a compute unit. (Eight waves and one workgroup
@@ -89,13 +92,6 @@ constexpr size_t kCounterBytes = 256;
 // acknowledgement comes later (1 x 32768 positions in fp16 of one kv head 17.8 against 16.6 us).
 constexpr int kPartPolicy = 16;
 
-using Half2 = _Float16 __attribute__((ext_vector_type(2)));
-using Half8 = _Float16 __attribute__((ext_vector_type(8)));
-using F32x4 = float __attribute__((ext_vector_type(4)));
-using I32x4 = int __attribute__((ext_vector_type(4)));
-using I32x2 = int __attribute__((ext_vector_type(2)));
-using S16x4 = short __attribute__((ext_vector_type(4)));
-
 constexpr int PartFloats(int d) { return d + 4; }  // in LDS: o[d], m, l, and two to keep rows 16-byte aligned
 constexpr uint32_t kLine = 128;
 // In the workspace: o[heads][d], and a line of (m, l)
@@ -103,32 +99,7 @@ __host__ __device__ constexpr uint32_t SlotBytes(int32_t d, int32_t heads) {
   return static_cast<uint32_t>(heads * d) * 4u + kLine;
 }
 
-// ---------------------------------------------------------------- lane exchange
-
-// x of the lane kBy before it in its row of 16, which goes round.
-template <int kBy>
-__device__ __forceinline__ float Ror(float x) {
-  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x120 + kBy, 0xF, 0xF, false));
-}
-
-// f over the four lanes l, l ^ 16, l ^ 32, l ^ 48; every one of them has the result.
-template <class F>
-__device__ __forceinline__ float AcrossRows(float x, F f) {
-  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_int(x), __float_as_int(x), false, false);
-  x = f(__int_as_float(a[0]), __int_as_float(a[1]));
-  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_int(x), __float_as_int(x), false, false);
-  return f(__int_as_float(b[0]), __int_as_float(b[1]));
-}
-__device__ __forceinline__ float MaxAcrossRows(float x) {
-  return AcrossRows(x, [](float a, float b) { return fmaxf(a, b); });
-}
-__device__ __forceinline__ float SumAcrossRows(float x) {
-  return AcrossRows(x, [](float a, float b) { return a + b; });
-}
-
 // ---------------------------------------------------------------- conversions
-
-__device__ __forceinline__ uint32_t Bits(Half2 h) { return __builtin_bit_cast(uint32_t, h); }
 
 // The hi (want_lo false) or lo terms of two values, packed.
 __device__ __forceinline__ uint32_t Term2(float a, float b, bool want_lo) {
@@ -143,11 +114,6 @@ __device__ __forceinline__ uint32_t Term2(float a, float b, bool want_lo) {
   return want_lo ? Bits(lo) : __builtin_bit_cast(uint32_t, hi);
 }
 
-__device__ __forceinline__ Half8 AsHalf8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  const dev::U32x4 w = {a, b, c, d};
-  return __builtin_bit_cast(Half8, w);
-}
-
 // Signed digit `at` (selector bytes: at, 4 + at) of four whole numbers given with
 // 0x80808080 added: x = sum of digit_i 256^i with digit_i = byte i - 128 there.
 __device__ __forceinline__ int Digit4(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t selector) {
@@ -155,90 +121,7 @@ __device__ __forceinline__ int Digit4(uint32_t a, uint32_t b, uint32_t c, uint32
   return static_cast<int>(__builtin_amdgcn_perm(hi, lo, 0x05040100u) ^ 0x80808080u);
 }
 
-// ---------------------------------------------------------------- LDS
-
-using Lds = __attribute__((address_space(3))) char;
-
-// Loads straight to LDS are written out, and so are the waits for them: the compiler
-// lets an LDS read wait for every such load before it, where the loop below needs it
-// to wait for the older half of them. The waits count on the kernel's main loop to
-// make no other vector memory access in between; any that the compiler does make
-// (a piece's queries and outputs) only makes a wait longer.
-using Resource = dev::U32x4;
-__device__ __forceinline__ Resource RowsResource(const void* base, uint32_t bytes) {
-  const uint64_t at = reinterpret_cast<uint64_t>(base);
-  return Resource{static_cast<uint32_t>(at), static_cast<uint32_t>(at >> 32) & 0xFFFFu, bytes, 0x00020000u};
-}
-__device__ __forceinline__ uint32_t LdsAddress(const void* p) {
-  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const Lds*)(static_cast<const char*>(p))));
-}
-// kN times 16 bytes a lane from rs: time i from byte off[i % kOff] + 1024 i, lane j's to LDS address `to` + 1024 i +
-// 16 j (an instruction's offset counts on both sides). What is read once is loaded with the streaming hint: without it
-// 32 x 4096 positions take 55.4 us and not 50.0, 128 x 8192 in 8 bits 214 and not 190. M0 holds the
-// LDS address: an operand, so that the compiler writes it and knows what is there. It is read one wait state after it is
-// written; five are waited, which M0 and a resource need where a vector instruction wrote them.
-template <int kN, int kOff>
-__device__ __forceinline__ void LoadToLds(Resource rs, const uint32_t (&off)[kOff], uint32_t to) {
-  static_assert(kN == 1 || kN == 2 || kN == 4, "");
-  if constexpr (kN == 1) {
-    asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds"
-                 :
-                 : "{m0}"(to), "v"(off[0]), "s"(rs)
-                 : "memory");
-  } else if constexpr (kN == 2) {
-    asm volatile(
-        "s_nop 4\n\t"
-        "buffer_load_dwordx4 %1, %3, 0 offen nt lds\n\t"
-        "buffer_load_dwordx4 %2, %3, 0 offen offset:1024 nt lds"
-        :
-        : "{m0}"(to), "v"(off[0]), "v"(off[1 % kOff]), "s"(rs)
-        : "memory");
-  } else {
-    asm volatile(
-        "s_nop 4\n\t"
-        "buffer_load_dwordx4 %1, %5, 0 offen nt lds\n\t"
-        "buffer_load_dwordx4 %2, %5, 0 offen offset:1024 nt lds\n\t"
-        "buffer_load_dwordx4 %3, %5, 0 offen offset:2048 nt lds\n\t"
-        "buffer_load_dwordx4 %4, %5, 0 offen offset:0xc00 nt lds"
-        :
-        : "{m0}"(to), "v"(off[0]), "v"(off[1 % kOff]), "v"(off[2 % kOff]), "v"(off[3 % kOff]), "s"(rs)
-        : "memory");
-  }
-}
-// 4 bytes a lane, from an address of its own.
-__device__ __forceinline__ void LoadWordToLds(const float* from, uint32_t to) {
-  asm volatile("s_nop 4\n\tglobal_load_lds_dword %1, off" : : "{m0}"(to), "v"(from) : "memory");
-}
-// Waits until at most kLeft vector memory accesses are under way.
-template <int kLeft>
-__device__ __forceinline__ void WaitLoads() {
-  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(kLeft) : "memory");
-}
-// Waits for the LDS reads under way, before what they read is loaded over.
-__device__ __forceinline__ void WaitLdsReads() { asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory"); }
-
-// A scalar load: p is the same in every lane, and what it points to does not change while the kernel runs.
-template <class T>
-__device__ __forceinline__ T ScalarLoad(const T* p) {
-  return *(const __attribute__((address_space(4))) T*)(p);
-}
-
-// Four halves, one of each of four rows: in each 16-lane group, lane j receives
-// element j % 4 of the 8 bytes addressed by lanes j / 4, 4 + j / 4, ...
-__device__ __forceinline__ uint2 ReadHalvesAcross(const char* at) {
-  const S16x4 v =
-      __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) S16x4*)(Lds*)(const_cast<char*>(at)));
-  return __builtin_bit_cast(uint2, v);
-}
-// Eight bytes, one of each of eight rows: in each 16-lane group, lane j receives
-// byte j % 8 of the 8 bytes addressed by lanes j / 8, 2 + j / 8, ...
-__device__ __forceinline__ I32x2 ReadBytesAcross(const char* at) {
-  return __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) I32x2*)(Lds*)(const_cast<char*>(at)));
-}
-
 // ---------------------------------------------------------------- sharing out
-
-__device__ __forceinline__ uint32_t Scalar(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
 
 // How a pair's units are cut into items, of which a workgroup takes whole ones. From kManyUnits in the batch on an item is
 // a unit, so that all workgroups get alike. With fewer, joining what two workgroups hold of a pair (a round trip to memory
@@ -261,23 +144,6 @@ struct Cut {
   }
   __device__ __forceinline__ uint32_t Items(uint32_t n) const {
     return units ? n : n <= kWholeUnits ? min(n, 1u) : (n + (1u << step) - 1u) >> step;
-  }
-};
-
-// Everything here is the same in every lane of a wave, and kept in scalar registers.
-struct Share {
-  uint32_t per;  // a workgroup's items: per, and one more in the first `rem` of them
-  uint32_t rem;
-
-  __device__ __forceinline__ Share(uint32_t items, uint32_t groups) {
-    per = Scalar(items / groups);
-    rem = items - per * groups;
-  }
-  __device__ __forceinline__ uint32_t Begin(uint32_t w) const { return w * per + min(w, rem); }
-  // The workgroup whose share holds item x.
-  __device__ __forceinline__ uint32_t Holder(uint32_t x) const {
-    const uint32_t big = rem * (per + 1);
-    return Scalar(x < big ? x / (per + 1) : rem + (x - big) / per);
   }
 };
 
@@ -308,17 +174,32 @@ struct Rows {
   }
 };
 
-// Sum of x over the lanes up to and with this one.
-__device__ __forceinline__ uint32_t ScanAdd(uint32_t x) {
-  int v = static_cast<int>(x);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr 1, 2, 4, 8: within rows of 16
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // lane 15's into row 1, lane 47's into row 3
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // lane 31's into rows 2 and 3
-  return static_cast<uint32_t>(v);
-}
+// No part of a batch's rows is shared.
+struct NotShared {
+  static constexpr bool kOn = false;
+  __device__ __forceinline__ int32_t PagesOfLane(const Rows&, int32_t, int32_t, int32_t) const { return 0; }
+  __device__ __forceinline__ int32_t PagesOf(const Rows&, int32_t, int32_t, int32_t) const { return 0; }
+};
+
+// Groups of rows that begin with the same pages (dev::SharedGroups): what a row has of them is attended to elsewhere, and
+// here only what is behind. That part's result, relative to its maximum m: o [row][head][D], (m, l) [row][head].
+struct Shared {
+  static constexpr bool kOn = true;
+  dev::SharedGroups groups;
+  int32_t page_shift;
+
+  // whole pages of row r before what is its own; r is the lane's
+  __device__ __forceinline__ int32_t PagesOfLane(const Rows& rows, int32_t r, int32_t seq, int32_t len) const {
+    return Taken(rows, groups.PagesOfLane(r), seq, len);
+  }
+  // r the same in every lane
+  __device__ __forceinline__ int32_t PagesOf(const Rows& rows, int32_t r, int32_t seq, int32_t len) const {
+    return Taken(rows, groups.PagesOf(r), seq, len);
+  }
+  __device__ __forceinline__ int32_t Taken(const Rows& rows, int32_t pages, int32_t seq, int32_t len) const {
+    return rows.Fine(seq, len) && dev::TakesPart(pages, page_shift, len) ? pages : 0;
+  }
+};
 
 // Unit c of `units` of `pair` of `row`.
 struct Place {
@@ -328,22 +209,31 @@ struct Place {
 
 // The batch as a wave sees it: rows are taken `each` to a lane, with the units and the items before them. (A short call's
 // start is bound by fetching its instructions, so what is needed in several places is written in one.)
+template <class S>
 struct Batch {
   const Rows& rows;
+  const S& shared;
   Cut cut{0};
   int lane;
   int32_t each;
   uint32_t units, items;
   uint32_t units_before, items_before;
-  int32_t own_len = 0, own_seq = -1;  // where each is 1: of row `lane`
+  int32_t own_len = 0, own_seq = -1, own_pages = 0;  // where each is 1: of row `lane`
   uint32_t own_units = 0;
 
-  __device__ __forceinline__ Batch(const Rows& r, int l) : rows(r), lane(l) {
+  __device__ __forceinline__ Batch(const Rows& r, const S& s, int l) : rows(r), shared(s), lane(l) {
     each = (rows.n_rows + 63) / 64;
-    if (__builtin_expect(each == 1, 1) && lane < rows.n_rows) {
-      own_len = rows.lens[lane];
-      own_seq = rows.Seq(lane);
-      own_units = rows.UnitsOf(own_seq, own_len);
+    if (__builtin_expect(each == 1, 1)) {
+      if (lane < rows.n_rows) {
+        own_len = rows.lens[lane];
+        own_seq = rows.Seq(lane);
+        if constexpr (!S::kOn) own_units = rows.UnitsOf(own_seq, own_len);
+      }
+      if constexpr (S::kOn) {
+        own_pages = shared.PagesOfLane(rows, lane, own_seq, own_len);
+        own_len -= own_pages << PageShift();
+        own_units = rows.UnitsOf(own_seq, own_len);
+      }
     }
     units_before = Before(0, rows.n_rows, each, false, &units);
     cut = Cut(units);
@@ -359,12 +249,18 @@ struct Batch {
       own = of_items ? cut.Items(own_units) : own_units;
     } else {
       const int64_t first = lo + static_cast<int64_t>(lane) * some;
-#pragma unroll 2
-      for (int32_t i = 0; i < some; ++i) {
+      const auto add = [&](int32_t i) {
         if (first + i < hi) {
-          const uint32_t n = rows.UnitsOf(static_cast<int32_t>(first + i));
+          const uint32_t n = LaneUnitsOf(static_cast<int32_t>(first + i));
           own += of_items ? cut.Items(n) : n;
         }
+      };
+      if constexpr (S::kOn) {
+#pragma unroll 1
+        for (int32_t i = 0; i < some; ++i) add(i);
+      } else {
+#pragma unroll 2
+        for (int32_t i = 0; i < some; ++i) add(i);
       }
     }
     own *= static_cast<uint32_t>(rows.pairs);
@@ -373,12 +269,31 @@ struct Batch {
     return sum - own;
   }
 
-  // Of one row, the same in every lane
+  // log2 of a page's positions
+  __device__ __forceinline__ int32_t PageShift() const {
+    if constexpr (S::kOn) return shared.page_shift;
+    return 0;
+  }
+  __device__ __forceinline__ uint32_t LaneUnitsOf(int32_t r) const {
+    if constexpr (!S::kOn) return rows.UnitsOf(r);
+    const int32_t seq = rows.Seq(r), len = rows.lens[r];
+    return rows.UnitsOf(seq, len - (shared.PagesOfLane(rows, r, seq, len) << PageShift()));
+  }
+
+  // Of one row, the same in every lane: pages that are not its own, units and positions behind them
+  __device__ __forceinline__ int32_t PagesOf(int32_t r) const {
+    if constexpr (!S::kOn) return 0;
+    return __builtin_expect(each == 1, 1) ? __builtin_amdgcn_readlane(own_pages, r)
+                                          : shared.PagesOf(rows, r, rows.ScalarSeq(r), ScalarLoad(rows.lens + r));
+  }
   __device__ __forceinline__ uint32_t UnitsOf(int32_t r) const {
-    return __builtin_expect(each == 1, 1) ? __builtin_amdgcn_readlane(own_units, r) : rows.ScalarUnitsOf(r);
+    if (__builtin_expect(each == 1, 1)) return __builtin_amdgcn_readlane(own_units, r);
+    if constexpr (!S::kOn) return rows.ScalarUnitsOf(r);
+    return rows.UnitsOf(rows.ScalarSeq(r), LenOf(r));
   }
   __device__ __forceinline__ int32_t LenOf(int32_t r) const {
-    return __builtin_expect(each == 1, 1) ? __builtin_amdgcn_readlane(own_len, r) : ScalarLoad(rows.lens + r);
+    if (__builtin_expect(each == 1, 1)) return __builtin_amdgcn_readlane(own_len, r);
+    return ScalarLoad(rows.lens + r) - (PagesOf(r) << PageShift());
   }
   __device__ __forceinline__ int64_t SeqOf(int32_t r) const {
     return __builtin_expect(each == 1, 1) ? __builtin_amdgcn_readlane(own_seq, r) : rows.ScalarSeq(r);
@@ -478,7 +393,8 @@ struct Parts {
   bool leads = false;  // the pair's first part is the first thing that workgroup wa holds
 
   __device__ __forceinline__ Parts() {}
-  __device__ __forceinline__ Parts(const Piece& p, const Batch& batch, const Share& share, uint32_t me) {
+  template <class S>
+  __device__ __forceinline__ Parts(const Piece& p, const Batch<S>& batch, const Share& share, uint32_t me) {
     const uint32_t item = batch.ItemOfPair(p.first, p.row, p.pair, p.n);
     wa = share.Holder(item);
     leads = share.Begin(wa) == item;
@@ -495,14 +411,6 @@ struct Parts {
   }
 };
 
-// Counts in at a counter; whether that was the last of `all`, which leaves the counter ready for the next call.
-__device__ __forceinline__ int Count(char* workspace, uint32_t counter, uint32_t all) {
-  uint32_t* at = reinterpret_cast<uint32_t*>(workspace) + counter;
-  const bool last = __hip_atomic_fetch_add(at, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == all - 1;
-  if (last) __hip_atomic_store(at, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  return last ? 1 : 0;
-}
-
 // One argument: a launch takes longer for every pointer among its arguments (0.06 us of host time).
 struct AttentionArgs {
   PagedView view;
@@ -517,9 +425,33 @@ struct AttentionArgs {
   float scale_log2;
 };
 
+// The same, and what the shared positions came to.
+struct SharedAttentionArgs : AttentionArgs {
+  const int32_t* group_rows;
+  const int32_t* group_pages;
+  int32_t n_groups;
+  const float* prefix_o;
+  const float* prefix_ml;
+};
+
+// A row's and head's result over the positions behind the shared ones, o under m with sum l, joined with that over them
+// (row_head's of prefix_o and prefix_ml), elements d to d + 3.
+__device__ __forceinline__ float4 JoinPrefix(const SharedAttentionArgs& args, int64_t row_head, int32_t head_dim,
+                                             int32_t d, float4 o, float m, float l) {
+  const float2 ml = *reinterpret_cast<const float2*>(args.prefix_ml + 2 * row_head);
+  const float4 p = dev::Load4(args.prefix_o + row_head * head_dim + d);
+  const float top = fmaxf(m, ml.x);
+  const float safe = top == -INFINITY ? 0.0f : top;
+  const float f = __builtin_amdgcn_exp2f(m - safe), g = __builtin_amdgcn_exp2f(ml.x - safe);
+  const float inv = 1.0f / fmaf(l, f, ml.y * g);
+  return make_float4(fmaf(o.x, f, p.x * g) * inv, fmaf(o.y, f, p.y * g) * inv, fmaf(o.z, f, p.z * g) * inv,
+                     fmaf(o.w, f, p.w * g) * inv);
+}
+
 // kTiles: 8-bit caches, column tiles of up to 4 heads (1 or 2); else 1, of up to 8.
-template <int D, bool kQ8, int kTiles>
-__global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const AttentionArgs args) {
+template <int D, bool kQ8, int kTiles, class Args>
+__global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Args args) {
+  constexpr bool kShared = std::is_same_v<Args, SharedAttentionArgs>;
   const PagedView& view = args.view;
   const Rows& rows = args.rows;
   const float* __restrict__ q = args.q;
@@ -562,7 +494,16 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Att
   const int copy = n / kHeadCols;
 
   // the batch's units, and this wave's share
-  const Batch batch(rows, lane);
+  const auto shared = [&] {
+    if constexpr (kShared) {
+      return Shared{dev::SharedGroups(args.group_rows, args.group_pages, args.n_groups, rows.n_rows, view.max_pages, lane),
+                    view.page_shift};
+    } else {
+      return NotShared{};
+    }
+  }();
+  using S = std::conditional_t<kShared, Shared, NotShared>;
+  const Batch<S> batch(rows, shared, lane);
   const uint32_t groups = min(gridDim.x, batch.cut.units ? (batch.units + 3) / 4 : batch.items);
   const Share share(batch.items, max(groups, 1u));
   const uint32_t me = blockIdx.x;
@@ -640,7 +581,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Att
     int32_t row = first.row, pair = first.pair;
     uint32_t c = first.c, units = first.units;
     int32_t len = batch.LenOf(row);
-    const int32_t* table = view.pages + batch.SeqOf(row) * view.max_pages;
+    const int32_t* table = view.pages + batch.SeqOf(row) * view.max_pages + batch.PagesOf(row);
 
     // Rows of the pool that the 16-key tiles of unit c start at; a tile past the end repeats the unit's first, a page
     // out of range is read as page 0 and its tile marked.
@@ -910,7 +851,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Att
             } while (units == 0);
             row = min(row, rows.n_rows - 1);  // past the last only if the lengths change while this runs
             len = batch.LenOf(row);
-            table = view.pages + batch.SeqOf(row) * view.max_pages;
+            table = view.pages + batch.SeqOf(row) * view.max_pages + batch.PagesOf(row);
           }
         }
         find();
@@ -1108,6 +1049,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Att
 
       // ---- the piece's (m, l, o): out, or kept where it is not the whole of its pair
       const bool whole = c_first == 0 && c_end == piece_units;
+      const bool joins_prefix = kShared && whole && batch.PagesOf(piece_row) > 0;
       if (!whole) {
         const int which = more ? 0 : 1;
         if (lane == 0) pieces[wave][which] = Piece{u - c_end, c_first, c_end, piece_units, piece_row, piece_pair};
@@ -1120,7 +1062,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Att
         const float total = of_tile(t, l), top = of_tile(t, m);
         // 8-bit values: one factor after the other, since their product may be too small a number
         const float unit = kQ8 ? 1.0f / of_tile(t, shrink) : 1.0f;
-        const float by = (kQ8 ? 1.0f : 0x1p-14f) / (whole ? total : 1.0f);
+        const float by = (kQ8 ? 1.0f : 0x1p-14f) / (whole && !joins_prefix ? total : 1.0f);
         const int h = t * kHeadCols + head_col;
         F32x4 own[kOwn];
 #pragma unroll
@@ -1142,6 +1084,16 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Att
           kept_l[t] = total;
         } else if (h < heads) {
           float* to = whole ? out + (head_row + h) * D : reinterpret_cast<float*>(v_mine) + h * kPart;
+          if constexpr (kShared) {
+            if (joins_prefix) {
+#pragma unroll
+              for (int i = 0; i < kOwn; ++i) {
+                const float4 x = JoinPrefix(args, head_row + h, D, 16 * (copy * kOwn + i) + 4 * g,
+                                            make_float4(own[i][0], own[i][1], own[i][2], own[i][3]), top, total);
+                own[i] = F32x4{x.x, x.y, x.z, x.w};
+              }
+            }
+          }
 #pragma unroll
           for (int i = 0; i < kOwn; ++i) *reinterpret_cast<F32x4*>(to + 16 * (copy * kOwn + i) + 4 * g) = own[i];
           if (!whole && copy == 0 && g == 0) {
@@ -1203,6 +1155,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Att
     const bool leads = run.first + run.c0 == begin;  // the workgroup's first piece
     const __amdgpu_buffer_rsrc_t rs =
         dev::OutResource(slots + (2 * static_cast<int64_t>(me) + (leads ? 0 : 1)) * slot_bytes, slot_bytes);
+    const bool joins_prefix = kShared && whole && batch.PagesOf(run.row) > 0;
     for (int i = threadIdx.x; i < of.heads * (D / 4); i += 64 * kWaves) {
       const int h = i / (D / 4), d = 4 * (i % (D / 4));
       float4 x[2 * kWaves];
@@ -1230,6 +1183,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Att
         }
       }
       if (whole) {
+        if constexpr (kShared) {
+          if (joins_prefix) {
+            dev::Store4(out + (of.head_row + h) * D + d, JoinPrefix(args, of.head_row + h, D, d, o, top, l));
+            continue;
+          }
+        }
         const float inv = 1.0f / l;
         dev::Store4(out + (of.head_row + h) * D + d, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
       } else {
@@ -1354,7 +1313,15 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Att
         done = true;
       }
       if (!done) continue;
+      const bool joins_prefix = kShared && batch.PagesOf(run.row) > 0;
       if (set == 0) {
+        if constexpr (kShared) {
+          if (joins_prefix) {
+            dev::Store4(out + heads.head_row * D + 4 * column,
+                        JoinPrefix(args, heads.head_row + h, D, 4 * column - h * D, o, top, l));
+            continue;
+          }
+        }
         const float inv = 1.0f / l;
         dev::Store4(out + heads.head_row * D + 4 * column, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
       }
@@ -1368,6 +1335,17 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Att
     if (seq < 0) continue;
     const bool fine = rows.Fine(seq, len);
     if (fine && len > 0) continue;
+    if constexpr (kShared) {
+      if (batch.PagesOf(static_cast<int32_t>(r)) > 0) {  // nothing but what it shares
+        for (int64_t i = threadIdx.x; i < static_cast<int64_t>(n_heads) * (D / 4); i += 64 * kWaves) {
+          const int64_t row_head = r * n_heads + i / (D / 4);
+          const int32_t d = 4 * static_cast<int32_t>(i % (D / 4));
+          dev::Store4(out + row_head * D + d,
+                      JoinPrefix(args, row_head, D, d, make_float4(0.0f, 0.0f, 0.0f, 0.0f), -INFINITY, 0.0f));
+        }
+        continue;
+      }
+    }
     const float x = fine ? 0.0f : NAN;
     for (int64_t i = threadIdx.x; i < static_cast<int64_t>(n_heads) * (D / 4); i += 64 * kWaves) {
       dev::Store4(out + r * n_heads * D + 4 * i, make_float4(x, x, x, x));
@@ -1389,6 +1367,17 @@ void TilesOf(int32_t group, int32_t* tiles, int32_t* tile_heads) {
   *tile_heads = (group + *tiles - 1) / *tiles;
 }
 
+template <class Args>
+auto* KernelFor(const GpuPagedKv& kv, int32_t tile_heads) {
+  if (kv.type != kKvQ8) {
+    return kv.head_dim == 128 ? PagedAttentionKernel<128, false, 1, Args> : PagedAttentionKernel<64, false, 1, Args>;
+  }
+  if (tile_heads > 4) {
+    return kv.head_dim == 128 ? PagedAttentionKernel<128, true, 2, Args> : PagedAttentionKernel<64, true, 2, Args>;
+  }
+  return kv.head_dim == 128 ? PagedAttentionKernel<128, true, 1, Args> : PagedAttentionKernel<64, true, 1, Args>;
+}
+
 }  // namespace
 
 size_t GpuAttentionPagedWorkspaceBytes(int32_t n_heads, int32_t n_kv_heads, int32_t head_dim) {
@@ -1404,29 +1393,33 @@ void GpuAttentionPagedWorkspaceInit(void* workspace, size_t bytes) {
   GpuStreamFill(workspace, static_cast<int64_t>(bytes), 0);
 }
 
-void GpuAttentionPaged(const GpuPagedKv& kv, const GpuPageTable& table, const int32_t* seq_ids, const int32_t* lens,
-                       const float* q_dev, int32_t n_heads, int64_t n_rows, float* out_dev, void* workspace,
-                       size_t workspace_bytes) {
-  CheckPagedKv("AttentionPaged", kv, table);
-  CheckHeads("AttentionPaged", n_heads, kv.n_kv_heads, kv.head_dim);
-  RPG_CHECK(n_rows >= 0 && n_rows <= 0x7FFFFFFF, "AttentionPaged: %lld rows", static_cast<long long>(n_rows));
+void AttendPaged(const GpuPagedKv& kv, const GpuPageTable& table, const int32_t* seq_ids, const int32_t* lens,
+                 const float* q_dev, int32_t n_heads, int64_t n_rows, float* out_dev, void* workspace,
+                 size_t workspace_bytes, PagedPrefix* prefix) {
+  const char* what = prefix == nullptr ? "AttentionPaged" : "AttentionPagedShared";
+  CheckPagedKv(what, kv, table);
+  CheckHeads(what, n_heads, kv.n_kv_heads, kv.head_dim);
+  RPG_CHECK(n_rows >= 0 && n_rows <= 0x7FFFFFFF, "%s: %lld rows", what, static_cast<long long>(n_rows));
   if (n_rows == 0) return;
-  RPG_CHECK(lens != nullptr && q_dev != nullptr && out_dev != nullptr && workspace != nullptr,
-            "AttentionPaged got a null pointer");
-  RPG_CHECK(seq_ids != nullptr || n_rows <= table.n_seqs, "AttentionPaged: %lld rows without seq_ids, but %lld sequences",
+  RPG_CHECK(lens != nullptr && q_dev != nullptr && out_dev != nullptr && workspace != nullptr, "%s got a null pointer",
+            what);
+  RPG_CHECK(seq_ids != nullptr || n_rows <= table.n_seqs, "%s: %lld rows without seq_ids, but %lld sequences", what,
             static_cast<long long>(n_rows), static_cast<long long>(table.n_seqs));
   RPG_CHECK(((reinterpret_cast<uintptr_t>(q_dev) | reinterpret_cast<uintptr_t>(out_dev)) & 15) == 0,
-            "AttentionPaged: q and out have to be 16-byte aligned");
+            "%s: q and out have to be 16-byte aligned", what);
   RPG_CHECK(((reinterpret_cast<uintptr_t>(seq_ids) | reinterpret_cast<uintptr_t>(lens)) & 3) == 0,
-            "AttentionPaged: seq_ids and lens have to be 4-byte aligned");
+            "%s: seq_ids and lens have to be 4-byte aligned", what);
   const int64_t q_bytes = n_rows * n_heads * kv.head_dim * 4;
-  RPG_CHECK(!Overlap(q_dev, q_bytes, out_dev, q_bytes), "AttentionPaged: out must not overlap q");
-  const size_t need = GpuAttentionPagedWorkspaceBytes(n_heads, kv.n_kv_heads, kv.head_dim);
+  RPG_CHECK(!Overlap(q_dev, q_bytes, out_dev, q_bytes), "%s: out must not overlap q", what);
+  const size_t own = GpuAttentionPagedWorkspaceBytes(n_heads, kv.n_kv_heads, kv.head_dim);
+  const size_t need = prefix == nullptr
+                          ? own
+                          : GpuAttentionPagedSharedWorkspaceBytes(n_heads, kv.n_kv_heads, kv.head_dim, n_rows);
   RPG_CHECK((reinterpret_cast<uintptr_t>(workspace) & 255) == 0 && workspace_bytes >= need,
-            "AttentionPaged: a workspace of %zu bytes, 256-byte aligned, is needed (%zu given)", need, workspace_bytes);
+            "%s: a workspace of %zu bytes, 256-byte aligned, is needed (%zu given)", what, need, workspace_bytes);
   RPG_CHECK(!Overlap(out_dev, q_bytes, workspace, static_cast<int64_t>(need)) &&
                 !Overlap(q_dev, q_bytes, workspace, static_cast<int64_t>(need)),
-            "AttentionPaged: the workspace must not overlap q or out");
+            "%s: the workspace must not overlap q or out", what);
   int32_t tiles, tile_heads;
   TilesOf(n_heads / kv.n_kv_heads, &tiles, &tile_heads);
   const Rows rows{seq_ids, lens, static_cast<int32_t>(table.n_seqs),
@@ -1434,7 +1427,7 @@ void GpuAttentionPaged(const GpuPagedKv& kv, const GpuPageTable& table, const in
                   static_cast<int32_t>(n_rows), kv.n_kv_heads * tiles, kv.head_dim == 128 && kv.type == kKvF16 ? 5 : 6};
   const int64_t most = (static_cast<int64_t>(rows.capacity) >> rows.unit_shift) + 1;
   RPG_CHECK(n_rows <= 0x7FFFFFFF / most / rows.pairs,
-            "AttentionPaged: %lld rows of up to %lld positions and %d heads are too many for one call",
+            "%s: %lld rows of up to %lld positions and %d heads are too many for one call", what,
             static_cast<long long>(n_rows), static_cast<long long>(rows.capacity), rows.pairs);
   // no more workgroups than the longest possible rows would give work to; for a few pairs one to a compute unit, since more
   // parts of a pair cost more to join than the card gives for them, also at great lengths. With two to a compute unit instead, 8 pairs of one row in 8 bits: of 32768 positions 21.8 us against 20.5, of 131072 54.2
@@ -1445,14 +1438,28 @@ void GpuAttentionPaged(const GpuPagedKv& kv, const GpuPageTable& table, const in
   const int64_t groups = std::min<int64_t>(at_once, all_pairs * ((most + (1 << kLeastStep) - 1) >> kLeastStep));
   const float scale_log2 =
       static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(kv.head_dim)));
-  auto* kern = kv.head_dim == 128 ? PagedAttentionKernel<128, false, 1> : PagedAttentionKernel<64, false, 1>;
-  if (kv.type == kKvQ8) {
-    kern = tile_heads > 4 ? (kv.head_dim == 128 ? PagedAttentionKernel<128, true, 2> : PagedAttentionKernel<64, true, 2>)
-                          : (kv.head_dim == 128 ? PagedAttentionKernel<128, true, 1> : PagedAttentionKernel<64, true, 1>);
+  const AttentionArgs args{dev::ViewOf(kv, table), rows, q_dev, out_dev, static_cast<char*>(workspace), n_heads,
+                           n_heads / kv.n_kv_heads, tiles, tile_heads, scale_log2};
+  const dim3 grid(static_cast<unsigned>(groups)), block(64 * kWaves);
+  if (prefix == nullptr || prefix->n_groups == 0) {
+    Launch("PagedAttentionKernel", KernelFor<AttentionArgs>(kv, tile_heads), grid, block, args);
+    return;
   }
-  Launch("PagedAttentionKernel", kern, dim3(static_cast<unsigned>(groups)), dim3(64 * kWaves),
-         AttentionArgs{dev::ViewOf(kv, table), rows, q_dev, out_dev, static_cast<char*>(workspace), n_heads,
-                       n_heads / kv.n_kv_heads, tiles, tile_heads, scale_log2});
+  AttendPrefix(kv, table, seq_ids, lens, q_dev, n_heads, n_rows, static_cast<char*>(workspace) + own, prefix);
+  SharedAttentionArgs shared;
+  static_cast<AttentionArgs&>(shared) = args;
+  shared.group_rows = prefix->group_rows;
+  shared.group_pages = prefix->group_pages;
+  shared.n_groups = prefix->n_groups;
+  shared.prefix_o = prefix->o;
+  shared.prefix_ml = prefix->ml;
+  Launch("PagedAttentionKernel", KernelFor<SharedAttentionArgs>(kv, tile_heads), grid, block, shared);
+}
+
+void GpuAttentionPaged(const GpuPagedKv& kv, const GpuPageTable& table, const int32_t* seq_ids, const int32_t* lens,
+                       const float* q_dev, int32_t n_heads, int64_t n_rows, float* out_dev, void* workspace,
+                       size_t workspace_bytes) {
+  AttendPaged(kv, table, seq_ids, lens, q_dev, n_heads, n_rows, out_dev, workspace, workspace_bytes, nullptr);
 }
 
 }  // namespace rpg

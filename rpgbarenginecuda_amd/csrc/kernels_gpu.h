@@ -373,6 +373,29 @@ void GpuAttentionPaged(const GpuPagedKv& kv, const GpuPageTable& table, const in
 size_t GpuAttentionPagedWorkspaceBytes(int32_t n_heads, int32_t n_kv_heads, int32_t head_dim);
 void GpuAttentionPagedWorkspaceInit(void* workspace, size_t bytes);
 
+// GpuAttentionPaged for a batch whose sequences share their beginnings (a system
+// prompt, a world's description): rows [group_rows[g], group_rows[g + 1]) form group
+// g, whose sequences' tables begin with the same group_pages[g] pages. These are
+// attended to once for the group, what is behind them by each row. group_rows
+// ([n_groups + 1]) and group_pages ([n_groups]) are device arrays, read when the call
+// runs as lens and tables are; n_groups is at most 64.
+//
+// Which pages a group shares is read from the table of its first row that has them
+// all; the tables of the others have to name the same ones. A row that does not reach
+// behind them, or is in no group, is attended to by itself; one in several groups
+// belongs to the first of these. Of a group out of range, what lies inside [0, n_rows)
+// counts; one of no pages, fewer or more than a table has, shares none. Results and limits are
+// GpuAttentionPaged's, but that an infinity or a NaN among a group's keys and values,
+// or a page out of range, gives NaN in all of the group's rows whose output it reaches.
+//
+// workspace: GpuAttentionPagedSharedWorkspaceBytes for n_rows or more, else as for
+// GpuAttentionPaged (GpuAttentionPagedWorkspaceInit zeroes it).
+void GpuAttentionPagedShared(const GpuPagedKv& kv, const GpuPageTable& table, const int32_t* seq_ids,
+                             const int32_t* lens, const int32_t* group_rows, const int32_t* group_pages,
+                             int32_t n_groups, const float* q_dev, int32_t n_heads, int64_t n_rows, float* out_dev,
+                             void* workspace, size_t workspace_bytes);
+size_t GpuAttentionPagedSharedWorkspaceBytes(int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, int64_t n_rows);
+
 // ---------------------------------------------------------------- quantised matmul
 
 // OUT[t, r] = dot(row r of W, row t of X), i.e. OUT = X . W^T (src/kernels_gpu.h:42-49):

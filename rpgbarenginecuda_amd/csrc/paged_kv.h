@@ -20,6 +20,26 @@ inline bool Overlap(const void* a, int64_t na, const void* b, int64_t nb) {
   return x < y + static_cast<uint64_t>(nb) && y < x + static_cast<uint64_t>(na);
 }
 
+// What the shared positions of a call's groups came to (k_attention_prefix.hip), for the rows' own attention to join:
+// for row r and head h, relative to the maximum m of its scores (as powers of two), o[r][h] = sum 2^(s - m) v and
+// ml[r][h] = (m, sum 2^(s - m)).
+struct PagedPrefix {
+  const int32_t* group_rows;
+  const int32_t* group_pages;
+  int32_t n_groups;
+  float* o = nullptr;
+  float* ml = nullptr;
+};
+
+// GpuAttentionPaged, over what is behind the shared positions if there is a prefix.
+void AttendPaged(const GpuPagedKv& kv, const GpuPageTable& table, const int32_t* seq_ids, const int32_t* lens,
+                 const float* q_dev, int32_t n_heads, int64_t n_rows, float* out_dev, void* workspace,
+                 size_t workspace_bytes, PagedPrefix* prefix);
+
+// The shared positions' attention, into prefix->o and prefix->ml, which it places in the workspace.
+void AttendPrefix(const GpuPagedKv& kv, const GpuPageTable& table, const int32_t* seq_ids, const int32_t* lens,
+                  const float* q_dev, int32_t n_heads, int64_t n_rows, char* workspace, PagedPrefix* prefix);
+
 namespace dev {
 
 // Passed to kernels by value.
@@ -65,6 +85,55 @@ __device__ __forceinline__ Slot FindSlot(const PagedView& view, int64_t seq, int
   s.state = SlotState::kOk;
   s.first = ((static_cast<int64_t>(page) * view.n_kv) << view.page_shift) + (pos & ((1 << view.page_shift) - 1));
   return s;
+}
+
+constexpr int kMaxSharedGroups = 64;
+
+// A call's groups, one to a lane. Rows [first, last) of a group begin with the same `pages` pages; a row that several
+// groups name is of the first of them. What is out of range is cut off.
+struct SharedGroups {
+  int32_t n;
+  int32_t first = 0, last = 0, pages = 0;
+
+  __device__ __forceinline__ SharedGroups(const int32_t* group_rows, const int32_t* group_pages, int32_t n_groups,
+                                          int32_t n_rows, int64_t max_pages, int lane)
+      : n(n_groups) {
+    if (lane < n_groups) {
+      first = min(max(group_rows[lane], 0), n_rows);
+      last = min(max(group_rows[lane + 1], first), n_rows);
+      const int32_t p = group_pages[lane];
+      pages = p > 0 && p <= max_pages ? p : 0;
+    }
+  }
+  // The group of row r, the lane's; -1 if there is none.
+  __device__ __forceinline__ int32_t OfLane(int32_t r) const {
+    int32_t found = -1;
+#pragma unroll 1
+    for (int32_t g = n - 1; g >= 0; --g) {
+      const bool in = r >= __builtin_amdgcn_readlane(first, g) && r < __builtin_amdgcn_readlane(last, g);
+      found = in ? g : found;
+    }
+    return found;
+  }
+  __device__ __forceinline__ int32_t PagesOfLane(int32_t r) const {
+    int32_t found = 0;
+#pragma unroll 1
+    for (int32_t g = n - 1; g >= 0; --g) {
+      const bool in = r >= __builtin_amdgcn_readlane(first, g) && r < __builtin_amdgcn_readlane(last, g);
+      found = in ? __builtin_amdgcn_readlane(pages, g) : found;
+    }
+    return found;
+  }
+  // r the same in every lane.
+  __device__ __forceinline__ int32_t PagesOf(int32_t r) const {
+    const uint64_t in = __ballot(r >= first && r < last);
+    return in == 0 ? 0 : __builtin_amdgcn_readlane(pages, __builtin_ctzll(in));
+  }
+};
+
+// Whether a row of len positions begins with all of these pages: one that does not is attended to by itself.
+__device__ __forceinline__ bool TakesPart(int32_t pages, int32_t page_shift, int32_t len) {
+  return pages > 0 && pages <= (len >> page_shift);
 }
 
 }  // namespace dev

@@ -132,7 +132,10 @@ class PagedOpsC(ctypes.Structure):
                 ("kv_read", ctypes.CFUNCTYPE(_i32, _vp, _vp, _vp, _vp, _i64, _i32, _vp, _vp, _i64, _i64)),
                 ("attention", ctypes.CFUNCTYPE(_i32, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _vp, _vp, _i64)),
                 ("attention_workspace", ctypes.CFUNCTYPE(_i64, _i32, _i32, _i32)),
-                ("attention_workspace_init", ctypes.CFUNCTYPE(_i32, _vp, _i64))]
+                ("attention_workspace_init", ctypes.CFUNCTYPE(_i32, _vp, _i64)),
+                ("attention_shared", ctypes.CFUNCTYPE(_i32, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _i32, _i64, _vp, _vp,
+                                                      _i64)),
+                ("attention_shared_workspace", ctypes.CFUNCTYPE(_i64, _i32, _i32, _i32, _i64))]
 
 
 class RopeScalingC(ctypes.Structure):
@@ -1093,6 +1096,36 @@ def GpuAttentionPaged(kv: GpuPagedKv, table: GpuPageTable, lens, q, n_heads: int
         workspace_bytes = workspace.nbytes
     _check(_paged_call(kv, table).attention(
         kv.ref, table.ref, int_at(seq_ids, 4 * n_rows, "seq_ids"), int_at(lens, 4 * n_rows, "lens"),
+        float_at(q, span, "q"), n_heads, n_rows, float_at(out, span, "out"),
+        kv.at(dtype)(workspace, workspace_bytes, "workspace"), workspace_bytes))
+
+
+def GpuAttentionPagedSharedWorkspace(n_heads: int, n_kv_heads: int, head_dim: int, n_rows: int) -> int:
+    """Bytes of the workspace of GpuAttentionPagedShared for these heads and up to n_rows rows."""
+    return _check(paged_ops().attention_shared_workspace(n_heads, n_kv_heads, head_dim, n_rows))
+
+
+def GpuAttentionPagedShared(kv: GpuPagedKv, table: GpuPageTable, lens, group_rows, group_pages, q, n_heads: int,
+                            n_rows: int, out, workspace, seq_ids=None, workspace_bytes: Optional[int] = None,
+                            n_groups: Optional[int] = None) -> None:
+    """GpuAttentionPaged for a batch whose sequences share their beginnings: rows [group_rows[g], group_rows[g + 1])
+    form group g, whose sequences' tables begin with the same group_pages[g] pages, attended to once for the group.
+    group_rows [n_groups + 1] and group_pages [n_groups] are int32 tensors (n_groups goes with raw addresses), of at most
+    64 groups. The workspace is zero before its first call, and belongs to one call at a time."""
+    int_at, float_at = kv.int_at, kv.float_at
+    span = 4 * n_rows * n_heads * kv.head_dim
+    dtype = getattr(workspace, "dtype", None)
+    if workspace_bytes is None:
+        if dtype is None:
+            raise RpgError("GpuAttentionPagedShared: a raw workspace needs workspace_bytes")
+        workspace_bytes = workspace.nbytes
+    if n_groups is None:
+        if not hasattr(group_pages, "numel"):
+            raise RpgError("GpuAttentionPagedShared: raw groups need n_groups")
+        n_groups = group_pages.numel()
+    _check(_paged_call(kv, table).attention_shared(
+        kv.ref, table.ref, int_at(seq_ids, 4 * n_rows, "seq_ids"), int_at(lens, 4 * n_rows, "lens"),
+        int_at(group_rows, 4 * (n_groups + 1), "group_rows"), int_at(group_pages, 4 * n_groups, "group_pages"), n_groups,
         float_at(q, span, "q"), n_heads, n_rows, float_at(out, span, "out"),
         kv.at(dtype)(workspace, workspace_bytes, "workspace"), workspace_bytes))
 
