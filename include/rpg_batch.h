@@ -67,8 +67,8 @@ typedef struct {
    * the first always is. The token is the first in index order up to which the kept
    * weights add up to more than u times their sum; u is taken into [0, 1).
    * temperature <= 0 or NaN takes the first in order, with probability 1. A logit
-   * that is a NaN counts as minus infinity; a row of nothing else gives token -1 and
-   * probability 0. Beside rpg_op_sample_token_dev, whose random numbers
+   * that is a NaN counts as minus infinity, plus infinity as the largest finite
+   * number; a row of nothing but minus infinity gives token -1 and probability 0. Beside rpg_op_sample_token_dev, whose random numbers
    * rpg_sample_counter_uniform gives.
    *
    * workspace: sample_workspace bytes (negative on error), 256-byte aligned, zeroed

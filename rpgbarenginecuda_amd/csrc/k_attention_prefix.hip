@@ -310,12 +310,11 @@ __global__ __launch_bounds__(kThreads, 2) void SharedPrefixKernel(const PrefixAr
       if (lane == 0) st.bad[wave] = bad_new;
     };
 
-    // ---- kN tiles of 16 keys, from tile `from` of a step, against kT tiles of 16 columns
+    // ---- two tiles of 16 keys, from tile `from` of a step, against kT tiles of 16 columns
     const uint32_t k_at = static_cast<uint32_t>(n * kRow + 16 * (g ^ k_swap(n)));
     const uint32_t v_at = static_cast<uint32_t>((4 * g + (n >> 2)) * kRow + 16 * (((n & 3) >> 1) ^ v_swap(n >> 2)) + 8 * (n & 1));
-    const auto attend = [&](const Stage& st, uint32_t c, auto tiles_of_keys, auto tiles_of_cols) {
-      constexpr int kN = decltype(tiles_of_keys)::value, kT = decltype(tiles_of_cols)::value;
-      const int from = key_wave * kN;
+    const auto attend = [&](const Stage& st, uint32_t c, int from, auto tiles_of_cols) {
+      constexpr int kN = 2, kT = decltype(tiles_of_cols)::value;
       const int valid = min(kTiles, (positions - static_cast<int32_t>(c) * kStep) / 16) - from;
       if (valid <= 0) return;
       F32x4 s[kT][kN];
@@ -383,59 +382,55 @@ __global__ __launch_bounds__(kThreads, 2) void SharedPrefixKernel(const PrefixAr
         }
         safe[t] = m[t] == -INFINITY ? 0.0f : m[t];
       }
+      uint32_t w[kT][kQ8 ? 3 : 2][4];
 #pragma unroll
-      for (int j2 = 0; j2 < kN; j2 += 2) {
-        uint32_t w[kT][kQ8 ? 3 : 2][4];
+      for (int t = 0; t < kT; ++t) {
+#pragma unroll
+        for (int j = 0; j < kN; ++j) {
+          float p[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            p[i] = __builtin_amdgcn_exp2f(s[t][j][i] - safe[t]);
+            l[t] += p[i];
+          }
+          if constexpr (kQ8) {
+            const float by[4] = {vs[j].x, vs[j].y, vs[j].z, vs[j].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[i] *= by[i];
+#pragma unroll
+            for (int term = 0; term < 3; ++term) {
+              w[t][term][2 * j] = Uppers(p[0], p[1]);
+              w[t][term][2 * j + 1] = Uppers(p[2], p[3]);
+              if (term < 2) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) p[i] -= Upper(p[i]);
+              }
+            }
+          } else {
+            // weights of up to 2^4 times 2^11: what fp16's low end loses is below 2^-35
+            const Terms a = TermsOf(p[0] * 0x1p11f, p[1] * 0x1p11f), b = TermsOf(p[2] * 0x1p11f, p[3] * 0x1p11f);
+            w[t][0][2 * j] = a.hi;
+            w[t][0][2 * j + 1] = b.hi;
+            w[t][1][2 * j] = a.lo;
+            w[t][1][2 * j + 1] = b.lo;
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kE; ++i) {
+        const char* at = st.v + from * 16 * kRow + (v_at ^ (32u * i));
+        const uint2 a = ReadHalvesAcross(at), b = ReadHalvesAcross(at + 16 * kRow);
+        const Half8 v = AsHalf8(a.x, a.y, b.x, b.y);
 #pragma unroll
         for (int t = 0; t < kT; ++t) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int j = j2 + h;
-            float p[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              p[i] = __builtin_amdgcn_exp2f(s[t][j][i] - safe[t]);
-              l[t] += p[i];
-            }
+          for (int term = 0; term < (kQ8 ? 3 : 2); ++term) {
+            const Half8 p = AsHalf8(w[t][term][0], w[t][term][1], w[t][term][2], w[t][term][3]);
             if constexpr (kQ8) {
-              const float by[4] = {vs[j].x, vs[j].y, vs[j].z, vs[j].w};
-#pragma unroll
-              for (int i = 0; i < 4; ++i) p[i] *= by[i];
-#pragma unroll
-              for (int term = 0; term < 3; ++term) {
-                w[t][term][2 * h] = Uppers(p[0], p[1]);
-                w[t][term][2 * h + 1] = Uppers(p[2], p[3]);
-                if (term < 2) {
-#pragma unroll
-                  for (int i = 0; i < 4; ++i) p[i] -= Upper(p[i]);
-                }
-              }
+              acc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(BHalf8, v),
+                                                                  __builtin_bit_cast(BHalf8, p), acc[t][i], 0, 0, 0);
             } else {
-              // weights of up to 2^4 times 2^11: what fp16's low end loses is below 2^-35
-              const Terms a = TermsOf(p[0] * 0x1p11f, p[1] * 0x1p11f), b = TermsOf(p[2] * 0x1p11f, p[3] * 0x1p11f);
-              w[t][0][2 * h] = a.hi;
-              w[t][0][2 * h + 1] = b.hi;
-              w[t][1][2 * h] = a.lo;
-              w[t][1][2 * h + 1] = b.lo;
-            }
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < kE; ++i) {
-          const char* at = st.v + (from + j2) * 16 * kRow + (v_at ^ (32u * i));
-          const uint2 a = ReadHalvesAcross(at), b = ReadHalvesAcross(at + 16 * kRow);
-          const Half8 v = AsHalf8(a.x, a.y, b.x, b.y);
-#pragma unroll
-          for (int t = 0; t < kT; ++t) {
-#pragma unroll
-            for (int term = 0; term < (kQ8 ? 3 : 2); ++term) {
-              const Half8 p = AsHalf8(w[t][term][0], w[t][term][1], w[t][term][2], w[t][term][3]);
-              if constexpr (kQ8) {
-                acc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(BHalf8, v),
-                                                                    __builtin_bit_cast(BHalf8, p), acc[t][i], 0, 0, 0);
-              } else {
-                acc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p, acc[t][i], 0, 0, 0);
-              }
+              acc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p, acc[t][i], 0, 0, 0);
             }
           }
         }
@@ -456,13 +451,14 @@ __global__ __launch_bounds__(kThreads, 2) void SharedPrefixKernel(const PrefixAr
         next_page = page_of(min(c + 2, c1 - 1));
       }
       if (works) {
-        using std::integral_constant;
-        if (key_waves == 2) {
-          attend(st, c, integral_constant<int, 4>{}, integral_constant<int, 2>{});
-        } else if (tile_cols > 16) {
-          attend(st, c, integral_constant<int, 2>{}, integral_constant<int, 2>{});
-        } else {
-          attend(st, c, integral_constant<int, 2>{}, integral_constant<int, 1>{});
+        const int each = kTiles / key_waves;
+#pragma unroll 1
+        for (int from = key_wave * each; from < (key_wave + 1) * each; from += 2) {
+          if (tile_cols > 16) {
+            attend(st, c, from, std::integral_constant<int, 2>{});
+          } else {
+            attend(st, c, from, std::integral_constant<int, 1>{});
+          }
         }
       }
       if (more) store(stages[(c + 1 - c0) & 1]);

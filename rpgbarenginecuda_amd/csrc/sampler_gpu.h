@@ -86,12 +86,13 @@ void GpuSamplerWarmup();
 // The token is the first in index order up to which the kept weights add up to more
 // than u times their sum. u is taken into [0, 1), a NaN as 0. temperature <= 0 or NaN
 // takes the first in order, with probability 1. A NaN logit counts as minus infinity,
-// whose weight is 0; a row of nothing else gives token -1 and probability 0. Where the
-// largest is plus infinity all others weigh 0.
+// whose weight is 0, plus infinity as the largest finite number; a row of nothing but
+// minus infinity gives token -1 and probability 0.
 //
-// Weights are formed in double (within 2^-50 of their value) and summed as integers of
-// 2^-s, s = 62 - ceil(log2 n), so that no order of summing shows and ties add up to
-// what they should: borders lie within n 2^-(s+1) of where exact weights have them.
+// Weights are formed in double, within 2^-36 of their value, and summed in units of
+// 2^-38 of the largest, as integers, so that no order of summing shows and ties add up
+// to what they should: a sum of weights, and with it a border, lies within n 2^-39 +
+// 2^-36 of the whole of where exact weights have it (typically within 10^-9).
 struct SampleBatchOptions {
   // device arrays of n_rows, each may be null: 1, off, off, off
   const float* temperature = nullptr;

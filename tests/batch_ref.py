@@ -9,9 +9,9 @@ import numpy as np
 def sample(x, t, k, p, m, u, exact_sums=False):
     """What may come of one row: a list of (token, probability).
 
-    Weights are rounded to whole numbers of 2^-s of the largest, s = 62 - ceil(log2 n): each is off by half of that, a sum
-    of them by n 2^-(s+1) at most, and the sums here by n 2^-52 of their value. Where a border is nearer than that, either
-    side of it is allowed; exact_sums (for weights that are small whole numbers of a power of two) leaves no such room."""
+    Weights are within 2^-36 of their value and rounded to units of 2^-38 of the largest: a sum of n is off by n 2^-39 and
+    2^-36 of it at most, and the sums here by n 2^-52 of their value. Where a border is nearer than that, either side of it
+    is allowed; exact_sums (for weights that are small whole numbers of a power of two) leaves no such room."""
     n = len(x)
     x = np.where(np.isnan(x), -np.inf, np.asarray(x, np.float64)) + 0.0
     live = np.flatnonzero(x > -np.inf)
@@ -26,8 +26,7 @@ def sample(x, t, k, p, m, u, exact_sums=False):
     with np.errstate(all="ignore"):
         w = np.exp(np.where(x[ranked] == top, 0.0, (x[ranked] - top) / np.float64(t)))
     w = np.where(np.isnan(w), 0.0, w)
-    bits = max(0, math.ceil(math.log2(n)))
-    near = 0.0 if exact_sums else n * 2.0 ** (bits - 63) + n * 2.0 ** -52 * w.sum()
+    near = 0.0 if exact_sums else n * 2.0 ** -39 + (n * 2.0 ** -52 + 2.0 ** -36) * w.sum()
     upto = np.cumsum(w)
     counts = {len(w)}
     if 0 < p < 1:
@@ -35,7 +34,7 @@ def sample(x, t, k, p, m, u, exact_sums=False):
         counts = {min(len(w), 1 + int(np.searchsorted(upto, g))) for g in (goal - near, goal, goal + near)}
     least = {0.0}
     if m > 0:
-        least = {min(np.float64(m), 1.0) * f for f in ((1.0,) if exact_sums else (1 - 2.0 ** -45, 1.0, 1 + 2.0 ** -45))}
+        least = {min(np.float64(m), 1.0) * f for f in ((1.0,) if exact_sums else (1 - 2.0 ** -35, 1.0, 1 + 2.0 ** -35))}
         least = {min(v, 1.0) for v in least}
     found = []
     u = u if u > 0 else 0.0
