@@ -1,16 +1,15 @@
 // The next tokens of a batch of conversations, from given random numbers (the semantics
 // are listed in sampler_gpu.h).
 //
-// Three launches, the first of which reads the logits once, in slices of 4096:
-//   SampleSlices   each workgroup keeps a slice in registers: its largest value m_s, and of what its weights
+// Two launches, the first of which reads the logits once, in slices of 4096:
+//   SampleSlices   a workgroup for each keeps it in registers: its largest value m_s, and of what its weights
 //                  2^((x - m_s) log2(e) / T) come to, sums by value: bins an eighth of an octave wide (a twelfth of a nat,
-//                  for T above 1), whose borders are the same in all slices, counted and weighed upwards from the top. The
-//                  row's last workgroup to arrive joins the slices, each by 2^((m_s - m) log2(e) / T), and finds between
-//                  which bins each filter cuts: what lies above these bins is kept, what lies below is not;
-//   SampleCollect  what lies in them (some dozen to a few thousand values) is collected, in index order, from the slices that
-//                  have any;
-//   SampleChoose   a workgroup for each row cuts there exactly, by radix selection, adds up the slices' kept weights, finds
-//                  u's place among them and walks that one slice.
+//                  for T above 1), whose borders are the same in all slices, counted and weighed upwards from the top;
+//                  and each value's bin, a byte;
+//   SampleChoose   a workgroup for each row joins the slices, each by 2^((m_s - m) log2(e) / T), and finds between which
+//                  bins each filter cuts: what lies above these bins is kept, what lies below is not. The values in them
+//                  (some dozen to a few thousand) it collects by their bytes, and cuts there exactly, by radix selection;
+//                  it adds up the slices' kept weights, finds u's place among them, and walks that one slice.
 // Weights are formed in double, which on this card costs what fp32 does, and summed as integers wherever atomics or a
 // border depend on it, so that results are the same from run to run.
 //
@@ -37,16 +36,15 @@ using namespace block;
 constexpr int kSlice = 4096;
 constexpr int kEach = kSlice / kThreads;
 constexpr int kMaxSlices = static_cast<int>(kSamplerMaxVocab / kSlice);
-constexpr int kSlicesEach = kMaxSlices / kThreads;
+constexpr int kRowThreads = 1024;  // of a workgroup for a row
+constexpr int kRowWaves = kRowThreads / 64;
+static_assert(kMaxSlices <= kRowThreads, "a slice to a thread");
 constexpr int kBins = 256;         // of a slice; the last has all that is further down
 constexpr int kInLds = 8192;       // candidates that are kept there
-constexpr int kRowsAtOnce = 2048;  // rows of a launch: their counters have a place of their own in the workspace
-constexpr int kCounterBytes = 128;
 // A slice's sums, in one number: count in the upper 13 bits, weight in units of 2^-38 of its largest in the lower 51.
 constexpr int kWeightBits = 51;
 constexpr int kSliceUnits = 38;
 static_assert((int64_t(kSlice) << kSliceUnits) < (int64_t(1) << kWeightBits) && kSlice < (1 << (64 - kWeightBits)), "");
-constexpr int kDevicePolicy = 16;  // of stores that the last workgroup to arrive reads
 
 // ---------------------------------------------------------------- order and weights
 
@@ -63,34 +61,53 @@ __device__ __forceinline__ float ValueOf(uint32_t key) {
 }
 
 // 2^f for f in [-1/2, 1/2], 1 + f g(f) with g the polynomial of degree 7 through 2^f's own at the Chebyshev nodes: within
-// 2^-38 of the value, and exactly 1 at 0.
-__device__ __forceinline__ double Exp2Near(double f) {
-  double p = fma(0x1.63b2d797a3663p-20, f, 0x1.00c0e4e151fbep-16);
-  p = fma(p, f, 0x1.4308c7183cd99p-13);
-  p = fma(p, f, 0x1.5d877598350dap-10);
-  p = fma(p, f, 0x1.3b2ab70ad256bp-7);
-  p = fma(p, f, 0x1.c6b08da70cce3p-5);
-  p = fma(p, f, 0x1.ebfbdff82a734p-3);
-  p = fma(p, f, 0x1.62e42fef9cc69p-1);
-  return fma(p, f, 1.0);
-}
+// 2^-38 of the value, and exactly 1 at 0. The coefficients, times 2^kBits, in scalar registers: written as constants, the
+// compiler moves each to a vector register for every use.
+template <int kBits>
+struct Exp2Near {
+  double c[9];
+  __device__ __forceinline__ Exp2Near() {
+    constexpr double kC[9] = {1.0,
+                              0x1.62e42fef9cc69p-1,
+                              0x1.ebfbdff82a734p-3,
+                              0x1.c6b08da70cce3p-5,
+                              0x1.3b2ab70ad256bp-7,
+                              0x1.5d877598350dap-10,
+                              0x1.4308c7183cd99p-13,
+                              0x1.00c0e4e151fbep-16,
+                              0x1.63b2d797a3663p-20};
+#pragma unroll
+    for (int i = 0; i < 9; ++i) {
+      c[i] = kC[i] * static_cast<double>(uint64_t(1) << kBits);
+      asm volatile("" : "+s"(c[i]));
+    }
+  }
+  __device__ __forceinline__ double Of(double f) const {
+    double p = fma(c[8], f, c[7]);
+#pragma unroll
+    for (int i = 6; i >= 0; --i) p = fma(p, f, c[i]);
+    return p;
+  }
+};
 // 2^(v + bits) for v <= 0; below 2^-1000, and for a NaN, next to nothing.
-__device__ __forceinline__ double Exp2Down(double v, int bits) {
+__device__ __forceinline__ double Exp2Down(const Exp2Near<0>& near, double v, int bits) {
   v = fmax(v, -1000.0);
   const double k = rint(v);
-  return ldexp(Exp2Near(v - k), static_cast<int>(k) + bits);
+  return ldexp(near.Of(v - k), static_cast<int>(k) + bits);
 }
 // A slice's sum of one value of weight 2^v, v <= 0 (any that counts for nothing, down to minus infinity).
-__device__ __forceinline__ uint64_t OneOf(double v) {
+__device__ __forceinline__ uint64_t OneOf(const Exp2Near<kSliceUnits>& near, double v) {
   v = fmax(v, -200.0);
   // 1.5 * 2^52 added rounds v to a whole number, the low word; 2^52 added to a weight leaves its whole units
   const double shifted = v + 0x1.8p52;
-  const int k = static_cast<int>(__builtin_bit_cast(uint64_t, shifted));
-  const uint64_t near = __builtin_bit_cast(uint64_t, Exp2Near(v - (shifted - 0x1.8p52)));
-  const double scaled =
-      __builtin_bit_cast(double, near + (static_cast<uint64_t>(static_cast<uint32_t>(k + kSliceUnits) << 20) << 32));
-  const uint64_t bits = __builtin_bit_cast(uint64_t, scaled + 0x1p52);
-  return bits - (uint64_t(0x43300000u - (1u << (kWeightBits - 32))) << 32);
+  const uint64_t part = __builtin_bit_cast(uint64_t, near.Of(v - (shifted - 0x1.8p52)));
+  const uint32_t exponent = static_cast<uint32_t>(__builtin_bit_cast(uint64_t, shifted)) << 20;
+  const uint64_t scaled = (static_cast<uint64_t>(static_cast<uint32_t>(part >> 32) + exponent) << 32) |
+                          static_cast<uint32_t>(part);
+  const uint64_t bits = __builtin_bit_cast(uint64_t, __builtin_bit_cast(double, scaled) + 0x1p52);
+  constexpr uint32_t kOne = 1u << (kWeightBits - 32);
+  return (static_cast<uint64_t>(static_cast<uint32_t>(bits >> 32) - (0x43300000u - kOne)) << 32) |
+         static_cast<uint32_t>(bits);
 }
 __device__ __forceinline__ uint32_t CountOf(uint64_t sum) { return static_cast<uint32_t>(sum >> kWeightBits); }
 __device__ __forceinline__ double WeightOf(uint64_t sum) {
@@ -131,7 +148,6 @@ struct SampleArgs {
   int32_t* tokens;
   float* probs;
   char* workspace;
-  int32_t first_row;
 };
 
 __device__ __forceinline__ Setting SettingOf(const SampleArgs& a, int64_t r) {
@@ -155,32 +171,16 @@ struct SliceSums {  // of one slice
   uint64_t sum;
 };
 
-enum class Kind : int32_t { kDone, kAll, kCut };
-struct Plan {  // what the first launch finds out for the others
-  Kind kind;
-  float top;
-  int32_t top_bin;
-  int32_t hi, lo;                // the bins below the row's top one that are collected
-  uint32_t cut_k, cut_p, cut_m;  // filters that may cut there; cut_p 2: of what top_k leaves
-  uint32_t base_count;           // values above these bins
-  uint32_t candidates;
-  double base;                   // their weight
-  double all;                    // the weight of all
-};
-
 __host__ __device__ constexpr int64_t RoundUp(int64_t x) { return (x + 127) / 128 * 128; }
 struct RowPlace {
-  int64_t sums, above, offsets, bins, keys, bytes;  // the plan is in front
+  int64_t bins, bytes_of, keys, size;  // the slices' sums are in front
   __host__ __device__ explicit RowPlace(int32_t slices) {
-    sums = RoundUp(sizeof(Plan));
-    above = sums + RoundUp(slices * sizeof(SliceSums));
-    offsets = above + RoundUp(slices * 8);
-    bins = offsets + RoundUp((slices + 1) * 4);
-    keys = bins + RoundUp(static_cast<int64_t>(slices) * kBins * 8);
-    bytes = keys + static_cast<int64_t>(slices) * kSlice * 4;
+    bins = RoundUp(slices * sizeof(SliceSums));
+    bytes_of = bins + static_cast<int64_t>(slices) * kBins * 8;
+    keys = bytes_of + static_cast<int64_t>(slices) * kSlice;
+    size = keys + static_cast<int64_t>(slices) * kSlice * 4;
   }
 };
-constexpr int64_t kCounters = static_cast<int64_t>(kRowsAtOnce) * kCounterBytes;
 
 struct Row {  // of the logits and the workspace
   int64_t r;
@@ -189,20 +189,20 @@ struct Row {  // of the logits and the workspace
   __amdgpu_buffer_rsrc_t logits;
   int32_t n;
 
-  __device__ __forceinline__ Row(const SampleArgs& a, uint32_t in_launch)
-      : r(a.first_row + static_cast<int64_t>(in_launch)),
+  __device__ __forceinline__ Row(const SampleArgs& a, uint32_t row)
+      : r(row),
         place(a.slices),
-        at(a.workspace + kCounters + in_launch * place.bytes),
+        at(a.workspace + row * place.size),
         logits(dev::OutResource(const_cast<float*>(a.logits) + r * a.row_stride, 4u * static_cast<uint32_t>(a.n))),
         n(a.n) {}
-  __device__ __forceinline__ Plan* ThePlan() const { return reinterpret_cast<Plan*>(at); }
-  __device__ __forceinline__ SliceSums* Sums() const { return reinterpret_cast<SliceSums*>(at + place.sums); }
-  __device__ __forceinline__ double* Above() const { return reinterpret_cast<double*>(at + place.above); }
-  __device__ __forceinline__ int32_t* Offsets() const { return reinterpret_cast<int32_t*>(at + place.offsets); }
+  __device__ __forceinline__ SliceSums* Sums() const { return reinterpret_cast<SliceSums*>(at); }
   // Of slice s, the sums of its bins down to each.
   __device__ __forceinline__ uint64_t* Bins(int s) const {
     return reinterpret_cast<uint64_t*>(at + place.bins) + static_cast<int64_t>(s) * kBins;
   }
+  // Of slice s, each value's bin.
+  __device__ __forceinline__ char* BytesOf(int s) const { return at + place.bytes_of + static_cast<int64_t>(s) * kSlice; }
+  // Candidates that do not fit into LDS.
   __device__ __forceinline__ uint32_t* Keys() const { return reinterpret_cast<uint32_t*>(at + place.keys); }
   // Four logits from i on; what lies behind the row's end is minus infinity.
   __device__ __forceinline__ float4 Load(int32_t i) const {
@@ -210,211 +210,17 @@ struct Row {  // of the logits and the workspace
     return make_float4(i < n ? Clean(x.x) : -INFINITY, i + 1 < n ? Clean(x.y) : -INFINITY,
                        i + 2 < n ? Clean(x.z) : -INFINITY, i + 3 < n ? Clean(x.w) : -INFINITY);
   }
+  __device__ __forceinline__ float LoadOne(int32_t i) const {
+    return i < n ? Clean(dev::LoadBuf1<0>(logits, 4u * static_cast<uint32_t>(i))) : -INFINITY;
+  }
 };
-
-// ---------------------------------------------------------------- a workgroup's sums
-
-__device__ __forceinline__ uint64_t BlockSum(uint64_t x, uint64_t* sh) {
-  uint64_t total;
-  BlockExclScan(x, sh, &total);
-  return total;
-}
-__device__ __forceinline__ uint64_t BlockMaxU64(uint64_t x, uint64_t* sh) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    const uint64_t o = __shfl_xor(x, off, 64);
-    x = o > x ? o : x;
-  }
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = x;
-  __syncthreads();
-  uint64_t r = sh[0];
-#pragma unroll
-  for (int w = 1; w < kWaves; ++w) r = sh[w] > r ? sh[w] : r;
-  __syncthreads();
-  return r;
-}
-// The sum of doubles over the threads before this one, in one order; *total that over all.
-__device__ __forceinline__ double BlockBeforeD(double x, double* sh, double* total) {
-  double upto = x;
-  upto += DppDbl<0x111>(upto, 0.0);
-  upto += DppDbl<0x112>(upto, 0.0);
-  upto += DppDbl<0x114>(upto, 0.0);
-  upto += DppDbl<0x118>(upto, 0.0);
-  upto += DppDbl<0x142, 0xA>(upto, 0.0);
-  upto += DppDbl<0x143, 0xC>(upto, 0.0);
-  const double mine = __shfl_up(upto, 1, 64);
-  if ((threadIdx.x & 63) == 63) sh[threadIdx.x >> 6] = upto;
-  __syncthreads();
-  double base = 0.0, all = 0.0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    if (w == static_cast<int>(threadIdx.x >> 6)) base = all;
-    all += sh[w];
-  }
-  __syncthreads();
-  *total = all;
-  return (threadIdx.x & 63) == 0 ? base : base + mine;
-}
 
 // ---------------------------------------------------------------- the slices
 
-struct JoinShared {
-  double scale[kMaxSlices];  // of a slice's weights
-  int32_t off[kMaxSlices];   // bins that a slice's top one lies below the row's, at most all
-  double weight[kBins];      // of all bins down to one
-  uint32_t count[kBins];
-  uint32_t found[4];
-};
-
-// The row's last workgroup: where its filters cut.
-__device__ __forceinline__ void JoinSlices(const SampleArgs& a, const Setting& set, const Row& row, JoinShared& sh,
-                                           uint64_t* parts, double* dparts, float* fparts) {
-  const int tid = threadIdx.x;
-  SliceSums mine[kSlicesEach];
-  float top = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < kSlicesEach; ++i) {
-    const int s = tid + i * kThreads;
-    mine[i] = s < a.slices ? row.Sums()[s] : SliceSums{-INFINITY, 0, 0};
-    top = fmaxf(top, mine[i].top);
-  }
-  top = BlockMax(top, fparts);
-  if (top == -INFINITY || set.greedy) {
-    uint64_t first = 0;
-#pragma unroll
-    for (int i = 0; i < kSlicesEach; ++i) {
-      if (mine[i].top == top) first = max(first, static_cast<uint64_t>(0x7FFFFFFF - mine[i].top_index));
-    }
-    first = BlockMaxU64(first, parts);
-    if (tid == 0) {
-      const bool none = top == -INFINITY;
-      a.tokens[row.r] = none ? -1 : 0x7FFFFFFF - static_cast<int32_t>(first);
-      if (a.probs != nullptr) a.probs[row.r] = none ? 0.0f : 1.0f;
-      row.ThePlan()->kind = Kind::kDone;
-    }
-    return;
-  }
-  const int32_t top_bin = set.BinOf(top);
-  double all = 0.0;
-  uint64_t live = 0;
-#pragma unroll
-  for (int i = 0; i < kSlicesEach; ++i) {
-    const int s = tid + i * kThreads;
-    if (s < a.slices) {
-      const bool any = mine[i].top > -INFINITY;
-      const double scale =
-          any ? Exp2Down((static_cast<double>(mine[i].top) - static_cast<double>(top)) * set.by, 0) : 0.0;
-      sh.scale[s] = scale;
-      sh.off[s] = any ? set.BinBelow(top_bin, mine[i].top) : kBins - 1;
-      all += scale * WeightOf(mine[i].sum);
-      live += CountOf(mine[i].sum);
-    }
-  }
-  if (tid < 4) sh.found[tid] = kBins - 1;
-  all = BlockSumD(all, dparts);
-  live = BlockSum(live, parts);
-
-  // a slice's sum over the row's bins down to j
-  const auto sum_at = [&](int s, int j) -> uint64_t {
-    const int in_slice = j == kBins - 1 ? j : j - sh.off[s];
-    return in_slice >= 0 ? row.Bins(s)[in_slice] : 0;
-  };
-  const bool on_k = set.k > 0 && static_cast<uint64_t>(set.k) < live, on_p = set.OnP(), on_m = set.m > 0.0f;
-  if (!on_k && !on_p && !on_m) {
-#pragma unroll
-    for (int i = 0; i < kSlicesEach; ++i) {
-      const int s = tid + i * kThreads;
-      if (s < a.slices) row.Above()[s] = sh.scale[s] * WeightOf(mine[i].sum);
-    }
-    if (tid == 0) *row.ThePlan() = Plan{Kind::kAll, top, top_bin, kBins, kBins, 0, 0, 0, 0, 0, 0.0, all};
-    return;
-  }
-  double weight = 0.0;
-  uint32_t count = 0;
-  static_assert(kThreads == kBins, "a bin to a thread");
-  constexpr int kBatch = 16;
-#pragma unroll 1
-  for (int s0 = 0; s0 < a.slices; s0 += kBatch) {
-    uint64_t sums[kBatch];
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) sums[i] = s0 + i < a.slices ? sum_at(s0 + i, tid) : 0;
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      if (s0 + i < a.slices) weight += sh.scale[s0 + i] * WeightOf(sums[i]);
-      count += CountOf(sums[i]);
-    }
-  }
-  sh.weight[tid] = weight;
-  sh.count[tid] = count;
-  __syncthreads();
-  const uint32_t before_count = tid == 0 ? 0 : sh.count[tid - 1];
-  const double before_weight = tid == 0 ? 0.0 : sh.weight[tid - 1];
-  // top_k's bin
-  const uint32_t k = static_cast<uint32_t>(set.k);
-  if (on_k && before_count < k && k <= count) sh.found[0] = static_cast<uint32_t>(tid);
-  __syncthreads();
-  const int bin_k = on_k ? static_cast<int>(sh.found[0]) : kBins - 1;
-  // top_p's: between those of the least and the most that what top_k leaves may weigh, and a rounding more
-  const double most = sh.weight[bin_k], least = !on_k ? most : bin_k == 0 ? 0.0 : sh.weight[bin_k - 1];
-  const double p = static_cast<double>(set.p);
-  const double goal_hi = p * least * (1.0 - 0x1p-40), goal_lo = fmin(p * most * (1.0 + 0x1p-40), most);
-  if (on_p && weight >= goal_hi && (tid == 0 || before_weight < goal_hi)) sh.found[1] = static_cast<uint32_t>(tid);
-  if (on_p && weight >= goal_lo && (tid == 0 || before_weight < goal_lo)) sh.found[2] = static_cast<uint32_t>(tid);
-  __syncthreads();
-  const int p_hi = static_cast<int>(sh.found[1]), p_lo = static_cast<int>(sh.found[2]);
-  // min_p's: from the next number above its border to the next below
-  int m_hi = kBins - 1, m_lo = kBins - 1;
-  if (on_m) {
-    const double border = static_cast<double>(top) + log(static_cast<double>(set.m)) * static_cast<double>(set.t);
-    const float near = static_cast<float>(fmax(border, -static_cast<double>(FLT_MAX)));
-    m_hi = set.BinBelow(top_bin, fminf(nextafterf(near, INFINITY), top));
-    m_lo = set.BinBelow(top_bin, nextafterf(near, -INFINITY));
-  }
-
-  // The cut that counts is the highest: filters that start below where another has cut for sure do not matter. top_p's
-  // place needs what top_k leaves, and so the bins down to its.
-  const int sure = min(on_k ? bin_k : kBins - 1, min(on_p ? p_lo : kBins - 1, m_lo));
-  const bool cut_k = on_k && bin_k <= sure, cut_p = on_p && p_hi <= sure, cut_m = on_m && m_hi <= sure;
-  int hi = kBins - 1, lo = 0;
-  if (cut_k) hi = min(hi, bin_k), lo = max(lo, bin_k);
-  if (cut_p) hi = min(hi, p_hi), lo = max(lo, on_k ? bin_k : p_lo);
-  if (cut_m) hi = min(hi, m_hi), lo = max(lo, m_lo);
-
-  // of each slice: the weight above these bins, and where its values in them go
-  uint32_t placed = 0;
-#pragma unroll 1
-  for (int s0 = 0; s0 < a.slices; s0 += kThreads) {
-    const int s = s0 + tid;
-    uint64_t in = 0;
-    if (s < a.slices) {
-      const uint64_t above = hi > 0 ? sum_at(s, hi - 1) : 0, upto = sum_at(s, lo);
-      row.Above()[s] = sh.scale[s] * WeightOf(above);
-      in = CountOf(upto) - CountOf(above);
-    }
-    uint64_t sum;
-    const uint64_t before = BlockExclScan(in, parts, &sum);
-    if (s < a.slices) row.Offsets()[s] = static_cast<int32_t>(placed + before);
-    placed += static_cast<uint32_t>(sum);
-  }
-  if (tid == 0) {
-    row.Offsets()[a.slices] = static_cast<int32_t>(placed);
-    *row.ThePlan() = Plan{Kind::kCut, top, top_bin, hi, lo, cut_k ? 1u : 0u, cut_p ? (on_k ? 2u : 1u) : 0u,
-                          cut_m ? 1u : 0u, hi > 0 ? sh.count[hi - 1] : 0u, placed, hi > 0 ? sh.weight[hi - 1] : 0.0,
-                          sh.weight[kBins - 1]};
-  }
-}
-
 // Grid: slices times rows.
 __global__ __launch_bounds__(kThreads) void SampleSlicesKernel(const SampleArgs a) {
-  struct SliceShared {
-    uint64_t bins[kWaves][kBins];
-  };
-  __shared__ union {
-    SliceShared slice;
-    JoinShared join;
-  } sh;
+  __shared__ uint64_t bins[kWaves][kBins];
   __shared__ uint64_t parts[kWaves];
-  __shared__ double dparts[kWaves];
   __shared__ float fparts[kWaves];
   __shared__ int first;
   const int tid = threadIdx.x;
@@ -430,114 +236,141 @@ __global__ __launch_bounds__(kThreads) void SampleSlicesKernel(const SampleArgs 
   const Setting set = SettingOf(a, row.r);
   const bool filters = !set.greedy && set.Filters();
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) sh.slice.bins[w][tid] = 0;
+  for (int w = 0; w < kWaves; ++w) bins[w][tid] = 0;
   if (tid == 0) first = 0x7FFFFFFF;
   float top = x[0];
 #pragma unroll
   for (int i = 1; i < kEach; ++i) top = fmaxf(top, x[i]);
   top = BlockMax(top, fparts);
   uint64_t sum = 0;
+  const Exp2Near<kSliceUnits> near;
+  const double dtop = static_cast<double>(top);
   if (set.greedy) {
 #pragma unroll
     for (int i = kEach - 1; i >= 0; --i) {
       if (x[i] == top) atomicMin(&first, slice * kSlice + (i & ~3) * kThreads + 4 * tid + (i & 3));
     }
     __syncthreads();
-  } else {
+  } else if (filters) {
     const int32_t top_bin = set.BinOf(top);
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      if (x[i] == -INFINITY) continue;
-      const uint64_t add = OneOf((static_cast<double>(x[i]) - static_cast<double>(top)) * set.by);
-      if (filters) {
-        atomicAdd(reinterpret_cast<unsigned long long*>(&sh.slice.bins[tid >> 6][set.BinBelow(top_bin, x[i])]),
-                  static_cast<unsigned long long>(add));
-      } else {
-        sum += add;
-      }
-    }
-    if (filters) {
-      __syncthreads();
-      uint64_t mine = 0;
+    for (int i = 0; i < kEach; i += 4) {
+      uint32_t bytes = 0;
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) mine += sh.slice.bins[w][tid];
-      const uint64_t before = BlockExclScan(mine, parts, &sum);
-      __hip_atomic_store(row.Bins(slice) + tid, before + mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    } else {
-      sum = BlockSum(sum, parts);
+      for (int c = 0; c < 4; ++c) {
+        const int j = x[i + c] > -INFINITY ? set.BinBelow(top_bin, x[i + c]) : kBins - 1;
+        const uint64_t add = OneOf(near, (static_cast<double>(x[i + c]) - dtop) * set.by);
+        if (x[i + c] > -INFINITY) {
+          atomicAdd(reinterpret_cast<unsigned long long*>(&bins[tid >> 6][j]), static_cast<unsigned long long>(add));
+        }
+        bytes |= static_cast<uint32_t>(j) << (8 * c);
+      }
+      *reinterpret_cast<uint32_t*>(row.BytesOf(slice) + i * kThreads + 4 * tid) = bytes;
     }
+    __syncthreads();
+    uint64_t mine = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) mine += bins[w][tid];
+    const uint64_t before = BlockExclScan(mine, parts, &sum);
+    row.Bins(slice)[tid] = before + mine;
+  } else {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const uint64_t add = OneOf(near, (static_cast<double>(x[i]) - dtop) * set.by);
+      sum += x[i] > -INFINITY ? add : 0;
+    }
+    uint64_t total;
+    BlockExclScan(sum, parts, &total);
+    sum = total;
   }
-  if (tid == 0) {
-    const __amdgpu_buffer_rsrc_t rs = dev::OutResource(row.Sums() + slice, sizeof(SliceSums));
-    dev::StoreBufU4<kDevicePolicy>(rs, 0, make_uint4(__float_as_uint(top), static_cast<uint32_t>(first),
-                                                     static_cast<uint32_t>(sum), static_cast<uint32_t>(sum >> 32)));
-  }
-  // stored at device scope, acknowledged, counted: the last one sees all of it behind its fence
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  if (tid == 0) first = attn::Count(a.workspace, in_launch * (kCounterBytes / 4), static_cast<uint32_t>(a.slices));
-  __syncthreads();
-  if (__builtin_amdgcn_readfirstlane(first) == 0) return;
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-  JoinSlices(a, set, row, sh.join, parts, dparts, fparts);
+  if (tid == 0) row.Sums()[slice] = SliceSums{top, first, sum};
 }
 
-// ---------------------------------------------------------------- the candidates
+// ---------------------------------------------------------------- a row's sums
 
-// Grid: slices times rows. In index order: four rounds of four neighbours to a thread, whose counts are summed as one number.
-__global__ __launch_bounds__(kThreads) void SampleCollectKernel(const SampleArgs a) {
-  __shared__ uint64_t parts[kWaves];
-  const int tid = threadIdx.x;
-  const uint32_t in_launch = blockIdx.x / static_cast<uint32_t>(a.slices);
-  const int slice = static_cast<int>(blockIdx.x - in_launch * static_cast<uint32_t>(a.slices));
-  const Row row(a, in_launch);
-  const Plan plan = *row.ThePlan();
-  const int32_t to = row.Offsets()[slice], end = row.Offsets()[slice + 1];
-  if (plan.kind != Kind::kCut || to == end) return;
-  const Setting set = SettingOf(a, row.r);
-  float x[kEach];
+__device__ __forceinline__ uint64_t RowMax(uint64_t x, uint64_t* sh) {
 #pragma unroll
-  for (int i = 0; i < kEach; i += 4) {
-    const float4 v = row.Load(slice * kSlice + i * kThreads + 4 * tid);
-    x[i] = v.x, x[i + 1] = v.y, x[i + 2] = v.z, x[i + 3] = v.w;
+  for (int off = 32; off > 0; off >>= 1) {
+    const uint64_t o = __shfl_xor(x, off, 64);
+    x = o > x ? o : x;
   }
-  uint32_t in = 0;
-  uint64_t counts = 0;
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = x;
+  __syncthreads();
+  uint64_t r = sh[0];
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const int j = set.BinBelow(plan.top_bin, x[i]);
-    const bool takes = x[i] > -INFINITY && j >= plan.hi && j <= plan.lo;
-    in |= takes ? 1u << i : 0u;
-    counts += takes ? uint64_t(1) << (16 * (i / 4)) : 0;
+  for (int w = 1; w < kRowWaves; ++w) r = sh[w] > r ? sh[w] : r;
+  __syncthreads();
+  return r;
+}
+// The sum over the threads before this one; *total that over all.
+__device__ __forceinline__ uint64_t RowBefore(uint64_t x, uint64_t* sh, uint64_t* total) {
+  const uint64_t upto = WaveInclScanU64(x);
+  if ((threadIdx.x & 63) == 63) sh[threadIdx.x >> 6] = upto;
+  __syncthreads();
+  uint64_t before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kRowWaves; ++w) {
+    if (w == static_cast<int>(threadIdx.x >> 6)) before = all;
+    all += sh[w];
   }
+  __syncthreads();
+  *total = all;
+  return before + upto - x;
+}
+__device__ __forceinline__ uint64_t RowSum(uint64_t x, uint64_t* sh) {
   uint64_t total;
-  const uint64_t before = BlockExclScan(counts, parts, &total);
-  uint32_t* const keys = row.Keys() + to;
-  uint32_t round = 0;
+  RowBefore(x, sh, &total);
+  return total;
+}
+// The same of doubles, in one order.
+__device__ __forceinline__ double RowBeforeD(double x, double* sh, double* total) {
+  double upto = x;
+  upto += DppDbl<0x111>(upto, 0.0);
+  upto += DppDbl<0x112>(upto, 0.0);
+  upto += DppDbl<0x114>(upto, 0.0);
+  upto += DppDbl<0x118>(upto, 0.0);
+  upto += DppDbl<0x142, 0xA>(upto, 0.0);
+  upto += DppDbl<0x143, 0xC>(upto, 0.0);
+  const double mine = __shfl_up(upto, 1, 64);
+  if ((threadIdx.x & 63) == 63) sh[threadIdx.x >> 6] = upto;
+  __syncthreads();
+  double base = 0.0, all = 0.0;
 #pragma unroll
-  for (int i = 0; i < kEach; i += 4) {
-    uint32_t next = round + static_cast<uint32_t>(before >> (4 * i) & 0xFFFF);
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      if (in >> (i + c) & 1) keys[next++] = KeyOf(x[i + c]);
-    }
-    round += static_cast<uint32_t>(total >> (4 * i) & 0xFFFF);
+  for (int w = 0; w < kRowWaves; ++w) {
+    if (w == static_cast<int>(threadIdx.x >> 6)) base = all;
+    all += sh[w];
   }
+  __syncthreads();
+  *total = all;
+  return (threadIdx.x & 63) == 0 ? base : base + mine;
 }
 
 // ---------------------------------------------------------------- the choice
 
+constexpr int kJoiners = kRowThreads / kBins;  // threads to a bin, each for every kJoiners-th slice
+
 struct ChooseShared {
-  uint32_t keys[kInLds];
-  uint64_t bins[256];
+  union {
+    uint32_t keys[kInLds];
+    struct {
+      double weight[kJoiners][kBins];
+      uint32_t count[kJoiners][kBins];
+    } join;
+  };
+  double weight[kBins];  // of all bins down to one
+  uint32_t count[kBins];
+  uint64_t digits[256];
+  double scale[kMaxSlices];      // of a slice's weights
+  int32_t off[kMaxSlices];       // bins that a slice's top one lies below the row's, at most all
+  int32_t offsets[kMaxSlices + 1];  // of its candidates
   double kept[kMaxSlices];       // weight of a slice
   uint64_t kept_in[kMaxSlices];  // of its candidates, in whole units
   uint32_t ties[kMaxSlices];     // candidates of the cut's key
   uint32_t first[kMaxSlices];    // of these those that are kept
-  int32_t offsets[kMaxSlices + 1];
   uint64_t found[2];
-  uint64_t parts[kWaves];
-  double dparts[kWaves];
+  uint32_t bin[3];
+  uint64_t parts[kRowWaves];
+  double dparts[kRowWaves];
   int32_t slice;
   double before;
 };
@@ -548,13 +381,14 @@ struct Cut {
   uint64_t ties = 0;
 };
 
-// A row's weights, in units of 2^-bits.
+// A row's weights, in units of 2^-s.
 struct Units {
-  float top;
+  Exp2Near<0> near;
+  double top;
   double by;
   int32_t bits;
   __device__ __forceinline__ double Of(float x) const {
-    return Exp2Down((static_cast<double>(x) - static_cast<double>(top)) * by, bits);
+    return Exp2Down(near, (static_cast<double>(x) - top) * by, bits);
   }
   static __device__ __forceinline__ uint64_t Whole(double of) { return static_cast<uint64_t>(of + 0.5); }
   __device__ __forceinline__ uint64_t OfKey(uint32_t key) const { return Whole(Of(ValueOf(key))); }
@@ -571,20 +405,20 @@ __device__ __forceinline__ Cut Select(const Keys& key_at, uint32_t n, uint32_t l
 #pragma unroll 1
   while (width > 0) {
     const int bits = min(width, 8), shift = width - bits;
-    sh.bins[threadIdx.x] = 0;
+    if (threadIdx.x < 256) sh.digits[threadIdx.x] = 0;
     __syncthreads();
 #pragma unroll 1
-    for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+    for (uint32_t i = threadIdx.x; i < n; i += kRowThreads) {
       const uint32_t key = key_at(i), part = key - least;
       if (key < cut.key || (width < 32 && (part >> width) != prefix)) continue;
-      atomicAdd(reinterpret_cast<unsigned long long*>(&sh.bins[(part >> shift) & 255]),
+      atomicAdd(reinterpret_cast<unsigned long long*>(&sh.digits[(part >> shift) & 255]),
                 static_cast<unsigned long long>(by_weight ? units.OfKey(key) : 1));
     }
     __syncthreads();
     const int digit = 255 - static_cast<int>(threadIdx.x);
-    const uint64_t mine = sh.bins[digit];
+    const uint64_t mine = digit >= 0 ? sh.digits[digit] : 0;
     uint64_t unused;
-    const uint64_t before = above + BlockExclScan(mine, sh.parts, &unused);
+    const uint64_t before = above + RowBefore(mine, sh.parts, &unused);
     if (before < goal && goal <= before + mine) {
       sh.found[0] = static_cast<uint64_t>(digit);
       sh.found[1] = before;
@@ -600,82 +434,254 @@ __device__ __forceinline__ Cut Select(const Keys& key_at, uint32_t n, uint32_t l
   return Cut{key, (goal - above + each - 1) / each};
 }
 
+// Whether each of four bytes lies in [lo, hi], as 0 or 1 in it: lo and hi - lo are of 8 bits.
+__device__ __forceinline__ uint32_t BytesWithin(uint32_t bytes, uint32_t lo, uint32_t span) {
+  uint32_t r = 0;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) r |= ((bytes >> (8 * c) & 255) - lo <= span ? 1u : 0u) << (8 * c);
+  return r;
+}
+
 // Grid: rows.
-__global__ __launch_bounds__(kThreads) void SampleChooseKernel(const SampleArgs a) {
+__global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleArgs a) {
   __shared__ ChooseShared sh;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const Row row(a, blockIdx.x);
-  const Plan plan = *row.ThePlan();
-  if (plan.kind == Kind::kDone) return;
   const Setting set = SettingOf(a, row.r);
-  const Units units{plan.top, set.by, a.units};
-  const double unit = ldexp(1.0, -a.units);
-  const uint32_t n = plan.candidates;
-  const bool in_lds = n <= kInLds;
-  const uint32_t* const keys = row.Keys();
-  if (in_lds) {
-#pragma unroll 4
-    for (uint32_t i = tid; i < n; i += kThreads) sh.keys[i] = keys[i];
+
+  // ---- the slices joined: a slice to a thread
+  const SliceSums mine_of = tid < a.slices ? row.Sums()[tid] : SliceSums{-INFINITY, 0, 0};
+  // the largest, and of those of it the one that is first
+  const uint64_t best = RowMax(static_cast<uint64_t>(KeyOf(mine_of.top)) << 32 |
+                                   (0xFFFFFFFFu - static_cast<uint32_t>(mine_of.top_index)), sh.parts);
+  const float top = ValueOf(static_cast<uint32_t>(best >> 32));
+  if (top == -INFINITY || set.greedy) {
+    if (tid == 0) {
+      const bool none = top == -INFINITY;
+      a.tokens[row.r] = none ? -1 : static_cast<int32_t>(0xFFFFFFFFu - static_cast<uint32_t>(best));
+      if (a.probs != nullptr) a.probs[row.r] = none ? 0.0f : 1.0f;
+    }
+    return;
   }
-  for (int s = tid; s < a.slices; s += kThreads) {
-    sh.kept[s] = row.Above()[s];
-    sh.kept_in[s] = 0;
-    sh.ties[s] = 0;
-    sh.first[s] = 0;
-    if (n > 0) sh.offsets[s] = row.Offsets()[s];
+  const int32_t top_bin = set.BinOf(top);
+  const Units units{Exp2Near<0>(), static_cast<double>(top), set.by, a.units};
+  const double unit = __builtin_bit_cast(double, static_cast<uint64_t>(1023 - a.units) << 52);
+  double scale = 0.0;
+  if (tid < a.slices) {
+    const bool any = mine_of.top > -INFINITY;
+    scale = any ? units.Of(mine_of.top) * unit : 0.0;
+    sh.scale[tid] = scale;
+    sh.off[tid] = any ? set.BinBelow(top_bin, mine_of.top) : kBins - 1;
+    sh.kept_in[tid] = 0;
+    sh.ties[tid] = 0;
+    sh.first[tid] = 0;
+  }
+  if (tid < 3) sh.bin[tid] = kBins - 1;
+  const uint64_t live = RowSum(tid < a.slices ? CountOf(mine_of.sum) : 0, sh.parts);
+  // a slice's sum over the row's bins down to j
+  const auto sum_at = [&](int s, int j) -> uint64_t {
+    const int in_slice = j == kBins - 1 ? j : j - sh.off[s];
+    return in_slice >= 0 ? row.Bins(s)[in_slice] : 0;
+  };
+  const bool on_k = set.k > 0 && static_cast<uint64_t>(set.k) < live, on_p = set.OnP(), on_m = set.m > 0.0f;
+  const bool filters = on_k || on_p || on_m;
+
+  // ---- between which bins the filters cut
+  int hi = kBins, lo = -1;  // none: all that is live is above them
+  bool cut_k = false, cut_p = false, cut_m = false;
+  uint32_t base_count = 0, n = 0;
+  double base = 0.0, all_weight = 0.0;
+  if (filters) {
+    const int j = tid % kBins, joiner = tid / kBins;
+    double weight = 0.0;
+    uint32_t count = 0;
+    constexpr int kBatch = 10;
+#pragma unroll 1
+    for (int s0 = joiner; s0 < a.slices; s0 += kBatch * kJoiners) {
+      uint64_t sums[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) sums[i] = s0 + i * kJoiners < a.slices ? sum_at(s0 + i * kJoiners, j) : 0;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        if (s0 + i * kJoiners < a.slices) weight += sh.scale[s0 + i * kJoiners] * WeightOf(sums[i]);
+        count += CountOf(sums[i]);
+      }
+    }
+    sh.join.weight[joiner][j] = weight;
+    sh.join.count[joiner][j] = count;
+    __syncthreads();
+    if (tid < kBins) {
+      weight = 0.0;
+      count = 0;
+#pragma unroll
+      for (int i = 0; i < kJoiners; ++i) {
+        weight += sh.join.weight[i][tid];
+        count += sh.join.count[i][tid];
+      }
+      sh.weight[tid] = weight;
+      sh.count[tid] = count;
+    }
+    __syncthreads();
+    const bool first_bin = tid == 0, a_bin = tid < kBins;
+    const uint32_t before_count = first_bin || !a_bin ? 0 : sh.count[tid - 1];
+    const double before_weight = first_bin || !a_bin ? 0.0 : sh.weight[tid - 1];
+    // top_k's bin
+    const uint32_t k = static_cast<uint32_t>(set.k);
+    if (a_bin && on_k && before_count < k && k <= count) sh.bin[0] = static_cast<uint32_t>(tid);
+    __syncthreads();
+    const int bin_k = on_k ? static_cast<int>(sh.bin[0]) : kBins - 1;
+    // top_p's: between those of the least and the most that what top_k leaves may weigh, and a rounding more
+    const double most = sh.weight[bin_k], least = !on_k ? most : bin_k == 0 ? 0.0 : sh.weight[bin_k - 1];
+    const double p = static_cast<double>(set.p);
+    const double goal_hi = p * least * (1.0 - 0x1p-40), goal_lo = fmin(p * most * (1.0 + 0x1p-40), most);
+    if (a_bin && on_p) {
+      if (weight >= goal_hi && (first_bin || before_weight < goal_hi)) sh.bin[1] = static_cast<uint32_t>(tid);
+      if (weight >= goal_lo && (first_bin || before_weight < goal_lo)) sh.bin[2] = static_cast<uint32_t>(tid);
+    }
+    __syncthreads();
+    const int p_hi = static_cast<int>(sh.bin[1]), p_lo = static_cast<int>(sh.bin[2]);
+    // min_p's: from the next number above its border to the next below
+    int m_hi = kBins - 1, m_lo = kBins - 1;
+    if (on_m) {
+      const double border = static_cast<double>(top) + log(static_cast<double>(set.m)) * static_cast<double>(set.t);
+      const float near = static_cast<float>(fmax(border, -static_cast<double>(FLT_MAX)));
+      m_hi = set.BinBelow(top_bin, fminf(nextafterf(near, INFINITY), top));
+      m_lo = set.BinBelow(top_bin, nextafterf(near, -INFINITY));
+    }
+    // The cut that counts is the highest: filters that start below where another has cut for sure do not matter. top_p's
+    // place needs what top_k leaves, and so the bins down to its.
+    const int sure = min(on_k ? bin_k : kBins - 1, min(on_p ? p_lo : kBins - 1, m_lo));
+    cut_k = on_k && bin_k <= sure, cut_p = on_p && p_hi <= sure, cut_m = on_m && m_hi <= sure;
+    hi = kBins - 1, lo = 0;
+    if (cut_k) hi = min(hi, bin_k), lo = max(lo, bin_k);
+    if (cut_p) hi = min(hi, p_hi), lo = max(lo, on_k ? bin_k : p_lo);
+    if (cut_m) hi = min(hi, m_hi), lo = max(lo, m_lo);
+    cut_k = cut_k || (cut_p && on_k);
+    base_count = hi > 0 ? sh.count[hi - 1] : 0;
+    base = hi > 0 ? sh.weight[hi - 1] : 0.0;
+    all_weight = sh.weight[kBins - 1];
+  }
+
+  // ---- of each slice: the weight above these bins, and where its candidates go
+  uint64_t in = 0;
+  if (tid < a.slices) {
+    uint64_t above = mine_of.sum;
+    if (filters) {
+      above = hi > 0 ? sum_at(tid, hi - 1) : 0;
+      in = CountOf(sum_at(tid, lo)) - CountOf(above);
+    }
+    sh.kept[tid] = scale * WeightOf(above);
+  }
+  uint64_t placed;
+  const uint64_t before_in = RowBefore(in, sh.parts, &placed);
+  if (tid < a.slices) sh.offsets[tid] = static_cast<int32_t>(before_in);
+  n = static_cast<uint32_t>(placed);
+  if (tid == 0) sh.offsets[a.slices] = static_cast<int32_t>(n);
+  __syncthreads();
+
+  // ---- the candidates, in index order: a wave to a slice, sixteen neighbours to a lane, four rounds
+  const bool in_lds = n <= kInLds;
+  uint32_t* const keys = row.Keys();
+  const auto key_at = [&](uint32_t i) { return in_lds ? sh.keys[i] : keys[i]; };
+#pragma unroll 1
+  for (int s = n > 0 ? wave : a.slices; s < a.slices; s += kRowWaves) {
+    uint32_t to = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(sh.offsets[s]));
+    const uint32_t end = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(sh.offsets[s + 1]));
+    if (to == end) continue;
+    const int off = __builtin_amdgcn_readfirstlane(sh.off[s]);
+    // the slice's own bins: its last is the row's last
+    const int from = max(0, hi - off);
+    const int upto = lo == kBins - 1 ? lo : lo - off;
+    uint4 b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b[i] = *reinterpret_cast<const uint4*>(row.BytesOf(s) + 1024 * i + 16 * lane);
+#pragma unroll 1
+    for (int i = 0; i < 4; ++i) {
+      const uint4 v = i == 0 ? b[0] : i == 1 ? b[1] : i == 2 ? b[2] : b[3];
+      const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+      uint32_t takes = 0;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const uint32_t w = BytesWithin(words[c], static_cast<uint32_t>(from), static_cast<uint32_t>(upto - from));
+        takes |= ((w | w >> 7 | w >> 14 | w >> 21) & 15u) << (4 * c);
+      }
+      const int32_t at = s * kSlice + 1024 * i + 16 * lane;
+      if (lo == kBins - 1) {  // minus infinity has the last bin's byte too
+        for (uint32_t left = takes; left != 0; left &= left - 1) {
+          const int c = __builtin_ctz(left);
+          if (row.LoadOne(at + c) == -INFINITY) takes &= ~(1u << c);
+        }
+      }
+      const uint32_t count = static_cast<uint32_t>(__builtin_popcount(takes));
+      const uint32_t sum = attn::ScanAdd(count);
+      uint32_t next = to + sum - count;
+      to += __builtin_amdgcn_readlane(sum, 63);
+      while (takes != 0) {
+        const int c = __builtin_ctz(takes);
+        takes &= takes - 1;
+        const uint32_t key = KeyOf(row.LoadOne(at + c));
+        if (in_lds) {
+          sh.keys[next] = key;
+        } else {
+          keys[next] = key;
+        }
+        ++next;
+      }
+    }
   }
   __syncthreads();
-  const auto key_at = [&](uint32_t i) { return in_lds ? sh.keys[i] : keys[i]; };
 
   // ---- the cut
-  const double least = plan.cut_m ? static_cast<double>(set.m) / unit : 0.0;  // in units
+  const double least = cut_m ? static_cast<double>(set.m) / unit : 0.0;  // in units
   Cut cut;
-  bool ties_count = false;
+  uint64_t tie = 0;  // weight of a tie, if it counts
   if (n > 0) {
-    if (plan.cut_k || plan.cut_p) {
+    if (cut_k || cut_p) {
       uint32_t low = 0xFFFFFFFFu, high = 0;
 #pragma unroll 1
-      for (uint32_t i = tid; i < n; i += kThreads) {
+      for (uint32_t i = tid; i < n; i += kRowThreads) {
         const uint32_t key = key_at(i);
         low = min(low, key);
         high = max(high, key);
       }
-      high = static_cast<uint32_t>(BlockMaxU64(high, sh.parts));
-      low = ~static_cast<uint32_t>(BlockMaxU64(~low, sh.parts));
+      high = static_cast<uint32_t>(RowMax(high, sh.parts));
+      low = ~static_cast<uint32_t>(RowMax(~low, sh.parts));
       const int width = 32 - __builtin_clz((high - low) | 1);
       // first top_k's among its candidates, then top_p's among what that keeps
 #pragma unroll 1
-      for (int filter = plan.cut_k || plan.cut_p == 2 ? 0 : 1; filter < (plan.cut_p ? 2 : 1); ++filter) {
+      for (int filter = cut_k ? 0 : 1; filter < (cut_p ? 2 : 1); ++filter) {
         uint64_t goal;
         if (filter == 0) {
-          goal = static_cast<uint64_t>(set.k) - plan.base_count;
+          goal = static_cast<uint64_t>(set.k) - base_count;
         } else {
           uint64_t whole = 0;
 #pragma unroll 1
-          for (uint32_t i = tid; i < n; i += kThreads) {
+          for (uint32_t i = tid; i < n; i += kRowThreads) {
             const uint32_t key = key_at(i);
             if (key > cut.key) whole += units.OfKey(key);
           }
-          whole = BlockSum(whole, sh.parts);
+          whole = RowSum(whole, sh.parts);
           if (cut.ties > 0) whole += cut.ties * units.OfKey(cut.key);
           if (whole == 0) break;
-          const double all = plan.cut_p == 2 ? plan.base + static_cast<double>(whole) * unit : plan.all;
-          const double of = ceil((static_cast<double>(set.p) * all - plan.base) / unit);
+          const double of_all = on_k ? base + static_cast<double>(whole) * unit : all_weight;
+          const double of = ceil((static_cast<double>(set.p) * of_all - base) / unit);
           goal = of < 1.0 ? 1 : of < static_cast<double>(whole) ? static_cast<uint64_t>(of) : whole;
         }
         cut = Select(key_at, n, low, width, units, filter == 1, cut, goal, sh);
       }
     }
-    ties_count = cut.ties > 0 && units.Of(ValueOf(cut.key)) >= least;
+    if (cut.ties > 0) {
+      const double of = units.Of(ValueOf(cut.key));
+      tie = of >= least ? Units::Whole(of) : 0;
+      if (of < least) cut.ties = 0;
+    }
 
     // ---- what it keeps of each slice's candidates
-    sh.offsets[a.slices] = static_cast<int32_t>(n);
-    __syncthreads();
 #pragma unroll 1
-    for (uint32_t i = tid; i < n; i += kThreads) {
+    for (uint32_t i = tid; i < n; i += kRowThreads) {
       const uint32_t key = key_at(i);
       if (key < cut.key) continue;
-      int s = 0;  // the last slice that begins at or before i, of those that have any
+      int s = 0;  // the last slice that begins at or before i
       for (int step = kMaxSlices / 2; step > 0; step >>= 1) {
         if (s + step < a.slices && sh.offsets[s + step] <= static_cast<int32_t>(i)) s += step;
       }
@@ -689,119 +695,90 @@ __global__ __launch_bounds__(kThreads) void SampleChooseKernel(const SampleArgs 
       }
     }
     __syncthreads();
-    const uint64_t tie = ties_count ? units.OfKey(cut.key) : 0;
-    uint64_t ties_before = 0;
-#pragma unroll 1
-    for (int s0 = 0; s0 < a.slices; s0 += kThreads) {
-      const int s = s0 + tid;
-      const uint64_t mine = s < a.slices && ties_count ? sh.ties[s] : 0;
-      uint64_t all;
-      const uint64_t before = ties_before + BlockExclScan(mine, sh.parts, &all);
-      ties_before += all;
-      if (s < a.slices) {
-        const uint64_t left = before < cut.ties ? cut.ties - before : 0;
-        const uint64_t kept = mine < left ? mine : left;
-        sh.first[s] = static_cast<uint32_t>(kept);
-        sh.kept[s] += static_cast<double>(sh.kept_in[s] + kept * tie) * unit;
-      }
+    const uint64_t ties = tid < a.slices ? sh.ties[tid] : 0;
+    uint64_t unused;
+    const uint64_t before = RowBefore(ties, sh.parts, &unused);
+    if (tid < a.slices) {
+      const uint64_t left = before < cut.ties ? cut.ties - before : 0;
+      const uint64_t first = ties < left ? ties : left;
+      sh.first[tid] = static_cast<uint32_t>(first);
+      sh.kept[tid] += static_cast<double>(sh.kept_in[tid] + first * tie) * unit;
     }
-    __syncthreads();
   }
 
   // ---- u's slice, by sums in index order: the first whose end passes it, or the last that has any weight
-  double weight = 0.0;
-  for (int s = tid; s < a.slices; s += kThreads) weight += sh.kept[s];
   if (tid == 0) sh.slice = 0x7FFFFFFF;
-  weight = BlockSumD(weight, sh.dparts);
+  const double mine = tid < a.slices ? sh.kept[tid] : 0.0;
+  double weight;
+  const double before = RowBeforeD(mine, sh.dparts, &weight);
   const double goal = (set.u > 0.0f ? fmin(static_cast<double>(set.u), 1.0) : 0.0) * weight;
-  double upto = 0.0;
-#pragma unroll 1
-  for (int s0 = 0; s0 < a.slices; s0 += kThreads) {
-    const int s = s0 + tid;
-    const double mine = s < a.slices ? sh.kept[s] : 0.0;
-    double all;
-    const double before = upto + BlockBeforeD(mine, sh.dparts, &all);
-    if (mine > 0.0 && goal < before + mine) atomicMin(&sh.slice, s);
-    __syncthreads();
-    const bool found = sh.slice != 0x7FFFFFFF;
-    if (sh.slice == s) sh.before = before;
-    __syncthreads();
-    if (found) break;
-    upto += all;
-  }
+  if (mine > 0.0 && goal < before + mine) atomicMin(&sh.slice, tid);
+  __syncthreads();
+  if (sh.slice == tid) sh.before = before;
   if (sh.slice == 0x7FFFFFFF) {  // u of 1, or rounding: the last
-    int last = 0;
-    for (int s = tid; s < a.slices; s += kThreads) last = sh.kept[s] > 0.0 ? s : last;
-    const uint64_t of_all = BlockMaxU64(static_cast<uint64_t>(last), sh.parts);
+    const uint64_t last = RowMax(mine > 0.0 ? static_cast<uint64_t>(tid) : 0, sh.parts);
     if (tid == 0) {
-      sh.slice = static_cast<int32_t>(of_all);
+      sh.slice = static_cast<int32_t>(last);
       sh.before = -1.0;  // the last of it
     }
-    __syncthreads();
   }
+  __syncthreads();
   const int slice = __builtin_amdgcn_readfirstlane(sh.slice);
   const double inside = sh.before < 0.0 ? 0x1p63 : floor(fmax(goal - sh.before, 0.0) / unit);
   const uint64_t place = inside < 0x1p63 ? static_cast<uint64_t>(inside) : ~uint64_t(0);
 
-  // ---- the walk: four rounds of four neighbours to a thread
+  // ---- the walk: four neighbours to a thread
+  static_assert(kSlice == 4 * kRowThreads, "");
   const uint64_t ties_kept = sh.first[slice];
   const bool some_ties = ties_kept > 0 && ties_kept < sh.ties[slice];  // and not all: their order counts
-  uint64_t seen = 0, ties_seen = 0;
-  uint64_t last = 0;  // the last kept one, before all those of a weight above 0
-#pragma unroll 1
-  for (int round = 0; round < kEach / 4; ++round) {
-    const int at = slice * kSlice + round * 4 * kThreads + 4 * tid;
-    const float4 v = row.Load(at);
-    const float x[4] = {v.x, v.y, v.z, v.w};
-    uint64_t tie_at = 0;
-    if (some_ties) {
-      uint64_t mine = 0, all;
+  const int at = slice * kSlice + 4 * tid;
+  const float4 v = row.Load(at);
+  const float x[4] = {v.x, v.y, v.z, v.w};
+  uint64_t tie_at = 0;
+  if (some_ties) {
+    uint64_t ties = 0, unused;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) mine += x[c] > -INFINITY && KeyOf(x[c]) == cut.key ? 1 : 0;
-      tie_at = ties_seen + BlockExclScan(mine, sh.parts, &all);
-      ties_seen += all;
-    }
-    uint64_t w[4], sum = 0;
-    double of[4];
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const uint32_t key = KeyOf(x[c]);
-      const int j = set.BinBelow(plan.top_bin, x[c]);
-      of[c] = units.Of(x[c]);
-      bool keep = plan.kind == Kind::kAll || j < plan.hi;
-      if (!keep && j <= plan.lo && of[c] >= least) {
-        keep = key > cut.key;
-        if (key == cut.key) {
-          keep = some_ties ? tie_at < ties_kept : ties_kept > 0;
-          ++tie_at;
-        }
-      }
-      keep = keep && x[c] > -INFINITY;
-      w[c] = keep ? Units::Whole(of[c]) : 0;
-      sum += w[c];
-      if (keep) last = max(last, (w[c] > 0 ? uint64_t(1) << 32 : 0) + static_cast<uint64_t>(at + c + 1));
-    }
-    uint64_t all;
-    uint64_t before = seen + BlockExclScan(sum, sh.parts, &all);
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      if (before <= place && place < before + w[c]) {
-        a.tokens[row.r] = at + c;
-        if (a.probs != nullptr) a.probs[row.r] = static_cast<float>(of[c] * unit / weight);
-      }
-      before += w[c];
-    }
-    seen += all;
-    if (seen > place) return;
+    for (int c = 0; c < 4; ++c) ties += x[c] > -INFINITY && KeyOf(x[c]) == cut.key ? 1 : 0;
+    tie_at = RowBefore(ties, sh.parts, &unused);
   }
+  uint64_t w[4], sum = 0;
+  double of[4];
+  uint64_t last = 0;  // the last kept one, before all those of a weight above 0
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const uint32_t key = KeyOf(x[c]);
+    const int j = set.BinBelow(top_bin, x[c]);
+    of[c] = units.Of(x[c]);
+    bool keep = j < hi;
+    if (!keep && j <= lo && of[c] >= least) {
+      keep = key > cut.key;
+      if (key == cut.key) {
+        keep = some_ties ? tie_at < ties_kept : ties_kept > 0;
+        ++tie_at;
+      }
+    }
+    keep = keep && x[c] > -INFINITY;
+    w[c] = keep ? Units::Whole(of[c]) : 0;
+    sum += w[c];
+    if (keep) last = max(last, (w[c] > 0 ? uint64_t(1) << 32 : 0) + static_cast<uint64_t>(at + c + 1));
+  }
+  uint64_t total;
+  uint64_t seen = RowBefore(sum, sh.parts, &total);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    if (seen <= place && place < seen + w[c]) {
+      a.tokens[row.r] = at + c;
+      if (a.probs != nullptr) a.probs[row.r] = static_cast<float>(of[c] * unit / weight);
+    }
+    seen += w[c];
+  }
+  if (total > place) return;
   // rounding, u of 1, or weights of less than half a unit each, of which one is as near as another
-  last = BlockMaxU64(last, sh.parts);
+  last = RowMax(last, sh.parts);
   if (tid == 0) {
     const int32_t token = static_cast<int32_t>(last & 0xFFFFFFFFu) - 1;
     a.tokens[row.r] = token;
-    if (a.probs != nullptr) {
-      a.probs[row.r] = static_cast<float>(units.Of(Clean(a.logits[row.r * a.row_stride + token])) * unit / weight);
-    }
+    if (a.probs != nullptr) a.probs[row.r] = static_cast<float>(units.Of(row.LoadOne(token)) * unit / weight);
   }
 }
 
@@ -825,7 +802,7 @@ void CheckSizes(const char* what, int64_t n_rows, int64_t n) {
 
 size_t GpuSampleBatchWorkspaceBytes(int64_t n_rows, int64_t n) {
   CheckSizes("SampleBatchWorkspace", n_rows, n);
-  return static_cast<size_t>(kCounters + std::min<int64_t>(n_rows, kRowsAtOnce) * RowPlace(SlicesOf(n)).bytes);
+  return static_cast<size_t>(std::max<int64_t>(n_rows, 1) * RowPlace(SlicesOf(n)).size);
 }
 
 void GpuSampleBatchWorkspaceInit(void* workspace, size_t bytes) {
@@ -867,15 +844,12 @@ void GpuSampleBatch(const float* logits_dev, int64_t n_rows, int64_t n, int64_t 
                   !Overlap(workspace, static_cast<int64_t>(need), probs_dev, bytes))),
             "SampleBatch: logits, outputs and the workspace must not overlap");
   const int32_t slices = SlicesOf(n);
-  for (int64_t first = 0; first < n_rows; first += kRowsAtOnce) {
-    const unsigned rows = static_cast<unsigned>(std::min<int64_t>(n_rows - first, kRowsAtOnce));
-    const SampleArgs a{logits_dev,     row_stride, static_cast<int32_t>(n), slices,   UnitsFor(n), opt.temperature,
-                       opt.top_k,      opt.top_p,  opt.min_p,               u_dev,    tokens_dev,  probs_dev,
-                       static_cast<char*>(workspace), static_cast<int32_t>(first)};
-    Launch("SampleSlicesKernel", SampleSlicesKernel, dim3(rows * slices), dim3(kThreads), a);
-    Launch("SampleCollectKernel", SampleCollectKernel, dim3(rows * slices), dim3(kThreads), a);
-    Launch("SampleChooseKernel", SampleChooseKernel, dim3(rows), dim3(kThreads), a);
-  }
+  RPG_CHECK(n_rows * slices <= 0x7FFFFFFF, "SampleBatch: %lld rows of %lld logits are too many for one call",
+            static_cast<long long>(n_rows), static_cast<long long>(n));
+  const SampleArgs a{logits_dev, row_stride, static_cast<int32_t>(n), slices, UnitsFor(n), opt.temperature, opt.top_k,
+                     opt.top_p,  opt.min_p,  u_dev,                   tokens_dev, probs_dev, static_cast<char*>(workspace)};
+  Launch("SampleSlicesKernel", SampleSlicesKernel, dim3(static_cast<unsigned>(n_rows * slices)), dim3(kThreads), a);
+  Launch("SampleChooseKernel", SampleChooseKernel, dim3(static_cast<unsigned>(n_rows)), dim3(kRowThreads), a);
 }
 
 }  // namespace rpg
