@@ -288,18 +288,25 @@ __global__ __launch_bounds__(kThreads) void SampleSlicesKernel(const SampleArgs 
 
 // ---------------------------------------------------------------- a row's sums
 
+// Over the workgroup of a row. `sh` has room for kRowWaves, and is not to be used again before a barrier: calls take turns
+// with two of them.
+template <int kCtrl, int kRowMask = 0xF>
+__device__ __forceinline__ uint64_t MaxStep(uint64_t x) {
+  const uint64_t o = DppU64<kCtrl, kRowMask>(x, 0);
+  return o > x ? o : x;
+}
 __device__ __forceinline__ uint64_t RowMax(uint64_t x, uint64_t* sh) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    const uint64_t o = __shfl_xor(x, off, 64);
-    x = o > x ? o : x;
-  }
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = x;
+  x = MaxStep<0x111>(x);
+  x = MaxStep<0x112>(x);
+  x = MaxStep<0x114>(x);
+  x = MaxStep<0x118>(x);
+  x = MaxStep<0x142, 0xA>(x);
+  x = MaxStep<0x143, 0xC>(x);
+  if ((threadIdx.x & 63) == 63) sh[threadIdx.x >> 6] = x;
   __syncthreads();
   uint64_t r = sh[0];
 #pragma unroll
   for (int w = 1; w < kRowWaves; ++w) r = sh[w] > r ? sh[w] : r;
-  __syncthreads();
   return r;
 }
 // The sum over the threads before this one; *total that over all.
@@ -310,17 +317,11 @@ __device__ __forceinline__ uint64_t RowBefore(uint64_t x, uint64_t* sh, uint64_t
   uint64_t before = 0, all = 0;
 #pragma unroll
   for (int w = 0; w < kRowWaves; ++w) {
-    if (w == static_cast<int>(threadIdx.x >> 6)) before = all;
+    before = w == static_cast<int>(threadIdx.x >> 6) ? all : before;
     all += sh[w];
   }
-  __syncthreads();
   *total = all;
   return before + upto - x;
-}
-__device__ __forceinline__ uint64_t RowSum(uint64_t x, uint64_t* sh) {
-  uint64_t total;
-  RowBefore(x, sh, &total);
-  return total;
 }
 // The same of doubles, in one order.
 __device__ __forceinline__ double RowBeforeD(double x, double* sh, double* total) {
@@ -337,10 +338,9 @@ __device__ __forceinline__ double RowBeforeD(double x, double* sh, double* total
   double base = 0.0, all = 0.0;
 #pragma unroll
   for (int w = 0; w < kRowWaves; ++w) {
-    if (w == static_cast<int>(threadIdx.x >> 6)) base = all;
+    base = w == static_cast<int>(threadIdx.x >> 6) ? all : base;
     all += sh[w];
   }
-  __syncthreads();
   *total = all;
   return (threadIdx.x & 63) == 0 ? base : base + mine;
 }
@@ -359,7 +359,7 @@ struct ChooseShared {
   };
   double weight[kBins];  // of all bins down to one
   uint32_t count[kBins];
-  uint64_t digits[256];
+  uint64_t digits[kRowThreads];
   double scale[kMaxSlices];      // of a slice's weights
   int32_t off[kMaxSlices];       // bins that a slice's top one lies below the row's, at most all
   int32_t offsets[kMaxSlices + 1];  // of its candidates
@@ -369,7 +369,7 @@ struct ChooseShared {
   uint32_t first[kMaxSlices];    // of these those that are kept
   uint64_t found[2];
   uint32_t bin[3];
-  uint64_t parts[kRowWaves];
+  uint64_t parts[2][kRowWaves];
   double dparts[kRowWaves];
   int32_t slice;
   double before;
@@ -394,31 +394,35 @@ struct Units {
   __device__ __forceinline__ uint64_t OfKey(uint32_t key) const { return Whole(Of(ValueOf(key))); }
 };
 
-// The cut after the fewest first candidates, in order, whose amounts (1, or their weight) reach `goal`, among those that
-// `cut` keeps: radix selection from the upper of the `width` bits down in which keys, less the least, differ. The amounts
-// of all ties of cut.key enter, which decides nothing: it is the last key.
+// The cut after the fewest first candidates, in order, whose amounts (1, or their weight) reach `goal` (or all of them),
+// among those that `cut` keeps: radix selection from the upper of the `width` bits down in which keys, less the least,
+// differ. The amounts of all ties of cut.key enter, which decides nothing: it is the last key.
 template <class Keys>
 __device__ __forceinline__ Cut Select(const Keys& key_at, uint32_t n, uint32_t least, int width, const Units& units,
                                       bool by_weight, const Cut& cut, uint64_t goal, ChooseShared& sh) {
+  constexpr int kDigit = 10;
+  static_assert(1 << kDigit == kRowThreads, "a digit to a thread");
   uint32_t prefix = 0;
   uint64_t above = 0;
+  sh.digits[threadIdx.x] = 0;
+  __syncthreads();
 #pragma unroll 1
-  while (width > 0) {
-    const int bits = min(width, 8), shift = width - bits;
-    if (threadIdx.x < 256) sh.digits[threadIdx.x] = 0;
-    __syncthreads();
+  for (bool first = true; width > 0; first = false) {
+    const int bits = min(width, kDigit), shift = width - bits;
 #pragma unroll 1
     for (uint32_t i = threadIdx.x; i < n; i += kRowThreads) {
       const uint32_t key = key_at(i), part = key - least;
-      if (key < cut.key || (width < 32 && (part >> width) != prefix)) continue;
-      atomicAdd(reinterpret_cast<unsigned long long*>(&sh.digits[(part >> shift) & 255]),
+      if (key < cut.key || (!first && (part >> width) != prefix)) continue;
+      atomicAdd(reinterpret_cast<unsigned long long*>(&sh.digits[(part >> shift) & (kRowThreads - 1)]),
                 static_cast<unsigned long long>(by_weight ? units.OfKey(key) : 1));
     }
     __syncthreads();
-    const int digit = 255 - static_cast<int>(threadIdx.x);
-    const uint64_t mine = digit >= 0 ? sh.digits[digit] : 0;
-    uint64_t unused;
-    const uint64_t before = above + RowBefore(mine, sh.parts, &unused);
+    const int digit = kRowThreads - 1 - static_cast<int>(threadIdx.x);
+    const uint64_t mine = sh.digits[digit];
+    sh.digits[digit] = 0;
+    uint64_t all;
+    const uint64_t before = above + RowBefore(mine, sh.parts[first ? 0 : 1], &all);
+    if (first) goal = goal < all ? goal : all;
     if (before < goal && goal <= before + mine) {
       sh.found[0] = static_cast<uint64_t>(digit);
       sh.found[1] = before;
@@ -427,19 +431,11 @@ __device__ __forceinline__ Cut Select(const Keys& key_at, uint32_t n, uint32_t l
     prefix = prefix << bits | static_cast<uint32_t>(sh.found[0]);
     above = sh.found[1];
     width = shift;
-    __syncthreads();
   }
+  __syncthreads();
   const uint32_t key = least + prefix;
   const uint64_t each = by_weight ? units.OfKey(key) : 1;
-  return Cut{key, (goal - above + each - 1) / each};
-}
-
-// Whether each of four bytes lies in [lo, hi], as 0 or 1 in it: lo and hi - lo are of 8 bits.
-__device__ __forceinline__ uint32_t BytesWithin(uint32_t bytes, uint32_t lo, uint32_t span) {
-  uint32_t r = 0;
-#pragma unroll
-  for (int c = 0; c < 4; ++c) r |= ((bytes >> (8 * c) & 255) - lo <= span ? 1u : 0u) << (8 * c);
-  return r;
+  return Cut{key, each > 0 ? (goal - above + each - 1) / each : 0};
 }
 
 // Grid: rows.
@@ -453,7 +449,7 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
   const SliceSums mine_of = tid < a.slices ? row.Sums()[tid] : SliceSums{-INFINITY, 0, 0};
   // the largest, and of those of it the one that is first
   const uint64_t best = RowMax(static_cast<uint64_t>(KeyOf(mine_of.top)) << 32 |
-                                   (0xFFFFFFFFu - static_cast<uint32_t>(mine_of.top_index)), sh.parts);
+                                   (0xFFFFFFFFu - static_cast<uint32_t>(mine_of.top_index)), sh.parts[0]);
   const float top = ValueOf(static_cast<uint32_t>(best >> 32));
   if (top == -INFINITY || set.greedy) {
     if (tid == 0) {
@@ -477,14 +473,14 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
     sh.first[tid] = 0;
   }
   if (tid < 3) sh.bin[tid] = kBins - 1;
-  const uint64_t live = RowSum(tid < a.slices ? CountOf(mine_of.sum) : 0, sh.parts);
+  __syncthreads();
   // a slice's sum over the row's bins down to j
   const auto sum_at = [&](int s, int j) -> uint64_t {
     const int in_slice = j == kBins - 1 ? j : j - sh.off[s];
     return in_slice >= 0 ? row.Bins(s)[in_slice] : 0;
   };
-  const bool on_k = set.k > 0 && static_cast<uint64_t>(set.k) < live, on_p = set.OnP(), on_m = set.m > 0.0f;
-  const bool filters = on_k || on_p || on_m;
+  bool on_k = false;
+  const bool on_p = set.OnP(), on_m = set.m > 0.0f, filters = set.Filters();
 
   // ---- between which bins the filters cut
   int hi = kBins, lo = -1;  // none: all that is live is above them
@@ -523,6 +519,7 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
     }
     __syncthreads();
     const bool first_bin = tid == 0, a_bin = tid < kBins;
+    on_k = set.k > 0 && static_cast<uint32_t>(set.k) < sh.count[kBins - 1];  // else it keeps all that is live
     const uint32_t before_count = first_bin || !a_bin ? 0 : sh.count[tid - 1];
     const double before_weight = first_bin || !a_bin ? 0.0 : sh.weight[tid - 1];
     // top_k's bin
@@ -552,13 +549,13 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
     // place needs what top_k leaves, and so the bins down to its.
     const int sure = min(on_k ? bin_k : kBins - 1, min(on_p ? p_lo : kBins - 1, m_lo));
     cut_k = on_k && bin_k <= sure, cut_p = on_p && p_hi <= sure, cut_m = on_m && m_hi <= sure;
-    hi = kBins - 1, lo = 0;
+    if (on_k || on_p || on_m) hi = kBins - 1, lo = 0;
     if (cut_k) hi = min(hi, bin_k), lo = max(lo, bin_k);
     if (cut_p) hi = min(hi, p_hi), lo = max(lo, on_k ? bin_k : p_lo);
     if (cut_m) hi = min(hi, m_hi), lo = max(lo, m_lo);
     cut_k = cut_k || (cut_p && on_k);
-    base_count = hi > 0 ? sh.count[hi - 1] : 0;
-    base = hi > 0 ? sh.weight[hi - 1] : 0.0;
+    base_count = hi > 0 ? sh.count[min(hi, kBins) - 1] : 0;
+    base = hi > 0 ? sh.weight[min(hi, kBins) - 1] : 0.0;
     all_weight = sh.weight[kBins - 1];
   }
 
@@ -566,44 +563,41 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
   uint64_t in = 0;
   if (tid < a.slices) {
     uint64_t above = mine_of.sum;
-    if (filters) {
+    if (lo >= 0) {
       above = hi > 0 ? sum_at(tid, hi - 1) : 0;
       in = CountOf(sum_at(tid, lo)) - CountOf(above);
     }
     sh.kept[tid] = scale * WeightOf(above);
   }
   uint64_t placed;
-  const uint64_t before_in = RowBefore(in, sh.parts, &placed);
+  const uint64_t before_in = RowBefore(in, sh.parts[1], &placed);
   if (tid < a.slices) sh.offsets[tid] = static_cast<int32_t>(before_in);
   n = static_cast<uint32_t>(placed);
   if (tid == 0) sh.offsets[a.slices] = static_cast<int32_t>(n);
   __syncthreads();
 
-  // ---- the candidates, in index order: a wave to a slice, sixteen neighbours to a lane, four rounds
+  // ---- the candidates, in index order: first where they are, a wave to a slice, sixteen neighbours to a lane in each of
+  // four rounds; then what they are, all at once
   const bool in_lds = n <= kInLds;
-  uint32_t* const keys = row.Keys();
-  const auto key_at = [&](uint32_t i) { return in_lds ? sh.keys[i] : keys[i]; };
+  uint32_t* const keys = in_lds ? sh.keys : row.Keys();
 #pragma unroll 1
   for (int s = n > 0 ? wave : a.slices; s < a.slices; s += kRowWaves) {
     uint32_t to = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(sh.offsets[s]));
-    const uint32_t end = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(sh.offsets[s + 1]));
-    if (to == end) continue;
+    if (to == static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(sh.offsets[s + 1]))) continue;
     const int off = __builtin_amdgcn_readfirstlane(sh.off[s]);
-    // the slice's own bins: its last is the row's last
-    const int from = max(0, hi - off);
-    const int upto = lo == kBins - 1 ? lo : lo - off;
+    // in the slice's own bins, whose last is the row's last
+    const int from = max(0, hi - off), upto = lo == kBins - 1 ? lo : lo - off;
     uint4 b[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) b[i] = *reinterpret_cast<const uint4*>(row.BytesOf(s) + 1024 * i + 16 * lane);
-#pragma unroll 1
+#pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint4 v = i == 0 ? b[0] : i == 1 ? b[1] : i == 2 ? b[2] : b[3];
-      const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+      const uint32_t words[4] = {b[i].x, b[i].y, b[i].z, b[i].w};
       uint32_t takes = 0;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const uint32_t w = BytesWithin(words[c], static_cast<uint32_t>(from), static_cast<uint32_t>(upto - from));
-        takes |= ((w | w >> 7 | w >> 14 | w >> 21) & 15u) << (4 * c);
+      for (int c = 0; c < 16; ++c) {
+        const uint32_t byte = words[c / 4] >> (8 * (c % 4)) & 255;
+        takes |= (byte - static_cast<uint32_t>(from) <= static_cast<uint32_t>(upto - from) ? 1u : 0u) << c;
       }
       const int32_t at = s * kSlice + 1024 * i + 16 * lane;
       if (lo == kBins - 1) {  // minus infinity has the last bin's byte too
@@ -616,20 +610,30 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
       const uint32_t sum = attn::ScanAdd(count);
       uint32_t next = to + sum - count;
       to += __builtin_amdgcn_readlane(sum, 63);
-      while (takes != 0) {
-        const int c = __builtin_ctz(takes);
-        takes &= takes - 1;
-        const uint32_t key = KeyOf(row.LoadOne(at + c));
-        if (in_lds) {
-          sh.keys[next] = key;
-        } else {
-          keys[next] = key;
-        }
-        ++next;
-      }
+      for (; takes != 0; takes &= takes - 1) keys[next++] = static_cast<uint32_t>(at + __builtin_ctz(takes));
     }
   }
   __syncthreads();
+  uint32_t low = 0xFFFFFFFFu, high = 0;
+#pragma unroll 1
+  for (uint32_t i0 = tid; i0 < n; i0 += 4 * kRowThreads) {
+    float x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t at = i0 + i * kRowThreads;
+      x[i] = row.LoadOne(static_cast<int32_t>(at < n ? keys[at] : 0));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t at = i0 + i * kRowThreads;
+      if (at < n) {
+        keys[at] = KeyOf(x[i]);
+        low = min(low, KeyOf(x[i]));
+        high = max(high, KeyOf(x[i]));
+      }
+    }
+  }
+  const auto key_at = [&](uint32_t i) { return keys[i]; };
 
   // ---- the cut
   const double least = cut_m ? static_cast<double>(set.m) / unit : 0.0;  // in units
@@ -637,37 +641,25 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
   uint64_t tie = 0;  // weight of a tie, if it counts
   if (n > 0) {
     if (cut_k || cut_p) {
-      uint32_t low = 0xFFFFFFFFu, high = 0;
-#pragma unroll 1
-      for (uint32_t i = tid; i < n; i += kRowThreads) {
-        const uint32_t key = key_at(i);
-        low = min(low, key);
-        high = max(high, key);
-      }
-      high = static_cast<uint32_t>(RowMax(high, sh.parts));
-      low = ~static_cast<uint32_t>(RowMax(~low, sh.parts));
+      high = static_cast<uint32_t>(RowMax(high, sh.parts[0]));
+      low = ~static_cast<uint32_t>(RowMax(~low, sh.parts[1]));
       const int width = 32 - __builtin_clz((high - low) | 1);
       // first top_k's among its candidates, then top_p's among what that keeps
-#pragma unroll 1
-      for (int filter = cut_k ? 0 : 1; filter < (cut_p ? 2 : 1); ++filter) {
-        uint64_t goal;
-        if (filter == 0) {
-          goal = static_cast<uint64_t>(set.k) - base_count;
-        } else {
-          uint64_t whole = 0;
+      if (cut_k) cut = Select(key_at, n, low, width, units, false, cut, static_cast<uint64_t>(set.k) - base_count, sh);
+      if (cut_p) {
+        double of_all = all_weight;
+        if (on_k) {
+          uint64_t whole = 0, total;
 #pragma unroll 1
           for (uint32_t i = tid; i < n; i += kRowThreads) {
             const uint32_t key = key_at(i);
             if (key > cut.key) whole += units.OfKey(key);
           }
-          whole = RowSum(whole, sh.parts);
-          if (cut.ties > 0) whole += cut.ties * units.OfKey(cut.key);
-          if (whole == 0) break;
-          const double of_all = on_k ? base + static_cast<double>(whole) * unit : all_weight;
-          const double of = ceil((static_cast<double>(set.p) * of_all - base) / unit);
-          goal = of < 1.0 ? 1 : of < static_cast<double>(whole) ? static_cast<uint64_t>(of) : whole;
+          RowBefore(whole, sh.parts[0], &total);
+          of_all = base + static_cast<double>(total + cut.ties * units.OfKey(cut.key)) * unit;
         }
-        cut = Select(key_at, n, low, width, units, filter == 1, cut, goal, sh);
+        const double of = ceil((static_cast<double>(set.p) * of_all - base) / unit);
+        cut = Select(key_at, n, low, width, units, true, cut, of < 1.0 ? 1 : static_cast<uint64_t>(fmin(of, 0x1p62)), sh);
       }
     }
     if (cut.ties > 0) {
@@ -682,7 +674,7 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
       const uint32_t key = key_at(i);
       if (key < cut.key) continue;
       int s = 0;  // the last slice that begins at or before i
-      for (int step = kMaxSlices / 2; step > 0; step >>= 1) {
+      for (int step = 1 << (31 - __builtin_clz(a.slices)); step > 0; step >>= 1) {
         if (s + step < a.slices && sh.offsets[s + step] <= static_cast<int32_t>(i)) s += step;
       }
       if (key == cut.key) {
@@ -697,7 +689,7 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
     __syncthreads();
     const uint64_t ties = tid < a.slices ? sh.ties[tid] : 0;
     uint64_t unused;
-    const uint64_t before = RowBefore(ties, sh.parts, &unused);
+    const uint64_t before = RowBefore(ties, sh.parts[0], &unused);
     if (tid < a.slices) {
       const uint64_t left = before < cut.ties ? cut.ties - before : 0;
       const uint64_t first = ties < left ? ties : left;
@@ -716,7 +708,7 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
   __syncthreads();
   if (sh.slice == tid) sh.before = before;
   if (sh.slice == 0x7FFFFFFF) {  // u of 1, or rounding: the last
-    const uint64_t last = RowMax(mine > 0.0 ? static_cast<uint64_t>(tid) : 0, sh.parts);
+    const uint64_t last = RowMax(mine > 0.0 ? static_cast<uint64_t>(tid) : 0, sh.parts[1]);
     if (tid == 0) {
       sh.slice = static_cast<int32_t>(last);
       sh.before = -1.0;  // the last of it
@@ -739,7 +731,8 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
     uint64_t ties = 0, unused;
 #pragma unroll
     for (int c = 0; c < 4; ++c) ties += x[c] > -INFINITY && KeyOf(x[c]) == cut.key ? 1 : 0;
-    tie_at = RowBefore(ties, sh.parts, &unused);
+    tie_at = RowBefore(ties, sh.parts[1], &unused);
+    __syncthreads();
   }
   uint64_t w[4], sum = 0;
   double of[4];
@@ -763,7 +756,7 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
     if (keep) last = max(last, (w[c] > 0 ? uint64_t(1) << 32 : 0) + static_cast<uint64_t>(at + c + 1));
   }
   uint64_t total;
-  uint64_t seen = RowBefore(sum, sh.parts, &total);
+  uint64_t seen = RowBefore(sum, sh.parts[0], &total);
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     if (seen <= place && place < seen + w[c]) {
@@ -774,7 +767,7 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
   }
   if (total > place) return;
   // rounding, u of 1, or weights of less than half a unit each, of which one is as near as another
-  last = RowMax(last, sh.parts);
+  last = RowMax(last, sh.parts[1]);
   if (tid == 0) {
     const int32_t token = static_cast<int32_t>(last & 0xFFFFFFFFu) - 1;
     a.tokens[row.r] = token;
