@@ -36,9 +36,6 @@ using namespace block;
 constexpr int kSlice = 4096;
 constexpr int kEach = kSlice / kThreads;
 constexpr int kMaxSlices = static_cast<int>(kSamplerMaxVocab / kSlice);
-constexpr int kRowThreads = 1024;  // of a workgroup for a row
-constexpr int kRowWaves = kRowThreads / 64;
-static_assert(kMaxSlices <= kRowThreads, "a slice to a thread");
 constexpr int kBins = 256;         // of a slice; the last has all that is further down
 constexpr int kInLds = 8192;       // candidates that are kept there
 // A slice's sums, in one number: count in the upper 13 bits, weight in units of 2^-38 of its largest in the lower 51.
@@ -110,8 +107,10 @@ __device__ __forceinline__ uint64_t OneOf(const Exp2Near<kSliceUnits>& near, dou
          static_cast<uint32_t>(bits);
 }
 __device__ __forceinline__ uint32_t CountOf(uint64_t sum) { return static_cast<uint32_t>(sum >> kWeightBits); }
+// In units of 2^-38: 2^52 and it are one double, bit for bit.
 __device__ __forceinline__ double WeightOf(uint64_t sum) {
-  return static_cast<double>(sum & ((uint64_t(1) << kWeightBits) - 1)) * (1.0 / static_cast<double>(uint64_t(1) << kSliceUnits));
+  const uint64_t whole = sum & ((uint64_t(1) << kWeightBits) - 1);
+  return __builtin_bit_cast(double, whole | uint64_t(0x433) << 52) - 0x1p52;
 }
 
 // A row's settings.
@@ -286,68 +285,32 @@ __global__ __launch_bounds__(kThreads) void SampleSlicesKernel(const SampleArgs 
   if (tid == 0) row.Sums()[slice] = SliceSums{top, first, sum};
 }
 
-// ---------------------------------------------------------------- a row's sums
-
-// Over the workgroup of a row. `sh` has room for kRowWaves, and is not to be used again before a barrier: calls take turns
-// with two of them.
-template <int kCtrl, int kRowMask = 0xF>
-__device__ __forceinline__ uint64_t MaxStep(uint64_t x) {
-  const uint64_t o = DppU64<kCtrl, kRowMask>(x, 0);
-  return o > x ? o : x;
-}
-__device__ __forceinline__ uint64_t RowMax(uint64_t x, uint64_t* sh) {
-  x = MaxStep<0x111>(x);
-  x = MaxStep<0x112>(x);
-  x = MaxStep<0x114>(x);
-  x = MaxStep<0x118>(x);
-  x = MaxStep<0x142, 0xA>(x);
-  x = MaxStep<0x143, 0xC>(x);
-  if ((threadIdx.x & 63) == 63) sh[threadIdx.x >> 6] = x;
-  __syncthreads();
-  uint64_t r = sh[0];
-#pragma unroll
-  for (int w = 1; w < kRowWaves; ++w) r = sh[w] > r ? sh[w] : r;
-  return r;
-}
-// The sum over the threads before this one; *total that over all.
-__device__ __forceinline__ uint64_t RowBefore(uint64_t x, uint64_t* sh, uint64_t* total) {
-  const uint64_t upto = WaveInclScanU64(x);
-  if ((threadIdx.x & 63) == 63) sh[threadIdx.x >> 6] = upto;
-  __syncthreads();
-  uint64_t before = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < kRowWaves; ++w) {
-    before = w == static_cast<int>(threadIdx.x >> 6) ? all : before;
-    all += sh[w];
-  }
-  *total = all;
-  return before + upto - x;
-}
-// The same of doubles, in one order.
-__device__ __forceinline__ double RowBeforeD(double x, double* sh, double* total) {
-  double upto = x;
-  upto += DppDbl<0x111>(upto, 0.0);
-  upto += DppDbl<0x112>(upto, 0.0);
-  upto += DppDbl<0x114>(upto, 0.0);
-  upto += DppDbl<0x118>(upto, 0.0);
-  upto += DppDbl<0x142, 0xA>(upto, 0.0);
-  upto += DppDbl<0x143, 0xC>(upto, 0.0);
-  const double mine = __shfl_up(upto, 1, 64);
-  if ((threadIdx.x & 63) == 63) sh[threadIdx.x >> 6] = upto;
-  __syncthreads();
-  double base = 0.0, all = 0.0;
-#pragma unroll
-  for (int w = 0; w < kRowWaves; ++w) {
-    base = w == static_cast<int>(threadIdx.x >> 6) ? all : base;
-    all += sh[w];
-  }
-  *total = all;
-  return (threadIdx.x & 63) == 0 ? base : base + mine;
-}
-
 // ---------------------------------------------------------------- the choice
 
+// Sums over a wave: upto and with this lane.
+__device__ __forceinline__ double WaveInclScanD(double v) {
+  v += DppDbl<0x111>(v, 0.0);
+  v += DppDbl<0x112>(v, 0.0);
+  v += DppDbl<0x114>(v, 0.0);
+  v += DppDbl<0x118>(v, 0.0);
+  v += DppDbl<0x142, 0xA>(v, 0.0);
+  return v + DppDbl<0x143, 0xC>(v, 0.0);
+}
+template <class T>
+__device__ __forceinline__ T LastLane(T x) {
+  const uint64_t bits = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(bits), 63);
+  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(bits >> 32), 63);
+  return __builtin_bit_cast(T, static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+// The four waves of a SIMD take turns, so that what one wave can do (sums over slices and digits) is done by one, the
+// others waiting at the barrier: with sums over all sixteen the kernel took 22 us for one row and 35 for 128.
+constexpr int kRowThreads = 1024;
+constexpr int kRowWaves = kRowThreads / 64;
 constexpr int kJoiners = kRowThreads / kBins;  // threads to a bin, each for every kJoiners-th slice
+constexpr int kDigitBits = 8;
+constexpr int kDigits = 1 << kDigitBits;
 
 struct ChooseShared {
   union {
@@ -359,20 +322,25 @@ struct ChooseShared {
   };
   double weight[kBins];  // of all bins down to one
   uint32_t count[kBins];
-  uint64_t digits[kRowThreads];
-  double scale[kMaxSlices];      // of a slice's weights
-  int32_t off[kMaxSlices];       // bins that a slice's top one lies below the row's, at most all
+  uint64_t digits[kDigits];
+  uint64_t sum[kMaxSlices];         // a slice's
+  double scale[kMaxSlices];         // of its weights' units
+  int32_t off[kMaxSlices];          // bins that its top one lies below the row's, at most all
   int32_t offsets[kMaxSlices + 1];  // of its candidates
-  double kept[kMaxSlices];       // weight of a slice
-  uint64_t kept_in[kMaxSlices];  // of its candidates, in whole units
-  uint32_t ties[kMaxSlices];     // candidates of the cut's key
-  uint32_t first[kMaxSlices];    // of these those that are kept
+  double kept[kMaxSlices];          // its weight
+  uint64_t kept_in[kMaxSlices];     // that of its candidates, in whole units
+  uint32_t ties[kMaxSlices];        // its candidates of the cut's key
+  uint32_t first[kMaxSlices];       // of these those that are kept
   uint64_t found[2];
-  uint32_t bin[3];
-  uint64_t parts[2][kRowWaves];
-  double dparts[kRowWaves];
-  int32_t slice;
+  uint64_t wave_sum[kRowWaves];
+  uint64_t wave_last[kRowWaves];
+  double weight_of_all;
   double before;
+  float top;
+  int32_t top_index;
+  uint32_t low, high;
+  uint32_t bin[3];
+  int32_t slice;
 };
 
 // Kept are the keys above `key`, and of those equal to it the first `ties` in index order.
@@ -396,46 +364,61 @@ struct Units {
 
 // The cut after the fewest first candidates, in order, whose amounts (1, or their weight) reach `goal` (or all of them),
 // among those that `cut` keeps: radix selection from the upper of the `width` bits down in which keys, less the least,
-// differ. The amounts of all ties of cut.key enter, which decides nothing: it is the last key.
-template <class Keys>
-__device__ __forceinline__ Cut Select(const Keys& key_at, uint32_t n, uint32_t least, int width, const Units& units,
+// differ. The amounts of all ties of cut.key enter, which decides nothing: it is the last key. sh.digits are 0, and are so
+// again.
+__device__ __forceinline__ Cut Select(const uint32_t* keys, uint32_t n, uint32_t least, int width, const Units& units,
                                       bool by_weight, const Cut& cut, uint64_t goal, ChooseShared& sh) {
-  constexpr int kDigit = 10;
-  static_assert(1 << kDigit == kRowThreads, "a digit to a thread");
   uint32_t prefix = 0;
-  uint64_t above = 0;
-  sh.digits[threadIdx.x] = 0;
-  __syncthreads();
+  if (threadIdx.x == 0) sh.found[0] = sh.found[1] = 0;  // candidates of no weight at all: the last
 #pragma unroll 1
   for (bool first = true; width > 0; first = false) {
-    const int bits = min(width, kDigit), shift = width - bits;
+    const int bits = min(width, kDigitBits), shift = width - bits;
 #pragma unroll 1
     for (uint32_t i = threadIdx.x; i < n; i += kRowThreads) {
-      const uint32_t key = key_at(i), part = key - least;
+      const uint32_t key = keys[i], part = key - least;
       if (key < cut.key || (!first && (part >> width) != prefix)) continue;
-      atomicAdd(reinterpret_cast<unsigned long long*>(&sh.digits[(part >> shift) & (kRowThreads - 1)]),
+      atomicAdd(reinterpret_cast<unsigned long long*>(&sh.digits[kDigits - 1 - ((part >> shift) & (kDigits - 1))]),
                 static_cast<unsigned long long>(by_weight ? units.OfKey(key) : 1));
     }
     __syncthreads();
-    const int digit = kRowThreads - 1 - static_cast<int>(threadIdx.x);
-    const uint64_t mine = sh.digits[digit];
-    sh.digits[digit] = 0;
-    uint64_t all;
-    const uint64_t before = above + RowBefore(mine, sh.parts[first ? 0 : 1], &all);
-    if (first) goal = goal < all ? goal : all;
-    if (before < goal && goal <= before + mine) {
-      sh.found[0] = static_cast<uint64_t>(digit);
-      sh.found[1] = before;
+    if (threadIdx.x < 64) {  // four digits to a lane, from the highest down
+      uint64_t d[kDigits / 64], mine = 0;
+#pragma unroll
+      for (int i = 0; i < kDigits / 64; ++i) {
+        d[i] = sh.digits[kDigits / 64 * threadIdx.x + i];
+        sh.digits[kDigits / 64 * threadIdx.x + i] = 0;
+        mine += d[i];
+      }
+      const uint64_t upto = WaveInclScanU64(mine);
+      if (first) goal = min(goal, LastLane(upto));
+      uint64_t before = upto - mine;
+#pragma unroll
+      for (int i = 0; i < kDigits / 64; ++i) {
+        if (before < goal && goal <= before + d[i]) {
+          sh.found[0] = static_cast<uint64_t>(kDigits - 1 - (kDigits / 64 * threadIdx.x + i));
+          sh.found[1] = goal - before;
+        }
+        before += d[i];
+      }
     }
     __syncthreads();
     prefix = prefix << bits | static_cast<uint32_t>(sh.found[0]);
-    above = sh.found[1];
+    goal = sh.found[1];  // of what has this prefix
     width = shift;
   }
   __syncthreads();
   const uint32_t key = least + prefix;
   const uint64_t each = by_weight ? units.OfKey(key) : 1;
-  return Cut{key, each > 0 ? (goal - above + each - 1) / each : 0};
+  return Cut{key, each > 0 ? (goal + each - 1) / each : 0};
+}
+
+// Of four bytes those in [from, from + span], as their highest bits. (Bytes are subtracted and added without carries
+// between them; a byte less `from` exceeds the span where adding 255 - span carries out.)
+__device__ __forceinline__ uint32_t BytesWithin(uint32_t bytes, uint32_t from4, uint32_t beyond4) {
+  constexpr uint32_t kHigh = 0x80808080u;
+  const uint32_t less = ((bytes | kHigh) - (from4 & ~kHigh)) ^ ((bytes ^ ~from4) & kHigh);
+  const uint32_t low = (less & ~kHigh) + (beyond4 & ~kHigh);
+  return ~((less & beyond4) | ((less | beyond4) & low)) & kHigh;
 }
 
 // Grid: rows.
@@ -444,71 +427,99 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const Row row(a, blockIdx.x);
   const Setting set = SettingOf(a, row.r);
+  const bool on_p = set.OnP(), on_m = set.m > 0.0f, filters = set.Filters();
+  const auto slices64 = [&](auto f) {  // by the first wave
+#pragma unroll 1
+    for (int s0 = 0; s0 < a.slices; s0 += 64) f(s0 + lane, s0 + lane < a.slices);
+  };
 
-  // ---- the slices joined: a slice to a thread
-  const SliceSums mine_of = tid < a.slices ? row.Sums()[tid] : SliceSums{-INFINITY, 0, 0};
-  // the largest, and of those of it the one that is first
-  const uint64_t best = RowMax(static_cast<uint64_t>(KeyOf(mine_of.top)) << 32 |
-                                   (0xFFFFFFFFu - static_cast<uint32_t>(mine_of.top_index)), sh.parts[0]);
-  const float top = ValueOf(static_cast<uint32_t>(best >> 32));
+  // ---- the slices' largest, and what their weights are multiplied by
+  if (wave == 0) {
+    float top = -INFINITY;
+    slices64([&](int s, bool there) { top = fmaxf(top, there ? row.Sums()[s].top : -INFINITY); });
+    top = WaveMaxTo63(top);
+    top = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(top), 63));
+    int32_t index = 0x7FFFFFFF;
+    const int32_t top_bin = set.BinOf(top);
+    const Exp2Near<0> near;
+    slices64([&](int s, bool there) {
+      if (!there) return;
+      const SliceSums mine = row.Sums()[s];
+      if (set.greedy) {
+        if (mine.top == top) index = min(index, mine.top_index);
+        return;
+      }
+      const bool any = mine.top > -INFINITY;
+      sh.sum[s] = mine.sum;
+      sh.scale[s] = any ? Exp2Down(near, (static_cast<double>(mine.top) - static_cast<double>(top)) * set.by, -kSliceUnits) : 0.0;
+      sh.off[s] = any ? set.BinBelow(top_bin, mine.top) : kBins - 1;
+      sh.kept_in[s] = 0;
+      sh.ties[s] = 0;
+      sh.first[s] = 0;
+    });
+    if (set.greedy) {
+#pragma unroll
+      for (int by = 32; by > 0; by >>= 1) index = min(index, __shfl_xor(index, by, 64));
+    }
+    if (lane == 0) {
+      sh.top = top;
+      sh.top_index = index;
+      sh.low = 0xFFFFFFFFu;
+      sh.high = 0;
+      sh.slice = 0x7FFFFFFF;
+    }
+  } else if (wave < 5) {
+    sh.digits[tid - 64] = 0;
+    if (tid < 64 + 3) sh.bin[tid - 64] = kBins - 1;
+  }
+  __syncthreads();
+  const float top = sh.top;
   if (top == -INFINITY || set.greedy) {
     if (tid == 0) {
-      const bool none = top == -INFINITY;
-      a.tokens[row.r] = none ? -1 : static_cast<int32_t>(0xFFFFFFFFu - static_cast<uint32_t>(best));
-      if (a.probs != nullptr) a.probs[row.r] = none ? 0.0f : 1.0f;
+      a.tokens[row.r] = top == -INFINITY ? -1 : sh.top_index;
+      if (a.probs != nullptr) a.probs[row.r] = top == -INFINITY ? 0.0f : 1.0f;
     }
     return;
   }
   const int32_t top_bin = set.BinOf(top);
   const Units units{Exp2Near<0>(), static_cast<double>(top), set.by, a.units};
   const double unit = __builtin_bit_cast(double, static_cast<uint64_t>(1023 - a.units) << 52);
-  double scale = 0.0;
-  if (tid < a.slices) {
-    const bool any = mine_of.top > -INFINITY;
-    scale = any ? units.Of(mine_of.top) * unit : 0.0;
-    sh.scale[tid] = scale;
-    sh.off[tid] = any ? set.BinBelow(top_bin, mine_of.top) : kBins - 1;
-    sh.kept_in[tid] = 0;
-    sh.ties[tid] = 0;
-    sh.first[tid] = 0;
-  }
-  if (tid < 3) sh.bin[tid] = kBins - 1;
-  __syncthreads();
   // a slice's sum over the row's bins down to j
   const auto sum_at = [&](int s, int j) -> uint64_t {
     const int in_slice = j == kBins - 1 ? j : j - sh.off[s];
     return in_slice >= 0 ? row.Bins(s)[in_slice] : 0;
   };
-  bool on_k = false;
-  const bool on_p = set.OnP(), on_m = set.m > 0.0f, filters = set.Filters();
 
   // ---- between which bins the filters cut
+  bool on_k = false;
   int hi = kBins, lo = -1;  // none: all that is live is above them
   bool cut_k = false, cut_p = false, cut_m = false;
-  uint32_t base_count = 0, n = 0;
+  uint32_t base_count = 0;
   double base = 0.0, all_weight = 0.0;
   if (filters) {
-    const int j = tid % kBins, joiner = tid / kBins;
+    {
+      const int j = tid % kBins, joiner = tid / kBins;
+      double weight = 0.0;
+      uint32_t count = 0;
+      constexpr int kBatch = 10;
+#pragma unroll 1
+      for (int s0 = joiner; s0 < a.slices; s0 += kBatch * kJoiners) {
+        uint64_t sums[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) sums[i] = s0 + i * kJoiners < a.slices ? sum_at(s0 + i * kJoiners, j) : 0;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          if (s0 + i * kJoiners < a.slices) weight = fma(sh.scale[s0 + i * kJoiners], WeightOf(sums[i]), weight);
+          count += CountOf(sums[i]);
+        }
+      }
+      sh.join.weight[joiner][j] = weight;
+      sh.join.count[joiner][j] = count;
+    }
+    __syncthreads();
     double weight = 0.0;
     uint32_t count = 0;
-    constexpr int kBatch = 10;
-#pragma unroll 1
-    for (int s0 = joiner; s0 < a.slices; s0 += kBatch * kJoiners) {
-      uint64_t sums[kBatch];
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) sums[i] = s0 + i * kJoiners < a.slices ? sum_at(s0 + i * kJoiners, j) : 0;
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        if (s0 + i * kJoiners < a.slices) weight += sh.scale[s0 + i * kJoiners] * WeightOf(sums[i]);
-        count += CountOf(sums[i]);
-      }
-    }
-    sh.join.weight[joiner][j] = weight;
-    sh.join.count[joiner][j] = count;
-    __syncthreads();
     if (tid < kBins) {
-      weight = 0.0;
-      count = 0;
 #pragma unroll
       for (int i = 0; i < kJoiners; ++i) {
         weight += sh.join.weight[i][tid];
@@ -518,24 +529,27 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
       sh.count[tid] = count;
     }
     __syncthreads();
-    const bool first_bin = tid == 0, a_bin = tid < kBins;
     on_k = set.k > 0 && static_cast<uint32_t>(set.k) < sh.count[kBins - 1];  // else it keeps all that is live
-    const uint32_t before_count = first_bin || !a_bin ? 0 : sh.count[tid - 1];
-    const double before_weight = first_bin || !a_bin ? 0.0 : sh.weight[tid - 1];
+    const bool first_bin = tid == 0;
     // top_k's bin
     const uint32_t k = static_cast<uint32_t>(set.k);
-    if (a_bin && on_k && before_count < k && k <= count) sh.bin[0] = static_cast<uint32_t>(tid);
-    __syncthreads();
+    if (on_k) {
+      if (tid < kBins && (first_bin ? 0 : sh.count[tid - 1]) < k && k <= count) sh.bin[0] = static_cast<uint32_t>(tid);
+      __syncthreads();
+    }
     const int bin_k = on_k ? static_cast<int>(sh.bin[0]) : kBins - 1;
     // top_p's: between those of the least and the most that what top_k leaves may weigh, and a rounding more
-    const double most = sh.weight[bin_k], least = !on_k ? most : bin_k == 0 ? 0.0 : sh.weight[bin_k - 1];
-    const double p = static_cast<double>(set.p);
-    const double goal_hi = p * least * (1.0 - 0x1p-40), goal_lo = fmin(p * most * (1.0 + 0x1p-40), most);
-    if (a_bin && on_p) {
-      if (weight >= goal_hi && (first_bin || before_weight < goal_hi)) sh.bin[1] = static_cast<uint32_t>(tid);
-      if (weight >= goal_lo && (first_bin || before_weight < goal_lo)) sh.bin[2] = static_cast<uint32_t>(tid);
+    if (on_p) {
+      if (tid < kBins) {
+        const double before = first_bin ? 0.0 : sh.weight[tid - 1];
+        const double most = sh.weight[bin_k], least = !on_k ? most : bin_k == 0 ? 0.0 : sh.weight[bin_k - 1];
+        const double p = static_cast<double>(set.p);
+        const double goal_hi = p * least * (1.0 - 0x1p-40), goal_lo = fmin(p * most * (1.0 + 0x1p-40), most);
+        if (weight >= goal_hi && (first_bin || before < goal_hi)) sh.bin[1] = static_cast<uint32_t>(tid);
+        if (weight >= goal_lo && (first_bin || before < goal_lo)) sh.bin[2] = static_cast<uint32_t>(tid);
+      }
+      __syncthreads();
     }
-    __syncthreads();
     const int p_hi = static_cast<int>(sh.bin[1]), p_lo = static_cast<int>(sh.bin[2]);
     // min_p's: from the next number above its border to the next below
     int m_hi = kBins - 1, m_lo = kBins - 1;
@@ -560,107 +574,123 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
   }
 
   // ---- of each slice: the weight above these bins, and where its candidates go
-  uint64_t in = 0;
-  if (tid < a.slices) {
-    uint64_t above = mine_of.sum;
-    if (lo >= 0) {
-      above = hi > 0 ? sum_at(tid, hi - 1) : 0;
-      in = CountOf(sum_at(tid, lo)) - CountOf(above);
-    }
-    sh.kept[tid] = scale * WeightOf(above);
-  }
-  uint64_t placed;
-  const uint64_t before_in = RowBefore(in, sh.parts[1], &placed);
-  if (tid < a.slices) sh.offsets[tid] = static_cast<int32_t>(before_in);
-  n = static_cast<uint32_t>(placed);
-  if (tid == 0) sh.offsets[a.slices] = static_cast<int32_t>(n);
-  __syncthreads();
-
-  // ---- the candidates, in index order: first where they are, a wave to a slice, sixteen neighbours to a lane in each of
-  // four rounds; then what they are, all at once
-  const bool in_lds = n <= kInLds;
-  uint32_t* const keys = in_lds ? sh.keys : row.Keys();
-#pragma unroll 1
-  for (int s = n > 0 ? wave : a.slices; s < a.slices; s += kRowWaves) {
-    uint32_t to = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(sh.offsets[s]));
-    if (to == static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(sh.offsets[s + 1]))) continue;
-    const int off = __builtin_amdgcn_readfirstlane(sh.off[s]);
-    // in the slice's own bins, whose last is the row's last
-    const int from = max(0, hi - off), upto = lo == kBins - 1 ? lo : lo - off;
-    uint4 b[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) b[i] = *reinterpret_cast<const uint4*>(row.BytesOf(s) + 1024 * i + 16 * lane);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t words[4] = {b[i].x, b[i].y, b[i].z, b[i].w};
-      uint32_t takes = 0;
-#pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        const uint32_t byte = words[c / 4] >> (8 * (c % 4)) & 255;
-        takes |= (byte - static_cast<uint32_t>(from) <= static_cast<uint32_t>(upto - from) ? 1u : 0u) << c;
-      }
-      const int32_t at = s * kSlice + 1024 * i + 16 * lane;
-      if (lo == kBins - 1) {  // minus infinity has the last bin's byte too
-        for (uint32_t left = takes; left != 0; left &= left - 1) {
-          const int c = __builtin_ctz(left);
-          if (row.LoadOne(at + c) == -INFINITY) takes &= ~(1u << c);
+  if (wave == 0) {
+    uint64_t placed = 0;
+    slices64([&](int s, bool there) {
+      uint64_t in = 0;
+      if (there) {
+        uint64_t above = sh.sum[s];
+        if (lo >= 0) {
+          above = hi > 0 ? sum_at(s, hi - 1) : 0;
+          in = CountOf(sum_at(s, lo)) - CountOf(above);
         }
+        sh.kept[s] = sh.scale[s] * WeightOf(above);
       }
-      const uint32_t count = static_cast<uint32_t>(__builtin_popcount(takes));
-      const uint32_t sum = attn::ScanAdd(count);
-      uint32_t next = to + sum - count;
-      to += __builtin_amdgcn_readlane(sum, 63);
-      for (; takes != 0; takes &= takes - 1) keys[next++] = static_cast<uint32_t>(at + __builtin_ctz(takes));
-    }
+      const uint64_t upto = WaveInclScanU64(in);
+      if (there) sh.offsets[s] = static_cast<int32_t>(placed + upto - in);
+      placed += LastLane(upto);
+    });
+    if (lane == 0) sh.offsets[a.slices] = static_cast<int32_t>(placed);
   }
   __syncthreads();
-  uint32_t low = 0xFFFFFFFFu, high = 0;
-#pragma unroll 1
-  for (uint32_t i0 = tid; i0 < n; i0 += 4 * kRowThreads) {
-    float x[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t at = i0 + i * kRowThreads;
-      x[i] = row.LoadOne(static_cast<int32_t>(at < n ? keys[at] : 0));
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t at = i0 + i * kRowThreads;
-      if (at < n) {
-        keys[at] = KeyOf(x[i]);
-        low = min(low, KeyOf(x[i]));
-        high = max(high, KeyOf(x[i]));
-      }
-    }
-  }
-  const auto key_at = [&](uint32_t i) { return keys[i]; };
+  const uint32_t n = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(sh.offsets[a.slices]));
 
-  // ---- the cut
   const double least = cut_m ? static_cast<double>(set.m) / unit : 0.0;  // in units
   Cut cut;
   uint64_t tie = 0;  // weight of a tie, if it counts
   if (n > 0) {
-    if (cut_k || cut_p) {
-      high = static_cast<uint32_t>(RowMax(high, sh.parts[0]));
-      low = ~static_cast<uint32_t>(RowMax(~low, sh.parts[1]));
-      const int width = 32 - __builtin_clz((high - low) | 1);
-      // first top_k's among its candidates, then top_p's among what that keeps
-      if (cut_k) cut = Select(key_at, n, low, width, units, false, cut, static_cast<uint64_t>(set.k) - base_count, sh);
-      if (cut_p) {
-        double of_all = all_weight;
-        if (on_k) {
-          uint64_t whole = 0, total;
+    // ---- the candidates, in index order: first where they are, a wave to a slice, sixteen neighbours to a lane in each of
+    // four rounds; then what they are, all at once
+    uint32_t* const keys = n <= kInLds ? sh.keys : row.Keys();
 #pragma unroll 1
-          for (uint32_t i = tid; i < n; i += kRowThreads) {
-            const uint32_t key = key_at(i);
-            if (key > cut.key) whole += units.OfKey(key);
+    for (int s = wave; s < a.slices; s += kRowWaves) {
+      uint32_t to = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(sh.offsets[s]));
+      if (to == static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(sh.offsets[s + 1]))) continue;
+      const int off = __builtin_amdgcn_readfirstlane(sh.off[s]);
+      // in the slice's own bins, whose last is the row's last
+      const int from = max(0, hi - off), upto = lo == kBins - 1 ? lo : lo - off;
+      const uint32_t from4 = static_cast<uint32_t>(from) * 0x01010101u;
+      const uint32_t beyond4 = static_cast<uint32_t>(255 - (upto - from)) * 0x01010101u;
+      uint4 b[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) b[i] = *reinterpret_cast<const uint4*>(row.BytesOf(s) + 1024 * i + 16 * lane);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int32_t at = s * kSlice + 1024 * i + 16 * lane;
+        uint32_t takes = BytesWithin(b[i].x, from4, beyond4) >> 7 | BytesWithin(b[i].y, from4, beyond4) >> 6 |
+                         BytesWithin(b[i].z, from4, beyond4) >> 5 | BytesWithin(b[i].w, from4, beyond4) >> 4;
+        // bit 8 c + w is element 4 w + c
+        const auto place_of = [](int bit) { return 4 * (bit & 7) + (bit >> 3); };
+        if (lo == kBins - 1) {  // minus infinity has the last bin's byte too
+          for (uint32_t left = takes; left != 0; left &= left - 1) {
+            const int bit = __builtin_ctz(left);
+            if (row.LoadOne(at + place_of(bit)) == -INFINITY) takes &= ~(1u << bit);
           }
-          RowBefore(whole, sh.parts[0], &total);
-          of_all = base + static_cast<double>(total + cut.ties * units.OfKey(cut.key)) * unit;
         }
-        const double of = ceil((static_cast<double>(set.p) * of_all - base) / unit);
-        cut = Select(key_at, n, low, width, units, true, cut, of < 1.0 ? 1 : static_cast<uint64_t>(fmin(of, 0x1p62)), sh);
+        const uint32_t count = static_cast<uint32_t>(__builtin_popcount(takes));
+        const uint32_t sum = attn::ScanAdd(count);
+        uint32_t next = to + sum - count;
+        to += __builtin_amdgcn_readlane(sum, 63);
+        if (__ballot(takes != 0) != 0) {
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            for (uint32_t left = takes & (0x01010101u << w); left != 0; left &= left - 1) {
+              keys[next++] = static_cast<uint32_t>(at + place_of(__builtin_ctz(left)));
+            }
+          }
+        }
       }
+    }
+    __syncthreads();
+    {
+      uint32_t low = 0xFFFFFFFFu, high = 0;
+#pragma unroll 1
+      for (uint32_t i0 = tid; i0 < n; i0 += 4 * kRowThreads) {
+        float x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t at = i0 + i * kRowThreads;
+          x[i] = at < n ? row.LoadOne(static_cast<int32_t>(keys[at])) : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t at = i0 + i * kRowThreads;
+          if (at < n) {
+            keys[at] = KeyOf(x[i]);
+            low = min(low, KeyOf(x[i]));
+            high = max(high, KeyOf(x[i]));
+          }
+        }
+      }
+      if (high != 0) {
+        atomicMin(&sh.low, low);
+        atomicMax(&sh.high, high);
+      }
+    }
+    __syncthreads();
+
+    // ---- the cut: first top_k's, then top_p's among what that keeps
+    const int width = 32 - __builtin_clz((sh.high - sh.low) | 1);
+    if (cut_k) cut = Select(keys, n, sh.low, width, units, false, cut, static_cast<uint64_t>(set.k) - base_count, sh);
+    if (cut_p) {
+      double of_all = all_weight;
+      if (on_k) {
+        if (tid == 0) sh.found[0] = 0;
+        __syncthreads();
+        uint64_t whole = 0;
+#pragma unroll 1
+        for (uint32_t i = tid; i < n; i += kRowThreads) {
+          if (keys[i] > cut.key) whole += units.OfKey(keys[i]);
+        }
+        if (whole != 0) {
+          atomicAdd(reinterpret_cast<unsigned long long*>(&sh.found[0]), static_cast<unsigned long long>(whole));
+        }
+        __syncthreads();
+        of_all = base + static_cast<double>(sh.found[0] + cut.ties * units.OfKey(cut.key)) * unit;
+        __syncthreads();
+      }
+      const double of = ceil((static_cast<double>(set.p) * of_all - base) / unit);
+      cut = Select(keys, n, sh.low, width, units, true, cut, of < 1.0 ? 1 : static_cast<uint64_t>(fmin(of, 0x1p62)), sh);
     }
     if (cut.ties > 0) {
       const double of = units.Of(ValueOf(cut.key));
@@ -671,7 +701,7 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
     // ---- what it keeps of each slice's candidates
 #pragma unroll 1
     for (uint32_t i = tid; i < n; i += kRowThreads) {
-      const uint32_t key = key_at(i);
+      const uint32_t key = keys[i];
       if (key < cut.key) continue;
       int s = 0;  // the last slice that begins at or before i
       for (int step = 1 << (31 - __builtin_clz(a.slices)); step > 0; step >>= 1) {
@@ -687,56 +717,79 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
       }
     }
     __syncthreads();
-    const uint64_t ties = tid < a.slices ? sh.ties[tid] : 0;
-    uint64_t unused;
-    const uint64_t before = RowBefore(ties, sh.parts[0], &unused);
-    if (tid < a.slices) {
-      const uint64_t left = before < cut.ties ? cut.ties - before : 0;
-      const uint64_t first = ties < left ? ties : left;
-      sh.first[tid] = static_cast<uint32_t>(first);
-      sh.kept[tid] += static_cast<double>(sh.kept_in[tid] + first * tie) * unit;
-    }
   }
 
   // ---- u's slice, by sums in index order: the first whose end passes it, or the last that has any weight
-  if (tid == 0) sh.slice = 0x7FFFFFFF;
-  const double mine = tid < a.slices ? sh.kept[tid] : 0.0;
-  double weight;
-  const double before = RowBeforeD(mine, sh.dparts, &weight);
-  const double goal = (set.u > 0.0f ? fmin(static_cast<double>(set.u), 1.0) : 0.0) * weight;
-  if (mine > 0.0 && goal < before + mine) atomicMin(&sh.slice, tid);
-  __syncthreads();
-  if (sh.slice == tid) sh.before = before;
-  if (sh.slice == 0x7FFFFFFF) {  // u of 1, or rounding: the last
-    const uint64_t last = RowMax(mine > 0.0 ? static_cast<uint64_t>(tid) : 0, sh.parts[1]);
-    if (tid == 0) {
-      sh.slice = static_cast<int32_t>(last);
-      sh.before = -1.0;  // the last of it
+  if (wave == 0) {
+    uint64_t ties_before = 0;
+    double all = 0.0;
+    slices64([&](int s, bool there) {
+      uint64_t ties = 0;
+      if (n > 0) {
+        ties = there ? sh.ties[s] : 0;
+        const uint64_t upto = WaveInclScanU64(ties), before = ties_before + upto - ties;
+        ties_before += LastLane(upto);
+        ties = min(ties, before < cut.ties ? cut.ties - before : 0);
+      }
+      double kept = 0.0;
+      if (there) {
+        kept = sh.kept[s] + static_cast<double>(sh.kept_in[s] + ties * tie) * unit;
+        sh.first[s] = static_cast<uint32_t>(ties);
+      }
+      const double upto = all + WaveInclScanD(kept);
+      if (there) sh.kept[s] = kept > 0.0 ? upto : -1.0;  // where it ends
+      all = LastLane(upto);
+    });
+    const double goal = (set.u > 0.0f ? fmin(static_cast<double>(set.u), 1.0) : 0.0) * all;
+    int32_t found = 0x7FFFFFFF, last = 0;
+    double end_before = 0.0, before = 0.0;  // the end of the last slice of any weight, and that before the one found
+    slices64([&](int s, bool there) {
+      const double end = there ? sh.kept[s] : -1.0;
+      const uint64_t some = __ballot(end >= 0.0), past = __ballot(end > goal);
+      if (found == 0x7FFFFFFF && past != 0) {
+        const int at = __builtin_ctzll(past);
+        const uint64_t earlier = some & ((uint64_t(1) << at) - 1);
+        found = s - lane + at;
+        before = earlier != 0 ? sh.kept[s - lane + 63 - __builtin_clzll(earlier)] : end_before;
+      }
+      if (some != 0) {
+        last = s - lane + 63 - __builtin_clzll(some);
+        end_before = sh.kept[last];
+      }
+    });
+    if (lane == 0) {
+      sh.slice = found != 0x7FFFFFFF ? found : last;
+      sh.before = found != 0x7FFFFFFF ? floor((goal - before) / unit) : 0x1p63;  // u's place in it, in units
+      sh.weight_of_all = all;
     }
   }
   __syncthreads();
   const int slice = __builtin_amdgcn_readfirstlane(sh.slice);
-  const double inside = sh.before < 0.0 ? 0x1p63 : floor(fmax(goal - sh.before, 0.0) / unit);
+  const double inside = sh.before;
   const uint64_t place = inside < 0x1p63 ? static_cast<uint64_t>(inside) : ~uint64_t(0);
 
   // ---- the walk: four neighbours to a thread
   static_assert(kSlice == 4 * kRowThreads, "");
-  const uint64_t ties_kept = sh.first[slice];
-  const bool some_ties = ties_kept > 0 && ties_kept < sh.ties[slice];  // and not all: their order counts
   const int at = slice * kSlice + 4 * tid;
   const float4 v = row.Load(at);
   const float x[4] = {v.x, v.y, v.z, v.w};
+  const uint64_t ties_kept = sh.first[slice];
+  const bool some_ties = ties_kept > 0 && ties_kept < sh.ties[slice];  // and not all: their order counts
   uint64_t tie_at = 0;
   if (some_ties) {
-    uint64_t ties = 0, unused;
+    uint64_t ties = 0;
 #pragma unroll
     for (int c = 0; c < 4; ++c) ties += x[c] > -INFINITY && KeyOf(x[c]) == cut.key ? 1 : 0;
-    tie_at = RowBefore(ties, sh.parts[1], &unused);
+    const uint64_t upto = WaveInclScanU64(ties);
+    if (lane == 63) sh.wave_sum[wave] = upto;
+    __syncthreads();
+    tie_at = upto - ties;
+    for (int w = 0; w < wave; ++w) tie_at += sh.wave_sum[w];
     __syncthreads();
   }
   uint64_t w[4], sum = 0;
   double of[4];
-  uint64_t last = 0;  // the last kept one, before all those of a weight above 0
+  uint32_t last = 0;  // the last kept one, above all those of no weight
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     const uint32_t key = KeyOf(x[c]);
@@ -753,10 +806,21 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
     keep = keep && x[c] > -INFINITY;
     w[c] = keep ? Units::Whole(of[c]) : 0;
     sum += w[c];
-    if (keep) last = max(last, (w[c] > 0 ? uint64_t(1) << 32 : 0) + static_cast<uint64_t>(at + c + 1));
+    if (keep) last = max(last, (w[c] > 0 ? 0x80000000u : 0u) + static_cast<uint32_t>(at + c + 1));
   }
-  uint64_t total;
-  uint64_t seen = RowBefore(sum, sh.parts[0], &total);
+  const uint64_t upto = WaveInclScanU64(sum);
+  if (lane == 63) sh.wave_sum[wave] = upto;
+#pragma unroll
+  for (int by = 32; by > 0; by >>= 1) last = max(last, static_cast<uint32_t>(__shfl_xor(static_cast<int>(last), by, 64)));
+  if (lane == 0) sh.wave_last[wave] = last;
+  __syncthreads();
+  uint64_t seen = upto - sum, total = 0;
+#pragma unroll
+  for (int i = 0; i < kRowWaves; ++i) {
+    if (i < wave) seen += sh.wave_sum[i];
+    total += sh.wave_sum[i];
+  }
+  const double weight = sh.weight_of_all;
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     if (seen <= place && place < seen + w[c]) {
@@ -765,14 +829,13 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
     }
     seen += w[c];
   }
-  if (total > place) return;
+  if (total > place || tid != 0) return;
   // rounding, u of 1, or weights of less than half a unit each, of which one is as near as another
-  last = RowMax(last, sh.parts[1]);
-  if (tid == 0) {
-    const int32_t token = static_cast<int32_t>(last & 0xFFFFFFFFu) - 1;
-    a.tokens[row.r] = token;
-    if (a.probs != nullptr) a.probs[row.r] = static_cast<float>(units.Of(row.LoadOne(token)) * unit / weight);
-  }
+  uint64_t which = 0;
+  for (int i = 0; i < kRowWaves; ++i) which = max(which, sh.wave_last[i]);
+  const int32_t token = static_cast<int32_t>(which & 0x7FFFFFFFu) - 1;
+  a.tokens[row.r] = token;
+  if (a.probs != nullptr) a.probs[row.r] = static_cast<float>(units.Of(row.LoadOne(token)) * unit / weight);
 }
 
 // ---------------------------------------------------------------- host side
