@@ -362,11 +362,26 @@ struct Units {
   __device__ __forceinline__ uint64_t OfKey(uint32_t key) const { return Whole(Of(ValueOf(key))); }
 };
 
+// The candidates' keys: in LDS where they fit.
+struct Keys {
+  uint32_t* lds;
+  uint32_t* rest;
+  bool in_lds;
+  __device__ __forceinline__ uint32_t operator[](uint32_t i) const { return in_lds ? lds[i] : rest[i]; }
+  __device__ __forceinline__ void Put(uint32_t i, uint32_t key) const {
+    if (in_lds) {
+      lds[i] = key;
+    } else {
+      rest[i] = key;
+    }
+  }
+};
+
 // The cut after the fewest first candidates, in order, whose amounts (1, or their weight) reach `goal` (or all of them),
 // among those that `cut` keeps: radix selection from the upper of the `width` bits down in which keys, less the least,
 // differ. The amounts of all ties of cut.key enter, which decides nothing: it is the last key. sh.digits are 0, and are so
 // again.
-__device__ __forceinline__ Cut Select(const uint32_t* keys, uint32_t n, uint32_t least, int width, const Units& units,
+__device__ __forceinline__ Cut Select(const Keys& keys, uint32_t n, uint32_t least, int width, const Units& units,
                                       bool by_weight, const Cut& cut, uint64_t goal, ChooseShared& sh) {
   uint32_t prefix = 0;
   if (threadIdx.x == 0) sh.found[0] = sh.found[1] = 0;  // candidates of no weight at all: the last
@@ -412,13 +427,13 @@ __device__ __forceinline__ Cut Select(const uint32_t* keys, uint32_t n, uint32_t
   return Cut{key, each > 0 ? (goal + each - 1) / each : 0};
 }
 
-// Of four bytes those in [from, from + span], as their highest bits. (Bytes are subtracted and added without carries
+// Of four bytes those in [from, from + span], as a 1 in each. (Bytes are subtracted and added without carries
 // between them; a byte less `from` exceeds the span where adding 255 - span carries out.)
 __device__ __forceinline__ uint32_t BytesWithin(uint32_t bytes, uint32_t from4, uint32_t beyond4) {
   constexpr uint32_t kHigh = 0x80808080u;
   const uint32_t less = ((bytes | kHigh) - (from4 & ~kHigh)) ^ ((bytes ^ ~from4) & kHigh);
   const uint32_t low = (less & ~kHigh) + (beyond4 & ~kHigh);
-  return ~((less & beyond4) | ((less | beyond4) & low)) & kHigh;
+  return (~((less & beyond4) | ((less | beyond4) & low)) & kHigh) >> 7;
 }
 
 // Grid: rows.
@@ -551,13 +566,15 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
       __syncthreads();
     }
     const int p_hi = static_cast<int>(sh.bin[1]), p_lo = static_cast<int>(sh.bin[2]);
-    // min_p's: from the next number above its border to the next below
+    // min_p's: that of the nearest number to its border, and the next in either direction, where the border's rounding (the
+    // hardware's logarithm is within 2^-20 of an octave here, a bin an eighth of one) and its number's may have it
     int m_hi = kBins - 1, m_lo = kBins - 1;
     if (on_m) {
-      const double border = static_cast<double>(top) + log(static_cast<double>(set.m)) * static_cast<double>(set.t);
-      const float near = static_cast<float>(fmax(border, -static_cast<double>(FLT_MAX)));
-      m_hi = set.BinBelow(top_bin, fminf(nextafterf(near, INFINITY), top));
-      m_lo = set.BinBelow(top_bin, nextafterf(near, -INFINITY));
+      const double octaves = static_cast<double>(__builtin_amdgcn_logf(set.m));
+      const double border = static_cast<double>(top) + octaves / set.by;
+      const uint32_t near = KeyOf(static_cast<float>(fmax(border, -static_cast<double>(FLT_MAX))));
+      m_hi = max(set.BinBelow(top_bin, fminf(ValueOf(near + 1), top)) - 1, 0);
+      m_lo = min(set.BinBelow(top_bin, ValueOf(near - 1)) + 1, kBins - 1);
     }
     // The cut that counts is the highest: filters that start below where another has cut for sure do not matter. top_p's
     // place needs what top_k leaves, and so the bins down to its.
@@ -599,47 +616,55 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
   Cut cut;
   uint64_t tie = 0;  // weight of a tie, if it counts
   if (n > 0) {
-    // ---- the candidates, in index order: first where they are, a wave to a slice, sixteen neighbours to a lane in each of
-    // four rounds; then what they are, all at once
-    uint32_t* const keys = n <= kInLds ? sh.keys : row.Keys();
+    // ---- the candidates, in index order: first where they are, a wave to a slice, 64 neighbours to a lane; then what they
+    // are, all at once
+    const Keys keys{sh.keys, row.Keys(), n <= kInLds};
+    const auto next_with = [&](int s) {  // from s on, of this wave's slices the next with candidates
+      while (s < a.slices && sh.offsets[s] == sh.offsets[s + 1]) s += kRowWaves;
+      return __builtin_amdgcn_readfirstlane(s);
+    };
+    uint4 bytes[4];
+    const auto load = [&](int s) {
+      if (s >= a.slices) return;
+      const uint4* const from = reinterpret_cast<const uint4*>(row.BytesOf(s)) + 4 * lane;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) bytes[i] = from[i];
+    };
+    int s = next_with(wave);
+    load(s);
 #pragma unroll 1
-    for (int s = wave; s < a.slices; s += kRowWaves) {
-      uint32_t to = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(sh.offsets[s]));
-      if (to == static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(sh.offsets[s + 1]))) continue;
+    while (s < a.slices) {
       const int off = __builtin_amdgcn_readfirstlane(sh.off[s]);
       // in the slice's own bins, whose last is the row's last
       const int from = max(0, hi - off), upto = lo == kBins - 1 ? lo : lo - off;
       const uint32_t from4 = static_cast<uint32_t>(from) * 0x01010101u;
       const uint32_t beyond4 = static_cast<uint32_t>(255 - (upto - from)) * 0x01010101u;
-      uint4 b[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) b[i] = *reinterpret_cast<const uint4*>(row.BytesOf(s) + 1024 * i + 16 * lane);
+      uint32_t part[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int32_t at = s * kSlice + 1024 * i + 16 * lane;
-        uint32_t takes = BytesWithin(b[i].x, from4, beyond4) >> 7 | BytesWithin(b[i].y, from4, beyond4) >> 6 |
-                         BytesWithin(b[i].z, from4, beyond4) >> 5 | BytesWithin(b[i].w, from4, beyond4) >> 4;
-        // bit 8 c + w is element 4 w + c
-        const auto place_of = [](int bit) { return 4 * (bit & 7) + (bit >> 3); };
-        if (lo == kBins - 1) {  // minus infinity has the last bin's byte too
-          for (uint32_t left = takes; left != 0; left &= left - 1) {
-            const int bit = __builtin_ctz(left);
-            if (row.LoadOne(at + place_of(bit)) == -INFINITY) takes &= ~(1u << bit);
-          }
-        }
-        const uint32_t count = static_cast<uint32_t>(__builtin_popcount(takes));
-        const uint32_t sum = attn::ScanAdd(count);
-        uint32_t next = to + sum - count;
-        to += __builtin_amdgcn_readlane(sum, 63);
-        if (__ballot(takes != 0) != 0) {
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            for (uint32_t left = takes & (0x01010101u << w); left != 0; left &= left - 1) {
-              keys[next++] = static_cast<uint32_t>(at + place_of(__builtin_ctz(left)));
-            }
-          }
+        // sixteen bits in order, by sums of 1, 2, 4, ... for each byte that is in
+        const uint32_t low = __builtin_amdgcn_udot4(
+            BytesWithin(bytes[i].x, from4, beyond4), 0x08040201u,
+            __builtin_amdgcn_udot4(BytesWithin(bytes[i].y, from4, beyond4), 0x80402010u, 0, false), false);
+        const uint32_t high = __builtin_amdgcn_udot4(
+            BytesWithin(bytes[i].z, from4, beyond4), 0x08040201u,
+            __builtin_amdgcn_udot4(BytesWithin(bytes[i].w, from4, beyond4), 0x80402010u, 0, false), false);
+        part[i] = high << 8 | low;
+      }
+      uint64_t takes = static_cast<uint64_t>(part[3] << 16 | part[2]) << 32 | (part[1] << 16 | part[0]);
+      const int32_t at = s * kSlice + 64 * lane;
+      uint32_t next = static_cast<uint32_t>(sh.offsets[s]);
+      s = next_with(s + kRowWaves);
+      load(s);
+      if (lo == kBins - 1) {  // minus infinity has the last bin's byte too
+        for (uint64_t left = takes; left != 0; left &= left - 1) {
+          const int c = __builtin_ctzll(left);
+          if (row.LoadOne(at + c) == -INFINITY) takes &= ~(uint64_t(1) << c);
         }
       }
+      const uint32_t count = static_cast<uint32_t>(__builtin_popcountll(takes));
+      next += attn::ScanAdd(count) - count;
+      for (; takes != 0; takes &= takes - 1) keys.Put(next++, static_cast<uint32_t>(at + __builtin_ctzll(takes)));
     }
     __syncthreads();
     {
@@ -656,7 +681,7 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
         for (int i = 0; i < 4; ++i) {
           const uint32_t at = i0 + i * kRowThreads;
           if (at < n) {
-            keys[at] = KeyOf(x[i]);
+            keys.Put(at, KeyOf(x[i]));
             low = min(low, KeyOf(x[i]));
             high = max(high, KeyOf(x[i]));
           }
@@ -671,26 +696,31 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
 
     // ---- the cut: first top_k's, then top_p's among what that keeps
     const int width = 32 - __builtin_clz((sh.high - sh.low) | 1);
-    if (cut_k) cut = Select(keys, n, sh.low, width, units, false, cut, static_cast<uint64_t>(set.k) - base_count, sh);
-    if (cut_p) {
-      double of_all = all_weight;
-      if (on_k) {
-        if (tid == 0) sh.found[0] = 0;
-        __syncthreads();
-        uint64_t whole = 0;
 #pragma unroll 1
-        for (uint32_t i = tid; i < n; i += kRowThreads) {
-          if (keys[i] > cut.key) whole += units.OfKey(keys[i]);
+    for (int filter = cut_k ? 0 : 1; filter < (cut_p ? 2 : 1); ++filter) {
+      uint64_t goal = static_cast<uint64_t>(set.k) - base_count;
+      if (filter == 1) {
+        double of_all = all_weight;
+        if (on_k) {
+          if (tid == 0) sh.found[0] = 0;
+          __syncthreads();
+          uint64_t whole = 0;
+#pragma unroll 1
+          for (uint32_t i = tid; i < n; i += kRowThreads) {
+            const uint32_t key = keys[i];
+            if (key > cut.key) whole += units.OfKey(key);
+          }
+          if (whole != 0) {
+            atomicAdd(reinterpret_cast<unsigned long long*>(&sh.found[0]), static_cast<unsigned long long>(whole));
+          }
+          __syncthreads();
+          of_all = base + static_cast<double>(sh.found[0] + cut.ties * units.OfKey(cut.key)) * unit;
+          __syncthreads();
         }
-        if (whole != 0) {
-          atomicAdd(reinterpret_cast<unsigned long long*>(&sh.found[0]), static_cast<unsigned long long>(whole));
-        }
-        __syncthreads();
-        of_all = base + static_cast<double>(sh.found[0] + cut.ties * units.OfKey(cut.key)) * unit;
-        __syncthreads();
+        const double of = ceil((static_cast<double>(set.p) * of_all - base) / unit);
+        goal = of < 1.0 ? 1 : static_cast<uint64_t>(fmin(of, 0x1p62));
       }
-      const double of = ceil((static_cast<double>(set.p) * of_all - base) / unit);
-      cut = Select(keys, n, sh.low, width, units, true, cut, of < 1.0 ? 1 : static_cast<uint64_t>(fmin(of, 0x1p62)), sh);
+      cut = Select(keys, n, sh.low, width, units, filter == 1, cut, goal, sh);
     }
     if (cut.ties > 0) {
       const double of = units.Of(ValueOf(cut.key));
