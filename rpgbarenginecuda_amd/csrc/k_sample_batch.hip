@@ -46,7 +46,7 @@ static_assert((int64_t(kSlice) << kSliceUnits) < (int64_t(1) << kWeightBits) && 
 // ---------------------------------------------------------------- order and weights
 
 // What a logit counts as: NaN as minus infinity, plus infinity as the largest number.
-__device__ __forceinline__ float Clean(float x) { return x != x ? -INFINITY : fminf(x, FLT_MAX); }
+__device__ __forceinline__ float Clean(float x) { return fminf(fmaxf(x, -INFINITY), FLT_MAX); }
 
 // Order-preserving map onto uint32, both zeros alike, and its inverse.
 __device__ __forceinline__ uint32_t KeyOf(float x) {
@@ -76,7 +76,11 @@ struct Exp2Near {
 #pragma unroll
     for (int i = 0; i < 9; ++i) {
       c[i] = kC[i] * static_cast<double>(uint64_t(1) << kBits);
-      asm volatile("" : "+s"(c[i]));
+      if (i == 7) {  // c[8] f + c[7] has room for one scalar
+        asm volatile("" : "+v"(c[i]));
+      } else {
+        asm volatile("" : "+s"(c[i]));
+      }
     }
   }
   __device__ __forceinline__ double Of(double f) const {
@@ -97,14 +101,12 @@ __device__ __forceinline__ uint64_t OneOf(const Exp2Near<kSliceUnits>& near, dou
   v = fmax(v, -200.0);
   // 1.5 * 2^52 added rounds v to a whole number, the low word; 2^52 added to a weight leaves its whole units
   const double shifted = v + 0x1.8p52;
-  const uint64_t part = __builtin_bit_cast(uint64_t, near.Of(v - (shifted - 0x1.8p52)));
-  const uint32_t exponent = static_cast<uint32_t>(__builtin_bit_cast(uint64_t, shifted)) << 20;
-  const uint64_t scaled = (static_cast<uint64_t>(static_cast<uint32_t>(part >> 32) + exponent) << 32) |
-                          static_cast<uint32_t>(part);
-  const uint64_t bits = __builtin_bit_cast(uint64_t, __builtin_bit_cast(double, scaled) + 0x1p52);
+  dev::U32x2 part = __builtin_bit_cast(dev::U32x2, near.Of(v - (shifted - 0x1.8p52)));
+  part[1] += __builtin_bit_cast(dev::U32x2, shifted)[0] << 20;
+  dev::U32x2 bits = __builtin_bit_cast(dev::U32x2, __builtin_bit_cast(double, part) + 0x1p52);
   constexpr uint32_t kOne = 1u << (kWeightBits - 32);
-  return (static_cast<uint64_t>(static_cast<uint32_t>(bits >> 32) - (0x43300000u - kOne)) << 32) |
-         static_cast<uint32_t>(bits);
+  bits[1] -= 0x43300000u - kOne;
+  return __builtin_bit_cast(uint64_t, bits);
 }
 __device__ __forceinline__ uint32_t CountOf(uint64_t sum) { return static_cast<uint32_t>(sum >> kWeightBits); }
 // In units of 2^-38: 2^52 and it are one double, bit for bit.
@@ -204,8 +206,8 @@ struct Row {  // of the logits and the workspace
   // Candidates that do not fit into LDS.
   __device__ __forceinline__ uint32_t* Keys() const { return reinterpret_cast<uint32_t*>(at + place.keys); }
   // Four logits from i on; what lies behind the row's end is minus infinity.
-  __device__ __forceinline__ float4 Load(int32_t i) const {
-    const float4 x = dev::LoadBuf4<0>(logits, 4u * static_cast<uint32_t>(i));
+  __device__ __forceinline__ float4 Load(int32_t i) const { return Checked(dev::LoadBuf4<0>(logits, 4u * static_cast<uint32_t>(i)), i); }
+  __device__ __forceinline__ float4 Checked(float4 x, int32_t i) const {
     return make_float4(i < n ? Clean(x.x) : -INFINITY, i + 1 < n ? Clean(x.y) : -INFINITY,
                        i + 2 < n ? Clean(x.z) : -INFINITY, i + 3 < n ? Clean(x.w) : -INFINITY);
   }
@@ -229,11 +231,21 @@ __global__ __launch_bounds__(kThreads) void SampleSlicesKernel(const SampleArgs 
   float x[kEach];
 #pragma unroll
   for (int i = 0; i < kEach; i += 4) {
-    const float4 v = row.Load(slice * kSlice + i * kThreads + 4 * tid);
+    const float4 v = dev::LoadBuf4<0>(row.logits, 4u * static_cast<uint32_t>(slice * kSlice + i * kThreads + 4 * tid));
     x[i] = v.x, x[i + 1] = v.y, x[i + 2] = v.z, x[i + 3] = v.w;
   }
   const Setting set = SettingOf(a, row.r);
   const bool filters = !set.greedy && set.Filters();
+  if (__builtin_expect(slice + 1 < a.slices, 1)) {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) x[i] = Clean(x[i]);
+  } else {  // the row may end in it
+#pragma unroll
+    for (int i = 0; i < kEach; i += 4) {
+      const float4 v = row.Checked(make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]), slice * kSlice + i * kThreads + 4 * tid);
+      x[i] = v.x, x[i + 1] = v.y, x[i + 2] = v.z, x[i + 3] = v.w;
+    }
+  }
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) bins[w][tid] = 0;
   if (tid == 0) first = 0x7FFFFFFF;
@@ -257,9 +269,10 @@ __global__ __launch_bounds__(kThreads) void SampleSlicesKernel(const SampleArgs 
       uint32_t bytes = 0;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const int j = x[i + c] > -INFINITY ? set.BinBelow(top_bin, x[i + c]) : kBins - 1;
+        const bool live = x[i + c] > -INFINITY;
+        const int j = live ? set.BinBelow(top_bin, x[i + c]) : kBins - 1;
         const uint64_t add = OneOf(near, (static_cast<double>(x[i + c]) - dtop) * set.by);
-        if (x[i + c] > -INFINITY) {
+        if (live) {
           atomicAdd(reinterpret_cast<unsigned long long*>(&bins[tid >> 6][j]), static_cast<unsigned long long>(add));
         }
         bytes |= static_cast<uint32_t>(j) << (8 * c);
