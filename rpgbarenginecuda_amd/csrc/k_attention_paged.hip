@@ -182,7 +182,7 @@ struct NotShared {
 };
 
 // Groups of rows that begin with the same pages (dev::SharedGroups): what a row has of them is attended to elsewhere, and
-// here only what is behind. That part's result, relative to its maximum m: o [row][head][D], (m, l) [row][head].
+// here only what is behind.
 struct Shared {
   static constexpr bool kOn = true;
   dev::SharedGroups groups;
@@ -425,27 +425,16 @@ struct AttentionArgs {
   float scale_log2;
 };
 
-// The same, and what the shared positions came to.
+// The same for rows that share their beginnings: what is behind these, and where (m, l) of each row and head go.
 struct SharedAttentionArgs : AttentionArgs {
   const int32_t* group_rows;
   const int32_t* group_pages;
   int32_t n_groups;
-  const float* prefix_o;
-  const float* prefix_ml;
+  float* ml;
 };
 
-// A row's and head's result over the positions behind the shared ones, o under m with sum l, joined with that over them
-// (row_head's of prefix_o and prefix_ml), elements d to d + 3.
-__device__ __forceinline__ float4 JoinPrefix(const SharedAttentionArgs& args, int64_t row_head, int32_t head_dim,
-                                             int32_t d, float4 o, float m, float l) {
-  const float2 ml = *reinterpret_cast<const float2*>(args.prefix_ml + 2 * row_head);
-  const float4 p = dev::Load4(args.prefix_o + row_head * head_dim + d);
-  const float top = fmaxf(m, ml.x);
-  const float safe = top == -INFINITY ? 0.0f : top;
-  const float f = __builtin_amdgcn_exp2f(m - safe), g = __builtin_amdgcn_exp2f(ml.x - safe);
-  const float inv = 1.0f / fmaf(l, f, ml.y * g);
-  return make_float4(fmaf(o.x, f, p.x * g) * inv, fmaf(o.y, f, p.y * g) * inv, fmaf(o.z, f, p.z * g) * inv,
-                     fmaf(o.w, f, p.w * g) * inv);
+__device__ __forceinline__ void StoreMl(const SharedAttentionArgs& args, int64_t row_head, float m, float l) {
+  *reinterpret_cast<float2*>(args.ml + 2 * row_head) = make_float2(m, l);
 }
 
 // kTiles: 8-bit caches, column tiles of up to 4 heads (1 or 2); else 1, of up to 8.
@@ -1049,7 +1038,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Arg
 
       // ---- the piece's (m, l, o): out, or kept where it is not the whole of its pair
       const bool whole = c_first == 0 && c_end == piece_units;
-      const bool joins_prefix = kShared && whole && batch.PagesOf(piece_row) > 0;
       if (!whole) {
         const int which = more ? 0 : 1;
         if (lane == 0) pieces[wave][which] = Piece{u - c_end, c_first, c_end, piece_units, piece_row, piece_pair};
@@ -1062,7 +1050,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Arg
         const float total = of_tile(t, l), top = of_tile(t, m);
         // 8-bit values: one factor after the other, since their product may be too small a number
         const float unit = kQ8 ? 1.0f / of_tile(t, shrink) : 1.0f;
-        const float by = (kQ8 ? 1.0f : 0x1p-14f) / (whole && !joins_prefix ? total : 1.0f);
+        const float by = (kQ8 ? 1.0f : 0x1p-14f) / (whole ? total : 1.0f);
         const int h = t * kHeadCols + head_col;
         F32x4 own[kOwn];
 #pragma unroll
@@ -1084,21 +1072,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Arg
           kept_l[t] = total;
         } else if (h < heads) {
           float* to = whole ? out + (head_row + h) * D : reinterpret_cast<float*>(v_mine) + h * kPart;
-          if constexpr (kShared) {
-            if (joins_prefix) {
-#pragma unroll
-              for (int i = 0; i < kOwn; ++i) {
-                const float4 x = JoinPrefix(args, head_row + h, D, 16 * (copy * kOwn + i) + 4 * g,
-                                            make_float4(own[i][0], own[i][1], own[i][2], own[i][3]), top, total);
-                own[i] = F32x4{x.x, x.y, x.z, x.w};
-              }
-            }
-          }
 #pragma unroll
           for (int i = 0; i < kOwn; ++i) *reinterpret_cast<F32x4*>(to + 16 * (copy * kOwn + i) + 4 * g) = own[i];
           if (!whole && copy == 0 && g == 0) {
             to[D] = top;
             to[D + 1] = total;
+          }
+          if constexpr (kShared) {
+            if (whole && copy == 0 && g == 0) StoreMl(args, head_row + h, top, total);
           }
         }
       }
@@ -1155,7 +1136,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Arg
     const bool leads = run.first + run.c0 == begin;  // the workgroup's first piece
     const __amdgpu_buffer_rsrc_t rs =
         dev::OutResource(slots + (2 * static_cast<int64_t>(me) + (leads ? 0 : 1)) * slot_bytes, slot_bytes);
-    const bool joins_prefix = kShared && whole && batch.PagesOf(run.row) > 0;
     for (int i = threadIdx.x; i < of.heads * (D / 4); i += 64 * kWaves) {
       const int h = i / (D / 4), d = 4 * (i % (D / 4));
       float4 x[2 * kWaves];
@@ -1184,10 +1164,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Arg
       }
       if (whole) {
         if constexpr (kShared) {
-          if (joins_prefix) {
-            dev::Store4(out + (of.head_row + h) * D + d, JoinPrefix(args, of.head_row + h, D, d, o, top, l));
-            continue;
-          }
+          if (d == 0) StoreMl(args, of.head_row + h, top, l);
         }
         const float inv = 1.0f / l;
         dev::Store4(out + (of.head_row + h) * D + d, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
@@ -1313,14 +1290,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Arg
         done = true;
       }
       if (!done) continue;
-      const bool joins_prefix = kShared && batch.PagesOf(run.row) > 0;
       if (set == 0) {
         if constexpr (kShared) {
-          if (joins_prefix) {
-            dev::Store4(out + heads.head_row * D + 4 * column,
-                        JoinPrefix(args, heads.head_row + h, D, 4 * column - h * D, o, top, l));
-            continue;
-          }
+          if (4 * column == h * D) StoreMl(args, heads.head_row + h, top, l);
         }
         const float inv = 1.0f / l;
         dev::Store4(out + heads.head_row * D + 4 * column, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
@@ -1335,16 +1307,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Arg
     if (seq < 0) continue;
     const bool fine = rows.Fine(seq, len);
     if (fine && len > 0) continue;
-    if constexpr (kShared) {
-      if (batch.PagesOf(static_cast<int32_t>(r)) > 0) {  // nothing but what it shares
-        for (int64_t i = threadIdx.x; i < static_cast<int64_t>(n_heads) * (D / 4); i += 64 * kWaves) {
-          const int64_t row_head = r * n_heads + i / (D / 4);
-          const int32_t d = 4 * static_cast<int32_t>(i % (D / 4));
-          dev::Store4(out + row_head * D + d,
-                      JoinPrefix(args, row_head, D, d, make_float4(0.0f, 0.0f, 0.0f, 0.0f), -INFINITY, 0.0f));
-        }
-        continue;
-      }
+    if constexpr (kShared) {  // a row of nothing but what it shares has zeros of no weight
+      for (int32_t h = threadIdx.x; h < n_heads; h += 64 * kWaves) StoreMl(args, r * n_heads + h, -INFINITY, 0.0f);
     }
     const float x = fine ? 0.0f : NAN;
     for (int64_t i = threadIdx.x; i < static_cast<int64_t>(n_heads) * (D / 4); i += 64 * kWaves) {
@@ -1445,15 +1409,15 @@ void AttendPaged(const GpuPagedKv& kv, const GpuPageTable& table, const int32_t*
     Launch("PagedAttentionKernel", KernelFor<AttentionArgs>(kv, tile_heads), grid, block, args);
     return;
   }
-  AttendPrefix(kv, table, seq_ids, lens, q_dev, n_heads, n_rows, static_cast<char*>(workspace) + own, prefix);
+  CheckPrefix(kv, table, n_heads, n_rows, static_cast<char*>(workspace) + own, prefix);
   SharedAttentionArgs shared;
   static_cast<AttentionArgs&>(shared) = args;
   shared.group_rows = prefix->group_rows;
   shared.group_pages = prefix->group_pages;
   shared.n_groups = prefix->n_groups;
-  shared.prefix_o = prefix->o;
-  shared.prefix_ml = prefix->ml;
+  shared.ml = prefix->ml;
   Launch("PagedAttentionKernel", KernelFor<SharedAttentionArgs>(kv, tile_heads), grid, block, shared);
+  AttendPrefix(kv, table, seq_ids, lens, q_dev, n_heads, n_rows, out_dev, *prefix);
 }
 
 void GpuAttentionPaged(const GpuPagedKv& kv, const GpuPageTable& table, const int32_t* seq_ids, const int32_t* lens,

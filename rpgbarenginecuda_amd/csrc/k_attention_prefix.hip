@@ -1,24 +1,25 @@
 // Attention of one new token per row over a paged cache whose rows share their beginnings:
-// here the shared positions, once for all rows of a group; what is each row's own, and the
-// join with this, is k_attention_paged.hip's.
+// here the shared positions, once for all rows of a group, and the join with what each row's own
+// positions came to, which k_attention_paged.hip has left in the output just before.
 //
 // For row r of a group, query head h, over the group's positions j < pages * page_size:
-//   m = max_j s_j,  l = sum_j 2^(s_j - m),  o = sum_j 2^(s_j - m) v_j,  s_j = (q . k_j) log2(e) / sqrt(D).
-// A row's own positions give another (m', l', o'); its output is (o f + o' f') / (l f + l' f') with f = 2^(m - M),
+//   m = max_j s_j,  l = sum_j 2^(s_j - m),  o = sum_j 2^(s_j - m) v_j,  s_j = (q . k_j) log2(e) / sqrt(D),
+// over its own ones m', l' and the output o' / l'; joined (o f + o' f') / (l f + l' f') with f = 2^(m - M),
 // f' = 2^(m' - M), M the larger of m and m'.
 //
 // What bounds it: keys and values are read once for up to 128 columns (the queries of a kv head: rows times heads of a
 // group), so that from some 64 columns on the matrix cores do, which run each product twice: queries and weights, which
-// are fp32, enter as two fp16 terms of 11 bits each, together 22. Over 8-bit pages codes are numbers of fp16 (keys) and of
-// bf16 (values), and weights times their rows' scales enter as three bf16 terms, whose range is fp32's: a scale of any
-// size needs no common power of two.
+// are fp32, enter as two fp16 terms of 11 bits each, together 22. Over 8-bit pages codes are fp16 numbers as they are;
+// keys' scales multiply the scores, and weights times values' scales are brought to fp16's range by a power of two of the
+// column's, which moves with their maximum.
 //
 // A workgroup takes steps of 128 positions through LDS, two of them at a time (one being read, one being filled), for a
 // tile of up to 128 columns; of its eight waves each has 32 columns and a half of the step's keys, a quarter where the
-// tile has no more than 64 columns. The products are those of k_attention_paged.hip: rows of S = K Q^T are 16 keys, rows
-// of O^T = V^T P^T 16 elements, so that a lane ends the first with the weights of the keys that it holds in the second.
-// The units (kv head, column tile, step) of all groups are shared out evenly and contiguously; a tile that several
-// workgroups hold parts of is joined by the last of them to arrive, in order.
+// tile has no more than 64 columns, or 16 columns and a quarter for no more than 32. The products are those of
+// k_attention_paged.hip: rows of S = K Q^T are 16 keys, rows of O^T = V^T P^T 16 elements, so that a lane ends the first
+// with the weights of the keys that it holds in the second. The units (kv head, column tile, step) of all groups are
+// shared out evenly and contiguously; a tile that several workgroups hold parts of is joined by the last of them to
+// arrive, in order.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -40,14 +41,11 @@ using dev::PagedView;
 constexpr int kWaves = 8;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kCols = 128;     // columns of a tile
-constexpr int kWaveCols = 32;  // of a wave
 constexpr int kStep = 128;     // positions of a unit: 16 for each wave to bring in
 constexpr int kGroups = 256;   // workgroups: one to a compute unit
 constexpr uint32_t kLeast = 2;  // units of a workgroup, where there are few
 constexpr size_t kCounterBytes = 256;
 constexpr int kPartPolicy = 16;  // device scope, as the parts in k_attention_paged.hip
-
-using BHalf8 = __bf16 __attribute__((ext_vector_type(8)));
 
 // What a workgroup leaves of a tile that it has a part of: o [column][D], then (m, l) [column].
 __host__ __device__ constexpr uint32_t SlotBytes(int d) { return kCols * (4u * d + 8u); }
@@ -58,6 +56,7 @@ struct PrefixArgs {
   const int32_t* seq_ids;
   const int32_t* lens;
   const float* q;
+  float* out;
   char* workspace;  // counters, slots
   int32_t n_rows;
   int32_t capacity;  // positions that a table row has pages for, at most the largest int32
@@ -77,12 +76,6 @@ __device__ __forceinline__ Terms TermsOf(float a, float b) {
   return Terms{Bits(hi), Bits(lo)};
 }
 
-// The upper halves of two words, packed: bf16 terms cut off, of a in the low half.
-__device__ __forceinline__ uint32_t Uppers(float a, float b) {
-  return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
-}
-__device__ __forceinline__ float Upper(float a) { return __uint_as_float(__float_as_uint(a) & 0xFFFF0000u); }
-
 // Four codes as fp16: 1024 + 128 + code by their bits, less 1152.
 __device__ __forceinline__ uint2 CodesToHalves(uint32_t codes) {
   const uint32_t u = codes ^ 0x80808080u;
@@ -91,14 +84,78 @@ __device__ __forceinline__ uint2 CodesToHalves(uint32_t codes) {
   const Half2 hi = __builtin_bit_cast(Half2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) + by;
   return make_uint2(Bits(lo), Bits(hi));
 }
-// Four codes as bf16, which holds whole numbers to 256.
-__device__ __forceinline__ uint2 CodesToBf16(uint32_t codes) {
-  const auto at = [codes](int i) { return static_cast<float>(static_cast<int8_t>(codes >> (8 * i))); };
-  return make_uint2(Uppers(at(0), at(1)), Uppers(at(2), at(3)));
+// What row_head's own positions came to: the maximum and the sum of its output, which is divided by that.
+struct Own {
+  float m, l;
+};
+__device__ __forceinline__ Own OwnOf(const PrefixArgs& a, int64_t row_head) {
+  const float2 ml = *reinterpret_cast<const float2*>(a.prefix.ml + 2 * row_head);
+  return Own{ml.x, ml.y};
 }
+// The two joined. (An own part of no weight, all of whose scores are minus infinity, is no number: it is left out.)
+struct Both {
+  float of_own, of_shared;
+  bool none;
+  __device__ __forceinline__ Both(const Own& own, float m, float l) {
+    const float top = fmaxf(own.m, m);
+    const float safe = top == -INFINITY ? 0.0f : top;
+    const float f = own.l * __builtin_amdgcn_exp2f(own.m - safe), g = __builtin_amdgcn_exp2f(m - safe);
+    const float inv = 1.0f / fmaf(l, g, f);
+    of_own = f * inv;
+    of_shared = g * inv;
+    none = own.l == 0.0f;
+  }
+  __device__ __forceinline__ float4 Of(float4 own, float4 o) const {
+    if (none) own = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    return make_float4(fmaf(own.x, of_own, o.x * of_shared), fmaf(own.y, of_own, o.y * of_shared),
+                       fmaf(own.z, of_own, o.z * of_shared), fmaf(own.w, of_own, o.w * of_shared));
+  }
+};
+
+// What a workgroup does of a tile: steps [c0, c1) of its `steps`.
+struct Piece {
+  uint32_t first_unit, c0, c1, steps;
+  int32_t of;  // group
+  int32_t first_row, last_row, pages, positions;
+  int32_t kv_head, tile, cols;  // cols: of the tile
+  bool leads;  // the first thing that the workgroup does
+};
 
 template <int D, bool kQ8>
-__global__ __launch_bounds__(kThreads, 2) void SharedPrefixKernel(const PrefixArgs args) {
+struct Stage {
+  static constexpr int kRow = 2 * D;
+  alignas(16) char k[kStep * kRow];
+  alignas(16) char v[kStep * kRow];
+  float k_scale[kQ8 ? kStep : 4], v_scale[kQ8 ? kStep : 4];
+  uint32_t bad[kStep / 16];  // pages out of range
+};
+
+template <int D, bool kQ8>
+struct PrefixShared {
+  Stage<D, kQ8> stages[2];
+  uint8_t takes[kCols];
+  int flag;
+};
+
+// Whether row r, the lane's, is one of group `of` and begins with all of its pages; *seq its sequence.
+__device__ __forceinline__ bool TakesPart(const PrefixArgs& a, const dev::SharedGroups& groups, int32_t r, int32_t of,
+                                          int32_t pages, bool there, int32_t* seq) {
+  const bool first = groups.n == 1 ? true : groups.OfLane(there ? r : -1) == of;
+  int32_t len = 0;
+  *seq = -1;
+  if (there) {
+    *seq = a.seq_ids != nullptr ? a.seq_ids[r] : r;
+    len = a.lens[r];
+  }
+  return there && first && *seq >= 0 && *seq < a.view.n_seqs && len >= 0 && len <= a.capacity &&
+         dev::TakesPart(pages, a.view.page_shift, len);
+}
+
+// kT: tiles of 16 columns of a wave.
+template <int D, bool kQ8, int kT>
+__device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::SharedGroups& groups, const Share& share,
+                                            uint32_t me, const Piece& piece, const int32_t* table,
+                                            PrefixShared<D, kQ8>& sh) {
   constexpr int kRow = 2 * D;              // bytes of a row in LDS
   constexpr int kPieces = kRow / 16;       // of 16 bytes
   constexpr int kSource = kQ8 ? D : 2 * D;  // bytes of a cached row
@@ -108,24 +165,452 @@ __global__ __launch_bounds__(kThreads, 2) void SharedPrefixKernel(const PrefixAr
   constexpr int kE = D / 16;               // tiles of 16 elements of a value row
   constexpr int kTiles = kStep / 16;
   constexpr int kPart = D + 4;             // floats of a joined column: o, m, l
+  constexpr int kWaveCols = 16 * kT;
+  constexpr int kAhead = kQ8 ? 2 : 1;      // steps whose loads are under way
   static_assert(kTiles == kWaves, "a wave brings in 16 positions");
-
-  struct alignas(16) Stage {
-    char k[kStep * kRow];
-    char v[kStep * kRow];
-    float k_scale[kQ8 ? kStep : 4], v_scale[kQ8 ? kStep : 4];
-    uint32_t bad[kTiles];  // pages out of range
-  };
-  __shared__ Stage stages[2];
-  __shared__ uint8_t takes[kCols];
-  __shared__ int flag;
-  static_assert(3 * 64 * kPart * 4 <= sizeof(stages) && kCols * kPart * 4 <= sizeof(stages), "joins fit where keys were");
+  static_assert(kCols * kPart * 4 <= sizeof(sh.stages) && 3 * 64 * kPart * 4 <= sizeof(sh.stages), "joins fit where keys were");
 
   const PagedView& view = args.view;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int n = lane & 15;
   const int g = lane >> 4;
+  const int32_t positions = piece.positions, kh = piece.kv_head;
+  const uint32_t c0 = piece.c0, c1 = piece.c1;
+
+  // ---- bringing in: this wave's 16 positions of a step, their pieces permuted as the reads below need them
+  const auto k_swap = [](int r) { return kPieces == 16 ? r & 15 : r & 7; };
+  const auto v_swap = [](int r) { return 2 * (r & 3); };
+  struct Loaded {
+    uint4 k[kLoads], v[kLoads];
+    float scale;  // lane i: of key i, lane 16 + i of value i
+    uint32_t bad;
+    bool got;
+  };
+  Loaded loaded[kAhead];
+  const auto page_of = [&](uint32_t c) {
+    const int32_t pos = static_cast<int32_t>(c) * kStep + 16 * wave;
+    return c < c1 && pos < positions ? ScalarLoad(table + (pos >> view.page_shift)) : 0;
+  };
+  const auto load = [&](Loaded& to, uint32_t c, int32_t page) {
+    const int32_t pos = static_cast<int32_t>(c) * kStep + 16 * wave;
+    to.got = c < c1 && pos < positions;
+    to.bad = 0;
+    if (!to.got) return;
+    const bool fine = static_cast<uint32_t>(page) < static_cast<uint32_t>(view.n_pages);
+    to.bad = fine ? 0 : 1;
+    const int64_t at = ((static_cast<int64_t>(fine ? page : 0) * view.n_kv + kh) << view.page_shift) +
+                       (pos & ((1 << view.page_shift) - 1));
+    const uint4* k = reinterpret_cast<const uint4*>(static_cast<const char*>(view.k) + at * kSource) + lane;
+    const uint4* v = reinterpret_cast<const uint4*>(static_cast<const char*>(view.v) + at * kSource) + lane;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      to.k[i] = k[64 * i];
+      to.v[i] = v[64 * i];
+    }
+    if constexpr (kQ8) {
+      if (lane < 32) to.scale = (lane < 16 ? view.k_scale : view.v_scale)[at + (lane & 15)];
+    }
+  };
+  const auto store = [&](Loaded& from, Stage<D, kQ8>& st) {
+    if (!from.got) {  // positions behind the last: weights of 0 times values of 0
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) from.k[i] = from.v[i] = make_uint4(0u, 0u, 0u, 0u);
+      from.scale = 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int r = (64 * i + lane) / kSourcePieces, p = (64 * i + lane) % kSourcePieces;
+      char* const k = st.k + (16 * wave + r) * kRow;
+      char* const v = st.v + (16 * wave + r) * kRow;
+      if constexpr (!kQ8) {
+        *reinterpret_cast<uint4*>(k + 16 * (p ^ k_swap(r))) = from.k[i];
+        *reinterpret_cast<uint4*>(v + 16 * (p ^ v_swap(r))) = from.v[i];
+      } else {
+        const uint32_t kw[4] = {from.k[i].x, from.k[i].y, from.k[i].z, from.k[i].w};
+        const uint32_t vw[4] = {from.v[i].x, from.v[i].y, from.v[i].z, from.v[i].w};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint2 a = CodesToHalves(kw[2 * h]), b = CodesToHalves(kw[2 * h + 1]);
+          *reinterpret_cast<uint4*>(k + 16 * ((2 * p + h) ^ k_swap(r))) = make_uint4(a.x, a.y, b.x, b.y);
+          const uint2 c = CodesToHalves(vw[2 * h]), d = CodesToHalves(vw[2 * h + 1]);
+          *reinterpret_cast<uint4*>(v + 16 * ((2 * p + h) ^ v_swap(r))) = make_uint4(c.x, c.y, d.x, d.y);
+        }
+      }
+    }
+    if constexpr (kQ8) {
+      if (lane < 32) (lane < 16 ? st.k_scale : st.v_scale)[16 * wave + (lane & 15)] = from.scale;
+    }
+    if (lane == 0) st.bad[wave] = from.bad;
+  };
+  int32_t next_page;
+  {
+    int32_t pages[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) pages[i] = page_of(c0 + i);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) load(loaded[i], c0 + i, pages[i]);
+    next_page = page_of(c0 + kAhead);
+  }
+
+  // ---- this wave's columns and part of the keys, while the first keys are on their way
+  const int col_waves = piece.cols > 2 * kWaveCols ? 4 : piece.cols > kWaveCols ? 2 : 1;
+  const int key_waves = col_waves == 4 ? 2 : 4;
+  const int col_wave = wave % col_waves, key_wave = wave / col_waves;
+  const bool works = key_wave < key_waves && col_wave * kWaveCols < piece.cols;
+  float to_score[kT], m[kT], l[kT];
+  float down[kT];  // 8-bit values: the power of two that acc holds them multiplied by
+  F32x4 acc[kT][kE];
+  Half8 q_hi[kT][kSteps], q_lo[kT][kSteps];
+  int64_t row_head[kT];
+  bool there[kT];
+  {
+    float4 raw[kT][kSteps][2];
+#pragma unroll
+    for (int t = 0; t < kT; ++t) {
+      const int32_t in_tile = col_wave * kWaveCols + 16 * t + n;
+      const int32_t col = piece.tile * kCols + in_tile;
+      const bool a_column = works && in_tile < piece.cols;
+      const int32_t in_group = a_column ? col / args.group : 0, row = piece.first_row + in_group;
+      row_head[t] = static_cast<int64_t>(row) * args.n_heads + kh * args.group + (a_column ? col - in_group * args.group : 0);
+      const float* qr = args.q + row_head[t] * D;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        raw[t][s][0] = dev::Load4(qr + (4 * s + g) * 8);
+        raw[t][s][1] = dev::Load4(qr + (4 * s + g) * 8 + 4);
+      }
+      int32_t seq;
+      there[t] = TakesPart(args, groups, row, piece.of, piece.pages, a_column, &seq);
+      if (key_wave == 0 && g == 0 && works) sh.takes[in_tile] = there[t] ? 1 : 0;
+    }
+#pragma unroll
+    for (int t = 0; t < kT; ++t) {
+      float x[kSteps][8];
+      float top = 0.0f;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float e[4] = {raw[t][s][i].x, raw[t][s][i].y, raw[t][s][i].z, raw[t][s][i].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            x[s][4 * i + k] = there[t] ? e[k] : 0.0f;
+            top = fmaxf(top, fabsf(x[s][4 * i + k]));
+          }
+        }
+      }
+      top = MaxAcrossRows(top);
+      const int e = min(max(268 - (__float_as_int(top) >> 23), 1), 254);  // brings top to [2^14, 2^15)
+      const float up = __int_as_float(e << 23);
+      to_score[t] = ldexpf(args.scale_log2, 127 - e);
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        Terms w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = TermsOf(x[s][2 * i] * up, x[s][2 * i + 1] * up);
+        q_hi[t][s] = AsHalf8(w[0].hi, w[1].hi, w[2].hi, w[3].hi);
+        q_lo[t][s] = AsHalf8(w[0].lo, w[1].lo, w[2].lo, w[3].lo);
+      }
+#pragma unroll
+      for (int i = 0; i < kE; ++i) acc[t][i] = F32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      m[t] = -INFINITY;
+      l[t] = 0.0f;
+      down[t] = 0x1p126f;
+    }
+  }
+
+  // ---- two tiles of 16 keys, from tile `from` of a step, against kT tiles of 16 columns
+  const uint32_t k_at = static_cast<uint32_t>(n * kRow + 16 * (g ^ k_swap(n)));
+  const uint32_t v_at = static_cast<uint32_t>((4 * g + (n >> 2)) * kRow + 16 * (((n & 3) >> 1) ^ v_swap(n >> 2)) + 8 * (n & 1));
+  const auto attend = [&](const Stage<D, kQ8>& st, uint32_t c, int from) {
+    const int valid = min(kTiles, (positions - static_cast<int32_t>(c) * kStep) / 16) - from;
+    if (valid <= 0) return;
+    F32x4 s[kT][2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int t = 0; t < kT; ++t) s[t][j] = F32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        const Half8 a = *reinterpret_cast<const Half8*>(st.k + (from + j) * 16 * kRow + (k_at ^ (64u * i)));
+#pragma unroll
+        for (int t = 0; t < kT; ++t) {
+          s[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q_hi[t][i], s[t][j], 0, 0, 0);
+          s[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q_lo[t][i], s[t][j], 0, 0, 0);
+        }
+      }
+    }
+    const uint32_t bad = Scalar(st.bad[from] | st.bad[from + 1] << 1);
+    float4 vs[2];
+    if constexpr (kQ8) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float4 ks = *reinterpret_cast<const float4*>(st.k_scale + 16 * (from + j) + 4 * g);
+        vs[j] = *reinterpret_cast<const float4*>(st.v_scale + 16 * (from + j) + 4 * g);
+        const float by[4] = {ks.x, ks.y, ks.z, ks.w};
+#pragma unroll
+        for (int t = 0; t < kT; ++t) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[t][j][i] *= by[i];
+        }
+      }
+    }
+    if (__builtin_expect(valid < 2 || bad != 0, 0)) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int t = 0; t < kT; ++t) {
+          if (bad >> j & 1) s[t][j] = F32x4{NAN, NAN, NAN, NAN};
+          if (j >= valid) s[t][j] = F32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        }
+      }
+    }
+    // Weights are relative to a maximum that moves only where a score exceeds it by 4 (a factor of 16). Over fp16 values
+    // they come multiplied by 2^11: with the 16, fp16's largest, and what its low end loses is below 2^-35.
+    constexpr float kUp = kQ8 ? 0.0f : 11.0f;
+    uint32_t w[kT][2][4];
+#pragma unroll
+    for (int t = 0; t < kT; ++t) {
+      float top = s[t][0][0];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, s[t][j][i]);
+      }
+      top = MaxAcrossRows(top) * to_score[t];
+      if (__any(top > m[t] + 4.0f)) {
+        const float to = top > m[t] + 4.0f ? top : m[t];
+        const float back = __builtin_amdgcn_exp2f(m[t] - (to == -INFINITY ? 0.0f : to));
+        m[t] = to;
+        l[t] *= back;
+#pragma unroll
+        for (int i = 0; i < kE; ++i) acc[t][i] *= back;
+      }
+      const float less = m[t] == -INFINITY ? 0.0f : m[t] - kUp;
+      float p[2][4];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          p[j][i] = __builtin_amdgcn_exp2f(fmaf(s[t][j][i], to_score[t], -less));
+          l[t] += p[j][i];
+        }
+      }
+      if constexpr (kQ8) {
+        // weights times scales, brought to fp16's range by a power of two that moves only where they pass it
+        float big = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float by[4] = {vs[j].x, vs[j].y, vs[j].z, vs[j].w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            p[j][i] *= by[i];
+            big = fmaxf(big, fabsf(p[j][i]));
+          }
+        }
+        big = MaxAcrossRows(big);
+        if (__any(big * down[t] > 0x1p15f)) {
+          const bool passes = big * down[t] > 0x1p15f;
+          const int e = static_cast<int>(__float_as_uint(big) >> 23);  // brings big to [2^12, 2^13)
+          const float to = __uint_as_float(static_cast<uint32_t>(max(266 - e, 1)) << 23);
+          const float back = passes ? to / down[t] : 1.0f;
+          down[t] = passes ? to : down[t];
+#pragma unroll
+          for (int i = 0; i < kE; ++i) acc[t][i] *= back;
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) p[j][i] *= down[t];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const Terms a = TermsOf(p[j][0], p[j][1]), b = TermsOf(p[j][2], p[j][3]);
+        w[t][0][2 * j] = a.hi;
+        w[t][0][2 * j + 1] = b.hi;
+        w[t][1][2 * j] = a.lo;
+        w[t][1][2 * j + 1] = b.lo;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kE; ++i) {
+      const char* at = st.v + from * 16 * kRow + (v_at ^ (32u * i));
+      const uint2 a = ReadHalvesAcross(at), b = ReadHalvesAcross(at + 16 * kRow);
+      const Half8 v = AsHalf8(a.x, a.y, b.x, b.y);
+#pragma unroll
+      for (int t = 0; t < kT; ++t) {
+#pragma unroll
+        for (int term = 0; term < 2; ++term) {
+          const Half8 p = AsHalf8(w[t][term][0], w[t][term][1], w[t][term][2], w[t][term][3]);
+          acc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p, acc[t][i], 0, 0, 0);
+        }
+      }
+    }
+  };
+
+  // ---- the steps: one being attended to in one stage, the next on its way into the other
+  store(loaded[0], sh.stages[0]);
+  __syncthreads();
+  const int each = kTiles / key_waves;
+#pragma unroll 1
+  for (uint32_t c = c0; c < c1; c += kAhead) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (i > 0 && c + i >= c1) break;
+      const Stage<D, kQ8>& st = sh.stages[kAhead == 1 ? (c - c0) & 1 : i & 1];
+      load(loaded[i], c + i + kAhead, next_page);
+      next_page = page_of(c + i + kAhead + 1);
+      if (works) {
+#pragma unroll 1
+        for (int from = key_wave * each; from < (key_wave + 1) * each; from += 2) attend(st, c + i, from);
+      }
+      if (c + i + 1 < c1) store(loaded[(i + 1) % kAhead], sh.stages[kAhead == 1 ? (c + 1 - c0) & 1 : (i + 1) & 1]);
+      __syncthreads();
+    }
+  }
+
+  // ---- the waves' parts of a column joined, in order
+  const bool whole = c0 == 0 && c1 == piece.steps;
+  float* const joins = reinterpret_cast<float*>(sh.stages);  // [key wave - 1][column]
+  const auto join_at = [&](int from, int t) {
+    return joins + ((from - 1) * (col_waves * kWaveCols) + col_wave * kWaveCols + 16 * t + n) * kPart;
+  };
+#pragma unroll
+  for (int t = 0; t < kT; ++t) {
+    l[t] = SumAcrossRows(l[t]) * (kQ8 ? 1.0f : 0x1p-11f);
+    const float by = kQ8 ? 1.0f / down[t] : 0x1p-11f;
+#pragma unroll
+    for (int i = 0; i < kE; ++i) acc[t][i] *= by;
+  }
+  if (works && key_wave > 0) {
+#pragma unroll
+    for (int t = 0; t < kT; ++t) {
+      float* to = join_at(key_wave, t);
+#pragma unroll
+      for (int i = 0; i < kE; ++i) *reinterpret_cast<F32x4*>(to + 16 * i + 4 * g) = acc[t][i];
+      if (g == 0) {
+        to[D] = m[t];
+        to[D + 1] = l[t];
+      }
+    }
+  }
+  __syncthreads();
+  char* const slots = args.workspace + kGroups * kCounterBytes;
+  const __amdgpu_buffer_rsrc_t rs = dev::OutResource(slots, 2 * kGroups * SlotBytes(D));
+  const uint32_t my_slot = (2 * me + (piece.leads ? 0 : 1)) * SlotBytes(D);
+  if (works && key_wave == 0) {
+#pragma unroll
+    for (int t = 0; t < kT; ++t) {
+      Own own{};
+      float4 own_o[kE];
+      if (whole && there[t]) {  // requested before the join
+        own = OwnOf(args, row_head[t]);
+#pragma unroll
+        for (int i = 0; i < kE; ++i) own_o[i] = dev::Load4(args.out + row_head[t] * D + 16 * i + 4 * g);
+      }
+#pragma unroll 1
+      for (int k = 1; k < key_waves; ++k) {
+        const float* from = join_at(k, t);
+        const float m2 = from[D], l2 = from[D + 1];
+        const float to = fmaxf(m[t], m2);
+        const float safe = to == -INFINITY ? 0.0f : to;
+        const float f = __builtin_amdgcn_exp2f(m[t] - safe), f2 = __builtin_amdgcn_exp2f(m2 - safe);
+        m[t] = to;
+        l[t] = fmaf(l2, f2, l[t] * f);
+#pragma unroll
+        for (int i = 0; i < kE; ++i) {
+          const F32x4 x = *reinterpret_cast<const F32x4*>(from + 16 * i + 4 * g);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[t][i][r] = fmaf(x[r], f2, acc[t][i][r] * f);
+        }
+      }
+      if (!there[t]) continue;
+      if (whole) {
+        const Both both(own, m[t], l[t]);
+#pragma unroll
+        for (int i = 0; i < kE; ++i) {
+          dev::Store4(args.out + row_head[t] * D + 16 * i + 4 * g,
+                      both.Of(own_o[i], make_float4(acc[t][i][0], acc[t][i][1], acc[t][i][2], acc[t][i][3])));
+        }
+      } else {
+        const int32_t in_tile = col_wave * kWaveCols + 16 * t + n;
+#pragma unroll
+        for (int i = 0; i < kE; ++i) {
+          dev::StoreBuf4<kPartPolicy>(rs, my_slot + 4u * (in_tile * D + 16 * i + 4 * g),
+                                      make_float4(acc[t][i][0], acc[t][i][1], acc[t][i][2], acc[t][i][3]));
+        }
+        if (g == 0) {
+          dev::StoreBufU2<kPartPolicy>(rs, my_slot + 4u * kCols * D + 8u * in_tile,
+                                       make_uint2(__float_as_uint(m[t]), __float_as_uint(l[t])));
+        }
+      }
+    }
+  }
+  if (whole) {
+    __syncthreads();  // before the next piece's keys
+    return;
+  }
+
+  // ---- the tile's parts, by the last workgroup to arrive: what the others stored at device scope, acknowledged before
+  // they counted, it reads past its own caches
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  const uint32_t wa = share.Holder(piece.first_unit);
+  const uint32_t parts = share.Holder(piece.first_unit + piece.steps - 1) - wa + 1;
+  if (threadIdx.x == 0) sh.flag = Count(args.workspace, wa * (kCounterBytes / 4), parts);
+  __syncthreads();
+  if (__builtin_amdgcn_readfirstlane(sh.flag)) {
+    const uint32_t first_slot = 2 * wa + (share.Begin(wa) == piece.first_unit ? 0 : 1);
+    const auto slot_of = [&](uint32_t p) { return (p == 0 ? first_slot : 2 * (wa + p)) * SlotBytes(D); };
+    constexpr int kBatch = 4;
+#pragma unroll 1
+    for (int32_t i = threadIdx.x; i < piece.cols * (D / 4); i += kThreads) {
+      const int32_t in_tile = i / (D / 4), d = 4 * (i % (D / 4));
+      if (!sh.takes[in_tile]) continue;
+      const int32_t col = piece.tile * kCols + in_tile, in_group = col / args.group;
+      const int64_t at = static_cast<int64_t>(piece.first_row + in_group) * args.n_heads + kh * args.group +
+                         (col - in_group * args.group);
+      const Own own = OwnOf(args, at);
+      const float4 own_o = dev::Load4(args.out + at * D + d);
+      float top = -INFINITY, sum = 0.0f;
+      float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+      for (uint32_t p = 0; p < parts; p += kBatch) {
+        uint2 ml[kBatch];
+        float4 x[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          if (p + k < parts) {
+            const uint32_t from = slot_of(p + k);
+            ml[k] = dev::LoadBufU2<dev::kLoadDevicePolicy>(rs, from + 4u * kCols * D + 8u * in_tile);
+            x[k] = dev::LoadBuf4<dev::kLoadDevicePolicy>(rs, from + 4u * (in_tile * D + d));
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          if (p + k < parts) {
+            const float m2 = __uint_as_float(ml[k].x), to = fmaxf(top, m2);
+            const float safe = to == -INFINITY ? 0.0f : to;
+            const float f = __builtin_amdgcn_exp2f(top - safe), f2 = __builtin_amdgcn_exp2f(m2 - safe);
+            top = to;
+            sum = fmaf(__uint_as_float(ml[k].y), f2, sum * f);
+            o = make_float4(fmaf(x[k].x, f2, o.x * f), fmaf(x[k].y, f2, o.y * f), fmaf(x[k].z, f2, o.z * f),
+                            fmaf(x[k].w, f2, o.w * f));
+          }
+        }
+      }
+      dev::Store4(args.out + at * D + d, Both(own, top, sum).Of(own_o, o));
+    }
+  }
+  __syncthreads();  // before the next piece's keys, columns and flag
+}
+
+template <int D, bool kQ8>
+__global__ __launch_bounds__(kThreads, 2) void SharedPrefixKernel(const PrefixArgs args) {
+  __shared__ PrefixShared<D, kQ8> sh;
+  const PagedView& view = args.view;
+  const int lane = threadIdx.x & 63;
 
   // the groups' units, a group to a lane, and this workgroup's share
   const dev::SharedGroups groups(args.prefix.group_rows, args.prefix.group_pages, args.prefix.n_groups, args.n_rows,
@@ -147,444 +632,44 @@ __global__ __launch_bounds__(kThreads, 2) void SharedPrefixKernel(const PrefixAr
   const uint32_t me = sharers == kGroups ? (blockIdx.x % 8) * (kGroups / 8) + blockIdx.x / 8 : blockIdx.x;
   if (me >= sharers) return;
   const uint32_t begin = share.Begin(me), end = share.Begin(me + 1);
-
-  char* const slots = args.workspace + kGroups * kCounterBytes;
-  const __amdgpu_buffer_rsrc_t rs = dev::OutResource(slots, 2 * kGroups * SlotBytes(D));
-
-  // whether row r, the lane's, is one of group `of` and begins with all of its pages
-  const auto takes_part = [&](int32_t r, int32_t of, int32_t pages, bool there, int32_t* seq_out) {
-    const bool first = groups.OfLane(there ? r : -1) == of;
-    int32_t seq = -1, len = 0;
-    if (there) {
-      seq = args.seq_ids != nullptr ? args.seq_ids[r] : r;
-      len = args.lens[r];
-    }
-    *seq_out = seq;
-    return there && first && seq >= 0 && seq < view.n_seqs && len >= 0 && len <= args.capacity &&
-           dev::TakesPart(pages, view.page_shift, len);
-  };
-
   uint32_t u = begin;
 #pragma unroll 1
   while (u < end) {
-    // ---- the piece: steps [c0, c1) of a tile of columns of a kv head of a group
+    Piece piece;
     const int of = static_cast<int>(__builtin_popcountll(__ballot(lane_upto <= u)));
     const uint32_t before = __builtin_amdgcn_readlane(lane_upto - lane_amount, of);
-    const uint32_t steps = __builtin_amdgcn_readlane(lane_steps, of), tiles = __builtin_amdgcn_readlane(lane_tiles, of);
-    const uint32_t cols = __builtin_amdgcn_readlane(lane_cols, of);
-    const int32_t first_row = __builtin_amdgcn_readlane(groups.first, of);
-    const int32_t last_row = __builtin_amdgcn_readlane(groups.last, of);
-    const int32_t pages = __builtin_amdgcn_readlane(groups.pages, of);
-    const uint32_t pair = Scalar((u - before) / steps);
-    const uint32_t first_unit = before + pair * steps;
-    const uint32_t c0 = u - first_unit, c1 = min(steps, c0 + (end - u));
-    const int32_t kh = static_cast<int32_t>(Scalar(pair / tiles));
-    const int32_t tile = static_cast<int32_t>(pair) - kh * static_cast<int32_t>(tiles);
-    const int32_t tile_cols = min(kCols, static_cast<int32_t>(cols) - tile * kCols);
-    const uint32_t piece_at = u;
-    u += c1 - c0;
+    const uint32_t tiles = __builtin_amdgcn_readlane(lane_tiles, of), cols = __builtin_amdgcn_readlane(lane_cols, of);
+    piece.of = of;
+    piece.steps = __builtin_amdgcn_readlane(lane_steps, of);
+    piece.first_row = __builtin_amdgcn_readlane(groups.first, of);
+    piece.last_row = __builtin_amdgcn_readlane(groups.last, of);
+    piece.pages = __builtin_amdgcn_readlane(groups.pages, of);
+    piece.positions = static_cast<int32_t>(positions_of(piece.pages));
+    const uint32_t pair = Scalar((u - before) / piece.steps);
+    piece.first_unit = before + pair * piece.steps;
+    piece.c0 = u - piece.first_unit;
+    piece.c1 = min(piece.steps, piece.c0 + (end - u));
+    piece.kv_head = static_cast<int32_t>(Scalar(pair / tiles));
+    piece.tile = static_cast<int32_t>(pair) - piece.kv_head * static_cast<int32_t>(tiles);
+    piece.cols = min(kCols, static_cast<int32_t>(cols) - piece.tile * kCols);
+    piece.leads = u == begin;
+    u += piece.c1 - piece.c0;
 
     // the sequence whose table names the group's pages: the first row's that takes part
     int32_t leader = -1;
 #pragma unroll 1
-    for (int32_t r = first_row; r < last_row && leader < 0; r += 64) {
+    for (int32_t r = piece.first_row; r < piece.last_row && leader < 0; r += 64) {
       int32_t seq;
-      const uint64_t good = __ballot(takes_part(r + lane, of, pages, r + lane < last_row, &seq));
+      const uint64_t good = __ballot(TakesPart(args, groups, r + lane, of, piece.pages, r + lane < piece.last_row, &seq));
       if (good != 0) leader = __builtin_amdgcn_readlane(seq, __builtin_ctzll(good));
     }
     if (leader < 0) continue;  // the same for every workgroup that has a part of the tile
     const int32_t* table = view.pages + static_cast<int64_t>(leader) * view.max_pages;
-    const int32_t positions = static_cast<int32_t>(positions_of(pages));
-
-    // ---- this wave's columns and part of the keys
-    const int col_waves = tile_cols > 64 ? 4 : tile_cols > 32 ? 2 : 1;
-    const int key_waves = col_waves == 4 ? 2 : 4;
-    const int col_wave = wave % col_waves, key_wave = wave / col_waves;
-    const bool works = key_wave < key_waves && col_wave * kWaveCols < tile_cols;
-    float to_score[2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-    F32x4 acc[2][kE];
-    Half8 q_hi[2][kSteps], q_lo[2][kSteps];
-    int64_t row_head[2];
-    bool there[2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int32_t in_tile = col_wave * kWaveCols + 16 * t + n;
-      const int32_t col = tile * kCols + in_tile;
-      const int32_t row = first_row + col / args.group;
-      int32_t seq;
-      there[t] = takes_part(row, of, pages, works && in_tile < tile_cols, &seq);
-      row_head[t] = static_cast<int64_t>(row) * args.n_heads + kh * args.group + col % args.group;
-      if (key_wave == 0 && g == 0 && works) takes[in_tile] = there[t] ? 1 : 0;
-      const float* qr = args.q + (there[t] ? row_head[t] : 0) * D;
-      float x[kSteps][8];
-      float top = 0.0f;
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-#pragma unroll
-        for (int i = 0; i < 8; i += 4) {
-          const float4 a = dev::Load4(qr + (4 * s + g) * 8 + i);
-          const float e[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            x[s][i + k] = there[t] ? e[k] : 0.0f;
-            top = fmaxf(top, fabsf(x[s][i + k]));
-          }
-        }
-      }
-      top = MaxAcrossRows(top);
-      const int e = min(max(268 - (__float_as_int(top) >> 23), 1), 254);  // brings top to [2^14, 2^15)
-      const float up = __int_as_float(e << 23);
-      to_score[t] = ldexpf(args.scale_log2, 127 - e);
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        Terms w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = TermsOf(x[s][2 * i] * up, x[s][2 * i + 1] * up);
-        q_hi[t][s] = AsHalf8(w[0].hi, w[1].hi, w[2].hi, w[3].hi);
-        q_lo[t][s] = AsHalf8(w[0].lo, w[1].lo, w[2].lo, w[3].lo);
-      }
-#pragma unroll
-      for (int i = 0; i < kE; ++i) acc[t][i] = F32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (piece.cols > 32) {
+      AttendPiece<D, kQ8, 2>(args, groups, share, me, piece, table, sh);
+    } else {
+      AttendPiece<D, kQ8, 1>(args, groups, share, me, piece, table, sh);
     }
-
-    // ---- bringing in: this wave's 16 positions of a step, their pieces permuted as the reads below need them
-    const auto k_swap = [](int r) { return kPieces == 16 ? r & 15 : r & 7; };
-    const auto v_swap = [](int r) { return 2 * (r & 3); };
-    uint4 k_new[kLoads], v_new[kLoads];
-    float scale_new = 0.0f;  // lane i: of key i, lane 16 + i of value i
-    uint32_t bad_new = 0;
-    bool got = false;
-    const auto page_of = [&](uint32_t c) {
-      const int32_t pos = static_cast<int32_t>(c) * kStep + 16 * wave;
-      return pos < positions ? ScalarLoad(table + (pos >> view.page_shift)) : 0;
-    };
-    const auto load = [&](uint32_t c, int32_t page) {
-      const int32_t pos = static_cast<int32_t>(c) * kStep + 16 * wave;
-      got = pos < positions;
-      bad_new = 0;
-      if (!got) return;
-      const bool fine = static_cast<uint32_t>(page) < static_cast<uint32_t>(view.n_pages);
-      bad_new = fine ? 0 : 1;
-      const int64_t at = ((static_cast<int64_t>(fine ? page : 0) * view.n_kv + kh) << view.page_shift) +
-                         (pos & ((1 << view.page_shift) - 1));
-      const uint4* k = reinterpret_cast<const uint4*>(static_cast<const char*>(view.k) + at * kSource) + lane;
-      const uint4* v = reinterpret_cast<const uint4*>(static_cast<const char*>(view.v) + at * kSource) + lane;
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        k_new[i] = k[64 * i];
-        v_new[i] = v[64 * i];
-      }
-      if constexpr (kQ8) {
-        if (lane < 32) scale_new = (lane < 16 ? view.k_scale : view.v_scale)[at + (lane & 15)];
-      }
-    };
-    const auto store = [&](Stage& st) {
-      if (!got) {  // positions behind the last: weights of 0 times values of 0
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) k_new[i] = v_new[i] = make_uint4(0u, 0u, 0u, 0u);
-        scale_new = 0.0f;
-      }
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const int r = (64 * i + lane) / kSourcePieces, p = (64 * i + lane) % kSourcePieces;
-        char* const k = st.k + (16 * wave + r) * kRow;
-        char* const v = st.v + (16 * wave + r) * kRow;
-        if constexpr (!kQ8) {
-          *reinterpret_cast<uint4*>(k + 16 * (p ^ k_swap(r))) = k_new[i];
-          *reinterpret_cast<uint4*>(v + 16 * (p ^ v_swap(r))) = v_new[i];
-        } else {
-          const uint32_t kw[4] = {k_new[i].x, k_new[i].y, k_new[i].z, k_new[i].w};
-          const uint32_t vw[4] = {v_new[i].x, v_new[i].y, v_new[i].z, v_new[i].w};
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint2 a = CodesToHalves(kw[2 * h]), b = CodesToHalves(kw[2 * h + 1]);
-            *reinterpret_cast<uint4*>(k + 16 * ((2 * p + h) ^ k_swap(r))) = make_uint4(a.x, a.y, b.x, b.y);
-            const uint2 c = CodesToBf16(vw[2 * h]), d = CodesToBf16(vw[2 * h + 1]);
-            *reinterpret_cast<uint4*>(v + 16 * ((2 * p + h) ^ v_swap(r))) = make_uint4(c.x, c.y, d.x, d.y);
-          }
-        }
-      }
-      if constexpr (kQ8) {
-        if (lane < 32) (lane < 16 ? st.k_scale : st.v_scale)[16 * wave + (lane & 15)] = scale_new;
-      }
-      if (lane == 0) st.bad[wave] = bad_new;
-    };
-
-    // ---- two tiles of 16 keys, from tile `from` of a step, against kT tiles of 16 columns
-    const uint32_t k_at = static_cast<uint32_t>(n * kRow + 16 * (g ^ k_swap(n)));
-    const uint32_t v_at = static_cast<uint32_t>((4 * g + (n >> 2)) * kRow + 16 * (((n & 3) >> 1) ^ v_swap(n >> 2)) + 8 * (n & 1));
-    const auto attend = [&](const Stage& st, uint32_t c, int from, auto tiles_of_cols) {
-      constexpr int kN = 2, kT = decltype(tiles_of_cols)::value;
-      const int valid = min(kTiles, (positions - static_cast<int32_t>(c) * kStep) / 16) - from;
-      if (valid <= 0) return;
-      F32x4 s[kT][kN];
-#pragma unroll
-      for (int j = 0; j < kN; ++j) {
-#pragma unroll
-        for (int t = 0; t < kT; ++t) s[t][j] = F32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-          const Half8 a = *reinterpret_cast<const Half8*>(st.k + (from + j) * 16 * kRow + (k_at ^ (64u * i)));
-#pragma unroll
-          for (int t = 0; t < kT; ++t) {
-            s[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q_hi[t][i], s[t][j], 0, 0, 0);
-            s[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q_lo[t][i], s[t][j], 0, 0, 0);
-          }
-        }
-      }
-      uint32_t bad = 0;
-#pragma unroll
-      for (int j = 0; j < kN; ++j) bad |= st.bad[from + j] << j;
-      bad = Scalar(bad);
-      float4 vs[kN];
-#pragma unroll
-      for (int j = 0; j < kN; ++j) {
-        float4 ks = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
-        if constexpr (kQ8) {
-          ks = *reinterpret_cast<const float4*>(st.k_scale + 16 * (from + j) + 4 * g);
-          vs[j] = *reinterpret_cast<const float4*>(st.v_scale + 16 * (from + j) + 4 * g);
-        }
-        const float by[4] = {ks.x, ks.y, ks.z, ks.w};
-#pragma unroll
-        for (int t = 0; t < kT; ++t) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[t][j][i] = kQ8 ? s[t][j][i] * to_score[t] * by[i] : s[t][j][i] * to_score[t];
-        }
-      }
-      if (__builtin_expect(valid < kN || bad != 0, 0)) {
-#pragma unroll
-        for (int j = 0; j < kN; ++j) {
-#pragma unroll
-          for (int t = 0; t < kT; ++t) {
-            if (bad >> j & 1) s[t][j] = F32x4{NAN, NAN, NAN, NAN};
-            if (j >= valid) s[t][j] = F32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          }
-        }
-      }
-      // Weights are relative to a maximum that moves only where a score exceeds it by 4 (a factor of 16).
-      float safe[kT];
-#pragma unroll
-      for (int t = 0; t < kT; ++t) {
-        float top = s[t][0][0];
-#pragma unroll
-        for (int j = 0; j < kN; ++j) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) top = fmaxf(top, s[t][j][i]);
-        }
-        top = MaxAcrossRows(top);
-        if (__any(top > m[t] + 4.0f)) {
-          const float to = top > m[t] + 4.0f ? top : m[t];
-          const float back = __builtin_amdgcn_exp2f(m[t] - (to == -INFINITY ? 0.0f : to));
-          m[t] = to;
-          l[t] *= back;
-#pragma unroll
-          for (int i = 0; i < kE; ++i) acc[t][i] *= back;
-        }
-        safe[t] = m[t] == -INFINITY ? 0.0f : m[t];
-      }
-      uint32_t w[kT][kQ8 ? 3 : 2][4];
-#pragma unroll
-      for (int t = 0; t < kT; ++t) {
-#pragma unroll
-        for (int j = 0; j < kN; ++j) {
-          float p[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            p[i] = __builtin_amdgcn_exp2f(s[t][j][i] - safe[t]);
-            l[t] += p[i];
-          }
-          if constexpr (kQ8) {
-            const float by[4] = {vs[j].x, vs[j].y, vs[j].z, vs[j].w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) p[i] *= by[i];
-#pragma unroll
-            for (int term = 0; term < 3; ++term) {
-              w[t][term][2 * j] = Uppers(p[0], p[1]);
-              w[t][term][2 * j + 1] = Uppers(p[2], p[3]);
-              if (term < 2) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) p[i] -= Upper(p[i]);
-              }
-            }
-          } else {
-            // weights of up to 2^4 times 2^11: what fp16's low end loses is below 2^-35
-            const Terms a = TermsOf(p[0] * 0x1p11f, p[1] * 0x1p11f), b = TermsOf(p[2] * 0x1p11f, p[3] * 0x1p11f);
-            w[t][0][2 * j] = a.hi;
-            w[t][0][2 * j + 1] = b.hi;
-            w[t][1][2 * j] = a.lo;
-            w[t][1][2 * j + 1] = b.lo;
-          }
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < kE; ++i) {
-        const char* at = st.v + from * 16 * kRow + (v_at ^ (32u * i));
-        const uint2 a = ReadHalvesAcross(at), b = ReadHalvesAcross(at + 16 * kRow);
-        const Half8 v = AsHalf8(a.x, a.y, b.x, b.y);
-#pragma unroll
-        for (int t = 0; t < kT; ++t) {
-#pragma unroll
-          for (int term = 0; term < (kQ8 ? 3 : 2); ++term) {
-            const Half8 p = AsHalf8(w[t][term][0], w[t][term][1], w[t][term][2], w[t][term][3]);
-            if constexpr (kQ8) {
-              acc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(BHalf8, v),
-                                                                  __builtin_bit_cast(BHalf8, p), acc[t][i], 0, 0, 0);
-            } else {
-              acc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p, acc[t][i], 0, 0, 0);
-            }
-          }
-        }
-      }
-    };
-
-    // ---- the steps
-    load(c0, page_of(c0));
-    int32_t next_page = page_of(min(c0 + 1, c1 - 1));
-    store(stages[0]);
-    __syncthreads();
-#pragma unroll 1
-    for (uint32_t c = c0; c < c1; ++c) {
-      const Stage& st = stages[(c - c0) & 1];
-      const bool more = c + 1 < c1;
-      if (more) {
-        load(c + 1, next_page);
-        next_page = page_of(min(c + 2, c1 - 1));
-      }
-      if (works) {
-        const int each = kTiles / key_waves;
-#pragma unroll 1
-        for (int from = key_wave * each; from < (key_wave + 1) * each; from += 2) {
-          if (tile_cols > 16) {
-            attend(st, c, from, std::integral_constant<int, 2>{});
-          } else {
-            attend(st, c, from, std::integral_constant<int, 1>{});
-          }
-        }
-      }
-      if (more) store(stages[(c + 1 - c0) & 1]);
-      __syncthreads();
-    }
-
-    // ---- the waves' parts of a column joined, in order
-    float* const joins = reinterpret_cast<float*>(stages);  // [key wave - 1][column]
-    const auto join_at = [&](int from, int t) {
-      return joins + ((from - 1) * (col_waves * kWaveCols) + col_wave * kWaveCols + 16 * t + n) * kPart;
-    };
-#pragma unroll
-    for (int t = 0; t < 2; ++t) l[t] = SumAcrossRows(l[t]);
-    if (works && key_wave > 0) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        float* to = join_at(key_wave, t);
-#pragma unroll
-        for (int i = 0; i < kE; ++i) *reinterpret_cast<F32x4*>(to + 16 * i + 4 * g) = acc[t][i];
-        if (g == 0) {
-          to[D] = m[t];
-          to[D + 1] = l[t];
-        }
-      }
-    }
-    __syncthreads();
-    const bool whole = c0 == 0 && c1 == steps;
-    const uint32_t my_slot = (2 * me + (piece_at == begin ? 0 : 1)) * SlotBytes(D);
-    if (works && key_wave == 0) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-#pragma unroll 1
-        for (int k = 1; k < key_waves; ++k) {
-          const float* from = join_at(k, t);
-          const float m2 = from[D], l2 = from[D + 1];
-          const float to = fmaxf(m[t], m2);
-          const float safe = to == -INFINITY ? 0.0f : to;
-          const float f = __builtin_amdgcn_exp2f(m[t] - safe), f2 = __builtin_amdgcn_exp2f(m2 - safe);
-          m[t] = to;
-          l[t] = fmaf(l2, f2, l[t] * f);
-#pragma unroll
-          for (int i = 0; i < kE; ++i) {
-            const F32x4 x = *reinterpret_cast<const F32x4*>(from + 16 * i + 4 * g);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) acc[t][i][r] = fmaf(x[r], f2, acc[t][i][r] * f);
-          }
-        }
-        const int32_t in_tile = col_wave * kWaveCols + 16 * t + n;
-        constexpr float kDown = kQ8 ? 1.0f : 0x1p-11f;
-        if (there[t]) {
-          if (whole) {
-            float* to = args.prefix.o + row_head[t] * D;
-#pragma unroll
-            for (int i = 0; i < kE; ++i) *reinterpret_cast<F32x4*>(to + 16 * i + 4 * g) = acc[t][i] * kDown;
-            if (g == 0) *reinterpret_cast<float2*>(args.prefix.ml + 2 * row_head[t]) = make_float2(m[t], l[t]);
-          } else {
-#pragma unroll
-            for (int i = 0; i < kE; ++i) {
-              const F32x4 x = acc[t][i] * kDown;
-              dev::StoreBuf4<kPartPolicy>(rs, my_slot + 4u * (in_tile * D + 16 * i + 4 * g),
-                                          make_float4(x[0], x[1], x[2], x[3]));
-            }
-            if (g == 0) {
-              dev::StoreBufU2<kPartPolicy>(rs, my_slot + 4u * kCols * D + 8u * in_tile,
-                                           make_uint2(__float_as_uint(m[t]), __float_as_uint(l[t])));
-            }
-          }
-        }
-      }
-    }
-    if (whole) {
-      __syncthreads();  // before the next piece's keys
-      continue;
-    }
-
-    // ---- the tile's parts, by the last workgroup to arrive: what the others stored at device scope, acknowledged before
-    // they counted, it reads past its own caches
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    const uint32_t wa = share.Holder(first_unit);
-    const uint32_t parts = share.Holder(first_unit + steps - 1) - wa + 1;
-    if (threadIdx.x == 0) flag = Count(args.workspace, wa * (kCounterBytes / 4), parts);
-    __syncthreads();
-    if (__builtin_amdgcn_readfirstlane(flag)) {
-      const uint32_t first_slot = 2 * wa + (share.Begin(wa) == first_unit ? 0 : 1);
-      const auto slot_of = [&](uint32_t p) { return (p == 0 ? first_slot : 2 * (wa + p)) * SlotBytes(D); };
-      constexpr int kBatch = 4;
-#pragma unroll 1
-      for (int32_t i = threadIdx.x; i < tile_cols * (D / 4); i += kThreads) {
-        const int32_t in_tile = i / (D / 4), d = 4 * (i % (D / 4));
-        if (!takes[in_tile]) continue;
-        float top = -INFINITY, sum = 0.0f;
-        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 1
-        for (uint32_t p = 0; p < parts; p += kBatch) {
-          uint2 ml[kBatch];
-          float4 x[kBatch];
-#pragma unroll
-          for (int k = 0; k < kBatch; ++k) {
-            if (p + k < parts) {
-              const uint32_t at = slot_of(p + k);
-              ml[k] = dev::LoadBufU2<dev::kLoadDevicePolicy>(rs, at + 4u * kCols * D + 8u * in_tile);
-              x[k] = dev::LoadBuf4<dev::kLoadDevicePolicy>(rs, at + 4u * (in_tile * D + d));
-            }
-          }
-#pragma unroll
-          for (int k = 0; k < kBatch; ++k) {
-            if (p + k < parts) {
-              const float m2 = __uint_as_float(ml[k].x), to = fmaxf(top, m2);
-              const float safe = to == -INFINITY ? 0.0f : to;
-              const float f = __builtin_amdgcn_exp2f(top - safe), f2 = __builtin_amdgcn_exp2f(m2 - safe);
-              top = to;
-              sum = fmaf(__uint_as_float(ml[k].y), f2, sum * f);
-              o = make_float4(fmaf(x[k].x, f2, o.x * f), fmaf(x[k].y, f2, o.y * f), fmaf(x[k].z, f2, o.z * f),
-                              fmaf(x[k].w, f2, o.w * f));
-            }
-          }
-        }
-        const int32_t col = tile * kCols + in_tile;
-        const int64_t at = static_cast<int64_t>(first_row + col / args.group) * args.n_heads + kh * args.group +
-                           col % args.group;
-        dev::Store4(args.prefix.o + at * D + d, o);
-        if (d == 0) *reinterpret_cast<float2*>(args.prefix.ml + 2 * at) = make_float2(top, sum);
-      }
-    }
-    __syncthreads();  // before the next piece's keys, columns and flag
   }
 }
 
@@ -592,31 +677,36 @@ size_t MlBytes(int32_t n_heads, int64_t n_rows) {
   return (static_cast<size_t>(n_rows) * n_heads * 8 + 255) / 256 * 256;
 }
 size_t PrefixBytes(int32_t n_heads, int32_t head_dim, int64_t n_rows) {
-  return kGroups * (kCounterBytes + 2 * static_cast<size_t>(SlotBytes(head_dim))) + MlBytes(n_heads, n_rows) +
-         static_cast<size_t>(n_rows) * n_heads * 4 * head_dim;
+  return kGroups * (kCounterBytes + 2 * static_cast<size_t>(SlotBytes(head_dim))) + MlBytes(n_heads, n_rows);
 }
 
 }  // namespace
 
-void AttendPrefix(const GpuPagedKv& kv, const GpuPageTable& table, const int32_t* seq_ids, const int32_t* lens,
-                  const float* q_dev, int32_t n_heads, int64_t n_rows, char* workspace, PagedPrefix* prefix) {
-  const int32_t capacity = static_cast<int32_t>(std::min<int64_t>(table.max_pages * kv.page_size, 0x7FFFFFFF));
+void CheckPrefix(const GpuPagedKv& kv, const GpuPageTable& table, int32_t n_heads, int64_t n_rows, char* workspace,
+                 PagedPrefix* prefix) {
+  const int64_t capacity = std::min<int64_t>(table.max_pages * kv.page_size, 0x7FFFFFFF);
   const int64_t group = n_heads / kv.n_kv_heads;
   const int64_t most = ((n_rows * group + kCols - 1) / kCols) * kv.n_kv_heads * (capacity / kStep + 1);
   RPG_CHECK(n_rows * group <= 0x7FFFFFFF && most <= 0x7FFFFFFF / std::max(prefix->n_groups, 1),
-            "AttentionPagedShared: %d groups of %lld rows of up to %d positions are too many for one call",
-            prefix->n_groups, static_cast<long long>(n_rows), capacity);
-  // counters, slots, (m, l), o
-  char* const ml = workspace + kGroups * (kCounterBytes + 2 * static_cast<size_t>(SlotBytes(kv.head_dim)));
-  prefix->ml = reinterpret_cast<float*>(ml);
-  prefix->o = reinterpret_cast<float*>(ml + MlBytes(n_heads, n_rows));
+            "AttentionPagedShared: %d groups of %lld rows of up to %lld positions are too many for one call",
+            prefix->n_groups, static_cast<long long>(n_rows), static_cast<long long>(capacity));
+  // counters, slots, (m, l)
+  prefix->workspace = workspace;
+  prefix->ml = reinterpret_cast<float*>(workspace +
+                                        kGroups * (kCounterBytes + 2 * static_cast<size_t>(SlotBytes(kv.head_dim))));
+}
+
+void AttendPrefix(const GpuPagedKv& kv, const GpuPageTable& table, const int32_t* seq_ids, const int32_t* lens,
+                  const float* q_dev, int32_t n_heads, int64_t n_rows, float* out_dev, const PagedPrefix& prefix) {
   const float scale_log2 = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(kv.head_dim)));
   const bool q8 = kv.type == kKvQ8;
   auto* kern = kv.head_dim == 128 ? (q8 ? SharedPrefixKernel<128, true> : SharedPrefixKernel<128, false>)
                                   : (q8 ? SharedPrefixKernel<64, true> : SharedPrefixKernel<64, false>);
   Launch("SharedPrefixKernel", kern, dim3(kGroups), dim3(kThreads),
-         PrefixArgs{dev::ViewOf(kv, table), *prefix, seq_ids, lens, q_dev, workspace, static_cast<int32_t>(n_rows),
-                    capacity, n_heads, static_cast<int32_t>(group), scale_log2});
+         PrefixArgs{dev::ViewOf(kv, table), prefix, seq_ids, lens, q_dev, out_dev, prefix.workspace,
+                    static_cast<int32_t>(n_rows),
+                    static_cast<int32_t>(std::min<int64_t>(table.max_pages * kv.page_size, 0x7FFFFFFF)), n_heads,
+                    n_heads / kv.n_kv_heads, scale_log2});
 }
 
 size_t GpuAttentionPagedSharedWorkspaceBytes(int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, int64_t n_rows) {

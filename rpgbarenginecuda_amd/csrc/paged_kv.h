@@ -20,25 +20,28 @@ inline bool Overlap(const void* a, int64_t na, const void* b, int64_t nb) {
   return x < y + static_cast<uint64_t>(nb) && y < x + static_cast<uint64_t>(na);
 }
 
-// What the shared positions of a call's groups came to (k_attention_prefix.hip), for the rows' own attention to join:
-// for row r and head h, relative to the maximum m of its scores (as powers of two), o[r][h] = sum 2^(s - m) v and
-// ml[r][h] = (m, sum 2^(s - m)).
+// Attention of a batch whose rows share their beginnings: AttendPaged, given one of these, attends to what is each
+// row's own and leaves for row r and head h, besides the output, ml[r][h] = (m, l), the maximum of its scores (as powers
+// of two) and the sum of weights that the output is divided by; AttendPrefix (k_attention_prefix.hip) then attends to the
+// shared positions and joins both in the output.
 struct PagedPrefix {
   const int32_t* group_rows;
   const int32_t* group_pages;
   int32_t n_groups;
-  float* o = nullptr;
+  char* workspace = nullptr;
   float* ml = nullptr;
 };
 
-// GpuAttentionPaged, over what is behind the shared positions if there is a prefix.
+// GpuAttentionPaged, of what is behind the shared positions if there is a prefix (and then of the rest).
 void AttendPaged(const GpuPagedKv& kv, const GpuPageTable& table, const int32_t* seq_ids, const int32_t* lens,
                  const float* q_dev, int32_t n_heads, int64_t n_rows, float* out_dev, void* workspace,
                  size_t workspace_bytes, PagedPrefix* prefix);
 
-// The shared positions' attention, into prefix->o and prefix->ml, which it places in the workspace.
+// Refuses what AttendPrefix cannot serve, and places prefix's part in the workspace.
+void CheckPrefix(const GpuPagedKv& kv, const GpuPageTable& table, int32_t n_heads, int64_t n_rows, char* workspace,
+                 PagedPrefix* prefix);
 void AttendPrefix(const GpuPagedKv& kv, const GpuPageTable& table, const int32_t* seq_ids, const int32_t* lens,
-                  const float* q_dev, int32_t n_heads, int64_t n_rows, char* workspace, PagedPrefix* prefix);
+                  const float* q_dev, int32_t n_heads, int64_t n_rows, float* out_dev, const PagedPrefix& prefix);
 
 namespace dev {
 

@@ -290,6 +290,25 @@ def test_keys_of_minus_infinite_score(gpu):
         assert np.all(got[r, 0] == v[best, 0].astype(np.float32))
 
 
+def test_own_keys_of_minus_infinite_score(gpu):
+    """Of every own position: what is shared is attended to alone; with no weight in either, NaN."""
+    rng = np.random.default_rng(13)
+    d, page = 64, 16
+    pages, lens, starts, shared = batch(rng, F16, 1, d, page, [(9, [20, 0, 200])])
+    for r in (0, 2):
+        for pos in range(9 * page, lens[r]):
+            p, s = pages.slot(r, pos)
+            pages.k.view(np.float16)[p, 0, s] = 0
+            pages.k.view(np.float16)[p, 0, s, 3] = -np.inf
+    q = np.abs(rng.normal(0, 1, (3, 2, d))).astype(np.float32) + np.float32(0.01)
+    kv, table = pages.device(gpu)
+    got = attend(gpu, kv, table, lens, starts, shared, q)
+    check(got, pages, [9 * page] * 3, q)
+    pages.k[pages.table[0, :9]] = pages.k[pages.table[0, 9]][:, :1]
+    kv, table = pages.device(gpu)
+    assert np.all(np.isnan(attend(gpu, kv, table, lens, starts, shared, q)))
+
+
 @pytest.mark.parametrize("kind,d", [(F16, 128), (Q8, 64)])
 def test_captured(gpu, kind, d):
     """A captured call holds for any groups, lengths and rows at replay; eager calls between the replays agree."""
