@@ -137,6 +137,14 @@ struct PrefixShared {
   int flag;
 };
 
+// x, from which what follows is worked out where it stands: hoisted out of the loop of steps, the addresses that come of it
+// take more registers than there are, and a value that comes back from memory waits for all loads before it.
+template <class T>
+__device__ __forceinline__ T Afresh(T x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 // Whether row r, the lane's, is one of group `of` and begins with all of its pages; *seq its sequence.
 __device__ __forceinline__ bool TakesPart(const PrefixArgs& a, const dev::SharedGroups& groups, int32_t r, int32_t of,
                                           int32_t pages, bool there, int32_t* seq) {
@@ -182,8 +190,8 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
   const auto k_swap = [](int r) { return kPieces == 16 ? r & 15 : r & 7; };
   const auto v_swap = [](int r) { return 2 * (r & 3); };
   struct Loaded {
-    uint4 k[kLoads], v[kLoads];
-    float scale;  // lane i: of key i, lane 16 + i of value i
+    float4 k[kLoads], v[kLoads];
+    float k_scale, v_scale;  // of row lane % 16
     uint32_t bad;
     bool got;
   };
@@ -201,47 +209,54 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
     to.bad = fine ? 0 : 1;
     const int64_t at = ((static_cast<int64_t>(fine ? page : 0) * view.n_kv + kh) << view.page_shift) +
                        (pos & ((1 << view.page_shift) - 1));
-    const uint4* k = reinterpret_cast<const uint4*>(static_cast<const char*>(view.k) + at * kSource) + lane;
-    const uint4* v = reinterpret_cast<const uint4*>(static_cast<const char*>(view.v) + at * kSource) + lane;
+    const auto rows = [&](const void* base, int64_t bytes) {
+      return dev::OutResource(const_cast<char*>(static_cast<const char*>(base)) + at * bytes, static_cast<uint32_t>(16 * bytes));
+    };
+    const __amdgpu_buffer_rsrc_t k = rows(view.k, kSource), v = rows(view.v, kSource);
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      to.k[i] = k[64 * i];
-      to.v[i] = v[64 * i];
+      to.k[i] = dev::LoadBuf4<0>(k, 1024u * i + 16u * lane);
+      to.v[i] = dev::LoadBuf4<0>(v, 1024u * i + 16u * lane);
     }
     if constexpr (kQ8) {
-      if (lane < 32) to.scale = (lane < 16 ? view.k_scale : view.v_scale)[at + (lane & 15)];
+      to.k_scale = dev::LoadBuf1<0>(rows(view.k_scale, 4), 4u * n);
+      to.v_scale = dev::LoadBuf1<0>(rows(view.v_scale, 4), 4u * n);
     }
   };
   const auto store = [&](Loaded& from, Stage<D, kQ8>& st) {
     if (!from.got) {  // positions behind the last: weights of 0 times values of 0
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) from.k[i] = from.v[i] = make_uint4(0u, 0u, 0u, 0u);
-      from.scale = 0.0f;
+      for (int i = 0; i < kLoads; ++i) from.k[i] = from.v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      from.k_scale = from.v_scale = 0.0f;
     }
+    const int own = Afresh(lane);
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int r = (64 * i + lane) / kSourcePieces, p = (64 * i + lane) % kSourcePieces;
+      const int r = (64 * i + own) / kSourcePieces, p = (64 * i + own) % kSourcePieces;
       char* const k = st.k + (16 * wave + r) * kRow;
       char* const v = st.v + (16 * wave + r) * kRow;
       if constexpr (!kQ8) {
-        *reinterpret_cast<uint4*>(k + 16 * (p ^ k_swap(r))) = from.k[i];
-        *reinterpret_cast<uint4*>(v + 16 * (p ^ v_swap(r))) = from.v[i];
+        *reinterpret_cast<float4*>(k + 16 * (p ^ k_swap(r))) = from.k[i];
+        *reinterpret_cast<float4*>(v + 16 * (p ^ v_swap(r))) = from.v[i];
       } else {
-        const uint32_t kw[4] = {from.k[i].x, from.k[i].y, from.k[i].z, from.k[i].w};
-        const uint32_t vw[4] = {from.v[i].x, from.v[i].y, from.v[i].z, from.v[i].w};
+        const float kw[4] = {from.k[i].x, from.k[i].y, from.k[i].z, from.k[i].w};
+        const float vw[4] = {from.v[i].x, from.v[i].y, from.v[i].z, from.v[i].w};
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const uint2 a = CodesToHalves(kw[2 * h]), b = CodesToHalves(kw[2 * h + 1]);
+          const uint2 a = CodesToHalves(__float_as_uint(kw[2 * h])), b = CodesToHalves(__float_as_uint(kw[2 * h + 1]));
           *reinterpret_cast<uint4*>(k + 16 * ((2 * p + h) ^ k_swap(r))) = make_uint4(a.x, a.y, b.x, b.y);
-          const uint2 c = CodesToHalves(vw[2 * h]), d = CodesToHalves(vw[2 * h + 1]);
+          const uint2 c = CodesToHalves(__float_as_uint(vw[2 * h])), d = CodesToHalves(__float_as_uint(vw[2 * h + 1]));
           *reinterpret_cast<uint4*>(v + 16 * ((2 * p + h) ^ v_swap(r))) = make_uint4(c.x, c.y, d.x, d.y);
         }
       }
     }
     if constexpr (kQ8) {
-      if (lane < 32) (lane < 16 ? st.k_scale : st.v_scale)[16 * wave + (lane & 15)] = from.scale;
+      if (own < 16) {
+        st.k_scale[16 * wave + own] = from.k_scale;
+        st.v_scale[16 * wave + own] = from.v_scale;
+      }
     }
-    if (lane == 0) st.bad[wave] = from.bad;
+    if (own == 0) st.bad[wave] = from.bad;
   };
   int32_t next_page;
   {
@@ -320,11 +335,12 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
   }
 
   // ---- two tiles of 16 keys, from tile `from` of a step, against kT tiles of 16 columns
-  const uint32_t k_at = static_cast<uint32_t>(n * kRow + 16 * (g ^ k_swap(n)));
-  const uint32_t v_at = static_cast<uint32_t>((4 * g + (n >> 2)) * kRow + 16 * (((n & 3) >> 1) ^ v_swap(n >> 2)) + 8 * (n & 1));
+  const uint32_t k_lane = static_cast<uint32_t>(n * kRow + 16 * (g ^ k_swap(n)));
+  const uint32_t v_lane = static_cast<uint32_t>((4 * g + (n >> 2)) * kRow + 16 * (((n & 3) >> 1) ^ v_swap(n >> 2)) + 8 * (n & 1));
   const auto attend = [&](const Stage<D, kQ8>& st, uint32_t c, int from) {
     const int valid = min(kTiles, (positions - static_cast<int32_t>(c) * kStep) / 16) - from;
     if (valid <= 0) return;
+    const uint32_t k_at = Afresh(k_lane), v_at = Afresh(v_lane);
     F32x4 s[kT][2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
