@@ -149,8 +149,11 @@ struct Share {
   __device__ __forceinline__ uint32_t Begin(uint32_t w) const { return w * per + min(w, rem); }
   // The workgroup whose share holds item x.
   __device__ __forceinline__ uint32_t Holder(uint32_t x) const {
+    return Scalar(HolderOfLane(x));
+  }
+  __device__ __forceinline__ uint32_t HolderOfLane(uint32_t x) const {
     const uint32_t big = rem * (per + 1);
-    return Scalar(x < big ? x / (per + 1) : rem + (x - big) / per);
+    return x < big ? x / (per + 1) : rem + (x - big) / per;
   }
 };
 

@@ -18,8 +18,9 @@
 // tile has no more than 64 columns, or 16 columns and a quarter for no more than 32. The products are those of
 // k_attention_paged.hip: rows of S = K Q^T are 16 keys, rows of O^T = V^T P^T 16 elements, so that a lane ends the first
 // with the weights of the keys that it holds in the second. The units (kv head, column tile, step) of all groups are
-// shared out evenly and contiguously; a tile that several workgroups hold parts of is joined by the last of them to
-// arrive, in order.
+// shared out evenly and contiguously. A tile that one workgroup holds it joins with the rows' own parts by itself; the
+// parts of others are left in the workspace for a small kernel that joins them in order, over all compute units: the last
+// workgroup of a tile to arrive, on its one, took 18 us for four parts of 128 columns where that takes 4.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -43,9 +44,7 @@ constexpr int kThreads = 64 * kWaves;
 constexpr int kCols = 128;     // columns of a tile
 constexpr int kStep = 128;     // positions of a unit: 16 for each wave to bring in
 constexpr int kGroups = 256;   // workgroups: one to a compute unit
-constexpr uint32_t kLeast = 2;  // units of a workgroup, where there are few
-constexpr size_t kCounterBytes = 256;
-constexpr int kPartPolicy = 16;  // device scope, as the parts in k_attention_paged.hip
+constexpr int kJoinThreads = 64;
 
 // What a workgroup leaves of a tile that it has a part of: o [column][D], then (m, l) [column].
 __host__ __device__ constexpr uint32_t SlotBytes(int d) { return kCols * (4u * d + 8u); }
@@ -57,7 +56,7 @@ struct PrefixArgs {
   const int32_t* lens;
   const float* q;
   float* out;
-  char* workspace;  // counters, slots
+  char* workspace;  // slots: two of a workgroup, for the first tile that it has a part of and for another
   int32_t n_rows;
   int32_t capacity;  // positions that a table row has pages for, at most the largest int32
   int32_t n_heads;
@@ -130,11 +129,25 @@ struct Stage {
   uint32_t bad[kStep / 16];  // pages out of range
 };
 
-template <int D, bool kQ8>
-struct PrefixShared {
-  Stage<D, kQ8> stages[2];
-  uint8_t takes[kCols];
-  int flag;
+// The groups' units, a group to a lane: those of kv head, column tile and step count up, in this order.
+struct Units {
+  dev::SharedGroups groups;
+  uint32_t cols, tiles, steps, amount, upto;
+  uint32_t all, sharers;  // the workgroups that share them out
+
+  __device__ __forceinline__ Units(const PrefixArgs& a, int lane)
+      : groups(a.prefix.group_rows, a.prefix.group_pages, a.prefix.n_groups, a.n_rows, a.view.max_pages, lane) {
+    cols = static_cast<uint32_t>(groups.last - groups.first) * a.group;
+    tiles = (cols + kCols - 1) / kCols;
+    steps = (PositionsOf(a, groups.pages) + kStep - 1) / kStep;
+    amount = tiles * steps * a.view.n_kv;
+    upto = ScanAdd(amount);
+    all = __builtin_amdgcn_readlane(upto, 63);
+    sharers = min(static_cast<uint32_t>(kGroups), all);
+  }
+  static __device__ __forceinline__ uint32_t PositionsOf(const PrefixArgs& a, int32_t pages) {
+    return pages <= (a.capacity >> a.view.page_shift) ? static_cast<uint32_t>(pages) << a.view.page_shift : 0u;
+  }
 };
 
 // x, from which what follows is worked out where it stands: hoisted out of the loop of steps, the addresses that come of it
@@ -145,25 +158,27 @@ __device__ __forceinline__ T Afresh(T x) {
   return x;
 }
 
-// Whether row r, the lane's, is one of group `of` and begins with all of its pages; *seq its sequence.
-__device__ __forceinline__ bool TakesPart(const PrefixArgs& a, const dev::SharedGroups& groups, int32_t r, int32_t of,
-                                          int32_t pages, bool there, int32_t* seq) {
-  const bool first = groups.n == 1 ? true : groups.OfLane(there ? r : -1) == of;
+// Whether row r, the lane's and its group's, begins with all of the group's pages; *seq its sequence.
+__device__ __forceinline__ bool BeginsWith(const PrefixArgs& a, int32_t r, int32_t pages, bool there, int32_t* seq) {
   int32_t len = 0;
   *seq = -1;
   if (there) {
     *seq = a.seq_ids != nullptr ? a.seq_ids[r] : r;
     len = a.lens[r];
   }
-  return there && first && *seq >= 0 && *seq < a.view.n_seqs && len >= 0 && len <= a.capacity &&
+  return there && *seq >= 0 && *seq < a.view.n_seqs && len >= 0 && len <= a.capacity &&
          dev::TakesPart(pages, a.view.page_shift, len);
+}
+// The same of a row among those that group `of` names.
+__device__ __forceinline__ bool TakesPart(const PrefixArgs& a, const dev::SharedGroups& groups, int32_t r, int32_t of,
+                                          int32_t pages, bool there, int32_t* seq) {
+  return BeginsWith(a, r, pages, there && (groups.n == 1 || groups.OfLane(there ? r : -1) == of), seq);
 }
 
 // kT: tiles of 16 columns of a wave.
 template <int D, bool kQ8, int kT>
-__device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::SharedGroups& groups, const Share& share,
-                                            uint32_t me, const Piece& piece, const int32_t* table,
-                                            PrefixShared<D, kQ8>& sh) {
+__device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::SharedGroups& groups, uint32_t me,
+                                            const Piece& piece, const int32_t* table, Stage<D, kQ8> (&stages)[2]) {
   constexpr int kRow = 2 * D;              // bytes of a row in LDS
   constexpr int kPieces = kRow / 16;       // of 16 bytes
   constexpr int kSource = kQ8 ? D : 2 * D;  // bytes of a cached row
@@ -174,9 +189,8 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
   constexpr int kTiles = kStep / 16;
   constexpr int kPart = D + 4;             // floats of a joined column: o, m, l
   constexpr int kWaveCols = 16 * kT;
-  constexpr int kAhead = kQ8 ? 2 : 1;      // steps whose loads are under way
   static_assert(kTiles == kWaves, "a wave brings in 16 positions");
-  static_assert(kCols * kPart * 4 <= sizeof(sh.stages) && 3 * 64 * kPart * 4 <= sizeof(sh.stages), "joins fit where keys were");
+  static_assert(kCols * kPart * 4 <= sizeof(stages) && 3 * 64 * kPart * 4 <= sizeof(stages), "joins fit where keys were");
 
   const PagedView& view = args.view;
   const int lane = threadIdx.x & 63;
@@ -195,7 +209,7 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
     uint32_t bad;
     bool got;
   };
-  Loaded loaded[kAhead];
+  Loaded loaded;
   const auto page_of = [&](uint32_t c) {
     const int32_t pos = static_cast<int32_t>(c) * kStep + 16 * wave;
     return c < c1 && pos < positions ? ScalarLoad(table + (pos >> view.page_shift)) : 0;
@@ -258,17 +272,7 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
     }
     if (own == 0) st.bad[wave] = from.bad;
   };
-  int32_t next_page;
-  {
-    int32_t pages[kAhead];
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) pages[i] = page_of(c0 + i);
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) load(loaded[i], c0 + i, pages[i]);
-    next_page = page_of(c0 + kAhead);
-  }
-
-  // ---- this wave's columns and part of the keys, while the first keys are on their way
+  // ---- this wave's columns and part of the keys; its queries are requested before the first keys, which take longer
   const int col_waves = piece.cols > 2 * kWaveCols ? 4 : piece.cols > kWaveCols ? 2 : 1;
   const int key_waves = col_waves == 4 ? 2 : 4;
   const int col_wave = wave % col_waves, key_wave = wave / col_waves;
@@ -279,6 +283,7 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
   Half8 q_hi[kT][kSteps], q_lo[kT][kSteps];
   int64_t row_head[kT];
   bool there[kT];
+  int32_t next_page;
   {
     float4 raw[kT][kSteps][2];
 #pragma unroll
@@ -296,8 +301,9 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
       }
       int32_t seq;
       there[t] = TakesPart(args, groups, row, piece.of, piece.pages, a_column, &seq);
-      if (key_wave == 0 && g == 0 && works) sh.takes[in_tile] = there[t] ? 1 : 0;
     }
+    load(loaded, c0, page_of(c0));
+    next_page = page_of(c0 + 1);
 #pragma unroll
     for (int t = 0; t < kT; ++t) {
       float x[kSteps][8];
@@ -466,29 +472,24 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
   };
 
   // ---- the steps: one being attended to in one stage, the next on its way into the other
-  store(loaded[0], sh.stages[0]);
+  store(loaded, stages[0]);
   __syncthreads();
   const int each = kTiles / key_waves;
 #pragma unroll 1
-  for (uint32_t c = c0; c < c1; c += kAhead) {
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      if (i > 0 && c + i >= c1) break;
-      const Stage<D, kQ8>& st = sh.stages[kAhead == 1 ? (c - c0) & 1 : i & 1];
-      load(loaded[i], c + i + kAhead, next_page);
-      next_page = page_of(c + i + kAhead + 1);
-      if (works) {
+  for (uint32_t c = c0; c < c1; ++c) {
+    load(loaded, c + 1, next_page);
+    next_page = page_of(c + 2);
+    if (works) {
 #pragma unroll 1
-        for (int from = key_wave * each; from < (key_wave + 1) * each; from += 2) attend(st, c + i, from);
-      }
-      if (c + i + 1 < c1) store(loaded[(i + 1) % kAhead], sh.stages[kAhead == 1 ? (c + 1 - c0) & 1 : (i + 1) & 1]);
-      __syncthreads();
+      for (int from = key_wave * each; from < (key_wave + 1) * each; from += 2) attend(stages[(c - c0) & 1], c, from);
     }
+    if (c + 1 < c1) store(loaded, stages[(c + 1 - c0) & 1]);
+    __syncthreads();
   }
 
   // ---- the waves' parts of a column joined, in order
   const bool whole = c0 == 0 && c1 == piece.steps;
-  float* const joins = reinterpret_cast<float*>(sh.stages);  // [key wave - 1][column]
+  float* const joins = reinterpret_cast<float*>(stages);  // [key wave - 1][column]
   const auto join_at = [&](int from, int t) {
     return joins + ((from - 1) * (col_waves * kWaveCols) + col_wave * kWaveCols + 16 * t + n) * kPart;
   };
@@ -512,8 +513,7 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
     }
   }
   __syncthreads();
-  char* const slots = args.workspace + kGroups * kCounterBytes;
-  const __amdgpu_buffer_rsrc_t rs = dev::OutResource(slots, 2 * kGroups * SlotBytes(D));
+  const __amdgpu_buffer_rsrc_t rs = dev::OutResource(args.workspace, 2 * kGroups * SlotBytes(D));
   const uint32_t my_slot = (2 * me + (piece.leads ? 0 : 1)) * SlotBytes(D);
   if (works && key_wave == 0) {
 #pragma unroll
@@ -524,6 +524,9 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
         own = OwnOf(args, row_head[t]);
 #pragma unroll
         for (int i = 0; i < kE; ++i) own_o[i] = dev::Load4(args.out + row_head[t] * D + 16 * i + 4 * g);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kE; ++i) own_o[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       }
 #pragma unroll 1
       for (int k = 1; k < key_waves; ++k) {
@@ -553,96 +556,28 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
         const int32_t in_tile = col_wave * kWaveCols + 16 * t + n;
 #pragma unroll
         for (int i = 0; i < kE; ++i) {
-          dev::StoreBuf4<kPartPolicy>(rs, my_slot + 4u * (in_tile * D + 16 * i + 4 * g),
+          dev::StoreBuf4<0>(rs, my_slot + 4u * (in_tile * D + 16 * i + 4 * g),
                                       make_float4(acc[t][i][0], acc[t][i][1], acc[t][i][2], acc[t][i][3]));
         }
         if (g == 0) {
-          dev::StoreBufU2<kPartPolicy>(rs, my_slot + 4u * kCols * D + 8u * in_tile,
+          dev::StoreBufU2<0>(rs, my_slot + 4u * kCols * D + 8u * in_tile,
                                        make_uint2(__float_as_uint(m[t]), __float_as_uint(l[t])));
         }
       }
     }
   }
-  if (whole) {
-    __syncthreads();  // before the next piece's keys
-    return;
-  }
-
-  // ---- the tile's parts, by the last workgroup to arrive: what the others stored at device scope, acknowledged before
-  // they counted, it reads past its own caches
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  const uint32_t wa = share.Holder(piece.first_unit);
-  const uint32_t parts = share.Holder(piece.first_unit + piece.steps - 1) - wa + 1;
-  if (threadIdx.x == 0) sh.flag = Count(args.workspace, wa * (kCounterBytes / 4), parts);
-  __syncthreads();
-  if (__builtin_amdgcn_readfirstlane(sh.flag)) {
-    const uint32_t first_slot = 2 * wa + (share.Begin(wa) == piece.first_unit ? 0 : 1);
-    const auto slot_of = [&](uint32_t p) { return (p == 0 ? first_slot : 2 * (wa + p)) * SlotBytes(D); };
-    constexpr int kBatch = 4;
-#pragma unroll 1
-    for (int32_t i = threadIdx.x; i < piece.cols * (D / 4); i += kThreads) {
-      const int32_t in_tile = i / (D / 4), d = 4 * (i % (D / 4));
-      if (!sh.takes[in_tile]) continue;
-      const int32_t col = piece.tile * kCols + in_tile, in_group = col / args.group;
-      const int64_t at = static_cast<int64_t>(piece.first_row + in_group) * args.n_heads + kh * args.group +
-                         (col - in_group * args.group);
-      const Own own = OwnOf(args, at);
-      const float4 own_o = dev::Load4(args.out + at * D + d);
-      float top = -INFINITY, sum = 0.0f;
-      float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 1
-      for (uint32_t p = 0; p < parts; p += kBatch) {
-        uint2 ml[kBatch];
-        float4 x[kBatch];
-#pragma unroll
-        for (int k = 0; k < kBatch; ++k) {
-          if (p + k < parts) {
-            const uint32_t from = slot_of(p + k);
-            ml[k] = dev::LoadBufU2<dev::kLoadDevicePolicy>(rs, from + 4u * kCols * D + 8u * in_tile);
-            x[k] = dev::LoadBuf4<dev::kLoadDevicePolicy>(rs, from + 4u * (in_tile * D + d));
-          }
-        }
-#pragma unroll
-        for (int k = 0; k < kBatch; ++k) {
-          if (p + k < parts) {
-            const float m2 = __uint_as_float(ml[k].x), to = fmaxf(top, m2);
-            const float safe = to == -INFINITY ? 0.0f : to;
-            const float f = __builtin_amdgcn_exp2f(top - safe), f2 = __builtin_amdgcn_exp2f(m2 - safe);
-            top = to;
-            sum = fmaf(__uint_as_float(ml[k].y), f2, sum * f);
-            o = make_float4(fmaf(x[k].x, f2, o.x * f), fmaf(x[k].y, f2, o.y * f), fmaf(x[k].z, f2, o.z * f),
-                            fmaf(x[k].w, f2, o.w * f));
-          }
-        }
-      }
-      dev::Store4(args.out + at * D + d, Both(own, top, sum).Of(own_o, o));
-    }
-  }
-  __syncthreads();  // before the next piece's keys, columns and flag
 }
 
 template <int D, bool kQ8>
 __global__ __launch_bounds__(kThreads, 2) void SharedPrefixKernel(const PrefixArgs args) {
-  __shared__ PrefixShared<D, kQ8> sh;
+  __shared__ Stage<D, kQ8> stages[2];
   const PagedView& view = args.view;
   const int lane = threadIdx.x & 63;
 
-  // the groups' units, a group to a lane, and this workgroup's share
-  const dev::SharedGroups groups(args.prefix.group_rows, args.prefix.group_pages, args.prefix.n_groups, args.n_rows,
-                                 view.max_pages, lane);
-  const auto positions_of = [&](int32_t pages) {
-    return pages <= (args.capacity >> view.page_shift) ? static_cast<uint32_t>(pages) << view.page_shift : 0u;
-  };
-  const uint32_t lane_cols = static_cast<uint32_t>(groups.last - groups.first) * args.group;
-  const uint32_t lane_tiles = (lane_cols + kCols - 1) / kCols;
-  const uint32_t lane_steps = (positions_of(groups.pages) + kStep - 1) / kStep;
-  const uint32_t lane_amount = lane_tiles * lane_steps * view.n_kv;
-  const uint32_t lane_upto = ScanAdd(lane_amount);
-  const uint32_t all = __builtin_amdgcn_readlane(lane_upto, 63);
-  const uint32_t sharers = min(static_cast<uint32_t>(kGroups), (all + kLeast - 1) / kLeast);
+  const Units units(args, lane);
+  const uint32_t sharers = units.sharers;
   if (sharers == 0) return;
-  const Share share(all, sharers);
+  const Share share(units.all, sharers);
   // Workgroups are dealt out to the eight dies in turn: with all of them at work those of one die take neighbouring shares,
   // whose tiles read the same keys and values through its cache.
   const uint32_t me = sharers == kGroups ? (blockIdx.x % 8) * (kGroups / 8) + blockIdx.x / 8 : blockIdx.x;
@@ -652,15 +587,15 @@ __global__ __launch_bounds__(kThreads, 2) void SharedPrefixKernel(const PrefixAr
 #pragma unroll 1
   while (u < end) {
     Piece piece;
-    const int of = static_cast<int>(__builtin_popcountll(__ballot(lane_upto <= u)));
-    const uint32_t before = __builtin_amdgcn_readlane(lane_upto - lane_amount, of);
-    const uint32_t tiles = __builtin_amdgcn_readlane(lane_tiles, of), cols = __builtin_amdgcn_readlane(lane_cols, of);
+    const int of = static_cast<int>(__builtin_popcountll(__ballot(units.upto <= u)));
+    const uint32_t before = __builtin_amdgcn_readlane(units.upto - units.amount, of);
+    const uint32_t tiles = __builtin_amdgcn_readlane(units.tiles, of), cols = __builtin_amdgcn_readlane(units.cols, of);
     piece.of = of;
-    piece.steps = __builtin_amdgcn_readlane(lane_steps, of);
-    piece.first_row = __builtin_amdgcn_readlane(groups.first, of);
-    piece.last_row = __builtin_amdgcn_readlane(groups.last, of);
-    piece.pages = __builtin_amdgcn_readlane(groups.pages, of);
-    piece.positions = static_cast<int32_t>(positions_of(piece.pages));
+    piece.steps = __builtin_amdgcn_readlane(units.steps, of);
+    piece.first_row = __builtin_amdgcn_readlane(units.groups.first, of);
+    piece.last_row = __builtin_amdgcn_readlane(units.groups.last, of);
+    piece.pages = __builtin_amdgcn_readlane(units.groups.pages, of);
+    piece.positions = static_cast<int32_t>(Units::PositionsOf(args, piece.pages));
     const uint32_t pair = Scalar((u - before) / piece.steps);
     piece.first_unit = before + pair * piece.steps;
     piece.c0 = u - piece.first_unit;
@@ -676,24 +611,87 @@ __global__ __launch_bounds__(kThreads, 2) void SharedPrefixKernel(const PrefixAr
 #pragma unroll 1
     for (int32_t r = piece.first_row; r < piece.last_row && leader < 0; r += 64) {
       int32_t seq;
-      const uint64_t good = __ballot(TakesPart(args, groups, r + lane, of, piece.pages, r + lane < piece.last_row, &seq));
+      const uint64_t good = __ballot(TakesPart(args, units.groups, r + lane, of, piece.pages, r + lane < piece.last_row, &seq));
       if (good != 0) leader = __builtin_amdgcn_readlane(seq, __builtin_ctzll(good));
     }
     if (leader < 0) continue;  // the same for every workgroup that has a part of the tile
     const int32_t* table = view.pages + static_cast<int64_t>(leader) * view.max_pages;
     if (piece.cols > 32) {
-      AttendPiece<D, kQ8, 2>(args, groups, share, me, piece, table, sh);
+      AttendPiece<D, kQ8, 2>(args, units.groups, me, piece, table, stages);
     } else {
-      AttendPiece<D, kQ8, 1>(args, groups, share, me, piece, table, sh);
+      AttendPiece<D, kQ8, 1>(args, units.groups, me, piece, table, stages);
+    }
+    __syncthreads();  // before the next piece's keys
+  }
+}
+
+// The parts of tiles that several workgroups have held joined, in order, and with the rows' own part: four elements of a
+// column to a thread.
+template <int D>
+__global__ __launch_bounds__(kJoinThreads) void SharedJoinKernel(const PrefixArgs args) {
+  constexpr int kLanes = D / 4;  // of a column
+  constexpr int kBatch = 16;     // parts under way
+  const int lane = threadIdx.x & 63;
+  const int64_t row_head = static_cast<int64_t>(blockIdx.x) * (kJoinThreads / kLanes) + threadIdx.x / kLanes;
+  const int32_t d = 4 * (threadIdx.x % kLanes);
+  const int32_t row = static_cast<int32_t>(row_head / args.n_heads), head = static_cast<int32_t>(row_head % args.n_heads);
+  const bool there = row < args.n_rows;
+  const Units units(args, lane);
+  if (units.sharers == 0) return;
+  const int32_t in = units.groups.OfLane(there ? row : -1), of = max(in, 0);
+  int32_t seq;
+  const bool takes = BeginsWith(args, row, __shfl(units.groups.pages, of), there && in >= 0, &seq);
+  const uint32_t steps = __shfl(units.steps, of), tiles = __shfl(units.tiles, of);
+  const uint32_t before = __shfl(units.upto - units.amount, of);
+  const int32_t first_row = __shfl(units.groups.first, of);
+  if (!takes) return;
+
+  const int32_t kh = head / args.group, col = (row - first_row) * args.group + (head - kh * args.group);
+  const uint32_t tile = static_cast<uint32_t>(col) / kCols, in_tile = static_cast<uint32_t>(col) % kCols;
+  const uint32_t first_unit = before + (kh * tiles + tile) * steps;
+  const Share share(units.all, units.sharers);
+  const uint32_t wa = share.HolderOfLane(first_unit);
+  const uint32_t parts = share.HolderOfLane(first_unit + steps - 1) - wa + 1;
+  if (parts == 1) return;  // joined where it was made
+  const Own own = OwnOf(args, row_head);
+  float* const to = args.out + row_head * D + d;
+  const float4 own_o = dev::Load4(to);
+  const uint32_t first_slot = 2 * wa + (share.Begin(wa) == first_unit ? 0 : 1);
+  const __amdgpu_buffer_rsrc_t rs = dev::OutResource(args.workspace, 2 * kGroups * SlotBytes(D));
+  float top = -INFINITY, sum = 0.0f;
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+  for (uint32_t p = 0; p < parts; p += kBatch) {
+    uint2 ml[kBatch];
+    float4 x[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const uint32_t part = min(p + k, parts - 1);  // the last once more behind the last, for nothing
+      const uint32_t from = (part == 0 ? first_slot : 2 * (wa + part)) * SlotBytes(D);
+      ml[k] = dev::LoadBufU2<0>(rs, from + 4u * kCols * D + 8u * in_tile);
+      x[k] = dev::LoadBuf4<0>(rs, from + 4u * (in_tile * D + d));
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      if (p + k < parts) {
+        const float m2 = __uint_as_float(ml[k].x), most = fmaxf(top, m2);
+        const float safe = most == -INFINITY ? 0.0f : most;
+        const float f = __builtin_amdgcn_exp2f(top - safe), f2 = __builtin_amdgcn_exp2f(m2 - safe);
+        top = most;
+        sum = fmaf(__uint_as_float(ml[k].y), f2, sum * f);
+        o = make_float4(fmaf(x[k].x, f2, o.x * f), fmaf(x[k].y, f2, o.y * f), fmaf(x[k].z, f2, o.z * f),
+                        fmaf(x[k].w, f2, o.w * f));
+      }
     }
   }
+  dev::Store4(to, Both(own, top, sum).Of(own_o, o));
 }
 
 size_t MlBytes(int32_t n_heads, int64_t n_rows) {
   return (static_cast<size_t>(n_rows) * n_heads * 8 + 255) / 256 * 256;
 }
 size_t PrefixBytes(int32_t n_heads, int32_t head_dim, int64_t n_rows) {
-  return kGroups * (kCounterBytes + 2 * static_cast<size_t>(SlotBytes(head_dim))) + MlBytes(n_heads, n_rows);
+  return 2 * kGroups * static_cast<size_t>(SlotBytes(head_dim)) + MlBytes(n_heads, n_rows);
 }
 
 }  // namespace
@@ -706,10 +704,9 @@ void CheckPrefix(const GpuPagedKv& kv, const GpuPageTable& table, int32_t n_head
   RPG_CHECK(n_rows * group <= 0x7FFFFFFF && most <= 0x7FFFFFFF / std::max(prefix->n_groups, 1),
             "AttentionPagedShared: %d groups of %lld rows of up to %lld positions are too many for one call",
             prefix->n_groups, static_cast<long long>(n_rows), static_cast<long long>(capacity));
-  // counters, slots, (m, l)
+  // slots, (m, l)
   prefix->workspace = workspace;
-  prefix->ml = reinterpret_cast<float*>(workspace +
-                                        kGroups * (kCounterBytes + 2 * static_cast<size_t>(SlotBytes(kv.head_dim))));
+  prefix->ml = reinterpret_cast<float*>(workspace + 2 * kGroups * static_cast<size_t>(SlotBytes(kv.head_dim)));
 }
 
 void AttendPrefix(const GpuPagedKv& kv, const GpuPageTable& table, const int32_t* seq_ids, const int32_t* lens,
@@ -718,11 +715,14 @@ void AttendPrefix(const GpuPagedKv& kv, const GpuPageTable& table, const int32_t
   const bool q8 = kv.type == kKvQ8;
   auto* kern = kv.head_dim == 128 ? (q8 ? SharedPrefixKernel<128, true> : SharedPrefixKernel<128, false>)
                                   : (q8 ? SharedPrefixKernel<64, true> : SharedPrefixKernel<64, false>);
-  Launch("SharedPrefixKernel", kern, dim3(kGroups), dim3(kThreads),
-         PrefixArgs{dev::ViewOf(kv, table), prefix, seq_ids, lens, q_dev, out_dev, prefix.workspace,
-                    static_cast<int32_t>(n_rows),
-                    static_cast<int32_t>(std::min<int64_t>(table.max_pages * kv.page_size, 0x7FFFFFFF)), n_heads,
-                    n_heads / kv.n_kv_heads, scale_log2});
+  const PrefixArgs args{dev::ViewOf(kv, table), prefix, seq_ids, lens, q_dev, out_dev, prefix.workspace,
+                        static_cast<int32_t>(n_rows),
+                        static_cast<int32_t>(std::min<int64_t>(table.max_pages * kv.page_size, 0x7FFFFFFF)), n_heads,
+                        n_heads / kv.n_kv_heads, scale_log2};
+  Launch("SharedPrefixKernel", kern, dim3(kGroups), dim3(kThreads), args);
+  const int64_t join_groups = (n_rows * n_heads * (kv.head_dim / 4) + kJoinThreads - 1) / kJoinThreads;
+  Launch("SharedJoinKernel", kv.head_dim == 128 ? SharedJoinKernel<128> : SharedJoinKernel<64>,
+         dim3(static_cast<uint32_t>(join_groups)), dim3(kJoinThreads), args);
 }
 
 size_t GpuAttentionPagedSharedWorkspaceBytes(int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, int64_t n_rows) {
