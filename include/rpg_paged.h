@@ -106,12 +106,15 @@ typedef struct {
    * group, by itself. Both are device arrays, read when the call runs; at most 64
    * groups. The pages are taken from the group's first row that has them all. Limits
    * as for attention; an infinity or a NaN among a group's keys and values, or a page
-   * out of range, gives NaN. The workspace is attention_shared_workspace's (zeroed by
+   * out of range, may give NaN in all of its rows. Groups that together save less than
+   * least_saving bytes of reading (all rows of a group but one, times its pages) share
+   * nothing; negative: what was measured to break even, 160 MB and one for each row;
+   * 0: share always. The workspace is attention_shared_workspace's (zeroed by
    * attention_workspace_init), for n_rows or more. */
   int32_t (*attention_shared)(const rpg_paged_kv_t* kv, const rpg_page_table_t* table, const int32_t* seq_ids,
                               const int32_t* lens, const int32_t* group_rows, const int32_t* group_pages,
                               int32_t n_groups, const float* q, int32_t n_heads, int64_t n_rows, float* out,
-                              void* workspace, int64_t workspace_bytes);
+                              void* workspace, int64_t workspace_bytes, int64_t least_saving);
   int64_t (*attention_shared_workspace)(int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, int64_t n_rows);
 } rpg_paged_ops_t;
 

@@ -102,11 +102,11 @@ int32_t AttentionWorkspaceInit(void* workspace, int64_t bytes) {
 int32_t AttentionShared(const rpg_paged_kv_t* kv, const rpg_page_table_t* table, const int32_t* seq_ids,
                         const int32_t* lens, const int32_t* group_rows, const int32_t* group_pages, int32_t n_groups,
                         const float* q, int32_t n_heads, int64_t n_rows, float* out, void* workspace,
-                        int64_t workspace_bytes) {
+                        int64_t workspace_bytes, int64_t least_saving) {
   return Guard([&] {
     RPG_CHECK(workspace_bytes >= 0, "AttentionPagedShared: a workspace of negative size");
     rpg::GpuAttentionPagedShared(Kv(kv), Table(table), seq_ids, lens, group_rows, group_pages, n_groups, q, n_heads,
-                                 n_rows, out, workspace, static_cast<size_t>(workspace_bytes));
+                                 n_rows, out, workspace, static_cast<size_t>(workspace_bytes), least_saving);
   });
 }
 

@@ -430,6 +430,7 @@ struct SharedAttentionArgs : AttentionArgs {
   const int32_t* group_rows;
   const int32_t* group_pages;
   int32_t n_groups;
+  uint32_t least;
   float* ml;
 };
 
@@ -485,7 +486,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PagedAttentionKernel(const Arg
   // the batch's units, and this wave's share
   const auto shared = [&] {
     if constexpr (kShared) {
-      return Shared{dev::SharedGroups(args.group_rows, args.group_pages, args.n_groups, rows.n_rows, view.max_pages, lane),
+      return Shared{dev::SharedGroups(args.group_rows, args.group_pages, args.n_groups, args.least, rows.n_rows, view.max_pages, lane),
                     view.page_shift};
     } else {
       return NotShared{};
@@ -1405,7 +1406,8 @@ void AttendPaged(const GpuPagedKv& kv, const GpuPageTable& table, const int32_t*
   const AttentionArgs args{dev::ViewOf(kv, table), rows, q_dev, out_dev, static_cast<char*>(workspace), n_heads,
                            n_heads / kv.n_kv_heads, tiles, tile_heads, scale_log2};
   const dim3 grid(static_cast<unsigned>(groups)), block(64 * kWaves);
-  if (prefix == nullptr || prefix->n_groups == 0) {
+  // what a group of all rows with all of their pages would save, at the most
+  if (prefix == nullptr || prefix->n_groups == 0 || (n_rows - 1) * std::min<int64_t>(table.max_pages, kMostSaving) < prefix->least) {
     Launch("PagedAttentionKernel", KernelFor<AttentionArgs>(kv, tile_heads), grid, block, args);
     return;
   }
@@ -1415,6 +1417,7 @@ void AttendPaged(const GpuPagedKv& kv, const GpuPageTable& table, const int32_t*
   shared.group_rows = prefix->group_rows;
   shared.group_pages = prefix->group_pages;
   shared.n_groups = prefix->n_groups;
+  shared.least = prefix->least;
   shared.ml = prefix->ml;
   Launch("PagedAttentionKernel", KernelFor<SharedAttentionArgs>(kv, tile_heads), grid, block, shared);
   AttendPrefix(kv, table, seq_ids, lens, q_dev, n_heads, n_rows, out_dev, *prefix);

@@ -136,7 +136,7 @@ struct Units {
   uint32_t all, sharers;  // the workgroups that share them out
 
   __device__ __forceinline__ Units(const PrefixArgs& a, int lane)
-      : groups(a.prefix.group_rows, a.prefix.group_pages, a.prefix.n_groups, a.n_rows, a.view.max_pages, lane) {
+      : groups(a.prefix.group_rows, a.prefix.group_pages, a.prefix.n_groups, a.prefix.least, a.n_rows, a.view.max_pages, lane) {
     cols = static_cast<uint32_t>(groups.last - groups.first) * a.group;
     tiles = (cols + kCols - 1) / kCols;
     steps = (PositionsOf(a, groups.pages) + kStep - 1) / kStep;
@@ -687,6 +687,15 @@ __global__ __launch_bounds__(kJoinThreads) void SharedJoinKernel(const PrefixArg
   dev::Store4(to, Both(own, top, sum).Of(own_o, o));
 }
 
+// The bytes of keys and values from which on it pays to share them, 160 MB and one more for each row. Three kernels instead
+// of one cost some 15 us, and 10 more for many rows, whose queries and outputs pass through two of them; the kernel of single
+// rows reads what neighbours have just read at some 6 TB/s. Shared against by themselves, us, 16 query and 8 kv heads of
+// 128, fp16: 2 rows saving 128 MB 45.5 / 48.7, 4 rows 64 MB 30.4 / 19.4 and 144 MB 29.0 / 39.3, 16 rows 64 MB 22.3 / 15.9
+// and 208 MB 26.9 / 33.2, 64 rows 144 MB 33.2 / 27.3 and 256 MB 34.1 / 34.8, 128 rows 256 MB 41.1 / 40.5; 32 and 8 heads
+// in 8 bits: 4 rows 64 MB 32.7 / 22.0 and 144 MB 37.1 / 43.6, 16 rows 144 MB 46.8 / 29.4 and 256 MB 39.7 / 45.1, 64 rows
+// 256 MB 38.1 / 34.6.
+int64_t LeastSaving(int64_t n_rows) { return (160 + n_rows) << 20; }
+
 size_t MlBytes(int32_t n_heads, int64_t n_rows) {
   return (static_cast<size_t>(n_rows) * n_heads * 8 + 255) / 256 * 256;
 }
@@ -735,13 +744,17 @@ size_t GpuAttentionPagedSharedWorkspaceBytes(int32_t n_heads, int32_t n_kv_heads
 void GpuAttentionPagedShared(const GpuPagedKv& kv, const GpuPageTable& table, const int32_t* seq_ids,
                              const int32_t* lens, const int32_t* group_rows, const int32_t* group_pages,
                              int32_t n_groups, const float* q_dev, int32_t n_heads, int64_t n_rows, float* out_dev,
-                             void* workspace, size_t workspace_bytes) {
+                             void* workspace, size_t workspace_bytes, int64_t least_saving) {
   RPG_CHECK(n_groups >= 0 && n_groups <= dev::kMaxSharedGroups, "AttentionPagedShared: %d groups, at most %d", n_groups,
             dev::kMaxSharedGroups);
   RPG_CHECK(n_groups == 0 || (group_rows != nullptr && group_pages != nullptr), "AttentionPagedShared got null groups");
   RPG_CHECK(((reinterpret_cast<uintptr_t>(group_rows) | reinterpret_cast<uintptr_t>(group_pages)) & 3) == 0,
             "AttentionPagedShared: groups have to be 4-byte aligned");
-  PagedPrefix prefix{group_rows, group_pages, n_groups};
+  if (least_saving < 0) least_saving = LeastSaving(n_rows);
+  const int64_t row = int64_t{kv.type == kKvQ8 ? kv.head_dim + 4 : 2 * kv.head_dim} * 2;  // a position's of a kv head
+  const int64_t page = std::max<int64_t>(row * std::max(kv.page_size, 1) * std::max(kv.n_kv_heads, 1), 1);
+  const int64_t least = least_saving / page + (least_saving % page != 0 ? 1 : 0);
+  PagedPrefix prefix{group_rows, group_pages, n_groups, static_cast<uint32_t>(std::min<int64_t>(least, kMostSaving))};
   AttendPaged(kv, table, seq_ids, lens, q_dev, n_heads, n_rows, out_dev, workspace, workspace_bytes, &prefix);
 }
 

@@ -386,14 +386,22 @@ void GpuAttentionPagedWorkspaceInit(void* workspace, size_t bytes);
 // belongs to the first of these. Of a group out of range, what lies inside [0, n_rows)
 // counts; one of no pages, fewer or more than a table has, shares none. Results and limits are
 // GpuAttentionPaged's, but that an infinity or a NaN among a group's keys and values,
-// or a page out of range, gives NaN in all of the group's rows whose output it reaches.
+// or a page out of range, may give NaN in all of the group's rows whose output it
+// reaches.
+//
+// Sharing pays where it saves much reading: groups that together save less than
+// least_saving bytes of keys and values (of each group all rows but one, times its
+// pages) share nothing, and each row is attended to by itself. A negative least_saving
+// stands for what was measured to break even, 160 MB and one more for each row; 0
+// shares always. Where not even all rows with all pages of a table would save as much,
+// the call is GpuAttentionPaged's one launch.
 //
 // workspace: GpuAttentionPagedSharedWorkspaceBytes for n_rows or more, else as for
 // GpuAttentionPaged (GpuAttentionPagedWorkspaceInit zeroes it).
 void GpuAttentionPagedShared(const GpuPagedKv& kv, const GpuPageTable& table, const int32_t* seq_ids,
                              const int32_t* lens, const int32_t* group_rows, const int32_t* group_pages,
                              int32_t n_groups, const float* q_dev, int32_t n_heads, int64_t n_rows, float* out_dev,
-                             void* workspace, size_t workspace_bytes);
+                             void* workspace, size_t workspace_bytes, int64_t least_saving = -1);
 size_t GpuAttentionPagedSharedWorkspaceBytes(int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, int64_t n_rows);
 
 // ---------------------------------------------------------------- quantised matmul

@@ -7,6 +7,7 @@
 
 #include <cstdint>
 
+#include "attention_dev.h"
 #include "kernels_gpu.h"
 
 namespace rpg {
@@ -28,9 +29,11 @@ struct PagedPrefix {
   const int32_t* group_rows;
   const int32_t* group_pages;
   int32_t n_groups;
+  uint32_t least = 0;  // pages times rows that sharing has to save, at most kMostSaving
   char* workspace = nullptr;
   float* ml = nullptr;
 };
+constexpr uint32_t kMostSaving = 1u << 25;  // of a group: what exceeds it counts as this
 
 // GpuAttentionPaged, of what is behind the shared positions if there is a prefix (and then of the rest).
 void AttendPaged(const GpuPagedKv& kv, const GpuPageTable& table, const int32_t* seq_ids, const int32_t* lens,
@@ -93,13 +96,14 @@ __device__ __forceinline__ Slot FindSlot(const PagedView& view, int64_t seq, int
 constexpr int kMaxSharedGroups = 64;
 
 // A call's groups, one to a lane. Rows [first, last) of a group begin with the same `pages` pages; a row that several
-// groups name is of the first of them. What is out of range is cut off.
+// groups name is of the first of them. What is out of range is cut off. Groups that together save less than `least` pages
+// times rows share nothing: their rows are attended to by themselves, in one kernel's work instead of three's.
 struct SharedGroups {
   int32_t n;
   int32_t first = 0, last = 0, pages = 0;
 
   __device__ __forceinline__ SharedGroups(const int32_t* group_rows, const int32_t* group_pages, int32_t n_groups,
-                                          int32_t n_rows, int64_t max_pages, int lane)
+                                          uint32_t least, int32_t n_rows, int64_t max_pages, int lane)
       : n(n_groups) {
     if (lane < n_groups) {
       first = min(max(group_rows[lane], 0), n_rows);
@@ -107,6 +111,9 @@ struct SharedGroups {
       const int32_t p = group_pages[lane];
       pages = p > 0 && p <= max_pages ? p : 0;
     }
+    const uint64_t saving = last > first ? static_cast<uint64_t>(last - first - 1) * static_cast<uint32_t>(pages) : 0;
+    const uint32_t all = attn::ScanAdd(static_cast<uint32_t>(saving < kMostSaving ? saving : kMostSaving));
+    if (static_cast<uint32_t>(__builtin_amdgcn_readlane(all, 63)) < least) pages = 0;
   }
   // The group of row r, the lane's; -1 if there is none.
   __device__ __forceinline__ int32_t OfLane(int32_t r) const {

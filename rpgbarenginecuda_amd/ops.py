@@ -134,7 +134,7 @@ class PagedOpsC(ctypes.Structure):
                 ("attention_workspace", ctypes.CFUNCTYPE(_i64, _i32, _i32, _i32)),
                 ("attention_workspace_init", ctypes.CFUNCTYPE(_i32, _vp, _i64)),
                 ("attention_shared", ctypes.CFUNCTYPE(_i32, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _i32, _i64, _vp, _vp,
-                                                      _i64)),
+                                                      _i64, _i64)),
                 ("attention_shared_workspace", ctypes.CFUNCTYPE(_i64, _i32, _i32, _i32, _i64))]
 
 
@@ -1107,11 +1107,13 @@ def GpuAttentionPagedSharedWorkspace(n_heads: int, n_kv_heads: int, head_dim: in
 
 def GpuAttentionPagedShared(kv: GpuPagedKv, table: GpuPageTable, lens, group_rows, group_pages, q, n_heads: int,
                             n_rows: int, out, workspace, seq_ids=None, workspace_bytes: Optional[int] = None,
-                            n_groups: Optional[int] = None) -> None:
+                            n_groups: Optional[int] = None, least_saving: int = -1) -> None:
     """GpuAttentionPaged for a batch whose sequences share their beginnings: rows [group_rows[g], group_rows[g + 1])
     form group g, whose sequences' tables begin with the same group_pages[g] pages, attended to once for the group.
     group_rows [n_groups + 1] and group_pages [n_groups] are int32 tensors (n_groups goes with raw addresses), of at most
-    64 groups. The workspace is zero before its first call, and belongs to one call at a time."""
+    64 groups. Groups that together save less than least_saving bytes of reading share nothing: -1 stands for what was
+    measured to break even, 160 MB and one for each row, 0 shares always. The workspace is zero before its first call, and
+    belongs to one call at a time."""
     int_at, float_at = kv.int_at, kv.float_at
     span = 4 * n_rows * n_heads * kv.head_dim
     dtype = getattr(workspace, "dtype", None)
@@ -1127,7 +1129,7 @@ def GpuAttentionPagedShared(kv: GpuPagedKv, table: GpuPageTable, lens, group_row
         kv.ref, table.ref, int_at(seq_ids, 4 * n_rows, "seq_ids"), int_at(lens, 4 * n_rows, "lens"),
         int_at(group_rows, 4 * (n_groups + 1), "group_rows"), int_at(group_pages, 4 * n_groups, "group_pages"), n_groups,
         float_at(q, span, "q"), n_heads, n_rows, float_at(out, span, "out"),
-        kv.at(dtype)(workspace, workspace_bytes, "workspace"), workspace_bytes))
+        kv.at(dtype)(workspace, workspace_bytes, "workspace"), workspace_bytes, least_saving))
 
 
 # ----------------------------------------------------------------------------- a step of many conversations

@@ -46,14 +46,14 @@ def batch(rng, kind, n_kv, d, page, groups, k_amp=1.0):
     return p, lens, starts, shared
 
 
-def attend(gpu, kv, table, lens, starts, shared, q, work=None, seq_ids=None, fill=np.nan):
+def attend(gpu, kv, table, lens, starts, shared, q, work=None, seq_ids=None, fill=np.nan, least=0):
     import torch
 
     n, heads, d = q.shape
     out = torch.full((n, heads, d), fill, dtype=torch.float32, device="cuda")
     work = workspace(gpu, heads, kv.n_kv_heads, d, n) if work is None else work
     gpu.GpuAttentionPagedShared(kv, table, dev(lens, np.int32), dev(starts, np.int32), dev(shared, np.int32), dev(q), heads,
-                                n, out, work, seq_ids=None if seq_ids is None else dev(seq_ids, np.int32))
+                                n, out, work, seq_ids=None if seq_ids is None else dev(seq_ids, np.int32), least_saving=least)
     return host(out)
 
 
@@ -199,6 +199,36 @@ def test_a_group_reads_its_first_rows_table(gpu):
 
 
 @pytest.mark.parametrize("kind", [F16, Q8])
+def test_where_sharing_does_not_pay(gpu, kind):
+    """Where not even a full table would save what is asked for, the call is that of rows by themselves; where the groups do
+    not, which the device finds, their rows are by themselves; a byte less asked for, and they share, which shows in what
+    pages out of range reach."""
+    import torch
+
+    rng = np.random.default_rng(12)
+    n_kv, d, page, heads = 2, 64, 16, 4
+    cell = 2 * n_kv * page * (2 * d if kind == F16 else d + 4)
+    pages, lens, starts, shared = batch(rng, kind, n_kv, d, page, [(9, [20, 30, 40]), (5, [7, 60])])
+    q = rng.normal(0, 1, (5, heads, d)).astype(np.float32)
+    saving = (2 * 9 + 1 * 5) * cell
+    good = pages.table.copy()
+    pages.table[1, 3] = pages.table[4, 2] = -1
+    kv, table = pages.device(gpu)
+    out = torch.zeros(5, heads, d, device="cuda")
+    gpu.GpuAttentionPaged(kv, table, dev(lens, np.int32), dev(q), heads, 5, out, workspace(gpu, heads, n_kv, d, 5))
+    alone = host(out)
+    assert np.isnan(alone[[1, 4]]).all() and np.isfinite(alone[[0, 2, 3]]).all()
+    for least in (-1, 1 << 62):
+        assert np.array_equal(attend(gpu, kv, table, lens, starts, shared, q, least=least), alone, equal_nan=True), least
+    found = attend(gpu, kv, table, lens, starts, shared, q, least=saving + 1)
+    together = attend(gpu, kv, table, lens, starts, shared, q, least=saving)
+    pages.table = good
+    assert np.array_equal(np.isnan(found), np.isnan(alone))
+    check(found, pages, lens, q, look=[0, 2, 3])
+    check(together, pages, lens, q)
+
+
+@pytest.mark.parametrize("kind", [F16, Q8])
 def test_magnitudes(gpu, kind):
     """Queries and keys that make one position take everything, or all count alike, on either side of where the shared part
     ends; tiny, huge and zero queries; each element held to the weighted magnitudes that it is made of."""
@@ -325,7 +355,7 @@ def test_captured(gpu, kind, d):
     stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
     torch.cuda.synchronize()
     with torch.cuda.graph(graph, stream=stream), gpu.ScopedEngineStream(stream):
-        gpu.GpuAttentionPagedShared(kv, table, lens, starts, shared, q, heads, n, out, work)
+        gpu.GpuAttentionPagedShared(kv, table, lens, starts, shared, q, heads, n, out, work, least_saving=0)
     for ask, where, what in ((lens0, [0, 4, 7], [40, 10]), (lens0, [0, 4, 7], [1, 2]), ([1] * n, [0, 4, 7], [40, 10]),
                              (lens0, [0, 2, 2], [33, 0]), ([0] * n, [0, 4, 7], [40, 10]), (lens0, [0, 4, 7], [40, 10])):
         x = rng.normal(0, 1, (n, heads, d)).astype(np.float32)
@@ -354,7 +384,7 @@ def test_two_streams_at_once(gpu):
     for i in range(4):
         for s, q, w, o in zip(streams, qs, works, outs):
             with gpu.ScopedEngineStream(s):
-                gpu.GpuAttentionPagedShared(kv, table, n, a, b, q, heads, 5, o[i], w)
+                gpu.GpuAttentionPagedShared(kv, table, n, a, b, q, heads, 5, o[i], w, least_saving=0)
     torch.cuda.synchronize()
     for q, o in zip(qs, outs):
         check(host(o[0]), pages, lens, host(q))
