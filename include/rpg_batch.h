@@ -68,17 +68,16 @@ typedef struct {
    * weights add up to more than u times their sum; u is taken into [0, 1).
    * temperature <= 0 or NaN takes the first in order, with probability 1. A logit
    * that is a NaN counts as minus infinity, plus infinity as the largest finite
-   * number; a row of nothing but minus infinity gives token -1 and probability 0. Beside rpg_op_sample_token_dev, whose random numbers
-   * rpg_sample_counter_uniform gives.
+   * number; a row of nothing but minus infinity gives token -1 and probability 0.
+   * Beside rpg_op_sample_token_dev, whose random numbers rpg_sample_counter_uniform
+   * gives.
    *
-   * workspace: sample_workspace bytes (negative on error), 256-byte aligned, zeroed
-   * once by sample_workspace_init; calls that may run at the same time need one
-   * each. */
+   * workspace: sample_workspace bytes (negative on error), 256-byte aligned, of any
+   * contents; calls that may run at the same time need one each. */
   int32_t (*sample)(const float* logits, int64_t n_rows, int64_t n, int64_t row_stride, const float* temperature,
                     const int32_t* top_k, const float* top_p, const float* min_p, const float* u, int32_t* tokens,
                     float* probs, void* workspace, int64_t workspace_bytes);
   int64_t (*sample_workspace)(int64_t n_rows, int64_t n);
-  int32_t (*sample_workspace_init)(void* workspace, int64_t bytes);
 } rpg_batch_ops_t;
 
 RPG_OPS_API extern const rpg_batch_ops_t rpg_batch_ops;

@@ -74,19 +74,11 @@ int64_t SampleWorkspace(int64_t n_rows, int64_t n) {
   return rc < 0 ? rc : bytes;
 }
 
-int32_t SampleWorkspaceInit(void* workspace, int64_t bytes) {
-  return Guard([&] {
-    RPG_CHECK(bytes >= 0, "SampleBatchWorkspaceInit: a workspace of negative size");
-    rpg::GpuSampleBatchWorkspaceInit(workspace, static_cast<size_t>(bytes));
-  });
-}
-
 }  // namespace
 
 // hipcc passes over a .cc for the device too and would place a constant there.
 #ifndef __HIP_DEVICE_COMPILE__
 extern "C" {
-const rpg_batch_ops_t rpg_batch_ops = {sizeof(rpg_batch_ops_t), RopeTable, RopeRows, Sample, SampleWorkspace,
-                                       SampleWorkspaceInit};
+const rpg_batch_ops_t rpg_batch_ops = {sizeof(rpg_batch_ops_t), RopeTable, RopeRows, Sample, SampleWorkspace};
 }
 #endif

@@ -904,12 +904,6 @@ size_t GpuSampleBatchWorkspaceBytes(int64_t n_rows, int64_t n) {
   return static_cast<size_t>(std::max<int64_t>(n_rows, 1) * RowPlace(SlicesOf(n)).size);
 }
 
-void GpuSampleBatchWorkspaceInit(void* workspace, size_t bytes) {
-  RPG_CHECK(workspace != nullptr && bytes > 0 && bytes % 16 == 0 && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0,
-            "SampleBatchWorkspaceInit: a workspace is 256-byte aligned and a multiple of 16 bytes");
-  GpuStreamFill(workspace, static_cast<int64_t>(bytes), 0);
-}
-
 void GpuSampleBatch(const float* logits_dev, int64_t n_rows, int64_t n, int64_t row_stride,
                     const SampleBatchOptions& opt, const float* u_dev, int32_t* tokens_dev, float* probs_dev,
                     void* workspace, size_t workspace_bytes) {

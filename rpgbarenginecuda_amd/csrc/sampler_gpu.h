@@ -103,15 +103,13 @@ struct SampleBatchOptions {
 
 // probs_dev (may be null): the token's share of the kept weight. All arrays are read on
 // the device: a captured call holds for what stands there at replay. workspace:
-// GpuSampleBatchWorkspaceBytes of device memory, 256-byte aligned, whose bytes are zero
-// before the first call (GpuSampleBatchWorkspaceInit does that); each call leaves it
-// ready for the next on the same stream, of any n_rows and n that need no more. Calls
-// that may run at the same time need a workspace each.
+// GpuSampleBatchWorkspaceBytes of device memory, 256-byte aligned, of any contents; it
+// serves calls one after the other, of any n_rows and n that need no more. Calls that
+// may run at the same time need a workspace each.
 void GpuSampleBatch(const float* logits_dev, int64_t n_rows, int64_t n, int64_t row_stride,
                     const SampleBatchOptions& opt, const float* u_dev, int32_t* tokens_dev, float* probs_dev,
                     void* workspace, size_t workspace_bytes);
 size_t GpuSampleBatchWorkspaceBytes(int64_t n_rows, int64_t n);
-void GpuSampleBatchWorkspaceInit(void* workspace, size_t bytes);
 
 }  // namespace rpg
 

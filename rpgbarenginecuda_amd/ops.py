@@ -151,8 +151,7 @@ class BatchOpsC(ctypes.Structure):
                 ("rope_rows", ctypes.CFUNCTYPE(_i32, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _i64, _vp, _i64, _vp,
                                                _vp)),
                 ("sample", ctypes.CFUNCTYPE(_i32, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64)),
-                ("sample_workspace", ctypes.CFUNCTYPE(_i64, _i64, _i64)),
-                ("sample_workspace_init", ctypes.CFUNCTYPE(_i32, _vp, _i64))]
+                ("sample_workspace", ctypes.CFUNCTYPE(_i64, _i64, _i64))]
 
 
 class RpgError(RuntimeError):
@@ -1158,21 +1157,31 @@ def build_rope_table_scaled(rot_dim: int, theta: float, n_pos: int, scaling: str
     return out
 
 
-class _Here:
-    """Addresses of one call's tensors, which all have to be on the current device."""
+def _here(first):
+    """(buffer, bytes, name) -> address for float32 and for int32 buffers of a call whose first is this, of which every
+    tensor has to be on the current device: as _paged_addr's, a tensor that is in order passes few checks."""
+    torch = _t()
+    tensor, f32, i32 = torch.Tensor, torch.float32, torch.int32
+    index = _current_device() if type(first) is tensor and first.is_cuda else None
 
-    def __init__(self, what: str):
-        self.what = what
-        self.device = None
+    def at(dtype):
+        def of(buf, nbytes: int, name: str):
+            if (type(buf) is tensor and buf.dtype is dtype and buf.get_device() == index and buf.nbytes >= nbytes
+                    and buf.is_contiguous()):
+                return buf.data_ptr()
+            addr = _addr(buf, nbytes, dtype, name)
+            if isinstance(buf, tensor) and buf.get_device() != _current_device():
+                raise RpgError(f"{name} is on {buf.device}, which is not the current device")
+            return addr
 
-    def __call__(self, buf, nbytes: int, dtype, name: str):
-        addr = _addr(buf, nbytes, dtype, name)
-        if buf is not None and not isinstance(buf, int):
-            if self.device is None:
-                self.device = _t().cuda.current_device()
-            if buf.get_device() != self.device:
-                raise RpgError(f"{self.what}: {name} is on device {buf.get_device()}, not the current device {self.device}")
-        return addr
+        return of
+
+    return at(f32), at(i32)
+
+
+def _current_device() -> int:
+    torch = _t()
+    return getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)()
 
 
 def GpuRopeRows(q, k, n_heads: int, n_kv_heads: int, head_dim: int, rot_dim: int, interleaved: bool, rope_tab,
@@ -1180,14 +1189,12 @@ def GpuRopeRows(q, k, n_heads: int, n_kv_heads: int, head_dim: int, rot_dim: int
     """q_out <- q [n_rows, n_heads, head_dim] and k_out <- k [n_rows, n_kv_heads, head_dim], the first rot_dim elements of
     each head rotated by row positions[r] (int32) of rope_tab [rope_rows, rot_dim]: pairs (i, i + rot_dim / 2), or
     (2 i, 2 i + 1) if interleaved. Outputs may be the inputs; k and k_out may be None with n_kv_heads 0."""
-    torch = _t()
-    at, f32 = _Here("GpuRopeRows"), torch.float32
+    float_at, int_at = _here(q)
     qb, kb = 4 * n_rows * n_heads * head_dim, 4 * n_rows * n_kv_heads * head_dim
     _check((_batch or batch_ops()).rope_rows(
-        at(q, qb, f32, "q"), at(k, kb, f32, "k"), n_heads, n_kv_heads, head_dim, rot_dim, 1 if interleaved else 0,
-        at(rope_tab, 4 * rope_rows * rot_dim, f32, "rope_tab"), rope_rows,
-        at(positions, 4 * n_rows, torch.int32, "positions"), n_rows, at(q_out, qb, f32, "q_out"),
-        at(k_out, kb, f32, "k_out")))
+        float_at(q, qb, "q"), float_at(k, kb, "k"), n_heads, n_kv_heads, head_dim, rot_dim, 1 if interleaved else 0,
+        float_at(rope_tab, 4 * rope_rows * rot_dim, "rope_tab"), rope_rows, int_at(positions, 4 * n_rows, "positions"),
+        n_rows, float_at(q_out, qb, "q_out"), float_at(k_out, kb, "k_out")))
 
 
 def GpuSampleBatchWorkspace(n_rows: int, n: int) -> int:
@@ -1195,31 +1202,32 @@ def GpuSampleBatchWorkspace(n_rows: int, n: int) -> int:
     return _check(batch_ops().sample_workspace(n_rows, n))
 
 
-def GpuSampleBatchWorkspaceInit(workspace, nbytes: int) -> None:
-    """Zeroes a workspace, as its first call needs it (a tensor made by torch.zeros is ready)."""
-    _check(batch_ops().sample_workspace_init(_addr(workspace, nbytes, name="workspace"), nbytes))
-
-
 def GpuSampleBatch(logits, n_rows: int, n: int, u, tokens, workspace, temperature=None, top_k=None, top_p=None,
                    min_p=None, probs=None, row_stride: Optional[int] = None,
                    workspace_bytes: Optional[int] = None) -> None:
     """tokens[r] (int32) <- a token of row r of logits [n_rows, n] (rows row_stride floats apart, n if not given), chosen
     by u[r] in [0, 1) after temperature, top_k, top_p and min_p, each a device tensor of n_rows settings (top_k int32,
-    else float32) or None; probs[r] <- its share of the weight that these leave. The workspace is zero before its first
-    call, and belongs to one call at a time (workspace_bytes goes with a raw address)."""
-    torch = _t()
-    at, f32, i32 = _Here("GpuSampleBatch"), torch.float32, torch.int32
+    else float32) or None; probs[r] <- its share of the weight that these leave. The workspace, of any contents, belongs
+    to one call at a time (workspace_bytes goes with a raw address)."""
+    float_at, int_at = _here(logits)
     row_stride = n if row_stride is None else row_stride
     if workspace_bytes is None:
-        if not isinstance(workspace, torch.Tensor):
+        workspace_bytes = getattr(workspace, "nbytes", None)
+        if workspace_bytes is None:
             raise RpgError("GpuSampleBatch: a raw workspace needs workspace_bytes")
-        workspace_bytes = workspace.nbytes
     each = 4 * n_rows
     _check((_batch or batch_ops()).sample(
-        at(logits, 4 * ((n_rows - 1) * row_stride + n) if n_rows > 0 else 0, f32, "logits"), n_rows, n, row_stride,
-        at(temperature, each, f32, "temperature"), at(top_k, each, i32, "top_k"), at(top_p, each, f32, "top_p"),
-        at(min_p, each, f32, "min_p"), at(u, each, f32, "u"), at(tokens, each, i32, "tokens"),
-        at(probs, each, f32, "probs"), at(workspace, workspace_bytes, None, "workspace"), workspace_bytes))
+        float_at(logits, 4 * ((n_rows - 1) * row_stride + n) if n_rows > 0 else 0, "logits"), n_rows, n, row_stride,
+        float_at(temperature, each, "temperature"), int_at(top_k, each, "top_k"), float_at(top_p, each, "top_p"),
+        float_at(min_p, each, "min_p"), float_at(u, each, "u"), int_at(tokens, each, "tokens"),
+        float_at(probs, each, "probs"), _workspace_at(workspace, workspace_bytes), workspace_bytes))
+
+
+def _workspace_at(workspace, nbytes: int):
+    addr = _addr(workspace, nbytes, None, "workspace")
+    if hasattr(workspace, "get_device") and workspace.get_device() != _current_device():
+        raise RpgError(f"workspace is on {workspace.device}, which is not the current device")
+    return addr
 
 
 # ----------------------------------------------------------------------------- measurement

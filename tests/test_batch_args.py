@@ -158,9 +158,6 @@ def test_sample_workspaces(ops):
     for r, n in ((-1, 5), (1, 0), (1, (1 << 22) + 1), ((1 << 20) + 1, 5)):
         with pytest.raises(ops.RpgError):
             ops.GpuSampleBatchWorkspace(r, n)
-    for ptr, n in ((None, 256), (FAKE + 16, 256), (FAKE, 0), (FAKE, 24), (FAKE, -16)):
-        with pytest.raises(ops.RpgError):
-            ops.GpuSampleBatchWorkspaceInit(ptr, n)
 
 
 def test_tensors_are_checked(ops):

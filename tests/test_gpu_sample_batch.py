@@ -29,7 +29,7 @@ def host(t):
 def workspace(gpu, rows, n):
     import torch
 
-    return torch.zeros(gpu.GpuSampleBatchWorkspace(rows, n), dtype=torch.uint8, device="cuda")
+    return torch.full((gpu.GpuSampleBatchWorkspace(rows, n),), 255, dtype=torch.uint8, device="cuda")  # of any contents
 
 
 def settings(rows, t=1.0, k=0, p=1.0, m=0.0, u=0.5):
