@@ -318,7 +318,7 @@ __device__ __forceinline__ T LastLane(T x) {
 }
 
 // The four waves of a SIMD take turns, so that what one wave can do (sums over slices and digits) is done by one, the
-// others waiting at the barrier: with sums over all sixteen the kernel took 22 us for one row and 35 for 128.
+// others waiting at the barrier: sums over all sixteen took 4 us more for one row and 2 for 128.
 constexpr int kRowThreads = 1024;
 constexpr int kRowWaves = kRowThreads / 64;
 constexpr int kJoiners = kRowThreads / kBins;  // threads to a bin, each for every kJoiners-th slice
@@ -340,6 +340,7 @@ struct ChooseShared {
   double scale[kMaxSlices];         // of its weights' units
   int32_t off[kMaxSlices];          // bins that its top one lies below the row's, at most all
   int32_t offsets[kMaxSlices + 1];  // of its candidates
+  int32_t with[kMaxSlices];         // the slices that have some, `n_with` of them
   double kept[kMaxSlices];          // its weight
   uint64_t kept_in[kMaxSlices];     // that of its candidates, in whole units
   uint32_t ties[kMaxSlices];        // its candidates of the cut's key
@@ -353,6 +354,9 @@ struct ChooseShared {
   int32_t top_index;
   uint32_t low, high;
   uint32_t bin[3];
+  int32_t n_with;
+  uint32_t cut_key;
+  uint64_t cut_ties;
   int32_t slice;
 };
 
@@ -439,6 +443,47 @@ __device__ __forceinline__ Cut Select(const Keys& keys, uint32_t n, uint32_t lea
   const uint64_t each = by_weight ? units.OfKey(key) : 1;
   return Cut{key, each > 0 ? (goal + each - 1) / each : 0};
 }
+
+// The same of up to 64 candidates, one to a lane of a wave: each lane sums what is above its own. A filter takes some 1 us
+// so, and 2.6 by the digits above, whose rounds of atomics and barriers cost the same for few as for many (48 rows of 31999,
+// top-k and top-p over some 35 candidates: the kernel 16 us against 20).
+struct Few {
+  uint32_t n, key;
+  uint64_t weight;
+
+  __device__ __forceinline__ Few(const Keys& keys, uint32_t count, const Units& units) : n(count) {
+    const uint32_t lane = threadIdx.x & 63;
+    key = lane < n ? keys[lane] : 0;  // of no candidate's: minus infinity's is above it
+    weight = lane < n ? units.OfKey(key) : 0;
+  }
+  static __device__ __forceinline__ uint64_t FromLane(uint64_t x, uint32_t lane) {
+    return static_cast<uint64_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(x >> 32), lane)) << 32 |
+           static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(x), lane));
+  }
+  __device__ __forceinline__ uint64_t WeightKept(const Cut& cut) const {
+    const uint64_t ties = __ballot(key == cut.key);
+    return LastLane(WaveInclScanU64(key > cut.key ? weight : 0)) +
+           (ties != 0 ? cut.ties * FromLane(weight, __builtin_ctzll(ties)) : 0);
+  }
+  __device__ __forceinline__ Cut Select(bool by_weight, const Cut& cut, uint64_t goal, uint32_t least) const {
+    const uint64_t each = key == 0 || key < cut.key ? 0 : by_weight ? weight : 1;
+    uint64_t above = 0;
+    uint32_t alike = 0;
+#pragma unroll 1
+    for (uint32_t j = 0; j < n; ++j) {
+      const uint32_t other = __builtin_amdgcn_readlane(key, j);
+      const uint64_t amount = FromLane(each, j);
+      above += other > key ? amount : 0;
+      alike += other == key ? 1 : 0;
+    }
+    goal = min(goal, LastLane(WaveInclScanU64(each)));
+    const uint64_t here = __ballot(above < goal && goal <= above + alike * each);
+    if (here == 0) return Cut{least, 0};  // candidates of no weight at all: the last
+    const uint32_t lane = __builtin_ctzll(here);
+    const uint64_t one = FromLane(each, lane);
+    return Cut{static_cast<uint32_t>(__builtin_amdgcn_readlane(key, lane)), (goal - FromLane(above, lane) + one - 1) / one};
+  }
+};
 
 // Of four bytes those in [from, from + span], as a 1 in each. (Bytes are subtracted and added without carries
 // between them; a byte less `from` exceeds the span where adding 255 - span carries out.)
@@ -606,6 +651,7 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
   // ---- of each slice: the weight above these bins, and where its candidates go
   if (wave == 0) {
     uint64_t placed = 0;
+    int32_t n_with = 0;
     slices64([&](int s, bool there) {
       uint64_t in = 0;
       if (there) {
@@ -619,8 +665,14 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
       const uint64_t upto = WaveInclScanU64(in);
       if (there) sh.offsets[s] = static_cast<int32_t>(placed + upto - in);
       placed += LastLane(upto);
+      const uint64_t some = __ballot(in > 0);
+      if (in > 0) sh.with[n_with + __builtin_popcountll(some & ((uint64_t(1) << lane) - 1))] = s;
+      n_with += __builtin_popcountll(some);
     });
-    if (lane == 0) sh.offsets[a.slices] = static_cast<int32_t>(placed);
+    if (lane == 0) {
+      sh.offsets[a.slices] = static_cast<int32_t>(placed);
+      sh.n_with = n_with;
+    }
   }
   __syncthreads();
   const uint32_t n = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(sh.offsets[a.slices]));
@@ -632,21 +684,18 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
     // ---- the candidates, in index order: first where they are, a wave to a slice, 64 neighbours to a lane; then what they
     // are, all at once
     const Keys keys{sh.keys, row.Keys(), n <= kInLds};
-    const auto next_with = [&](int s) {  // from s on, of this wave's slices the next with candidates
-      while (s < a.slices && sh.offsets[s] == sh.offsets[s + 1]) s += kRowWaves;
-      return __builtin_amdgcn_readfirstlane(s);
-    };
+    const int n_with = __builtin_amdgcn_readfirstlane(sh.n_with);
+    const auto slice_of = [&](int i) { return __builtin_amdgcn_readfirstlane(sh.with[min(i, n_with - 1)]); };
     uint4 bytes[4];
     const auto load = [&](int s) {
-      if (s >= a.slices) return;
       const uint4* const from = reinterpret_cast<const uint4*>(row.BytesOf(s)) + 4 * lane;
 #pragma unroll
       for (int i = 0; i < 4; ++i) bytes[i] = from[i];
     };
-    int s = next_with(wave);
-    load(s);
+    int s = slice_of(wave);
+    if (wave < n_with) load(s);
 #pragma unroll 1
-    while (s < a.slices) {
+    for (int i = wave; i < n_with; i += kRowWaves) {
       const int off = __builtin_amdgcn_readfirstlane(sh.off[s]);
       // in the slice's own bins, whose last is the row's last
       const int from = max(0, hi - off), upto = lo == kBins - 1 ? lo : lo - off;
@@ -667,8 +716,10 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
       uint64_t takes = static_cast<uint64_t>(part[3] << 16 | part[2]) << 32 | (part[1] << 16 | part[0]);
       const int32_t at = s * kSlice + 64 * lane;
       uint32_t next = static_cast<uint32_t>(sh.offsets[s]);
-      s = next_with(s + kRowWaves);
-      load(s);
+      if (i + kRowWaves < n_with) {
+        s = slice_of(i + kRowWaves);
+        load(s);
+      }
       if (lo == kBins - 1) {  // minus infinity has the last bin's byte too
         for (uint64_t left = takes; left != 0; left &= left - 1) {
           const int c = __builtin_ctzll(left);
@@ -700,7 +751,13 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
           }
         }
       }
-      if (high != 0) {
+      // (a wave's first: a thousand atomics on one place took 5 us)
+#pragma unroll
+      for (int by = 32; by > 0; by >>= 1) {
+        low = min(low, static_cast<uint32_t>(__shfl_xor(static_cast<int>(low), by, 64)));
+        high = max(high, static_cast<uint32_t>(__shfl_xor(static_cast<int>(high), by, 64)));
+      }
+      if (lane == 0 && high != 0) {
         atomicMin(&sh.low, low);
         atomicMax(&sh.high, high);
       }
@@ -708,32 +765,53 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
     __syncthreads();
 
     // ---- the cut: first top_k's, then top_p's among what that keeps
-    const int width = 32 - __builtin_clz((sh.high - sh.low) | 1);
-#pragma unroll 1
-    for (int filter = cut_k ? 0 : 1; filter < (cut_p ? 2 : 1); ++filter) {
-      uint64_t goal = static_cast<uint64_t>(set.k) - base_count;
-      if (filter == 1) {
-        double of_all = all_weight;
-        if (on_k) {
-          if (tid == 0) sh.found[0] = 0;
-          __syncthreads();
-          uint64_t whole = 0;
-#pragma unroll 1
-          for (uint32_t i = tid; i < n; i += kRowThreads) {
-            const uint32_t key = keys[i];
-            if (key > cut.key) whole += units.OfKey(key);
-          }
-          if (whole != 0) {
-            atomicAdd(reinterpret_cast<unsigned long long*>(&sh.found[0]), static_cast<unsigned long long>(whole));
-          }
-          __syncthreads();
-          of_all = base + static_cast<double>(sh.found[0] + cut.ties * units.OfKey(cut.key)) * unit;
-          __syncthreads();
+    const auto goal_p = [&](double of_all) {
+      const double of = ceil((static_cast<double>(set.p) * of_all - base) / unit);
+      return of < 1.0 ? 1 : static_cast<uint64_t>(fmin(of, 0x1p62));
+    };
+    const uint64_t goal_k = static_cast<uint64_t>(set.k) - base_count;
+    if (n <= 64) {
+      if (wave == 0) {
+        const Few few(keys, n, units);
+        if (cut_k) cut = few.Select(false, cut, goal_k, sh.low);
+        if (cut_p) {
+          const double of_all = on_k ? base + static_cast<double>(few.WeightKept(cut)) * unit : all_weight;
+          cut = few.Select(true, cut, goal_p(of_all), sh.low);
         }
-        const double of = ceil((static_cast<double>(set.p) * of_all - base) / unit);
-        goal = of < 1.0 ? 1 : static_cast<uint64_t>(fmin(of, 0x1p62));
+        if (lane == 0) {
+          sh.cut_key = cut.key;
+          sh.cut_ties = cut.ties;
+        }
       }
-      cut = Select(keys, n, sh.low, width, units, filter == 1, cut, goal, sh);
+      __syncthreads();
+      cut = Cut{sh.cut_key, sh.cut_ties};
+    } else {
+      const int width = 32 - __builtin_clz((sh.high - sh.low) | 1);
+#pragma unroll 1
+      for (int filter = cut_k ? 0 : 1; filter < (cut_p ? 2 : 1); ++filter) {
+        uint64_t goal = goal_k;
+        if (filter == 1) {
+          double of_all = all_weight;
+          if (on_k) {
+            if (tid == 0) sh.found[0] = 0;
+            __syncthreads();
+            uint64_t whole = 0;
+#pragma unroll 1
+            for (uint32_t i = tid; i < n; i += kRowThreads) {
+              const uint32_t key = keys[i];
+              if (key > cut.key) whole += units.OfKey(key);
+            }
+            if (whole != 0) {
+              atomicAdd(reinterpret_cast<unsigned long long*>(&sh.found[0]), static_cast<unsigned long long>(whole));
+            }
+            __syncthreads();
+            of_all = base + static_cast<double>(sh.found[0] + cut.ties * units.OfKey(cut.key)) * unit;
+            __syncthreads();
+          }
+          goal = goal_p(of_all);
+        }
+        cut = Select(keys, n, sh.low, width, units, filter == 1, cut, goal, sh);
+      }
     }
     if (cut.ties > 0) {
       const double of = units.Of(ValueOf(cut.key));
@@ -741,22 +819,27 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
       if (of < least) cut.ties = 0;
     }
 
-    // ---- what it keeps of each slice's candidates
+    // ---- what it keeps of each slice's candidates, a wave to a slice
 #pragma unroll 1
-    for (uint32_t i = tid; i < n; i += kRowThreads) {
-      const uint32_t key = keys[i];
-      if (key < cut.key) continue;
-      int s = 0;  // the last slice that begins at or before i
-      for (int step = 1 << (31 - __builtin_clz(a.slices)); step > 0; step >>= 1) {
-        if (s + step < a.slices && sh.offsets[s + step] <= static_cast<int32_t>(i)) s += step;
-      }
-      if (key == cut.key) {
-        atomicAdd(&sh.ties[s], 1u);
-      } else {
-        const double w = units.Of(ValueOf(key));
-        if (w >= least) {
-          atomicAdd(reinterpret_cast<unsigned long long*>(&sh.kept_in[s]), static_cast<unsigned long long>(Units::Whole(w)));
+    for (int i = wave; i < n_with; i += kRowWaves) {
+      const int of = slice_of(i);
+      const uint32_t end = static_cast<uint32_t>(sh.offsets[of + 1]);
+      uint64_t kept = 0;
+      uint32_t ties = 0;
+#pragma unroll 1
+      for (uint32_t c = static_cast<uint32_t>(sh.offsets[of]) + lane; c < end; c += 64) {
+        const uint32_t key = keys[c];
+        if (key == cut.key) ++ties;
+        if (key > cut.key) {
+          const double w = units.Of(ValueOf(key));
+          if (w >= least) kept += Units::Whole(w);
         }
+      }
+      kept = WaveInclScanU64(kept);
+      ties = attn::ScanAdd(ties);
+      if (lane == 63) {
+        sh.kept_in[of] = kept;
+        sh.ties[of] = ties;
       }
     }
     __syncthreads();
