@@ -175,8 +175,7 @@ __device__ __forceinline__ bool TakesPart(const PrefixArgs& a, const dev::Shared
   return BeginsWith(a, r, pages, there && (groups.n == 1 || groups.OfLane(there ? r : -1) == of), seq);
 }
 
-// kT: tiles of 16 columns of a wave.
-template <int D, bool kQ8, int kT>
+template <int D, bool kQ8>
 __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::SharedGroups& groups, uint32_t me,
                                             const Piece& piece, const int32_t* table, Stage<D, kQ8> (&stages)[2]) {
   constexpr int kRow = 2 * D;              // bytes of a row in LDS
@@ -188,9 +187,9 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
   constexpr int kE = D / 16;               // tiles of 16 elements of a value row
   constexpr int kTiles = kStep / 16;
   constexpr int kPart = D + 4;             // floats of a joined column: o, m, l
-  constexpr int kWaveCols = 16 * kT;
+  constexpr int kWaveCols = 16;
   static_assert(kTiles == kWaves, "a wave brings in 16 positions");
-  static_assert(kCols * kPart * 4 <= sizeof(stages) && 3 * 64 * kPart * 4 <= sizeof(stages), "joins fit where keys were");
+  static_assert(3 * 32 * kPart * 4 <= sizeof(stages), "joins fit where keys were");
 
   const PagedView& view = args.view;
   const int lane = threadIdx.x & 63;
@@ -272,94 +271,85 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
     }
     if (own == 0) st.bad[wave] = from.bad;
   };
+
   // ---- this wave's columns and part of the keys; its queries are requested before the first keys, which take longer
-  const int col_waves = piece.cols > 2 * kWaveCols ? 4 : piece.cols > kWaveCols ? 2 : 1;
-  const int key_waves = col_waves == 4 ? 2 : 4;
+  const int col_waves = piece.cols > 64 ? 8 : piece.cols > 32 ? 4 : piece.cols > 16 ? 2 : 1;
+  const int key_waves = min(kWaves / col_waves, 4);
   const int col_wave = wave % col_waves, key_wave = wave / col_waves;
   const bool works = key_wave < key_waves && col_wave * kWaveCols < piece.cols;
-  float to_score[kT], m[kT], l[kT];
-  float down[kT];  // 8-bit values: the power of two that acc holds them multiplied by
-  F32x4 acc[kT][kE];
-  Half8 q_hi[kT][kSteps], q_lo[kT][kSteps];
-  int64_t row_head[kT];
-  bool there[kT];
+  float to_score, m, l;
+  float down;  // 8-bit values: the power of two that acc holds them multiplied by
+  F32x4 acc[kE];
+  Half8 q_hi[kSteps], q_lo[kSteps];
+  int64_t row_head;
+  bool there;
   int32_t next_page;
   {
-    float4 raw[kT][kSteps][2];
+    float4 raw[kSteps][2];
+    const int32_t in_tile = col_wave * kWaveCols + n;
+    const int32_t col = piece.tile * kCols + in_tile;
+    const bool a_column = works && in_tile < piece.cols;
+    const int32_t in_group = a_column ? col / args.group : 0, row = piece.first_row + in_group;
+    row_head = static_cast<int64_t>(row) * args.n_heads + kh * args.group + (a_column ? col - in_group * args.group : 0);
+    const float* qr = args.q + row_head * D;
 #pragma unroll
-    for (int t = 0; t < kT; ++t) {
-      const int32_t in_tile = col_wave * kWaveCols + 16 * t + n;
-      const int32_t col = piece.tile * kCols + in_tile;
-      const bool a_column = works && in_tile < piece.cols;
-      const int32_t in_group = a_column ? col / args.group : 0, row = piece.first_row + in_group;
-      row_head[t] = static_cast<int64_t>(row) * args.n_heads + kh * args.group + (a_column ? col - in_group * args.group : 0);
-      const float* qr = args.q + row_head[t] * D;
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        raw[t][s][0] = dev::Load4(qr + (4 * s + g) * 8);
-        raw[t][s][1] = dev::Load4(qr + (4 * s + g) * 8 + 4);
-      }
-      int32_t seq;
-      there[t] = TakesPart(args, groups, row, piece.of, piece.pages, a_column, &seq);
+    for (int s = 0; s < kSteps; ++s) {
+      raw[s][0] = dev::Load4(qr + (4 * s + g) * 8);
+      raw[s][1] = dev::Load4(qr + (4 * s + g) * 8 + 4);
     }
+    int32_t seq;
+    there = TakesPart(args, groups, row, piece.of, piece.pages, a_column, &seq);
     load(loaded, c0, page_of(c0));
     next_page = page_of(c0 + 1);
+    float x[kSteps][8];
+    float top = 0.0f;
 #pragma unroll
-    for (int t = 0; t < kT; ++t) {
-      float x[kSteps][8];
-      float top = 0.0f;
+    for (int s = 0; s < kSteps; ++s) {
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
+      for (int i = 0; i < 2; ++i) {
+        const float e[4] = {raw[s][i].x, raw[s][i].y, raw[s][i].z, raw[s][i].w};
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float e[4] = {raw[t][s][i].x, raw[t][s][i].y, raw[t][s][i].z, raw[t][s][i].w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            x[s][4 * i + k] = there[t] ? e[k] : 0.0f;
-            top = fmaxf(top, fabsf(x[s][4 * i + k]));
-          }
+        for (int k = 0; k < 4; ++k) {
+          x[s][4 * i + k] = there ? e[k] : 0.0f;
+          top = fmaxf(top, fabsf(x[s][4 * i + k]));
         }
       }
-      top = MaxAcrossRows(top);
-      const int e = min(max(268 - (__float_as_int(top) >> 23), 1), 254);  // brings top to [2^14, 2^15)
-      const float up = __int_as_float(e << 23);
-      to_score[t] = ldexpf(args.scale_log2, 127 - e);
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        Terms w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = TermsOf(x[s][2 * i] * up, x[s][2 * i + 1] * up);
-        q_hi[t][s] = AsHalf8(w[0].hi, w[1].hi, w[2].hi, w[3].hi);
-        q_lo[t][s] = AsHalf8(w[0].lo, w[1].lo, w[2].lo, w[3].lo);
-      }
-#pragma unroll
-      for (int i = 0; i < kE; ++i) acc[t][i] = F32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      m[t] = -INFINITY;
-      l[t] = 0.0f;
-      down[t] = 0x1p126f;
     }
+    top = MaxAcrossRows(top);
+    const int e = min(max(268 - (__float_as_int(top) >> 23), 1), 254);  // brings top to [2^14, 2^15)
+    const float up = __int_as_float(e << 23);
+    to_score = ldexpf(args.scale_log2, 127 - e);
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      Terms w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = TermsOf(x[s][2 * i] * up, x[s][2 * i + 1] * up);
+      q_hi[s] = AsHalf8(w[0].hi, w[1].hi, w[2].hi, w[3].hi);
+      q_lo[s] = AsHalf8(w[0].lo, w[1].lo, w[2].lo, w[3].lo);
+    }
+#pragma unroll
+    for (int i = 0; i < kE; ++i) acc[i] = F32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    m = -INFINITY;
+    l = 0.0f;
+    down = 0x1p126f;
   }
 
-  // ---- two tiles of 16 keys, from tile `from` of a step, against kT tiles of 16 columns
+  // ---- two tiles of 16 keys, from tile `from` of a step, against 16 columns
   const uint32_t k_lane = static_cast<uint32_t>(n * kRow + 16 * (g ^ k_swap(n)));
   const uint32_t v_lane = static_cast<uint32_t>((4 * g + (n >> 2)) * kRow + 16 * (((n & 3) >> 1) ^ v_swap(n >> 2)) + 8 * (n & 1));
   const auto attend = [&](const Stage<D, kQ8>& st, uint32_t c, int from) {
     const int valid = min(kTiles, (positions - static_cast<int32_t>(c) * kStep) / 16) - from;
     if (valid <= 0) return;
     const uint32_t k_at = Afresh(k_lane), v_at = Afresh(v_lane);
-    F32x4 s[kT][2];
+    F32x4 s[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-#pragma unroll
-      for (int t = 0; t < kT; ++t) s[t][j] = F32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      s[j] = F32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
         const Half8 a = *reinterpret_cast<const Half8*>(st.k + (from + j) * 16 * kRow + (k_at ^ (64u * i)));
-#pragma unroll
-        for (int t = 0; t < kT; ++t) {
-          s[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q_hi[t][i], s[t][j], 0, 0, 0);
-          s[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q_lo[t][i], s[t][j], 0, 0, 0);
-        }
+        s[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q_hi[i], s[j], 0, 0, 0);
+        s[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q_lo[i], s[j], 0, 0, 0);
       }
     }
     const uint32_t bad = Scalar(st.bad[from] | st.bad[from + 1] << 1);
@@ -371,89 +361,80 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
         vs[j] = *reinterpret_cast<const float4*>(st.v_scale + 16 * (from + j) + 4 * g);
         const float by[4] = {ks.x, ks.y, ks.z, ks.w};
 #pragma unroll
-        for (int t = 0; t < kT; ++t) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[t][j][i] *= by[i];
-        }
+        for (int i = 0; i < 4; ++i) s[j][i] *= by[i];
       }
     }
     if (__builtin_expect(valid < 2 || bad != 0, 0)) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-#pragma unroll
-        for (int t = 0; t < kT; ++t) {
-          if (bad >> j & 1) s[t][j] = F32x4{NAN, NAN, NAN, NAN};
-          if (j >= valid) s[t][j] = F32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        }
+        if (bad >> j & 1) s[j] = F32x4{NAN, NAN, NAN, NAN};
+        if (j >= valid) s[j] = F32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
       }
     }
     // Weights are relative to a maximum that moves only where a score exceeds it by 4 (a factor of 16). Over fp16 values
     // they come multiplied by 2^11: with the 16, fp16's largest, and what its low end loses is below 2^-35.
     constexpr float kUp = kQ8 ? 0.0f : 11.0f;
-    uint32_t w[kT][2][4];
+    uint32_t w[2][4];
+    float top = s[0][0];
 #pragma unroll
-    for (int t = 0; t < kT; ++t) {
-      float top = s[t][0][0];
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = fmaxf(top, s[j][i]);
+    }
+    top = MaxAcrossRows(top) * to_score;
+    if (__any(top > m + 4.0f)) {
+      const float to = top > m + 4.0f ? top : m;
+      const float back = __builtin_amdgcn_exp2f(m - (to == -INFINITY ? 0.0f : to));
+      m = to;
+      l *= back;
+#pragma unroll
+      for (int i = 0; i < kE; ++i) acc[i] *= back;
+    }
+    const float less = m == -INFINITY ? 0.0f : m - kUp;
+    float p[2][4];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[j][i] = __builtin_amdgcn_exp2f(fmaf(s[j][i], to_score, -less));
+        l += p[j][i];
+      }
+    }
+    if constexpr (kQ8) {
+      // weights times scales, brought to fp16's range by a power of two that moves only where they pass it
+      float big = 0.0f;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top = fmaxf(top, s[t][j][i]);
-      }
-      top = MaxAcrossRows(top) * to_score[t];
-      if (__any(top > m[t] + 4.0f)) {
-        const float to = top > m[t] + 4.0f ? top : m[t];
-        const float back = __builtin_amdgcn_exp2f(m[t] - (to == -INFINITY ? 0.0f : to));
-        m[t] = to;
-        l[t] *= back;
-#pragma unroll
-        for (int i = 0; i < kE; ++i) acc[t][i] *= back;
-      }
-      const float less = m[t] == -INFINITY ? 0.0f : m[t] - kUp;
-      float p[2][4];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
+        const float by[4] = {vs[j].x, vs[j].y, vs[j].z, vs[j].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          p[j][i] = __builtin_amdgcn_exp2f(fmaf(s[t][j][i], to_score[t], -less));
-          l[t] += p[j][i];
+          p[j][i] *= by[i];
+          big = fmaxf(big, fabsf(p[j][i]));
         }
       }
-      if constexpr (kQ8) {
-        // weights times scales, brought to fp16's range by a power of two that moves only where they pass it
-        float big = 0.0f;
+      big = MaxAcrossRows(big);
+      if (__any(big * down > 0x1p15f)) {
+        const bool passes = big * down > 0x1p15f;
+        const int e = static_cast<int>(__float_as_uint(big) >> 23);  // brings big to [2^12, 2^13)
+        const float to = __uint_as_float(static_cast<uint32_t>(max(266 - e, 1)) << 23);
+        const float back = passes ? to / down : 1.0f;
+        down = passes ? to : down;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float by[4] = {vs[j].x, vs[j].y, vs[j].z, vs[j].w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            p[j][i] *= by[i];
-            big = fmaxf(big, fabsf(p[j][i]));
-          }
-        }
-        big = MaxAcrossRows(big);
-        if (__any(big * down[t] > 0x1p15f)) {
-          const bool passes = big * down[t] > 0x1p15f;
-          const int e = static_cast<int>(__float_as_uint(big) >> 23);  // brings big to [2^12, 2^13)
-          const float to = __uint_as_float(static_cast<uint32_t>(max(266 - e, 1)) << 23);
-          const float back = passes ? to / down[t] : 1.0f;
-          down[t] = passes ? to : down[t];
-#pragma unroll
-          for (int i = 0; i < kE; ++i) acc[t][i] *= back;
-        }
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) p[j][i] *= down[t];
-        }
+        for (int i = 0; i < kE; ++i) acc[i] *= back;
       }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const Terms a = TermsOf(p[j][0], p[j][1]), b = TermsOf(p[j][2], p[j][3]);
-        w[t][0][2 * j] = a.hi;
-        w[t][0][2 * j + 1] = b.hi;
-        w[t][1][2 * j] = a.lo;
-        w[t][1][2 * j + 1] = b.lo;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[j][i] *= down;
       }
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const Terms a = TermsOf(p[j][0], p[j][1]), b = TermsOf(p[j][2], p[j][3]);
+      w[0][2 * j] = a.hi;
+      w[0][2 * j + 1] = b.hi;
+      w[1][2 * j] = a.lo;
+      w[1][2 * j + 1] = b.lo;
     }
 #pragma unroll
     for (int i = 0; i < kE; ++i) {
@@ -461,12 +442,9 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
       const uint2 a = ReadHalvesAcross(at), b = ReadHalvesAcross(at + 16 * kRow);
       const Half8 v = AsHalf8(a.x, a.y, b.x, b.y);
 #pragma unroll
-      for (int t = 0; t < kT; ++t) {
-#pragma unroll
-        for (int term = 0; term < 2; ++term) {
-          const Half8 p = AsHalf8(w[t][term][0], w[t][term][1], w[t][term][2], w[t][term][3]);
-          acc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p, acc[t][i], 0, 0, 0);
-        }
+      for (int term = 0; term < 2; ++term) {
+        const Half8 p = AsHalf8(w[term][0], w[term][1], w[term][2], w[term][3]);
+        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p, acc[i], 0, 0, 0);
       }
     }
   };
@@ -490,79 +468,69 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
   // ---- the waves' parts of a column joined, in order
   const bool whole = c0 == 0 && c1 == piece.steps;
   float* const joins = reinterpret_cast<float*>(stages);  // [key wave - 1][column]
-  const auto join_at = [&](int from, int t) {
-    return joins + ((from - 1) * (col_waves * kWaveCols) + col_wave * kWaveCols + 16 * t + n) * kPart;
+  const auto join_at = [&](int from) {
+    return joins + ((from - 1) * (col_waves * kWaveCols) + col_wave * kWaveCols + n) * kPart;
   };
+  l = SumAcrossRows(l) * (kQ8 ? 1.0f : 0x1p-11f);
+  const float by = kQ8 ? 1.0f / down : 0x1p-11f;
 #pragma unroll
-  for (int t = 0; t < kT; ++t) {
-    l[t] = SumAcrossRows(l[t]) * (kQ8 ? 1.0f : 0x1p-11f);
-    const float by = kQ8 ? 1.0f / down[t] : 0x1p-11f;
-#pragma unroll
-    for (int i = 0; i < kE; ++i) acc[t][i] *= by;
-  }
+  for (int i = 0; i < kE; ++i) acc[i] *= by;
   if (works && key_wave > 0) {
+    float* to = join_at(key_wave);
 #pragma unroll
-    for (int t = 0; t < kT; ++t) {
-      float* to = join_at(key_wave, t);
-#pragma unroll
-      for (int i = 0; i < kE; ++i) *reinterpret_cast<F32x4*>(to + 16 * i + 4 * g) = acc[t][i];
-      if (g == 0) {
-        to[D] = m[t];
-        to[D + 1] = l[t];
-      }
+    for (int i = 0; i < kE; ++i) *reinterpret_cast<F32x4*>(to + 16 * i + 4 * g) = acc[i];
+    if (g == 0) {
+      to[D] = m;
+      to[D + 1] = l;
     }
   }
   __syncthreads();
   const __amdgpu_buffer_rsrc_t rs = dev::OutResource(args.workspace, 2 * kGroups * SlotBytes(D));
   const uint32_t my_slot = (2 * me + (piece.leads ? 0 : 1)) * SlotBytes(D);
   if (works && key_wave == 0) {
+    Own own{};
+    float4 own_o[kE];
+    if (whole && there) {  // requested before the join
+      own = OwnOf(args, row_head);
 #pragma unroll
-    for (int t = 0; t < kT; ++t) {
-      Own own{};
-      float4 own_o[kE];
-      if (whole && there[t]) {  // requested before the join
-        own = OwnOf(args, row_head[t]);
+      for (int i = 0; i < kE; ++i) own_o[i] = dev::Load4(args.out + row_head * D + 16 * i + 4 * g);
+    } else {
 #pragma unroll
-        for (int i = 0; i < kE; ++i) own_o[i] = dev::Load4(args.out + row_head[t] * D + 16 * i + 4 * g);
-      } else {
-#pragma unroll
-        for (int i = 0; i < kE; ++i) own_o[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      }
+      for (int i = 0; i < kE; ++i) own_o[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
 #pragma unroll 1
-      for (int k = 1; k < key_waves; ++k) {
-        const float* from = join_at(k, t);
-        const float m2 = from[D], l2 = from[D + 1];
-        const float to = fmaxf(m[t], m2);
-        const float safe = to == -INFINITY ? 0.0f : to;
-        const float f = __builtin_amdgcn_exp2f(m[t] - safe), f2 = __builtin_amdgcn_exp2f(m2 - safe);
-        m[t] = to;
-        l[t] = fmaf(l2, f2, l[t] * f);
+    for (int k = 1; k < key_waves; ++k) {
+      const float* from = join_at(k);
+      const float m2 = from[D], l2 = from[D + 1];
+      const float to = fmaxf(m, m2);
+      const float safe = to == -INFINITY ? 0.0f : to;
+      const float f = __builtin_amdgcn_exp2f(m - safe), f2 = __builtin_amdgcn_exp2f(m2 - safe);
+      m = to;
+      l = fmaf(l2, f2, l * f);
 #pragma unroll
-        for (int i = 0; i < kE; ++i) {
-          const F32x4 x = *reinterpret_cast<const F32x4*>(from + 16 * i + 4 * g);
+      for (int i = 0; i < kE; ++i) {
+        const F32x4 x = *reinterpret_cast<const F32x4*>(from + 16 * i + 4 * g);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) acc[t][i][r] = fmaf(x[r], f2, acc[t][i][r] * f);
-        }
+        for (int r = 0; r < 4; ++r) acc[i][r] = fmaf(x[r], f2, acc[i][r] * f);
       }
-      if (!there[t]) continue;
-      if (whole) {
-        const Both both(own, m[t], l[t]);
+    }
+    if (whole && there) {
+      const Both both(own, m, l);
 #pragma unroll
-        for (int i = 0; i < kE; ++i) {
-          dev::Store4(args.out + row_head[t] * D + 16 * i + 4 * g,
-                      both.Of(own_o[i], make_float4(acc[t][i][0], acc[t][i][1], acc[t][i][2], acc[t][i][3])));
-        }
-      } else {
-        const int32_t in_tile = col_wave * kWaveCols + 16 * t + n;
+      for (int i = 0; i < kE; ++i) {
+        dev::Store4(args.out + row_head * D + 16 * i + 4 * g,
+                    both.Of(own_o[i], make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3])));
+      }
+    } else if (there) {
+      const int32_t in_tile = col_wave * kWaveCols + n;
 #pragma unroll
-        for (int i = 0; i < kE; ++i) {
-          dev::StoreBuf4<0>(rs, my_slot + 4u * (in_tile * D + 16 * i + 4 * g),
-                                      make_float4(acc[t][i][0], acc[t][i][1], acc[t][i][2], acc[t][i][3]));
-        }
-        if (g == 0) {
-          dev::StoreBufU2<0>(rs, my_slot + 4u * kCols * D + 8u * in_tile,
-                                       make_uint2(__float_as_uint(m[t]), __float_as_uint(l[t])));
-        }
+      for (int i = 0; i < kE; ++i) {
+        dev::StoreBuf4<0>(rs, my_slot + 4u * (in_tile * D + 16 * i + 4 * g),
+                          make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]));
+      }
+      if (g == 0) {
+        dev::StoreBufU2<0>(rs, my_slot + 4u * kCols * D + 8u * in_tile,
+                           make_uint2(__float_as_uint(m), __float_as_uint(l)));
       }
     }
   }
@@ -616,11 +584,7 @@ __global__ __launch_bounds__(kThreads, 2) void SharedPrefixKernel(const PrefixAr
     }
     if (leader < 0) continue;  // the same for every workgroup that has a part of the tile
     const int32_t* table = view.pages + static_cast<int64_t>(leader) * view.max_pages;
-    if (piece.cols > 32) {
-      AttendPiece<D, kQ8, 2>(args, units.groups, me, piece, table, stages);
-    } else {
-      AttendPiece<D, kQ8, 1>(args, units.groups, me, piece, table, stages);
-    }
+    AttendPiece<D, kQ8>(args, units.groups, me, piece, table, stages);
     __syncthreads();  // before the next piece's keys
   }
 }
