@@ -108,7 +108,7 @@ typedef struct {
    * as for attention; an infinity or a NaN among a group's keys and values, or a page
    * out of range, may give NaN in all of its rows. Groups that together save less than
    * least_saving bytes of reading (all rows of a group but one, times its pages) share
-   * nothing; negative: what was measured to break even, 160 MB and one for each row;
+   * nothing; negative: what was measured to break even, 144 MB and one for each row;
    * 0: share always. The workspace is attention_shared_workspace's (zeroed by
    * attention_workspace_init), for n_rows or more. */
   int32_t (*attention_shared)(const rpg_paged_kv_t* kv, const rpg_page_table_t* table, const int32_t* seq_ids,

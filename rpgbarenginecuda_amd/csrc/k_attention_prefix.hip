@@ -210,11 +210,11 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
   };
   Loaded loaded;
   const auto page_of = [&](uint32_t c) {
-    const int32_t pos = static_cast<int32_t>(c) * kStep + 16 * wave;
+    const int32_t pos = static_cast<int32_t>(c * kStep) + 16 * wave;
     return c < c1 && pos < positions ? ScalarLoad(table + (pos >> view.page_shift)) : 0;
   };
   const auto load = [&](Loaded& to, uint32_t c, int32_t page) {
-    const int32_t pos = static_cast<int32_t>(c) * kStep + 16 * wave;
+    const int32_t pos = static_cast<int32_t>(c * kStep) + 16 * wave;
     to.got = c < c1 && pos < positions;
     to.bad = 0;
     if (!to.got) return;
@@ -338,7 +338,7 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
   const uint32_t k_lane = static_cast<uint32_t>(n * kRow + 16 * (g ^ k_swap(n)));
   const uint32_t v_lane = static_cast<uint32_t>((4 * g + (n >> 2)) * kRow + 16 * (((n & 3) >> 1) ^ v_swap(n >> 2)) + 8 * (n & 1));
   const auto attend = [&](const Stage<D, kQ8>& st, uint32_t c, int from) {
-    const int valid = min(kTiles, (positions - static_cast<int32_t>(c) * kStep) / 16) - from;
+    const int valid = min(kTiles, (positions - static_cast<int32_t>(c * kStep)) / 16) - from;
     if (valid <= 0) return;
     const uint32_t k_at = Afresh(k_lane), v_at = Afresh(v_lane);
     F32x4 s[2];
@@ -651,14 +651,14 @@ __global__ __launch_bounds__(kJoinThreads) void SharedJoinKernel(const PrefixArg
   dev::Store4(to, Both(own, top, sum).Of(own_o, o));
 }
 
-// The bytes of keys and values from which on it pays to share them, 160 MB and one more for each row. Three kernels instead
+// The bytes of keys and values from which on it pays to share them, 144 MB and one more for each row. Three kernels instead
 // of one cost some 15 us, and 10 more for many rows, whose queries and outputs pass through two of them; the kernel of single
-// rows reads what neighbours have just read at some 6 TB/s. Shared against by themselves, us, 16 query and 8 kv heads of
-// 128, fp16: 2 rows saving 128 MB 45.5 / 48.7, 4 rows 64 MB 30.4 / 19.4 and 144 MB 29.0 / 39.3, 16 rows 64 MB 22.3 / 15.9
-// and 208 MB 26.9 / 33.2, 64 rows 144 MB 33.2 / 27.3 and 256 MB 34.1 / 34.8, 128 rows 256 MB 41.1 / 40.5; 32 and 8 heads
-// in 8 bits: 4 rows 64 MB 32.7 / 22.0 and 144 MB 37.1 / 43.6, 16 rows 144 MB 46.8 / 29.4 and 256 MB 39.7 / 45.1, 64 rows
-// 256 MB 38.1 / 34.6.
-int64_t LeastSaving(int64_t n_rows) { return (160 + n_rows) << 20; }
+// rows reads what neighbours have just read at some 6 TB/s. Shared against by themselves, us, at 96 / 128 / 160 / 192 / 256 MB
+// saved: 16 query and 8 kv heads of 128, fp16, 4 rows 27:30 32:36 34:42 31:48 40:60, 16 rows 24:18 25:29 26:29 27:31 30:44,
+// 64 rows 29:16 30:26 30:28 30:31 31:34, 128 rows 37:26 37:29 38:32 38:35 38:41; 32 and 8 heads in 8 bits, 4 rows 32:24 39:40
+// 42:43 41:50 50:67, 16 rows 29:20 33:27 35:28 36:35 37:45, 64 rows 33:18 33:27 34:29 35:31 35:35; 32 and 4 heads of 64,
+// fp16, 8 rows 32:19 32:33 32:34 35:44 40:54, 32 rows 26:18 30:24 31:25 32:29 33:37.
+int64_t LeastSaving(int64_t n_rows) { return (144 + n_rows) << 20; }
 
 size_t MlBytes(int32_t n_heads, int64_t n_rows) {
   return (static_cast<size_t>(n_rows) * n_heads * 8 + 255) / 256 * 256;

@@ -392,7 +392,7 @@ void GpuAttentionPagedWorkspaceInit(void* workspace, size_t bytes);
 // Sharing pays where it saves much reading: groups that together save less than
 // least_saving bytes of keys and values (of each group all rows but one, times its
 // pages) share nothing, and each row is attended to by itself. A negative least_saving
-// stands for what was measured to break even, 160 MB and one more for each row; 0
+// stands for what was measured to break even, 144 MB and one more for each row; 0
 // shares always. Where not even all rows with all pages of a table would save as much,
 // the call is GpuAttentionPaged's one launch.
 //
