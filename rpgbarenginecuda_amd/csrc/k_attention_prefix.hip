@@ -341,25 +341,45 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
     const int valid = min(kTiles, (positions - static_cast<int32_t>(c * kStep)) / 16) - from;
     if (valid <= 0) return;
     const uint32_t k_at = Afresh(k_lane), v_at = Afresh(v_lane);
-    F32x4 s[2];
+    // All that the products read is requested ahead of them: left to itself, the compiler saves registers by reading each
+    // operand just before its product, and waits for every one.
+    Half8 k[2][kSteps];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      s[j] = F32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < kSteps; ++i) {
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        const Half8 a = *reinterpret_cast<const Half8*>(st.k + (from + j) * 16 * kRow + (k_at ^ (64u * i)));
-        s[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q_hi[i], s[j], 0, 0, 0);
-        s[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q_lo[i], s[j], 0, 0, 0);
-      }
+      for (int j = 0; j < 2; ++j) k[j][i] = *reinterpret_cast<const Half8*>(st.k + (from + j) * 16 * kRow + (k_at ^ (64u * i)));
     }
-    const uint32_t bad = Scalar(st.bad[from] | st.bad[from + 1] << 1);
-    float4 vs[2];
+    const uint32_t bads[2] = {st.bad[from], st.bad[from + 1]};
+    float4 ks[2], vs[2];
     if constexpr (kQ8) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const float4 ks = *reinterpret_cast<const float4*>(st.k_scale + 16 * (from + j) + 4 * g);
+        ks[j] = *reinterpret_cast<const float4*>(st.k_scale + 16 * (from + j) + 4 * g);
         vs[j] = *reinterpret_cast<const float4*>(st.v_scale + 16 * (from + j) + 4 * g);
-        const float by[4] = {ks.x, ks.y, ks.z, ks.w};
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    F32x4 s[2] = {};
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) s[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[j][i], q_hi[i], s[j], 0, 0, 0);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) s[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[j][i], q_lo[i], s[j], 0, 0, 0);
+    }
+    uint2 v[kE][2];
+#pragma unroll
+    for (int i = 0; i < kE; ++i) {
+      const char* at = st.v + from * 16 * kRow + (v_at ^ (32u * i));
+      v[i][0] = ReadHalvesAcross(at);
+      v[i][1] = ReadHalvesAcross(at + 16 * kRow);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    const uint32_t bad = Scalar(bads[0] | bads[1] << 1);
+    if constexpr (kQ8) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float by[4] = {ks[j].x, ks[j].y, ks[j].z, ks[j].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) s[j][i] *= by[i];
       }
@@ -438,13 +458,10 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
     }
 #pragma unroll
     for (int i = 0; i < kE; ++i) {
-      const char* at = st.v + from * 16 * kRow + (v_at ^ (32u * i));
-      const uint2 a = ReadHalvesAcross(at), b = ReadHalvesAcross(at + 16 * kRow);
-      const Half8 v = AsHalf8(a.x, a.y, b.x, b.y);
 #pragma unroll
       for (int term = 0; term < 2; ++term) {
         const Half8 p = AsHalf8(w[term][0], w[term][1], w[term][2], w[term][3]);
-        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p, acc[i], 0, 0, 0);
+        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(AsHalf8(v[i][0].x, v[i][0].y, v[i][1].x, v[i][1].y), p, acc[i], 0, 0, 0);
       }
     }
   };
