@@ -7,20 +7,26 @@
 // over its own ones m', l' and the output o' / l'; joined (o f + o' f') / (l f + l' f') with f = 2^(m - M),
 // f' = 2^(m' - M), M the larger of m and m'.
 //
-// What bounds it: keys and values are read once for up to 128 columns (the queries of a kv head: rows times heads of a
-// group), so that from some 64 columns on the matrix cores do, which run each product twice: queries and weights, which
-// are fp32, enter as two fp16 terms of 11 bits each, together 22. Over 8-bit pages codes are fp16 numbers as they are;
-// keys' scales multiply the scores, and weights times values' scales are brought to fp16's range by a power of two of the
-// column's, which moves with their maximum.
+// Keys and values are read once for up to 128 columns (the queries of a kv head: rows times heads of a group). Queries and
+// weights, which are fp32, enter the matrix cores as two fp16 terms of 11 bits each, together 22, so that each product runs
+// twice. Over 8-bit pages codes are fp16 numbers as they are; keys' scales multiply the scores, and weights times values'
+// scales are brought to fp16's range by a power of two of the column's, which moves with their maximum.
 //
 // A workgroup takes steps of 128 positions through LDS, two of them at a time (one being read, one being filled), for a
-// tile of up to 128 columns; of its eight waves each has 32 columns and a half of the step's keys, a quarter where the
-// tile has no more than 64 columns, or 16 columns and a quarter for no more than 32. The products are those of
-// k_attention_paged.hip: rows of S = K Q^T are 16 keys, rows of O^T = V^T P^T 16 elements, so that a lane ends the first
-// with the weights of the keys that it holds in the second. The units (kv head, column tile, step) of all groups are
-// shared out evenly and contiguously. A tile that one workgroup holds it joins with the rows' own parts by itself; the
-// parts of others are left in the workspace for a small kernel that joins them in order, over all compute units: the last
-// workgroup of a tile to arrive, on its one, took 18 us for four parts of 128 columns where that takes 4.
+// tile of up to 128 columns; of its eight waves each has 16 columns and all of a step's keys, a half or a quarter of them
+// where the tile has no more than 64 or 32 columns. The products are those of k_attention_paged.hip: rows of S = K Q^T are
+// 16 keys, rows of O^T = V^T P^T 16 elements, so that a lane ends the first with the weights of the keys that it holds in
+// the second. The units (kv head, column tile, step) of all groups are shared out evenly and contiguously. A tile that one
+// workgroup holds it joins with the rows' own parts by itself; the parts of others are left in the workspace for a small
+// kernel that joins them in order, over all compute units: the last workgroup of a tile to arrive, on its one, took 18 us for
+// four parts of 128 columns where that takes 4.
+//
+// What bounds it: 32 positions of 128 columns take a compute unit 2700 cycles, of which the matrix cores are busy for 1030
+// and vector arithmetic for 1360, by two waves that mostly wait for the same; 32 columns to a wave (half the reads of LDS)
+// and sixteen waves were no faster, and their code and joins cost the short pieces 4 us. Behind few columns it is memory
+// (4 TB/s), and for one or two steps the chain of groups, lengths, table, keys and the first pass through the code, 9 us.
+// 128 rows and 4 heads to a kv head over 8192 positions in 8 bits 58 us (0.59 PFLOP/s of formed products), 8 rows over
+// 32768 26.5 us, 32 rows and 2 heads over 2816 in fp16 11.7 us.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -64,14 +70,15 @@ struct PrefixArgs {
   float scale_log2;
 };
 
-// The two fp16 terms of a pair of values: rounded to 11 bits, and what that leaves rounded to 11.
+// The two fp16 terms of a pair of values times `by`, a power of two: rounded to 11 bits, and what that leaves rounded to 11.
+// (Instructions that multiply, add and round to either half of a register: two for each value.)
 struct Terms {
   uint32_t hi, lo;
 };
-__device__ __forceinline__ Terms TermsOf(float a, float b) {
-  const Half2 hi = {static_cast<_Float16>(a), static_cast<_Float16>(b)};
-  const Half2 lo = {static_cast<_Float16>(a - static_cast<float>(hi[0])),
-                    static_cast<_Float16>(b - static_cast<float>(hi[1]))};
+__device__ __forceinline__ Terms TermsOf(float a, float b, float by) {
+  const Half2 hi = {static_cast<_Float16>(fmaf(a, by, 0.0f)), static_cast<_Float16>(fmaf(b, by, 0.0f))};
+  const Half2 lo = {static_cast<_Float16>(fmaf(a, by, -static_cast<float>(hi[0]))),
+                    static_cast<_Float16>(fmaf(b, by, -static_cast<float>(hi[1])))};
   return Terms{Bits(hi), Bits(lo)};
 }
 
@@ -201,7 +208,7 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
 
   // ---- bringing in: this wave's 16 positions of a step, their pieces permuted as the reads below need them
   const auto k_swap = [](int r) { return kPieces == 16 ? r & 15 : r & 7; };
-  const auto v_swap = [](int r) { return 2 * (r & 3); };
+  const auto v_swap = [](int r) { return 2 * (r & (kPieces == 16 ? 7 : 3)); };
   struct Loaded {
     float4 k[kLoads], v[kLoads];
     float k_scale, v_scale;  // of row lane % 16
@@ -278,7 +285,7 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
   const int col_wave = wave % col_waves, key_wave = wave / col_waves;
   const bool works = key_wave < key_waves && col_wave * kWaveCols < piece.cols;
   float to_score, m, l;
-  float down;  // 8-bit values: the power of two that acc holds them multiplied by
+  float down;  // the power of two that weights enter multiplied by
   F32x4 acc[kE];
   Half8 q_hi[kSteps], q_lo[kSteps];
   int64_t row_head;
@@ -323,7 +330,7 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
     for (int s = 0; s < kSteps; ++s) {
       Terms w[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = TermsOf(x[s][2 * i] * up, x[s][2 * i + 1] * up);
+      for (int i = 0; i < 4; ++i) w[i] = TermsOf(x[s][2 * i], x[s][2 * i + 1], up);
       q_hi[s] = AsHalf8(w[0].hi, w[1].hi, w[2].hi, w[3].hi);
       q_lo[s] = AsHalf8(w[0].lo, w[1].lo, w[2].lo, w[3].lo);
     }
@@ -331,12 +338,12 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
     for (int i = 0; i < kE; ++i) acc[i] = F32x4{0.0f, 0.0f, 0.0f, 0.0f};
     m = -INFINITY;
     l = 0.0f;
-    down = 0x1p126f;
+    down = kQ8 ? 0x1p126f : 1.0f;
   }
 
   // ---- two tiles of 16 keys, from tile `from` of a step, against 16 columns
   const uint32_t k_lane = static_cast<uint32_t>(n * kRow + 16 * (g ^ k_swap(n)));
-  const uint32_t v_lane = static_cast<uint32_t>((4 * g + (n >> 2)) * kRow + 16 * (((n & 3) >> 1) ^ v_swap(n >> 2)) + 8 * (n & 1));
+  const uint32_t v_lane = static_cast<uint32_t>((4 * g + (n >> 2)) * kRow + 16 * (((n & 3) >> 1) ^ v_swap(4 * g + (n >> 2))) + 8 * (n & 1));
   const auto attend = [&](const Stage<D, kQ8>& st, uint32_t c, int from) {
     const int valid = min(kTiles, (positions - static_cast<int32_t>(c * kStep)) / 16) - from;
     if (valid <= 0) return;
@@ -442,15 +449,10 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
 #pragma unroll
         for (int i = 0; i < kE; ++i) acc[i] *= back;
       }
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[j][i] *= down;
-      }
     }
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const Terms a = TermsOf(p[j][0], p[j][1]), b = TermsOf(p[j][2], p[j][3]);
+      const Terms a = TermsOf(p[j][0], p[j][1], down), b = TermsOf(p[j][2], p[j][3], down);
       w[0][2 * j] = a.hi;
       w[0][2 * j + 1] = b.hi;
       w[1][2 * j] = a.lo;
