@@ -368,6 +368,25 @@ def test_captured(gpu, kind, d):
         assert np.array_equal(got, eager)
 
 
+def test_pages_past_32_bit_offsets(gpu):
+    """A group whose pages start past 2^32 elements of the pool; one of its sequences has two rows."""
+    import torch
+
+    rng = np.random.default_rng(30)
+    n_kv, d, page, heads = 8, 128, 256, 16
+    few, lens, starts, shared = batch(rng, Q8, n_kv, d, page, [(3, [5, 300])])
+    n_pages = (1 << 32) // (n_kv * d * page) + few.n_pages
+    far = n_pages - few.n_pages
+    k, v = (torch.zeros((n_pages, n_kv, page, d), dtype=torch.int8, device="cuda") for _ in range(2))
+    ks, vs = (torch.zeros((n_pages, n_kv, page), device="cuda") for _ in range(2))
+    for big, small in ((k, few.k), (v, few.v), (ks, few.ks), (vs, few.vs)):
+        big[far:] = dev(small)
+    kv, table = gpu.GpuPagedKv(k, v, ks, vs), gpu.GpuPageTable(dev(few.table + far, np.int32))
+    q = rng.normal(0, 1, (3, heads, d)).astype(np.float32)
+    lens, seqs = [lens[0], lens[1], lens[1] - 7], [0, 1, 1]
+    check(attend(gpu, kv, table, lens, [0, 3], shared, q, seq_ids=seqs), few, lens, q, seqs)
+
+
 def test_two_streams_at_once(gpu):
     import torch
 

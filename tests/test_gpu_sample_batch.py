@@ -95,6 +95,44 @@ def test_sizes(gpu, n):
     assert np.array_equal(got[0], again[0]) and np.array_equal(got[1], again[1])
 
 
+@pytest.mark.parametrize("n", [300_007, (1 << 22) - 1, 1 << 22])
+def test_vocabularies_of_many_slices(gpu, n):
+    """More slices than a wave has lanes, up to the largest vocabulary there is."""
+    rng = np.random.default_rng(n)
+    x, how = logits(rng, 13, n), mixed(rng, 13)
+    check(choose(gpu, x, how), x, how)
+
+
+@pytest.mark.parametrize("alike", [1, 2, 63, 64, 65, 1024, 1025, 8191, 8192, 8193])
+def test_so_many_values_around_the_cut(gpu, alike):
+    """From where a wave's lanes hold the values that lie between the cut's borders to where LDS no longer does: all within
+    an eighth of an octave, every third with a double, beside others far below."""
+    rng = np.random.default_rng(alike)
+    rows, n = 26, 30_011
+    x = rng.normal(-30, 1, (rows, n)).astype(np.float32)
+    for r in range(rows):
+        at = rng.permutation(n)[:alike]
+        x[r, at] = rng.uniform(4.0, 4.03, alike).astype(np.float32)
+        x[r, at[1::3]] = x[r, at[:len(at[1::3])]]
+    p, k = (0.6, 1.0, 0.9, 0.03, 1.0), (0, 1 + alike // 2, 2 * alike // 3 + 1, 0, alike)
+    how = settings(rows, 1.0, [k[r % 5] for r in range(rows)], [p[r % 5] for r in range(rows)],
+                   [0.0 if r % 3 else 0.99 for r in range(rows)], rng.random(rows).astype(np.float32))
+    check(choose(gpu, x, how), x, how)
+
+
+def test_rows_past_32_bit_offsets(gpu):
+    import torch
+
+    rng = np.random.default_rng(21)
+    n, stride = 5003, (1 << 30) + 77
+    x, (t, k, p, m, u) = logits(rng, 2, n), mixed(rng, 2)
+    far = torch.zeros(stride + n, device="cuda")
+    far[:n], far[stride:] = dev(x[0]), dev(x[1])
+    tokens, probs = torch.zeros(2, dtype=torch.int32, device="cuda"), torch.zeros(2, device="cuda")
+    gpu.GpuSampleBatch(far, 2, n, dev(u), tokens, workspace(gpu, 2, n), dev(t), dev(k), dev(p), dev(m), probs, row_stride=stride)
+    check((host(tokens), host(probs)), x, (t, k, p, m, u))
+
+
 @pytest.mark.parametrize("spread", [0.01, 1.0, 8.0])
 def test_flat_and_steep(gpu, spread):
     """From where nearly every token is kept to where a few are."""
