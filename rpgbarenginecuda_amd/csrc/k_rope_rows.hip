@@ -9,7 +9,8 @@
 // token. A thread has two chunks of four elements, the same of kHeads heads of one
 // token, for which it reads the table once; of a rotated part the chunks lie half of
 // that part apart in either layout, so that a lane has both members of its pairs and
-// the lanes of a head read and write whole lines.
+// the lanes of a head read and write whole lines. 2811 tokens of 24 heads of 128 take 12.5 us (5.6 TB/s), 9001
+// of 40, half of each rotated, 62 (6.0 TB/s), a single one 2.2, the launch.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -178,11 +179,14 @@ void GpuRopeRows(const float* q, const float* k, int32_t n_heads, int32_t n_kv_h
             "RopeRows: outputs must not overlap the table or the positions");
   RopeArgs a{q,         k,       q_out,      k_out,    rope_tab, positions,
              rope_rows, n_heads, n_kv_heads, head_dim, rot_dim,  static_cast<uint32_t>(per_token), 0};
+  // whole chunks of four elements, aligned; else a pair to a thread (2811 rows of 24 heads of 128: 12.5 us against 21, one row
+  // the same)
   if (head_dim % 8 == 0 && rot_dim % 8 == 0 && (all & 15) == 0) {
     constexpr int kHeads = 4;
     const dim3 block(head_dim / 8, std::max(1, kThreads / (head_dim / 8)));
-    // one head to a thread for few rows, so that more of the card works
-    const bool few = n_rows * per_token * (head_dim / 8) <= 256 * kThreads;
+    // one head to a thread up to six workgroups to a compute unit, so that more of the card works; then four, which read the
+    // table's row once (24 heads of 128, us, one against four: 1 row 2.4 / 3.0, 341 3.5 / 4.3, 1024 5.5 / 5.6, 2811 13.9 / 12.5)
+    const bool few = n_rows * per_token * (head_dim / 8) <= 6 * 256 * kThreads;
     a.groups = few ? per_token : (per_token + kHeads - 1) / kHeads;
     a.units = static_cast<uint32_t>(n_rows) * a.groups;
     auto* kern = few ? (interleaved ? RopeRowsKernel<1, true> : RopeRowsKernel<1, false>)
