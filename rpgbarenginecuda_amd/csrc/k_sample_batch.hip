@@ -468,23 +468,44 @@ struct Few {
     return LastLane(WaveInclScanU64(key > cut.key ? weight : 0)) +
            (ties != 0 ? cut.ties * FromLane(weight, __builtin_ctzll(ties)) : 0);
   }
-  __device__ __forceinline__ Cut Select(bool by_weight, const Cut& cut, uint64_t goal, uint32_t least) const {
-    const uint64_t each = key == 0 || key < cut.key ? 0 : by_weight ? weight : 1;
-    uint64_t above = 0;
+  // (Four candidates a turn, whose steps overlap; those behind the last, of key and weight 0, change nothing.)
+  __device__ __forceinline__ Cut SelectCount(uint64_t goal) const {
+    uint32_t above = 0, alike = 0;
+#pragma unroll 1
+    for (uint32_t j = 0; j < n; j += 4) {
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i) {
+        const uint32_t other = __builtin_amdgcn_readlane(key, j + i);
+        above += other > key ? 1 : 0;
+        alike += other == key ? 1 : 0;
+      }
+    }
+    const uint32_t want = static_cast<uint32_t>(min(goal, static_cast<uint64_t>(n)));
+    const uint32_t lane = __builtin_ctzll(__ballot(key != 0 && above < want && want <= above + alike));
+    return Cut{static_cast<uint32_t>(__builtin_amdgcn_readlane(key, lane)),
+               want - static_cast<uint32_t>(__builtin_amdgcn_readlane(above, lane))};
+  }
+  __device__ __forceinline__ Cut SelectWeight(const Cut& cut, uint64_t goal, uint32_t least) const {
+    const uint64_t each = key == 0 || key < cut.key ? 0 : weight;
+    uint64_t above[2] = {0, 0};
     uint32_t alike = 0;
 #pragma unroll 1
-    for (uint32_t j = 0; j < n; ++j) {
-      const uint32_t other = __builtin_amdgcn_readlane(key, j);
-      const uint64_t amount = FromLane(each, j);
-      above += other > key ? amount : 0;
-      alike += other == key ? 1 : 0;
+    for (uint32_t j = 0; j < n; j += 4) {
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i) {
+        const uint32_t other = __builtin_amdgcn_readlane(key, j + i);
+        const uint64_t amount = FromLane(each, j + i);
+        above[i & 1] += other > key ? amount : 0;
+        alike += other == key ? 1 : 0;
+      }
     }
+    above[0] += above[1];
     goal = min(goal, LastLane(WaveInclScanU64(each)));
-    const uint64_t here = __ballot(above < goal && goal <= above + alike * each);
+    const uint64_t here = __ballot(above[0] < goal && goal <= above[0] + alike * each);
     if (here == 0) return Cut{least, 0};  // candidates of no weight at all: the last
     const uint32_t lane = __builtin_ctzll(here);
     const uint64_t one = FromLane(each, lane);
-    return Cut{static_cast<uint32_t>(__builtin_amdgcn_readlane(key, lane)), (goal - FromLane(above, lane) + one - 1) / one};
+    return Cut{static_cast<uint32_t>(__builtin_amdgcn_readlane(key, lane)), (goal - FromLane(above[0], lane) + one - 1) / one};
   }
 };
 
@@ -511,8 +532,11 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
 
   // ---- the slices' largest, and what their weights are multiplied by
   if (wave == 0) {
-    float top = -INFINITY;
-    slices64([&](int s, bool there) { top = fmaxf(top, there ? row.Sums()[s].top : -INFINITY); });
+    SliceSums firsts{-INFINITY, 0, 0};  // of the first 64 slices
+    if (lane < a.slices) firsts = row.Sums()[lane];
+    float top = firsts.top;
+#pragma unroll 1
+    for (int s = 64 + lane; s < a.slices; s += 64) top = fmaxf(top, row.Sums()[s].top);
     top = WaveMaxTo63(top);
     top = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(top), 63));
     int32_t index = 0x7FFFFFFF;
@@ -520,7 +544,7 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
     const Exp2Near<0> near;
     slices64([&](int s, bool there) {
       if (!there) return;
-      const SliceSums mine = row.Sums()[s];
+      const SliceSums mine = s < 64 ? firsts : row.Sums()[s];
       if (set.greedy) {
         if (mine.top == top) index = min(index, mine.top_index);
         return;
@@ -776,10 +800,10 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
     if (n <= 64) {
       if (wave == 0) {
         const Few few(keys, n, units);
-        if (cut_k) cut = few.Select(false, cut, goal_k, sh.low);
+        if (cut_k) cut = few.SelectCount(goal_k);
         if (cut_p) {
           const double of_all = on_k ? base + static_cast<double>(few.WeightKept(cut)) * unit : all_weight;
-          cut = few.Select(true, cut, goal_p(of_all), sh.low);
+          cut = few.SelectWeight(cut, goal_p(of_all), sh.low);
         }
         if (lane == 0) {
           sh.cut_key = cut.key;
@@ -916,26 +940,33 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
     for (int w = 0; w < wave; ++w) tie_at += sh.wave_sum[w];
     __syncthreads();
   }
-  uint64_t w[4], sum = 0;
+  uint64_t w[4] = {0, 0, 0, 0}, sum = 0;
   double of[4];
   uint32_t last = 0;  // the last kept one, above all those of no weight
+  int bin[4];
+  bool some = false;
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
-    const uint32_t key = KeyOf(x[c]);
-    const int j = set.BinBelow(top_bin, x[c]);
-    of[c] = units.Of(x[c]);
-    bool keep = j < hi;
-    if (!keep && j <= lo && of[c] >= least) {
-      keep = key > cut.key;
-      if (key == cut.key) {
-        keep = some_ties ? tie_at < ties_kept : ties_kept > 0;
-        ++tie_at;
+    bin[c] = x[c] > -INFINITY ? set.BinBelow(top_bin, x[c]) : 1 << 30;
+    some = some || bin[c] < hi || bin[c] <= lo;
+  }
+  if (__any(some)) {  // in most waves nothing is kept
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const uint32_t key = KeyOf(x[c]);
+      of[c] = units.Of(x[c]);
+      bool keep = bin[c] < hi;
+      if (!keep && bin[c] <= lo && of[c] >= least) {
+        keep = key > cut.key;
+        if (key == cut.key) {
+          keep = some_ties ? tie_at < ties_kept : ties_kept > 0;
+          ++tie_at;
+        }
       }
+      w[c] = keep ? Units::Whole(of[c]) : 0;
+      sum += w[c];
+      if (keep) last = max(last, (w[c] > 0 ? 0x80000000u : 0u) + static_cast<uint32_t>(at + c + 1));
     }
-    keep = keep && x[c] > -INFINITY;
-    w[c] = keep ? Units::Whole(of[c]) : 0;
-    sum += w[c];
-    if (keep) last = max(last, (w[c] > 0 ? 0x80000000u : 0u) + static_cast<uint32_t>(at + c + 1));
   }
   const uint64_t upto = WaveInclScanU64(sum);
   if (lane == 63) sh.wave_sum[wave] = upto;
