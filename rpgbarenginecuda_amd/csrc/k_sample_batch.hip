@@ -350,7 +350,7 @@ struct ChooseShared {
   uint32_t first[kMaxSlices];       // of these those that are kept
   uint64_t found[2];
   uint64_t wave_sum[kRowWaves];
-  uint64_t wave_last[kRowWaves];
+  uint32_t wave_last[kRowWaves];
   double weight_of_all;
   double before;
   float top;
@@ -523,6 +523,8 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
   __shared__ ChooseShared sh;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const Row row(a, blockIdx.x);
+  SliceSums firsts{-INFINITY, 0, 0};  // of the first 64 slices, for the first wave
+  if (tid < min(a.slices, 64)) firsts = row.Sums()[tid];
   const Setting set = SettingOf(a, row.r);
   const bool on_p = set.OnP(), on_m = set.m > 0.0f, filters = set.Filters();
   const auto slices64 = [&](auto f) {  // by the first wave
@@ -532,8 +534,6 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
 
   // ---- the slices' largest, and what their weights are multiplied by
   if (wave == 0) {
-    SliceSums firsts{-INFINITY, 0, 0};  // of the first 64 slices
-    if (lane < a.slices) firsts = row.Sums()[lane];
     float top = firsts.top;
 #pragma unroll 1
     for (int s = 64 + lane; s < a.slices; s += 64) top = fmaxf(top, row.Sums()[s].top);
@@ -942,7 +942,7 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
   }
   uint64_t w[4] = {0, 0, 0, 0}, sum = 0;
   double of[4];
-  uint32_t last = 0;  // the last kept one, above all those of no weight
+  bool kept[4] = {false, false, false, false};
   int bin[4];
   bool some = false;
 #pragma unroll
@@ -963,23 +963,17 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
           ++tie_at;
         }
       }
+      kept[c] = keep;
       w[c] = keep ? Units::Whole(of[c]) : 0;
       sum += w[c];
-      if (keep) last = max(last, (w[c] > 0 ? 0x80000000u : 0u) + static_cast<uint32_t>(at + c + 1));
     }
   }
   const uint64_t upto = WaveInclScanU64(sum);
   if (lane == 63) sh.wave_sum[wave] = upto;
-#pragma unroll
-  for (int by = 32; by > 0; by >>= 1) last = max(last, static_cast<uint32_t>(__shfl_xor(static_cast<int>(last), by, 64)));
-  if (lane == 0) sh.wave_last[wave] = last;
   __syncthreads();
-  uint64_t seen = upto - sum, total = 0;
-#pragma unroll
-  for (int i = 0; i < kRowWaves; ++i) {
-    if (i < wave) seen += sh.wave_sum[i];
-    total += sh.wave_sum[i];
-  }
+  const uint64_t waves_upto = WaveInclScanU64(lane < kRowWaves ? sh.wave_sum[lane] : 0);
+  const uint64_t total = LastLane(waves_upto);
+  uint64_t seen = upto - sum + (wave > 0 ? Few::FromLane(waves_upto, wave - 1) : 0);
   const double weight = sh.weight_of_all;
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
@@ -989,11 +983,21 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
     }
     seen += w[c];
   }
-  if (total > place || tid != 0) return;
-  // rounding, u of 1, or weights of less than half a unit each, of which one is as near as another
-  uint64_t which = 0;
-  for (int i = 0; i < kRowWaves; ++i) which = max(which, sh.wave_last[i]);
-  const int32_t token = static_cast<int32_t>(which & 0x7FFFFFFFu) - 1;
+  if (total > place) return;  // all of the workgroup, or none
+  // rounding, u of 1, or weights of less than half a unit each, of which one is as near as another: the last kept one, those of
+  // some weight before all of none
+  uint32_t last = 0;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    if (kept[c]) last = max(last, (w[c] > 0 ? 0x80000000u : 0u) + static_cast<uint32_t>(at + c + 1));
+  }
+#pragma unroll
+  for (int by = 32; by > 0; by >>= 1) last = max(last, static_cast<uint32_t>(__shfl_xor(static_cast<int>(last), by, 64)));
+  if (lane == 0) sh.wave_last[wave] = last;
+  __syncthreads();
+  if (tid != 0) return;
+  for (int i = 0; i < kRowWaves; ++i) last = max(last, sh.wave_last[i]);
+  const int32_t token = static_cast<int32_t>(last & 0x7FFFFFFFu) - 1;
   a.tokens[row.r] = token;
   if (a.probs != nullptr) a.probs[row.r] = static_cast<float>(units.Of(row.LoadOne(token)) * unit / weight);
 }
