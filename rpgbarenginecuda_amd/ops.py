@@ -1157,26 +1157,36 @@ def build_rope_table_scaled(rot_dim: int, theta: float, n_pos: int, scaling: str
     return out
 
 
+_here_at: dict = {}  # by current device (None: not asked for): the functions for float32 and int32
+_tensor = None
+
+
 def _here(first):
     """(buffer, bytes, name) -> address for float32 and for int32 buffers of a call whose first is this, of which every
     tensor has to be on the current device: as _paged_addr's, a tensor that is in order passes few checks."""
-    torch = _t()
-    tensor, f32, i32 = torch.Tensor, torch.float32, torch.int32
-    index = _current_device() if type(first) is tensor and first.is_cuda else None
+    global _tensor
+    if _tensor is None:
+        _tensor = _t().Tensor
+    index = _current_device() if type(first) is _tensor and first.is_cuda else None
+    found = _here_at.get(index)
+    if found is None:
+        found = _here_at[index] = (_here_addr(index, _t().float32), _here_addr(index, _t().int32))
+    return found
 
-    def at(dtype):
-        def of(buf, nbytes: int, name: str):
-            if (type(buf) is tensor and buf.dtype is dtype and buf.get_device() == index and buf.nbytes >= nbytes
-                    and buf.is_contiguous()):
-                return buf.data_ptr()
-            addr = _addr(buf, nbytes, dtype, name)
-            if isinstance(buf, tensor) and buf.get_device() != _current_device():
-                raise RpgError(f"{name} is on {buf.device}, which is not the current device")
-            return addr
 
-        return of
+def _here_addr(index, dtype):
+    tensor = _tensor
 
-    return at(f32), at(i32)
+    def at(buf, nbytes: int, name: str):
+        if (type(buf) is tensor and buf.dtype is dtype and buf.get_device() == index and buf.nbytes >= nbytes
+                and buf.is_contiguous()):
+            return buf.data_ptr()
+        addr = _addr(buf, nbytes, dtype, name)
+        if isinstance(buf, tensor) and buf.get_device() != _current_device():
+            raise RpgError(f"{name} is on {buf.device}, which is not the current device")
+        return addr
+
+    return at
 
 
 def _current_device() -> int:
