@@ -325,7 +325,7 @@ __device__ __forceinline__ T LastLane(T x) {
 constexpr int kRowThreads = 1024;
 constexpr int kRowWaves = kRowThreads / 64;
 constexpr int kJoiners = kRowThreads / kBins;  // threads to a bin, each for every kJoiners-th slice
-constexpr int kDigitBits = 8;
+constexpr int kDigitBits = 9;  // a bin's keys differ in some 18 bits: two digits
 constexpr int kDigits = 1 << kDigitBits;
 
 struct ChooseShared {
@@ -416,7 +416,7 @@ __device__ __forceinline__ Cut Select(const Keys& keys, uint32_t n, uint32_t lea
                 static_cast<unsigned long long>(by_weight ? units.OfKey(key) : 1));
     }
     __syncthreads();
-    if (threadIdx.x < 64) {  // four digits to a lane, from the highest down
+    if (threadIdx.x < 64) {  // some digits to a lane, from the highest down
       uint64_t d[kDigits / 64], mine = 0;
 #pragma unroll
       for (int i = 0; i < kDigits / 64; ++i) {
@@ -518,6 +518,23 @@ __device__ __forceinline__ uint32_t BytesWithin(uint32_t bytes, uint32_t from4, 
   return (~((less & beyond4) | ((less | beyond4) & low)) & kHigh) >> 7;
 }
 
+// The same of those that are the byte repeated in of4: of a byte and it the exclusive or is 0, and then no sum of its lower
+// bits and 127 reaches the highest. (A third of the work; most cuts lie in one bin.)
+__device__ __forceinline__ uint32_t BytesEqual(uint32_t bytes, uint32_t of4) {
+  constexpr uint32_t kHigh = 0x80808080u;
+  const uint32_t x = bytes ^ of4;
+  return (~(((x & ~kHigh) + ~kHigh) | x) & kHigh) >> 7;
+}
+// Sixteen bits in order, of bytes that are in: sums of 1, 2, 4, ... for each.
+template <class F>
+__device__ __forceinline__ uint32_t BitsOf(const uint4& bytes, F in) {
+  const uint32_t low =
+      __builtin_amdgcn_udot4(in(bytes.x), 0x08040201u, __builtin_amdgcn_udot4(in(bytes.y), 0x80402010u, 0, false), false);
+  const uint32_t high =
+      __builtin_amdgcn_udot4(in(bytes.z), 0x08040201u, __builtin_amdgcn_udot4(in(bytes.w), 0x80402010u, 0, false), false);
+  return high << 8 | low;
+}
+
 // Grid: rows.
 __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleArgs a) {
   __shared__ ChooseShared sh;
@@ -568,7 +585,7 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
       sh.high = 0;
       sh.slice = 0x7FFFFFFF;
     }
-  } else if (wave < 5) {
+  } else if (wave < 1 + kDigits / 64) {
     sh.digits[tid - 64] = 0;
     if (tid < 64 + 3) sh.bin[tid - 64] = kBins - 1;
   }
@@ -729,16 +746,12 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
       const uint32_t from4 = static_cast<uint32_t>(from) * 0x01010101u;
       const uint32_t beyond4 = static_cast<uint32_t>(255 - (upto - from)) * 0x01010101u;
       uint32_t part[4];
+      if (upto == from) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        // sixteen bits in order, by sums of 1, 2, 4, ... for each byte that is in
-        const uint32_t low = __builtin_amdgcn_udot4(
-            BytesWithin(bytes[i].x, from4, beyond4), 0x08040201u,
-            __builtin_amdgcn_udot4(BytesWithin(bytes[i].y, from4, beyond4), 0x80402010u, 0, false), false);
-        const uint32_t high = __builtin_amdgcn_udot4(
-            BytesWithin(bytes[i].z, from4, beyond4), 0x08040201u,
-            __builtin_amdgcn_udot4(BytesWithin(bytes[i].w, from4, beyond4), 0x80402010u, 0, false), false);
-        part[i] = high << 8 | low;
+        for (int i = 0; i < 4; ++i) part[i] = BitsOf(bytes[i], [&](uint32_t x) { return BytesEqual(x, from4); });
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) part[i] = BitsOf(bytes[i], [&](uint32_t x) { return BytesWithin(x, from4, beyond4); });
       }
       uint64_t takes = static_cast<uint64_t>(part[3] << 16 | part[2]) << 32 | (part[1] << 16 | part[0]);
       const int32_t at = s * kSlice + 64 * lane;
