@@ -325,8 +325,17 @@ __device__ __forceinline__ T LastLane(T x) {
 constexpr int kRowThreads = 1024;
 constexpr int kRowWaves = kRowThreads / 64;
 constexpr int kJoiners = kRowThreads / kBins;  // threads to a bin, each for every kJoiners-th slice
-constexpr int kDigitBits = 9;  // a bin's keys differ in some 18 bits: two digits
+// A bin's keys differ in some 19 bits. (128 rows of 2300 candidates: 23.8 us with digits of 7 or 8 bits, 24.6 with 9, 25.5
+// with 10, which one wave sums up.)
+constexpr int kDigitBits = 8;
 constexpr int kDigits = 1 << kDigitBits;
+constexpr int kLaneDigits = kDigits / 64;
+static_assert(kDigits <= kRowThreads && kDigits % 64 == 0, "");
+// Where digit d's amount is: from the highest down kLaneDigits to a lane, a lane's beside the next lane's.
+__device__ __forceinline__ uint32_t DigitAt(uint32_t d) {
+  const uint32_t down = kDigits - 1 - d;
+  return down % kLaneDigits * 64 + down / kLaneDigits;
+}
 
 struct ChooseShared {
   union {
@@ -412,25 +421,25 @@ __device__ __forceinline__ Cut Select(const Keys& keys, uint32_t n, uint32_t lea
     for (uint32_t i = threadIdx.x; i < n; i += kRowThreads) {
       const uint32_t key = keys[i], part = key - least;
       if (key < cut.key || (!first && (part >> width) != prefix)) continue;
-      atomicAdd(reinterpret_cast<unsigned long long*>(&sh.digits[kDigits - 1 - ((part >> shift) & (kDigits - 1))]),
+      atomicAdd(reinterpret_cast<unsigned long long*>(&sh.digits[DigitAt((part >> shift) & (kDigits - 1))]),
                 static_cast<unsigned long long>(by_weight ? units.OfKey(key) : 1));
     }
     __syncthreads();
     if (threadIdx.x < 64) {  // some digits to a lane, from the highest down
-      uint64_t d[kDigits / 64], mine = 0;
+      uint64_t d[kLaneDigits], mine = 0;
 #pragma unroll
-      for (int i = 0; i < kDigits / 64; ++i) {
-        d[i] = sh.digits[kDigits / 64 * threadIdx.x + i];
-        sh.digits[kDigits / 64 * threadIdx.x + i] = 0;
+      for (int i = 0; i < kLaneDigits; ++i) {
+        d[i] = sh.digits[64 * i + threadIdx.x];
+        sh.digits[64 * i + threadIdx.x] = 0;
         mine += d[i];
       }
       const uint64_t upto = WaveInclScanU64(mine);
       if (first) goal = min(goal, LastLane(upto));
       uint64_t before = upto - mine;
 #pragma unroll
-      for (int i = 0; i < kDigits / 64; ++i) {
+      for (int i = 0; i < kLaneDigits; ++i) {
         if (before < goal && goal <= before + d[i]) {
-          sh.found[0] = static_cast<uint64_t>(kDigits - 1 - (kDigits / 64 * threadIdx.x + i));
+          sh.found[0] = static_cast<uint64_t>(kDigits - 1 - (kLaneDigits * threadIdx.x + i));
           sh.found[1] = goal - before;
         }
         before += d[i];
@@ -585,10 +594,10 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
       sh.high = 0;
       sh.slice = 0x7FFFFFFF;
     }
-  } else if (wave < 1 + kDigits / 64) {
-    sh.digits[tid - 64] = 0;
-    if (tid < 64 + 3) sh.bin[tid - 64] = kBins - 1;
+  } else if (tid < 64 + 3) {
+    sh.bin[tid - 64] = kBins - 1;
   }
+  if (tid < kDigits) sh.digits[tid] = 0;
   __syncthreads();
   const float top = sh.top;
   if (top == -INFINITY || set.greedy) {
