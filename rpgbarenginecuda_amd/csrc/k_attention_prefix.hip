@@ -165,21 +165,23 @@ __device__ __forceinline__ T Afresh(T x) {
   return x;
 }
 
-// Whether row r, the lane's and its group's, begins with all of the group's pages; *seq its sequence.
-__device__ __forceinline__ bool BeginsWith(const PrefixArgs& a, int32_t r, int32_t pages, bool there, int32_t* seq) {
-  int32_t len = 0;
-  *seq = -1;
-  if (there) {
-    *seq = a.seq_ids != nullptr ? a.seq_ids[r] : r;
-    len = a.lens[r];
+// A row, the lane's, as asked for: requested apart from where it is looked at, so that other loads go out in between.
+struct AskedRow {
+  int32_t seq = -1, len = 0;
+  __device__ __forceinline__ AskedRow(const PrefixArgs& a, int32_t r, bool there) {
+    if (there) {
+      seq = a.seq_ids != nullptr ? a.seq_ids[r] : r;
+      len = a.lens[r];
+    }
   }
-  return there && *seq >= 0 && *seq < a.view.n_seqs && len >= 0 && len <= a.capacity &&
-         dev::TakesPart(pages, a.view.page_shift, len);
-}
-// The same of a row among those that group `of` names.
-__device__ __forceinline__ bool TakesPart(const PrefixArgs& a, const dev::SharedGroups& groups, int32_t r, int32_t of,
-                                          int32_t pages, bool there, int32_t* seq) {
-  return BeginsWith(a, r, pages, there && (groups.n == 1 || groups.OfLane(there ? r : -1) == of), seq);
+  // whether it begins with all of its group's pages
+  __device__ __forceinline__ bool BeginsWith(const PrefixArgs& a, int32_t pages) const {
+    return seq >= 0 && seq < a.view.n_seqs && len >= 0 && len <= a.capacity && dev::TakesPart(pages, a.view.page_shift, len);
+  }
+};
+// Whether r, among the rows that group `of` names, is its own: no earlier group's.
+__device__ __forceinline__ bool IsOf(const dev::SharedGroups& groups, int32_t r, int32_t of, bool there) {
+  return there && (groups.n == 1 || groups.OfLane(there ? r : -1) == of);
 }
 
 template <int D, bool kQ8>
@@ -304,10 +306,10 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
       raw[s][0] = dev::Load4(qr + (4 * s + g) * 8);
       raw[s][1] = dev::Load4(qr + (4 * s + g) * 8 + 4);
     }
-    int32_t seq;
-    there = TakesPart(args, groups, row, piece.of, piece.pages, a_column, &seq);
+    const AskedRow asked(args, row, a_column);
     load(loaded, c0, page_of(c0));
     next_page = page_of(c0 + 1);
+    there = IsOf(groups, row, piece.of, a_column) && asked.BeginsWith(args, piece.pages);
     float x[kSteps][8];
     float top = 0.0f;
 #pragma unroll
@@ -597,9 +599,10 @@ __global__ __launch_bounds__(kThreads, 2) void SharedPrefixKernel(const PrefixAr
     int32_t leader = -1;
 #pragma unroll 1
     for (int32_t r = piece.first_row; r < piece.last_row && leader < 0; r += 64) {
-      int32_t seq;
-      const uint64_t good = __ballot(TakesPart(args, units.groups, r + lane, of, piece.pages, r + lane < piece.last_row, &seq));
-      if (good != 0) leader = __builtin_amdgcn_readlane(seq, __builtin_ctzll(good));
+      const AskedRow asked(args, r + lane, r + lane < piece.last_row);
+      const uint64_t good =
+          __ballot(IsOf(units.groups, r + lane, of, r + lane < piece.last_row) && asked.BeginsWith(args, piece.pages));
+      if (good != 0) leader = __builtin_amdgcn_readlane(asked.seq, __builtin_ctzll(good));
     }
     if (leader < 0) continue;  // the same for every workgroup that has a part of the tile
     const int32_t* table = view.pages + static_cast<int64_t>(leader) * view.max_pages;
@@ -619,11 +622,19 @@ __global__ __launch_bounds__(kJoinThreads) void SharedJoinKernel(const PrefixArg
   const int32_t d = 4 * (threadIdx.x % kLanes);
   const int32_t row = static_cast<int32_t>(row_head / args.n_heads), head = static_cast<int32_t>(row_head % args.n_heads);
   const bool there = row < args.n_rows;
+  const AskedRow asked(args, row, there);
+  Own own{};
+  float4 own_o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float* const to = args.out + row_head * D + d;
+  if (there) {
+    own = OwnOf(args, row_head);
+    own_o = dev::Load4(to);
+  }
   const Units units(args, lane);
   if (units.sharers == 0) return;
   const int32_t in = units.groups.OfLane(there ? row : -1), of = max(in, 0);
-  int32_t seq;
-  const bool takes = BeginsWith(args, row, __shfl(units.groups.pages, of), there && in >= 0, &seq);
+  const int32_t pages = __shfl(units.groups.pages, of);
+  const bool takes = in >= 0 && asked.BeginsWith(args, pages);
   const uint32_t steps = __shfl(units.steps, of), tiles = __shfl(units.tiles, of);
   const uint32_t before = __shfl(units.upto - units.amount, of);
   const int32_t first_row = __shfl(units.groups.first, of);
@@ -636,9 +647,6 @@ __global__ __launch_bounds__(kJoinThreads) void SharedJoinKernel(const PrefixArg
   const uint32_t wa = share.HolderOfLane(first_unit);
   const uint32_t parts = share.HolderOfLane(first_unit + steps - 1) - wa + 1;
   if (parts == 1) return;  // joined where it was made
-  const Own own = OwnOf(args, row_head);
-  float* const to = args.out + row_head * D + d;
-  const float4 own_o = dev::Load4(to);
   const uint32_t first_slot = 2 * wa + (share.Begin(wa) == first_unit ? 0 : 1);
   const __amdgpu_buffer_rsrc_t rs = dev::OutResource(args.workspace, 2 * kGroups * SlotBytes(D));
   float top = -INFINITY, sum = 0.0f;
