@@ -24,9 +24,9 @@
 // What bounds it: 32 positions of 128 columns take a compute unit 2700 cycles, of which the matrix cores are busy for 1030
 // and vector arithmetic for 1360, by two waves that mostly wait for the same; 32 columns to a wave (half the reads of LDS)
 // and sixteen waves were no faster, and their code and joins cost the short pieces 4 us. Behind few columns it is memory
-// (4 TB/s), and for one or two steps the chain of groups, lengths, table, keys and the first pass through the code, 9 us.
+// (4 TB/s), and for one or two steps the chain of groups, lengths, table, keys and the first pass through the code, 8 us.
 // 128 rows and 4 heads to a kv head over 8192 positions in 8 bits 58 us (0.59 PFLOP/s of formed products), 8 rows over
-// 32768 26.5 us, 32 rows and 2 heads over 2816 in fp16 11.7 us.
+// 32768 26 us, 32 rows and 2 heads over 2816 in fp16 10.7 us.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
