@@ -681,10 +681,10 @@ __global__ __launch_bounds__(kJoinThreads) void SharedJoinKernel(const PrefixArg
 // The bytes of keys and values from which on it pays to share them, 144 MB and one more for each row. Three kernels instead
 // of one cost some 15 us, and 10 more for many rows, whose queries and outputs pass through two of them; the kernel of single
 // rows reads what neighbours have just read at some 6 TB/s. Shared against by themselves, us, at 96 / 128 / 160 / 192 / 256 MB
-// saved: 16 query and 8 kv heads of 128, fp16, 4 rows 27:30 32:36 34:42 31:48 40:60, 16 rows 24:18 25:29 26:29 27:31 30:44,
-// 64 rows 29:16 30:26 30:28 30:31 31:34, 128 rows 37:26 37:29 38:32 38:35 38:41; 32 and 8 heads in 8 bits, 4 rows 32:24 39:40
-// 42:43 41:50 50:67, 16 rows 29:20 33:27 35:28 36:35 37:45, 64 rows 33:18 33:27 34:29 35:31 35:35; 32 and 4 heads of 64,
-// fp16, 8 rows 32:19 32:33 32:34 35:44 40:54, 32 rows 26:18 30:24 31:25 32:29 33:37.
+// saved: 16 query and 8 kv heads of 128, fp16, 4 rows 27:30 32:36 33:42 31:48 38:60, 16 rows 23:18 25:29 25:28 26:32 28:44,
+// 64 rows 28:16 29:26 30:28 30:31 30:35, 128 rows 36:26 36:29 37:32 37:34 37:40; 32 and 8 heads in 8 bits, 4 rows 31:24 37:41
+// 39:44 39:52 46:67, 16 rows 28:20 32:28 33:28 34:35 35:46, 64 rows 31:18 32:27 32:29 33:31 34:34; 32 and 4 heads of 64,
+// fp16, 8 rows 32:19 32:34 32:34 33:43 38:54, 32 rows 25:17 29:24 30:24 32:29 32:37.
 int64_t LeastSaving(int64_t n_rows) { return (144 + n_rows) << 20; }
 
 size_t MlBytes(int32_t n_heads, int64_t n_rows) {
