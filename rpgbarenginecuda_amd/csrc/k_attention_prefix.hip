@@ -10,7 +10,8 @@
 // Keys and values are read once for up to 128 columns (the queries of a kv head: rows times heads of a group). Queries and
 // weights, which are fp32, enter the matrix cores as two fp16 terms of 11 bits each, together 22, so that each product runs
 // twice. Over 8-bit pages codes are fp16 numbers as they are; keys' scales multiply the scores, and weights times values'
-// scales are brought to fp16's range by a power of two of the column's, which moves with their maximum.
+// scales are brought to fp16's range by a power of two of the column's, relative to the largest yet and what that counts for
+// now: a row of a large scale that has lost its weight costs the others nothing.
 //
 // A workgroup takes steps of 128 positions through LDS, two of them at a time (one being read, one being filled), for a
 // tile of up to 128 columns; of its eight waves each has 16 columns and all of a step's keys, a half or a quarter of them
@@ -411,13 +412,18 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
       for (int i = 0; i < 4; ++i) top = fmaxf(top, s[j][i]);
     }
     top = MaxAcrossRows(top) * to_score;
-    if (__any(top > m + 4.0f)) {
+    const bool moves = __any(top > m + 4.0f);
+    float rise = 0.0f;  // of m, with its sign turned
+    if (moves) {
       const float to = top > m + 4.0f ? top : m;
-      const float back = __builtin_amdgcn_exp2f(m - (to == -INFINITY ? 0.0f : to));
+      rise = m - (to == -INFINITY ? 0.0f : to);
+      const float back = __builtin_amdgcn_exp2f(rise);
       m = to;
       l *= back;
+      if constexpr (!kQ8) {
 #pragma unroll
-      for (int i = 0; i < kE; ++i) acc[i] *= back;
+        for (int i = 0; i < kE; ++i) acc[i] *= back;
+      }
     }
     const float less = m == -INFINITY ? 0.0f : m - kUp;
     float p[2][4];
@@ -430,7 +436,9 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
       }
     }
     if constexpr (kQ8) {
-      // weights times scales, brought to fp16's range by a power of two that moves only where they pass it
+      // Weights times scales, brought to fp16's range by a power of two that rises with m and falls where they pass it, so
+      // that the largest yet, by what it counts for now, enters as 2^12 to 2^15. The two terms end at 2^-24: each is off by
+      // at most 2^-37 of that largest.
       float big = 0.0f;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -442,12 +450,12 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
         }
       }
       big = MaxAcrossRows(big);
-      if (__any(big * down > 0x1p15f)) {
-        const bool passes = big * down > 0x1p15f;
-        const int e = static_cast<int>(__float_as_uint(big) >> 23);  // brings big to [2^12, 2^13)
-        const float to = __uint_as_float(static_cast<uint32_t>(max(266 - e, 1)) << 23);
-        const float back = passes ? to / down : 1.0f;
-        down = passes ? to : down;
+      if (moves || __any(big * down > 0x1p15f)) {
+        const int from = static_cast<int>(__float_as_uint(down) >> 23);
+        int to = min(from + static_cast<int>(fminf(-rise, 300.0f)), 253);
+        if (ldexpf(big, to - 127) > 0x1p15f) to = max(266 - static_cast<int>(__float_as_uint(big) >> 23), 1);  // to [2^12, 2^13)
+        const float back = __builtin_amdgcn_exp2f(rise + static_cast<float>(to - from));
+        down = __int_as_float(to << 23);
 #pragma unroll
         for (int i = 0; i < kE; ++i) acc[i] *= back;
       }

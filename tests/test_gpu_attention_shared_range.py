@@ -1,0 +1,129 @@
+"""Attention of a batch that shares its beginnings, where values, scores, queries or keys differ widely in size: what the
+operator over rows by themselves is held to (test_gpu_attention_paged_range.py), at shared positions."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from paged_ref import F16, Q8, Pages, attention_within
+from test_gpu_attention_paged_range import hold, scored
+from test_gpu_attention_shared import attend
+
+pytestmark = pytest.mark.gpu
+
+
+def shared(gpu, kind, q, ks, vs, copies, page=16):
+    """Rows q [n, heads, d] over sequences of keys ks[i] and values vs[i], each asked for `copies` times: a group of as many
+    rows, which shares all whole pages. Outputs [n, copies, heads, d], and the pages."""
+    lens = [len(k) for k in ks]
+    n, d, n_kv = len(lens), q.shape[-1], ks[0].shape[1]
+    pages = Pages(np.random.default_rng(1), kind, n_kv, d, page, lens)
+    for i, (k, v) in enumerate(zip(ks, vs)):
+        hold(pages, i, k, v)
+    kv, table = pages.device(gpu)
+    seqs = np.repeat(np.arange(n), copies)
+    got = attend(gpu, kv, table, np.repeat(lens, copies), np.arange(n + 1) * copies, [m // page for m in lens],
+                 np.repeat(np.asarray(q, np.float32), copies, 0), seq_ids=seqs)
+    return got.reshape(n, copies, *q.shape[1:]), pages
+
+
+def check(gpu, kind, q, ks, vs, copies, page=16):
+    got, pages = shared(gpu, kind, q, ks, vs, copies, page)
+    for r in range(len(ks)):
+        n = len(ks[r])
+        want, limit = attention_within(q[r], pages.rows("k", r, n), pages.rows("v", r, n), kind)
+        worst = (np.abs(got[r] - want).max(0) / np.maximum(limit, 1e-300)).max()
+        assert worst <= 1, (r, n)
+    return got
+
+
+# heads of one kv head, d, copies: tiles of up to 16, 32, 64 and 128 columns, of which a wave takes 32, 32, 64 and 128 keys of
+# a step in turn
+TILES = [(4, 128, 1), (4, 64, 8), (8, 128, 8), (8, 64, 16), (4, 128, 40)]
+
+
+@pytest.mark.parametrize("d", [128, 64])
+@pytest.mark.parametrize("rows,group", [(4, 4), (8, 4), (16, 4), (32, 4)])
+def test_large_value_rows_of_early_keys(gpu, rows, group, d):
+    """Value rows 2^R larger than the others, of scores R + 12 octaves lower, in every second step of 128 positions and in
+    the first 32 positions of the others: they come first, and count for a 2^-12th. There are more units than workgroups, so
+    that a wave meets steps of both kinds."""
+    rng = np.random.default_rng(rows + d)
+    n_kv, n, page = 64, 768, 16
+    pages = Pages(rng, Q8, n_kv, d, page, [n], spare=0)
+    pos = np.arange(n)
+    early = (pos // 128 % 2 == 0) | (pos % 128 < 32)
+    k, v = rng.normal(0, 0.1, (n, n_kv, d)), rng.normal(0, 1, (n, n_kv, d))
+    k[early] = 0
+    k[early, :, 0] = -1
+    hold(pages, 0, k, v)
+    p, s = pages.table[0, pos // page], pos % page
+    ks, vs = pages.ks.copy(), pages.vs.copy()
+    q = rng.normal(0, 0.1, (rows, n_kv * group, d)).astype(np.float32)
+    q[:, :, 0] = 4
+    for octaves in (0, 20, 28, 36, 44, 60):
+        pages.ks, pages.vs = ks.copy(), vs.copy()
+        pages.ks[p[early], :, s[early]] *= np.float32((octaves + 12) * np.log(2) * np.sqrt(d) / 4)
+        pages.vs[p[early], :, s[early]] *= np.float32(2.0 ** octaves)
+        kv, table = pages.device(gpu)
+        got = attend(gpu, kv, table, [n] * rows, [0, rows], [n // page], q, seq_ids=[0] * rows)
+        kk, vv = pages.rows("k", 0, n), pages.rows("v", 0, n)
+        for h in (0, 7, 20, 41, 63):
+            at = slice(h * group, (h + 1) * group)
+            for r in (0, rows // 2, rows - 1):
+                want, limit = attention_within(q[r, at], kk[:, h:h + 1], vv[:, h:h + 1], Q8)
+                worst = (np.abs(got[r, at] - want) / limit).max()
+                assert worst <= 1, (octaves, h, r)
+
+
+@pytest.mark.parametrize("heads,d,copies", TILES)
+def test_scores_and_sizes_that_move_together(gpu, heads, d, copies):
+    """Scores that rise or fall along the row by 40, against value rows whose sizes fall or rise as much, or twice as
+    much; rows of zeros first, last, and everywhere."""
+    rng = np.random.default_rng(heads * d + copies)
+    q1 = rng.normal(0, 1, d).astype(np.float32)
+    n = 896
+    up = np.linspace(0, 40, n)
+    ks, vs = [], []
+    for s, by in ((up, -up), (up[::-1], -up[::-1]), (up, -2 * up), (up[::-1], up), (up, up), (up, 0 * up), (up[::-1], 0 * up)):
+        ks.append(scored(rng, q1, s))
+        vs.append(rng.normal(0, 1, (n, 1, d)) * np.exp(by)[:, None, None])
+    for zero in (slice(0, 200), slice(700, n), slice(0, n)):
+        v = rng.normal(0, 1, (n, 1, d))
+        v[zero] = 0
+        ks.append(scored(rng, q1, up / 10))
+        vs.append(v)
+    got = check(gpu, Q8, np.repeat(q1[None, None], len(ks), 0).repeat(heads, 1), ks, vs, copies)
+    assert np.all(got[-1] == 0)
+
+
+@pytest.mark.parametrize("heads,d,copies", TILES)
+def test_a_large_row_of_no_weight(gpu, heads, d, copies):
+    """One value row far larger than all others, of no weight or of a weight that makes it count as much as they do, in
+    the first, a middle and the last position."""
+    rng = np.random.default_rng(heads + d + copies)
+    cases = [(size, at, n) for size in (1e3, 1e6, 1e9, 1e30) for at in (0, 70, -1) for n in (128, 512)]
+    q1 = rng.normal(0, 1, d).astype(np.float32)
+    q = np.repeat(q1[None], len(cases), 0)[:, None] * (1 + 0.01 * rng.normal(0, 1, (len(cases), heads, 1)))
+    for score in (-150.0, -60.0, None):
+        ks, vs = [], []
+        for size, at, n in cases:
+            s = rng.normal(0, 1, n)
+            s[at] = -np.log(size) if score is None else score
+            v = rng.normal(0, 1, (n, 1, d))
+            v[at] *= size
+            ks.append(scored(rng, q1, s))
+            vs.append(v)
+        check(gpu, Q8, q.astype(np.float32), ks, vs, copies)
+
+
+@pytest.mark.parametrize("heads,d,copies", TILES)
+@pytest.mark.parametrize("exponent", [-119, -100, 60, 105])
+def test_values_all_small_or_all_large(gpu, heads, d, copies, exponent):
+    """Rows whose scales all lie near one power of two, down to the smallest normal ones."""
+    rng = np.random.default_rng(heads + 1000 + exponent)
+    lens = [16, 100, 704]
+    ks = [rng.normal(0, 1, (n, 1, d)) for n in lens]
+    vs = [rng.normal(0, 1, (n, 1, d)) * 2.0 ** exponent for n in lens]
+    got = check(gpu, Q8, rng.normal(0, 1, (3, heads, d)).astype(np.float32), ks, vs, copies)
+    assert np.all(np.abs(got).max(-1) > 0.02 * 2.0 ** exponent)
