@@ -341,7 +341,7 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
     for (int i = 0; i < kE; ++i) acc[i] = F32x4{0.0f, 0.0f, 0.0f, 0.0f};
     m = -INFINITY;
     l = 0.0f;
-    down = kQ8 ? 0x1p126f : 1.0f;
+    down = kQ8 ? 0x1p126f : 0x1p11f;
   }
 
   // ---- two tiles of 16 keys, from tile `from` of a step, against 16 columns
@@ -402,20 +402,20 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
       }
     }
     // Weights are relative to a maximum that moves only where a score exceeds it by 4 (a factor of 16). Over fp16 values
-    // they come multiplied by 2^11: with the 16, fp16's largest, and what its low end loses is below 2^-35.
-    constexpr float kUp = kQ8 ? 0.0f : 11.0f;
+    // they enter multiplied by 2^11: with the 16, half of fp16's largest, and what its low end loses is below 2^-35.
     uint32_t w[2][4];
+    float by = to_score;
     float top = s[0][0];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) top = fmaxf(top, s[j][i]);
     }
-    top = MaxAcrossRows(top) * to_score;
-    const bool moves = __any(top > m + 4.0f);
+    top = MaxAcrossRows(top) * by;
+    const bool moves = __any(top - m > 4.0f);
     float rise = 0.0f;  // of m, with its sign turned
     if (moves) {
-      const float to = top > m + 4.0f ? top : m;
+      const float to = top - m > 4.0f ? top : m;
       rise = m - (to == -INFINITY ? 0.0f : to);
       const float back = __builtin_amdgcn_exp2f(rise);
       m = to;
@@ -425,13 +425,20 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
         for (int i = 0; i < kE; ++i) acc[i] *= back;
       }
     }
-    const float less = m == -INFINITY ? 0.0f : m - kUp;
+    // m is a score as rounded. From 2^22 on, where the rounding is half an octave and more, the others are rounded too: not
+    // rounded, their weights could pass what they have room for.
+    if (__builtin_expect(__any(fabsf(m) >= 0x1p22f), 0)) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) s[j] *= by;
+      by = 1.0f;
+    }
+    const float less = m == -INFINITY ? 0.0f : m;
     float p[2][4];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        p[j][i] = __builtin_amdgcn_exp2f(fmaf(s[j][i], to_score, -less));
+        p[j][i] = __builtin_amdgcn_exp2f(fmaf(s[j][i], by, -less));
         l += p[j][i];
       }
     }
@@ -500,8 +507,8 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
   const auto join_at = [&](int from) {
     return joins + ((from - 1) * (col_waves * kWaveCols) + col_wave * kWaveCols + n) * kPart;
   };
-  l = SumAcrossRows(l) * (kQ8 ? 1.0f : 0x1p-11f);
-  const float by = kQ8 ? 1.0f / down : 0x1p-11f;
+  l = SumAcrossRows(l);
+  const float by = 1.0f / down;
 #pragma unroll
   for (int i = 0; i < kE; ++i) acc[i] *= by;
   if (works && key_wave > 0) {

@@ -127,3 +127,29 @@ def test_values_all_small_or_all_large(gpu, heads, d, copies, exponent):
     vs = [rng.normal(0, 1, (n, 1, d)) * 2.0 ** exponent for n in lens]
     got = check(gpu, Q8, rng.normal(0, 1, (3, heads, d)).astype(np.float32), ks, vs, copies)
     assert np.all(np.abs(got).max(-1) > 0.02 * 2.0 ** exponent)
+
+
+@pytest.mark.parametrize("kind", [F16, Q8])
+@pytest.mark.parametrize("heads,d,copies", TILES)
+def test_scores_of_any_size(gpu, heads, d, copies, kind):
+    """Scores of 2^23 to 2^100 octaves: every second key has the score S, of bits that are the same in all of them, the
+    others S / 2. Those of the higher score count alike and the rest for nothing, so that the output is the mean of their
+    values, to within n + 64 roundings, the weights' and values' own (8) and, over 8-bit pages, 2^-24 of what it is made of."""
+    rng = np.random.default_rng(heads + d + copies)
+    exponents = [23.0, 25.3, 26.6, 27.5, 28.2, 31.5, 40.0, 60.0, 100.0]
+    k0 = rng.normal(0, 1, d).astype(np.float32)
+    n, own = 384, 5
+    odd = np.arange(n) % 2 == 1
+    k = np.where(odd[:, None], k0, k0 / 2)[:, None]
+    cases = []  # keys, values, the positions that count, the exponent
+    for e in exponents:
+        for sign, behind in ((1, 0), (-1, 0), (1, own), (-1, own)):
+            best = np.flatnonzero(odd if sign > 0 else ~odd) if sign > 0 or not behind else np.arange(n, n + own)
+            cases.append((np.concatenate([sign * k, np.zeros((behind, 1, d))]), rng.normal(0, 1, (n + behind, 1, d)), best, e))
+    by = np.array([2.0 ** c[3] * np.sqrt(d) / (float(k0.astype(np.float64) @ k0) * np.log2(np.e)) for c in cases])
+    q = by[:, None, None] * k0 * (1 + np.arange(heads)[:, None] / 16)
+    got, pages = shared(gpu, kind, q, [c[0] for c in cases], [c[1] for c in cases], copies)
+    for r, (k, v, best, e) in enumerate(cases):
+        v = pages.rows("v", r, len(k))[best, 0]
+        worst = np.abs(got[r] - v.mean(0)).max() / ((n + own + 64 + 8 + 1) * 2.0 ** -24 * np.abs(v).max(-1).mean())
+        assert worst <= 1, (e, r % 4)
