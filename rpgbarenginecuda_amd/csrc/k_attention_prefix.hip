@@ -341,7 +341,7 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
     for (int i = 0; i < kE; ++i) acc[i] = F32x4{0.0f, 0.0f, 0.0f, 0.0f};
     m = -INFINITY;
     l = 0.0f;
-    down = kQ8 ? 0x1p126f : 0x1p11f;
+    down = kQ8 ? 0x1p126f : 0x1p14f;
   }
 
   // ---- two tiles of 16 keys, from tile `from` of a step, against 16 columns
@@ -401,8 +401,9 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
         if (j >= valid) s[j] = F32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
       }
     }
-    // Weights are relative to a maximum that moves only where a score exceeds it by 4 (a factor of 16). Over fp16 values
-    // they enter multiplied by 2^11: with the 16, half of fp16's largest, and what its low end loses is below 2^-35.
+    // Weights are relative to a maximum that moves only where a score exceeds it by 4 (a factor of 16), over fp16 values by
+    // 1: there they enter multiplied by 2^14, with the factor half of fp16's largest, and the low end loses less than 2^-38.
+    constexpr float kLag = kQ8 ? 4.0f : 1.0f;
     uint32_t w[2][4];
     float by = to_score;
     float top = s[0][0];
@@ -412,10 +413,10 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
       for (int i = 0; i < 4; ++i) top = fmaxf(top, s[j][i]);
     }
     top = MaxAcrossRows(top) * by;
-    const bool moves = __any(top - m > 4.0f);
+    const bool moves = __any(top - m > kLag);
     float rise = 0.0f;  // of m, with its sign turned
     if (moves) {
-      const float to = top - m > 4.0f ? top : m;
+      const float to = top - m > kLag ? top : m;
       rise = m - (to == -INFINITY ? 0.0f : to);
       const float back = __builtin_amdgcn_exp2f(rise);
       m = to;

@@ -153,3 +153,22 @@ def test_scores_of_any_size(gpu, heads, d, copies, kind):
         v = pages.rows("v", r, len(k))[best, 0]
         worst = np.abs(got[r] - v.mean(0)).max() / ((n + own + 64 + 8 + 1) * 2.0 ** -24 * np.abs(v).max(-1).mean())
         assert worst <= 1, (e, r % 4)
+
+
+@pytest.mark.parametrize("exponent", [-30.4, -33.4, -35.6, -37.4])
+@pytest.mark.parametrize("kind", [F16, Q8])
+@pytest.mark.parametrize("heads,d,copies", TILES)
+def test_small_weights_that_are_all_alike(gpu, heads, d, copies, kind, exponent):
+    """One weight of 1 and all others of 2^exponent, in elements of their own: what is rounded in one is rounded in all."""
+    q = np.zeros((2, heads, d), np.float32)
+    q[..., 0] = np.sqrt(d)
+    ks, vs = [], []
+    for n in (128, 1024):
+        k, v = np.zeros((n, 1, d)), np.zeros((n, 1, d))
+        k[:, :, 0] = exponent * np.log(2)
+        k[77] = 0
+        v[:, :, d // 2:] = 1
+        v[77] = np.concatenate([np.ones(d // 2), np.zeros(d // 2)])
+        ks.append(k)
+        vs.append(v)
+    check(gpu, kind, q, ks, vs, copies)
