@@ -128,13 +128,16 @@ struct Piece {
   bool leads;  // the first thing that the workgroup does
 };
 
+// Products of queries' and keys' codes, below 2^29, times scales up to this stay in fp32's range.
+constexpr float kFarScale = 0x1p60f;
+
 template <int D, bool kQ8>
 struct Stage {
   static constexpr int kRow = 2 * D;
   alignas(16) char k[kStep * kRow];
   alignas(16) char v[kStep * kRow];
   float k_scale[kQ8 ? kStep : 4], v_scale[kQ8 ? kStep : 4];
-  uint32_t bad[kStep / 16];  // pages out of range
+  uint32_t bad[kStep / 16];  // 1: pages out of range, 2: keys' scales past kFarScale
 };
 
 // The groups' units, a group to a lane: those of kv head, column tile and step count up, in this order.
@@ -274,6 +277,7 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
       }
     }
     if constexpr (kQ8) {
+      from.bad |= __any(fabsf(from.k_scale) > kFarScale) ? 2 : 0;
       if (own < 16) {
         st.k_scale[16 * wave + own] = from.k_scale;
         st.v_scale[16 * wave + own] = from.v_scale;
@@ -288,6 +292,7 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
   const int col_wave = wave % col_waves, key_wave = wave / col_waves;
   const bool works = key_wave < key_waves && col_wave * kWaveCols < piece.cols;
   float to_score, m, l;
+  int q_exp;  // 8 bits: the power of two that to_score gives back to queries
   float down;  // the power of two that weights enter multiplied by
   F32x4 acc[kE];
   Half8 q_hi[kSteps], q_lo[kSteps];
@@ -326,9 +331,23 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
       }
     }
     top = MaxAcrossRows(top);
+    q_exp = 127;
+    if constexpr (kQ8) {  // keys of 8 bits may make scores of queries that 2^127 does not bring to [2^14, 2^15)
+      if (__any(top < 0x1p-112f)) {
+        const float first = top < 0x1p-112f ? 0x1p40f : 1.0f;
+        q_exp = top < 0x1p-112f ? 127 - 40 : 127;
+        top *= first;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[s][i] *= first;
+        }
+      }
+    }
     const int e = min(max(268 - (__float_as_int(top) >> 23), 1), 254);  // brings top to [2^14, 2^15)
     const float up = __int_as_float(e << 23);
-    to_score = ldexpf(args.scale_log2, 127 - e);
+    q_exp -= e;
+    to_score = ldexpf(args.scale_log2, max(q_exp, -140));  // below, scores of scales up to kFarScale count for nothing
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       Terms w[4];
@@ -385,27 +404,40 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
       v[i][1] = ReadHalvesAcross(at + 16 * kRow);
     }
     __builtin_amdgcn_sched_barrier(0);
-    const uint32_t bad = Scalar(bads[0] | bads[1] << 1);
+    const uint32_t bad = Scalar(bads[0] | bads[1] << 2);
+    float by = to_score;  // what makes scores of s
+    if (__builtin_expect(valid < 2 || bad != 0, 0)) {
+      if constexpr (kQ8) {
+        if (bad & 10) {  // small queries' power of two goes to the scales
+          const int first = min(q_exp, 0);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            ks[j] = make_float4(ldexpf(ks[j].x, first), ldexpf(ks[j].y, first), ldexpf(ks[j].z, first), ldexpf(ks[j].w, first));
+          }
+          by = ldexpf(args.scale_log2, q_exp - first);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (bad >> (2 * j) & 1) s[j] = F32x4{NAN, NAN, NAN, NAN};
+        if (j >= valid) {
+          s[j] = F32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          if constexpr (kQ8) ks[j] = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+        }
+      }
+    }
     if constexpr (kQ8) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const float by[4] = {ks[j].x, ks[j].y, ks[j].z, ks[j].w};
+        const float scales[4] = {ks[j].x, ks[j].y, ks[j].z, ks[j].w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[j][i] *= by[i];
-      }
-    }
-    if (__builtin_expect(valid < 2 || bad != 0, 0)) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        if (bad >> j & 1) s[j] = F32x4{NAN, NAN, NAN, NAN};
-        if (j >= valid) s[j] = F32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        for (int i = 0; i < 4; ++i) s[j][i] *= scales[i];
       }
     }
     // Weights are relative to a maximum that moves only where a score exceeds it by 4 (a factor of 16), over fp16 values by
     // 1: there they enter multiplied by 2^14, with the factor half of fp16's largest, and the low end loses less than 2^-38.
     constexpr float kLag = kQ8 ? 4.0f : 1.0f;
     uint32_t w[2][4];
-    float by = to_score;
     float top = s[0][0];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {

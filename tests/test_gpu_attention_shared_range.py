@@ -172,3 +172,34 @@ def test_small_weights_that_are_all_alike(gpu, heads, d, copies, kind, exponent)
         ks.append(k)
         vs.append(v)
     check(gpu, kind, q, ks, vs, copies)
+
+
+@pytest.mark.parametrize("heads,d,copies", TILES)
+def test_queries_and_keys_far_from_one(gpu, heads, d, copies):
+    """Queries of 2^e and 8-bit keys of 2^-e, and down to 2^-20 of that: scores of ordinary size, between queries whose
+    products with one code pass fp32's range on either side."""
+    rng = np.random.default_rng(heads * d + 3)
+    exponents, n = [118, 100, 60, -60, -80, -100, -110, -125], 208
+    sizes = 2.0 ** rng.integers(-20, 1, (n, 1, 1))
+    sizes[rng.permutation(n)[:60]] = 1
+    ks = [rng.normal(0, 1, (n, 1, d)) * sizes ** (e < 0) * 2.0 ** -e for e in exponents]
+    vs = [rng.normal(0, 1, (n, 1, d)) for _ in exponents]
+    q = rng.normal(0, 1, (len(exponents), heads, d)) * 2.0 ** np.array(exponents, np.float64)[:, None, None]
+    q[0, 0] = 0
+    q[1, 1] *= 2.0 ** -140  # beside heads of another size
+    check(gpu, Q8, q.astype(np.float32), ks, vs, copies)
+
+
+@pytest.mark.parametrize("heads,d,copies", TILES)
+@pytest.mark.parametrize("of_q,of_k", [(120, 100), (-10, 125), (-120, 125), (120, -100)])
+def test_large_queries_and_keys_in_elements_apart(gpu, heads, d, copies, of_q, of_k):
+    """Queries in one half of the elements and 8-bit keys in the other: every score is 0, every weight 1 / n, and the outputs
+    are the values' means to within n + 64 roundings and the values' own rounding to 2^-24."""
+    rng = np.random.default_rng(heads + d + 4)
+    n = 144
+    k, q = np.zeros((n, 1, d)), np.zeros((1, heads, d), np.float32)
+    k[:, :, d // 2:] = rng.normal(0, 1, (n, 1, d // 2)) * 2.0 ** of_k
+    q[:, :, :d // 2] = rng.normal(0, 1, (1, heads, d // 2)) * 2.0 ** of_q
+    got, pages = shared(gpu, Q8, q, [k], [rng.normal(0, 1, (n, 1, d))], copies)
+    v = pages.rows("v", 0, n)[:, 0]
+    assert np.abs(got[0] - v.mean(0)).max() <= (n + 64 + 2) * 2.0 ** -24 * np.abs(v).max(-1).mean()
