@@ -677,8 +677,10 @@ __global__ __launch_bounds__(kRowThreads) void SampleChooseKernel(const SampleAr
       __syncthreads();
     }
     const int p_hi = static_cast<int>(sh.bin[1]), p_lo = static_cast<int>(sh.bin[2]);
-    // min_p's: that of the nearest number to its border, and the next in either direction, where the border's rounding (the
-    // hardware's logarithm is within 2^-20 of an octave here, a bin an eighth of one) and its number's may have it
+    // min_p's: that of the nearest number to its border, and the next in either direction, where the border's rounding and its
+    // number's may have it. The hardware's logarithm is within 2^-23 of its value from 2^-40 to 1, and a border further than
+    // all bins, 32 octaves or (T above 1) 22 logits below the largest, is in the last: any other is off by at most 2^-18
+    // octaves or logits, of which a bin is an eighth and a twelfth, at any temperature
     int m_hi = kBins - 1, m_lo = kBins - 1;
     if (on_m) {
       const double octaves = static_cast<double>(__builtin_amdgcn_logf(set.m));
