@@ -431,7 +431,7 @@ struct SharedAttentionArgs : AttentionArgs {
   const int32_t* group_rows;
   const int32_t* group_pages;
   int32_t n_groups;
-  uint32_t least;
+  int64_t least;
   float* ml;
 };
 
@@ -1408,7 +1408,7 @@ void AttendPaged(const GpuPagedKv& kv, const GpuPageTable& table, const int32_t*
                            n_heads / kv.n_kv_heads, tiles, tile_heads, scale_log2};
   const dim3 grid(static_cast<unsigned>(groups)), block(64 * kWaves);
   // what a group of all rows with all of their pages would save, at the most
-  if (prefix == nullptr || prefix->n_groups == 0 || (n_rows - 1) * std::min<int64_t>(table.max_pages, kMostSaving) < prefix->least) {
+  if (prefix == nullptr || prefix->n_groups == 0 || (n_rows - 1) * std::min<int64_t>(table.max_pages, 0x7FFFFFFF) < prefix->least) {
     Launch("PagedAttentionKernel", KernelFor<AttentionArgs>(kv, tile_heads), grid, block, args);
     return;
   }

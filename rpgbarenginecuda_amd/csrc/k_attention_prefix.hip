@@ -793,7 +793,7 @@ void GpuAttentionPagedShared(const GpuPagedKv& kv, const GpuPageTable& table, co
   const int64_t row = int64_t{kv.type == kKvQ8 ? kv.head_dim + 4 : 2 * kv.head_dim} * 2;  // a position's of a kv head
   const int64_t page = std::max<int64_t>(row * std::max(kv.page_size, 1) * std::max(kv.n_kv_heads, 1), 1);
   const int64_t least = least_saving / page + (least_saving % page != 0 ? 1 : 0);
-  PagedPrefix prefix{group_rows, group_pages, n_groups, static_cast<uint32_t>(std::min<int64_t>(least, kMostSaving))};
+  PagedPrefix prefix{group_rows, group_pages, n_groups, std::min(least, kMostSaving)};
   AttendPaged(kv, table, seq_ids, lens, q_dev, n_heads, n_rows, out_dev, workspace, workspace_bytes, &prefix);
 }
 

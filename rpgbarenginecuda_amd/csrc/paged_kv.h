@@ -29,11 +29,11 @@ struct PagedPrefix {
   const int32_t* group_rows;
   const int32_t* group_pages;
   int32_t n_groups;
-  uint32_t least = 0;  // pages times rows that sharing has to save, at most kMostSaving
+  int64_t least = 0;  // pages times rows that sharing has to save, at most kMostSaving
   char* workspace = nullptr;
   float* ml = nullptr;
 };
-constexpr uint32_t kMostSaving = 1u << 25;  // of a group: what exceeds it counts as this
+constexpr int64_t kMostSaving = int64_t(1) << 50;  // of a group: what exceeds it counts as this
 
 // GpuAttentionPaged, of what is behind the shared positions if there is a prefix (and then of the rest).
 void AttendPaged(const GpuPagedKv& kv, const GpuPageTable& table, const int32_t* seq_ids, const int32_t* lens,
@@ -103,7 +103,7 @@ struct SharedGroups {
   int32_t first = 0, last = 0, pages = 0;
 
   __device__ __forceinline__ SharedGroups(const int32_t* group_rows, const int32_t* group_pages, int32_t n_groups,
-                                          uint32_t least, int32_t n_rows, int64_t max_pages, int lane)
+                                          int64_t least, int32_t n_rows, int64_t max_pages, int lane)
       : n(n_groups) {
     if (lane < n_groups) {
       first = min(max(group_rows[lane], 0), n_rows);
@@ -111,9 +111,11 @@ struct SharedGroups {
       const int32_t p = group_pages[lane];
       pages = p > 0 && p <= max_pages ? p : 0;
     }
-    const uint64_t saving = last > first ? static_cast<uint64_t>(last - first - 1) * static_cast<uint32_t>(pages) : 0;
-    const uint32_t all = attn::ScanAdd(static_cast<uint32_t>(saving < kMostSaving ? saving : kMostSaving));
-    if (static_cast<uint32_t>(__builtin_amdgcn_readlane(all, 63)) < least) pages = 0;
+    const int64_t rows_less_one = last > first ? last - first - 1 : 0, saving = min(rows_less_one * pages, kMostSaving);
+    const uint32_t high = attn::ScanAdd(static_cast<uint32_t>(saving >> 25));  // in two parts, of 25 bits each
+    const uint32_t low = attn::ScanAdd(static_cast<uint32_t>(saving) & ((1u << 25) - 1));
+    const uint32_t high_all = __builtin_amdgcn_readlane(high, 63), low_all = __builtin_amdgcn_readlane(low, 63);
+    if ((static_cast<int64_t>(high_all) << 25) + low_all < least) pages = 0;
   }
   // The group of row r, the lane's; -1 if there is none.
   __device__ __forceinline__ int32_t OfLane(int32_t r) const {

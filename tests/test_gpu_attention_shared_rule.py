@@ -1,4 +1,4 @@
-"""Whether a batch shares its beginnings, at the border that callers get: told by a page out of
+"""Whether a batch shares its beginnings, at the border that callers get and at borders of any size: told by a page out of
 range in the table of a row that is not its group's first, which is looked at only where rows are by themselves."""
 from __future__ import annotations
 
@@ -44,3 +44,19 @@ def test_the_default_border(gpu, kind, enough, padding):
         for r in range(2 if together else 1):
             want, limit = attention_within(q[r, 2 * h:2 * h + 2], k[:, None], v[:, None], kind)
             assert (np.abs(got[r, 2 * h:2 * h + 2] - want) / limit).max() <= 1, (n, r)
+
+
+@pytest.mark.parametrize("rows", [4097, (1 << 19) + 1])
+def test_borders_past_32_bits(gpu, rows):
+    """As many rows by 8192 pages of 4 KB: a border of just what they save, a byte more, and any that is larger."""
+    rng = np.random.default_rng(rows)
+    n, page, d = 8192, 16, 64
+    pages, _ = behind(rng, F16, 1, d, page, n + 10)
+    kv, table = pages.device(gpu)
+    q = rng.normal(0, 1, (rows, 1, d)).astype(np.float32)
+    lens = np.full(rows, 1)
+    lens[:2] = n * page
+    saving = (rows - 1) * n * 4096
+    for least, together in ((saving, True), (saving + 1, False), ((1 << 63) - 1, False), (saving - 1, True)):
+        got = attend(gpu, kv, table, lens, [0, rows], [n], q, seq_ids=np.arange(rows) % 2, least=least)
+        assert np.isfinite(got[1]).all() == together and np.isfinite(got[2:]).all() and np.isfinite(got[0]).all(), least
