@@ -49,7 +49,8 @@ typedef struct {
    * rest of a head is copied. rope_tab [rope_rows][rot_dim] (cos | sin). A position
    * outside [0, rope_rows) gives NaN in the rotated elements. An output may be its
    * input; else it overlaps neither input nor the other output. k and k_out may be
-   * NULL with n_kv_heads 0. Beside rpg_op_rope. */
+   * NULL with n_kv_heads 0. At most 2^31 - 1 heads in all, 2^28 - 4 where head_dim or
+   * rot_dim is no multiple of 8 or a buffer not 16-byte aligned. Beside rpg_op_rope. */
   int32_t (*rope_rows)(const float* q, const float* k, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
                        int32_t rot_dim, int32_t interleaved, const float* rope_tab, int64_t rope_rows,
                        const int32_t* positions, int64_t n_rows, float* q_out, float* k_out);

@@ -109,8 +109,10 @@ typedef struct {
    * out of range, may give NaN in all of its rows. Groups that together save less than
    * least_saving bytes of reading (all rows of a group but one, times its pages) share
    * nothing; negative: what was measured to break even, 144 MB and one for each row;
-   * 0: share always. The workspace is attention_shared_workspace's (zeroed by
-   * attention_workspace_init), for n_rows or more. */
+   * 0: share always. Calls that may share are refused from outputs of 2^34 elements, or
+   * 2^31 units of 128 positions and 128 rows times heads, on. The workspace is
+   * attention_shared_workspace's (zeroed by attention_workspace_init), for n_rows or
+   * more. */
   int32_t (*attention_shared)(const rpg_paged_kv_t* kv, const rpg_page_table_t* table, const int32_t* seq_ids,
                               const int32_t* lens, const int32_t* group_rows, const int32_t* group_pages,
                               int32_t n_groups, const float* q, int32_t n_heads, int64_t n_rows, float* out,

@@ -735,6 +735,10 @@ __global__ __launch_bounds__(kJoinThreads) void SharedJoinKernel(const PrefixArg
 // fp16, 8 rows 32:19 32:34 32:34 33:43 38:54, 32 rows 25:17 29:24 30:24 32:29 32:37.
 int64_t LeastSaving(int64_t n_rows) { return (144 + n_rows) << 20; }
 
+int64_t JoinGroups(int64_t n_rows, int32_t n_heads, int32_t head_dim) {
+  return (n_rows * n_heads * (head_dim / 4) + kJoinThreads - 1) / kJoinThreads;
+}
+
 size_t MlBytes(int32_t n_heads, int64_t n_rows) {
   return (static_cast<size_t>(n_rows) * n_heads * 8 + 255) / 256 * 256;
 }
@@ -752,6 +756,8 @@ void CheckPrefix(const GpuPagedKv& kv, const GpuPageTable& table, int32_t n_head
   RPG_CHECK(n_rows * group <= 0x7FFFFFFF && most <= 0x7FFFFFFF / std::max(prefix->n_groups, 1),
             "AttentionPagedShared: %d groups of %lld rows of up to %lld positions are too many for one call",
             prefix->n_groups, static_cast<long long>(n_rows), static_cast<long long>(capacity));
+  RPG_CHECK(FitsLaunch(JoinGroups(n_rows, n_heads, kv.head_dim), kJoinThreads),
+            "AttentionPagedShared: %lld rows of %d heads are too many for one call", static_cast<long long>(n_rows), n_heads);
   // slots, (m, l)
   prefix->workspace = workspace;
   prefix->ml = reinterpret_cast<float*>(workspace + 2 * kGroups * static_cast<size_t>(SlotBytes(kv.head_dim)));
@@ -768,9 +774,8 @@ void AttendPrefix(const GpuPagedKv& kv, const GpuPageTable& table, const int32_t
                         static_cast<int32_t>(std::min<int64_t>(table.max_pages * kv.page_size, 0x7FFFFFFF)), n_heads,
                         n_heads / kv.n_kv_heads, scale_log2};
   Launch("SharedPrefixKernel", kern, dim3(kGroups), dim3(kThreads), args);
-  const int64_t join_groups = (n_rows * n_heads * (kv.head_dim / 4) + kJoinThreads - 1) / kJoinThreads;
   Launch("SharedJoinKernel", kv.head_dim == 128 ? SharedJoinKernel<128> : SharedJoinKernel<64>,
-         dim3(static_cast<uint32_t>(join_groups)), dim3(kJoinThreads), args);
+         dim3(static_cast<uint32_t>(JoinGroups(n_rows, n_heads, kv.head_dim))), dim3(kJoinThreads), args);
 }
 
 size_t GpuAttentionPagedSharedWorkspaceBytes(int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, int64_t n_rows) {

@@ -189,15 +189,21 @@ void GpuRopeRows(const float* q, const float* k, int32_t n_heads, int32_t n_kv_h
     const bool few = n_rows * per_token * (head_dim / 8) <= 6 * 256 * kThreads;
     a.groups = few ? per_token : (per_token + kHeads - 1) / kHeads;
     a.units = static_cast<uint32_t>(n_rows) * a.groups;
+    const int64_t blocks = (int64_t{a.units} + block.y - 1) / block.y;
+    RPG_CHECK(FitsLaunch(blocks, block.x), "RopeRows: %lld rows of %d heads are too many for one call",
+              static_cast<long long>(n_rows), per_token);
     auto* kern = few ? (interleaved ? RopeRowsKernel<1, true> : RopeRowsKernel<1, false>)
                      : (interleaved ? RopeRowsKernel<kHeads, true> : RopeRowsKernel<kHeads, false>);
-    Launch("RopeRowsKernel", kern, dim3((a.units + block.y - 1) / block.y), block, a);
+    Launch("RopeRowsKernel", kern, dim3(static_cast<uint32_t>(blocks)), block, a);
     return;
   }
   const dim3 block(64, kThreads / 64);
   a.units = static_cast<uint32_t>(n_rows) * a.groups;
+  const int64_t blocks = (int64_t{a.units} + block.y - 1) / block.y;
+  RPG_CHECK(FitsLaunch(blocks, block.x), "RopeRows: %lld rows of %d heads, in single elements, are too many for one call",
+            static_cast<long long>(n_rows), per_token);
   Launch("RopeRowsPairKernel", interleaved ? RopeRowsPairKernel<true> : RopeRowsPairKernel<false>,
-         dim3((a.units + block.y - 1) / block.y), block, a);
+         dim3(static_cast<uint32_t>(blocks)), block, a);
 }
 
 }  // namespace rpg

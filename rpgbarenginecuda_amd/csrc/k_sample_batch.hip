@@ -1082,7 +1082,7 @@ void GpuSampleBatch(const float* logits_dev, int64_t n_rows, int64_t n, int64_t 
                   !Overlap(workspace, static_cast<int64_t>(need), probs_dev, bytes))),
             "SampleBatch: logits, outputs and the workspace must not overlap");
   const int32_t slices = SlicesOf(n);
-  RPG_CHECK(n_rows * slices <= 0x7FFFFFFF, "SampleBatch: %lld rows of %lld logits are too many for one call",
+  RPG_CHECK(FitsLaunch(n_rows * slices, kThreads), "SampleBatch: %lld rows of %lld logits are too many for one call",
             static_cast<long long>(n_rows), static_cast<long long>(n));
   const SampleArgs a{logits_dev, row_stride, static_cast<int32_t>(n), slices, UnitsFor(n), opt.temperature, opt.top_k,
                      opt.top_p,  opt.min_p,  u_dev,                   tokens_dev, probs_dev, static_cast<char*>(workspace)};

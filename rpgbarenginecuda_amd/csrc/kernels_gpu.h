@@ -192,7 +192,9 @@ void GpuEmbeddingLookup(const GpuTensor& emb, const int32_t* toks_dev, int64_t s
 // with row positions[r] of rope_tab ([rope_rows][rot_dim], cos | sin), and the others
 // copied. A position outside [0, rope_rows) gives NaN in the rotated elements. An
 // output may be its input; else it must overlap neither an input nor the other
-// output. k and k_out may be null with n_kv_heads 0. No counterpart in the reference,
+// output. k and k_out may be null with n_kv_heads 0. A call may have 2^31 - 1 heads in
+// all, 2^28 - 4 where head_dim or rot_dim is no multiple of 8 or a buffer not 16-byte
+// aligned. No counterpart in the reference,
 // whose rows stand at consecutive positions (src/kernels_gpu.h:71-72).
 void GpuRopeRows(const float* q, const float* k, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
                  int32_t rot_dim, bool interleaved, const float* rope_tab, int64_t rope_rows,
@@ -394,7 +396,9 @@ void GpuAttentionPagedWorkspaceInit(void* workspace, size_t bytes);
 // pages) share nothing, and each row is attended to by itself. A negative least_saving
 // stands for what was measured to break even, 144 MB and one more for each row; 0
 // shares always. Where not even all rows with all pages of a table would save as much,
-// the call is GpuAttentionPaged's one launch.
+// the call is GpuAttentionPaged's one launch. One that may share is refused where its
+// outputs reach 2^34 elements, or where the groups, each of all rows, would have room
+// for 2^31 units (128 positions of a kv head, for 128 rows times query heads).
 //
 // workspace: GpuAttentionPagedSharedWorkspaceBytes for n_rows or more, else as for
 // GpuAttentionPaged (GpuAttentionPagedWorkspaceInit zeroes it).

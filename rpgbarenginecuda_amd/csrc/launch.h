@@ -17,7 +17,11 @@
 
 namespace rpg {
 
-// The same with `shmem` bytes of dynamic LDS.
+// Whether a launch has room for `groups` workgroups of `threads` in x: a dimension holds less than 2^32 work items. Asked
+// where sizes are checked, so that nothing of a call has been launched when it is refused.
+inline bool FitsLaunch(int64_t groups, int64_t threads) { return groups <= 0xFFFFFFFFLL / threads; }
+
+// Launch with `shmem` bytes of dynamic LDS.
 template <typename... KArgs, typename... Args>
 inline void LaunchShared(const char* name, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t shmem,
                          Args... args) {
