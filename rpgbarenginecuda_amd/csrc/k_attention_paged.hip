@@ -250,18 +250,20 @@ struct Batch {
       own = of_items ? cut.Items(own_units) : own_units;
     } else {
       const int64_t first = lo + static_cast<int64_t>(lane) * some;
-      const auto add = [&](int32_t i) {
-        if (first + i < hi) {
-          const uint32_t n = LaneUnitsOf(static_cast<int32_t>(first + i));
-          own += of_items ? cut.Items(n) : n;
-        }
-      };
-      if constexpr (S::kOn) {
+      if constexpr (S::kOn) {  // groups are looked up by all lanes, those behind the last row too
 #pragma unroll 1
-        for (int32_t i = 0; i < some; ++i) add(i);
+        for (int32_t i = 0; i < some; ++i) {
+          const uint32_t n = LaneUnitsOf(static_cast<int32_t>(min(first + i, static_cast<int64_t>(hi) - 1)));
+          if (first + i < hi) own += of_items ? cut.Items(n) : n;
+        }
       } else {
 #pragma unroll 2
-        for (int32_t i = 0; i < some; ++i) add(i);
+        for (int32_t i = 0; i < some; ++i) {
+          if (first + i < hi) {
+            const uint32_t n = LaneUnitsOf(static_cast<int32_t>(first + i));
+            own += of_items ? cut.Items(n) : n;
+          }
+        }
       }
     }
     own *= static_cast<uint32_t>(rows.pairs);

@@ -183,9 +183,10 @@ struct AskedRow {
     return seq >= 0 && seq < a.view.n_seqs && len >= 0 && len <= a.capacity && dev::TakesPart(pages, a.view.page_shift, len);
   }
 };
-// Whether r, among the rows that group `of` names, is its own: no earlier group's.
+// Whether r, among the rows that group `of` names, is its own: no earlier group's. Of all lanes at once, as OfLane is.
 __device__ __forceinline__ bool IsOf(const dev::SharedGroups& groups, int32_t r, int32_t of, bool there) {
-  return there && (groups.n == 1 || groups.OfLane(there ? r : -1) == of);
+  const bool own = groups.n == 1 || groups.OfLane(there ? r : -1) == of;
+  return there && own;
 }
 
 template <int D, bool kQ8>
@@ -315,7 +316,8 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
     const AskedRow asked(args, row, a_column);
     load(loaded, c0, page_of(c0));
     next_page = page_of(c0 + 1);
-    there = IsOf(groups, row, piece.of, a_column) && asked.BeginsWith(args, piece.pages);
+    there = IsOf(groups, row, piece.of, a_column);
+    there = asked.BeginsWith(args, piece.pages) && there;
     float x[kSteps][8];
     float top = 0.0f;
 #pragma unroll

@@ -117,13 +117,14 @@ struct SharedGroups {
     const uint32_t high_all = __builtin_amdgcn_readlane(high, 63), low_all = __builtin_amdgcn_readlane(low, 63);
     if ((static_cast<int64_t>(high_all) << 25) + low_all < least) pages = 0;
   }
-  // The group of row r, the lane's; -1 if there is none.
+  // The group of row r, the lane's; -1 if there is none. Every lane has to be active, here and at PagesOfLane: what a lane
+  // holds is read by all, and a lane that is not at work may hold anything.
   __device__ __forceinline__ int32_t OfLane(int32_t r) const {
     int32_t found = -1;
 #pragma unroll 1
     for (int32_t g = n - 1; g >= 0; --g) {
-      const bool in = r >= __builtin_amdgcn_readlane(first, g) && r < __builtin_amdgcn_readlane(last, g);
-      found = in ? g : found;
+      const int32_t from = __builtin_amdgcn_readlane(first, g), to = __builtin_amdgcn_readlane(last, g);
+      found = (r >= from) & (r < to) ? g : found;
     }
     return found;
   }
@@ -131,8 +132,9 @@ struct SharedGroups {
     int32_t found = 0;
 #pragma unroll 1
     for (int32_t g = n - 1; g >= 0; --g) {
-      const bool in = r >= __builtin_amdgcn_readlane(first, g) && r < __builtin_amdgcn_readlane(last, g);
-      found = in ? __builtin_amdgcn_readlane(pages, g) : found;
+      const int32_t from = __builtin_amdgcn_readlane(first, g), to = __builtin_amdgcn_readlane(last, g);
+      const int32_t shared = __builtin_amdgcn_readlane(pages, g);
+      found = (r >= from) & (r < to) ? shared : found;
     }
     return found;
   }
