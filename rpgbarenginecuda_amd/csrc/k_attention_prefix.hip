@@ -32,7 +32,6 @@
 
 #include <algorithm>
 #include <cmath>
-#include <type_traits>
 
 #include "attention_dev.h"
 #include "dev_util.h"
@@ -294,6 +293,7 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
   const bool works = key_wave < key_waves && col_wave * kWaveCols < piece.cols;
   float to_score, m, l;
   int q_exp;  // 8 bits: the power of two that to_score gives back to queries
+  bool rounds = false;  // whether scores are rounded as m is
   float down;  // the power of two that weights enter multiplied by
   F32x4 acc[kE];
   Half8 q_hi[kSteps], q_lo[kSteps];
@@ -459,10 +459,11 @@ __device__ __forceinline__ void AttendPiece(const PrefixArgs& args, const dev::S
 #pragma unroll
         for (int i = 0; i < kE; ++i) acc[i] *= back;
       }
+      rounds = __any(fabsf(m) >= 0x1p22f);
     }
     // m is a score as rounded. From 2^22 on, where the rounding is half an octave and more, the others are rounded too: not
     // rounded, their weights could pass what they have room for.
-    if (__builtin_expect(__any(fabsf(m) >= 0x1p22f), 0)) {
+    if (__builtin_expect(rounds, 0)) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) s[j] *= by;
       by = 1.0f;
