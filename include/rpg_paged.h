@@ -107,8 +107,8 @@ typedef struct {
    * groups. The pages are taken from the group's first row that has them all. Limits
    * as for attention; an infinity or a NaN among a group's keys and values, or a page
    * out of range, may give NaN in all of its rows. Groups that together save less than
-   * least_saving bytes of reading (all rows of a group but one, times its pages) share
-   * nothing; negative: what was measured to break even, 144 MB and one for each row;
+   * least_saving bytes of reading (all rows of a group but one, idle ones too, times its
+   * pages) share nothing; negative: what was measured to break even, 144 MB and one for each row;
    * 0: share always. Calls that may share are refused from outputs of 2^34 elements, or
    * 2^31 units of 128 positions and 128 rows times heads, on. The workspace is
    * attention_shared_workspace's (zeroed by attention_workspace_init), for n_rows or

@@ -22,12 +22,12 @@
 // kernel that joins them in order, over all compute units: the last workgroup of a tile to arrive, on its one, took 18 us for
 // four parts of 128 columns where that takes 4.
 //
-// What bounds it: 32 positions of 128 columns take a compute unit 2700 cycles, of which the matrix cores are busy for 1030
-// and vector arithmetic for 1360, by two waves that mostly wait for the same; 32 columns to a wave (half the reads of LDS)
+// What bounds it: 32 positions of 128 columns take a compute unit some 2750 cycles, of which the matrix cores are busy for
+// 1030 and vector arithmetic for 1360, by two waves that mostly wait for the same; 32 columns to a wave (half the reads of LDS)
 // and sixteen waves were no faster, and their code and joins cost the short pieces 4 us. Behind few columns it is memory
 // (4 TB/s), and for one or two steps the chain of groups, lengths, table, keys and the first pass through the code, 8 us.
-// 128 rows and 4 heads to a kv head over 8192 positions in 8 bits 58 us (0.59 PFLOP/s of formed products), 8 rows over
-// 32768 26 us, 32 rows and 2 heads over 2816 in fp16 10.7 us.
+// 128 rows and 4 heads to a kv head over 8192 positions in 8 bits 59 us (0.58 PFLOP/s of formed products), 8 rows over
+// 32768 26 us, 32 rows and 2 heads over 2816 in fp16 10.8 us.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -735,7 +735,10 @@ __global__ __launch_bounds__(kJoinThreads) void SharedJoinKernel(const PrefixArg
 // saved: 16 query and 8 kv heads of 128, fp16, 4 rows 27:30 32:36 33:42 31:48 38:60, 16 rows 23:18 25:29 25:28 26:32 28:44,
 // 64 rows 28:16 29:26 30:28 30:31 30:35, 128 rows 36:26 36:29 37:32 37:34 37:40; 32 and 8 heads in 8 bits, 4 rows 31:24 37:41
 // 39:44 39:52 46:67, 16 rows 28:20 32:28 33:28 34:35 35:46, 64 rows 31:18 32:27 32:29 33:31 34:34; 32 and 4 heads of 64,
-// fp16, 8 rows 32:19 32:34 32:34 33:43 38:54, 32 rows 25:17 29:24 30:24 32:29 32:37.
+// fp16, 8 rows 32:19 32:34 32:34 33:43 38:54, 32 rows 25:17 29:24 30:24 32:29 32:37. One line in rows for all of these:
+// it takes the slower side for 4 rows at 96 (fp16) and 128, for 16 at 128 (fp16) and 160 (8 bits), for heads of 64 at 128 (8
+// rows) and 192 (32 rows), and for 64 and 128 rows where both are alike, by 3 to 18%. Rows are counted without their
+// lengths: those of a batch that stand idle save nothing, but count.
 int64_t LeastSaving(int64_t n_rows) { return (144 + n_rows) << 20; }
 
 int64_t JoinGroups(int64_t n_rows, int32_t n_heads, int32_t head_dim) {

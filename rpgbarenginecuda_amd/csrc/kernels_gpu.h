@@ -360,7 +360,8 @@ void GpuKvReadPaged(const GpuPagedKv& kv, const GpuPageTable& table, const int32
 //
 // Scores, weights and sums have fp32's precision, within these limits: of a query,
 // what is below 2^-30 of its row's largest element (fp16 pages: 2^-38) does not
-// count; a weight below 2^-120 of the row's largest may count as none; weights times
+// count; a weight below 2^-120 of the row's largest may count as none, and over fp16 pages
+// any weight is off by up to 2^-39 of it; weights times
 // values that add up to more than fp32 holds before the sum of weights divides them
 // (values past 2^93) may give an infinity; an infinite value whose weight is below
 // 2^-23 of the largest may give NaN instead of the infinity.
@@ -389,11 +390,14 @@ void GpuAttentionPagedWorkspaceInit(void* workspace, size_t bytes);
 // counts; one of no pages, fewer or more than a table has, shares none. Results and limits are
 // GpuAttentionPaged's, but that an infinity or a NaN among a group's keys and values,
 // or a page out of range, may give NaN in all of the group's rows whose output it
-// reaches.
+// reaches. At shared positions queries and weights count to 2^-22 of their value; over
+// 8-bit pages weight times scale to 2^-37 of the largest besides.
 //
 // Sharing pays where it saves much reading: groups that together save less than
 // least_saving bytes of keys and values (of each group all rows but one, times its
-// pages) share nothing, and each row is attended to by itself. A negative least_saving
+// pages) share nothing, and each row is attended to by itself. Rows that stand idle or
+// do not reach behind the shared pages count with the others there: where a batch has
+// many, least_saving is the caller's to set. A negative least_saving
 // stands for what was measured to break even, 144 MB and one more for each row; 0
 // shares always. Where not even all rows with all pages of a table would save as much,
 // the call is GpuAttentionPaged's one launch. One that may share is refused where its
