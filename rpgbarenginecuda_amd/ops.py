@@ -1110,8 +1110,8 @@ def GpuAttentionPagedShared(kv: GpuPagedKv, table: GpuPageTable, lens, group_row
     """GpuAttentionPaged for a batch whose sequences share their beginnings: rows [group_rows[g], group_rows[g + 1])
     form group g, whose sequences' tables begin with the same group_pages[g] pages, attended to once for the group.
     group_rows [n_groups + 1] and group_pages [n_groups] are int32 tensors (n_groups goes with raw addresses), of at most
-    64 groups. Groups that together save less than least_saving bytes of reading share nothing: -1 stands for what was
-    measured to break even, 144 MB and one for each row, 0 shares always. The workspace is zero before its first call, and
+    64 groups. Groups that together save less than least_saving bytes of reading share nothing (all rows of a group but one
+    count, idle ones too): -1 stands for what was measured to break even, 144 MB and one for each row, 0 shares always. The workspace is zero before its first call, and
     belongs to one call at a time."""
     int_at, float_at = kv.int_at, kv.float_at
     span = 4 * n_rows * n_heads * kv.head_dim
